@@ -70,6 +70,14 @@ int lsx_ctx_architecture(lsx_ctx* ctx, int* architecture);
 /* The context's cudaStream_t, for callers that order their own work after ours. */
 int lsx_ctx_stream(lsx_ctx* ctx, void** stream);
 
+/* Ordering with a caller's cudaStream_t on the same device (0: the default stream).
+   lsx_ctx_wait_for: what is enqueued on the context's stream from here on runs after
+   all that `stream` holds now.  lsx_ctx_release_to: what is enqueued on `stream` from
+   here on runs after all that the context's stream holds now.  Neither waits on the
+   host; inside a stream capture they join the context's stream to it and back. */
+int lsx_ctx_wait_for(lsx_ctx* ctx, void* stream);
+int lsx_ctx_release_to(lsx_ctx* ctx, void* stream);
+
 /* ---------------------------------------------------------------- tensors -- */
 /* Gpu::upload_raw (src/gpu.rs:217-226): copies `bytes` of `kind` storage. */
 int lsx_upload_raw(lsx_ctx* ctx, const void* data, size_t bytes, lsx_dtype kind, lsx_tensor** out);
@@ -344,6 +352,70 @@ int lsx_readout_margin_fixed(lsx_ctx* ctx, const lsx_tensor* weight, const lsx_t
                              size_t vocab, size_t width, const void* hidden, lsx_dtype hidden_kind,
                              size_t rows, const uint32_t* targets, double* margin_out,
                              uint32_t* argmax_out, float* target_logit_out);
+
+/* ------------------------------------------------- distributions over tokens -- */
+/* Operators on rows of logits that lie on the device.  Row r is `vocab` elements of
+   `kind` (F32, F16 or BF16) from logits + r * stride (stride >= vocab, in elements;
+   any element alignment).  With z the row, T the `temperature` (1e-6..=1e6),
+   m = max z and s = ln sum_i exp((z_i - m) / T), its probabilities are
+   q_i = exp((z_i - m) / T - s); (m, s) are the row's statistics, so
+   m / T + s is its log-sum-exp.  Sums are held in f32 around the row's maximum or
+   in f64.  -inf logits are tokens that cannot occur; a row of nothing else has
+   statistics (-inf, 0), entropy 0, log probabilities -inf and a zero gradient.  A NaN
+   or +inf logit makes the row's results NaN.  In token lists 0xFFFFFFFF is an unused
+   slot; any other id >= vocab makes the results it enters NaN.  All pointers are
+   device pointers; calls only enqueue on the context's stream and use no workspace.
+
+   The reference scores one target per row on the host (attribution::loss,
+   src/attribution.rs:49-60, and argmax, src/diagnosis.rs:58-70). */
+/* For each row: ln q of `token_count` (0..=128) given tokens (tokens and
+   logprob_out [rows x token_count]; an unused slot gives 0), the entropy
+   -sum_i q_i ln q_i (entropy_out [rows]), the statistics (stats_out [rows x 2]) and
+   the `alternatives` (0..=128, at most vocab) largest logits in descending order,
+   the lower id first among equals (ids, logits as f32 and ln q, each
+   [rows x alternatives]; NaN counts as the largest).  Any output may be NULL. */
+int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
+                              size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
+                              size_t alternatives, float* logprob_out, float* entropy_out, float* stats_out,
+                              uint32_t* top_ids_out, float* top_logits_out, float* top_logprobs_out);
+/* Gradient of sum_n g_n ln q(t_n) + h entropy with respect to the logits,
+     dz_i = (1/T) (sum_n g_n [t_n = i] - q_i (sum_n g_n + h (ln q_i + entropy))),
+   from the forward call's statistics and entropy: logprob_gradient g
+   [rows x token_count] (tokens named twice add up), entropy_gradient h [rows] or
+   NULL (then entropy is NULL too).  gradient_out has the logits' kind, rows
+   `gradient_stride` elements apart: the logits themselves (in place, with their
+   stride) or memory that does not overlap them. */
+int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
+                                       size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
+                                       const float* stats, const float* entropy, const float* logprob_gradient,
+                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride);
+/* Distillation from a teacher's top logits: per row `teacher_count` (1..=128) tokens K
+   with the teacher's logits a (f32, both [rows x teacher_count]; a token listed twice
+   counts once, at its first slot).  Without teacher_stats the teacher is
+   p_j = softmax(a / T) over K and loss_out [rows] = sum_K p_j ln(p_j / q_j).  With
+   teacher_stats ([rows x 2], the teacher's (m, s) as lsx_token_logprobs_device gives
+   them at the same temperature) p_j are its probabilities over the whole vocabulary,
+   and all tokens outside K form one more outcome, p_r = max(0, 1 - sum_K p_j) against
+   the student's q_r: loss += p_r ln(p_r / q_r) (left out, p_r = 0, where q_r is below
+   2^-126, the smallest normal f32 number).  stats_out [rows x 3]: (m, s) of the student and the log of
+   sum_{i not in K} exp((z_i - m) / T) (-inf without teacher_stats).  With
+   gradient_out also the gradient of weights[r] * loss (weights NULL: 1), with
+   P = sum_K p_j + p_r:
+     dz_i = (w/T) (q_i P - p_i) for i in K,  (w/T) q_i (P - p_r / q_r) otherwise,
+   stored as lsx_token_logprobs_backward_device does.  loss_out and stats_out may be
+   NULL.  A row whose list is unused throughout has p = 0 (p_r = 1 with statistics):
+   loss and gradient 0. */
+int lsx_distill_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab, size_t stride,
+                       double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
+                       size_t teacher_count, const float* teacher_stats, const float* weights, float* loss_out,
+                       float* stats_out, void* gradient_out, size_t gradient_stride);
+/* The gradient alone, of loss_gradient[r] * loss, from the forward call's stats
+   ([rows x 3]) and the same teacher. */
+int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
+                                size_t stride, double temperature, const uint32_t* teacher_ids,
+                                const float* teacher_logits, size_t teacher_count, const float* teacher_stats,
+                                const float* stats, const float* loss_gradient, void* gradient_out,
+                                size_t gradient_stride);
 
 /* ------------------------------------------------ plane-candidate feasibility -- */
 /* FeasibleSet (src/interval.rs:47-212): the open forbidden intervals of a plane

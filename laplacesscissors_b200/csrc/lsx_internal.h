@@ -72,6 +72,8 @@ struct lsx_ctx {
     // last tensor is freed, so destruction order does not matter to callers.
     int refs = 0;
     bool destroyed = false;
+    // Order the stream after a caller's stream and the reverse (created on first use).
+    cudaEvent_t entered = nullptr, left = nullptr;
 };
 
 struct lsx_tensor {
@@ -83,6 +85,20 @@ struct lsx_tensor {
 };
 
 namespace lsx {
+
+// Makes the context's device current and puts the caller's back.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t status;
+    explicit DeviceScope(int device) {
+        status = cudaGetDevice(&before);
+        if (status == cudaSuccess && before != device) status = cudaSetDevice(device);
+        if (before == device) before = -1;
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+};
 
 // Allocates an owned tensor from the context pool (Gpu::reserve, src/gpu.rs:204-216:
 // 1..=i32::MAX elements).

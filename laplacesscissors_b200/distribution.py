@@ -1,0 +1,211 @@
+"""Distributions over tokens from rows of logits on the device: log probabilities of
+given tokens with the entropy and the top alternatives, distillation from a teacher's
+top logits, and the gradients of both (lsx_token_logprobs_device and the entries
+beside it, which state the formulas).
+
+The reference scores one target per row on the host (attribution::loss,
+src/attribution.rs:49-60); these work on torch CUDA tensors: `logits` [rows, vocab]
+of float32, float16 or bfloat16 with unit stride along the vocabulary and any stride
+between rows, token ids as int32 (-1 for an unused slot; another id outside the
+vocabulary makes the results it enters NaN).  Calls are ordered with torch's current
+stream on the Gpu's device: they run on the library's stream after what the current
+stream holds, and the current stream waits for them.  Nothing is copied to the host;
+under a stream capture the kernels join the captured graph.  `out` takes tensors to
+write instead of new ones, in the order of the results (None where a result is not
+wanted)."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from ._lib import BF16, F16, F32, check, lib
+from .gpu import Gpu
+
+_KINDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor | None       # f32 [rows, n]: ln q of the given tokens
+    entropy: torch.Tensor | None       # f32 [rows]
+    stats: torch.Tensor | None         # f32 [rows, 2]: m and ln sum exp((z - m) / T)
+    top_ids: torch.Tensor | None       # int32 [rows, k]
+    top_logits: torch.Tensor | None    # f32 [rows, k]
+    top_logprobs: torch.Tensor | None  # f32 [rows, k]
+
+
+class Distillation(NamedTuple):
+    loss: torch.Tensor | None      # f32 [rows]
+    stats: torch.Tensor | None     # f32 [rows, 3]: m, ln sum, ln of the sum outside the teacher's list
+    gradient: torch.Tensor | None  # [rows, vocab], the logits' dtype
+
+
+def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
+    """(rows, vocab, stride, kind) of a matrix of rows on the Gpu's device."""
+    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _KINDS:
+        raise ValueError(f"{name} must be a [rows, vocab] tensor of float32, float16 or bfloat16")
+    if not logits.is_cuda or logits.device.index != gpu.device:
+        raise ValueError(f"{name} must be on the Gpu's device")
+    rows, vocab = logits.shape
+    if vocab < 1:
+        raise ValueError("check the vocabulary size")
+    if vocab > 1 and logits.stride(1) != 1:
+        raise ValueError(f"{name} must have unit stride along the vocabulary")
+    stride = logits.stride(0) if rows > 1 else vocab
+    if stride < vocab:
+        raise ValueError(f"rows of {name} must not overlap")
+    return rows, vocab, stride, _KINDS[logits.dtype]
+
+
+def _vector(gpu: Gpu, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
+    """Address of a contiguous tensor of this shape and type on the Gpu's device."""
+    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype:
+        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}")
+    if not t.is_cuda or t.device.index != gpu.device or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous on the Gpu's device")
+    return t.data_ptr()
+
+
+def _count(t: torch.Tensor, rows: int, name: str) -> int:
+    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] > MAX_SLOTS:
+        raise ValueError(f"{name} must be [rows, at most {MAX_SLOTS}]")
+    return t.shape[1]
+
+
+def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
+    """The gradient's tensor and row stride: rows laid out like the logits'."""
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
+    elif out.shape != logits.shape or out.dtype != logits.dtype:
+        raise ValueError("the gradient must have the logits' shape and dtype")
+    return out, _rows(gpu, out, "the gradient")[2]
+
+
+class _Ordered:
+    """Runs a block on the library's stream, ordered with torch's current stream."""
+
+    def __init__(self, gpu: Gpu):
+        self.handle = gpu.handle
+        self.stream = torch.cuda.current_stream(gpu.device).cuda_stream
+
+    def __enter__(self):
+        check(lib.lsx_ctx_wait_for(self.handle, self.stream))
+
+    def __exit__(self, *exc):
+        check(lib.lsx_ctx_release_to(self.handle, self.stream))
+        return False
+
+
+def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0,
+                   temperature: float = 1.0, out=None) -> TokenLogprobs:
+    """Log probabilities of `tokens` (int32 [rows, n]), the entropy, the statistics
+    (m, s) and the `alternatives` largest logits of each row, in descending order
+    with the lower id first among equals (lsx_token_logprobs_device)."""
+    rows, vocab, stride, kind = _rows(gpu, logits)
+    n = _count(tokens, rows, "tokens") if tokens is not None else 0
+    k = int(alternatives)
+    if not 0 <= k <= min(MAX_SLOTS, vocab):
+        raise ValueError(f"alternatives must be at most {MAX_SLOTS} and at most the vocabulary")
+    shapes = (((rows, n), torch.float32), ((rows,), torch.float32), ((rows, 2), torch.float32),
+              ((rows, k), torch.int32), ((rows, k), torch.float32), ((rows, k), torch.float32))
+    if out is None:
+        out = tuple(torch.empty(s, dtype=d, device=logits.device) if (n or i != 0) and (k or i < 3) else None
+                    for i, (s, d) in enumerate(shapes))
+    elif len(out) != 6:
+        raise ValueError("out holds the six results")
+    at = [_vector(gpu, t, s, d, f"out[{i}]") if t is not None and t.numel() else None
+          for i, (t, (s, d)) in enumerate(zip(out, shapes))]
+    given = _vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None
+    result = TokenLogprobs(*out)
+    if rows:
+        with _Ordered(gpu):
+            check(lib.lsx_token_logprobs_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
+                                                given, n, k, *at))
+    return result
+
+
+def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None, stats: torch.Tensor,
+                            entropy: torch.Tensor | None, logprob_gradient: torch.Tensor | None,
+                            entropy_gradient: torch.Tensor | None = None, *, temperature: float = 1.0,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient with respect to the logits of sum(logprob_gradient * logprob) +
+    sum(entropy_gradient * entropy), from token_logprobs' stats and entropy
+    (lsx_token_logprobs_backward_device).  `out` may be the logits themselves."""
+    rows, vocab, stride, kind = _rows(gpu, logits)
+    n = _count(tokens, rows, "tokens") if tokens is not None else 0
+    out, out_stride = _gradient(gpu, logits, out)
+    if entropy_gradient is None:
+        entropy = None
+    f32 = torch.float32
+    at = (_vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None, n,
+          _vector(gpu, stats, (rows, 2), f32, "stats"),
+          _vector(gpu, entropy, (rows,), f32, "entropy") if entropy_gradient is not None else None,
+          _vector(gpu, logprob_gradient, (rows, n), f32, "logprob_gradient") if n else None,
+          _vector(gpu, entropy_gradient, (rows,), f32, "entropy_gradient") if entropy_gradient is not None else None)
+    if rows:
+        with _Ordered(gpu):
+            check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
+                                                         temperature, *at, out.data_ptr(), out_stride))
+    return out
+
+
+def _teacher(gpu: Gpu, rows: int, ids, values, stats):
+    k = _count(ids, rows, "teacher_ids")
+    if k < 1:
+        raise ValueError("the teacher lists at least one token")
+    return (_vector(gpu, ids, (rows, k), torch.int32, "teacher_ids"),
+            _vector(gpu, values, (rows, k), torch.float32, "teacher_logits"), k,
+            _vector(gpu, stats, (rows, 2), torch.float32, "teacher_stats") if stats is not None else None)
+
+
+def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
+            teacher_stats: torch.Tensor | None = None, weights: torch.Tensor | None = None, temperature: float = 1.0,
+            gradient: bool = False, out=None) -> Distillation:
+    """Divergence of the student's rows from a teacher's top tokens
+    (lsx_distill_device): teacher_ids int32 and teacher_logits f32 [rows, k],
+    teacher_stats [rows, 2] the teacher's statistics at the same temperature (with
+    them the tokens outside the list count as one outcome, without them the teacher
+    is normalised over its list).  With `gradient` also the gradient of
+    weights * loss with respect to the logits, which out[2] may be."""
+    rows, vocab, stride, kind = _rows(gpu, logits)
+    teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
+    if weights is not None and not gradient:
+        raise ValueError("weights scale the gradient only")
+    f32 = torch.float32
+    if out is None:
+        out = (torch.empty(rows, dtype=f32, device=logits.device),
+               torch.empty((rows, 3), dtype=f32, device=logits.device), None)
+    elif len(out) != 3 or (out[2] is not None and not gradient):
+        raise ValueError("out holds the three results, the last only with the gradient")
+    grad, grad_stride = _gradient(gpu, logits, out[2]) if gradient else (None, 0)
+    at = (_vector(gpu, weights, (rows,), f32, "weights") if weights is not None else None,
+          _vector(gpu, out[0], (rows,), f32, "out[0]") if out[0] is not None else None,
+          _vector(gpu, out[1], (rows, 3), f32, "out[1]") if out[1] is not None else None)
+    if rows:
+        with _Ordered(gpu):
+            check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
+                                         *teacher, *at, grad.data_ptr() if gradient else None, grad_stride))
+    return Distillation(out[0], out[1], grad)
+
+
+def distill_backward(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor,
+                     stats: torch.Tensor, loss_gradient: torch.Tensor, *, teacher_stats: torch.Tensor | None = None,
+                     temperature: float = 1.0, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Gradient of sum(loss_gradient * loss) with respect to the logits, from
+    distill's stats (lsx_distill_backward_device).  `out` may be the logits."""
+    rows, vocab, stride, kind = _rows(gpu, logits)
+    teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
+    out, out_stride = _gradient(gpu, logits, out)
+    at = (_vector(gpu, stats, (rows, 3), torch.float32, "stats"),
+          _vector(gpu, loss_gradient, (rows,), torch.float32, "loss_gradient"))
+    if rows:
+        with _Ordered(gpu):
+            check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
+                                                  temperature, *teacher, *at, out.data_ptr(), out_stride))
+    return out
+
+
+__all__ = ["TokenLogprobs", "Distillation", "token_logprobs", "token_logprobs_backward", "distill",
+           "distill_backward", "MAX_SLOTS"]
