@@ -258,9 +258,13 @@ __device__ __forceinline__ float block_sum(float v, float* scratch) {
 // ---- running sums of a softmax ---------------------------------------------------
 // S = sum 2^y and W = sum 2^y y over the elements seen, y against the reference r;
 // S == 0 exactly while only -inf has been seen.
-template <bool kWeighted>
+// With kRanked also the first vector holding the largest element, and the largest
+// element of the other vectors.
+template <bool kWeighted, bool kRanked = false>
 struct Running {
     float r = 0.f, limit = -INFINITY, S = 0.f, W = 0.f, m = -INFINITY;
+    float second = -INFINITY;
+    int at = -1;
     __device__ __forceinline__ void rise(float top, float L, float slack) {
         if (S != 0.f) {
             const float shift = (r - top) * L;
@@ -272,10 +276,14 @@ struct Running {
         limit = top + slack;
     }
     template <int n>
-    __device__ __forceinline__ void add(const float* v, float L, float slack) {
+    __device__ __forceinline__ void add(const float* v, int j, float L, float slack) {
         float top = v[0];
 #pragma unroll
         for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
+        if (kRanked) {
+            second = fmaxf(second, fminf(m, top));
+            at = top > m ? j : at;
+        }
         m = fmaxf(m, top);
         if (top > limit) rise(top, L, slack);
 #pragma unroll
@@ -297,9 +305,9 @@ struct Running {
     }
 };
 
-template <typename E, bool kWeighted, bool kExclude>
+template <typename E, bool kExclude, bool kWeighted, bool kRanked>
 __device__ __forceinline__ void stream_row(const Row<E>& row, const Marks* M, float L, float slack,
-                                           Running<kWeighted>& acc) {
+                                           Running<kWeighted, kRanked>& acc) {
     constexpr int n = Vec<E>::n;
     auto take = [&](int j, float* v) {
         if (kExclude && marked(*M, j)) {
@@ -311,10 +319,21 @@ __device__ __forceinline__ void stream_row(const Row<E>& row, const Marks* M, fl
                     ++pos;
                 }
         }
-        acc.template add<n>(v, L, slack);
+        acc.template add<n>(v, j, L, slack);
     };
     const int tid = threadIdx.x, T = blockDim.x;
     int j = row.full0 + tid;
+    // every thread meets its vectors in ascending order
+    if (row.head && tid == 0) {
+        float v[n];
+        row.ragged(0, v);
+        acc.at = 0;
+        take(0, v);
+    } else if (j < row.full1) {
+        acc.at = j;
+    } else if (row.last && tid == T - 1) {
+        acc.at = row.full1;
+    }
     for (; j + (kUnroll - 1) * T < row.full1; j += kUnroll * T) {
         uint4 w[kUnroll];
 #pragma unroll
@@ -330,11 +349,6 @@ __device__ __forceinline__ void stream_row(const Row<E>& row, const Marks* M, fl
         float v[n];
         Vec<E>::unpack(row.full(j), v);
         take(j, v);
-    }
-    if (row.head && tid == 0) {
-        float v[n];
-        row.ragged(0, v);
-        take(0, v);
     }
     if (row.last && tid == T - 1) {
         float v[n];
@@ -390,10 +404,17 @@ __device__ __forceinline__ unsigned long long order_key(float z, uint32_t id) {
 }
 __device__ __forceinline__ uint32_t key_id(unsigned long long k) { return 0xffffffffu - (uint32_t)k; }
 
+__device__ __forceinline__ float key_logit(unsigned long long k) { return total_order_value((uint32_t)(k >> 32)); }
+
+constexpr int kMaxGroups = 256;
+
 struct Selection {
-    unsigned long long keys[kListCap];
+    alignas(16) unsigned long long keys[kListCap];
+    alignas(16) unsigned long long group[kMaxGroups];
     unsigned long long best[kMaxSlots];
-    int count;
+    unsigned long long threshold;
+    int rescan[kRowThreads];
+    int count, rescans;
 };
 
 // The `top` largest of keys[0..n) (all distinct), in descending order, into best and
@@ -436,6 +457,97 @@ __device__ int select_by_pieces(Selection& P, const E* z, int vocab, int top) {
     return have;
 }
 
+// The row's `top` best tokens from what the threads met while they summed it.  The
+// threads form groups; the `top`-th best of the groups' best vectors, ordered by (its
+// largest logit, lower vector number first), bounds the row's `top`-th best element from
+// below: `top` elements, one in each better group, are at least as good.  So only elements
+// at or above that bound are candidates: about G ln(1 / (1 - top / G)) of them where the
+// tokens lie at random over G groups.  They are read again (from L2) at the threads' best vectors, and in
+// all vectors only of threads that have a second one to offer.  More candidates than the
+// list holds (rows in order) are left to select_by_pieces.
+template <typename E>
+__device__ void select_by_threads(Selection& P, const Row<E>& row, const E* z, int top, float m, float second, int at) {
+    constexpr int n = Vec<E>::n;
+    const int tid = threadIdx.x, lane = tid & 31, T = blockDim.x;
+    const int wide = top > 64 ? 2 : 4, groups = T / wide;
+    const unsigned long long mine =
+        at < 0 ? 0ull : ((unsigned long long)total_order_key(m + 0.f) << 32) | (0xffffffffu - (uint32_t)at);
+    unsigned long long best = mine;
+    for (int o = 1; o < wide; o <<= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+        best = other > best ? other : best;
+    }
+    if (tid % wide == 0) P.group[tid / wide] = best;
+    if (tid == 0) {
+        P.threshold = 0ull;
+        P.count = P.rescans = 0;
+    }
+    __syncthreads();
+    if (tid < groups) {
+        const unsigned long long key = P.group[tid];
+        int above = 0;
+        for (int i = 0; i < groups; i += 2) {
+            const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&P.group[i]);
+            above += (pair.x > key) + (pair.y > key);
+        }
+        if (above == top - 1 && key != 0ull) P.threshold = key;
+    }
+    __syncthreads();
+    const unsigned long long threshold = P.threshold;
+    auto offer = [&](int j, const float* v) {
+        const uint32_t low = 0xffffffffu - (uint32_t)j;
+#pragma unroll
+        for (int e = 0; e < n; ++e) {
+            const long long i = row.first(j) + e;
+            const unsigned long long key = ((unsigned long long)total_order_key(v[e] + 0.f) << 32) | low;
+            if (key >= threshold && i >= 0 && i < row.vocab) {
+                const int pos = atomicAdd(&P.count, 1);
+                if (pos < kListCap) P.keys[pos] = order_key(v[e], (uint32_t)i);
+            }
+        }
+    };
+    auto read = [&](int j, float* v) {
+        if (j >= row.full0 && j < row.full1)
+            Vec<E>::unpack(row.full(j), v);
+        else
+            row.ragged(j, v);
+    };
+    if (mine != 0ull && mine >= threshold) {
+        float v[n];
+        read(at, v);
+        offer(at, v);
+        if (total_order_key(second + 0.f) >= (uint32_t)(threshold >> 32)) P.rescan[atomicAdd(&P.rescans, 1)] = tid;
+    }
+    // the best vector of a rescanned thread was offered by the thread itself
+    __shared__ int offered[kRowThreads];
+    offered[tid] = at;
+    __syncthreads();
+    const int rescans = P.rescans;
+    for (int q = tid >> 5; q < rescans; q += T >> 5) {
+        const int who = P.rescan[q], skip = offered[who];
+        float v[n];
+        for (int j = row.full0 + who + lane * T; j < row.full1; j += 32 * T)
+            if (j != skip) {
+                read(j, v);
+                offer(j, v);
+            }
+        if (lane == 0 && row.head && who == 0 && skip != 0) {
+            row.ragged(0, v);
+            offer(0, v);
+        }
+        if (lane == 0 && row.last && who == T - 1 && skip != row.full1) {
+            row.ragged(row.full1, v);
+            offer(row.full1, v);
+        }
+    }
+    __syncthreads();
+    if (P.count > kListCap) {
+        select_by_pieces<E>(P, z, row.vocab, top);
+        return;
+    }
+    rank_keys(P, P.count, top);
+}
+
 // ---- token_logprobs ------------------------------------------------------------------
 template <typename E>
 __global__ void __launch_bounds__(kRowThreads) token_logprobs_kernel(
@@ -448,8 +560,8 @@ __global__ void __launch_bounds__(kRowThreads) token_logprobs_kernel(
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const float L = (float)(1.4426950408889634 / temperature), slack = kSlack / L;
-    Running<true> acc;
-    stream_row<E, true, false>(row, nullptr, L, slack, acc);
+    Running<true, true> acc;
+    stream_row<E, false>(row, nullptr, L, slack, acc);
     const float m = block_max(acc.m, scratch.f[0]);
     acc.rebase(m, L);
     float S = block_sum(acc.S, scratch.f[1]);
@@ -485,10 +597,13 @@ __global__ void __launch_bounds__(kRowThreads) token_logprobs_kernel(
                 t == kUnusedToken ? 0.f : t < (uint32_t)vocab ? logprob(Vec<E>::one(z[t])) : NAN;
         }
     if (top > 0) {
-        select_by_pieces<E>(selection, z, vocab, top);
+        if (S == S)
+            select_by_threads<E>(selection, row, z, top, acc.m, acc.second, acc.at);
+        else  // NaN or +inf in the row: NaN leads the order and the threads' maxima pass over it
+            select_by_pieces<E>(selection, z, vocab, top);
         for (int i = threadIdx.x; i < top; i += blockDim.x) {
             const uint32_t id = key_id(selection.best[i]);
-            const float x = Vec<E>::one(z[id]);
+            const float x = key_logit(selection.best[i]);
             if (out.top_ids) out.top_ids[r * top + i] = id;
             if (out.top_logits) out.top_logits[r * top + i] = x;
             if (out.top_logprobs) out.top_logprobs[r * top + i] = logprob(x);
@@ -719,7 +834,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(
         for (int i = threadIdx.x; i < count; i += blockDim.x)
             listed[i] = marks.slot_rank[i] >= 0 ? Vec<E>::one(z[marks.raw[i]]) : -INFINITY;
         Running<false> acc;
-        stream_row<E, false, true>(row, &marks, L, slack, acc);
+        stream_row<E, true>(row, &marks, L, slack, acc);
         m_rest = block_max(acc.m, scratch.f[0]);
         acc.rebase(m_rest, L);
         S = block_sum(acc.S, scratch.f[1]);
