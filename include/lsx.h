@@ -70,14 +70,6 @@ int lsx_ctx_architecture(lsx_ctx* ctx, int* architecture);
 /* The context's cudaStream_t, for callers that order their own work after ours. */
 int lsx_ctx_stream(lsx_ctx* ctx, void** stream);
 
-/* Ordering with a caller's cudaStream_t on the same device (0: the default stream).
-   lsx_ctx_wait_for: what is enqueued on the context's stream from here on runs after
-   all that `stream` holds now.  lsx_ctx_release_to: what is enqueued on `stream` from
-   here on runs after all that the context's stream holds now.  Neither waits on the
-   host; inside a stream capture they join the context's stream to it and back. */
-int lsx_ctx_wait_for(lsx_ctx* ctx, void* stream);
-int lsx_ctx_release_to(lsx_ctx* ctx, void* stream);
-
 /* ---------------------------------------------------------------- tensors -- */
 /* Gpu::upload_raw (src/gpu.rs:217-226): copies `bytes` of `kind` storage. */
 int lsx_upload_raw(lsx_ctx* ctx, const void* data, size_t bytes, lsx_dtype kind, lsx_tensor** out);
@@ -364,7 +356,9 @@ int lsx_readout_margin_fixed(lsx_ctx* ctx, const lsx_tensor* weight, const lsx_t
    statistics (-inf, 0), entropy 0, log probabilities -inf and a zero gradient.  A NaN
    or +inf logit makes the row's results NaN.  In token lists 0xFFFFFFFF is an unused
    slot; any other id >= vocab makes the results it enters NaN.  All pointers are
-   device pointers; calls only enqueue on the context's stream and use no workspace.
+   device pointers.  Calls only enqueue, use no workspace and touch nothing of the
+   context but its device: `stream` is the cudaStream_t they run on, NULL for the
+   context's own (the default stream is cudaStreamLegacy, 1).
 
    The reference scores one target per row on the host (attribution::loss,
    src/attribution.rs:49-60, and argmax, src/diagnosis.rs:58-70). */
@@ -377,7 +371,7 @@ int lsx_readout_margin_fixed(lsx_ctx* ctx, const lsx_tensor* weight, const lsx_t
 int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                               size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
                               size_t alternatives, float* logprob_out, float* entropy_out, float* stats_out,
-                              uint32_t* top_ids_out, float* top_logits_out, float* top_logprobs_out);
+                              uint32_t* top_ids_out, float* top_logits_out, float* top_logprobs_out, void* stream);
 /* Gradient of sum_n g_n ln q(t_n) + h entropy with respect to the logits,
      dz_i = (1/T) (sum_n g_n [t_n = i] - q_i (sum_n g_n + h (ln q_i + entropy))),
    from the forward call's statistics and entropy: logprob_gradient g
@@ -388,7 +382,7 @@ int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, 
 int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                                        size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
                                        const float* stats, const float* entropy, const float* logprob_gradient,
-                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride);
+                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride, void* stream);
 /* Distillation from a teacher's top logits: per row `teacher_count` (1..=128) tokens K
    with the teacher's logits a (f32, both [rows x teacher_count]; a token listed twice
    counts once, at its first slot).  Without teacher_stats the teacher is
@@ -408,14 +402,14 @@ int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dty
 int lsx_distill_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab, size_t stride,
                        double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
                        size_t teacher_count, const float* teacher_stats, const float* weights, float* loss_out,
-                       float* stats_out, void* gradient_out, size_t gradient_stride);
+                       float* stats_out, void* gradient_out, size_t gradient_stride, void* stream);
 /* The gradient alone, of loss_gradient[r] * loss, from the forward call's stats
    ([rows x 3]) and the same teacher. */
 int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                                 size_t stride, double temperature, const uint32_t* teacher_ids,
                                 const float* teacher_logits, size_t teacher_count, const float* teacher_stats,
                                 const float* stats, const float* loss_gradient, void* gradient_out,
-                                size_t gradient_stride);
+                                size_t gradient_stride, void* stream);
 
 /* ------------------------------------------------ plane-candidate feasibility -- */
 /* FeasibleSet (src/interval.rs:47-212): the open forbidden intervals of a plane

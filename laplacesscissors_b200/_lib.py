@@ -60,8 +60,6 @@ SIGNATURES = {
     "lsx_ctx_name": (I, [P, C.c_char_p, SZ]),
     "lsx_ctx_architecture": (I, [P, C.POINTER(I)]),
     "lsx_ctx_stream": (I, [P, PP]),
-    "lsx_ctx_wait_for": (I, [P, P]),
-    "lsx_ctx_release_to": (I, [P, P]),
     "lsx_upload_raw": (I, [P, P, SZ, I, PP]),
     "lsx_upload_f32": (I, [P, FP, SZ, PP]),
     "lsx_zeros": (I, [P, SZ, PP]),
@@ -112,10 +110,10 @@ SIGNATURES = {
     "lsx_readout_merge_device": (I, [P, P, P, P, SZ, P, P, P]),
     "lsx_readout_partials_device": (I, [P, P, P, SZ, SZ, SZ, P, I, SZ, P, P, P, P, SZ]),
     "lsx_readout_partials_merge_device": (I, [P, P, P, SZ, P, P, P]),
-    "lsx_token_logprobs_device": (I, [P, P, I, SZ, SZ, SZ, D, P, SZ, SZ, P, P, P, P, P, P]),
-    "lsx_token_logprobs_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, SZ, P, P, P, P, P, SZ]),
-    "lsx_distill_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, P, SZ]),
-    "lsx_distill_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, SZ]),
+    "lsx_token_logprobs_device": (I, [P, P, I, SZ, SZ, SZ, D, P, SZ, SZ, P, P, P, P, P, P, P]),
+    "lsx_token_logprobs_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, SZ, P, P, P, P, P, SZ, P]),
+    "lsx_distill_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, P, SZ, P]),
+    "lsx_distill_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, SZ, P]),
     "lsx_feasible_create": (I, [D, PP]),
     "lsx_feasible_free": (I, [P]),
     "lsx_feasible_constrain": (I, [P, D, D, D]),

@@ -997,7 +997,7 @@ extern "C" {
 int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                               size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
                               size_t alternatives, float* logprob_out, float* entropy_out, float* stats_out,
-                              uint32_t* top_ids_out, float* top_logits_out, float* top_logprobs_out) {
+                              uint32_t* top_ids_out, float* top_logits_out, float* top_logprobs_out, void* stream) {
     const LogitRows z{logits, kind, rows, vocab, stride, temperature};
     LSX_TRY(check_rows(z));
     LSX_ENSURE(token_count <= (size_t)kMaxSlots, "a row names at most 128 tokens");
@@ -1008,11 +1008,12 @@ int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, 
     LSX_ENSURE(alternatives > 0 || (!top_ids_out && !top_logits_out && !top_logprobs_out),
                "alternatives need a count");
     LSX_ENSURE(ctx, "context is NULL");
+    const cudaStream_t on = stream ? (cudaStream_t)stream : ctx->stream;
     DeviceScope scope(ctx->device);
     LSX_CUDA(scope.status, "select device");
     if (!top_ids_out && !top_logits_out && !top_logprobs_out) alternatives = 0;
     const LogprobOutputs out{logprob_out, entropy_out, stats_out, top_ids_out, top_logits_out, top_logprobs_out};
-    LSX_CUDA(launch_token_logprobs(ctx->stream, ctx->sm_count, z, tokens, token_count, alternatives, out),
+    LSX_CUDA(launch_token_logprobs(on, ctx->sm_count, z, tokens, token_count, alternatives, out),
              "token log probabilities");
     return LSX_OK;
 }
@@ -1020,7 +1021,7 @@ int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, 
 int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                                        size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
                                        const float* stats, const float* entropy, const float* logprob_gradient,
-                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride) {
+                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride, void* stream) {
     const LogitRows z{logits, kind, rows, vocab, stride, temperature};
     LSX_TRY(check_rows(z));
     LSX_TRY(check_gradient(z, gradient_out, gradient_stride));
@@ -1030,9 +1031,10 @@ int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dty
                "give the tokens, their count and their gradients together");
     LSX_ENSURE((entropy != nullptr) == (entropy_gradient != nullptr), "give the entropy and its gradient together");
     LSX_ENSURE(ctx, "context is NULL");
+    const cudaStream_t on = stream ? (cudaStream_t)stream : ctx->stream;
     DeviceScope scope(ctx->device);
     LSX_CUDA(scope.status, "select device");
-    LSX_CUDA(launch_logprobs_gradient(ctx->stream, ctx->sm_count, z, tokens, token_count, stats, entropy,
+    LSX_CUDA(launch_logprobs_gradient(on, ctx->sm_count, z, tokens, token_count, stats, entropy,
                                       logprob_gradient, entropy_gradient, gradient_out, gradient_stride),
              "token log probabilities' gradient");
     return LSX_OK;
@@ -1041,7 +1043,7 @@ int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dty
 int lsx_distill_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab, size_t stride,
                        double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
                        size_t teacher_count, const float* teacher_stats, const float* weights, float* loss_out,
-                       float* stats_out, void* gradient_out, size_t gradient_stride) {
+                       float* stats_out, void* gradient_out, size_t gradient_stride, void* stream) {
     const LogitRows z{logits, kind, rows, vocab, stride, temperature};
     const TeacherRows teacher{teacher_ids, teacher_logits, teacher_stats, teacher_count};
     LSX_TRY(check_rows(z));
@@ -1049,9 +1051,10 @@ int lsx_distill_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t 
     if (gradient_out) LSX_TRY(check_gradient(z, gradient_out, gradient_stride));
     LSX_ENSURE(gradient_out || !weights, "weights scale the gradient only");
     LSX_ENSURE(ctx, "context is NULL");
+    const cudaStream_t on = stream ? (cudaStream_t)stream : ctx->stream;
     DeviceScope scope(ctx->device);
     LSX_CUDA(scope.status, "select device");
-    LSX_CUDA(launch_distill(ctx->stream, ctx->sm_count, z, teacher, weights, loss_out, stats_out, gradient_out,
+    LSX_CUDA(launch_distill(on, ctx->sm_count, z, teacher, weights, loss_out, stats_out, gradient_out,
                             gradient_stride),
              "distillation");
     return LSX_OK;
@@ -1061,7 +1064,7 @@ int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind
                                 size_t stride, double temperature, const uint32_t* teacher_ids,
                                 const float* teacher_logits, size_t teacher_count, const float* teacher_stats,
                                 const float* stats, const float* loss_gradient, void* gradient_out,
-                                size_t gradient_stride) {
+                                size_t gradient_stride, void* stream) {
     const LogitRows z{logits, kind, rows, vocab, stride, temperature};
     const TeacherRows teacher{teacher_ids, teacher_logits, teacher_stats, teacher_count};
     LSX_TRY(check_rows(z));
@@ -1069,9 +1072,10 @@ int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind
     LSX_TRY(check_gradient(z, gradient_out, gradient_stride));
     LSX_ENSURE(stats && loss_gradient, "invalid argument");
     LSX_ENSURE(ctx, "context is NULL");
+    const cudaStream_t on = stream ? (cudaStream_t)stream : ctx->stream;
     DeviceScope scope(ctx->device);
     LSX_CUDA(scope.status, "select device");
-    LSX_CUDA(launch_distill_gradient(ctx->stream, ctx->sm_count, z, teacher, stats, loss_gradient, gradient_out,
+    LSX_CUDA(launch_distill_gradient(on, ctx->sm_count, z, teacher, stats, loss_gradient, gradient_out,
                                      gradient_stride),
              "distillation gradient");
     return LSX_OK;

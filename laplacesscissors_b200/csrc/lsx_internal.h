@@ -72,8 +72,6 @@ struct lsx_ctx {
     // last tensor is freed, so destruction order does not matter to callers.
     int refs = 0;
     bool destroyed = false;
-    // Order the stream after a caller's stream and the reverse (created on first use).
-    cudaEvent_t entered = nullptr, left = nullptr;
 };
 
 struct lsx_tensor {

@@ -96,8 +96,6 @@ static void release_context(lsx_ctx* ctx) {
     cudaStreamSynchronize(ctx->stream);
     delete ctx->pool;
     if (ctx->pinned) cudaFreeHost(ctx->pinned);
-    if (ctx->entered) cudaEventDestroy(ctx->entered);
-    if (ctx->left) cudaEventDestroy(ctx->left);
     cudaStreamDestroy(ctx->stream);
     delete ctx;
 }
@@ -263,28 +261,6 @@ int lsx_ctx_architecture(lsx_ctx* ctx, int* architecture) {
 int lsx_ctx_stream(lsx_ctx* ctx, void** stream) {
     LSX_ENSURE(ctx && stream, "invalid argument");
     *stream = (void*)ctx->stream;
-    return LSX_OK;
-}
-
-int lsx_ctx_wait_for(lsx_ctx* ctx, void* stream) {
-    LSX_ENSURE(ctx, "context is NULL");
-    if ((cudaStream_t)stream == ctx->stream) return LSX_OK;
-    DeviceScope scope(ctx->device);
-    LSX_CUDA(scope.status, "select device");
-    if (!ctx->entered) LSX_CUDA(cudaEventCreateWithFlags(&ctx->entered, cudaEventDisableTiming), "ordering event");
-    LSX_CUDA(cudaEventRecord(ctx->entered, (cudaStream_t)stream), "record on the caller's stream");
-    LSX_CUDA(cudaStreamWaitEvent(ctx->stream, ctx->entered, 0), "wait for the caller's stream");
-    return LSX_OK;
-}
-
-int lsx_ctx_release_to(lsx_ctx* ctx, void* stream) {
-    LSX_ENSURE(ctx, "context is NULL");
-    if ((cudaStream_t)stream == ctx->stream) return LSX_OK;
-    DeviceScope scope(ctx->device);
-    LSX_CUDA(scope.status, "select device");
-    if (!ctx->left) LSX_CUDA(cudaEventCreateWithFlags(&ctx->left, cudaEventDisableTiming), "ordering event");
-    LSX_CUDA(cudaEventRecord(ctx->left, ctx->stream), "record on the context's stream");
-    LSX_CUDA(cudaStreamWaitEvent((cudaStream_t)stream, ctx->left, 0), "wait for the context's stream");
     return LSX_OK;
 }
 

@@ -7,12 +7,10 @@ The reference scores one target per row on the host (attribution::loss,
 src/attribution.rs:49-60); these work on torch CUDA tensors: `logits` [rows, vocab]
 of float32, float16 or bfloat16 with unit stride along the vocabulary and any stride
 between rows, token ids as int32 (-1 for an unused slot; another id outside the
-vocabulary makes the results it enters NaN).  Calls are ordered with torch's current
-stream on the Gpu's device: they run on the library's stream after what the current
-stream holds, and the current stream waits for them.  Nothing is copied to the host;
-under a stream capture the kernels join the captured graph.  `out` takes tensors to
-write instead of new ones, in the order of the results (None where a result is not
-wanted)."""
+vocabulary makes the results it enters NaN).  Calls enqueue on torch's current stream
+on the Gpu's device, as torch's own operations do, copy nothing to the host and may be
+captured into a CUDA graph.  `out` takes tensors to write instead of new ones, in the
+order of the results (None where a result is not wanted)."""
 from __future__ import annotations
 
 import ctypes as C
@@ -24,6 +22,7 @@ from ._lib import BF16, F16, F32, check, lib
 from .gpu import Gpu
 
 _KINDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
+_DEFAULT_STREAM = 1  # cudaStreamLegacy
 MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
 
 
@@ -46,7 +45,7 @@ def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
     """(rows, vocab, stride, kind) of a matrix of rows on the Gpu's device."""
     if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _KINDS:
         raise ValueError(f"{name} must be a [rows, vocab] tensor of float32, float16 or bfloat16")
-    if not logits.is_cuda or logits.device.index != gpu.device:
+    if logits.get_device() != gpu.device:
         raise ValueError(f"{name} must be on the Gpu's device")
     rows, vocab = logits.shape
     if vocab < 1:
@@ -61,9 +60,9 @@ def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
 
 def _vector(gpu: Gpu, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
     """Address of a contiguous tensor of this shape and type on the Gpu's device."""
-    if not isinstance(t, torch.Tensor) or t.shape != shape or t.dtype != dtype:
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}")
-    if not t.is_cuda or t.device.index != gpu.device or not t.is_contiguous():
+    if t.get_device() != gpu.device or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous on the Gpu's device")
     return t.data_ptr()
 
@@ -83,19 +82,9 @@ def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
     return out, _rows(gpu, out, "the gradient")[2]
 
 
-class _Ordered:
-    """Runs a block on the library's stream, ordered with torch's current stream."""
-
-    def __init__(self, gpu: Gpu):
-        self.handle = gpu.handle
-        self.stream = torch.cuda.current_stream(gpu.device).cuda_stream
-
-    def __enter__(self):
-        check(lib.lsx_ctx_wait_for(self.handle, self.stream))
-
-    def __exit__(self, *exc):
-        check(lib.lsx_ctx_release_to(self.handle, self.stream))
-        return False
+def _stream(gpu: Gpu) -> int:
+    """torch's current stream on the Gpu's device, as lsx.h takes it."""
+    return torch.cuda.current_stream(gpu.device).cuda_stream or _DEFAULT_STREAM
 
 
 def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0,
@@ -118,12 +107,10 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
     at = [_vector(gpu, t, s, d, f"out[{i}]") if t is not None and t.numel() else None
           for i, (t, (s, d)) in enumerate(zip(out, shapes))]
     given = _vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None
-    result = TokenLogprobs(*out)
     if rows:
-        with _Ordered(gpu):
-            check(lib.lsx_token_logprobs_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
-                                                given, n, k, *at))
-    return result
+        check(lib.lsx_token_logprobs_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
+                                            given, n, k, *at, _stream(gpu)))
+    return TokenLogprobs(*out)
 
 
 def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None, stats: torch.Tensor,
@@ -145,9 +132,8 @@ def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor
           _vector(gpu, logprob_gradient, (rows, n), f32, "logprob_gradient") if n else None,
           _vector(gpu, entropy_gradient, (rows,), f32, "entropy_gradient") if entropy_gradient is not None else None)
     if rows:
-        with _Ordered(gpu):
-            check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
-                                                         temperature, *at, out.data_ptr(), out_stride))
+        check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
+                                                     temperature, *at, out.data_ptr(), out_stride, _stream(gpu)))
     return out
 
 
@@ -184,9 +170,8 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
           _vector(gpu, out[0], (rows,), f32, "out[0]") if out[0] is not None else None,
           _vector(gpu, out[1], (rows, 3), f32, "out[1]") if out[1] is not None else None)
     if rows:
-        with _Ordered(gpu):
-            check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
-                                         *teacher, *at, grad.data_ptr() if gradient else None, grad_stride))
+        check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature, *teacher,
+                                     *at, grad.data_ptr() if gradient else None, grad_stride, _stream(gpu)))
     return Distillation(out[0], out[1], grad)
 
 
@@ -201,9 +186,8 @@ def distill_backward(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, 
     at = (_vector(gpu, stats, (rows, 3), torch.float32, "stats"),
           _vector(gpu, loss_gradient, (rows,), torch.float32, "loss_gradient"))
     if rows:
-        with _Ordered(gpu):
-            check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
-                                                  temperature, *teacher, *at, out.data_ptr(), out_stride))
+        check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
+                                              *teacher, *at, out.data_ptr(), out_stride, _stream(gpu)))
     return out
 
 

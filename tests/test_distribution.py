@@ -18,28 +18,28 @@ def message():
 
 def logprobs(**change):
     a = dict(ctx=None, logits=A, kind=F32, rows=4, vocab=10, stride=10, temperature=1.0, tokens=B, count=2, k=3,
-             logprob=D, entropy=D, stats=D, ids=D, top=D, lp=D)
+             logprob=D, entropy=D, stats=D, ids=D, top=D, lp=D, stream=None)
     a.update(change)
     return lib.lsx_token_logprobs_device(*a.values())
 
 
 def logprobs_backward(**change):
     a = dict(ctx=None, logits=A, kind=F32, rows=4, vocab=10, stride=10, temperature=1.0, tokens=B, count=2, stats=D,
-             entropy=D, g=D, h=D, out=B, out_stride=10)
+             entropy=D, g=D, h=D, out=B, out_stride=10, stream=None)
     a.update(change)
     return lib.lsx_token_logprobs_backward_device(*a.values())
 
 
 def distill(**change):
     a = dict(ctx=None, logits=A, kind=F32, rows=4, vocab=10, stride=10, temperature=1.0, ids=D, values=D, count=2,
-             tstats=D, weights=D, loss=D, stats=D, out=B, out_stride=10)
+             tstats=D, weights=D, loss=D, stats=D, out=B, out_stride=10, stream=None)
     a.update(change)
     return lib.lsx_distill_device(*a.values())
 
 
 def distill_backward(**change):
     a = dict(ctx=None, logits=A, kind=F32, rows=4, vocab=10, stride=10, temperature=1.0, ids=D, values=D, count=2,
-             tstats=D, stats=D, g=D, out=B, out_stride=10)
+             tstats=D, stats=D, g=D, out=B, out_stride=10, stream=None)
     a.update(change)
     return lib.lsx_distill_backward_device(*a.values())
 
@@ -143,8 +143,3 @@ def test_python_refuses_what_is_not_on_the_device():
         distribution.token_logprobs(FakeGpu(), z[0])
     with pytest.raises(ValueError, match="float32"):
         distribution.distill(FakeGpu(), z.int(), z.int(), z)
-
-
-@pytest.mark.parametrize("stream", [1, 2])
-def test_ordering_needs_a_context(stream):
-    assert lib.lsx_ctx_wait_for(None, stream) == 1 and lib.lsx_ctx_release_to(None, stream) == 1
