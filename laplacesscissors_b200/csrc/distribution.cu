@@ -25,7 +25,6 @@ namespace lsx {
 namespace {
 
 constexpr int kRowThreads = 512;
-constexpr int kRowWarps = kRowThreads / 32;
 constexpr int kListCap = 2048;     // candidate keys of one selection
 constexpr int kMarkWords = 512;    // 32-bit words of the bitmap of marked vectors
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
@@ -36,6 +35,15 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kLowestExponent = -1e4f;
 // A thread's reference is moved up once a logit lies this many powers of two above it.
 constexpr float kSlack = 20.f;
+
+// What only the temperature decides.
+struct Scale {
+    float L;        // log2 e / T
+    float inverse;  // 1 / T
+    float slack;    // kSlack powers of two as a difference of logits
+    explicit Scale(double temperature)
+        : L((float)(1.4426950408889634 / temperature)), inverse((float)(1.0 / temperature)), slack(kSlack / L) {}
+};
 
 // ---- 16 bytes of logits ------------------------------------------------------
 template <typename E>
@@ -51,6 +59,10 @@ struct Vec<float> {
     }
     static __device__ __forceinline__ uint4 pack(const float* v) {
         return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static __device__ __forceinline__ float top(uint4 w) {
+        return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)),
+                     fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
     }
     static __device__ __forceinline__ float one(float x) { return x; }
     static __device__ __forceinline__ float store(float x) { return x; }
@@ -76,6 +88,11 @@ struct Vec<__half> {
         }
         return make_uint4(u[0], u[1], u[2], u[3]);
     }
+    static __device__ __forceinline__ float top(uint4 w) {
+        const __half2* h = reinterpret_cast<const __half2*>(&w);
+        const __half2 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(a), __high2float(a));
+    }
     static __device__ __forceinline__ float one(__half x) { return __half2float(x); }
     static __device__ __forceinline__ __half store(float x) { return __float2half_rn(x); }
 };
@@ -98,6 +115,11 @@ struct Vec<__nv_bfloat16> {
             u[i] = *reinterpret_cast<const uint32_t*>(&h);
         }
         return make_uint4(u[0], u[1], u[2], u[3]);
+    }
+    static __device__ __forceinline__ float top(uint4 w) {
+        const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+        const __nv_bfloat162 a = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+        return fmaxf(__low2float(a), __high2float(a));
     }
     static __device__ __forceinline__ float one(__nv_bfloat16 x) { return __bfloat162float(x); }
     static __device__ __forceinline__ __nv_bfloat16 store(float x) { return __float2bfloat16_rn(x); }
@@ -154,6 +176,23 @@ struct Row {
             const long long i = first(j) + e;
             v[e] = i >= 0 && i < vocab ? Vec<E>::one(base[(long long)j * Vec<E>::n + e]) : -INFINITY;
         }
+    }
+};
+
+// One block's share of a row that `parts` blocks divide.
+struct Slice {
+    int lo, hi;      // full vectors
+    int begin, end;  // elements, the ragged ends included
+    bool head, last;
+    template <typename E>
+    __device__ __forceinline__ Slice(const Row<E>& row, int part, int parts) {
+        const long long full = row.full1 - row.full0;
+        lo = row.full0 + (int)(full * part / parts);
+        hi = row.full0 + (int)(full * (part + 1) / parts);
+        head = row.head && part == 0;
+        last = row.last && part == parts - 1;
+        begin = part == 0 ? 0 : (int)row.first(lo);
+        end = part == parts - 1 ? row.vocab : (int)row.first(hi);
     }
 };
 
@@ -233,138 +272,147 @@ __device__ __forceinline__ int mark_position(const Marks& M, long long first) {
     return lo;
 }
 
-// ---- block reductions ----------------------------------------------------------
-struct BlockScratch {
-    float f[3][32];
-};
-__device__ __forceinline__ float block_max(float v, float* scratch) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = scratch[0];
-    for (int w = 1; w < (int)(blockDim.x >> 5); ++w) v = fmaxf(v, scratch[w]);
-    return v;
-}
-__device__ __forceinline__ float block_sum(float v, float* scratch) {
-    v = warp_allsum(v);
-    if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-    __syncthreads();
-    v = 0.f;
-    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) v += scratch[w];
-    return v;
-}
-
 // ---- running sums of a softmax ---------------------------------------------------
-// S = sum 2^y and W = sum 2^y y over the elements seen, y against the reference r;
-// S == 0 exactly while only -inf has been seen.
-// With kRanked also the first vector holding the largest element, and the largest
-// element of the other vectors.
-template <bool kWeighted, bool kRanked = false>
+// S = sum 2^y and W = sum 2^y y over the elements seen (in two halves), y against the
+// reference r; S == 0 exactly while only -inf has been seen.  m is the largest element,
+// `at` the first vector that holds it and `second` the largest element of the others.
 struct Running {
-    float r = 0.f, limit = -INFINITY, S = 0.f, W = 0.f, m = -INFINITY;
-    float second = -INFINITY;
+    float r = 0.f, limit = -INFINITY, m = -INFINITY, second = -INFINITY;
+    float2 S2 = {0.f, 0.f}, W2 = {0.f, 0.f};
     int at = -1;
-    __device__ __forceinline__ void rise(float top, float L, float slack) {
-        if (S != 0.f) {
-            const float shift = (r - top) * L;
+    __device__ __forceinline__ void rise(float top, const Scale& k) {
+        if (S2.x + S2.y != 0.f) {
+            const float shift = (r - top) * k.L;
             const float f = exp2_fast(shift);
-            if (kWeighted) W = f > 0.f ? f * fmaf(shift, S, W) : (f == 0.f ? 0.f : f);
-            S *= f;
+            const bool none = f == 0.f;
+            W2.x = none ? 0.f : f * fmaf(shift, S2.x, W2.x);
+            W2.y = none ? 0.f : f * fmaf(shift, S2.y, W2.y);
+            S2.x *= f;
+            S2.y *= f;
         }
         r = top;
-        limit = top + slack;
+        limit = top + k.slack;
     }
     template <int n>
-    __device__ __forceinline__ void add(const float* v, int j, float L, float slack) {
+    __device__ __forceinline__ void add(const float* v, float top, int j, const Scale& k) {
+        second = fmaxf(second, fminf(m, top));
+        at = top > m ? j : at;
+        m = fmaxf(m, top);
+        if (top > limit) rise(top, k);
+        const float2 back = {-r, -r}, scale = {k.L, k.L};
+#pragma unroll
+        for (int e = 0; e < n; e += 2) {
+            float2 y = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), back), scale);
+            y.x = max_nan(y.x, kLowestExponent);
+            y.y = max_nan(y.y, kLowestExponent);
+            const float2 p = {exp2_fast(y.x), exp2_fast(y.y)};
+            S2 = __fadd2_rn(S2, p);
+            W2 = __ffma2_rn(p, y, W2);
+        }
+    }
+};
+
+// Sums over several threads, against their own maximum.
+struct Sums {
+    float m, S, W;
+    // The same sums against M >= m.
+    __device__ __forceinline__ void rebase(float M, float L) {
+        if (S == 0.f) return;
+        const float shift = (m - M) * L;
+        const float f = exp2_fast(shift);
+        W = f == 0.f ? 0.f : f * fmaf(shift, S, W);
+        S = f == 0.f && S == S ? 0.f : f * S;
+    }
+};
+
+__device__ __forceinline__ Sums warp_sums(Sums x, float L) {
+    float M = x.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    x.rebase(M, L);
+    return {M, warp_allsum(x.S), warp_allsum(x.W)};
+}
+
+// The block's sums, in every thread.  `scratch` holds one entry per warp and is free
+// again after the caller's next block barrier.
+__device__ __forceinline__ Sums block_sums(const Running& a, float L, Sums* scratch) {
+    Sums x{a.r, a.S2.x + a.S2.y, a.W2.x + a.W2.y};
+    float M = a.m;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
+    x.rebase(M, L);
+    x = {M, warp_allsum(x.S), warp_allsum(x.W)};
+    const int lane = threadIdx.x & 31;
+    if (lane == 0) scratch[threadIdx.x >> 5] = x;
+    __syncthreads();
+    x = lane < (int)(blockDim.x >> 5) ? scratch[lane] : Sums{-INFINITY, 0.f, 0.f};
+    return warp_sums(x, L);
+}
+
+template <typename E, bool kExclude>
+__device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& part, const Marks* M, const Scale& k,
+                                             Running& acc) {
+    constexpr int n = Vec<E>::n;
+    auto exclude = [&](int j, float* v) {
+        int pos = mark_position(*M, row.first(j));
+#pragma unroll
+        for (int e = 0; e < n; ++e)
+            while (pos < M->count && (long long)M->ids[pos] == row.first(j) + e) {
+                v[e] = -INFINITY;
+                ++pos;
+            }
+    };
+    auto take = [&](int j, uint4 w) {
+        float v[n];
+        Vec<E>::unpack(w, v);
+        float top = Vec<E>::top(w);
+        if (kExclude && marked(*M, j)) {
+            exclude(j, v);
+            top = v[0];
+#pragma unroll
+            for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
+        }
+        acc.template add<n>(v, top, j, k);
+    };
+    auto take_ragged = [&](int j) {
+        float v[n];
+        row.ragged(j, v);
+        if (kExclude) exclude(j, v);
         float top = v[0];
 #pragma unroll
         for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
-        if (kRanked) {
-            second = fmaxf(second, fminf(m, top));
-            at = top > m ? j : at;
-        }
-        m = fmaxf(m, top);
-        if (top > limit) rise(top, L, slack);
-#pragma unroll
-        for (int e = 0; e < n; ++e) {
-            const float y = max_nan((v[e] - r) * L, kLowestExponent);
-            const float p = exp2_fast(y);
-            S += p;
-            if (kWeighted) W = fmaf(p, y, W);
-        }
-    }
-    // Moves the sums to the reference R >= every element seen.
-    __device__ __forceinline__ void rebase(float R, float L) {
-        if (S == 0.f) return;
-        const float shift = (r - R) * L;
-        const float f = exp2_fast(shift);
-        if (kWeighted) W = f > 0.f ? f * fmaf(shift, S, W) : (f == 0.f ? 0.f : f);
-        S = f == 0.f && S == S ? 0.f : f * S;
-        r = R;
-    }
-};
-
-template <typename E, bool kExclude, bool kWeighted, bool kRanked>
-__device__ __forceinline__ void stream_row(const Row<E>& row, const Marks* M, float L, float slack,
-                                           Running<kWeighted, kRanked>& acc) {
-    constexpr int n = Vec<E>::n;
-    auto take = [&](int j, float* v) {
-        if (kExclude && marked(*M, j)) {
-            int pos = mark_position(*M, row.first(j));
-#pragma unroll
-            for (int e = 0; e < n; ++e)
-                while (pos < M->count && (long long)M->ids[pos] == row.first(j) + e) {
-                    v[e] = -INFINITY;
-                    ++pos;
-                }
-        }
-        acc.template add<n>(v, j, L, slack);
+        acc.template add<n>(v, top, j, k);
     };
     const int tid = threadIdx.x, T = blockDim.x;
-    int j = row.full0 + tid;
+    int j = part.lo + tid;
     // every thread meets its vectors in ascending order
-    if (row.head && tid == 0) {
-        float v[n];
-        row.ragged(0, v);
+    if (part.head && tid == 0) {
         acc.at = 0;
-        take(0, v);
-    } else if (j < row.full1) {
+        take_ragged(0);
+    } else if (j < part.hi) {
         acc.at = j;
-    } else if (row.last && tid == T - 1) {
+    } else if (part.last && tid == T - 1) {
         acc.at = row.full1;
     }
-    for (; j + (kUnroll - 1) * T < row.full1; j += kUnroll * T) {
+    for (; j + (kUnroll - 1) * T < part.hi; j += kUnroll * T) {
         uint4 w[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float v[n];
-            Vec<E>::unpack(w[u], v);
-            take(j + u * T, v);
-        }
+        for (int u = 0; u < kUnroll; ++u) take(j + u * T, w[u]);
     }
-    for (; j < row.full1; j += T) {
-        float v[n];
-        Vec<E>::unpack(row.full(j), v);
-        take(j, v);
-    }
-    if (row.last && tid == T - 1) {
-        float v[n];
-        row.ragged(row.full1, v);
-        take(row.full1, v);
-    }
+    for (; j < part.hi; j += T) take(j, row.full(j));
+    if (part.last && tid == T - 1) take_ragged(row.full1);
 }
 
 // Where one token holds nearly all the mass, 1 + rest in f32 keeps little of the rest, and
-// ln(1 + rest) and the entropy are all rest.  For such rows one warp sums the vectors of
-// the thread that met the maximum `m` once more, leaving the maximum out; the other
-// threads' sums hold nothing of it.  Returns the sums over that thread's other elements.
+// ln(1 + rest) and the entropy are all rest.  For such sums one warp adds up the vectors of
+// the thread that met the maximum once more, leaving the maximum out; the other threads'
+// sums hold nothing of it.
 constexpr float kPeaked = 1.0625f;
 
 template <typename E>
-__device__ void sum_without_maximum(const Row<E>& row, int owner, float m, float L, float& S, float& W) {
+__device__ Sums sum_without_maximum(const Row<E>& row, const Slice& part, int owner, float m, float L) {
     constexpr int n = Vec<E>::n;
     float s = 0.f, w = 0.f;
     auto take = [&](const float* v) {
@@ -379,20 +427,93 @@ __device__ void sum_without_maximum(const Row<E>& row, int owner, float m, float
     };
     const int lane = threadIdx.x & 31, T = blockDim.x;
     float v[n];
-    for (long long j = (long long)row.full0 + owner + (long long)lane * T; j < row.full1; j += 32ll * T) {
+    for (long long j = (long long)part.lo + owner + (long long)lane * T; j < part.hi; j += 32ll * T) {
         Vec<E>::unpack(row.full((int)j), v);
         take(v);
     }
-    if (lane == 0 && row.head && owner == 0) {
+    if (lane == 0 && part.head && owner == 0) {
         row.ragged(0, v);
         take(v);
     }
-    if (lane == 0 && row.last && owner == T - 1) {
+    if (lane == 0 && part.last && owner == T - 1) {
         row.ragged(row.full1, v);
         take(v);
     }
-    S = warp_allsum(s);
-    W = warp_allsum(w);
+    return {m, warp_allsum(s), warp_allsum(w)};
+}
+
+// A block's share of a row's sums as the blocks of a cluster exchange it: the largest
+// element counted as 1 and the rest apart.
+struct Partial {
+    float m, rest, W;
+    int any;  // 0: nothing but -inf
+};
+
+template <typename E>
+__device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Running& acc, const Scale& k, Sums* scratch,
+                              int* owner) {
+    const Sums x = block_sums(acc, k.L, scratch);
+    Partial p{x.m, x.S - 1.f, x.W, x.S != 0.f};
+    if (x.S != 0.f && x.S < kPeaked) {  // the maximum is unique
+        if (acc.m == x.m) *owner = threadIdx.x;
+        __syncthreads();
+        Running others = acc;
+        if ((int)threadIdx.x == *owner) {
+            others = Running();
+            others.m = x.m;
+        }
+        if (threadIdx.x < 32) {
+            const Sums again = sum_without_maximum(row, part, *owner, x.m, k.L);
+            // (a thread's own element at x.m, if any, went with the owner's sums)
+            scratch[32] = again;
+        }
+        const Sums rest = block_sums(others, k.L, scratch);
+        __syncthreads();
+        p.rest = rest.S + scratch[32].S;
+        p.W = rest.W + scratch[32].W;
+    }
+    return p;
+}
+
+// The row's sums from its blocks' shares.
+__device__ __forceinline__ Partial combine(const Partial* parts, int count, float L) {
+    Partial t = parts[0];
+    if (count == 1) return t;
+    int first = 0;
+    for (int i = 1; i < count; ++i)
+        if (parts[i].any && (!t.any || parts[i].m > t.m)) {
+            t = parts[i];
+            first = i;
+        }
+    for (int i = 0; i < count; ++i) {
+        if (i == first || !parts[i].any) continue;
+        Sums x{parts[i].m, 1.f + parts[i].rest, parts[i].W};
+        x.rebase(t.m, L);
+        t.rest += x.S;
+        t.W += x.W;
+    }
+    return t;
+}
+
+// ---- thread-block clusters --------------------------------------------------------------
+__device__ __forceinline__ int cluster_size() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(n));
+    return (int)n;
+}
+__device__ __forceinline__ int cluster_rank() {
+    uint32_t n;
+    asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(n));
+    return (int)n;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
+// `local`, a shared-memory address of this block, in block `rank` of the cluster.
+template <typename V>
+__device__ __forceinline__ V* in_block(V* local, int rank) {
+    uint64_t p;
+    asm("mapa.u64 %0, %1, %2;" : "=l"(p) : "l"(reinterpret_cast<uint64_t>(local)), "r"(rank));
+    return reinterpret_cast<V*>(p);
 }
 
 // ---- top alternatives --------------------------------------------------------------
@@ -407,77 +528,86 @@ __device__ __forceinline__ uint32_t key_id(unsigned long long k) { return 0xffff
 __device__ __forceinline__ float key_logit(unsigned long long k) { return total_order_value((uint32_t)(k >> 32)); }
 
 constexpr int kMaxGroups = 256;
+constexpr int kMaxCluster = 8;     // the portable size
 
 struct Selection {
     alignas(16) unsigned long long keys[kListCap];
     alignas(16) unsigned long long group[kMaxGroups];
     unsigned long long best[kMaxSlots];
     unsigned long long threshold;
-    int rescan[kRowThreads];
+    int rescan[kRowThreads], offered[kRowThreads];
     int count, rescans;
 };
 
 // The `top` largest of keys[0..n) (all distinct), in descending order, into best and
-// to the front of keys; returns how many there are.  Ends with the block synchronised.
-__device__ int rank_keys(Selection& P, int n, int top) {
+// to the front of keys; returns how many there are.  `keys` has room for one key more.
+// Starts and ends with the block synchronised.
+__device__ int rank_keys(Selection& P, unsigned long long* keys, int n, int top) {
+    if (threadIdx.x == 0 && (n & 1)) keys[n] = 0ull;
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const unsigned long long key = P.keys[i];
+        const unsigned long long key = keys[i];
         int rank = 0;
-        for (int j = 0; j < n; ++j) rank += P.keys[j] > key;
+#pragma unroll 4
+        for (int j = 0; j < n; j += 2) {
+            const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&keys[j]);
+            rank += (pair.x > key) + (pair.y > key);
+        }
         if (rank < top) P.best[rank] = key;
     }
     __syncthreads();
-    const int have = n < top ? n : top;
-    for (int i = threadIdx.x; i < have; i += blockDim.x) P.keys[i] = P.best[i];
-    __syncthreads();
-    return have;
+    return n < top ? n : top;
 }
 
-// The row's `top` best tokens, piece by piece: what beats the worst kept key joins the
-// list, which is then cut to its best `top`.  Exact for any row.
+// The `top` best tokens of elements [begin, end) of a row, piece by piece: what beats the
+// worst kept key joins the list, which is then cut to its best `top`.  Exact for any row.
 template <typename E>
-__device__ int select_by_pieces(Selection& P, const E* z, int vocab, int top) {
+__device__ void select_by_pieces(Selection& P, const E* z, int begin, int end, int top, int cap) {
     int have = 0;
-    const int piece = kListCap - kMaxSlots;
-    for (int start = 0; start < vocab; start += piece) {
+    const int piece = cap - kMaxSlots - 1;
+    __syncthreads();
+    for (int start = begin; start < end; start += piece) {
         if (threadIdx.x == 0) P.count = have;
         __syncthreads();
         const unsigned long long worst = have == top ? P.keys[top - 1] : 0ull;
-        const int end = vocab - start < piece ? vocab : start + piece;
-        for (int i = start + threadIdx.x; i < end; i += blockDim.x) {
+        const int stop = end - start < piece ? end : start + piece;
+        for (int i = start + threadIdx.x; i < stop; i += blockDim.x) {
             const unsigned long long key = order_key(Vec<E>::one(z[i]), (uint32_t)i);
             if (key > worst) P.keys[atomicAdd(&P.count, 1)] = key;
         }
         __syncthreads();
         const int n = P.count;
-        if (n > have) have = rank_keys(P, n, top);
+        if (n > have) {
+            have = rank_keys(P, P.keys, n, top);
+            for (int i = threadIdx.x; i < have; i += blockDim.x) P.keys[i] = P.best[i];
+        }
         __syncthreads();
     }
-    return have;
 }
 
-// The row's `top` best tokens from what the threads met while they summed it.  The
+// The best tokens of a slice from what the threads met while they summed it.  The
 // threads form groups; the `top`-th best of the groups' best vectors, ordered by (its
-// largest logit, lower vector number first), bounds the row's `top`-th best element from
-// below: `top` elements, one in each better group, are at least as good.  So only elements
-// at or above that bound are candidates: about G ln(1 / (1 - top / G)) of them where the
-// tokens lie at random over G groups.  They are read again (from L2) at the threads' best vectors, and in
-// all vectors only of threads that have a second one to offer.  More candidates than the
-// list holds (rows in order) are left to select_by_pieces.
+// largest logit, lower vector number first), bounds the `top`-th best element from below:
+// `top` elements, one in each better group, are at least as good.  So only elements at or
+// above that bound are candidates, about G ln(1 / (1 - top / G)) of them where the tokens
+// lie at random over G groups.  They are read again (from L2) at the threads' best
+// vectors, and in all vectors only of threads that have a second one to offer.  More
+// candidates than the list holds (rows in order) are left to select_by_pieces.
 template <typename E>
-__device__ void select_by_threads(Selection& P, const Row<E>& row, const E* z, int top, float m, float second, int at) {
+__device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& part, const E* z, int top,
+                                  const Running& acc, int cap) {
     constexpr int n = Vec<E>::n;
     const int tid = threadIdx.x, lane = tid & 31, T = blockDim.x;
-    const int wide = top > 64 ? 2 : 4, groups = T / wide;
+    const int wide = top * 8 > T ? (top * 4 > T ? 1 : 2) : 4, groups = T / wide;
     const unsigned long long mine =
-        at < 0 ? 0ull : ((unsigned long long)total_order_key(m + 0.f) << 32) | (0xffffffffu - (uint32_t)at);
+        acc.at < 0 ? 0ull : ((unsigned long long)total_order_key(acc.m + 0.f) << 32) | (0xffffffffu - (uint32_t)acc.at);
     unsigned long long best = mine;
     for (int o = 1; o < wide; o <<= 1) {
         const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
         best = other > best ? other : best;
     }
     if (tid % wide == 0) P.group[tid / wide] = best;
+    P.offered[tid] = acc.at;
     if (tid == 0) {
         P.threshold = 0ull;
         P.count = P.rescans = 0;
@@ -486,6 +616,7 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const E* z, i
     if (tid < groups) {
         const unsigned long long key = P.group[tid];
         int above = 0;
+#pragma unroll 8
         for (int i = 0; i < groups; i += 2) {
             const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&P.group[i]);
             above += (pair.x > key) + (pair.y > key);
@@ -502,112 +633,112 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const E* z, i
             const unsigned long long key = ((unsigned long long)total_order_key(v[e] + 0.f) << 32) | low;
             if (key >= threshold && i >= 0 && i < row.vocab) {
                 const int pos = atomicAdd(&P.count, 1);
-                if (pos < kListCap) P.keys[pos] = order_key(v[e], (uint32_t)i);
+                if (pos < cap) P.keys[pos] = order_key(v[e], (uint32_t)i);
             }
         }
-    };
-    auto read = [&](int j, float* v) {
-        if (j >= row.full0 && j < row.full1)
-            Vec<E>::unpack(row.full(j), v);
-        else
-            row.ragged(j, v);
     };
     if (mine != 0ull && mine >= threshold) {
         float v[n];
-        read(at, v);
-        offer(at, v);
-        if (total_order_key(second + 0.f) >= (uint32_t)(threshold >> 32)) P.rescan[atomicAdd(&P.rescans, 1)] = tid;
+        if (acc.at >= row.full0 && acc.at < row.full1)
+            Vec<E>::unpack(row.full(acc.at), v);
+        else
+            row.ragged(acc.at, v);
+        offer(acc.at, v);
+        if (total_order_key(acc.second + 0.f) >= (uint32_t)(threshold >> 32)) P.rescan[atomicAdd(&P.rescans, 1)] = tid;
     }
-    // the best vector of a rescanned thread was offered by the thread itself
-    __shared__ int offered[kRowThreads];
-    offered[tid] = at;
     __syncthreads();
     const int rescans = P.rescans;
     for (int q = tid >> 5; q < rescans; q += T >> 5) {
-        const int who = P.rescan[q], skip = offered[who];
+        const int who = P.rescan[q], skip = P.offered[who];
         float v[n];
-        for (int j = row.full0 + who + lane * T; j < row.full1; j += 32 * T)
+        for (long long j = (long long)part.lo + who + (long long)lane * T; j < part.hi; j += 32ll * T)
             if (j != skip) {
-                read(j, v);
-                offer(j, v);
+                Vec<E>::unpack(row.full((int)j), v);
+                offer((int)j, v);
             }
-        if (lane == 0 && row.head && who == 0 && skip != 0) {
+        if (lane == 0 && part.head && who == 0 && skip != 0) {
             row.ragged(0, v);
             offer(0, v);
         }
-        if (lane == 0 && row.last && who == T - 1 && skip != row.full1) {
+        if (lane == 0 && part.last && who == T - 1 && skip != row.full1) {
             row.ragged(row.full1, v);
             offer(row.full1, v);
         }
     }
     __syncthreads();
-    if (P.count > kListCap) {
-        select_by_pieces<E>(P, z, row.vocab, top);
+    if (P.count >= cap) {
+        select_by_pieces<E>(P, z, part.begin, part.end, top, cap);
         return;
     }
-    rank_keys(P, P.count, top);
+    rank_keys(P, P.keys, P.count, top);
 }
 
 // ---- token_logprobs ------------------------------------------------------------------
-template <typename E>
-__global__ void __launch_bounds__(kRowThreads) token_logprobs_kernel(
-    const E* __restrict__ logits, int vocab, size_t stride, double temperature, const uint32_t* __restrict__ tokens,
-    int token_count, int top, LogprobOutputs out) {
-    __shared__ BlockScratch scratch;
+// One cluster of blocks per row (one block where there are rows enough): the blocks sum
+// and rank their slices and send sums and best keys to the first one's shared memory,
+// which puts them together and writes the row's results.
+template <typename E, int T>
+__global__ void __launch_bounds__(T) token_logprobs_kernel(const E* __restrict__ logits, int vocab, size_t stride,
+                                                          const Scale k, const uint32_t* __restrict__ tokens,
+                                                          int token_count, int top, LogprobOutputs out) {
+    __shared__ Sums scratch[33];
+    __shared__ Partial shares[kMaxCluster];
     __shared__ Selection selection;
     __shared__ int owner;
-    const size_t r = blockIdx.x;
+    const int parts = cluster_size(), part = cluster_rank();
+    if (parts > 1) cluster_arrive();  // waited for before the first store into another block
+    const size_t r = blockIdx.x / parts;
     const E* z = logits + r * stride;
-    const Row<E> row(z, vocab);
-    const float L = (float)(1.4426950408889634 / temperature), slack = kSlack / L;
-    Running<true, true> acc;
-    stream_row<E, false>(row, nullptr, L, slack, acc);
-    const float m = block_max(acc.m, scratch.f[0]);
-    acc.rebase(m, L);
-    float S = block_sum(acc.S, scratch.f[1]);
-    float W = block_sum(acc.W, scratch.f[2]);
-    const bool empty = S == 0.f;  // every logit is -inf
-    float log_sum = empty ? 0.f : logf(S);
-    if (!empty && S < kPeaked) {  // the maximum is unique
-        if (acc.m == m) owner = threadIdx.x;
-        __syncthreads();
-        float s = 0.f, w = 0.f;
-        if (threadIdx.x < 32) sum_without_maximum(row, owner, m, L, s, w);
-        const bool mine = (int)threadIdx.x == owner;
-        s = (mine ? 0.f : acc.S) + (threadIdx.x == 0 ? s : 0.f);
-        w = (mine ? 0.f : acc.W) + (threadIdx.x == 0 ? w : 0.f);
-        s = block_sum(s, scratch.f[0]);
-        W = block_sum(w, scratch.f[1]);
-        S = 1.f + s;
-        log_sum = log1pf(s);
+    // the given token's logit is on its way while the row streams
+    uint32_t token = kUnusedToken;
+    float given = 0.f;
+    const bool asked = part == 0 && out.logprob && (int)threadIdx.x < token_count;
+    if (asked) {
+        token = tokens[r * token_count + threadIdx.x];
+        if (token < (uint32_t)vocab) given = Vec<E>::one(z[token]);
     }
-    const float inverse = (float)(1.0 / temperature);
-    auto logprob = [&](float x) { return empty && x == x ? -INFINITY : (x - m) * inverse - log_sum; };
+    const Row<E> row(z, vocab);
+    const Slice slice(row, part, parts);
+    Running acc;
+    stream_slice<E, false>(row, slice, nullptr, k, acc);
+    Partial sums = slice_sums(row, slice, acc, k, scratch, &owner);
+    // clusters keep the upper half of the list for the blocks' best keys
+    const int cap = parts > 1 ? kListCap / 2 : kListCap;
+    if (top > 0) {
+        if (sums.rest == sums.rest)
+            select_by_threads<E>(selection, row, slice, z, top, acc, cap);
+        else  // NaN or +inf here: NaN leads the order and the threads' maxima pass over it
+            select_by_pieces<E>(selection, z, slice.begin, slice.end, top, cap);
+    }
+    if (parts > 1) {
+        cluster_wait();
+        if (threadIdx.x == 0) *in_block(&shares[part], 0) = sums;
+        for (int i = threadIdx.x; i < top; i += T)
+            *in_block(&selection.keys[kListCap / 2 + part * top + i], 0) = selection.best[i];
+        cluster_arrive();
+        cluster_wait();
+        if (part != 0) return;
+        sums = combine(shares, parts, k.L);
+        if (top > 0) rank_keys(selection, selection.keys + kListCap / 2, parts * top, top);
+    }
+    const bool empty = !sums.any;  // every logit is -inf
+    const float m = sums.m, log_sum = empty ? 0.f : log1pf(sums.rest);
+    auto logprob = [&](float x) { return empty ? -INFINITY : (x - m) * k.inverse - log_sum; };
     if (threadIdx.x == 0) {
-        if (out.entropy) out.entropy[r] = empty ? 0.f : log_sum - W / S * kLn2;
+        if (out.entropy) out.entropy[r] = empty ? 0.f : log_sum - sums.W / (1.f + sums.rest) * kLn2;
         if (out.stats) {
             out.stats[2 * r] = m;
             out.stats[2 * r + 1] = log_sum;
         }
     }
-    if (out.logprob)
-        for (int i = threadIdx.x; i < token_count; i += blockDim.x) {
-            const uint32_t t = tokens[r * token_count + i];
-            out.logprob[r * token_count + i] =
-                t == kUnusedToken ? 0.f : t < (uint32_t)vocab ? logprob(Vec<E>::one(z[t])) : NAN;
-        }
-    if (top > 0) {
-        if (S == S)
-            select_by_threads<E>(selection, row, z, top, acc.m, acc.second, acc.at);
-        else  // NaN or +inf in the row: NaN leads the order and the threads' maxima pass over it
-            select_by_pieces<E>(selection, z, vocab, top);
-        for (int i = threadIdx.x; i < top; i += blockDim.x) {
-            const uint32_t id = key_id(selection.best[i]);
-            const float x = key_logit(selection.best[i]);
-            if (out.top_ids) out.top_ids[r * top + i] = id;
-            if (out.top_logits) out.top_logits[r * top + i] = x;
-            if (out.top_logprobs) out.top_logprobs[r * top + i] = logprob(x);
-        }
+    if (asked)
+        out.logprob[r * token_count + threadIdx.x] =
+            token == kUnusedToken ? 0.f : token < (uint32_t)vocab ? logprob(given) : NAN;
+    for (int i = threadIdx.x; i < top; i += T) {
+        const float x = key_logit(selection.best[i]);
+        if (out.top_ids) out.top_ids[r * top + i] = key_id(selection.best[i]);
+        if (out.top_logits) out.top_logits[r * top + i] = x;
+        if (out.top_logprobs) out.top_logprobs[r * top + i] = logprob(x);
     }
 }
 
@@ -693,7 +824,7 @@ __device__ void write_gradient(const Marks& M, const Row<E>& row, E* out, const 
 
 template <typename E>
 __global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
-    const E* logits, int vocab, size_t stride, double temperature, const uint32_t* __restrict__ tokens, int token_count,
+    const E* logits, int vocab, size_t stride, const Scale k, const uint32_t* __restrict__ tokens, int token_count,
     const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ logprob_gradient,
     const float* __restrict__ entropy_gradient, E* gradient, size_t gradient_stride) {
     __shared__ Marks marks;
@@ -701,7 +832,7 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
     const size_t r = blockIdx.x;
     const Row<E> row(logits + r * stride, vocab);
     build_marks(marks, tokens + r * token_count, token_count, row);
-    const float inverse = (float)(1.0 / temperature);
+    const float inverse = k.inverse;
     if (threadIdx.x < 32) {
         float sum = 0.f;
         for (int i = threadIdx.x; i < token_count; i += 32) {
@@ -715,7 +846,7 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
         if (threadIdx.x == 0) total = marks.bad ? NAN : sum;
     }
     __syncthreads();
-    const float L = (float)(1.4426950408889634 / temperature);
+    const float L = k.L;
     const float h = entropy_gradient ? entropy_gradient[r] : 0.f;
     GradientRow g;
     g.m = stats[2 * r];
@@ -815,9 +946,9 @@ __device__ GradientRow distill_gradient_row(Marks& M, const TeacherSlots& slots,
 // are given and only the gradient is written.
 template <typename E, bool kTail, bool kStream>
 __global__ void __launch_bounds__(kRowThreads) distill_kernel(
-    const E* logits, int vocab, size_t stride, double temperature, TeacherRows teacher,
+    const E* logits, int vocab, size_t stride, const Scale k, double T, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
-    __shared__ BlockScratch scratch;
+    __shared__ Sums scratch[33];
     __shared__ Marks marks;
     __shared__ TeacherSlots slots;
     __shared__ GradientRow grow;
@@ -827,17 +958,16 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     build_marks(marks, teacher.ids + r * count, count, row);
-    const double T = temperature;
-    const float L = (float)(1.4426950408889634 / T), slack = kSlack / L;
+    const Slice slice(row, 0, 1);
     float m_rest = -INFINITY, S = 0.f;
     if (kStream) {
         for (int i = threadIdx.x; i < count; i += blockDim.x)
             listed[i] = marks.slot_rank[i] >= 0 ? Vec<E>::one(z[marks.raw[i]]) : -INFINITY;
-        Running<false> acc;
-        stream_row<E, true>(row, &marks, L, slack, acc);
-        m_rest = block_max(acc.m, scratch.f[0]);
-        acc.rebase(m_rest, L);
-        S = block_sum(acc.S, scratch.f[1]);
+        Running acc;
+        stream_slice<E, true>(row, slice, &marks, k, acc);
+        const Sums x = block_sums(acc, k.L, scratch);
+        m_rest = x.m;
+        S = x.S;
     }
     if (threadIdx.x < 32) {
         const TeacherSums t = teacher_row(marks, slots, teacher.logits + r * count,
@@ -892,7 +1022,7 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(
     }
     if (!gradient) return;
     __syncthreads();
-    write_gradient(marks, row, gradient + r * gradient_stride, grow, L, row.full0, row.full1, true, true);
+    write_gradient(marks, row, gradient + r * gradient_stride, grow, k.L, row.full0, row.full1, true, true);
 }
 
 template <typename F>
@@ -904,15 +1034,46 @@ cudaError_t by_kind(lsx_dtype kind, F&& f) {
     }
 }
 
+
+// How many blocks share a row: as many as fill the GPU, while each keeps a full pass of
+// its threads.
+int row_parts(int sm_count, size_t rows, size_t vectors, int threads, int resident) {
+    int parts = 1;
+    while (parts < kMaxCluster && rows * parts * 2 <= (size_t)sm_count * resident &&
+           vectors / (parts * 2) >= (size_t)threads)
+        parts *= 2;
+    return parts;
+}
+
+template <typename... Params, typename... Args>
+cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, cudaStream_t s,
+                            Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(rows * parts));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
+    cfg.attrs = attr;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 }  // namespace
 
-cudaError_t launch_token_logprobs(cudaStream_t s, int, const LogitRows& z, const uint32_t* tokens, size_t token_count,
-                                  size_t alternatives, const LogprobOutputs& out) {
+cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows& z, const uint32_t* tokens,
+                                  size_t token_count, size_t alternatives, const LogprobOutputs& out) {
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
-        token_logprobs_kernel<E><<<(unsigned)z.rows, kRowThreads, 0, s>>>(
-            (const E*)z.data, (int)z.vocab, z.stride, z.temperature, tokens, (int)token_count, (int)alternatives, out);
-        return cudaGetLastError();
+        const size_t vectors = z.vocab / Vec<E>::n;
+        const Scale k(z.temperature);
+        if (vectors < 1024)
+            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
+                                   z.stride, k, tokens, (int)token_count, (int)alternatives, out);
+        return launch_clusters(token_logprobs_kernel<E, 512>, z.rows, row_parts(sm_count, z.rows, vectors, 512, 4), 512,
+                               s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
+                               (int)alternatives, out);
     });
 }
 
@@ -923,7 +1084,7 @@ cudaError_t launch_logprobs_gradient(cudaStream_t s, int, const LogitRows& z, co
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         logprobs_gradient_kernel<E><<<(unsigned)z.rows, kRowThreads, 0, s>>>(
-            (const E*)z.data, (int)z.vocab, z.stride, z.temperature, tokens, (int)token_count, stats, entropy,
+            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), tokens, (int)token_count, stats, entropy,
             logprob_gradient, entropy_gradient, (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
@@ -934,8 +1095,8 @@ cudaError_t launch_distill(cudaStream_t s, int, const LogitRows& z, const Teache
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         auto kernel = teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>;
-        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride, z.temperature,
-                                                        teacher, weights, loss, stats, (E*)gradient, gradient_stride);
+        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride,
+                                                        Scale(z.temperature), z.temperature, teacher, weights, loss, stats, (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
 }
@@ -945,8 +1106,8 @@ cudaError_t launch_distill_gradient(cudaStream_t s, int, const LogitRows& z, con
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         auto kernel = teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>;
-        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride, z.temperature,
-                                                        teacher, weights, nullptr, const_cast<float*>(stats),
+        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride,
+                                                        Scale(z.temperature), z.temperature, teacher, weights, nullptr, const_cast<float*>(stats),
                                                         (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
