@@ -528,35 +528,95 @@ __device__ __forceinline__ uint32_t key_id(unsigned long long k) { return 0xffff
 __device__ __forceinline__ float key_logit(unsigned long long k) { return total_order_value((uint32_t)(k >> 32)); }
 
 constexpr int kMaxGroups = 256;
+constexpr int kFewerCap = 512;
 constexpr int kMaxCluster = 8;     // the portable size
 
 struct Selection {
     alignas(16) unsigned long long keys[kListCap];
+    alignas(16) unsigned long long fewer[kFewerCap];
     alignas(16) unsigned long long group[kMaxGroups];
     unsigned long long best[kMaxSlots];
     unsigned long long threshold;
-    int rescan[kRowThreads], offered[kRowThreads];
-    int count, rescans;
+    int count;
 };
 
-// The `top` largest of keys[0..n) (all distinct), in descending order, into best and
-// to the front of keys; returns how many there are.  `keys` has room for one key more.
-// Starts and ends with the block synchronised.
-__device__ int rank_keys(Selection& P, unsigned long long* keys, int n, int top) {
+// A bound for the `top`-th largest of keys that the threads hold: groups of threads take
+// their largest (`mine`, 0 for none), and the `top`-th largest of the groups' is returned (0
+// where there are not as many).  Distinct keys; `top` of all the keys are at or above the
+// bound.  Resets P.count.  Ends with the block synchronised.
+__device__ unsigned long long group_bound(Selection& P, unsigned long long mine, int top) {
+    const int tid = threadIdx.x, T = blockDim.x;
+    // groups as wide as leave 2.5 groups per wanted key
+    const int wide = top * 10 <= T ? 4 : top * 5 <= T ? 2 : 1, groups = T / wide;
+    for (int o = 1; o < wide; o <<= 1) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
+        mine = other > mine ? other : mine;
+    }
+    if (tid % wide == 0) P.group[tid / wide] = mine;
+    if (tid == 0) {
+        P.threshold = 0ull;
+        P.count = 0;
+    }
+    __syncthreads();
+    // a group's threads share the comparisons of its key
+    int above = 0;
+#pragma unroll 4
+    for (int i = 2 * (tid % wide); i < groups; i += 2 * wide) {
+        const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&P.group[i]);
+        above += (pair.x > mine) + (pair.y > mine);
+    }
+    for (int o = 1; o < wide; o <<= 1) above += __shfl_xor_sync(0xffffffffu, above, o);
+    if (above == top - 1 && mine != 0ull) P.threshold = mine;
+    __syncthreads();
+    return P.threshold;
+}
+
+// The `top` largest of keys[0..n) (distinct) in descending order into P.best; `keys` has
+// room for one more.  Four threads share the comparisons of a key.  Starts and ends with
+// the block synchronised.
+__device__ void rank_all(Selection& P, unsigned long long* keys, int n, int top) {
     if (threadIdx.x == 0 && (n & 1)) keys[n] = 0ull;
     __syncthreads();
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
-        const unsigned long long key = keys[i];
+    const int part = threadIdx.x & 3;
+    for (int base = 0; base < n; base += blockDim.x >> 2) {
+        const int i = base + (threadIdx.x >> 2);
+        const unsigned long long key = i < n ? keys[i] : 0ull;
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < n; j += 2) {
+        for (int j = 2 * part; j < n; j += 8) {
             const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&keys[j]);
             rank += (pair.x > key) + (pair.y > key);
         }
-        if (rank < top) P.best[rank] = key;
+        rank += __shfl_xor_sync(0xffffffffu, rank, 1);
+        rank += __shfl_xor_sync(0xffffffffu, rank, 2);
+        if (part == 0 && i < n && rank < top) P.best[rank] = key;
     }
     __syncthreads();
-    return n < top ? n : top;
+}
+
+// rank_all for any n: a long list (ties of a masked row, rows in order) is first cut to the
+// keys above a bound, since ranking takes n^2 comparisons.
+__device__ void rank_keys(Selection& P, unsigned long long* keys, int n, int top) {
+    if (n <= kFewerCap / 2) {
+        rank_all(P, keys, n, top);
+        return;
+    }
+    __syncthreads();
+    unsigned long long mine = 0ull;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) mine = keys[i] > mine ? keys[i] : mine;
+    const unsigned long long bound = group_bound(P, mine, top);
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const unsigned long long key = keys[i];
+        if (key < bound) continue;
+        const int pos = atomicAdd(&P.count, 1);
+        if (pos < kFewerCap) P.fewer[pos] = key;
+    }
+    __syncthreads();
+    const int count = P.count;
+    if (count < kFewerCap)
+        rank_all(P, P.fewer, count, top);
+    else
+        rank_all(P, keys, n, top);
 }
 
 // The `top` best tokens of elements [begin, end) of a row, piece by piece: what beats the
@@ -578,99 +638,73 @@ __device__ void select_by_pieces(Selection& P, const E* z, int begin, int end, i
         __syncthreads();
         const int n = P.count;
         if (n > have) {
-            have = rank_keys(P, P.keys, n, top);
+            rank_keys(P, P.keys, n, top);
+            have = n < top ? n : top;
             for (int i = threadIdx.x; i < have; i += blockDim.x) P.keys[i] = P.best[i];
         }
         __syncthreads();
     }
 }
 
-// The best tokens of a slice from what the threads met while they summed it.  The
-// threads form groups; the `top`-th best of the groups' best vectors, ordered by (its
-// largest logit, lower vector number first), bounds the `top`-th best element from below:
-// `top` elements, one in each better group, are at least as good.  So only elements at or
-// above that bound are candidates, about G ln(1 / (1 - top / G)) of them where the tokens
-// lie at random over G groups.  They are read again (from L2) at the threads' best
-// vectors, and in all vectors only of threads that have a second one to offer.  More
-// candidates than the list holds (rows in order) are left to select_by_pieces.
+// The best tokens of a slice from what the threads met while they summed it.  A thread's
+// key is its best vector, ordered by (largest logit, lower vector number first); the bound
+// from groups of threads lies below the `top`-th best element, since `top` elements, one in
+// each better group, are at least as good.  So only elements at or above it are candidates,
+// about G ln(1 / (1 - top / G)) of them where the tokens lie at random over G groups.  They
+// are read again (from L2) at the threads' best vectors, and in all their vectors only for
+// threads that have a second one to offer.  More candidates than the list holds are left
+// to select_by_pieces.
 template <typename E>
 __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& part, const E* z, int top,
                                   const Running& acc, int cap) {
     constexpr int n = Vec<E>::n;
     const int tid = threadIdx.x, lane = tid & 31, T = blockDim.x;
-    const int wide = top * 8 > T ? (top * 4 > T ? 1 : 2) : 4, groups = T / wide;
     const unsigned long long mine =
         acc.at < 0 ? 0ull : ((unsigned long long)total_order_key(acc.m + 0.f) << 32) | (0xffffffffu - (uint32_t)acc.at);
-    unsigned long long best = mine;
-    for (int o = 1; o < wide; o <<= 1) {
-        const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-        best = other > best ? other : best;
-    }
-    if (tid % wide == 0) P.group[tid / wide] = best;
-    P.offered[tid] = acc.at;
-    if (tid == 0) {
-        P.threshold = 0ull;
-        P.count = P.rescans = 0;
-    }
-    __syncthreads();
-    if (tid < groups) {
-        const unsigned long long key = P.group[tid];
-        int above = 0;
-#pragma unroll 8
-        for (int i = 0; i < groups; i += 2) {
-            const ulonglong2 pair = *reinterpret_cast<const ulonglong2*>(&P.group[i]);
-            above += (pair.x > key) + (pair.y > key);
-        }
-        if (above == top - 1 && key != 0ull) P.threshold = key;
-    }
-    __syncthreads();
-    const unsigned long long threshold = P.threshold;
+    const unsigned long long bound = group_bound(P, mine, top);
     auto offer = [&](int j, const float* v) {
         const uint32_t low = 0xffffffffu - (uint32_t)j;
 #pragma unroll
         for (int e = 0; e < n; ++e) {
             const long long i = row.first(j) + e;
             const unsigned long long key = ((unsigned long long)total_order_key(v[e] + 0.f) << 32) | low;
-            if (key >= threshold && i >= 0 && i < row.vocab) {
+            if (key >= bound && i >= 0 && i < row.vocab) {
                 const int pos = atomicAdd(&P.count, 1);
                 if (pos < cap) P.keys[pos] = order_key(v[e], (uint32_t)i);
             }
         }
     };
-    if (mine != 0ull && mine >= threshold) {
+    auto offer_vector = [&](int j) {
         float v[n];
-        if (acc.at >= row.full0 && acc.at < row.full1)
-            Vec<E>::unpack(row.full(acc.at), v);
+        if (j >= row.full0 && j < row.full1)
+            Vec<E>::unpack(row.full(j), v);
         else
-            row.ragged(acc.at, v);
-        offer(acc.at, v);
-        if (total_order_key(acc.second + 0.f) >= (uint32_t)(threshold >> 32)) P.rescan[atomicAdd(&P.rescans, 1)] = tid;
+            row.ragged(j, v);
+        offer(j, v);
+    };
+    const bool in = mine != 0ull && mine >= bound;
+    // a second vector counts where its largest logit beats the bound's, or equals it at a
+    // vector number up to the bound's
+    const uint32_t level = (uint32_t)(bound >> 32), second = total_order_key(acc.second + 0.f);
+    const long long bound_at = (long long)(0xffffffffu - (uint32_t)bound);
+    uint32_t again = __ballot_sync(0xffffffffu, in && second >= level);
+    if (in) offer_vector(acc.at);
+    for (; again; again &= again - 1) {
+        const int from = __ffs(again) - 1, who = (tid & ~31) + from;
+        const int skip = __shfl_sync(0xffffffffu, acc.at, from);
+        const bool tie = __shfl_sync(0xffffffffu, second, from) == level;
+        const long long end = tie && bound_at + 1 < part.hi ? bound_at + 1 : part.hi;
+        for (long long j = (long long)part.lo + who + (long long)lane * T; j < end; j += 32ll * T)
+            if (j != skip) offer_vector((int)j);
+        if (lane == 0 && part.head && who == 0 && skip != 0) offer_vector(0);
+        if (lane == 0 && part.last && who == T - 1 && skip != row.full1) offer_vector(row.full1);
     }
     __syncthreads();
-    const int rescans = P.rescans;
-    for (int q = tid >> 5; q < rescans; q += T >> 5) {
-        const int who = P.rescan[q], skip = P.offered[who];
-        float v[n];
-        for (long long j = (long long)part.lo + who + (long long)lane * T; j < part.hi; j += 32ll * T)
-            if (j != skip) {
-                Vec<E>::unpack(row.full((int)j), v);
-                offer((int)j, v);
-            }
-        if (lane == 0 && part.head && who == 0 && skip != 0) {
-            row.ragged(0, v);
-            offer(0, v);
-        }
-        if (lane == 0 && part.last && who == T - 1 && skip != row.full1) {
-            row.ragged(row.full1, v);
-            offer(row.full1, v);
-        }
-    }
-    __syncthreads();
-    if (P.count >= cap) {
+    const int count = P.count;
+    if (count >= cap)
         select_by_pieces<E>(P, z, part.begin, part.end, top, cap);
-        return;
-    }
-    rank_keys(P, P.keys, P.count, top);
+    else
+        rank_keys(P, P.keys, count, top);
 }
 
 // ---- token_logprobs ------------------------------------------------------------------
@@ -678,7 +712,7 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
 // and rank their slices and send sums and best keys to the first one's shared memory,
 // which puts them together and writes the row's results.
 template <typename E, int T>
-__global__ void __launch_bounds__(T) token_logprobs_kernel(const E* __restrict__ logits, int vocab, size_t stride,
+__global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __restrict__ logits, int vocab, size_t stride,
                                                           const Scale k, const uint32_t* __restrict__ tokens,
                                                           int token_count, int top, LogprobOutputs out) {
     __shared__ Sums scratch[33];
@@ -705,7 +739,10 @@ __global__ void __launch_bounds__(T) token_logprobs_kernel(const E* __restrict__
     // clusters keep the upper half of the list for the blocks' best keys
     const int cap = parts > 1 ? kListCap / 2 : kListCap;
     if (top > 0) {
-        if (sums.rest == sums.rest)
+        if (!sums.any) {  // nothing but -inf: the lowest ids
+            for (int i = threadIdx.x; i < top; i += T) selection.best[i] = order_key(-INFINITY, slice.begin + i);
+            __syncthreads();
+        } else if (sums.rest == sums.rest)
             select_by_threads<E>(selection, row, slice, z, top, acc, cap);
         else  // NaN or +inf here: NaN leads the order and the threads' maxima pass over it
             select_by_pieces<E>(selection, z, slice.begin, slice.end, top, cap);
@@ -1071,7 +1108,7 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         if (vectors < 1024)
             return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
-        return launch_clusters(token_logprobs_kernel<E, 512>, z.rows, row_parts(sm_count, z.rows, vectors, 512, 4), 512,
+        return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, row_parts(sm_count, z.rows, vectors, 256, 4), 256,
                                s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
                                (int)alternatives, out);
     });

@@ -23,6 +23,7 @@ from .gpu import Gpu
 
 _KINDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _DEFAULT_STREAM = 1  # cudaStreamLegacy
+_raw_stream = torch._C._cuda_getCurrentRawStream
 MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
 
 
@@ -43,24 +44,27 @@ class Distillation(NamedTuple):
 
 def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
     """(rows, vocab, stride, kind) of a matrix of rows on the Gpu's device."""
-    if not isinstance(logits, torch.Tensor) or logits.dim() != 2 or logits.dtype not in _KINDS:
+    kind = _KINDS.get(logits.dtype) if isinstance(logits, torch.Tensor) and logits.dim() == 2 else None
+    if kind is None:
         raise ValueError(f"{name} must be a [rows, vocab] tensor of float32, float16 or bfloat16")
     if logits.get_device() != gpu.device:
         raise ValueError(f"{name} must be on the Gpu's device")
     rows, vocab = logits.shape
+    stride, unit = logits.stride()
     if vocab < 1:
         raise ValueError("check the vocabulary size")
-    if vocab > 1 and logits.stride(1) != 1:
+    if unit != 1 and vocab > 1:
         raise ValueError(f"{name} must have unit stride along the vocabulary")
-    stride = logits.stride(0) if rows > 1 else vocab
-    if stride < vocab:
+    if rows <= 1:
+        stride = vocab
+    elif stride < vocab:
         raise ValueError(f"rows of {name} must not overlap")
-    return rows, vocab, stride, _KINDS[logits.dtype]
+    return rows, vocab, stride, kind
 
 
 def _vector(gpu: Gpu, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
     """Address of a contiguous tensor of this shape and type on the Gpu's device."""
-    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.shape != shape:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape:
         raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}")
     if t.get_device() != gpu.device or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous on the Gpu's device")
@@ -83,8 +87,9 @@ def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
 
 
 def _stream(gpu: Gpu) -> int:
-    """torch's current stream on the Gpu's device, as lsx.h takes it."""
-    return torch.cuda.current_stream(gpu.device).cuda_stream or _DEFAULT_STREAM
+    """torch's current stream on the Gpu's device, as lsx.h takes it (the raw handle that
+    torch.cuda.current_stream wraps in an object)."""
+    return _raw_stream(gpu.device) or _DEFAULT_STREAM
 
 
 def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0,
@@ -97,15 +102,14 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
     k = int(alternatives)
     if not 0 <= k <= min(MAX_SLOTS, vocab):
         raise ValueError(f"alternatives must be at most {MAX_SLOTS} and at most the vocabulary")
-    shapes = (((rows, n), torch.float32), ((rows,), torch.float32), ((rows, 2), torch.float32),
-              ((rows, k), torch.int32), ((rows, k), torch.float32), ((rows, k), torch.float32))
+    f32, i32 = torch.float32, torch.int32
+    shapes = ((rows, n), f32), ((rows,), f32), ((rows, 2), f32), ((rows, k), i32), ((rows, k), f32), ((rows, k), f32)
     if out is None:
-        out = tuple(torch.empty(s, dtype=d, device=logits.device) if (n or i != 0) and (k or i < 3) else None
-                    for i, (s, d) in enumerate(shapes))
+        wanted = n > 0, True, True, k > 0, k > 0, k > 0
+        out = [torch.empty(s, dtype=d, device=logits.device) if w else None for w, (s, d) in zip(wanted, shapes)]
     elif len(out) != 6:
         raise ValueError("out holds the six results")
-    at = [_vector(gpu, t, s, d, f"out[{i}]") if t is not None and t.numel() else None
-          for i, (t, (s, d)) in enumerate(zip(out, shapes))]
+    at = [None if t is None or 0 in s else _vector(gpu, t, s, d, "out") for t, (s, d) in zip(out, shapes)]
     given = _vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None
     if rows:
         check(lib.lsx_token_logprobs_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
