@@ -398,7 +398,9 @@ int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dty
      dz_i = (w/T) (q_i P - p_i) for i in K,  (w/T) q_i (P - p_r / q_r) otherwise,
    stored as lsx_token_logprobs_backward_device does.  loss_out and stats_out may be
    NULL.  A row whose list is unused throughout has p = 0 (p_r = 1 with statistics):
-   loss and gradient 0. */
+   loss and gradient 0; so has one whose teacher's statistics are those of a row
+   without tokens, (-inf, 0).  A student's row without tokens has loss +inf where the
+   teacher has listed mass, and gradient 0. */
 int lsx_distill_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab, size_t stride,
                        double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
                        size_t teacher_count, const float* teacher_stats, const float* weights, float* loss_out,

@@ -24,9 +24,13 @@
 namespace lsx {
 namespace {
 
-constexpr int kRowThreads = 512;
+constexpr int kRowThreads = 256;
 constexpr int kListCap = 2048;     // candidate keys of one selection
 constexpr int kMarkWords = 512;    // 32-bit words of the bitmap of marked vectors
+constexpr int kPlainShared = 36 << 10;   // dynamic shared memory that needs no opt-in beside the kernels' own
+constexpr int kStagedTarget = 40 << 10;  // a slice kept in shared memory: 4 blocks on an SM
+constexpr int kStagedMost = 200 << 10;   // and at most
+constexpr int kPieceVectors = 2048;      // a slice of the gradient kernels
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -197,33 +201,25 @@ struct Slice {
 };
 
 // ---- marked tokens -----------------------------------------------------------
-// The tokens a row lists, sorted, each with a value; a bitmap over vector numbers
-// (modulo its size) tells the streaming loop which vectors to look up.  One word
-// covers 32 consecutive vectors, which is what a warp holds.
+// The tokens a row lists, sorted; a bitmap over vector numbers (modulo its size) tells
+// the streaming loop which vectors to look up.  One word covers 32 consecutive vectors,
+// which is what a warp holds.
 struct Marks {
     uint32_t raw[kMaxSlots];
     uint32_t ids[kMaxSlots];
-    float value[kMaxSlots];
-    int slot_rank[kMaxSlots];  // position of each slot in `ids`; -1 unused, -2 - rank for a repeated token
     int count;
-    int bad;  // some slot names a token outside the vocabulary
     uint32_t bits[kMarkWords];
 };
 
-// Reads one row's token list and sorts it (four threads per slot count the smaller
-// ids); ends with the block synchronised.
+// Reads one row's token list and sorts it; ends with the block synchronised.
 template <typename E>
 __device__ void build_marks(Marks& M, const uint32_t* list, int slots, const Row<E>& row) {
     const int tid = threadIdx.x;
     for (int i = tid; i < kMarkWords; i += blockDim.x) M.bits[i] = 0;
-    if (tid == 0) M.count = M.bad = 0;
+    if (tid == 0) M.count = 0;
     __syncthreads();
     for (int i = tid; i < slots; i += blockDim.x) {
-        uint32_t id = list[i];
-        if (id != kUnusedToken && id >= (uint32_t)row.vocab) {
-            M.bad = 1;
-            id = kUnusedToken;
-        }
+        const uint32_t id = list[i] < (uint32_t)row.vocab ? list[i] : kUnusedToken;
         M.raw[i] = id;
         if (id != kUnusedToken) {
             atomicAdd(&M.count, 1);
@@ -232,25 +228,11 @@ __device__ void build_marks(Marks& M, const uint32_t* list, int slots, const Row
         }
     }
     __syncthreads();
-    for (int base = 0; base < slots * 4; base += blockDim.x) {
-        const int slot = (base + tid) >> 2, part = tid & 3;
-        const uint32_t id = slot < slots ? M.raw[slot] : 0;
-        int less = 0, same = 0;
-        if (slot < slots)
-            for (int j = part; j < slots; j += 4) {
-                const uint32_t other = M.raw[j];
-                less += other < id;
-                same += other == id && j < slot;
-            }
-        less += __shfl_xor_sync(0xffffffffu, less, 1);
-        less += __shfl_xor_sync(0xffffffffu, less, 2);
-        same += __shfl_xor_sync(0xffffffffu, same, 1);
-        same += __shfl_xor_sync(0xffffffffu, same, 2);
-        if (slot < slots && part == 0) {
-            const int rank = less + same;
-            if (id != kUnusedToken) M.ids[rank] = id;
-            M.slot_rank[slot] = id == kUnusedToken ? -1 : same ? -2 - rank : rank;
-        }
+    for (int slot = tid; slot < slots; slot += blockDim.x) {
+        const uint32_t id = M.raw[slot];
+        int rank = 0;
+        for (int j = 0; j < slots; ++j) rank += M.raw[j] < id || (M.raw[j] == id && j < slot);
+        if (id != kUnusedToken) M.ids[rank] = id;
     }
     __syncthreads();
 }
@@ -779,48 +761,89 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     }
 }
 
-// ---- gradients ---------------------------------------------------------------------------
-// What the gradient of one row needs: with y = (z - m) L - log2_sum an element gets
-// 2^y (a + b y); a marked one, against its own log2_marked, 2^y (a_marked + b y) + its
-// value.  `zero` rows get 0.
-struct GradientRow {
-    float m, log2_sum, a, b, log2_marked, a_marked;
-    bool zero;
+// ---- lists of tokens -------------------------------------------------------------------------
+// One row's listed tokens, a slot to a thread.
+struct List {
+    uint32_t ids[kMaxSlots];
+    bool kept[kMaxSlots];    // names a token, and is the first slot to name it
+    float logit[kMaxSlots];  // the row's logit of a kept token, else -inf
+    float value[kMaxSlots];  // what the operator keeps with the slot
+    int bad;                 // some slot names a token outside the vocabulary
 };
 
+// Reads a row's list and the logits it names.  Two threads per slot look for an earlier
+// slot of the same token.  Ends with the block synchronised.
 template <typename E>
-__device__ __forceinline__ void gradient_vector(const Marks& M, const Row<E>& row, const GradientRow& g, float L, int j,
-                                                float* v) {
-    constexpr int n = Vec<E>::n;
-    const bool look = marked(M, j);
-    int pos = look ? mark_position(M, row.first(j)) : 0;
+__device__ void read_list(List& list, const uint32_t* ids, int count, const E* z, int vocab) {
+    const int tid = threadIdx.x;
+    if (tid == 0) list.bad = 0;
+    __syncthreads();
+    if (tid < count) {
+        const uint32_t id = ids[tid];
+        const bool used = id < (uint32_t)vocab;
+        list.ids[tid] = id;
+        list.logit[tid] = used ? Vec<E>::one(z[id]) : -INFINITY;
+        list.value[tid] = 0.f;
+        if (!used && id != kUnusedToken) list.bad = 1;
+    }
+    __syncthreads();
+    const int slot = tid >> 1;
+    bool seen = false;
+    if (slot < count)
+        for (int j = tid & 1; j < slot; j += 2) seen |= list.ids[j] == list.ids[slot];
+    seen |= (bool)__shfl_xor_sync(0xffffffffu, (int)seen, 1);
+    if (slot < count && (tid & 1) == 0) {
+        const bool kept = !seen && list.ids[slot] < (uint32_t)vocab;
+        list.kept[slot] = kept;
+        if (!kept) list.logit[slot] = -INFINITY;
+    }
+    __syncthreads();
+}
+
+// ---- gradients ---------------------------------------------------------------------------
+// What the unlisted elements of a row's gradient need: with y = (z - m) L - offset an
+// element gets 2^y (a + b y).  Listed ones are written over them afterwards.
+struct Dense {
+    float m, offset, a, b;
+};
+// The gradient of a row without any token: 0 for every element (z - 0 = -inf).
+__device__ __forceinline__ Dense dense_zero() { return {0.f, 0.f, 0.f, 0.f}; }
+
+template <int n, bool kLinear>
+__device__ __forceinline__ void dense_vector(float* v, const Dense& d, float L) {
+    const float2 back = {-d.m, -d.m}, scale = {L, L}, offset = {-d.offset, -d.offset}, a = {d.a, d.a}, b = {d.b, d.b};
 #pragma unroll
-    for (int e = 0; e < n; ++e) {
-        float a = g.a, offset = g.log2_sum, add = 0.f;
-        if (look)
-            while (pos < M.count && (long long)M.ids[pos] == row.first(j) + e) {
-                add += M.value[pos];
-                a = g.a_marked;
-                offset = g.log2_marked;
-                ++pos;
-            }
-        const float y = max_nan(fmaf(v[e] - g.m, L, -offset), kLowestExponent);
-        v[e] = g.zero ? 0.f : fmaf(exp2_fast(y), fmaf(g.b, y, a), add);
+    for (int e = 0; e < n; e += 2) {
+        float2 y = __ffma2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), back), scale, offset);
+        y.x = max_nan(y.x, kLowestExponent);
+        y.y = max_nan(y.y, kLowestExponent);
+        const float2 p = {exp2_fast(y.x), exp2_fast(y.y)};
+        const float2 g = __fmul2_rn(p, kLinear ? __ffma2_rn(b, y, a) : a);
+        v[e] = g.x;
+        v[e + 1] = g.y;
     }
 }
 
-// Vectors [lo, hi) of the full ones, and the ragged ends where asked for.
-template <typename E>
-__device__ void write_gradient(const Marks& M, const Row<E>& row, E* out, const GradientRow& g, float L,
-                               int lo, int hi, bool head, bool last) {
+__device__ __forceinline__ void store16(void* p, uint4 w) {
+    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+}
+
+// The dense gradient of a slice into `out` (the row's first element): vectors from
+// `staged` (slot j - lo; the ragged ends behind the full ones) or, where it is null, from
+// the row itself.  `out` may be the row.
+template <typename E, bool kLinear>
+__device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, const Dense& d, float L) {
     constexpr int n = Vec<E>::n;
     const int tid = threadIdx.x, T = blockDim.x;
     // the output row may lie at another alignment than the logits
     const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (uintptr_t)(row.lead * sizeof(E));
     E* base = out - row.lead;
-    auto put = [&](int j, const float* v) {
+    auto put = [&](int j, uint4 w) {
+        float v[n];
+        Vec<E>::unpack(w, v);
+        dense_vector<n, kLinear>(v, d, L);
         if (same) {
-            *reinterpret_cast<uint4*>(base + (long long)j * n) = Vec<E>::pack(v);
+            store16(base + (long long)j * n, Vec<E>::pack(v));
         } else {
 #pragma unroll
             for (int e = 0; e < n; ++e) base[(long long)j * n + e] = Vec<E>::store(v[e]);
@@ -829,83 +852,93 @@ __device__ void write_gradient(const Marks& M, const Row<E>& row, E* out, const 
     auto put_ragged = [&](int j) {
         float v[n];
         row.ragged(j, v);
-        gradient_vector(M, row, g, L, j, v);
+        dense_vector<n, kLinear>(v, d, L);
 #pragma unroll
         for (int e = 0; e < n; ++e) {
             const long long i = row.first(j) + e;
             if (i >= 0 && i < row.vocab) out[i] = Vec<E>::store(v[e]);
         }
     };
-    int j = lo + tid;
-    for (; j + (kUnroll - 1) * T < hi; j += kUnroll * T) {
-        uint4 w[kUnroll];
+    int j = part.lo + tid;
+    if (staged) {
+        for (; j < part.hi; j += T) put(j, staged[j - part.lo]);
+    } else {
+        for (; j + (kUnroll - 1) * T < part.hi; j += kUnroll * T) {
+            uint4 w[kUnroll];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
+            for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            float v[n];
-            Vec<E>::unpack(w[u], v);
-            gradient_vector(M, row, g, L, j + u * T, v);
-            put(j + u * T, v);
+            for (int u = 0; u < kUnroll; ++u) put(j + u * T, w[u]);
         }
+        for (; j < part.hi; j += T) put(j, row.full(j));
     }
-    for (; j < hi; j += T) {
-        float v[n];
-        Vec<E>::unpack(row.full(j), v);
-        gradient_vector(M, row, g, L, j, v);
-        put(j, v);
-    }
-    if (head && row.head && tid == 0) put_ragged(0);
-    if (last && row.last && tid == T - 1) put_ragged(row.full1);
+    if (part.head && tid == 0) put_ragged(0);
+    if (part.last && tid == T - 1) put_ragged(row.full1);
 }
 
+// `parts` blocks share a row; none waits for another.
 template <typename E>
 __global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
-    const E* logits, int vocab, size_t stride, const Scale k, const uint32_t* __restrict__ tokens, int token_count,
-    const float* __restrict__ stats, const float* __restrict__ entropy, const float* __restrict__ logprob_gradient,
-    const float* __restrict__ entropy_gradient, E* gradient, size_t gradient_stride) {
-    __shared__ Marks marks;
+    const E* logits, int vocab, size_t stride, const Scale k, int parts, const uint32_t* __restrict__ tokens,
+    int token_count, const float* __restrict__ stats, const float* __restrict__ entropy,
+    const float* __restrict__ logprob_gradient, const float* __restrict__ entropy_gradient, E* gradient,
+    size_t gradient_stride) {
+    __shared__ List list;
     __shared__ float total;
-    const size_t r = blockIdx.x;
-    const Row<E> row(logits + r * stride, vocab);
-    build_marks(marks, tokens + r * token_count, token_count, row);
-    const float inverse = k.inverse;
-    if (threadIdx.x < 32) {
-        float sum = 0.f;
-        for (int i = threadIdx.x; i < token_count; i += 32) {
-            const int rank = marks.slot_rank[i];
-            if (rank == -1) continue;
-            const float v = logprob_gradient[r * token_count + i];
-            marks.value[rank >= 0 ? rank : -2 - rank] = v * inverse;
-            sum += v;
-        }
-        sum = warp_allsum(sum);
-        if (threadIdx.x == 0) total = marks.bad ? NAN : sum;
-    }
+    const size_t r = blockIdx.x / parts;
+    const int part = (int)(blockIdx.x - r * parts), tid = threadIdx.x;
+    const E* z = logits + r * stride;
+    const Row<E> row(z, vocab);
+    const Slice slice(row, part, parts);
+    const float m = stats[2 * r], log_sum = stats[2 * r + 1];
+    const float h = entropy_gradient ? entropy_gradient[r] : 0.f, H = entropy ? entropy[r] : 0.f;
+    const float mine = tid < token_count ? logprob_gradient[r * token_count + tid] : 0.f;
+    read_list(list, tokens + r * token_count, token_count, z, vocab);
+    if (tid < token_count) list.value[tid] = list.ids[tid] == kUnusedToken ? 0.f : mine;
     __syncthreads();
-    const float L = k.L;
-    const float h = entropy_gradient ? entropy_gradient[r] : 0.f;
-    GradientRow g;
-    g.m = stats[2 * r];
-    g.log2_sum = stats[2 * r + 1] * kLog2E;
-    g.a = -(total + (h != 0.f ? h * entropy[r] : 0.f)) * inverse;
-    g.b = -h * kLn2 * inverse;
-    g.a_marked = g.a;
-    g.log2_marked = g.log2_sum;
-    g.zero = g.m == -INFINITY && stats[2 * r + 1] == 0.f;
-    write_gradient(marks, row, gradient + r * gradient_stride, g, L, row.full0, row.full1, true, true);
+    if (tid < 32) {
+        float sum = 0.f;
+        for (int i = tid; i < token_count; i += 32) sum += list.value[i];
+        sum = warp_allsum(sum);
+        if (tid == 0) total = list.bad ? NAN : sum;
+    }
+    // a token named several times adds up at its first slot
+    const bool kept = tid < token_count && list.kept[tid];
+    float own = 0.f;
+    if (kept)
+        for (int i = tid; i < token_count; ++i) own += list.ids[i] == list.ids[tid] ? list.value[i] : 0.f;
+    __syncthreads();
+    const bool empty = m == -INFINITY && log_sum == 0.f;
+    Dense d = dense_zero();
+    if (!empty) {
+        d.m = m;
+        d.offset = log_sum * kLog2E;
+        d.a = -(total + (h != 0.f ? h * H : 0.f)) * k.inverse;
+        d.b = -h * kLn2 * k.inverse;
+    }
+    E* out = gradient + r * gradient_stride;
+    if (h != 0.f)
+        write_dense<E, true>(row, slice, nullptr, out, d, k.L);
+    else
+        write_dense<E, false>(row, slice, nullptr, out, d, k.L);
+    __syncthreads();
+    if (kept && (int)list.ids[tid] >= slice.begin && (int)list.ids[tid] < slice.end) {
+        const float y = max_nan(fmaf(list.logit[tid] - d.m, k.L, -d.offset), kLowestExponent), log_q = y * kLn2;
+        // own (1 - q) apart from the other tokens' share: own - q own loses a confident token's gradient
+        const float g = -expm1f(log_q) * own - exp2_fast(y) * (total - own + (h != 0.f ? h * (H + log_q) : 0.f));
+        out[list.ids[tid]] = Vec<E>::store(empty ? 0.f : g * k.inverse);
+    }
 }
 
 // ---- distillation --------------------------------------------------------------------------
-// The teacher's side of one row, by one warp, in 64 bits (its sums run over at most
-// kMaxSlots numbers, and 1 - sum p is next to 0 for a confident teacher).
-struct TeacherSums {
-    double mass;  // sum of the listed p
-    double rest;  // the teacher's mass outside the list (0 without its statistics)
-};
-
-struct TeacherSlots {
-    double log_p[kMaxSlots];
+// The listed tokens' side of one row in 64 bits, by one warp: sums over at most kMaxSlots
+// numbers, of which 1 - sum p is next to 0 for a confident teacher.
+struct Listed {
+    double mass;    // sum of p
+    double rest;    // the teacher's mass outside the list (0 without its statistics)
+    double m;       // the largest listed logit of the student
+    double inside;  // sum exp((z - m) / T) over the listed tokens
+    double cross;   // sum p (ln p - (z - m) / T)
 };
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -919,147 +952,264 @@ __device__ __forceinline__ double warp_max_f64(double v) {
     return v;
 }
 
-__device__ TeacherSums teacher_row(const Marks& M, TeacherSlots& slots, const float* values, const float* stats,
-                                   int count, double temperature) {
+// Also leaves scale * p in list.value.
+__device__ Listed listed_sums(List& list, const float* values, const float* stats, int count, double inverse,
+                              double scale, bool student) {
     const int lane = threadIdx.x & 31;
-    double top = -INFINITY;
-    for (int i = lane; i < count; i += 32)
-        if (M.slot_rank[i] >= 0) top = fmax(top, (double)values[i]);
-    top = warp_max_f64(top);
-    double norm = 0.0, shift = top == -INFINITY ? 0.0 : top;
+    constexpr int kPer = kMaxSlots / 32;
+    double a[kPer], top = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int i = lane + 32 * q;
+        a[q] = i < count && list.kept[i] ? (double)values[i] : -INFINITY;
+        top = fmax(top, a[q]);
+    }
+    double shift, norm;
+    bool none = false;  // the teacher's row holds no token: it asks for nothing
     if (stats) {
-        shift = (double)stats[0];
+        none = stats[0] == -INFINITY && stats[1] == 0.f;
+        shift = none ? 0.0 : (double)stats[0];
         norm = (double)stats[1];
     } else {
+        top = warp_max_f64(top);
+        shift = top == -INFINITY ? 0.0 : top;
         double sum = 0.0;
-        for (int i = lane; i < count; i += 32)
-            if (M.slot_rank[i] >= 0) sum += exp(((double)values[i] - shift) / temperature);
+#pragma unroll
+        for (int q = 0; q < kPer; ++q)
+            if (32 * q < count) sum += exp((a[q] - shift) * inverse);
         sum = warp_sum_f64(sum);
         norm = sum > 0.0 ? log(sum) : (sum == 0.0 ? 0.0 : sum);
     }
-    double mass = 0.0;
-    for (int i = lane; i < count; i += 32) {
-        const double log_p =
-            M.slot_rank[i] >= 0 ? ((double)values[i] - shift) / temperature - norm : -INFINITY;
-        slots.log_p[i] = log_p;
-        mass += exp(log_p);
+    Listed t{0.0, 0.0, -INFINITY, 0.0, 0.0};
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        if (32 * q >= count) break;
+        a[q] = (a[q] - shift) * inverse - norm;  // ln p
+        const double p = exp(a[q]);
+        t.mass += p;
+        const int i = lane + 32 * q;
+        if (i < count) list.value[i] = (float)(scale * p);
     }
-    mass = warp_sum_f64(mass);
-    __syncwarp();
-    return {mass, stats ? (mass < 1.0 ? 1.0 - mass : (mass >= 1.0 ? 0.0 : mass)) : 0.0};
+    t.mass = warp_sum_f64(t.mass);
+    if (stats && !none) t.rest = t.mass < 1.0 ? 1.0 - t.mass : (t.mass >= 1.0 ? 0.0 : t.mass);
+    if (!student) return t;
+    for (int i = lane; i < count; i += 32) t.m = fmax(t.m, (double)list.logit[i]);
+    t.m = warp_max_f64(t.m);
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int i = lane + 32 * q;
+        if (i >= count) break;
+        const double z = (double)list.logit[i];
+        const double log_q = z == -INFINITY ? -INFINITY : (z - t.m) * inverse;
+        t.inside += exp(log_q);
+        const double p = exp(a[q]);
+        if (p != 0.0) t.cross += p * (a[q] - log_q);
+    }
+    t.inside = warp_sum_f64(t.inside);
+    t.cross = warp_sum_f64(t.cross);
+    return t;
 }
 
 // The tokens outside the list are one outcome only where the student's share of them is
 // a normal f32 number (2^-126 and up).
 constexpr double kSmallestLogShare = -87.3365447505531;
 
-// The gradient's coefficients from the sums; also fills the marked values.  The tokens
-// outside the list are exponentiated against their own sum: 2^y = q_i / q_r stays in range
-// and (P q_r - p_r) is the whole coefficient, however small q_r is.
-__device__ GradientRow distill_gradient_row(Marks& M, const TeacherSlots& slots, const TeacherSums& t, int count,
-                                            float m, double log_sum, double log_rest, bool zero, float weight,
-                                            double temperature) {
-    const double scale = (double)weight / temperature;
+// What the gradient of one row needs beside its list: listed elements get q a - value, q
+// against `offset`.
+struct DistillRow {
+    Dense dense;
+    float m, offset, a;
+    bool zero;
+};
+
+// The tokens outside the list are exponentiated against their own sum: 2^y = q_i / q_r
+// stays in range and (P q_r - p_r) is the whole coefficient, however small q_r is.
+__device__ DistillRow distill_row(const Listed& t, double m, double log_sum, double log_rest, bool empty, bool bad,
+                                  double scale) {
     const double log_share = log_rest - log_sum;
     const bool tail = log_share >= kSmallestLogShare;
     const double mass = t.mass + (tail ? t.rest : 0.0);
-    for (int i = threadIdx.x & 31; i < count; i += 32) {
-        const int rank = M.slot_rank[i];
-        if (rank == -1) continue;
-        M.value[rank >= 0 ? rank : -2 - rank] = rank >= 0 ? (float)(-scale * exp(slots.log_p[i])) : 0.f;
-    }
-    GradientRow g;
-    g.m = m;
-    g.log2_marked = (float)(log_sum * 1.4426950408889634);
-    g.a_marked = M.bad ? NAN : (float)(scale * mass);
-    g.log2_sum = tail ? (float)(log_rest * 1.4426950408889634) : g.log2_marked;
-    g.a = M.bad ? NAN : (float)(scale * (tail ? mass * exp(log_share) - t.rest : mass));
-    g.b = 0.f;
-    g.zero = zero;
+    DistillRow g;
+    g.m = (float)m;
+    g.offset = (float)(log_sum * 1.4426950408889634);
+    g.a = bad ? NAN : (float)(scale * mass);
+    g.zero = empty;
+    g.dense.m = g.m;
+    g.dense.offset = tail ? (float)(log_rest * 1.4426950408889634) : g.offset;
+    g.dense.a = bad ? NAN : (float)(scale * (tail ? mass * exp(log_share) - t.rest : mass));
+    g.dense.b = 0.f;
+    if (empty) g.dense = dense_zero();
     return g;
 }
 
-// kStream: sums the row (loss, and optionally the gradient); otherwise the statistics
-// are given and only the gradient is written.
-template <typename E, bool kTail, bool kStream>
+// Writes a slice's listed elements over its dense gradient.  After a block barrier.
+template <typename E>
+__device__ __forceinline__ void write_listed(const List& list, int count, const Slice& slice, const DistillRow& g,
+                                             float L, E* out) {
+    const int tid = threadIdx.x;
+    if (tid >= count || !list.kept[tid]) return;
+    const int id = (int)list.ids[tid];
+    if (id < slice.begin || id >= slice.end) return;
+    const float y = max_nan(fmaf(list.logit[tid] - g.m, L, -g.offset), kLowestExponent);
+    out[id] = Vec<E>::store(g.zero ? 0.f : fmaf(exp2_fast(y), g.a, -list.value[tid]));
+}
+
+__device__ __forceinline__ void copy16_async(void* shared, const void* global) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
+}
+
+// Loss, statistics and, where wanted, the gradient.  A cluster of blocks shares a row.
+// kStaged: each block holds its slice in shared memory, so the row is read once: the
+// listed tokens are struck out there (their share is summed by itself, in 64 bits), the rest
+// is summed, the blocks exchange their sums, and the gradient is formed from the same
+// copy.  Without it (rows too long for that) the slice is read again for the gradient,
+// and a bitmap of marked vectors tells the sum which elements to leave out.
+template <typename E, bool kTail, bool kStaged>
 __global__ void __launch_bounds__(kRowThreads) distill_kernel(
-    const E* logits, int vocab, size_t stride, const Scale k, double T, TeacherRows teacher,
+    const E* logits, int vocab, size_t stride, const Scale k, double temperature, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
+    constexpr int n = Vec<E>::n;
+    extern __shared__ __align__(16) uint4 staged[];
     __shared__ Sums scratch[33];
-    __shared__ Marks marks;
-    __shared__ TeacherSlots slots;
-    __shared__ GradientRow grow;
-    __shared__ float listed[kMaxSlots];
-    const size_t r = blockIdx.x;
+    __shared__ List list;
+    __shared__ DistillRow grow;
+    __shared__ Sums shares[kMaxCluster];
+    const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x, T = blockDim.x;
+    if (parts > 1) cluster_arrive();  // waited for before the first store into another block
+    const size_t r = blockIdx.x / parts;
     const int count = (int)teacher.slots;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
-    build_marks(marks, teacher.ids + r * count, count, row);
-    const Slice slice(row, 0, 1);
-    float m_rest = -INFINITY, S = 0.f;
-    if (kStream) {
-        for (int i = threadIdx.x; i < count; i += blockDim.x)
-            listed[i] = marks.slot_rank[i] >= 0 ? Vec<E>::one(z[marks.raw[i]]) : -INFINITY;
-        Running acc;
-        stream_slice<E, true>(row, slice, &marks, k, acc);
-        const Sums x = block_sums(acc, k.L, scratch);
-        m_rest = x.m;
-        S = x.S;
+    const Slice slice(row, part, parts);
+    const int full = slice.hi - slice.lo;
+    if (kStaged) {
+        for (int i = tid; i < full; i += T) copy16_async(&staged[i], row.base + (long long)(slice.lo + i) * n);
+        // the ragged ends follow, -inf beyond the row
+        if (slice.head && tid == 0) {
+            float v[n];
+            row.ragged(0, v);
+            staged[full] = Vec<E>::pack(v);
+        }
+        if (slice.last && tid == T - 1) {
+            float v[n];
+            row.ragged(row.full1, v);
+            staged[full + 1] = Vec<E>::pack(v);
+        }
     }
-    if (threadIdx.x < 32) {
-        const TeacherSums t = teacher_row(marks, slots, teacher.logits + r * count,
-                                          kTail ? teacher.stats + 2 * r : nullptr, count, T);
-        double m, log_sum, log_rest = -INFINITY;
-        bool empty;
-        if (kStream) {
-            // the listed tokens' mass in f64, and the rest's around its own maximum
-            double top = -INFINITY, inside = 0.0;
-            bool nan = false;
-            for (int i = threadIdx.x; i < count; i += 32) {
-                top = fmax(top, (double)listed[i]);
-                nan |= listed[i] != listed[i];
+    read_list(list, teacher.ids + r * count, count, z, vocab);
+    const double inverse = 1.0 / temperature;
+    const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
+    Listed t;
+    if (tid < 32)
+        t = listed_sums(list, teacher.logits + r * count, kTail ? teacher.stats + 2 * r : nullptr, count, inverse,
+                        scale, true);
+    Running acc;
+    if (kStaged) {
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncthreads();
+        if (tid < count && list.kept[tid]) {
+            const int id = (int)list.ids[tid];
+            if (id >= slice.begin && id < slice.end) {
+                const long long at = (long long)id + row.lead;
+                const int j = (int)(at / n);
+                const int slot = j < row.full0 ? full : j >= row.full1 ? full + 1 : j - slice.lo;
+                reinterpret_cast<E*>(&staged[slot])[at % n] = Vec<E>::store(-INFINITY);
             }
-            m = fmax((double)m_rest, warp_max_f64(top));
-            for (int i = threadIdx.x; i < count; i += 32)
-                if (marks.slot_rank[i] >= 0 && listed[i] != -INFINITY) inside += exp(((double)listed[i] - m) / T);
-            inside = warp_sum_f64(inside);
-            const double rest = S == 0.f ? 0.0 : (double)S * exp(((double)m_rest - m) / T);
-            const double sum = __any_sync(0xffffffffu, nan) ? NAN : inside + rest;
-            if (kTail) log_rest = S == 0.f ? -INFINITY : log((double)S) + ((double)m_rest - m) / T;
-            empty = sum == 0.0;
-            log_sum = empty ? 0.0 : log(sum);
-            double part = 0.0;
-            for (int i = threadIdx.x; i < count; i += 32) {
-                const double log_p = slots.log_p[i], p = exp(log_p);
-                if (p == 0.0) continue;
-                const double log_q = empty ? -INFINITY : ((double)listed[i] - m) / T - log_sum;
-                part += p * (log_p - log_q);
-            }
-            part = warp_sum_f64(part);
-            if (kTail && t.rest > 0.0 && log_rest - log_sum >= kSmallestLogShare) part += t.rest * (log(t.rest) - log_rest + log_sum);
-            if (threadIdx.x == 0) {
-                if (loss) loss[r] = marks.bad || t.mass != t.mass || log_sum != log_sum ? NAN : (float)part;
-                if (stats) {
-                    stats[3 * r] = (float)m;
-                    stats[3 * r + 1] = (float)log_sum;
-                    stats[3 * r + 2] = (float)log_rest;
-                }
-            }
-        } else {
-            m = (double)stats[3 * r];
-            log_sum = (double)stats[3 * r + 1];
-            log_rest = (double)stats[3 * r + 2];
-            empty = m == -INFINITY && log_sum == 0.0;
         }
-        if (gradient) {
-            const GradientRow g = distill_gradient_row(marks, slots, t, count, (float)m, log_sum, log_rest, empty,
-                                                       weights ? weights[r] : 1.f, T);
-            if (threadIdx.x == 0) grow = g;
+        __syncthreads();
+        for (int i = tid; i < full; i += T) {
+            const uint4 w = staged[i];
+            float v[n];
+            Vec<E>::unpack(w, v);
+            acc.template add<n>(v, Vec<E>::top(w), i, k);
         }
+        const int ragged = slice.head && tid == 0 ? full : slice.last && tid == T - 1 ? full + 1 : -1;
+        if (ragged >= 0) {
+            const uint4 w = staged[ragged];
+            float v[n];
+            Vec<E>::unpack(w, v);
+            acc.template add<n>(v, Vec<E>::top(w), 0, k);
+        }
+    } else {
+        __shared__ Marks marks;
+        build_marks(marks, teacher.ids + r * count, count, row);
+        stream_slice<E, true>(row, slice, &marks, k, acc);
+    }
+    Sums rest = block_sums(acc, k.L, scratch);
+    if (parts > 1) {
+        cluster_wait();
+        if (tid < parts) *in_block(&shares[part], tid) = rest;
+        cluster_arrive();
+        cluster_wait();
+        rest = shares[0];
+        for (int i = 1; i < parts; ++i) rest.m = fmaxf(rest.m, shares[i].m);
+        rest.S = 0.f;
+        for (int i = 0; i < parts; ++i) {
+            Sums x = shares[i];
+            x.rebase(rest.m, k.L);
+            rest.S += x.S;
+        }
+    }
+    if (tid < 32) {
+        const double m = fmax((double)rest.m, t.m);
+        const double below = rest.S == 0.f ? -INFINITY : ((double)rest.m - m) * inverse;
+        const double sum = (t.inside == 0.0 ? 0.0 : t.inside * exp((t.m - m) * inverse)) +
+                           (rest.S == 0.f ? 0.0 : (double)rest.S * exp(below));
+        const bool empty = sum == 0.0;
+        const double log_sum = empty ? 0.0 : log(sum);
+        const double log_rest = kTail && rest.S != 0.f ? log((double)rest.S) + below : -INFINITY;
+        if (part == 0 && tid == 0) {
+            if (loss) {
+                double value = t.mass == 0.0        ? 0.0
+                               : t.cross == INFINITY ? INFINITY
+                                                     : t.cross + t.mass * ((m - t.m) * inverse + log_sum);
+                if (kTail && t.rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
+                    value += t.rest * (log(t.rest) - log_rest + log_sum);
+                loss[r] = list.bad || t.mass != t.mass || sum != sum ? NAN : (float)value;
+            }
+            if (stats) {
+                stats[3 * r] = (float)m;
+                stats[3 * r + 1] = (float)log_sum;
+                stats[3 * r + 2] = (float)log_rest;
+            }
+        }
+        if (gradient && tid == 0) grow = distill_row(t, m, log_sum, log_rest, empty, list.bad, scale);
     }
     if (!gradient) return;
     __syncthreads();
-    write_gradient(marks, row, gradient + r * gradient_stride, grow, k.L, row.full0, row.full1, true, true);
+    E* out = gradient + r * gradient_stride;
+    write_dense<E, false>(row, slice, kStaged ? staged : nullptr, out, grow.dense, k.L);
+    __syncthreads();
+    write_listed(list, count, slice, grow, k.L, out);
+}
+
+// The gradient from saved statistics; `parts` blocks share a row, none waits for another.
+template <typename E, bool kTail>
+__global__ void __launch_bounds__(kRowThreads) distill_gradient_kernel(
+    const E* logits, int vocab, size_t stride, const Scale k, double temperature, int parts, TeacherRows teacher,
+    const float* __restrict__ stats, const float* __restrict__ weights, E* gradient, size_t gradient_stride) {
+    __shared__ List list;
+    __shared__ DistillRow grow;
+    const size_t r = blockIdx.x / parts;
+    const int part = (int)(blockIdx.x - r * parts), count = (int)teacher.slots;
+    const E* z = logits + r * stride;
+    const Row<E> row(z, vocab);
+    const Slice slice(row, part, parts);
+    read_list(list, teacher.ids + r * count, count, z, vocab);
+    if (threadIdx.x < 32) {
+        const double inverse = 1.0 / temperature, scale = (double)weights[r] * inverse;
+        const Listed t = listed_sums(list, teacher.logits + r * count, kTail ? teacher.stats + 2 * r : nullptr, count,
+                                     inverse, scale, false);
+        const double m = (double)stats[3 * r], log_sum = (double)stats[3 * r + 1];
+        const double log_rest = kTail ? (double)stats[3 * r + 2] : -INFINITY;
+        if (threadIdx.x == 0)
+            grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.0, list.bad, scale);
+    }
+    __syncthreads();
+    E* out = gradient + r * gradient_stride;
+    write_dense<E, false>(row, slice, nullptr, out, grow.dense, k.L);
+    __syncthreads();
+    write_listed(list, count, slice, grow, k.L, out);
 }
 
 template <typename F>
@@ -1083,11 +1233,17 @@ int row_parts(int sm_count, size_t rows, size_t vectors, int threads, int reside
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, cudaStream_t s,
-                            Args... args) {
+cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, size_t shared,
+                            cudaStream_t s, Args... args) {
+    if (shared > (size_t)kPlainShared) {
+        const cudaError_t e =
+            cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+        if (e != cudaSuccess) return e;
+    }
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * parts));
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1095,6 +1251,14 @@ cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, i
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Blocks that share a row in the kernels whose blocks do not wait for one another: slices
+// of about kPieceVectors, more where there are few rows.
+int row_pieces(int sm_count, size_t rows, size_t vectors) {
+    size_t parts = vectors / kPieceVectors + 1;
+    while (rows * parts * 2 <= (size_t)sm_count * 4 && vectors / (parts * 2) >= (size_t)kRowThreads) parts *= 2;
+    return (int)parts;
 }
 
 }  // namespace
@@ -1106,46 +1270,59 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         const size_t vectors = z.vocab / Vec<E>::n;
         const Scale k(z.temperature);
         if (vectors < 1024)
-            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
+            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, 0, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
         return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, row_parts(sm_count, z.rows, vectors, 256, 4), 256,
-                               s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
+                               0, s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
                                (int)alternatives, out);
     });
 }
 
-cudaError_t launch_logprobs_gradient(cudaStream_t s, int, const LogitRows& z, const uint32_t* tokens,
+cudaError_t launch_logprobs_gradient(cudaStream_t s, int sm_count, const LogitRows& z, const uint32_t* tokens,
                                      size_t token_count, const float* stats, const float* entropy,
                                      const float* logprob_gradient, const float* entropy_gradient, void* gradient,
                                      size_t gradient_stride) {
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
-        logprobs_gradient_kernel<E><<<(unsigned)z.rows, kRowThreads, 0, s>>>(
-            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), tokens, (int)token_count, stats, entropy,
-            logprob_gradient, entropy_gradient, (E*)gradient, gradient_stride);
+        const int parts = row_pieces(sm_count, z.rows, z.vocab / Vec<E>::n);
+        if (z.rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
+        logprobs_gradient_kernel<E><<<(unsigned)(z.rows * parts), kRowThreads, 0, s>>>(
+            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), parts, tokens, (int)token_count, stats,
+            entropy, logprob_gradient, entropy_gradient, (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
 }
 
-cudaError_t launch_distill(cudaStream_t s, int, const LogitRows& z, const TeacherRows& teacher, const float* weights,
-                           float* loss, float* stats, void* gradient, size_t gradient_stride) {
+cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, const TeacherRows& teacher,
+                           const float* weights, float* loss, float* stats, void* gradient, size_t gradient_stride) {
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
-        auto kernel = teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>;
-        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride,
-                                                        Scale(z.temperature), z.temperature, teacher, weights, loss, stats, (E*)gradient, gradient_stride);
-        return cudaGetLastError();
+        const size_t vectors = z.vocab / Vec<E>::n;
+        int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
+        auto staged = [&](int p) { return ((vectors + p - 1) / p + 3) * 16; };
+        while (parts < kMaxCluster && staged(parts) > (size_t)kStagedTarget) parts *= 2;
+        if (staged(parts) <= (size_t)kStagedMost)
+            return launch_clusters(teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>,
+                                   z.rows, parts, kRowThreads, staged(parts), s, (const E*)z.data, (int)z.vocab,
+                                   z.stride, Scale(z.temperature), z.temperature, teacher, weights, loss, stats,
+                                   (E*)gradient, gradient_stride);
+        return launch_clusters(teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>, z.rows,
+                               parts, kRowThreads, 0, s, (const E*)z.data, (int)z.vocab, z.stride,
+                               Scale(z.temperature), z.temperature, teacher, weights, loss, stats, (E*)gradient,
+                               gradient_stride);
     });
 }
 
-cudaError_t launch_distill_gradient(cudaStream_t s, int, const LogitRows& z, const TeacherRows& teacher,
+cudaError_t launch_distill_gradient(cudaStream_t s, int sm_count, const LogitRows& z, const TeacherRows& teacher,
                                     const float* stats, const float* weights, void* gradient, size_t gradient_stride) {
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
-        auto kernel = teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>;
-        kernel<<<(unsigned)z.rows, kRowThreads, 0, s>>>((const E*)z.data, (int)z.vocab, z.stride,
-                                                        Scale(z.temperature), z.temperature, teacher, weights, nullptr, const_cast<float*>(stats),
-                                                        (E*)gradient, gradient_stride);
+        const int parts = row_pieces(sm_count, z.rows, z.vocab / Vec<E>::n);
+        if (z.rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
+        auto kernel = teacher.stats ? distill_gradient_kernel<E, true> : distill_gradient_kernel<E, false>;
+        kernel<<<(unsigned)(z.rows * parts), kRowThreads, 0, s>>>(
+            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), z.temperature, parts, teacher, stats,
+            weights, (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
 }

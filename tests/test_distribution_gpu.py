@@ -414,6 +414,33 @@ def test_distill_confident_student_keeps_its_rest(gpu, dev):
     assert bool((step.stats[:, 2] < -25).all()) and bool(step.loss.isfinite().all())
 
 
+def test_distill_padded_positions(gpu, dev):
+    """Positions where teacher and student hold no token, as token_logprobs hands them on."""
+    teacher, student = make(dev, 27, 3, 600, torch.bfloat16), make(dev, 28, 3, 600, torch.bfloat16)
+    teacher[1] = -math.inf
+    student[1] = -math.inf
+    teacher[2] = -math.inf
+    top = distribution.token_logprobs(gpu, teacher, alternatives=8)
+    for stats in (None, top.stats):
+        got = distribution.distill(gpu, student, top.top_ids, top.top_logits, teacher_stats=stats, gradient=True)
+        assert got.loss[1:].cpu().tolist() == [0.0, 0.0] and float(got.loss[0]) > 0
+        assert not bool(got.gradient[1:].any()) and bool(got.gradient[0].any())
+        back = distribution.distill_backward(gpu, student, top.top_ids, top.top_logits, got.stats,
+                                             torch.ones(3, device=dev), teacher_stats=stats)
+        assert torch.equal(back, got.gradient)
+
+
+@pytest.mark.parametrize("dtype, vocab", [(torch.float32, 420011), (torch.bfloat16, 850001)])
+def test_distill_of_very_long_rows(gpu, dev, dtype, vocab):
+    """Rows beyond what a cluster holds in shared memory are read again for the gradient."""
+    z = make(dev, 29, 2, vocab, dtype, pad=3)
+    ids, values, stats = teacher_of(dev, 30, z, 128, 1.0, unused=0.05)
+    for t in (None, stats):
+        check_distill(gpu, z, ids, values, t, torch.ones(2, device=dev), 1.0)
+    ids[1, 7] = ids[1, 9]
+    check_distill(gpu, z, ids, values, stats, torch.ones(2, device=dev), 1.0)
+
+
 def test_distill_bad_rows_are_nan(gpu, dev):
     z = make(dev, 23, 5, 300, torch.float32)
     ids, values, stats = teacher_of(dev, 24, z, 5, 1.0)
