@@ -25,6 +25,7 @@ namespace lsx {
 namespace {
 
 constexpr int kRowThreads = 256;
+constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;     // candidate keys of one selection
 constexpr int kMarkWords = 512;    // 32-bit words of the bitmap of marked vectors
 constexpr int kPlainShared = 36 << 10;   // dynamic shared memory that needs no opt-in beside the kernels' own
@@ -762,7 +763,7 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
 }
 
 // ---- lists of tokens -------------------------------------------------------------------------
-// One row's listed tokens, a slot to a thread.
+// One row's listed tokens.
 struct List {
     uint32_t ids[kMaxSlots];
     bool kept[kMaxSlots];    // names a token, and is the first slot to name it
@@ -771,33 +772,42 @@ struct List {
     int bad;                 // some slot names a token outside the vocabulary
 };
 
-// Reads a row's list and the logits it names.  Two threads per slot look for an earlier
-// slot of the same token.  Ends with the block synchronised.
+// Reads a row's list and the logits it names in [begin, end), by the first warp (slot
+// lane + 32 q).
 template <typename E>
-__device__ void read_list(List& list, const uint32_t* ids, int count, const E* z, int vocab) {
-    const int tid = threadIdx.x;
-    if (tid == 0) list.bad = 0;
-    __syncthreads();
-    if (tid < count) {
-        const uint32_t id = ids[tid];
-        const bool used = id < (uint32_t)vocab;
-        list.ids[tid] = id;
-        list.logit[tid] = used ? Vec<E>::one(z[id]) : -INFINITY;
-        list.value[tid] = 0.f;
-        if (!used && id != kUnusedToken) list.bad = 1;
+__device__ void read_list(List& list, const uint32_t* ids, int count, const E* z, int vocab, int begin, int end) {
+    constexpr int kPer = kMaxSlots / 32;
+    const int lane = threadIdx.x & 31;
+    uint32_t id[kPer];
+    bool bad = false;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        const int i = lane + 32 * q;
+        id[q] = i < count ? ids[i] : kUnusedToken;
     }
-    __syncthreads();
-    const int slot = tid >> 1;
-    bool seen = false;
-    if (slot < count)
-        for (int j = tid & 1; j < slot; j += 2) seen |= list.ids[j] == list.ids[slot];
-    seen |= (bool)__shfl_xor_sync(0xffffffffu, (int)seen, 1);
-    if (slot < count && (tid & 1) == 0) {
-        const bool kept = !seen && list.ids[slot] < (uint32_t)vocab;
-        list.kept[slot] = kept;
-        if (!kept) list.logit[slot] = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q) {
+        if (32 * q >= count) break;
+        const int i = lane + 32 * q;
+        const bool used = id[q] < (uint32_t)vocab;
+        const float logit = used && (int)id[q] >= begin && (int)id[q] < end ? Vec<E>::one(z[id[q]]) : -INFINITY;
+        bad |= !used && id[q] != kUnusedToken;
+        // the same token in an earlier slot: of these 32, or of the 32s before
+        bool again = (__match_any_sync(0xffffffffu, id[q]) & ((1u << lane) - 1)) != 0;
+#pragma unroll
+        for (int p = 0; p < q; ++p)
+#pragma unroll 8
+            for (int from = 0; from < 32; ++from) again |= __shfl_sync(0xffffffffu, id[p], from) == id[q];
+        if (i < count) {
+            list.ids[i] = id[q];
+            list.kept[i] = used && !again;
+            list.logit[i] = used && !again ? logit : -INFINITY;
+            list.value[i] = 0.f;
+        }
     }
-    __syncthreads();
+    const bool any = __any_sync(0xffffffffu, bad);
+    if (lane == 0) list.bad = any;
+    __syncwarp();
 }
 
 // ---- gradients ---------------------------------------------------------------------------
@@ -829,15 +839,16 @@ __device__ __forceinline__ void store16(void* p, uint4 w) {
 }
 
 // The dense gradient of a slice into `out` (the row's first element): vectors from
-// `staged` (slot j - lo; the ragged ends behind the full ones) or, where it is null, from
-// the row itself.  `out` may be the row.
-template <typename E, bool kLinear>
-__device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, const Dense& d, float L) {
+// `staged` (slot j - lo) or, where it is null, from the row itself.  `out` may be the row.
+// `ready` gives the coefficients, once, after the first loads are on their way.
+template <typename E, bool kLinear, typename F>
+__device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, float L, F&& ready) {
     constexpr int n = Vec<E>::n;
     const int tid = threadIdx.x, T = blockDim.x;
     // the output row may lie at another alignment than the logits
     const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (uintptr_t)(row.lead * sizeof(E));
     E* base = out - row.lead;
+    Dense d;
     auto put = [&](int j, uint4 w) {
         float v[n];
         Vec<E>::unpack(w, v);
@@ -861,16 +872,24 @@ __device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* s
     };
     int j = part.lo + tid;
     if (staged) {
+        d = ready();
         for (; j < part.hi; j += T) put(j, staged[j - part.lo]);
     } else {
-        for (; j + (kUnroll - 1) * T < part.hi; j += kUnroll * T) {
-            uint4 w[kUnroll];
+        uint4 w[kUnroll];
+        auto fetch = [&](int from) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
+            for (int u = 0; u < kUnroll; ++u)
+                if (from + u * T < part.hi) w[u] = row.full(from + u * T);
+        };
+        fetch(j);
+        d = ready();
+        while (j < part.hi) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u) put(j + u * T, w[u]);
+            for (int u = 0; u < kUnroll; ++u)
+                if (j + u * T < part.hi) put(j + u * T, w[u]);
+            j += kUnroll * T;
+            fetch(j);
         }
-        for (; j < part.hi; j += T) put(j, row.full(j));
     }
     if (part.head && tid == 0) put_ragged(0);
     if (part.last && tid == T - 1) put_ragged(row.full1);
@@ -878,13 +897,13 @@ __device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* s
 
 // `parts` blocks share a row; none waits for another.
 template <typename E>
-__global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
+__global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_gradient_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, int parts, const uint32_t* __restrict__ tokens,
     int token_count, const float* __restrict__ stats, const float* __restrict__ entropy,
     const float* __restrict__ logprob_gradient, const float* __restrict__ entropy_gradient, E* gradient,
     size_t gradient_stride) {
-    __shared__ List list;
-    __shared__ float total;
+    __shared__ uint32_t ids[kMaxSlots];
+    __shared__ float given[kMaxSlots];
     const size_t r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts), tid = threadIdx.x;
     const E* z = logits + r * stride;
@@ -892,53 +911,62 @@ __global__ void __launch_bounds__(kRowThreads) logprobs_gradient_kernel(
     const Slice slice(row, part, parts);
     const float m = stats[2 * r], log_sum = stats[2 * r + 1];
     const float h = entropy_gradient ? entropy_gradient[r] : 0.f, H = entropy ? entropy[r] : 0.f;
-    const float mine = tid < token_count ? logprob_gradient[r * token_count + tid] : 0.f;
-    read_list(list, tokens + r * token_count, token_count, z, vocab);
-    if (tid < token_count) list.value[tid] = list.ids[tid] == kUnusedToken ? 0.f : mine;
-    __syncthreads();
-    if (tid < 32) {
-        float sum = 0.f;
-        for (int i = tid; i < token_count; i += 32) sum += list.value[i];
-        sum = warp_allsum(sum);
-        if (tid == 0) total = list.bad ? NAN : sum;
+    // a slot to a thread; the listed logits are read before anything is written
+    uint32_t id = kUnusedToken;
+    float logit = 0.f;
+    if (tid < token_count) {
+        id = tokens[r * token_count + tid];
+        ids[tid] = id;
+        // NaN for a token outside the vocabulary goes through the sum into the whole row
+        given[tid] = id == kUnusedToken ? 0.f : id < (uint32_t)vocab ? logprob_gradient[r * token_count + tid] : NAN;
+        if (id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end) logit = Vec<E>::one(z[id]);
     }
-    // a token named several times adds up at its first slot
-    const bool kept = tid < token_count && list.kept[tid];
-    float own = 0.f;
-    if (kept)
-        for (int i = tid; i < token_count; ++i) own += list.ids[i] == list.ids[tid] ? list.value[i] : 0.f;
-    __syncthreads();
     const bool empty = m == -INFINITY && log_sum == 0.f;
-    Dense d = dense_zero();
-    if (!empty) {
-        d.m = m;
-        d.offset = log_sum * kLog2E;
-        d.a = -(total + (h != 0.f ? h * H : 0.f)) * k.inverse;
-        d.b = -h * kLn2 * k.inverse;
-    }
+    float total = 0.f;
+    Dense d;
+    auto ready = [&]() {
+        __syncthreads();
+        for (int i = 0; i < token_count; ++i) total += given[i];
+        d = dense_zero();
+        if (!empty) {
+            d.m = m;
+            d.offset = log_sum * kLog2E;
+            d.b = -h * kLn2 * k.inverse;
+            d.a = -(total + (h != 0.f ? h * H : 0.f)) * k.inverse;
+        } else if (total != total) {
+            d.a = NAN;
+        }
+        return d;
+    };
     E* out = gradient + r * gradient_stride;
     if (h != 0.f)
-        write_dense<E, true>(row, slice, nullptr, out, d, k.L);
+        write_dense<E, true>(row, slice, nullptr, out, k.L, ready);
     else
-        write_dense<E, false>(row, slice, nullptr, out, d, k.L);
+        write_dense<E, false>(row, slice, nullptr, out, k.L, ready);
     __syncthreads();
-    if (kept && (int)list.ids[tid] >= slice.begin && (int)list.ids[tid] < slice.end) {
-        const float y = max_nan(fmaf(list.logit[tid] - d.m, k.L, -d.offset), kLowestExponent), log_q = y * kLn2;
-        // own (1 - q) apart from the other tokens' share: own - q own loses a confident token's gradient
-        const float g = -expm1f(log_q) * own - exp2_fast(y) * (total - own + (h != 0.f ? h * (H + log_q) : 0.f));
-        out[list.ids[tid]] = Vec<E>::store(empty ? 0.f : g * k.inverse);
+    if (id >= (uint32_t)vocab || (int)id < slice.begin || (int)id >= slice.end) return;
+    // a token named several times adds up at its first slot
+    float own = 0.f;
+    for (int i = 0; i < token_count; ++i) {
+        if (ids[i] != id) continue;
+        if (i < tid) return;
+        own += given[i];
     }
+    const float y = max_nan(fmaf(logit - d.m, k.L, -d.offset), kLowestExponent), log_q = y * kLn2;
+    // own (1 - q) apart from the other tokens' share: own - q own loses a confident token's gradient
+    const float g = -expm1f(log_q) * own - exp2_fast(y) * (total - own + (h != 0.f ? h * (H + log_q) : 0.f));
+    out[id] = Vec<E>::store(empty ? total * 0.f : g * k.inverse);
 }
 
 // ---- distillation --------------------------------------------------------------------------
 // The listed tokens' side of one row in 64 bits, by one warp: sums over at most kMaxSlots
 // numbers, of which 1 - sum p is next to 0 for a confident teacher.
 struct Listed {
-    double mass;    // sum of p
-    double rest;    // the teacher's mass outside the list (0 without its statistics)
-    double m;       // the largest listed logit of the student
-    double inside;  // sum exp((z - m) / T) over the listed tokens
-    double cross;   // sum p (ln p - (z - m) / T)
+    double mass;   // sum of p
+    double rest;   // the teacher's mass outside the list (0 without its statistics)
+    float m;       // the largest listed logit of the student
+    double inside; // sum exp((z - m) / T) over the listed tokens
+    double cross;  // sum p (ln p - (z - m) / T)
 };
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -946,73 +974,72 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
-__device__ __forceinline__ double warp_max_f64(double v) {
+// max, NaN passed over
+__device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
 }
 
-// Also leaves scale * p in list.value.
-__device__ Listed listed_sums(List& list, const float* values, const float* stats, int count, double inverse,
-                              double scale, bool student) {
+// By the warp that read the list.  Also leaves scale * p in list.value.
+template <bool kStudent>
+__device__ Listed listed_sums(List& list, double* work, const float* values, const float* stats, int count,
+                              double inverse, double scale) {
     const int lane = threadIdx.x & 31;
-    constexpr int kPer = kMaxSlots / 32;
-    double a[kPer], top = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const int i = lane + 32 * q;
-        a[q] = i < count && list.kept[i] ? (double)values[i] : -INFINITY;
-        top = fmax(top, a[q]);
+    Listed t{0.0, 0.0, -INFINITY, 0.0, 0.0};
+    float top = -INFINITY;
+    for (int i = lane; i < count; i += 32) {
+        const float value = list.kept[i] ? values[i] : -INFINITY;
+        list.value[i] = value;
+        top = fmaxf(top, value);
+        if (kStudent) t.m = fmaxf(t.m, list.logit[i]);
     }
-    double shift, norm;
+    if (kStudent) t.m = warp_max(t.m);
+    double shift, norm = 0.0;
     bool none = false;  // the teacher's row holds no token: it asks for nothing
     if (stats) {
         none = stats[0] == -INFINITY && stats[1] == 0.f;
         shift = none ? 0.0 : (double)stats[0];
         norm = (double)stats[1];
     } else {
-        top = warp_max_f64(top);
-        shift = top == -INFINITY ? 0.0 : top;
-        double sum = 0.0;
-#pragma unroll
-        for (int q = 0; q < kPer; ++q)
-            if (32 * q < count) sum += exp((a[q] - shift) * inverse);
-        sum = warp_sum_f64(sum);
-        norm = sum > 0.0 ? log(sum) : (sum == 0.0 ? 0.0 : sum);
+        top = warp_max(top);
+        shift = top == -INFINITY ? 0.0 : (double)top;
     }
-    Listed t{0.0, 0.0, -INFINITY, 0.0, 0.0};
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        if (32 * q >= count) break;
-        a[q] = (a[q] - shift) * inverse - norm;  // ln p
-        const double p = exp(a[q]);
+    for (int i = lane; i < count; i += 32) {
+        const double log_p = ((double)list.value[i] - shift) * inverse - norm, p = exp(log_p);
         t.mass += p;
-        const int i = lane + 32 * q;
-        if (i < count) list.value[i] = (float)(scale * p);
+        if (kStudent) {
+            const float z = list.logit[i];
+            const double log_q = z == -INFINITY ? -INFINITY : ((double)z - (double)t.m) * inverse;
+            t.inside += exp(log_q);
+            work[i] = p != 0.0 ? log_p - log_q : 0.0;
+        }
+        work[kMaxSlots + i] = p;
     }
     t.mass = warp_sum_f64(t.mass);
-    if (stats && !none) t.rest = t.mass < 1.0 ? 1.0 - t.mass : (t.mass >= 1.0 ? 0.0 : t.mass);
-    if (!student) return t;
-    for (int i = lane; i < count; i += 32) t.m = fmax(t.m, (double)list.logit[i]);
-    t.m = warp_max_f64(t.m);
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const int i = lane + 32 * q;
-        if (i >= count) break;
-        const double z = (double)list.logit[i];
-        const double log_q = z == -INFINITY ? -INFINITY : (z - t.m) * inverse;
-        t.inside += exp(log_q);
-        const double p = exp(a[q]);
-        if (p != 0.0) t.cross += p * (a[q] - log_q);
+    if (kStudent) t.inside = warp_sum_f64(t.inside);
+    double share = 1.0;
+    norm = 0.0;
+    if (stats) {
+        if (!none) t.rest = t.mass < 1.0 ? 1.0 - t.mass : (t.mass >= 1.0 ? 0.0 : t.mass);
+    } else if (t.mass != 0.0) {  // normalised over the list
+        share = 1.0 / t.mass;
+        norm = log(t.mass);
+        t.mass = t.mass == t.mass ? 1.0 : t.mass;
     }
-    t.inside = warp_sum_f64(t.inside);
-    t.cross = warp_sum_f64(t.cross);
+    for (int i = lane; i < count; i += 32) {
+        const double p = work[kMaxSlots + i] * share;
+        list.value[i] = (float)(scale * p);
+        if (kStudent && p != 0.0) t.cross += p * (work[i] - norm);
+    }
+    if (kStudent) t.cross = warp_sum_f64(t.cross);
+    __syncwarp();
     return t;
 }
 
 // The tokens outside the list are one outcome only where the student's share of them is
 // a normal f32 number (2^-126 and up).
-constexpr double kSmallestLogShare = -87.3365447505531;
+constexpr float kSmallestLogShare = -87.33654475f;
 
 // What the gradient of one row needs beside its list: listed elements get q a - value, q
 // against `offset`.
@@ -1024,19 +1051,19 @@ struct DistillRow {
 
 // The tokens outside the list are exponentiated against their own sum: 2^y = q_i / q_r
 // stays in range and (P q_r - p_r) is the whole coefficient, however small q_r is.
-__device__ DistillRow distill_row(const Listed& t, double m, double log_sum, double log_rest, bool empty, bool bad,
+__device__ DistillRow distill_row(const Listed& t, float m, float log_sum, float log_rest, bool empty, bool bad,
                                   double scale) {
-    const double log_share = log_rest - log_sum;
+    const float log_share = log_rest - log_sum;
     const bool tail = log_share >= kSmallestLogShare;
     const double mass = t.mass + (tail ? t.rest : 0.0);
     DistillRow g;
-    g.m = (float)m;
-    g.offset = (float)(log_sum * 1.4426950408889634);
+    g.m = m;
+    g.offset = log_sum * kLog2E;
     g.a = bad ? NAN : (float)(scale * mass);
     g.zero = empty;
     g.dense.m = g.m;
-    g.dense.offset = tail ? (float)(log_rest * 1.4426950408889634) : g.offset;
-    g.dense.a = bad ? NAN : (float)(scale * (tail ? mass * exp(log_share) - t.rest : mass));
+    g.dense.offset = tail ? log_rest * kLog2E : g.offset;
+    g.dense.a = bad ? NAN : (float)(scale * (tail ? mass * (double)expf(log_share) - t.rest : mass));
     g.dense.b = 0.f;
     if (empty) g.dense = dense_zero();
     return g;
@@ -1058,20 +1085,27 @@ __device__ __forceinline__ void copy16_async(void* shared, const void* global) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
 }
 
+// Barrier of the warps behind the first.
+__device__ __forceinline__ void others_barrier() {
+    asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads - 32) : "memory");
+}
+
 // Loss, statistics and, where wanted, the gradient.  A cluster of blocks shares a row.
+// The first warp takes the list, the others the slice.
 // kStaged: each block holds its slice in shared memory, so the row is read once: the
 // listed tokens are struck out there (their share is summed by itself, in 64 bits), the rest
 // is summed, the blocks exchange their sums, and the gradient is formed from the same
-// copy.  Without it (rows too long for that) the slice is read again for the gradient,
-// and a bitmap of marked vectors tells the sum which elements to leave out.
+// copy.  Without it (no gradient, or rows too long for that) the slice streams through
+// registers, and a bitmap of marked vectors tells the sum which elements to leave out.
 template <typename E, bool kTail, bool kStaged>
-__global__ void __launch_bounds__(kRowThreads) distill_kernel(
+__global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double temperature, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     constexpr int n = Vec<E>::n;
     extern __shared__ __align__(16) uint4 staged[];
     __shared__ Sums scratch[33];
     __shared__ List list;
+    __shared__ double work[2 * kMaxSlots];
     __shared__ DistillRow grow;
     __shared__ Sums shares[kMaxCluster];
     const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x, T = blockDim.x;
@@ -1081,58 +1115,60 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    const int full = slice.hi - slice.lo;
-    if (kStaged) {
-        for (int i = tid; i < full; i += T) copy16_async(&staged[i], row.base + (long long)(slice.lo + i) * n);
-        // the ragged ends follow, -inf beyond the row
-        if (slice.head && tid == 0) {
-            float v[n];
-            row.ragged(0, v);
-            staged[full] = Vec<E>::pack(v);
-        }
-        if (slice.last && tid == T - 1) {
-            float v[n];
-            row.ragged(row.full1, v);
-            staged[full + 1] = Vec<E>::pack(v);
-        }
-    }
-    read_list(list, teacher.ids + r * count, count, z, vocab);
+    const bool lister = tid < 32;
+    const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
     const double inverse = 1.0 / temperature;
-    const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
     Listed t;
-    if (tid < 32)
-        t = listed_sums(list, teacher.logits + r * count, kTail ? teacher.stats + 2 * r : nullptr, count, inverse,
-                        scale, true);
     Running acc;
     if (kStaged) {
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        __syncthreads();
-        if (tid < count && list.kept[tid]) {
-            const int id = (int)list.ids[tid];
-            if (id >= slice.begin && id < slice.end) {
-                const long long at = (long long)id + row.lead;
+        const int full = slice.hi - slice.lo;
+        if (lister) {
+            read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
+            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
+            t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+        } else {
+            const int lane = tid - 32, others = T - 32;
+            const E* from = row.base + (long long)slice.lo * n;
+            for (int i = lane; i < full; i += others) copy16_async(&staged[i], from + (long long)i * n);
+            const uint32_t id = lane < count ? teacher.ids[r * count + lane] : kUnusedToken;
+            // the ragged ends follow, -inf beyond the row
+            if (slice.head && lane == 0) {
+                float v[n];
+                row.ragged(0, v);
+                staged[full] = Vec<E>::pack(v);
+            }
+            if (slice.last && lane == others - 1) {
+                float v[n];
+                row.ragged(row.full1, v);
+                staged[full + 1] = Vec<E>::pack(v);
+            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            others_barrier();
+            if (id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end) {
+                const uint32_t at = id + row.lead;
                 const int j = (int)(at / n);
                 const int slot = j < row.full0 ? full : j >= row.full1 ? full + 1 : j - slice.lo;
                 reinterpret_cast<E*>(&staged[slot])[at % n] = Vec<E>::store(-INFINITY);
             }
-        }
-        __syncthreads();
-        for (int i = tid; i < full; i += T) {
-            const uint4 w = staged[i];
-            float v[n];
-            Vec<E>::unpack(w, v);
-            acc.template add<n>(v, Vec<E>::top(w), i, k);
-        }
-        const int ragged = slice.head && tid == 0 ? full : slice.last && tid == T - 1 ? full + 1 : -1;
-        if (ragged >= 0) {
-            const uint4 w = staged[ragged];
-            float v[n];
-            Vec<E>::unpack(w, v);
-            acc.template add<n>(v, Vec<E>::top(w), 0, k);
+            others_barrier();
+            auto take = [&](int i) {
+                const uint4 w = staged[i];
+                float v[n];
+                Vec<E>::unpack(w, v);
+                acc.template add<n>(v, Vec<E>::top(w), i, k);
+            };
+            for (int i = lane; i < full; i += others) take(i);
+            if (slice.head && lane == 0) take(full);
+            if (slice.last && lane == others - 1) take(full + 1);
         }
     } else {
         __shared__ Marks marks;
         build_marks(marks, teacher.ids + r * count, count, row);
+        if (lister) {
+            read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
+            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
+            t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+        }
         stream_slice<E, true>(row, slice, &marks, k, acc);
     }
     Sums rest = block_sums(acc, k.L, scratch);
@@ -1150,64 +1186,72 @@ __global__ void __launch_bounds__(kRowThreads) distill_kernel(
             rest.S += x.S;
         }
     }
-    if (tid < 32) {
-        const double m = fmax((double)rest.m, t.m);
-        const double below = rest.S == 0.f ? -INFINITY : ((double)rest.m - m) * inverse;
-        const double sum = (t.inside == 0.0 ? 0.0 : t.inside * exp((t.m - m) * inverse)) +
-                           (rest.S == 0.f ? 0.0 : (double)rest.S * exp(below));
-        const bool empty = sum == 0.0;
-        const double log_sum = empty ? 0.0 : log(sum);
-        const double log_rest = kTail && rest.S != 0.f ? log((double)rest.S) + below : -INFINITY;
-        if (part == 0 && tid == 0) {
+    if (tid == 0) {
+        // both shares around the larger maximum; sum - 1 apart, since ln(sum) may be all of it
+        const float m = fmaxf(rest.m, t.m);
+        const float below = rest.S == 0.f ? -INFINITY : (rest.m - m) * k.inverse;
+        const double outside = rest.S == 0.f ? 0.0 : (double)rest.S * (double)expf(below);
+        const double inside = t.inside == 0.0 ? 0.0 : t.inside * (t.m == m ? 1.0 : (double)expf((t.m - m) * k.inverse));
+        const bool empty = inside + outside == 0.0;
+        const float log_sum = empty ? 0.f : log1pf((float)(inside - 1.0 + outside));
+        const float log_rest = kTail && rest.S != 0.f ? logf(rest.S) + below : -INFINITY;
+        if (gradient)
+            grow = distill_row(t, m, log_sum, log_rest, empty, list.bad,
+                               (weights ? (double)weights[r] : 1.0) * inverse);
+        if (part == 0) {
             if (loss) {
                 double value = t.mass == 0.0        ? 0.0
                                : t.cross == INFINITY ? INFINITY
-                                                     : t.cross + t.mass * ((m - t.m) * inverse + log_sum);
+                                                     : t.cross + t.mass * (((double)m - (double)t.m) * inverse + log_sum);
                 if (kTail && t.rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
                     value += t.rest * (log(t.rest) - log_rest + log_sum);
-                loss[r] = list.bad || t.mass != t.mass || sum != sum ? NAN : (float)value;
+                loss[r] = list.bad || t.mass != t.mass || log_sum != log_sum ? NAN : (float)value;
             }
             if (stats) {
-                stats[3 * r] = (float)m;
-                stats[3 * r + 1] = (float)log_sum;
-                stats[3 * r + 2] = (float)log_rest;
+                stats[3 * r] = m;
+                stats[3 * r + 1] = log_sum;
+                stats[3 * r + 2] = log_rest;
             }
         }
-        if (gradient && tid == 0) grow = distill_row(t, m, log_sum, log_rest, empty, list.bad, scale);
     }
     if (!gradient) return;
-    __syncthreads();
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, kStaged ? staged : nullptr, out, grow.dense, k.L);
+    write_dense<E, false>(row, slice, kStaged ? staged : nullptr, out, k.L, [&]() {
+        __syncthreads();
+        return grow.dense;
+    });
     __syncthreads();
     write_listed(list, count, slice, grow, k.L, out);
 }
 
 // The gradient from saved statistics; `parts` blocks share a row, none waits for another.
 template <typename E, bool kTail>
-__global__ void __launch_bounds__(kRowThreads) distill_gradient_kernel(
+__global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_gradient_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double temperature, int parts, TeacherRows teacher,
     const float* __restrict__ stats, const float* __restrict__ weights, E* gradient, size_t gradient_stride) {
     __shared__ List list;
+    __shared__ double work[2 * kMaxSlots];
     __shared__ DistillRow grow;
     const size_t r = blockIdx.x / parts;
     const int part = (int)(blockIdx.x - r * parts), count = (int)teacher.slots;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    read_list(list, teacher.ids + r * count, count, z, vocab);
-    if (threadIdx.x < 32) {
-        const double inverse = 1.0 / temperature, scale = (double)weights[r] * inverse;
-        const Listed t = listed_sums(list, teacher.logits + r * count, kTail ? teacher.stats + 2 * r : nullptr, count,
-                                     inverse, scale, false);
-        const double m = (double)stats[3 * r], log_sum = (double)stats[3 * r + 1];
-        const double log_rest = kTail ? (double)stats[3 * r + 2] : -INFINITY;
-        if (threadIdx.x == 0)
-            grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.0, list.bad, scale);
-    }
-    __syncthreads();
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, nullptr, out, grow.dense, k.L);
+    write_dense<E, false>(row, slice, nullptr, out, k.L, [&]() {
+        if (threadIdx.x < 32) {
+            const double inverse = 1.0 / temperature, scale = (double)weights[r] * inverse;
+            const float m = stats[3 * r], log_sum = stats[3 * r + 1], log_rest = kTail ? stats[3 * r + 2] : -INFINITY;
+            // (another block may be writing over the rest of the row)
+            read_list(list, teacher.ids + r * count, count, z, vocab, slice.begin, slice.end);
+            const Listed t = listed_sums<false>(list, work, teacher.logits + r * count,
+                                                kTail ? teacher.stats + 2 * r : nullptr, count, inverse, scale);
+            if (threadIdx.x == 0)
+                grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.f, list.bad, scale);
+        }
+        __syncthreads();
+        return grow.dense;
+    });
     __syncthreads();
     write_listed(list, count, slice, grow, k.L, out);
 }
@@ -1257,7 +1301,7 @@ cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, i
 // of about kPieceVectors, more where there are few rows.
 int row_pieces(int sm_count, size_t rows, size_t vectors) {
     size_t parts = vectors / kPieceVectors + 1;
-    while (rows * parts * 2 <= (size_t)sm_count * 4 && vectors / (parts * 2) >= (size_t)kRowThreads) parts *= 2;
+    while (rows * parts * 2 <= (size_t)sm_count * 8 && vectors / (parts * 2) >= (size_t)kPieceThreads) parts *= 2;
     return (int)parts;
 }
 
@@ -1286,7 +1330,7 @@ cudaError_t launch_logprobs_gradient(cudaStream_t s, int sm_count, const LogitRo
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const int parts = row_pieces(sm_count, z.rows, z.vocab / Vec<E>::n);
         if (z.rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
-        logprobs_gradient_kernel<E><<<(unsigned)(z.rows * parts), kRowThreads, 0, s>>>(
+        logprobs_gradient_kernel<E><<<(unsigned)(z.rows * parts), kPieceThreads, 0, s>>>(
             (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), parts, tokens, (int)token_count, stats,
             entropy, logprob_gradient, entropy_gradient, (E*)gradient, gradient_stride);
         return cudaGetLastError();
@@ -1300,8 +1344,9 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
         const size_t vectors = z.vocab / Vec<E>::n;
         int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
         auto staged = [&](int p) { return ((vectors + p - 1) / p + 3) * 16; };
-        while (parts < kMaxCluster && staged(parts) > (size_t)kStagedTarget) parts *= 2;
-        if (staged(parts) <= (size_t)kStagedMost)
+        if (gradient)
+            while (parts < kMaxCluster && staged(parts) > (size_t)kStagedTarget) parts *= 2;
+        if (gradient && staged(parts) <= (size_t)kStagedMost)
             return launch_clusters(teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>,
                                    z.rows, parts, kRowThreads, staged(parts), s, (const E*)z.data, (int)z.vocab,
                                    z.stride, Scale(z.temperature), z.temperature, teacher, weights, loss, stats,
@@ -1320,7 +1365,7 @@ cudaError_t launch_distill_gradient(cudaStream_t s, int sm_count, const LogitRow
         const int parts = row_pieces(sm_count, z.rows, z.vocab / Vec<E>::n);
         if (z.rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
         auto kernel = teacher.stats ? distill_gradient_kernel<E, true> : distill_gradient_kernel<E, false>;
-        kernel<<<(unsigned)(z.rows * parts), kRowThreads, 0, s>>>(
+        kernel<<<(unsigned)(z.rows * parts), kPieceThreads, 0, s>>>(
             (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), z.temperature, parts, teacher, stats,
             weights, (E*)gradient, gradient_stride);
         return cudaGetLastError();
