@@ -1091,7 +1091,7 @@ __device__ __forceinline__ void others_barrier() {
 }
 
 // Loss, statistics and, where wanted, the gradient.  A cluster of blocks shares a row.
-// The first warp takes the list, the others the slice.
+// The first block's first warp takes the list, the other warps the slices.
 // kStaged: each block holds its slice in shared memory, so the row is read once: the
 // listed tokens are struck out there (their share is summed by itself, in 64 bits), the rest
 // is summed, the blocks exchange their sums, and the gradient is formed from the same
@@ -1106,6 +1106,7 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
     __shared__ Sums scratch[33];
     __shared__ List list;
     __shared__ double work[2 * kMaxSlots];
+    __shared__ Listed listed;
     __shared__ DistillRow grow;
     __shared__ Sums shares[kMaxCluster];
     const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x, T = blockDim.x;
@@ -1118,14 +1119,16 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
     const bool lister = tid < 32;
     const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
     const double inverse = 1.0 / temperature;
-    Listed t;
+    const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
     Running acc;
     if (kStaged) {
         const int full = slice.hi - slice.lo;
         if (lister) {
-            read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
-            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
-            t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+            if (part == 0) {
+                read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
+                const Listed t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+                if (tid == 0) listed = t;
+            }
         } else {
             const int lane = tid - 32, others = T - 32;
             const E* from = row.base + (long long)slice.lo * n;
@@ -1164,10 +1167,10 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
     } else {
         __shared__ Marks marks;
         build_marks(marks, teacher.ids + r * count, count, row);
-        if (lister) {
+        if (lister && part == 0) {
             read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
-            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
-            t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+            const Listed t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
+            if (tid == 0) listed = t;
         }
         stream_slice<E, true>(row, slice, &marks, k, acc);
     }
@@ -1175,6 +1178,21 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
     if (parts > 1) {
         cluster_wait();
         if (tid < parts) *in_block(&shares[part], tid) = rest;
+        if (part == 0) {  // the list too, a block to a warp
+            for (int to = 1 + (tid >> 5); to < parts; to += T >> 5) {
+                List* there = in_block(&list, to);
+                for (int i = tid & 31; i < count; i += 32) {
+                    there->ids[i] = list.ids[i];
+                    there->kept[i] = list.kept[i];
+                    there->logit[i] = list.logit[i];
+                    there->value[i] = list.value[i];
+                }
+                if ((tid & 31) == 0) {
+                    there->bad = list.bad;
+                    *in_block(&listed, to) = listed;
+                }
+            }
+        }
         cluster_arrive();
         cluster_wait();
         rest = shares[0];
@@ -1187,6 +1205,7 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
         }
     }
     if (tid == 0) {
+        const Listed t = listed;
         // both shares around the larger maximum; sum - 1 apart, since ln(sum) may be all of it
         const float m = fmaxf(rest.m, t.m);
         const float below = rest.S == 0.f ? -INFINITY : (rest.m - m) * k.inverse;
@@ -1196,8 +1215,7 @@ __global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
         const float log_sum = empty ? 0.f : log1pf((float)(inside - 1.0 + outside));
         const float log_rest = kTail && rest.S != 0.f ? logf(rest.S) + below : -INFINITY;
         if (gradient)
-            grow = distill_row(t, m, log_sum, log_rest, empty, list.bad,
-                               (weights ? (double)weights[r] : 1.0) * inverse);
+            grow = distill_row(t, m, log_sum, log_rest, empty, list.bad, scale);
         if (part == 0) {
             if (loss) {
                 double value = t.mass == 0.0        ? 0.0
