@@ -14,7 +14,12 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
+#include <map>
+#include <mutex>
 #include <string>
+#include <tuple>
+#include <cstdlib>
+#include <cstdio>
 #include <type_traits>
 
 #include "device_common.cuh"
@@ -28,6 +33,7 @@ constexpr int kRowThreads = 256;
 constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;     // candidate keys of one selection
 constexpr int kMarkWords = 512;    // 32-bit words of the bitmap of marked vectors
+constexpr int kStepShared = 8448;        // what the step kernel holds beside its slice, the system's share included
 constexpr int kPlainShared = 36 << 10;   // dynamic shared memory that needs no opt-in beside the kernels' own
 constexpr int kStagedTarget = 40 << 10;  // a slice kept in shared memory: 4 blocks on an SM
 constexpr int kStagedMost = 200 << 10;   // and at most
@@ -256,46 +262,7 @@ __device__ __forceinline__ int mark_position(const Marks& M, long long first) {
 }
 
 // ---- running sums of a softmax ---------------------------------------------------
-// S = sum 2^y and W = sum 2^y y over the elements seen (in two halves), y against the
-// reference r; S == 0 exactly while only -inf has been seen.  m is the largest element,
-// `at` the first vector that holds it and `second` the largest element of the others.
-struct Running {
-    float r = 0.f, limit = -INFINITY, m = -INFINITY, second = -INFINITY;
-    float2 S2 = {0.f, 0.f}, W2 = {0.f, 0.f};
-    int at = -1;
-    __device__ __forceinline__ void rise(float top, const Scale& k) {
-        if (S2.x + S2.y != 0.f) {
-            const float shift = (r - top) * k.L;
-            const float f = exp2_fast(shift);
-            const bool none = f == 0.f;
-            W2.x = none ? 0.f : f * fmaf(shift, S2.x, W2.x);
-            W2.y = none ? 0.f : f * fmaf(shift, S2.y, W2.y);
-            S2.x *= f;
-            S2.y *= f;
-        }
-        r = top;
-        limit = top + k.slack;
-    }
-    template <int n>
-    __device__ __forceinline__ void add(const float* v, float top, int j, const Scale& k) {
-        second = fmaxf(second, fminf(m, top));
-        at = top > m ? j : at;
-        m = fmaxf(m, top);
-        if (top > limit) rise(top, k);
-        const float2 back = {-r, -r}, scale = {k.L, k.L};
-#pragma unroll
-        for (int e = 0; e < n; e += 2) {
-            float2 y = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), back), scale);
-            y.x = max_nan(y.x, kLowestExponent);
-            y.y = max_nan(y.y, kLowestExponent);
-            const float2 p = {exp2_fast(y.x), exp2_fast(y.y)};
-            S2 = __fadd2_rn(S2, p);
-            W2 = __ffma2_rn(p, y, W2);
-        }
-    }
-};
-
-// Sums over several threads, against their own maximum.
+// Sums over several elements, against one of them.
 struct Sums {
     float m, S, W;
     // The same sums against M >= m.
@@ -308,8 +275,57 @@ struct Sums {
     }
 };
 
-__device__ __forceinline__ Sums warp_sums(Sums x, float L) {
-    float M = x.m;
+// S = sum 2^y and W = sum 2^y y over the elements seen (in two halves), y against the
+// reference r; S == 0 exactly while only -inf has been seen.  m is the largest element,
+// `at` the first vector that holds it and `second` the largest element of the others.
+// Without kRanked only S and m.
+template <bool kRanked>
+struct Running {
+    float r = 0.f, limit = -INFINITY, m = -INFINITY, second = -INFINITY;
+    float2 S2 = {0.f, 0.f}, W2 = {0.f, 0.f};
+    int at = -1;
+    __device__ __forceinline__ void rise(float top, const Scale& k) {
+        if (S2.x + S2.y != 0.f) {
+            const float shift = (r - top) * k.L;
+            const float f = exp2_fast(shift);
+            const bool none = f == 0.f;
+            if (kRanked) {
+                W2.x = none ? 0.f : f * fmaf(shift, S2.x, W2.x);
+                W2.y = none ? 0.f : f * fmaf(shift, S2.y, W2.y);
+            }
+            S2.x *= f;
+            S2.y *= f;
+        }
+        r = top;
+        limit = top + k.slack;
+    }
+    template <int n>
+    __device__ __forceinline__ void add(const float* v, float top, int j, const Scale& k) {
+        if (kRanked) {
+            second = fmaxf(second, fminf(m, top));
+            at = top > m ? j : at;
+        }
+        m = fmaxf(m, top);
+        if (top > limit) rise(top, k);
+        const float2 back = {-r, -r}, scale = {k.L, k.L};
+#pragma unroll
+        for (int e = 0; e < n; e += 2) {
+            float2 y = __fmul2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), back), scale);
+            if (kRanked) {  // 0 * y stays 0
+                y.x = max_nan(y.x, kLowestExponent);
+                y.y = max_nan(y.y, kLowestExponent);
+            }
+            const float2 p = {exp2_fast(y.x), exp2_fast(y.y)};
+            S2 = __fadd2_rn(S2, p);
+            if (kRanked) W2 = __ffma2_rn(p, y, W2);
+        }
+    }
+    __device__ __forceinline__ Sums sums() const { return {r, S2.x + S2.y, W2.x + W2.y}; }
+};
+
+// A warp's sums, each lane's against its own reference x.m; `top` is a lane's largest element.
+__device__ __forceinline__ Sums warp_sums(Sums x, float top, float L) {
+    float M = top;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
     x.rebase(M, L);
@@ -318,23 +334,19 @@ __device__ __forceinline__ Sums warp_sums(Sums x, float L) {
 
 // The block's sums, in every thread.  `scratch` holds one entry per warp and is free
 // again after the caller's next block barrier.
-__device__ __forceinline__ Sums block_sums(const Running& a, float L, Sums* scratch) {
-    Sums x{a.r, a.S2.x + a.S2.y, a.W2.x + a.W2.y};
-    float M = a.m;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    x.rebase(M, L);
-    x = {M, warp_allsum(x.S), warp_allsum(x.W)};
+template <bool kRanked>
+__device__ __forceinline__ Sums block_sums(const Running<kRanked>& a, float L, Sums* scratch) {
+    Sums x = warp_sums(a.sums(), a.m, L);
     const int lane = threadIdx.x & 31;
     if (lane == 0) scratch[threadIdx.x >> 5] = x;
     __syncthreads();
     x = lane < (int)(blockDim.x >> 5) ? scratch[lane] : Sums{-INFINITY, 0.f, 0.f};
-    return warp_sums(x, L);
+    return warp_sums(x, x.m, L);
 }
 
-template <typename E, bool kExclude>
+template <typename E, bool kExclude, bool kRanked>
 __device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& part, const Marks* M, const Scale& k,
-                                             Running& acc) {
+                                             Running<kRanked>& acc) {
     constexpr int n = Vec<E>::n;
     auto exclude = [&](int j, float* v) {
         int pos = mark_position(*M, row.first(j));
@@ -433,16 +445,16 @@ struct Partial {
 };
 
 template <typename E>
-__device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Running& acc, const Scale& k, Sums* scratch,
+__device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Running<true>& acc, const Scale& k, Sums* scratch,
                               int* owner) {
     const Sums x = block_sums(acc, k.L, scratch);
     Partial p{x.m, x.S - 1.f, x.W, x.S != 0.f};
     if (x.S != 0.f && x.S < kPeaked) {  // the maximum is unique
         if (acc.m == x.m) *owner = threadIdx.x;
         __syncthreads();
-        Running others = acc;
+        Running<true> others = acc;
         if ((int)threadIdx.x == *owner) {
-            others = Running();
+            others = Running<true>();
             others.m = x.m;
         }
         if (threadIdx.x < 32) {
@@ -639,7 +651,7 @@ __device__ void select_by_pieces(Selection& P, const E* z, int begin, int end, i
 // to select_by_pieces.
 template <typename E>
 __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& part, const E* z, int top,
-                                  const Running& acc, int cap) {
+                                  const Running<true>& acc, int cap) {
     constexpr int n = Vec<E>::n;
     const int tid = threadIdx.x, lane = tid & 31, T = blockDim.x;
     const unsigned long long mine =
@@ -716,7 +728,7 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     }
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    Running acc;
+    Running<true> acc;
     stream_slice<E, false>(row, slice, nullptr, k, acc);
     Partial sums = slice_sums(row, slice, acc, k, scratch, &owner);
     // clusters keep the upper half of the list for the blocks' best keys
@@ -765,10 +777,9 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
 // ---- lists of tokens -------------------------------------------------------------------------
 // One row's listed tokens.
 struct List {
-    uint32_t ids[kMaxSlots];
-    bool kept[kMaxSlots];    // names a token, and is the first slot to name it
-    float logit[kMaxSlots];  // the row's logit of a kept token, else -inf
-    float value[kMaxSlots];  // what the operator keeps with the slot
+    uint32_t ids[kMaxSlots];  // kUnusedToken but in the first slot that names a token
+    float logit[kMaxSlots];   // the row's logit of that token, else -inf
+    float value[kMaxSlots];   // what the operator keeps with the slot
     int bad;                 // some slot names a token outside the vocabulary
 };
 
@@ -799,8 +810,7 @@ __device__ void read_list(List& list, const uint32_t* ids, int count, const E* z
 #pragma unroll 8
             for (int from = 0; from < 32; ++from) again |= __shfl_sync(0xffffffffu, id[p], from) == id[q];
         if (i < count) {
-            list.ids[i] = id[q];
-            list.kept[i] = used && !again;
+            list.ids[i] = used && !again ? id[q] : kUnusedToken;
             list.logit[i] = used && !again ? logit : -INFINITY;
             list.value[i] = 0.f;
         }
@@ -825,8 +835,10 @@ __device__ __forceinline__ void dense_vector(float* v, const Dense& d, float L) 
 #pragma unroll
     for (int e = 0; e < n; e += 2) {
         float2 y = __ffma2_rn(__fadd2_rn(make_float2(v[e], v[e + 1]), back), scale, offset);
-        y.x = max_nan(y.x, kLowestExponent);
-        y.y = max_nan(y.y, kLowestExponent);
+        if (kLinear) {  // 0 * y stays 0
+            y.x = max_nan(y.x, kLowestExponent);
+            y.y = max_nan(y.y, kLowestExponent);
+        }
         const float2 p = {exp2_fast(y.x), exp2_fast(y.y)};
         const float2 g = __fmul2_rn(p, kLinear ? __ffma2_rn(b, y, a) : a);
         v[e] = g.x;
@@ -839,12 +851,12 @@ __device__ __forceinline__ void store16(void* p, uint4 w) {
 }
 
 // The dense gradient of a slice into `out` (the row's first element): vectors from
-// `staged` (slot j - lo) or, where it is null, from the row itself.  `out` may be the row.
-// `ready` gives the coefficients, once, after the first loads are on their way.
+// `staged` (slot j - lo) or, where it is null, from the row itself, by T threads.  `out` may
+// be the row.  `ready` gives the coefficients, once, after the first loads are on their way.
 template <typename E, bool kLinear, typename F>
-__device__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, float L, F&& ready) {
+__device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, float L,
+                                            int tid, int T, F&& ready) {
     constexpr int n = Vec<E>::n;
-    const int tid = threadIdx.x, T = blockDim.x;
     // the output row may lie at another alignment than the logits
     const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (uintptr_t)(row.lead * sizeof(E));
     E* base = out - row.lead;
@@ -940,9 +952,9 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
     };
     E* out = gradient + r * gradient_stride;
     if (h != 0.f)
-        write_dense<E, true>(row, slice, nullptr, out, k.L, ready);
+        write_dense<E, true>(row, slice, nullptr, out, k.L, tid, kPieceThreads, ready);
     else
-        write_dense<E, false>(row, slice, nullptr, out, k.L, ready);
+        write_dense<E, false>(row, slice, nullptr, out, k.L, tid, kPieceThreads, ready);
     __syncthreads();
     if (id >= (uint32_t)vocab || (int)id < slice.begin || (int)id >= slice.end) return;
     // a token named several times adds up at its first slot
@@ -964,6 +976,7 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
 struct Listed {
     double mass;   // sum of p
     double rest;   // the teacher's mass outside the list (0 without its statistics)
+    double log_rest;
     float m;       // the largest listed logit of the student
     double inside; // sum exp((z - m) / T) over the listed tokens
     double cross;  // sum p (ln p - (z - m) / T)
@@ -986,10 +999,10 @@ template <bool kStudent>
 __device__ Listed listed_sums(List& list, double* work, const float* values, const float* stats, int count,
                               double inverse, double scale) {
     const int lane = threadIdx.x & 31;
-    Listed t{0.0, 0.0, -INFINITY, 0.0, 0.0};
+    Listed t{0.0, 0.0, 0.0, -INFINITY, 0.0, 0.0};
     float top = -INFINITY;
     for (int i = lane; i < count; i += 32) {
-        const float value = list.kept[i] ? values[i] : -INFINITY;
+        const float value = list.ids[i] != kUnusedToken ? values[i] : -INFINITY;
         list.value[i] = value;
         top = fmaxf(top, value);
         if (kStudent) t.m = fmaxf(t.m, list.logit[i]);
@@ -1022,6 +1035,7 @@ __device__ Listed listed_sums(List& list, double* work, const float* values, con
     norm = 0.0;
     if (stats) {
         if (!none) t.rest = t.mass < 1.0 ? 1.0 - t.mass : (t.mass >= 1.0 ? 0.0 : t.mass);
+        t.log_rest = log(t.rest);
     } else if (t.mass != 0.0) {  // normalised over the list
         share = 1.0 / t.mass;
         norm = log(t.mass);
@@ -1051,19 +1065,19 @@ struct DistillRow {
 
 // The tokens outside the list are exponentiated against their own sum: 2^y = q_i / q_r
 // stays in range and (P q_r - p_r) is the whole coefficient, however small q_r is.
-__device__ DistillRow distill_row(const Listed& t, float m, float log_sum, float log_rest, bool empty, bool bad,
-                                  double scale) {
+__device__ __forceinline__ DistillRow distill_row(const Listed& t, float m, float log_sum, float log_rest, bool empty,
+                                                  bool bad, float scale) {
     const float log_share = log_rest - log_sum;
     const bool tail = log_share >= kSmallestLogShare;
-    const double mass = t.mass + (tail ? t.rest : 0.0);
+    const float rest = (float)t.rest, mass = (float)(tail ? t.mass + t.rest : t.mass);
     DistillRow g;
     g.m = m;
     g.offset = log_sum * kLog2E;
-    g.a = bad ? NAN : (float)(scale * mass);
+    g.a = bad ? NAN : scale * mass;
     g.zero = empty;
     g.dense.m = g.m;
     g.dense.offset = tail ? log_rest * kLog2E : g.offset;
-    g.dense.a = bad ? NAN : (float)(scale * (tail ? mass * (double)expf(log_share) - t.rest : mass));
+    g.dense.a = bad ? NAN : scale * (tail ? fmaf(mass, expf(log_share), -rest) : mass);
     g.dense.b = 0.f;
     if (empty) g.dense = dense_zero();
     return g;
@@ -1072,10 +1086,9 @@ __device__ DistillRow distill_row(const Listed& t, float m, float log_sum, float
 // Writes a slice's listed elements over its dense gradient.  After a block barrier.
 template <typename E>
 __device__ __forceinline__ void write_listed(const List& list, int count, const Slice& slice, const DistillRow& g,
-                                             float L, E* out) {
-    const int tid = threadIdx.x;
-    if (tid >= count || !list.kept[tid]) return;
-    const int id = (int)list.ids[tid];
+                                             float L, E* out, int tid) {
+    if (tid >= count) return;
+    const int id = (int)list.ids[tid];  // (an unused slot's is negative)
     if (id < slice.begin || id >= slice.end) return;
     const float y = max_nan(fmaf(list.logit[tid] - g.m, L, -g.offset), kLowestExponent);
     out[id] = Vec<E>::store(g.zero ? 0.f : fmaf(exp2_fast(y), g.a, -list.value[tid]));
@@ -1085,167 +1098,261 @@ __device__ __forceinline__ void copy16_async(void* shared, const void* global) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
 }
 
-// Barrier of the warps behind the first.
-__device__ __forceinline__ void others_barrier() {
-    asm volatile("bar.sync 1, %0;" ::"n"(kRowThreads - 32) : "memory");
+// A row's statistics from its listed tokens' and its other tokens' sums: both shares around
+// the larger maximum, and sum - 1 apart, since ln(sum) may be all of it.
+struct RowSums {
+    float m, log_sum, log_rest;
+    bool empty;
+};
+__device__ __forceinline__ RowSums row_sums(const Listed& t, const Sums& rest, const Scale& k, bool tail) {
+    RowSums x;
+    x.m = fmaxf(rest.m, t.m);
+    const bool some = rest.S != 0.f, listed = t.inside != 0.0;
+    const float below = some ? (rest.m - x.m) * k.inverse : -INFINITY;
+    const float outside = some ? rest.S * expf(below) : 0.f;
+    const float over = t.m == x.m ? (float)(t.inside - 1.0) + outside
+                                  : (listed ? (float)t.inside * expf((t.m - x.m) * k.inverse) : 0.f) + (outside - 1.f);
+    x.empty = !some && !listed;
+    x.log_sum = x.empty ? 0.f : log1pf(over);
+    x.log_rest = tail && some ? logf(rest.S) + below : -INFINITY;
+    return x;
 }
 
-// Loss, statistics and, where wanted, the gradient.  A cluster of blocks shares a row.
-// The first block's first warp takes the list, the other warps the slices.
-// kStaged: each block holds its slice in shared memory, so the row is read once: the
-// listed tokens are struck out there (their share is summed by itself, in 64 bits), the rest
-// is summed, the blocks exchange their sums, and the gradient is formed from the same
-// copy.  Without it (no gradient, or rows too long for that) the slice streams through
-// registers, and a bitmap of marked vectors tells the sum which elements to leave out.
-template <typename E, bool kTail, bool kStaged>
-__global__ void __launch_bounds__(kRowThreads, kStaged ? 5 : 4) distill_kernel(
-    const E* logits, int vocab, size_t stride, const Scale k, double temperature, TeacherRows teacher,
+// Loss and statistics of a row; by one thread.
+__device__ __forceinline__ void write_row(const Listed& t, const RowSums& x, double inverse, bool tail, bool bad,
+                                          size_t r, float* loss, float* stats) {
+    if (loss) {
+        double value = t.mass == 0.0         ? 0.0
+                       : t.cross == INFINITY ? INFINITY
+                                             : t.cross + t.mass * (((double)x.m - (double)t.m) * inverse + x.log_sum);
+        if (tail && t.rest > 0.0 && x.log_rest - x.log_sum >= kSmallestLogShare)
+            value += t.rest * (t.log_rest - x.log_rest + x.log_sum);
+        loss[r] = bad || t.mass != t.mass || x.log_sum != x.log_sum ? NAN : (float)value;
+    }
+    if (stats) {
+        stats[3 * r] = x.m;
+        stats[3 * r + 1] = x.log_sum;
+        stats[3 * r + 2] = x.log_rest;
+    }
+}
+
+// The row's sums over its unlisted tokens from the blocks' shares, in every thread.
+__device__ __forceinline__ Sums combine_rest(const Sums* shares, int parts, float L) {
+    Sums rest = shares[0];
+    for (int i = 1; i < parts; ++i) rest.m = fmaxf(rest.m, shares[i].m);
+    rest.S = 0.f;
+    for (int i = 0; i < parts; ++i) {
+        Sums x = shares[i];
+        x.rebase(rest.m, L);
+        rest.S += x.S;
+    }
+    return rest;
+}
+
+// Loss and gradient of whole batches: clusters of blocks take row after row.  Each block
+// holds its slice of the row in shared memory, so the row is read once: the listed tokens
+// are struck out there (their share is summed by itself, in 64 bits), the rest is summed,
+// the blocks exchange their sums, and the gradient is formed from the same copy.
+// The first block's first warp works a row ahead: it reads the list, gathers its logits
+// and forms its sums (a chain of dependent loads and 64-bit functions as long as a
+// slice's work) while the other warps take the current row.  One cluster barrier per row
+// publishes both the blocks' sums and the list sent during the row before.
+constexpr int kOthers = kRowThreads - 32;  // the threads that take the slice
+__device__ __forceinline__ void others_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kOthers) : "memory"); }
+
+struct StepRow {  // what the first block sends for a row
+    List list;
+    Listed sums;
+    float scale;
+};
+
+template <typename E, bool kTail>
+__global__ void __launch_bounds__(kRowThreads, 5) distill_step_kernel(
+    const E* logits, int rows, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     constexpr int n = Vec<E>::n;
     extern __shared__ __align__(16) uint4 staged[];
+    __shared__ StepRow ready[2];
+    __shared__ Sums shares[2][kMaxCluster];
+    __shared__ Sums scratch[kOthers / 32];
+    __shared__ DistillRow grow;
+    const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
+    const int clusters = gridDim.x / parts, first = blockIdx.x / parts;
+    const int count = (int)teacher.slots;
+
+    if (tid < 32) {
+        __shared__ StepRow ahead;
+        __shared__ double work[2 * kMaxSlots];
+        auto prepare = [&](int r) {
+            const E* z = logits + (size_t)r * stride;
+            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
+            read_list(ahead.list, teacher.ids + (size_t)r * count, count, z, vocab, 0, vocab);
+            const Listed t = listed_sums<true>(ahead.list, work, teacher.logits + (size_t)r * count,
+                                               kTail ? teacher.stats + 2 * (size_t)r : nullptr, count, inverse, scale);
+            if (tid == 0) {
+                ahead.sums = t;
+                ahead.scale = (float)scale;
+            }
+            __syncwarp();
+        };
+        auto send = [&](int to_buffer) {
+            for (int to = 0; to < parts; ++to) {
+                StepRow* there = in_block(&ready[to_buffer], to);
+                for (int i = tid; i < count; i += 32) {
+                    there->list.ids[i] = ahead.list.ids[i];
+                    there->list.logit[i] = ahead.list.logit[i];
+                    there->list.value[i] = ahead.list.value[i];
+                }
+                if (tid == 0) {
+                    there->list.bad = ahead.list.bad;
+                    there->sums = ahead.sums;
+                    there->scale = ahead.scale;
+                }
+            }
+            __syncwarp();
+        };
+        cluster_arrive();  // every block of the cluster runs from here on
+        if (part == 0 && first < rows) prepare(first);
+        cluster_wait();
+        if (part == 0 && first < rows) send(0);
+        int buffer = 0;
+        for (int r = first; r < rows; r += clusters, buffer ^= 1) {
+            cluster_arrive();
+            const bool more = part == 0 && r + clusters < rows;
+            if (more) prepare(r + clusters);
+            // after this no block reads what the row before last left in the other buffer
+            cluster_wait();
+            if (more) send(buffer ^ 1);
+        }
+        return;
+    }
+
+    const int lane = tid - 32;
+    cluster_arrive();
+    cluster_wait();
+    int buffer = 0;
+    for (int r = first; r < rows; r += clusters, buffer ^= 1) {
+        const Row<E> row(logits + (size_t)r * stride, vocab);
+        const Slice slice(row, part, parts);
+        const int full = slice.hi - slice.lo;
+        const E* from = row.base + (long long)slice.lo * n;
+        for (int i = lane; i < full; i += kOthers) copy16_async(&staged[i], from + (long long)i * n);
+        const uint32_t id = lane < count ? teacher.ids[(size_t)r * count + lane] : kUnusedToken;
+        // the ragged ends follow, -inf beyond the row
+        if (slice.head && lane == 0) {
+            float v[n];
+            row.ragged(0, v);
+            staged[full] = Vec<E>::pack(v);
+        }
+        if (slice.last && lane == kOthers - 1) {
+            float v[n];
+            row.ragged(row.full1, v);
+            staged[full + 1] = Vec<E>::pack(v);
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        others_barrier();
+        if (id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end) {
+            const uint32_t at = id + row.lead;
+            const int j = (int)(at / n);
+            const int slot = j < row.full0 ? full : j >= row.full1 ? full + 1 : j - slice.lo;
+            reinterpret_cast<E*>(&staged[slot])[at % n] = Vec<E>::store(-INFINITY);
+        }
+        others_barrier();
+        Running<false> acc;
+        auto take = [&](int i) {
+            const uint4 w = staged[i];
+            float v[n];
+            Vec<E>::unpack(w, v);
+            acc.template add<n>(v, Vec<E>::top(w), i, k);
+        };
+        for (int i = lane; i < full; i += kOthers) take(i);
+        if (slice.head && lane == 0) take(full);
+        if (slice.last && lane == kOthers - 1) take(full + 1);
+        const Sums mine = warp_sums(acc.sums(), acc.m, k.L);
+        if ((lane & 31) == 0) scratch[lane >> 5] = mine;
+        others_barrier();
+        if (lane < 32) {
+            const Sums x = lane < kOthers / 32 ? scratch[lane] : Sums{-INFINITY, 0.f, 0.f};
+            const Sums sums = warp_sums(x, x.m, k.L);
+            if (lane < parts) *in_block(&shares[buffer][part], lane) = sums;
+        }
+        cluster_arrive();
+        cluster_wait();
+        const StepRow& given = ready[buffer];
+        // the coefficients by one warp, loss and statistics by another
+        if (lane == 0 || (lane == 32 && part == 0)) {
+            const RowSums x = row_sums(given.sums, combine_rest(shares[buffer], parts, k.L), k, kTail);
+            if (lane == 0)
+                grow = distill_row(given.sums, x.m, x.log_sum, x.log_rest, x.empty, given.list.bad, given.scale);
+            else
+                write_row(given.sums, x, inverse, kTail, given.list.bad, r, loss, stats);
+        }
+        E* out = gradient + (size_t)r * gradient_stride;
+        others_barrier();
+        write_dense<E, false>(row, slice, staged, out, k.L, lane, kOthers, [&]() { return grow.dense; });
+        others_barrier();
+        write_listed(given.list, count, slice, grow, k.L, out, lane);
+    }
+}
+
+// Loss and statistics of rows that stream through registers, a bitmap of marked vectors
+// telling the sum which elements to leave out; the gradient too of rows too long for
+// shared memory, which are then read twice.  A cluster of blocks shares a row.
+template <typename E, bool kTail>
+__global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(
+    const E* logits, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
+    const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     __shared__ Sums scratch[33];
     __shared__ List list;
     __shared__ double work[2 * kMaxSlots];
     __shared__ Listed listed;
     __shared__ DistillRow grow;
     __shared__ Sums shares[kMaxCluster];
-    const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x, T = blockDim.x;
+    __shared__ Marks marks;
+    const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
     if (parts > 1) cluster_arrive();  // waited for before the first store into another block
     const size_t r = blockIdx.x / parts;
     const int count = (int)teacher.slots;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    const bool lister = tid < 32;
-    const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
-    const double inverse = 1.0 / temperature;
     const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
-    Running acc;
-    if (kStaged) {
-        const int full = slice.hi - slice.lo;
-        if (lister) {
-            if (part == 0) {
-                read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
-                const Listed t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
-                if (tid == 0) listed = t;
-            }
-        } else {
-            const int lane = tid - 32, others = T - 32;
-            const E* from = row.base + (long long)slice.lo * n;
-            for (int i = lane; i < full; i += others) copy16_async(&staged[i], from + (long long)i * n);
-            const uint32_t id = lane < count ? teacher.ids[r * count + lane] : kUnusedToken;
-            // the ragged ends follow, -inf beyond the row
-            if (slice.head && lane == 0) {
-                float v[n];
-                row.ragged(0, v);
-                staged[full] = Vec<E>::pack(v);
-            }
-            if (slice.last && lane == others - 1) {
-                float v[n];
-                row.ragged(row.full1, v);
-                staged[full + 1] = Vec<E>::pack(v);
-            }
-            asm volatile("cp.async.wait_all;" ::: "memory");
-            others_barrier();
-            if (id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end) {
-                const uint32_t at = id + row.lead;
-                const int j = (int)(at / n);
-                const int slot = j < row.full0 ? full : j >= row.full1 ? full + 1 : j - slice.lo;
-                reinterpret_cast<E*>(&staged[slot])[at % n] = Vec<E>::store(-INFINITY);
-            }
-            others_barrier();
-            auto take = [&](int i) {
-                const uint4 w = staged[i];
-                float v[n];
-                Vec<E>::unpack(w, v);
-                acc.template add<n>(v, Vec<E>::top(w), i, k);
-            };
-            for (int i = lane; i < full; i += others) take(i);
-            if (slice.head && lane == 0) take(full);
-            if (slice.last && lane == others - 1) take(full + 1);
-        }
-    } else {
-        __shared__ Marks marks;
-        build_marks(marks, teacher.ids + r * count, count, row);
-        if (lister && part == 0) {
-            read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
-            const Listed t = listed_sums<true>(list, work, teacher.logits + r * count, saved, count, inverse, scale);
-            if (tid == 0) listed = t;
-        }
-        stream_slice<E, true>(row, slice, &marks, k, acc);
+    build_marks(marks, teacher.ids + r * count, count, row);
+    if (tid < 32 && (part == 0 || gradient)) {
+        read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
+        const Listed t = listed_sums<true>(list, work, teacher.logits + r * count,
+                                           kTail ? teacher.stats + 2 * r : nullptr, count, inverse, scale);
+        if (tid == 0) listed = t;
     }
+    Running<false> acc;
+    stream_slice<E, true>(row, slice, &marks, k, acc);
     Sums rest = block_sums(acc, k.L, scratch);
     if (parts > 1) {
         cluster_wait();
         if (tid < parts) *in_block(&shares[part], tid) = rest;
-        if (part == 0) {  // the list too, a block to a warp
-            for (int to = 1 + (tid >> 5); to < parts; to += T >> 5) {
-                List* there = in_block(&list, to);
-                for (int i = tid & 31; i < count; i += 32) {
-                    there->ids[i] = list.ids[i];
-                    there->kept[i] = list.kept[i];
-                    there->logit[i] = list.logit[i];
-                    there->value[i] = list.value[i];
-                }
-                if ((tid & 31) == 0) {
-                    there->bad = list.bad;
-                    *in_block(&listed, to) = listed;
-                }
-            }
-        }
         cluster_arrive();
         cluster_wait();
-        rest = shares[0];
-        for (int i = 1; i < parts; ++i) rest.m = fmaxf(rest.m, shares[i].m);
-        rest.S = 0.f;
-        for (int i = 0; i < parts; ++i) {
-            Sums x = shares[i];
-            x.rebase(rest.m, k.L);
-            rest.S += x.S;
-        }
+        rest = combine_rest(shares, parts, k.L);
     }
-    if (tid == 0) {
-        const Listed t = listed;
-        // both shares around the larger maximum; sum - 1 apart, since ln(sum) may be all of it
-        const float m = fmaxf(rest.m, t.m);
-        const float below = rest.S == 0.f ? -INFINITY : (rest.m - m) * k.inverse;
-        const double outside = rest.S == 0.f ? 0.0 : (double)rest.S * (double)expf(below);
-        const double inside = t.inside == 0.0 ? 0.0 : t.inside * (t.m == m ? 1.0 : (double)expf((t.m - m) * k.inverse));
-        const bool empty = inside + outside == 0.0;
-        const float log_sum = empty ? 0.f : log1pf((float)(inside - 1.0 + outside));
-        const float log_rest = kTail && rest.S != 0.f ? logf(rest.S) + below : -INFINITY;
-        if (gradient)
-            grow = distill_row(t, m, log_sum, log_rest, empty, list.bad, scale);
-        if (part == 0) {
-            if (loss) {
-                double value = t.mass == 0.0        ? 0.0
-                               : t.cross == INFINITY ? INFINITY
-                                                     : t.cross + t.mass * (((double)m - (double)t.m) * inverse + log_sum);
-                if (kTail && t.rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
-                    value += t.rest * (log(t.rest) - log_rest + log_sum);
-                loss[r] = list.bad || t.mass != t.mass || log_sum != log_sum ? NAN : (float)value;
-            }
-            if (stats) {
-                stats[3 * r] = m;
-                stats[3 * r + 1] = log_sum;
-                stats[3 * r + 2] = log_rest;
-            }
-        }
+    if (tid == 0 && (part == 0 || gradient)) {
+        const RowSums x = row_sums(listed, rest, k, kTail);
+        grow = distill_row(listed, x.m, x.log_sum, x.log_rest, x.empty, list.bad, (float)scale);
+        if (part == 0) write_row(listed, x, inverse, kTail, list.bad, r, loss, stats);
     }
     if (!gradient) return;
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, kStaged ? staged : nullptr, out, k.L, [&]() {
+    write_dense<E, false>(row, slice, nullptr, out, k.L, tid, kRowThreads, [&]() {
         __syncthreads();
         return grow.dense;
     });
     __syncthreads();
-    write_listed(list, count, slice, grow, k.L, out);
+    write_listed(list, count, slice, grow, k.L, out, tid);
 }
 
 // The gradient from saved statistics; `parts` blocks share a row, none waits for another.
 template <typename E, bool kTail>
 __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_gradient_kernel(
-    const E* logits, int vocab, size_t stride, const Scale k, double temperature, int parts, TeacherRows teacher,
+    const E* logits, int vocab, size_t stride, const Scale k, double inverse, int parts, TeacherRows teacher,
     const float* __restrict__ stats, const float* __restrict__ weights, E* gradient, size_t gradient_stride) {
     __shared__ List list;
     __shared__ double work[2 * kMaxSlots];
@@ -1256,22 +1363,22 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_g
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, nullptr, out, k.L, [&]() {
+    write_dense<E, false>(row, slice, nullptr, out, k.L, (int)threadIdx.x, kPieceThreads, [&]() {
         if (threadIdx.x < 32) {
-            const double inverse = 1.0 / temperature, scale = (double)weights[r] * inverse;
+            const double scale = (double)weights[r] * inverse;
             const float m = stats[3 * r], log_sum = stats[3 * r + 1], log_rest = kTail ? stats[3 * r + 2] : -INFINITY;
             // (another block may be writing over the rest of the row)
             read_list(list, teacher.ids + r * count, count, z, vocab, slice.begin, slice.end);
             const Listed t = listed_sums<false>(list, work, teacher.logits + r * count,
                                                 kTail ? teacher.stats + 2 * r : nullptr, count, inverse, scale);
             if (threadIdx.x == 0)
-                grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.f, list.bad, scale);
+                grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.f, list.bad, (float)scale);
         }
         __syncthreads();
         return grow.dense;
     });
     __syncthreads();
-    write_listed(list, count, slice, grow, k.L, out);
+    write_listed(list, count, slice, grow, k.L, out, (int)threadIdx.x);
 }
 
 template <typename F>
@@ -1313,6 +1420,43 @@ cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, i
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
+// Lowers *clusters to what the current device holds at a time: their blocks have to lie in
+// one GPC, so this is less than its SMs' room suggests.  Asked once per kernel and shape.
+template <typename... Params>
+cudaError_t resident_clusters(void (*kernel)(Params...), int parts, int threads, size_t shared, size_t* clusters) {
+    static std::mutex guard;
+    static std::map<std::tuple<const void*, int, size_t, int>, int> known;
+    int device = 0, most = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const std::lock_guard<std::mutex> lock(guard);
+    const auto key = std::make_tuple((const void*)kernel, parts, shared, device);
+    const auto found = known.find(key);
+    if (found != known.end()) {
+        most = found->second;
+    } else {
+        if (shared > (size_t)kPlainShared) {
+            e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
+            if (e != cudaSuccess) return e;
+        }
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)parts);
+        cfg.blockDim = dim3(threads);
+        cfg.dynamicSmemBytes = shared;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
+        if (e != cudaSuccess) return e;
+        if (getenv("LSX_SHOW")) fprintf(stderr, "parts %d shared %zu clusters %d\n", parts, shared, most);
+        known[key] = most;
+    }
+    if (most > 0 && *clusters > (size_t)most) *clusters = (size_t)most;
+    return cudaSuccess;
 }
 
 // Blocks that share a row in the kernels whose blocks do not wait for one another: slices
@@ -1360,19 +1504,26 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
+        const Scale k(z.temperature);
+        const double inverse = 1.0 / z.temperature;
         int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
         auto staged = [&](int p) { return ((vectors + p - 1) / p + 3) * 16; };
-        if (gradient)
+        if (gradient) {
             while (parts < kMaxCluster && staged(parts) > (size_t)kStagedTarget) parts *= 2;
-        if (gradient && staged(parts) <= (size_t)kStagedMost)
-            return launch_clusters(teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>,
-                                   z.rows, parts, kRowThreads, staged(parts), s, (const E*)z.data, (int)z.vocab,
-                                   z.stride, Scale(z.temperature), z.temperature, teacher, weights, loss, stats,
-                                   (E*)gradient, gradient_stride);
-        return launch_clusters(teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>, z.rows,
-                               parts, kRowThreads, 0, s, (const E*)z.data, (int)z.vocab, z.stride,
-                               Scale(z.temperature), z.temperature, teacher, weights, loss, stats, (E*)gradient,
-                               gradient_stride);
+            const size_t shared = staged(parts);
+            if (shared <= (size_t)kStagedMost) {
+                const auto kernel = teacher.stats ? distill_step_kernel<E, true> : distill_step_kernel<E, false>;
+                size_t clusters = z.rows;
+                const cudaError_t e = resident_clusters(kernel, parts, kRowThreads, shared, &clusters);
+                if (e != cudaSuccess) return e;
+                return launch_clusters(kernel, clusters, parts, kRowThreads, shared, s, (const E*)z.data, (int)z.rows,
+                                       (int)z.vocab, z.stride, k, inverse, teacher, weights, loss, stats, (E*)gradient,
+                                       gradient_stride);
+            }
+        }
+        return launch_clusters(teacher.stats ? distill_kernel<E, true> : distill_kernel<E, false>, z.rows, parts,
+                               kRowThreads, 0, s, (const E*)z.data, (int)z.vocab, z.stride, k, inverse, teacher, weights,
+                               loss, stats, (E*)gradient, gradient_stride);
     });
 }
 
@@ -1384,7 +1535,7 @@ cudaError_t launch_distill_gradient(cudaStream_t s, int sm_count, const LogitRow
         if (z.rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
         auto kernel = teacher.stats ? distill_gradient_kernel<E, true> : distill_gradient_kernel<E, false>;
         kernel<<<(unsigned)(z.rows * parts), kPieceThreads, 0, s>>>(
-            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), z.temperature, parts, teacher, stats,
+            (const E*)z.data, (int)z.vocab, z.stride, Scale(z.temperature), 1.0 / z.temperature, parts, teacher, stats,
             weights, (E*)gradient, gradient_stride);
         return cudaGetLastError();
     });
