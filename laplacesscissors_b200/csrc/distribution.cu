@@ -14,12 +14,7 @@
 #include <cuda_fp16.h>
 #include <math.h>
 
-#include <map>
-#include <mutex>
 #include <string>
-#include <tuple>
-#include <cstdlib>
-#include <cstdio>
 #include <type_traits>
 
 #include "device_common.cuh"
@@ -32,11 +27,7 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;     // candidate keys of one selection
-constexpr int kMarkWords = 512;    // 32-bit words of the bitmap of marked vectors
-constexpr int kStepShared = 8448;        // what the step kernel holds beside its slice, the system's share included
-constexpr int kPlainShared = 36 << 10;   // dynamic shared memory that needs no opt-in beside the kernels' own
-constexpr int kStagedTarget = 40 << 10;  // a slice kept in shared memory: 4 blocks on an SM
-constexpr int kStagedMost = 200 << 10;   // and at most
+constexpr int kAgainVectors = 10000;    // a slice that is read again for its gradient, at most
 constexpr int kPieceVectors = 2048;      // a slice of the gradient kernels
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr float kLog2E = 1.4426950408889634f;
@@ -208,57 +199,52 @@ struct Slice {
 };
 
 // ---- marked tokens -----------------------------------------------------------
-// The tokens a row lists, sorted; a bitmap over vector numbers (modulo its size) tells
-// the streaming loop which vectors to look up.  One word covers 32 consecutive vectors,
-// which is what a warp holds.
+// The tokens a row lists, and a bitmap over vector numbers (modulo its size) that tells the
+// streaming loop which vectors hold one.  One word covers 32 consecutive vectors, which is
+// what a warp holds.  Such vectors are put aside and summed without the listed elements
+// once the row has streamed.
+constexpr int kMarkWords = 512;
+constexpr int kAside = 256;
 struct Marks {
-    uint32_t raw[kMaxSlots];
-    uint32_t ids[kMaxSlots];
-    int count;
+    alignas(16) uint32_t ids[kMaxSlots];  // kUnusedToken in unused slots
     uint32_t bits[kMarkWords];
+    alignas(16) uint4 aside[kAside];
+    int aside_at[kAside];
+    short in_order[kAside];
+    int asides;
 };
-
-// Reads one row's token list and sorts it; ends with the block synchronised.
-template <typename E>
-__device__ void build_marks(Marks& M, const uint32_t* list, int slots, const Row<E>& row) {
-    const int tid = threadIdx.x;
-    for (int i = tid; i < kMarkWords; i += blockDim.x) M.bits[i] = 0;
-    if (tid == 0) M.count = 0;
-    __syncthreads();
-    for (int i = tid; i < slots; i += blockDim.x) {
-        const uint32_t id = list[i] < (uint32_t)row.vocab ? list[i] : kUnusedToken;
-        M.raw[i] = id;
-        if (id != kUnusedToken) {
-            atomicAdd(&M.count, 1);
-            const uint32_t j = (uint32_t)(((long long)id + row.lead) / Vec<E>::n);
-            atomicOr(&M.bits[(j >> 5) & (kMarkWords - 1)], 1u << (j & 31));
-        }
-    }
-    __syncthreads();
-    for (int slot = tid; slot < slots; slot += blockDim.x) {
-        const uint32_t id = M.raw[slot];
-        int rank = 0;
-        for (int j = 0; j < slots; ++j) rank += M.raw[j] < id || (M.raw[j] == id && j < slot);
-        if (id != kUnusedToken) M.ids[rank] = id;
-    }
-    __syncthreads();
-}
 
 __device__ __forceinline__ bool marked(const Marks& M, int j) {
     return (M.bits[((uint32_t)j >> 5) & (kMarkWords - 1)] >> (j & 31)) & 1u;
 }
 
-// First position of `ids` holding a token >= first.
-__device__ __forceinline__ int mark_position(const Marks& M, long long first) {
-    int lo = 0, hi = M.count;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if ((long long)M.ids[mid] < first)
-            lo = mid + 1;
-        else
-            hi = mid;
+// Sets the listed elements of vector j to -inf.
+template <typename E>
+__device__ __forceinline__ void strike(const Marks& M, int count, const Row<E>& row, int j, float* v) {
+    const uint32_t first = (uint32_t)row.first(j);
+#pragma unroll 4
+    for (int i = 0; i < count; i += 4) {
+        const uint4 ids = *reinterpret_cast<const uint4*>(&M.ids[i]);
+        const uint32_t at[4] = {ids.x - first, ids.y - first, ids.z - first, ids.w - first};
+        // (an unused slot, -1, can only fall before a row's first element)
+        if (min(min(at[0], at[1]), min(at[2], at[3])) >= (uint32_t)Vec<E>::n) continue;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+#pragma unroll
+            for (int e = 0; e < Vec<E>::n; ++e) v[e] = at[q] == (uint32_t)e ? -INFINITY : v[e];
     }
-    return lo;
+}
+
+// Whether an earlier slot names this slot's token; `ids` 16-byte aligned, kMaxSlots of them.
+__device__ __forceinline__ bool named_before(const uint32_t* ids, int slot) {
+    const uint32_t id = ids[slot];
+    bool seen = false;
+#pragma unroll 4
+    for (int j = 0; j < slot; j += 4) {
+        const uint4 o = *reinterpret_cast<const uint4*>(&ids[j]);
+        seen |= o.x == id | (o.y == id & j + 1 < slot) | (o.z == id & j + 2 < slot) | (o.w == id & j + 3 < slot);
+    }
+    return seen;
 }
 
 // ---- running sums of a softmax ---------------------------------------------------
@@ -344,42 +330,45 @@ __device__ __forceinline__ Sums block_sums(const Running<kRanked>& a, float L, S
     return warp_sums(x, x.m, L);
 }
 
-template <typename E, bool kExclude, bool kRanked>
-__device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& part, const Marks* M, const Scale& k,
-                                             Running<kRanked>& acc) {
+// `begun` is called once, when the first loads are on their way.
+template <typename E, bool kExclude, bool kRanked, typename F>
+__device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& part, Marks* M, int count, const Scale& k,
+                                             Running<kRanked>& acc, F&& begun) {
     constexpr int n = Vec<E>::n;
-    auto exclude = [&](int j, float* v) {
-        int pos = mark_position(*M, row.first(j));
-#pragma unroll
-        for (int e = 0; e < n; ++e)
-            while (pos < M->count && (long long)M->ids[pos] == row.first(j) + e) {
-                v[e] = -INFINITY;
-                ++pos;
-            }
-    };
-    auto take = [&](int j, uint4 w) {
-        float v[n];
-        Vec<E>::unpack(w, v);
-        float top = Vec<E>::top(w);
-        if (kExclude && marked(*M, j)) {
-            exclude(j, v);
-            top = v[0];
-#pragma unroll
-            for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
-        }
-        acc.template add<n>(v, top, j, k);
-    };
-    auto take_ragged = [&](int j) {
-        float v[n];
-        row.ragged(j, v);
-        if (kExclude) exclude(j, v);
+    auto add = [&](const float* v, int j) {
         float top = v[0];
 #pragma unroll
         for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
         acc.template add<n>(v, top, j, k);
     };
+    auto take = [&](int j, uint4 w) {
+        float v[n];
+        if (kExclude && marked(*M, j)) {
+            const int slot = atomicAdd(&M->asides, 1);
+            if (slot < kAside) {
+                M->aside[slot] = w;
+                M->aside_at[slot] = j;
+            }
+            return;
+        }
+        Vec<E>::unpack(w, v);
+        acc.template add<n>(v, Vec<E>::top(w), j, k);
+    };
+    auto take_ragged = [&](int j) {
+        float v[n];
+        row.ragged(j, v);
+        if (kExclude) strike(*M, count, row, j, v);
+        add(v, j);
+    };
     const int tid = threadIdx.x, T = blockDim.x;
     int j = part.lo + tid;
+    uint4 w[kUnroll];
+    bool whole = j + (kUnroll - 1) * T < part.hi;
+    if (whole) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
+    }
+    begun();
     // every thread meets its vectors in ascending order
     if (part.head && tid == 0) {
         acc.at = 0;
@@ -389,15 +378,50 @@ __device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& par
     } else if (part.last && tid == T - 1) {
         acc.at = row.full1;
     }
-    for (; j + (kUnroll - 1) * T < part.hi; j += kUnroll * T) {
-        uint4 w[kUnroll];
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
+    while (whole) {
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) take(j + u * T, w[u]);
+        j += kUnroll * T;
+        whole = j + (kUnroll - 1) * T < part.hi;
+        if (whole) {
+#pragma unroll
+            for (int u = 0; u < kUnroll; ++u) w[u] = row.full(j + u * T);
+        }
     }
     for (; j < part.hi; j += T) take(j, row.full(j));
     if (part.last && tid == T - 1) take_ragged(row.full1);
+}
+
+// The vectors put aside, without their listed elements: thread t takes the one of t-th
+// lowest number, whatever order they came in, so that sums repeat.  Where there are more
+// than were kept (bitmap words shared by many vectors of a long row) every thread reads its
+// own again.  After a block barrier.
+template <typename E>
+__device__ void add_asides(Marks& M, int count, const Row<E>& row, const Slice& part, const Scale& k,
+                           Running<false>& acc) {
+    constexpr int n = Vec<E>::n;
+    const int tid = threadIdx.x, T = blockDim.x, asides = M.asides;
+    auto take = [&](int j, uint4 w) {
+        float v[n];
+        Vec<E>::unpack(w, v);
+        strike(M, count, row, j, v);
+        float top = v[0];
+#pragma unroll
+        for (int e = 1; e < n; ++e) top = fmaxf(top, v[e]);
+        acc.template add<n>(v, top, 0, k);
+    };
+    if (asides > kAside) {
+        for (int j = part.lo + tid; j < part.hi; j += T)
+            if (marked(M, j)) take(j, row.full(j));
+        return;
+    }
+    for (int i = tid; i < asides; i += T) {
+        int rank = 0;
+        for (int o = 0; o < asides; ++o) rank += M.aside_at[o] < M.aside_at[i];
+        M.in_order[rank] = (short)i;
+    }
+    __syncthreads();
+    for (int i = tid; i < asides; i += T) take(M.aside_at[M.in_order[i]], M.aside[M.in_order[i]]);
 }
 
 // Where one token holds nearly all the mass, 1 + rest in f32 keeps little of the rest, and
@@ -729,7 +753,7 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
     Running<true> acc;
-    stream_slice<E, false>(row, slice, nullptr, k, acc);
+    stream_slice<E, false>(row, slice, nullptr, 0, k, acc, []() {});
     Partial sums = slice_sums(row, slice, acc, k, scratch, &owner);
     // clusters keep the upper half of the list for the blocks' best keys
     const int cap = parts > 1 ? kListCap / 2 : kListCap;
@@ -774,52 +798,6 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     }
 }
 
-// ---- lists of tokens -------------------------------------------------------------------------
-// One row's listed tokens.
-struct List {
-    uint32_t ids[kMaxSlots];  // kUnusedToken but in the first slot that names a token
-    float logit[kMaxSlots];   // the row's logit of that token, else -inf
-    float value[kMaxSlots];   // what the operator keeps with the slot
-    int bad;                 // some slot names a token outside the vocabulary
-};
-
-// Reads a row's list and the logits it names in [begin, end), by the first warp (slot
-// lane + 32 q).
-template <typename E>
-__device__ void read_list(List& list, const uint32_t* ids, int count, const E* z, int vocab, int begin, int end) {
-    constexpr int kPer = kMaxSlots / 32;
-    const int lane = threadIdx.x & 31;
-    uint32_t id[kPer];
-    bool bad = false;
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        const int i = lane + 32 * q;
-        id[q] = i < count ? ids[i] : kUnusedToken;
-    }
-#pragma unroll
-    for (int q = 0; q < kPer; ++q) {
-        if (32 * q >= count) break;
-        const int i = lane + 32 * q;
-        const bool used = id[q] < (uint32_t)vocab;
-        const float logit = used && (int)id[q] >= begin && (int)id[q] < end ? Vec<E>::one(z[id[q]]) : -INFINITY;
-        bad |= !used && id[q] != kUnusedToken;
-        // the same token in an earlier slot: of these 32, or of the 32s before
-        bool again = (__match_any_sync(0xffffffffu, id[q]) & ((1u << lane) - 1)) != 0;
-#pragma unroll
-        for (int p = 0; p < q; ++p)
-#pragma unroll 8
-            for (int from = 0; from < 32; ++from) again |= __shfl_sync(0xffffffffu, id[p], from) == id[q];
-        if (i < count) {
-            list.ids[i] = used && !again ? id[q] : kUnusedToken;
-            list.logit[i] = used && !again ? logit : -INFINITY;
-            list.value[i] = 0.f;
-        }
-    }
-    const bool any = __any_sync(0xffffffffu, bad);
-    if (lane == 0) list.bad = any;
-    __syncwarp();
-}
-
 // ---- gradients ---------------------------------------------------------------------------
 // What the unlisted elements of a row's gradient need: with y = (z - m) L - offset an
 // element gets 2^y (a + b y).  Listed ones are written over them afterwards.
@@ -847,15 +825,15 @@ __device__ __forceinline__ void dense_vector(float* v, const Dense& d, float L) 
 }
 
 __device__ __forceinline__ void store16(void* p, uint4 w) {
-    asm volatile("st.global.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
 }
 
-// The dense gradient of a slice into `out` (the row's first element): vectors from
-// `staged` (slot j - lo) or, where it is null, from the row itself, by T threads.  `out` may
-// be the row.  `ready` gives the coefficients, once, after the first loads are on their way.
+// The dense gradient of a slice into `out` (the row's first element) by T threads.  `out`
+// may be the row.  `ready` gives the coefficients, once, after the first loads are on their
+// way.
 template <typename E, bool kLinear, typename F>
-__device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part, const uint4* staged, E* out, float L,
-                                            int tid, int T, F&& ready) {
+__device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part, E* out, float L, int tid, int T,
+                                            F&& ready) {
     constexpr int n = Vec<E>::n;
     // the output row may lie at another alignment than the logits
     const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (uintptr_t)(row.lead * sizeof(E));
@@ -883,25 +861,20 @@ __device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part
         }
     };
     int j = part.lo + tid;
-    if (staged) {
-        d = ready();
-        for (; j < part.hi; j += T) put(j, staged[j - part.lo]);
-    } else {
-        uint4 w[kUnroll];
-        auto fetch = [&](int from) {
+    uint4 w[kUnroll];
+    auto fetch = [&](int from) {
 #pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (from + u * T < part.hi) w[u] = row.full(from + u * T);
-        };
+        for (int u = 0; u < kUnroll; ++u)
+            if (from + u * T < part.hi) w[u] = row.full(from + u * T);
+    };
+    fetch(j);
+    d = ready();
+    while (j < part.hi) {
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u)
+            if (j + u * T < part.hi) put(j + u * T, w[u]);
+        j += kUnroll * T;
         fetch(j);
-        d = ready();
-        while (j < part.hi) {
-#pragma unroll
-            for (int u = 0; u < kUnroll; ++u)
-                if (j + u * T < part.hi) put(j + u * T, w[u]);
-            j += kUnroll * T;
-            fetch(j);
-        }
     }
     if (part.head && tid == 0) put_ragged(0);
     if (part.last && tid == T - 1) put_ragged(row.full1);
@@ -952,9 +925,9 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
     };
     E* out = gradient + r * gradient_stride;
     if (h != 0.f)
-        write_dense<E, true>(row, slice, nullptr, out, k.L, tid, kPieceThreads, ready);
+        write_dense<E, true>(row, slice, out, k.L, tid, kPieceThreads, ready);
     else
-        write_dense<E, false>(row, slice, nullptr, out, k.L, tid, kPieceThreads, ready);
+        write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, ready);
     __syncthreads();
     if (id >= (uint32_t)vocab || (int)id < slice.begin || (int)id >= slice.end) return;
     // a token named several times adds up at its first slot
@@ -971,16 +944,9 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
 }
 
 // ---- distillation --------------------------------------------------------------------------
-// The listed tokens' side of one row in 64 bits, by one warp: sums over at most kMaxSlots
-// numbers, of which 1 - sum p is next to 0 for a confident teacher.
-struct Listed {
-    double mass;   // sum of p
-    double rest;   // the teacher's mass outside the list (0 without its statistics)
-    double log_rest;
-    float m;       // the largest listed logit of the student
-    double inside; // sum exp((z - m) / T) over the listed tokens
-    double cross;  // sum p (ln p - (z - m) / T)
-};
+// The listed tokens' side of a row is summed in 64 bits, a slot to a thread: at most
+// kMaxSlots numbers, of which 1 - sum p is next to 0 for a confident teacher.
+constexpr int kListWarps = kMaxSlots / 32;
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
 #pragma unroll
@@ -994,321 +960,73 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// By the warp that read the list.  Also leaves scale * p in list.value.
-template <bool kStudent>
-__device__ Listed listed_sums(List& list, double* work, const float* values, const float* stats, int count,
-                              double inverse, double scale) {
-    const int lane = threadIdx.x & 31;
-    Listed t{0.0, 0.0, 0.0, -INFINITY, 0.0, 0.0};
-    float top = -INFINITY;
-    for (int i = lane; i < count; i += 32) {
-        const float value = list.ids[i] != kUnusedToken ? values[i] : -INFINITY;
-        list.value[i] = value;
-        top = fmaxf(top, value);
-        if (kStudent) t.m = fmaxf(t.m, list.logit[i]);
-    }
-    if (kStudent) t.m = warp_max(t.m);
-    double shift, norm = 0.0;
-    bool none = false;  // the teacher's row holds no token: it asks for nothing
-    if (stats) {
-        none = stats[0] == -INFINITY && stats[1] == 0.f;
-        shift = none ? 0.0 : (double)stats[0];
-        norm = (double)stats[1];
-    } else {
-        top = warp_max(top);
-        shift = top == -INFINITY ? 0.0 : (double)top;
-    }
-    for (int i = lane; i < count; i += 32) {
-        const double log_p = ((double)list.value[i] - shift) * inverse - norm, p = exp(log_p);
-        t.mass += p;
-        if (kStudent) {
-            const float z = list.logit[i];
-            const double log_q = z == -INFINITY ? -INFINITY : ((double)z - (double)t.m) * inverse;
-            t.inside += exp(log_q);
-            work[i] = p != 0.0 ? log_p - log_q : 0.0;
-        }
-        work[kMaxSlots + i] = p;
-    }
-    t.mass = warp_sum_f64(t.mass);
-    if (kStudent) t.inside = warp_sum_f64(t.inside);
-    double share = 1.0;
-    norm = 0.0;
-    if (stats) {
-        if (!none) t.rest = t.mass < 1.0 ? 1.0 - t.mass : (t.mass >= 1.0 ? 0.0 : t.mass);
-        t.log_rest = log(t.rest);
-    } else if (t.mass != 0.0) {  // normalised over the list
-        share = 1.0 / t.mass;
-        norm = log(t.mass);
-        t.mass = t.mass == t.mass ? 1.0 : t.mass;
-    }
-    for (int i = lane; i < count; i += 32) {
-        const double p = work[kMaxSlots + i] * share;
-        list.value[i] = (float)(scale * p);
-        if (kStudent && p != 0.0) t.cross += p * (work[i] - norm);
-    }
-    if (kStudent) t.cross = warp_sum_f64(t.cross);
-    __syncwarp();
-    return t;
+// ln p of a slot up to the list's normalisation: against the teacher's statistics where
+// they are given, else against `top`, the list's largest logit.  -inf for an unused slot and
+// for a teacher's row without tokens, which asks for nothing.
+__device__ __forceinline__ double teacher_log(float value, const float* saved, float top, double inverse) {
+    if (value == -INFINITY) return -INFINITY;
+    if (!saved) return ((double)value - (double)top) * inverse;
+    return saved[0] == -INFINITY && saved[1] == 0.f ? -INFINITY
+                                                    : ((double)value - (double)saved[0]) * inverse - (double)saved[1];
+}
+
+// The teacher's mass outside its list, from the list's (0 without statistics).
+__device__ __forceinline__ double teacher_rest(double mass, const float* saved) {
+    if (!saved || (saved[0] == -INFINITY && saved[1] == 0.f)) return 0.0;
+    return mass < 1.0 ? 1.0 - mass : (mass >= 1.0 ? 0.0 : mass);
 }
 
 // The tokens outside the list are one outcome only where the student's share of them is
 // a normal f32 number (2^-126 and up).
 constexpr float kSmallestLogShare = -87.33654475f;
 
-// What the gradient of one row needs beside its list: listed elements get q a - value, q
-// against `offset`.
+// What a row's gradient needs beside its list: listed elements get q a - value, q against
+// `offset`; the others are exponentiated against their own sum: 2^y = q_i / q_r stays in
+// range and (P q_r - p_r) is the whole coefficient, however small q_r is.
 struct DistillRow {
     Dense dense;
     float m, offset, a;
-    bool zero;
+    bool empty;
 };
-
-// The tokens outside the list are exponentiated against their own sum: 2^y = q_i / q_r
-// stays in range and (P q_r - p_r) is the whole coefficient, however small q_r is.
-__device__ __forceinline__ DistillRow distill_row(const Listed& t, float m, float log_sum, float log_rest, bool empty,
-                                                  bool bad, float scale) {
+__device__ __forceinline__ DistillRow distill_row(float m, float log_sum, float log_rest, float mass, float rest,
+                                                  bool empty, bool bad, float scale) {
     const float log_share = log_rest - log_sum;
     const bool tail = log_share >= kSmallestLogShare;
-    const float rest = (float)t.rest, mass = (float)(tail ? t.mass + t.rest : t.mass);
+    if (tail) mass = (float)((double)mass + (double)rest);
+    if (bad) mass = NAN;
     DistillRow g;
     g.m = m;
     g.offset = log_sum * kLog2E;
-    g.a = bad ? NAN : scale * mass;
-    g.zero = empty;
-    g.dense.m = g.m;
-    g.dense.offset = tail ? log_rest * kLog2E : g.offset;
-    g.dense.a = bad ? NAN : scale * (tail ? fmaf(mass, expf(log_share), -rest) : mass);
-    g.dense.b = 0.f;
-    if (empty) g.dense = dense_zero();
+    g.a = scale * mass;
+    g.empty = empty;
+    g.dense = dense_zero();
+    if (!empty) {
+        g.dense.m = m;
+        g.dense.offset = tail ? log_rest * kLog2E : g.offset;
+        g.dense.a = scale * (tail ? fmaf(mass, expf(log_share), -rest) : mass);
+    }
     return g;
 }
-
-// Writes a slice's listed elements over its dense gradient.  After a block barrier.
-template <typename E>
-__device__ __forceinline__ void write_listed(const List& list, int count, const Slice& slice, const DistillRow& g,
-                                             float L, E* out, int tid) {
-    if (tid >= count) return;
-    const int id = (int)list.ids[tid];  // (an unused slot's is negative)
-    if (id < slice.begin || id >= slice.end) return;
-    const float y = max_nan(fmaf(list.logit[tid] - g.m, L, -g.offset), kLowestExponent);
-    out[id] = Vec<E>::store(g.zero ? 0.f : fmaf(exp2_fast(y), g.a, -list.value[tid]));
+// The gradient at a listed token with the student's logit and the teacher's w p / T.
+__device__ __forceinline__ float listed_gradient(const DistillRow& g, float logit, float value, float L) {
+    const float y = max_nan(fmaf(logit - g.m, L, -g.offset), kLowestExponent);
+    return g.empty ? 0.f : fmaf(exp2_fast(y), g.a, -value);
 }
 
-__device__ __forceinline__ void copy16_async(void* shared, const void* global) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(shared)), "l"(global) : "memory");
-}
-
-// A row's statistics from its listed tokens' and its other tokens' sums: both shares around
-// the larger maximum, and sum - 1 apart, since ln(sum) may be all of it.
-struct RowSums {
-    float m, log_sum, log_rest;
-    bool empty;
-};
-__device__ __forceinline__ RowSums row_sums(const Listed& t, const Sums& rest, const Scale& k, bool tail) {
-    RowSums x;
-    x.m = fmaxf(rest.m, t.m);
-    const bool some = rest.S != 0.f, listed = t.inside != 0.0;
-    const float below = some ? (rest.m - x.m) * k.inverse : -INFINITY;
-    const float outside = some ? rest.S * expf(below) : 0.f;
-    const float over = t.m == x.m ? (float)(t.inside - 1.0) + outside
-                                  : (listed ? (float)t.inside * expf((t.m - x.m) * k.inverse) : 0.f) + (outside - 1.f);
-    x.empty = !some && !listed;
-    x.log_sum = x.empty ? 0.f : log1pf(over);
-    x.log_rest = tail && some ? logf(rest.S) + below : -INFINITY;
-    return x;
-}
-
-// Loss and statistics of a row; by one thread.
-__device__ __forceinline__ void write_row(const Listed& t, const RowSums& x, double inverse, bool tail, bool bad,
-                                          size_t r, float* loss, float* stats) {
-    if (loss) {
-        double value = t.mass == 0.0         ? 0.0
-                       : t.cross == INFINITY ? INFINITY
-                                             : t.cross + t.mass * (((double)x.m - (double)t.m) * inverse + x.log_sum);
-        if (tail && t.rest > 0.0 && x.log_rest - x.log_sum >= kSmallestLogShare)
-            value += t.rest * (t.log_rest - x.log_rest + x.log_sum);
-        loss[r] = bad || t.mass != t.mass || x.log_sum != x.log_sum ? NAN : (float)value;
-    }
-    if (stats) {
-        stats[3 * r] = x.m;
-        stats[3 * r + 1] = x.log_sum;
-        stats[3 * r + 2] = x.log_rest;
-    }
-}
-
-// The row's sums over its unlisted tokens from the blocks' shares, in every thread.
-__device__ __forceinline__ Sums combine_rest(const Sums* shares, int parts, float L) {
-    Sums rest = shares[0];
-    for (int i = 1; i < parts; ++i) rest.m = fmaxf(rest.m, shares[i].m);
-    rest.S = 0.f;
-    for (int i = 0; i < parts; ++i) {
-        Sums x = shares[i];
-        x.rebase(rest.m, L);
-        rest.S += x.S;
-    }
-    return rest;
-}
-
-// Loss and gradient of whole batches: clusters of blocks take row after row.  Each block
-// holds its slice of the row in shared memory, so the row is read once: the listed tokens
-// are struck out there (their share is summed by itself, in 64 bits), the rest is summed,
-// the blocks exchange their sums, and the gradient is formed from the same copy.
-// The first block's first warp works a row ahead: it reads the list, gathers its logits
-// and forms its sums (a chain of dependent loads and 64-bit functions as long as a
-// slice's work) while the other warps take the current row.  One cluster barrier per row
-// publishes both the blocks' sums and the list sent during the row before.
-constexpr int kOthers = kRowThreads - 32;  // the threads that take the slice
-__device__ __forceinline__ void others_barrier() { asm volatile("bar.sync 1, %0;" ::"n"(kOthers) : "memory"); }
-
-struct StepRow {  // what the first block sends for a row
-    List list;
-    Listed sums;
-    float scale;
-};
-
-template <typename E, bool kTail>
-__global__ void __launch_bounds__(kRowThreads, 5) distill_step_kernel(
-    const E* logits, int rows, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
-    const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
-    constexpr int n = Vec<E>::n;
-    extern __shared__ __align__(16) uint4 staged[];
-    __shared__ StepRow ready[2];
-    __shared__ Sums shares[2][kMaxCluster];
-    __shared__ Sums scratch[kOthers / 32];
-    __shared__ DistillRow grow;
-    const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
-    const int clusters = gridDim.x / parts, first = blockIdx.x / parts;
-    const int count = (int)teacher.slots;
-
-    if (tid < 32) {
-        __shared__ StepRow ahead;
-        __shared__ double work[2 * kMaxSlots];
-        auto prepare = [&](int r) {
-            const E* z = logits + (size_t)r * stride;
-            const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
-            read_list(ahead.list, teacher.ids + (size_t)r * count, count, z, vocab, 0, vocab);
-            const Listed t = listed_sums<true>(ahead.list, work, teacher.logits + (size_t)r * count,
-                                               kTail ? teacher.stats + 2 * (size_t)r : nullptr, count, inverse, scale);
-            if (tid == 0) {
-                ahead.sums = t;
-                ahead.scale = (float)scale;
-            }
-            __syncwarp();
-        };
-        auto send = [&](int to_buffer) {
-            for (int to = 0; to < parts; ++to) {
-                StepRow* there = in_block(&ready[to_buffer], to);
-                for (int i = tid; i < count; i += 32) {
-                    there->list.ids[i] = ahead.list.ids[i];
-                    there->list.logit[i] = ahead.list.logit[i];
-                    there->list.value[i] = ahead.list.value[i];
-                }
-                if (tid == 0) {
-                    there->list.bad = ahead.list.bad;
-                    there->sums = ahead.sums;
-                    there->scale = ahead.scale;
-                }
-            }
-            __syncwarp();
-        };
-        cluster_arrive();  // every block of the cluster runs from here on
-        if (part == 0 && first < rows) prepare(first);
-        cluster_wait();
-        if (part == 0 && first < rows) send(0);
-        int buffer = 0;
-        for (int r = first; r < rows; r += clusters, buffer ^= 1) {
-            cluster_arrive();
-            const bool more = part == 0 && r + clusters < rows;
-            if (more) prepare(r + clusters);
-            // after this no block reads what the row before last left in the other buffer
-            cluster_wait();
-            if (more) send(buffer ^ 1);
-        }
-        return;
-    }
-
-    const int lane = tid - 32;
-    cluster_arrive();
-    cluster_wait();
-    int buffer = 0;
-    for (int r = first; r < rows; r += clusters, buffer ^= 1) {
-        const Row<E> row(logits + (size_t)r * stride, vocab);
-        const Slice slice(row, part, parts);
-        const int full = slice.hi - slice.lo;
-        const E* from = row.base + (long long)slice.lo * n;
-        for (int i = lane; i < full; i += kOthers) copy16_async(&staged[i], from + (long long)i * n);
-        const uint32_t id = lane < count ? teacher.ids[(size_t)r * count + lane] : kUnusedToken;
-        // the ragged ends follow, -inf beyond the row
-        if (slice.head && lane == 0) {
-            float v[n];
-            row.ragged(0, v);
-            staged[full] = Vec<E>::pack(v);
-        }
-        if (slice.last && lane == kOthers - 1) {
-            float v[n];
-            row.ragged(row.full1, v);
-            staged[full + 1] = Vec<E>::pack(v);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        others_barrier();
-        if (id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end) {
-            const uint32_t at = id + row.lead;
-            const int j = (int)(at / n);
-            const int slot = j < row.full0 ? full : j >= row.full1 ? full + 1 : j - slice.lo;
-            reinterpret_cast<E*>(&staged[slot])[at % n] = Vec<E>::store(-INFINITY);
-        }
-        others_barrier();
-        Running<false> acc;
-        auto take = [&](int i) {
-            const uint4 w = staged[i];
-            float v[n];
-            Vec<E>::unpack(w, v);
-            acc.template add<n>(v, Vec<E>::top(w), i, k);
-        };
-        for (int i = lane; i < full; i += kOthers) take(i);
-        if (slice.head && lane == 0) take(full);
-        if (slice.last && lane == kOthers - 1) take(full + 1);
-        const Sums mine = warp_sums(acc.sums(), acc.m, k.L);
-        if ((lane & 31) == 0) scratch[lane >> 5] = mine;
-        others_barrier();
-        if (lane < 32) {
-            const Sums x = lane < kOthers / 32 ? scratch[lane] : Sums{-INFINITY, 0.f, 0.f};
-            const Sums sums = warp_sums(x, x.m, k.L);
-            if (lane < parts) *in_block(&shares[buffer][part], lane) = sums;
-        }
-        cluster_arrive();
-        cluster_wait();
-        const StepRow& given = ready[buffer];
-        // the coefficients by one warp, loss and statistics by another
-        if (lane == 0 || (lane == 32 && part == 0)) {
-            const RowSums x = row_sums(given.sums, combine_rest(shares[buffer], parts, k.L), k, kTail);
-            if (lane == 0)
-                grow = distill_row(given.sums, x.m, x.log_sum, x.log_rest, x.empty, given.list.bad, given.scale);
-            else
-                write_row(given.sums, x, inverse, kTail, given.list.bad, r, loss, stats);
-        }
-        E* out = gradient + (size_t)r * gradient_stride;
-        others_barrier();
-        write_dense<E, false>(row, slice, staged, out, k.L, lane, kOthers, [&]() { return grow.dense; });
-        others_barrier();
-        write_listed(given.list, count, slice, grow, k.L, out, lane);
-    }
-}
-
-// Loss and statistics of rows that stream through registers, a bitmap of marked vectors
-// telling the sum which elements to leave out; the gradient too of rows too long for
-// shared memory, which are then read twice.  A cluster of blocks shares a row.
-template <typename E, bool kTail>
-__global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(
+// Loss and statistics of rows that stream through registers, without their listed
+// elements, which have their own sums; with kGradient the row is then read again, from L2,
+// for its gradient.  A cluster of blocks shares a row: they exchange their sums (with
+// kGradient each takes the list for itself, else the first one).
+template <typename E, bool kTail, bool kGradient>
+__global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     __shared__ Sums scratch[33];
-    __shared__ List list;
-    __shared__ double work[2 * kMaxSlots];
-    __shared__ Listed listed;
-    __shared__ DistillRow grow;
     __shared__ Sums shares[kMaxCluster];
     __shared__ Marks marks;
+    __shared__ float tops[kListWarps], highs[kListWarps];
+    __shared__ double masses[kListWarps], insides[kListWarps], crosses[kListWarps];
+    __shared__ int bad;
     const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
     if (parts > 1) cluster_arrive();  // waited for before the first store into another block
     const size_t r = blockIdx.x / parts;
@@ -1316,69 +1034,220 @@ __global__ void __launch_bounds__(kRowThreads, 4) distill_kernel(
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    const double scale = (weights ? (double)weights[r] : 1.0) * inverse;
-    build_marks(marks, teacher.ids + r * count, count, row);
-    if (tid < 32 && (part == 0 || gradient)) {
-        read_list(list, teacher.ids + r * count, count, z, vocab, 0, vocab);
-        const Listed t = listed_sums<true>(list, work, teacher.logits + r * count,
-                                           kTail ? teacher.stats + 2 * r : nullptr, count, inverse, scale);
-        if (tid == 0) listed = t;
+    const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
+    const bool lists = kGradient || part == 0;
+    uint32_t id = kUnusedToken;
+    float value = -INFINITY, logit = -INFINITY;
+    if (tid < count) {
+        id = teacher.ids[r * count + tid];
+        if (lists) value = teacher.logits[r * count + tid];
     }
+    bool kept = false;
     Running<false> acc;
-    stream_slice<E, true>(row, slice, &marks, k, acc);
+    stream_slice<E, true>(row, slice, &marks, count, k, acc, [&]() {
+        for (int i = tid; i < kMarkWords; i += kRowThreads) marks.bits[i] = 0;
+        if (tid == 0) marks.asides = bad = 0;
+        if (tid < kMaxSlots) marks.ids[tid] = id < (uint32_t)vocab ? id : kUnusedToken;
+        __syncthreads();
+        if (id != kUnusedToken && id >= (uint32_t)vocab) bad = 1;
+        kept = id < (uint32_t)vocab && !named_before(marks.ids, tid);
+        if (kept) {
+            const uint32_t j = (id + (uint32_t)row.lead) / Vec<E>::n;
+            atomicOr(&marks.bits[(j >> 5) & (kMarkWords - 1)], 1u << (j & 31));
+            if (lists) logit = Vec<E>::one(z[id]);
+        } else {
+            value = -INFINITY;
+        }
+        __syncthreads();
+    });
+    if (lists && tid < kMaxSlots) {
+        const float top = warp_max(value), high = warp_max(logit);
+        if ((tid & 31) == 0) {
+            tops[tid >> 5] = top;
+            highs[tid >> 5] = high;
+        }
+    }
+    __syncthreads();
+    add_asides(marks, count, row, slice, k, acc);
+    float top = -INFINITY, high = -INFINITY;
+    double p = 0.0;
+    if (lists) {
+#pragma unroll
+        for (int w = 0; w < kListWarps; ++w) {
+            top = fmaxf(top, tops[w]);
+            high = fmaxf(high, highs[w]);
+        }
+        if (tid < kMaxSlots) {
+            const double log_p = teacher_log(value, saved, top, inverse);
+            p = log_p == -INFINITY ? 0.0 : exp(log_p);
+            const double log_q = logit == -INFINITY ? -INFINITY : ((double)logit - (double)high) * inverse;
+            const double mass = warp_sum_f64(p);
+            const double inside = warp_sum_f64(log_q == -INFINITY ? 0.0 : exp(log_q));
+            const double cross = part == 0 ? warp_sum_f64(p != 0.0 ? p * (log_p - log_q) : 0.0) : 0.0;
+            if ((tid & 31) == 0) {
+                masses[tid >> 5] = mass;
+                insides[tid >> 5] = inside;
+                crosses[tid >> 5] = cross;
+            }
+        }
+    }
     Sums rest = block_sums(acc, k.L, scratch);
     if (parts > 1) {
         cluster_wait();
-        if (tid < parts) *in_block(&shares[part], tid) = rest;
+        if (tid < (kGradient ? parts : 1)) *in_block(&shares[part], tid) = rest;
         cluster_arrive();
-        cluster_wait();
-        rest = combine_rest(shares, parts, k.L);
     }
-    if (tid == 0 && (part == 0 || gradient)) {
-        const RowSums x = row_sums(listed, rest, k, kTail);
-        grow = distill_row(listed, x.m, x.log_sum, x.log_rest, x.empty, list.bad, (float)scale);
-        if (part == 0) write_row(listed, x, inverse, kTail, list.bad, r, loss, stats);
+    // the row from its blocks' sums and its list's, in every thread that asks
+    double mass = 0.0, p_rest = 0.0;
+    float m = 0.f, log_sum = 0.f, log_rest = -INFINITY;
+    bool empty = false;
+    auto put_together = [&]() {
+        if (parts > 1) {
+            rest = shares[0];
+            for (int i = 1; i < parts; ++i) rest.m = fmaxf(rest.m, shares[i].m);
+            rest.S = 0.f;
+            for (int i = 0; i < parts; ++i) {
+                Sums x = shares[i];
+                x.rebase(rest.m, k.L);
+                rest.S += x.S;
+            }
+        }
+        double inside = 0.0;
+#pragma unroll
+        for (int w = 0; w < kListWarps; ++w) {
+            mass += masses[w];
+            inside += insides[w];
+        }
+        p_rest = teacher_rest(mass, saved);
+        // both shares around the larger maximum; sum - 1 apart, since ln(sum) may be all of it
+        m = fmaxf(rest.m, high);
+        const bool some = rest.S != 0.f, listed = inside != 0.0;
+        empty = !some && !listed;
+        const float below = some ? (rest.m - m) * k.inverse : -INFINITY;
+        const float outside = some ? rest.S * expf(below) : 0.f;
+        const float over = high == m ? (float)(inside - 1.0) + outside
+                                     : (listed ? (float)inside * expf((high - m) * k.inverse) : 0.f) + (outside - 1.f);
+        log_sum = empty ? 0.f : log1pf(over);
+        if (kTail && some) log_rest = logf(rest.S) + below;
+    };
+    auto write_row = [&]() {
+        double x = mass, cross = 0.0;
+        for (int w = 0; w < kListWarps; ++w) cross += crosses[w];
+        if (!kTail && x != 0.0) {  // normalised over the list
+            cross = cross / x - log(x);
+            x = x == x ? 1.0 : x;
+        }
+        if (loss) {
+            double value = x == 0.0            ? 0.0
+                           : cross == INFINITY ? INFINITY
+                                               : cross + x * (((double)m - (double)high) * inverse + log_sum);
+            if (kTail && p_rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
+                value += p_rest * (log(p_rest) - log_rest + log_sum);
+            loss[r] = bad || x != x || log_sum != log_sum ? NAN : (float)value;
+        }
+        if (stats) {
+            stats[3 * r] = m;
+            stats[3 * r + 1] = log_sum;
+            stats[3 * r + 2] = log_rest;
+        }
+    };
+    if (!kGradient) {
+        if (parts > 1) cluster_wait();
+        if (part != 0 || tid != 0) return;
+        put_together();
+        write_row();
+        return;
     }
-    if (!gradient) return;
+    const double weight = weights ? (double)weights[r] * inverse : inverse;
+    DistillRow g;
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, nullptr, out, k.L, tid, kRowThreads, [&]() {
-        __syncthreads();
-        return grow.dense;
+    write_dense<E, false>(row, slice, out, k.L, tid, kRowThreads, [&]() {
+        if (parts > 1) cluster_wait();
+        put_together();
+        const float P = kTail ? (float)mass : mass == 0.0 ? 0.f : mass == mass ? 1.f : NAN;
+        g = distill_row(m, log_sum, log_rest, P, (float)p_rest, empty, bad, (float)weight);
+        return g.dense;
     });
     __syncthreads();
-    write_listed(list, count, slice, grow, k.L, out, tid);
+    if (kept && (int)id >= slice.begin && (int)id < slice.end) {
+        const double share = kTail || mass == 0.0 ? weight : weight / mass;
+        out[id] = Vec<E>::store(listed_gradient(g, logit, (float)(share * p), k.L));
+    }
+    if (part == 0 && tid == 0) write_row();
 }
 
 // The gradient from saved statistics; `parts` blocks share a row, none waits for another.
+// Without the teacher's statistics P is 1 and the unlisted elements do not wait for the
+// list's sums.
 template <typename E, bool kTail>
 __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_gradient_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double inverse, int parts, TeacherRows teacher,
     const float* __restrict__ stats, const float* __restrict__ weights, E* gradient, size_t gradient_stride) {
-    __shared__ List list;
-    __shared__ double work[2 * kMaxSlots];
-    __shared__ DistillRow grow;
+    static_assert(kPieceThreads == kMaxSlots, "a slot to a thread");
+    __shared__ __align__(16) uint32_t ids[kMaxSlots];
+    __shared__ double sums[kListWarps];
+    __shared__ float tops[kListWarps];
     const size_t r = blockIdx.x / parts;
-    const int part = (int)(blockIdx.x - r * parts), count = (int)teacher.slots;
+    const int part = (int)(blockIdx.x - r * parts), count = (int)teacher.slots, tid = threadIdx.x;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
-    E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, nullptr, out, k.L, (int)threadIdx.x, kPieceThreads, [&]() {
-        if (threadIdx.x < 32) {
-            const double scale = (double)weights[r] * inverse;
-            const float m = stats[3 * r], log_sum = stats[3 * r + 1], log_rest = kTail ? stats[3 * r + 2] : -INFINITY;
-            // (another block may be writing over the rest of the row)
-            read_list(list, teacher.ids + r * count, count, z, vocab, slice.begin, slice.end);
-            const Listed t = listed_sums<false>(list, work, teacher.logits + r * count,
-                                                kTail ? teacher.stats + 2 * r : nullptr, count, inverse, scale);
-            if (threadIdx.x == 0)
-                grow = distill_row(t, m, log_sum, log_rest, m == -INFINITY && log_sum == 0.f, list.bad, (float)scale);
-        }
+    const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
+    const float weight = weights[r], scale = weight * k.inverse;
+    // a slot to a thread; the listed logits are read before anything is written
+    uint32_t id = kUnusedToken;
+    float value = -INFINITY, logit = -INFINITY;
+    if (tid < count) {
+        id = teacher.ids[r * count + tid];
+        value = teacher.logits[r * count + tid];
+    }
+    const bool here = id < (uint32_t)vocab && (int)id >= slice.begin && (int)id < slice.end;
+    if (here) logit = Vec<E>::one(z[id]);
+    double p = 0.0;
+    bool kept = false;
+    DistillRow g;
+    auto list_mass = [&]() {  // in every thread
+        const double part_sum = warp_sum_f64(p);
+        if ((tid & 31) == 0) sums[tid >> 5] = part_sum;
         __syncthreads();
-        return grow.dense;
+        double all = 0.0;
+#pragma unroll
+        for (int w = 0; w < kListWarps; ++w) all += sums[w];
+        return all;
+    };
+    E* out = gradient + r * gradient_stride;
+    write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, [&]() {
+        ids[tid] = id < (uint32_t)vocab ? id : kUnusedToken;
+        const bool bad = __syncthreads_or(id != kUnusedToken && id >= (uint32_t)vocab) != 0;
+        kept = id < (uint32_t)vocab && !named_before(ids, tid);
+        if (!kept) value = -INFINITY;
+        float top = 0.f, mass, rest = 0.f;
+        if (!kTail) {
+            top = warp_max(value != value ? INFINITY : value);
+            if ((tid & 31) == 0) tops[tid >> 5] = top;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < kListWarps; ++w) top = fmaxf(top, tops[w]);
+            mass = top == -INFINITY ? 0.f : top == INFINITY ? NAN : 1.f;
+        }
+        const double log_p = teacher_log(value, saved, top, inverse);
+        p = log_p == -INFINITY ? 0.0 : exp(log_p);
+        if (kTail) {
+            const double all = list_mass();
+            rest = (float)teacher_rest(all, saved);
+            mass = (float)all;
+        }
+        const float m = stats[3 * r], log_sum = stats[3 * r + 1], log_rest = kTail ? stats[3 * r + 2] : -INFINITY;
+        g = distill_row(m, log_sum, log_rest, mass, rest, m == -INFINITY && log_sum == 0.f, bad, scale);
+        return g.dense;
     });
+    double share = (double)weight * inverse;
+    if (!kTail) {
+        const double all = list_mass();
+        if (all != 0.0) share /= all;
+    }
     __syncthreads();
-    write_listed(list, count, slice, grow, k.L, out, (int)threadIdx.x);
+    if (kept && here) out[id] = Vec<E>::store(listed_gradient(g, logit, (float)(share * p), k.L));
 }
 
 template <typename F>
@@ -1402,17 +1271,12 @@ int row_parts(int sm_count, size_t rows, size_t vectors, int threads, int reside
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, size_t shared,
-                            cudaStream_t s, Args... args) {
-    if (shared > (size_t)kPlainShared) {
-        const cudaError_t e =
-            cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-        if (e != cudaSuccess) return e;
-    }
+cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, cudaStream_t s,
+                            Args... args) {
+    if (rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * parts));
     cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = shared;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1420,43 +1284,6 @@ cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, i
     cfg.attrs = attr;
     cfg.numAttrs = parts > 1 ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
-// Lowers *clusters to what the current device holds at a time: their blocks have to lie in
-// one GPC, so this is less than its SMs' room suggests.  Asked once per kernel and shape.
-template <typename... Params>
-cudaError_t resident_clusters(void (*kernel)(Params...), int parts, int threads, size_t shared, size_t* clusters) {
-    static std::mutex guard;
-    static std::map<std::tuple<const void*, int, size_t, int>, int> known;
-    int device = 0, most = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return e;
-    const std::lock_guard<std::mutex> lock(guard);
-    const auto key = std::make_tuple((const void*)kernel, parts, shared, device);
-    const auto found = known.find(key);
-    if (found != known.end()) {
-        most = found->second;
-    } else {
-        if (shared > (size_t)kPlainShared) {
-            e = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)shared);
-            if (e != cudaSuccess) return e;
-        }
-        cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = dim3((unsigned)parts);
-        cfg.blockDim = dim3(threads);
-        cfg.dynamicSmemBytes = shared;
-        cudaLaunchAttribute attr[1];
-        attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim = {(unsigned)parts, 1, 1};
-        cfg.attrs = attr;
-        cfg.numAttrs = 1;
-        e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
-        if (e != cudaSuccess) return e;
-        if (getenv("LSX_SHOW")) fprintf(stderr, "parts %d shared %zu clusters %d\n", parts, shared, most);
-        known[key] = most;
-    }
-    if (most > 0 && *clusters > (size_t)most) *clusters = (size_t)most;
-    return cudaSuccess;
 }
 
 // Blocks that share a row in the kernels whose blocks do not wait for one another: slices
@@ -1476,10 +1303,10 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         const size_t vectors = z.vocab / Vec<E>::n;
         const Scale k(z.temperature);
         if (vectors < 1024)
-            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, 0, s, (const E*)z.data, (int)z.vocab,
+            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
         return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, row_parts(sm_count, z.rows, vectors, 256, 4), 256,
-                               0, s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
+                               s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
                                (int)alternatives, out);
     });
 }
@@ -1504,26 +1331,14 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
-        const Scale k(z.temperature);
-        const double inverse = 1.0 / z.temperature;
         int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
-        auto staged = [&](int p) { return ((vectors + p - 1) / p + 3) * 16; };
-        if (gradient) {
-            while (parts < kMaxCluster && staged(parts) > (size_t)kStagedTarget) parts *= 2;
-            const size_t shared = staged(parts);
-            if (shared <= (size_t)kStagedMost) {
-                const auto kernel = teacher.stats ? distill_step_kernel<E, true> : distill_step_kernel<E, false>;
-                size_t clusters = z.rows;
-                const cudaError_t e = resident_clusters(kernel, parts, kRowThreads, shared, &clusters);
-                if (e != cudaSuccess) return e;
-                return launch_clusters(kernel, clusters, parts, kRowThreads, shared, s, (const E*)z.data, (int)z.rows,
-                                       (int)z.vocab, z.stride, k, inverse, teacher, weights, loss, stats, (E*)gradient,
-                                       gradient_stride);
-            }
-        }
-        return launch_clusters(teacher.stats ? distill_kernel<E, true> : distill_kernel<E, false>, z.rows, parts,
-                               kRowThreads, 0, s, (const E*)z.data, (int)z.vocab, z.stride, k, inverse, teacher, weights,
-                               loss, stats, (E*)gradient, gradient_stride);
+        if (gradient)  // the rows in flight have to stay in L2 until they are read again
+            while (parts < kMaxCluster && vectors / parts > (size_t)kAgainVectors) parts *= 2;
+        auto kernel = gradient ? (teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>)
+                               : (teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>);
+        return launch_clusters(kernel, z.rows, parts, kRowThreads, s, (const E*)z.data, (int)z.vocab, z.stride,
+                               Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats, (E*)gradient,
+                               gradient_stride);
     });
 }
 
