@@ -235,6 +235,26 @@ int lsx_model_score_batch(lsx_model* model, const uint32_t* prompts, size_t case
                           const uint32_t* targets, size_t count, const lsx_rotation* rotation, double* nll_out,
                           uint32_t* argmax_out, double* margin_out, float* logits_out);
 
+/* lsx_model_score_batch's forward with the distribution at each scored position
+   (cases x count rows, host arrays, each may be NULL) in place of its scores, without
+   downloading vocabulary-wide logits: the target's log probability, the entropy, the
+   statistics and the `alternatives` largest logits, as lsx_token_logprobs_device
+   defines them, at `temperature`. */
+int lsx_model_distribution_batch(lsx_model* model, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                                 const uint32_t* targets, size_t count, const lsx_rotation* rotation,
+                                 double temperature, size_t alternatives, float* logprob_out, float* entropy_out,
+                                 float* stats_out, uint32_t* top_ids_out, float* top_logits_out,
+                                 float* top_logprobs_out);
+/* How far the distribution at each scored position is from a teacher's listed tokens
+   (host arrays [cases x count x teacher_count], teacher_stats [cases x count x 2] or
+   NULL, as lsx_model_distribution_batch leaves them): lsx_distill_device's loss.  With
+   the unedited model as teacher and `rotation` as student it measures what an edit of
+   the readout changes. */
+int lsx_model_divergence_batch(lsx_model* model, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                               const uint32_t* targets, size_t count, const lsx_rotation* rotation,
+                               double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
+                               size_t teacher_count, const float* teacher_stats, float* divergence_out);
+
 /* ------------------------------------------------------ readout validation -- */
 /* Fused readout margin over many hidden states (verify_cached's target rows,
    src/diagnosis.rs:512-537 with minimum_margin src/diagnosis.rs:490-492 and argmax

@@ -7,12 +7,12 @@ has a Python or CPU substitute.
 from . import _lib
 from ._lib import LsxError, library_path
 from .gpu import AttentionConfig, Gpu, NormConfig, RopeConfig, Tensor
-from .model import DeviceRotation, Frame, Model
+from .model import DeviceRotation, Frame, Model, ScoredDistribution
 from .rotation import ReadoutRotation, SubspaceRotation, random_subspace_rotation
 
 __version__ = "0.1.0"
 
 __all__ = [
-    "Gpu", "Tensor", "NormConfig", "RopeConfig", "AttentionConfig", "Model", "DeviceRotation", "Frame",
+    "Gpu", "Tensor", "NormConfig", "RopeConfig", "AttentionConfig", "Model", "DeviceRotation", "Frame", "ScoredDistribution",
     "ReadoutRotation", "SubspaceRotation", "random_subspace_rotation", "LsxError", "library_path",
 ]

@@ -100,6 +100,8 @@ SIGNATURES = {
     "lsx_model_score": (I, [P, UP, SZ, UP, SZ, P, DP, UP, FP, FP]),
     "lsx_model_generate_batch": (I, [P, UP, SZ, SZ, SZ, UP]),
     "lsx_model_score_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, DP, UP, DP, FP]),
+    "lsx_model_distribution_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, D, SZ, FP, FP, FP, UP, FP, FP]),
+    "lsx_model_divergence_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, D, UP, FP, SZ, FP, FP]),
     "lsx_readout_margin": (I, [P, P, P, SZ, SZ, P, I, SZ, UP, P, DP, UP, FP]),
     "lsx_readout_margin_device": (I, [P, P, P, SZ, SZ, P, I, SZ, P, P, P, P, P, P, SZ]),
     "lsx_readout_workspace_bytes": (SZ, [SZ, SZ, SZ, P]),

@@ -34,6 +34,7 @@
 #include <vector>
 
 #include "batched.cuh"
+#include "distribution.cuh"
 #include "device_common.cuh"
 
 namespace lsx {
@@ -1436,6 +1437,53 @@ int BatchedScorer::score(const uint32_t* tokens, size_t cases, size_t T, size_t 
     return run(tokens, cases, T, first, count, targets, rotation, out, false);
 }
 
+// The distributions of `rows` rows of logits on the device, their results to the host.
+int BatchedScorer::distributions(const float* logits, const uint32_t* targets, size_t rows, const Distribution& d) {
+    cudaStream_t s = ctx_->stream;
+    const size_t V = config_.vocab, k = d.alternatives, t = d.teacher_count;
+    auto up = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t lists = up(rows * std::max<size_t>(std::max(k, t), 1) * 4), pairs = up(rows * 8), ones = up(rows * 4);
+    void* block = nullptr;
+    LSX_TRY(device_alloc(ctx_, 3 * lists + pairs + 2 * ones, &block));
+    uint8_t* at = (uint8_t*)block;
+    uint32_t* ids = (uint32_t*)at;
+    float* values = (float*)(at + lists);
+    float* logprobs = (float*)(at + 2 * lists);
+    float* stats = (float*)(at + 3 * lists);
+    float* first = (float*)(at + 3 * lists + pairs);
+    float* second = (float*)(at + 3 * lists + pairs + ones);
+    const LogitRows z{logits, LSX_F32, rows, V, V, d.temperature};
+    cudaError_t e = cudaSuccess;
+    auto copy = [&](void* to, const void* from, size_t bytes, cudaMemcpyKind kind) {
+        if (e == cudaSuccess && to && from) e = cudaMemcpyAsync(to, from, bytes, kind, s);
+    };
+    if (d.divergence) {
+        copy(ids, d.teacher_ids, rows * t * 4, cudaMemcpyHostToDevice);
+        copy(values, d.teacher_logits, rows * t * 4, cudaMemcpyHostToDevice);
+        copy(stats, d.teacher_stats, rows * 8, cudaMemcpyHostToDevice);
+        const TeacherRows teacher{ids, values, d.teacher_stats ? stats : nullptr, t};
+        if (e == cudaSuccess)
+            e = launch_distill(s, ctx_->sm_count, z, teacher, nullptr, first, nullptr, nullptr, 0);
+        copy(d.divergence, first, rows * 4, cudaMemcpyDeviceToHost);
+    } else {
+        const LogprobOutputs out{first, second, stats, k ? ids : nullptr, k ? values : nullptr, k ? logprobs : nullptr};
+        e = launch_token_logprobs(s, ctx_->sm_count, z, targets, 1, k, out);
+        copy(d.logprob, first, rows * 4, cudaMemcpyDeviceToHost);
+        copy(d.entropy, second, rows * 4, cudaMemcpyDeviceToHost);
+        copy(d.stats, stats, rows * 8, cudaMemcpyDeviceToHost);
+        if (k) {
+            copy(d.top_ids, ids, rows * k * 4, cudaMemcpyDeviceToHost);
+            copy(d.top_logits, values, rows * k * 4, cudaMemcpyDeviceToHost);
+            copy(d.top_logprobs, logprobs, rows * k * 4, cudaMemcpyDeviceToHost);
+        }
+    }
+    const cudaError_t done = cudaStreamSynchronize(s);
+    device_release(ctx_, block);
+    if (e == cudaSuccess) e = done;
+    if (e != cudaSuccess) return fail(LSX_E_CUDA, cuda_message("distributions", e));
+    return LSX_OK;
+}
+
 int BatchedScorer::run(const uint32_t* tokens, size_t cases, size_t T, size_t first, size_t count,
                        const uint32_t* targets, const lsx_rotation* rotation, const Outputs& out, bool write_cache) {
     const FusedConfig& c = config_;
@@ -1573,8 +1621,11 @@ int BatchedScorer::run(const uint32_t* tokens, size_t cases, size_t T, size_t fi
     }
     LSX_CUDA(cudaGetLastError(), "final norm");
     LSX_TRY(gemm_planes_enqueue(ctx_, hi, lo, (int)scored, H, c.head, V, c.head_bias, logits, V, false, status));
-    row_scores_kernel<<<(int)scored, 1024, 0, s>>>(logits, V, d_targets, d_nll, d_argmax, d_margin);
-    LSX_CUDA(cudaGetLastError(), "scores");
+    if (out.nll || out.argmax || out.margin) {
+        row_scores_kernel<<<(int)scored, 1024, 0, s>>>(logits, V, d_targets, d_nll, d_argmax, d_margin);
+        LSX_CUDA(cudaGetLastError(), "scores");
+    }
+    if (out.distribution) LSX_TRY(distributions(logits, d_targets, scored, *out.distribution));
     if (out.nll) LSX_CUDA(cudaMemcpyAsync(out.nll, d_nll, scored * 8, cudaMemcpyDeviceToHost, s), "nll download");
     if (out.argmax)
         LSX_CUDA(cudaMemcpyAsync(out.argmax, d_argmax, scored * 4, cudaMemcpyDeviceToHost, s), "argmax download");

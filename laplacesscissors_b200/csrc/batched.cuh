@@ -12,6 +12,24 @@ namespace lsx {
 
 class BatchedScorer {
 public:
+    // What the scored rows' distributions are asked for (host arrays, rows = cases x count):
+    // log probabilities of the targets with entropy and alternatives, or the divergence
+    // from a teacher's listed tokens.
+    struct Distribution {
+        double temperature = 1.0;
+        size_t alternatives = 0;
+        float* logprob = nullptr;       // [rows]
+        float* entropy = nullptr;       // [rows]
+        float* stats = nullptr;         // [rows, 2]
+        uint32_t* top_ids = nullptr;    // [rows, alternatives] each
+        float* top_logits = nullptr;
+        float* top_logprobs = nullptr;
+        size_t teacher_count = 0;
+        const uint32_t* teacher_ids = nullptr;  // [rows, teacher_count] each
+        const float* teacher_logits = nullptr;
+        const float* teacher_stats = nullptr;   // [rows, 2] or NULL
+        float* divergence = nullptr;            // [rows]
+    };
     // Host destinations of the scores, [cases, count] each ([cases, count, vocab]
     // for logits); any may be NULL.
     struct Outputs {
@@ -19,6 +37,7 @@ public:
         uint32_t* argmax = nullptr;
         double* margin = nullptr;
         float* logits = nullptr;
+        const Distribution* distribution = nullptr;
     };
     ~BatchedScorer();
     static bool eligible(const FusedConfig& c, std::string* why);
@@ -42,6 +61,7 @@ private:
         size_t x, work, planes, logits, rope, tokens, targets, rows, nll, argmax, margin, status, total;
     };
     int reserve(size_t rows, size_t scored, size_t T);
+    int distributions(const float* logits, const uint32_t* targets, size_t rows, const Distribution& d);
     int run(const uint32_t* tokens, size_t cases, size_t T, size_t first, size_t count, const uint32_t* targets,
             const lsx_rotation* rotation, const Outputs& out, bool write_cache);
     // Per-sequence KV caches of generate_batch: per layer keys [batch, cap, kvheads *

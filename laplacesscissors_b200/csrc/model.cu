@@ -23,6 +23,7 @@
 #include <vector>
 
 #include "batched.cuh"
+#include "distribution.cuh"
 #include "decode.cuh"
 #include "persistent.cuh"
 #include "device_common.cuh"
@@ -1568,9 +1569,9 @@ int lsx_model_generate_batch(lsx_model* m, const uint32_t* prompts, size_t batch
     return m->batched->generate_batch(prompts, batch, prompt_length, maximum, tokens_out);
 }
 
-int lsx_model_score_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,
-                          const uint32_t* targets, size_t count, const lsx_rotation* rotation, double* nll_out,
-                          uint32_t* argmax_out, double* margin_out, float* logits_out) {
+static int score_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                       const uint32_t* targets, size_t count, const lsx_rotation* rotation,
+                       const BatchedScorer::Outputs& out) {
     LSX_ENSURE(m && prompts && targets, "invalid argument");
     LSX_ENSURE(cases > 0 && prompt_length > 0 && count > 0, "give at least one case, prompt token and target");
     LSX_ENSURE(prompt_length + count - 1 <= m->capacity, "give a context that fits the prompt and the continuation");
@@ -1586,12 +1587,65 @@ int lsx_model_score_batch(lsx_model* m, const uint32_t* prompts, size_t cases, s
         memcpy(fed.data() + c * T, prompts + c * prompt_length, prompt_length * 4);
         if (count > 1) memcpy(fed.data() + c * T + prompt_length, targets + c * count, (count - 1) * 4);
     }
+    return m->batched->score(fed.data(), cases, T, prompt_length - 1, count, targets, rotation, out);
+}
+
+int lsx_model_score_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                          const uint32_t* targets, size_t count, const lsx_rotation* rotation, double* nll_out,
+                          uint32_t* argmax_out, double* margin_out, float* logits_out) {
     BatchedScorer::Outputs out;
     out.nll = nll_out;
     out.argmax = argmax_out;
     out.margin = margin_out;
     out.logits = logits_out;
-    return m->batched->score(fed.data(), cases, T, prompt_length - 1, count, targets, rotation, out);
+    return score_batch(m, prompts, cases, prompt_length, targets, count, rotation, out);
+}
+
+// The same forward with the scored rows' distributions instead of scores.
+int lsx_model_distribution_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                                 const uint32_t* targets, size_t count, const lsx_rotation* rotation,
+                                 double temperature, size_t alternatives, float* logprob_out, float* entropy_out,
+                                 float* stats_out, uint32_t* top_ids_out, float* top_logits_out,
+                                 float* top_logprobs_out) {
+    LSX_ENSURE(m, "invalid argument");
+    LSX_ENSURE(temperature >= 1e-6 && temperature <= 1e6, "the temperature must be in 1e-6..=1e6");
+    LSX_ENSURE(alternatives <= (size_t)kMaxSlots && alternatives <= m->graph.vocab,
+               "the alternatives are at most 128 and at most the vocabulary");
+    LSX_ENSURE(alternatives > 0 || (!top_ids_out && !top_logits_out && !top_logprobs_out),
+               "alternatives need a count");
+    BatchedScorer::Distribution d;
+    d.temperature = temperature;
+    d.alternatives = alternatives;
+    d.logprob = logprob_out;
+    d.entropy = entropy_out;
+    d.stats = stats_out;
+    d.top_ids = top_ids_out;
+    d.top_logits = top_logits_out;
+    d.top_logprobs = top_logprobs_out;
+    BatchedScorer::Outputs out;
+    out.distribution = &d;
+    return score_batch(m, prompts, cases, prompt_length, targets, count, rotation, out);
+}
+
+int lsx_model_divergence_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,
+                               const uint32_t* targets, size_t count, const lsx_rotation* rotation,
+                               double temperature, const uint32_t* teacher_ids, const float* teacher_logits,
+                               size_t teacher_count, const float* teacher_stats, float* divergence_out) {
+    LSX_ENSURE(m && teacher_ids && teacher_logits && divergence_out, "invalid argument");
+    LSX_ENSURE(temperature >= 1e-6 && temperature <= 1e6, "the temperature must be in 1e-6..=1e6");
+    LSX_ENSURE(teacher_count > 0 && teacher_count <= (size_t)kMaxSlots, "the teacher lists 1..=128 tokens a row");
+    for (size_t i = 0; i < cases * count * teacher_count; ++i)
+        LSX_ENSURE(teacher_ids[i] < m->graph.vocab || teacher_ids[i] == kUnusedToken, "check the teacher's token range");
+    BatchedScorer::Distribution d;
+    d.temperature = temperature;
+    d.teacher_count = teacher_count;
+    d.teacher_ids = teacher_ids;
+    d.teacher_logits = teacher_logits;
+    d.teacher_stats = teacher_stats;
+    d.divergence = divergence_out;
+    BatchedScorer::Outputs out;
+    out.distribution = &d;
+    return score_batch(m, prompts, cases, prompt_length, targets, count, rotation, out);
 }
 
 }  // extern "C"

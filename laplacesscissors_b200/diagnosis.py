@@ -272,7 +272,7 @@ class CompactReadout:
 
 __all__ = [
     "argmax", "other", "minimum_margin", "prefill", "generate_frames", "generate", "Generation", "ObservedPath",
-    "Verification", "verify_cached", "CompactReadout", "readout_margin", "Deadline", "BudgetExpired",
+    "Verification", "verify_cached", "CompactReadout", "readout_margin", "Deadline", "BudgetExpired", "readout_divergence",
 ]
 
 
@@ -327,3 +327,21 @@ def evaluate_cases(model: Model, cases, rotation: DeviceRotation | None = None,
         records.append(ScoredCase(i, [int(x) for x in prompt], targets, case_before, case_after, path_before,
                                   path_after))
     return Evaluation(before, after, correct_before, correct_after, records)
+
+
+def readout_divergence(model: Model, prompts, targets, rotation: DeviceRotation, alternatives: int = 20,
+                       temperature: float = 1.0, deadline: Deadline | None = None):
+    """How far the edited readout's distributions are from the model's own at the scored
+    positions of equal-shape cases (prompts [cases, P], targets [cases, n]): the unedited
+    pass gives each position's top `alternatives` and statistics, the edited one its
+    divergence from them, the other tokens counted as one outcome.  verify_cached compares
+    logits one prefix at a time; this compares probabilities for many at once.  Returns
+    (divergence f32 [cases, n], the unedited ScoredDistribution)."""
+    if deadline is not None:
+        deadline.check()
+    before = model.score_distribution(prompts, targets, alternatives=alternatives, temperature=temperature)
+    if deadline is not None:
+        deadline.check()
+    divergence = model.score_divergence(prompts, targets, before.top_ids, before.top_logits, before.stats, rotation,
+                                        temperature)
+    return divergence, before

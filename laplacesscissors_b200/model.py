@@ -23,6 +23,17 @@ class Frame:  # src/model.rs:365-369
     logits: np.ndarray
 
 
+@dataclass
+class ScoredDistribution:
+    """Distributions at teacher-forced positions [cases, n] (Model.score_distribution)."""
+    logprob: np.ndarray       # f32 [cases, n]: ln q of the target
+    entropy: np.ndarray       # f32 [cases, n]
+    stats: np.ndarray         # f32 [cases, n, 2]: largest logit m, ln sum exp((z - m) / T)
+    top_ids: np.ndarray       # u32 [cases, n, k], logits descending, the lower id first among equals
+    top_logits: np.ndarray    # f32 [cases, n, k]
+    top_logprobs: np.ndarray  # f32 [cases, n, k]
+
+
 class DeviceRotation:
     """An edit uploaded for the readout (src/model.rs:285-364)."""
 
@@ -277,5 +288,52 @@ class Model:
                                         _up(amax), _dp(margin), _fp(lg) if logits else None))
         return nll, amax, margin, lg
 
+    def _cases(self, prompts, targets):
+        p = np.ascontiguousarray(prompts, dtype=np.uint32)
+        t = np.ascontiguousarray(targets, dtype=np.uint32)
+        if p.ndim != 2 or t.ndim != 2 or p.shape[0] != t.shape[0]:
+            raise ValueError("prompts and targets are [cases, length] arrays with one row per case")
+        return p, t
 
-__all__ = ["Model", "DeviceRotation", "Frame"]
+    def score_distribution(self, prompts, targets, rotation: DeviceRotation | None = None, alternatives: int = 0,
+                           temperature: float = 1.0) -> ScoredDistribution:
+        """score_batch's forward with each scored position's distribution: the target's log
+        probability, the entropy, the statistics and the top alternatives
+        (lsx_model_distribution_batch), optionally through the edited readout."""
+        p, t = self._cases(prompts, targets)
+        cases, n = t.shape
+        k = int(alternatives)
+        if k < 0:
+            raise ValueError("the alternatives are a count")
+        logprob, entropy = np.empty((cases, n), np.float32), np.empty((cases, n), np.float32)
+        stats = np.empty((cases, n, 2), np.float32)
+        ids = np.empty((cases, n, k), np.uint32)
+        values, logprobs = np.empty((cases, n, k), np.float32), np.empty((cases, n, k), np.float32)
+        check(lib.lsx_model_distribution_batch(self._h, _up(p), cases, p.shape[1], _up(t), n, _rot(rotation),
+                                               float(temperature), k, _fp(logprob), _fp(entropy), _fp(stats),
+                                               _up(ids) if k else None, _fp(values) if k else None,
+                                               _fp(logprobs) if k else None))
+        return ScoredDistribution(logprob, entropy, stats, ids, values, logprobs)
+
+    def score_divergence(self, prompts, targets, teacher_ids, teacher_logits, teacher_stats=None,
+                         rotation: DeviceRotation | None = None, temperature: float = 1.0) -> np.ndarray:
+        """Divergence f32 [cases, n] of each scored position from a teacher's listed tokens
+        [cases, n, k] (lsx_model_divergence_batch); with teacher_stats [cases, n, 2] the
+        tokens outside the list count as one outcome."""
+        p, t = self._cases(prompts, targets)
+        cases, n = t.shape
+        ids = np.ascontiguousarray(teacher_ids, dtype=np.uint32)
+        values = np.ascontiguousarray(teacher_logits, dtype=np.float32)
+        if ids.ndim != 3 or ids.shape[:2] != (cases, n) or values.shape != ids.shape:
+            raise ValueError("the teacher's ids and logits are [cases, n, k] arrays")
+        stats = None if teacher_stats is None else np.ascontiguousarray(teacher_stats, dtype=np.float32)
+        if stats is not None and stats.shape != (cases, n, 2):
+            raise ValueError("the teacher's statistics are a [cases, n, 2] array")
+        out = np.empty((cases, n), np.float32)
+        check(lib.lsx_model_divergence_batch(self._h, _up(p), cases, p.shape[1], _up(t), n, _rot(rotation),
+                                             float(temperature), _up(ids), _fp(values), ids.shape[2],
+                                             _fp(stats) if stats is not None else None, _fp(out)))
+        return out
+
+
+__all__ = ["Model", "DeviceRotation", "Frame", "ScoredDistribution"]
