@@ -166,16 +166,18 @@ struct Row {
         base = row - lead;
         head = lead != 0;
         full0 = head ? 1 : 0;
-        const int end = (int)(((long long)lead + vocab) / n);
-        last = ((long long)lead + vocab) % n != 0 && end >= full0;
+        const uint32_t reach = (uint32_t)lead + (uint32_t)vocab;
+        const int end = (int)(reach / n);
+        last = reach % n != 0 && end >= full0;
         full1 = end > full0 ? end : full0;
     }
-    __device__ __forceinline__ long long first(int j) const { return (long long)j * Vec<E>::n - lead; }
+    // the element that vector j starts with (rows have at most 2^30)
+    __device__ __forceinline__ int first(int j) const { return j * Vec<E>::n - lead; }
     __device__ __forceinline__ uint4 full(int j) const { return load16(base + (long long)j * Vec<E>::n); }
     __device__ __forceinline__ void ragged(int j, float* v) const {
 #pragma unroll
         for (int e = 0; e < Vec<E>::n; ++e) {
-            const long long i = first(j) + e;
+            const int i = first(j) + e;
             v[e] = i >= 0 && i < vocab ? Vec<E>::one(base[(long long)j * Vec<E>::n + e]) : -INFINITY;
         }
     }
@@ -188,13 +190,13 @@ struct Slice {
     bool head, last;
     template <typename E>
     __device__ __forceinline__ Slice(const Row<E>& row, int part, int parts) {
-        const long long full = row.full1 - row.full0;
-        lo = row.full0 + (int)(full * part / parts);
-        hi = row.full0 + (int)(full * (part + 1) / parts);
+        const uint32_t full = (uint32_t)(row.full1 - row.full0), step = (full + (uint32_t)parts - 1) / (uint32_t)parts;
+        lo = row.full0 + (int)min((uint32_t)part * step, full);
+        hi = row.full0 + (int)min((uint32_t)(part + 1) * step, full);
         head = row.head && part == 0;
         last = row.last && part == parts - 1;
-        begin = part == 0 ? 0 : (int)row.first(lo);
-        end = part == parts - 1 ? row.vocab : (int)row.first(hi);
+        begin = part == 0 ? 0 : row.first(lo);
+        end = part == parts - 1 ? row.vocab : row.first(hi);
     }
 };
 
@@ -446,8 +448,8 @@ __device__ Sums sum_without_maximum(const Row<E>& row, const Slice& part, int ow
     };
     const int lane = threadIdx.x & 31, T = blockDim.x;
     float v[n];
-    for (long long j = (long long)part.lo + owner + (long long)lane * T; j < part.hi; j += 32ll * T) {
-        Vec<E>::unpack(row.full((int)j), v);
+    for (int j = part.lo + owner + lane * T; j < part.hi; j += 32 * T) {
+        Vec<E>::unpack(row.full(j), v);
         take(v);
     }
     if (lane == 0 && part.head && owner == 0) {
@@ -681,40 +683,43 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
     const unsigned long long mine =
         acc.at < 0 ? 0ull : ((unsigned long long)total_order_key(acc.m + 0.f) << 32) | (0xffffffffu - (uint32_t)acc.at);
     const unsigned long long bound = group_bound(P, mine, top);
-    auto offer = [&](int j, const float* v) {
-        const uint32_t low = 0xffffffffu - (uint32_t)j;
+    const uint32_t level = (uint32_t)(bound >> 32);
+    const int bound_at = (int)(0xffffffffu - (uint32_t)bound);  // (with a bound)
+    // the bound's logit; without a bound everything passes
+    const float level_logit = bound ? total_order_value(level) : -INFINITY;
+    auto offer_vector = [&](int j) {
+        float v[n];
+        if (j >= row.full0 && j < row.full1) {
+            const uint4 w = row.full(j);
+            if (Vec<E>::top(w) < level_logit) return;
+            Vec<E>::unpack(w, v);
+        } else {
+            row.ragged(j, v);
+        }
 #pragma unroll
         for (int e = 0; e < n; ++e) {
-            const long long i = row.first(j) + e;
-            const unsigned long long key = ((unsigned long long)total_order_key(v[e] + 0.f) << 32) | low;
-            if (key >= bound && i >= 0 && i < row.vocab) {
+            if (v[e] < level_logit) continue;
+            const int i = row.first(j) + e;
+            const bool tie = bound && total_order_key(v[e] + 0.f) == level;
+            if ((!tie || j <= bound_at) && i >= 0 && i < row.vocab) {
                 const int pos = atomicAdd(&P.count, 1);
                 if (pos < cap) P.keys[pos] = order_key(v[e], (uint32_t)i);
             }
         }
     };
-    auto offer_vector = [&](int j) {
-        float v[n];
-        if (j >= row.full0 && j < row.full1)
-            Vec<E>::unpack(row.full(j), v);
-        else
-            row.ragged(j, v);
-        offer(j, v);
-    };
     const bool in = mine != 0ull && mine >= bound;
     // a second vector counts where its largest logit beats the bound's, or equals it at a
     // vector number up to the bound's
-    const uint32_t level = (uint32_t)(bound >> 32), second = total_order_key(acc.second + 0.f);
-    const long long bound_at = (long long)(0xffffffffu - (uint32_t)bound);
+    const uint32_t second = total_order_key(acc.second + 0.f);
     uint32_t again = __ballot_sync(0xffffffffu, in && second >= level);
     if (in) offer_vector(acc.at);
     for (; again; again &= again - 1) {
         const int from = __ffs(again) - 1, who = (tid & ~31) + from;
         const int skip = __shfl_sync(0xffffffffu, acc.at, from);
         const bool tie = __shfl_sync(0xffffffffu, second, from) == level;
-        const long long end = tie && bound_at + 1 < part.hi ? bound_at + 1 : part.hi;
-        for (long long j = (long long)part.lo + who + (long long)lane * T; j < end; j += 32ll * T)
-            if (j != skip) offer_vector((int)j);
+        const int end = bound && tie && bound_at < part.hi ? bound_at + 1 : part.hi;
+        for (int j = part.lo + who + lane * T; j < end; j += 32 * T)
+            if (j != skip) offer_vector(j);
         if (lane == 0 && part.head && who == 0 && skip != 0) offer_vector(0);
         if (lane == 0 && part.last && who == T - 1 && skip != row.full1) offer_vector(row.full1);
     }
@@ -740,7 +745,7 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     __shared__ int owner;
     const int parts = cluster_size(), part = cluster_rank();
     if (parts > 1) cluster_arrive();  // waited for before the first store into another block
-    const size_t r = blockIdx.x / parts;
+    const size_t r = blockIdx.x / (uint32_t)parts;
     const E* z = logits + r * stride;
     // the given token's logit is on its way while the row streams
     uint32_t token = kUnusedToken;
@@ -856,7 +861,7 @@ __device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part
         dense_vector<n, kLinear>(v, d, L);
 #pragma unroll
         for (int e = 0; e < n; ++e) {
-            const long long i = row.first(j) + e;
+            const int i = row.first(j) + e;
             if (i >= 0 && i < row.vocab) out[i] = Vec<E>::store(v[e]);
         }
     };
@@ -889,8 +894,8 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
     size_t gradient_stride) {
     __shared__ uint32_t ids[kMaxSlots];
     __shared__ float given[kMaxSlots];
-    const size_t r = blockIdx.x / parts;
-    const int part = (int)(blockIdx.x - r * parts), tid = threadIdx.x;
+    const size_t r = blockIdx.x / (uint32_t)parts;
+    const int part = (int)(blockIdx.x % (uint32_t)parts), tid = threadIdx.x;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
@@ -1029,7 +1034,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
     __shared__ int bad;
     const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
     if (parts > 1) cluster_arrive();  // waited for before the first store into another block
-    const size_t r = blockIdx.x / parts;
+    const size_t r = blockIdx.x / (uint32_t)parts;
     const int count = (int)teacher.slots;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
@@ -1187,8 +1192,8 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_g
     __shared__ __align__(16) uint32_t ids[kMaxSlots];
     __shared__ double sums[kListWarps];
     __shared__ float tops[kListWarps];
-    const size_t r = blockIdx.x / parts;
-    const int part = (int)(blockIdx.x - r * parts), count = (int)teacher.slots, tid = threadIdx.x;
+    const size_t r = blockIdx.x / (uint32_t)parts;
+    const int part = (int)(blockIdx.x % (uint32_t)parts), count = (int)teacher.slots, tid = threadIdx.x;
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
