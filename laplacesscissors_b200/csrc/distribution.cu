@@ -496,24 +496,31 @@ __device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Runnin
     return p;
 }
 
-// The row's sums from its blocks' shares.
-__device__ __forceinline__ Partial combine(const Partial* parts, int count, float L) {
-    Partial t = parts[0];
-    if (count == 1) return t;
-    int first = 0;
-    for (int i = 1; i < count; ++i)
-        if (parts[i].any && (!t.any || parts[i].m > t.m)) {
-            t = parts[i];
-            first = i;
-        }
-    for (int i = 0; i < count; ++i) {
-        if (i == first || !parts[i].any) continue;
-        Sums x{parts[i].m, 1.f + parts[i].rest, parts[i].W};
-        x.rebase(t.m, L);
-        t.rest += x.S;
-        t.W += x.W;
+// The row's sums from its blocks' shares, a share to a lane; by whole warps.
+__device__ __forceinline__ Partial combine(const Partial* shares, int count, float L) {
+    const int lane = threadIdx.x & 31;
+    const Partial mine = lane < count ? shares[lane] : Partial{-INFINITY, -1.f, 0.f, 0};
+    float m = mine.any ? mine.m : -INFINITY;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    m = __shfl_sync(0xffffffffu, m, 0);
+    // the first share that holds the maximum counts it as 1
+    const uint32_t holders = __ballot_sync(0xffffffffu, mine.any && mine.m == m);
+    const bool holder = lane == __ffs(holders) - 1;
+    Sums x{m, 0.f, 0.f};
+    if (mine.any && !holder) {
+        x = {mine.m, 1.f + mine.rest, mine.W};
+        x.rebase(m, L);
+    } else if (holder) {
+        x = {m, mine.rest, mine.W};
     }
-    return t;
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) {
+        x.S += __shfl_xor_sync(0xffffffffu, x.S, o);
+        x.W += __shfl_xor_sync(0xffffffffu, x.W, o);
+    }
+    return {m, __shfl_sync(0xffffffffu, x.S, 0), __shfl_sync(0xffffffffu, x.W, 0),
+            __any_sync(0xffffffffu, mine.any)};
 }
 
 // ---- thread-block clusters --------------------------------------------------------------
@@ -638,6 +645,26 @@ __device__ void rank_keys(Selection& P, unsigned long long* keys, int n, int top
         rank_all(P, P.fewer, count, top);
     else
         rank_all(P, keys, n, top);
+}
+
+// The `top` largest of `parts` descending lists of `top` keys each.  Every list's
+// ceil(top / parts)-th key is at or above the smallest of these, so `top` keys are, and the
+// others cannot be among them.
+__device__ void rank_lists(Selection& P, const unsigned long long* lists, int parts, int top) {
+    const int each = (top + parts - 1) / parts;
+    if (threadIdx.x == 0) P.count = 0;
+    unsigned long long bound = lists[each - 1];
+    for (int i = 1; i < parts; ++i) {
+        const unsigned long long key = lists[i * top + each - 1];
+        bound = key < bound ? key : bound;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < parts * top; i += blockDim.x) {
+        const unsigned long long key = lists[i];
+        if (key >= bound) P.keys[atomicAdd(&P.count, 1)] = key;
+    }
+    __syncthreads();
+    rank_keys(P, P.keys, P.count, top);
 }
 
 // The `top` best tokens of elements [begin, end) of a row, piece by piece: what beats the
@@ -780,7 +807,7 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
         cluster_wait();
         if (part != 0) return;
         sums = combine(shares, parts, k.L);
-        if (top > 0) rank_keys(selection, selection.keys + kListCap / 2, parts * top, top);
+        if (top > 0) rank_lists(selection, selection.keys + kListCap / 2, parts, top);
     }
     const bool empty = !sums.any;  // every logit is -inf
     const float m = sums.m, log_sum = empty ? 0.f : log1pf(sums.rest);
