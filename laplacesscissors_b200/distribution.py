@@ -24,6 +24,8 @@ from .gpu import Gpu
 _KINDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _DEFAULT_STREAM = 1  # cudaStreamLegacy
 _raw_stream = torch._C._cuda_getCurrentRawStream
+_F32, _I32 = torch.float32, torch.int32
+_logprobs = lib.lsx_token_logprobs_device
 MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
 
 
@@ -62,13 +64,12 @@ def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
     return rows, vocab, stride, kind
 
 
-def _vector(gpu: Gpu, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
-    """Address of a contiguous tensor of this shape and type on the Gpu's device."""
-    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.shape != shape:
-        raise ValueError(f"{name} must be a {dtype} tensor of shape {list(shape)}")
-    if t.get_device() != gpu.device or not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous on the Gpu's device")
-    return t.data_ptr()
+def _vector(device: int, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
+    """Address of a contiguous tensor of this shape and type on the device."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device \
+            and t.is_contiguous():
+        return t.data_ptr()
+    raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on the Gpu's device")
 
 
 def _count(t: torch.Tensor, rows: int, name: str) -> int:
@@ -86,10 +87,10 @@ def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
     return out, _rows(gpu, out, "the gradient")[2]
 
 
-def _stream(gpu: Gpu) -> int:
-    """torch's current stream on the Gpu's device, as lsx.h takes it (the raw handle that
+def _stream(device: int) -> int:
+    """torch's current stream on the device, as lsx.h takes it (the raw handle that
     torch.cuda.current_stream wraps in an object)."""
-    return _raw_stream(gpu.device) or _DEFAULT_STREAM
+    return _raw_stream(device) or _DEFAULT_STREAM
 
 
 def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None = None, *, alternatives: int = 0,
@@ -102,19 +103,26 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
     k = int(alternatives)
     if not 0 <= k <= min(MAX_SLOTS, vocab):
         raise ValueError(f"alternatives must be at most {MAX_SLOTS} and at most the vocabulary")
-    f32, i32 = torch.float32, torch.int32
-    shapes = ((rows, n), f32), ((rows,), f32), ((rows, 2), f32), ((rows, k), i32), ((rows, k), f32), ((rows, k), f32)
     if out is None:
-        wanted = n > 0, True, True, k > 0, k > 0, k > 0
-        out = [torch.empty(s, dtype=d, device=logits.device) if w else None for w, (s, d) in zip(wanted, shapes)]
+        def new(wanted, *shape, dtype=_F32):
+            return torch.empty(shape, dtype=dtype, device=logits.device) if wanted else None
+        out = (new(n, rows, n), new(True, rows), new(True, rows, 2), new(k, rows, k, dtype=_I32), new(k, rows, k),
+               new(k, rows, k))
     elif len(out) != 6:
         raise ValueError("out holds the six results")
-    at = [None if t is None or 0 in s else _vector(gpu, t, s, d, "out") for t, (s, d) in zip(out, shapes)]
-    given = _vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None
+    d = gpu.device
+    logprob, entropy, stats, ids, values, logprobs = out
     if rows:
-        check(lib.lsx_token_logprobs_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
-                                            given, n, k, *at, _stream(gpu)))
-    return TokenLogprobs(*out)
+        check(_logprobs(
+            gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
+            _vector(d, tokens, (rows, n), _I32, "tokens") if n else None, n, k,
+            None if logprob is None or not n else _vector(d, logprob, (rows, n), _F32, "out[0]"),
+            None if entropy is None else _vector(d, entropy, (rows,), _F32, "out[1]"),
+            None if stats is None else _vector(d, stats, (rows, 2), _F32, "out[2]"),
+            None if ids is None or not k else _vector(d, ids, (rows, k), _I32, "out[3]"),
+            None if values is None or not k else _vector(d, values, (rows, k), _F32, "out[4]"),
+            None if logprobs is None or not k else _vector(d, logprobs, (rows, k), _F32, "out[5]"), _stream(d)))
+    return TokenLogprobs(logprob, entropy, stats, ids, values, logprobs)
 
 
 def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None, stats: torch.Tensor,
@@ -129,15 +137,14 @@ def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor
     out, out_stride = _gradient(gpu, logits, out)
     if entropy_gradient is None:
         entropy = None
-    f32 = torch.float32
-    at = (_vector(gpu, tokens, (rows, n), torch.int32, "tokens") if n else None, n,
-          _vector(gpu, stats, (rows, 2), f32, "stats"),
-          _vector(gpu, entropy, (rows,), f32, "entropy") if entropy_gradient is not None else None,
-          _vector(gpu, logprob_gradient, (rows, n), f32, "logprob_gradient") if n else None,
-          _vector(gpu, entropy_gradient, (rows,), f32, "entropy_gradient") if entropy_gradient is not None else None)
+    at = (_vector(gpu.device, tokens, (rows, n), _I32, "tokens") if n else None, n,
+          _vector(gpu.device, stats, (rows, 2), _F32, "stats"),
+          _vector(gpu.device, entropy, (rows,), _F32, "entropy") if entropy_gradient is not None else None,
+          _vector(gpu.device, logprob_gradient, (rows, n), _F32, "logprob_gradient") if n else None,
+          _vector(gpu.device, entropy_gradient, (rows,), _F32, "entropy_gradient") if entropy_gradient is not None else None)
     if rows:
         check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
-                                                     temperature, *at, out.data_ptr(), out_stride, _stream(gpu)))
+                                                     temperature, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
     return out
 
 
@@ -145,9 +152,9 @@ def _teacher(gpu: Gpu, rows: int, ids, values, stats):
     k = _count(ids, rows, "teacher_ids")
     if k < 1:
         raise ValueError("the teacher lists at least one token")
-    return (_vector(gpu, ids, (rows, k), torch.int32, "teacher_ids"),
-            _vector(gpu, values, (rows, k), torch.float32, "teacher_logits"), k,
-            _vector(gpu, stats, (rows, 2), torch.float32, "teacher_stats") if stats is not None else None)
+    return (_vector(gpu.device, ids, (rows, k), _I32, "teacher_ids"),
+            _vector(gpu.device, values, (rows, k), _F32, "teacher_logits"), k,
+            _vector(gpu.device, stats, (rows, 2), _F32, "teacher_stats") if stats is not None else None)
 
 
 def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_logits: torch.Tensor, *,
@@ -163,19 +170,18 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
     if weights is not None and not gradient:
         raise ValueError("weights scale the gradient only")
-    f32 = torch.float32
     if out is None:
-        out = (torch.empty(rows, dtype=f32, device=logits.device),
-               torch.empty((rows, 3), dtype=f32, device=logits.device), None)
+        out = (torch.empty(rows, dtype=_F32, device=logits.device),
+               torch.empty((rows, 3), dtype=_F32, device=logits.device), None)
     elif len(out) != 3 or (out[2] is not None and not gradient):
         raise ValueError("out holds the three results, the last only with the gradient")
     grad, grad_stride = _gradient(gpu, logits, out[2]) if gradient else (None, 0)
-    at = (_vector(gpu, weights, (rows,), f32, "weights") if weights is not None else None,
-          _vector(gpu, out[0], (rows,), f32, "out[0]") if out[0] is not None else None,
-          _vector(gpu, out[1], (rows, 3), f32, "out[1]") if out[1] is not None else None)
+    at = (_vector(gpu.device, weights, (rows,), _F32, "weights") if weights is not None else None,
+          _vector(gpu.device, out[0], (rows,), _F32, "out[0]") if out[0] is not None else None,
+          _vector(gpu.device, out[1], (rows, 3), _F32, "out[1]") if out[1] is not None else None)
     if rows:
         check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature, *teacher,
-                                     *at, grad.data_ptr() if gradient else None, grad_stride, _stream(gpu)))
+                                     *at, grad.data_ptr() if gradient else None, grad_stride, _stream(gpu.device)))
     return Distillation(out[0], out[1], grad)
 
 
@@ -187,11 +193,11 @@ def distill_backward(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, 
     rows, vocab, stride, kind = _rows(gpu, logits)
     teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
     out, out_stride = _gradient(gpu, logits, out)
-    at = (_vector(gpu, stats, (rows, 3), torch.float32, "stats"),
-          _vector(gpu, loss_gradient, (rows,), torch.float32, "loss_gradient"))
+    at = (_vector(gpu.device, stats, (rows, 3), _F32, "stats"),
+          _vector(gpu.device, loss_gradient, (rows,), _F32, "loss_gradient"))
     if rows:
         check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
-                                              *teacher, *at, out.data_ptr(), out_stride, _stream(gpu)))
+                                              *teacher, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
     return out
 
 
