@@ -1162,19 +1162,27 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
         log_sum = empty ? 0.f : log1pf(over);
         if (kTail && some) log_rest = logf(rest.S) + below;
     };
+    // (the loss may be a small difference of these logarithms: in 64 bits)
     auto write_row = [&]() {
-        double x = mass, cross = 0.0;
-        for (int w = 0; w < kListWarps; ++w) cross += crosses[w];
-        if (!kTail && x != 0.0) {  // normalised over the list
-            cross = cross / x - log(x);
-            x = x == x ? 1.0 : x;
-        }
         if (loss) {
+            double inside = 0.0, cross = 0.0, x = mass;
+            for (int w = 0; w < kListWarps; ++w) {
+                inside += insides[w];
+                cross += crosses[w];
+            }
+            if (!kTail && x != 0.0) {  // normalised over the list
+                cross = cross / x - log(x);
+                x = x == x ? 1.0 : x;
+            }
+            const double down = rest.S == 0.f ? -INFINITY : ((double)rest.m - (double)m) * inverse;
+            const double outside = rest.S == 0.f ? 0.0 : (double)rest.S * exp(down);
+            const double listed = inside == 0.0 ? 0.0 : high == m ? inside : inside * exp(((double)high - (double)m) * inverse);
+            const double log_all = empty ? 0.0 : log(listed + outside);
             double value = x == 0.0            ? 0.0
                            : cross == INFINITY ? INFINITY
-                                               : cross + x * (((double)m - (double)high) * inverse + log_sum);
+                                               : cross + x * (((double)m - (double)high) * inverse + log_all);
             if (kTail && p_rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
-                value += p_rest * (log(p_rest) - log_rest + log_sum);
+                value += p_rest * (log(p_rest) - log((double)rest.S) - down + log_all);
             loss[r] = bad || x != x || log_sum != log_sum ? NAN : (float)value;
         }
         if (stats) {
