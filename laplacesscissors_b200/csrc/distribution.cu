@@ -29,6 +29,7 @@ constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;     // candidate keys of one selection
 constexpr int kAgainVectors = 10000;    // a slice that is read again for its gradient, at most
 constexpr int kPieceVectors = 2048;      // a slice of the gradient kernels
+constexpr int kBriefVectors = 512;       // rows shorter than this are distilled by blocks of 128
 constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -572,10 +573,10 @@ struct Selection {
 // their largest (`mine`, 0 for none), and the `top`-th largest of the groups' is returned (0
 // where there are not as many).  Distinct keys; `top` of all the keys are at or above the
 // bound.  Resets P.count.  Ends with the block synchronised.
-__device__ unsigned long long group_bound(Selection& P, unsigned long long mine, int top) {
+__device__ unsigned long long group_bound(Selection& P, unsigned long long mine, int top, int holders) {
     const int tid = threadIdx.x, T = blockDim.x;
     // groups as wide as leave 2.5 groups per wanted key
-    const int wide = top * 10 <= T ? 4 : top * 5 <= T ? 2 : 1, groups = T / wide;
+    const int wide = top * 10 <= holders ? 4 : top * 5 <= holders ? 2 : 1, groups = T / wide;
     for (int o = 1; o < wide; o <<= 1) {
         const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
         mine = other > mine ? other : mine;
@@ -632,7 +633,7 @@ __device__ void rank_keys(Selection& P, unsigned long long* keys, int n, int top
     __syncthreads();
     unsigned long long mine = 0ull;
     for (int i = threadIdx.x; i < n; i += blockDim.x) mine = keys[i] > mine ? keys[i] : mine;
-    const unsigned long long bound = group_bound(P, mine, top);
+    const unsigned long long bound = group_bound(P, mine, top, n < (int)blockDim.x ? n : (int)blockDim.x);
     for (int i = threadIdx.x; i < n; i += blockDim.x) {
         const unsigned long long key = keys[i];
         if (key < bound) continue;
@@ -702,6 +703,14 @@ __device__ void select_by_pieces(Selection& P, const E* z, int begin, int end, i
 // are read again (from L2) at the threads' best vectors, and in all their vectors only for
 // threads that have a second one to offer.  More candidates than the list holds are left
 // to select_by_pieces.
+// Slices that are ranked whole: the shortest ones, and short ones with hardly a vector for
+// each alternative.
+template <typename E>
+__device__ __forceinline__ bool ranked_whole(const Slice& part, int top) {
+    const int tokens = part.end - part.begin;
+    return tokens <= 96 || (tokens <= 256 && top * 4 > (part.hi - part.lo) * 3);
+}
+
 template <typename E>
 __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& part, const E* z, int top,
                                   const Running<true>& acc, int cap) {
@@ -709,7 +718,8 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
     const int tid = threadIdx.x, lane = tid & 31, T = blockDim.x;
     const unsigned long long mine =
         acc.at < 0 ? 0ull : ((unsigned long long)total_order_key(acc.m + 0.f) << 32) | (0xffffffffu - (uint32_t)acc.at);
-    const unsigned long long bound = group_bound(P, mine, top);
+    const int vectors = part.hi - part.lo;
+    const unsigned long long bound = group_bound(P, mine, top, vectors < T ? vectors : T);
     const uint32_t level = (uint32_t)(bound >> 32);
     const int bound_at = (int)(0xffffffffu - (uint32_t)bound);  // (with a bound)
     // the bound's logit; without a bound everything passes
@@ -738,7 +748,8 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
     // a second vector counts where its largest logit beats the bound's, or equals it at a
     // vector number up to the bound's
     const uint32_t second = total_order_key(acc.second + 0.f);
-    uint32_t again = __ballot_sync(0xffffffffu, in && second >= level);
+    const bool more = vectors - tid + (part.head && tid == 0) + (part.last && tid == T - 1) > 1;
+    uint32_t again = __ballot_sync(0xffffffffu, in && more && second >= level);
     if (in) offer_vector(acc.at);
     for (; again; again &= again - 1) {
         const int from = __ffs(again) - 1, who = (tid & ~31) + from;
@@ -790,7 +801,11 @@ __global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __
     // clusters keep the upper half of the list for the blocks' best keys
     const int cap = parts > 1 ? kListCap / 2 : kListCap;
     if (top > 0) {
-        if (!sums.any) {  // nothing but -inf: the lowest ids
+        if (ranked_whole<E>(slice, top)) {
+            for (int i = threadIdx.x; i < slice.end - slice.begin; i += T)
+                selection.keys[i] = order_key(Vec<E>::one(z[slice.begin + i]), (uint32_t)(slice.begin + i));
+            rank_all(selection, selection.keys, slice.end - slice.begin, top);
+        } else if (!sums.any) {  // nothing but -inf: the lowest ids
             for (int i = threadIdx.x; i < top; i += T) selection.best[i] = order_key(-INFINITY, slice.begin + i);
             __syncthreads();
         } else if (sums.rest == sums.rest)
@@ -1049,8 +1064,8 @@ __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logi
 // elements, which have their own sums; with kGradient the row is then read again, from L2,
 // for its gradient.  A cluster of blocks shares a row: they exchange their sums (with
 // kGradient each takes the list for itself, else the first one).
-template <typename E, bool kTail, bool kGradient>
-__global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
+template <typename E, bool kTail, bool kGradient, int T>
+__global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     __shared__ Sums scratch[33];
@@ -1077,7 +1092,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
     bool kept = false;
     Running<false> acc;
     stream_slice<E, true>(row, slice, &marks, count, k, acc, [&]() {
-        for (int i = tid; i < kMarkWords; i += kRowThreads) marks.bits[i] = 0;
+        for (int i = tid; i < kMarkWords; i += T) marks.bits[i] = 0;
         if (tid == 0) marks.asides = bad = 0;
         if (tid < kMaxSlots) marks.ids[tid] = id < (uint32_t)vocab ? id : kUnusedToken;
         __syncthreads();
@@ -1162,29 +1177,37 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
         log_sum = empty ? 0.f : log1pf(over);
         if (kTail && some) log_rest = logf(rest.S) + below;
     };
-    // (the loss may be a small difference of these logarithms: in 64 bits)
+    // By the first warp.  The loss may be a small difference of logarithms: they are taken
+    // in 64 bits, one to a lane, so that the row waits for one of each function.
     auto write_row = [&]() {
-        if (loss) {
-            double inside = 0.0, cross = 0.0, x = mass;
-            for (int w = 0; w < kListWarps; ++w) {
-                inside += insides[w];
-                cross += crosses[w];
-            }
-            if (!kTail && x != 0.0) {  // normalised over the list
-                cross = cross / x - log(x);
-                x = x == x ? 1.0 : x;
-            }
-            const double down = rest.S == 0.f ? -INFINITY : ((double)rest.m - (double)m) * inverse;
-            const double outside = rest.S == 0.f ? 0.0 : (double)rest.S * exp(down);
-            const double listed = inside == 0.0 ? 0.0 : high == m ? inside : inside * exp(((double)high - (double)m) * inverse);
-            const double log_all = empty ? 0.0 : log(listed + outside);
-            double value = x == 0.0            ? 0.0
-                           : cross == INFINITY ? INFINITY
-                                               : cross + x * (((double)m - (double)high) * inverse + log_all);
-            if (kTail && p_rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
-                value += p_rest * (log(p_rest) - log((double)rest.S) - down + log_all);
-            loss[r] = bad || x != x || log_sum != log_sum ? NAN : (float)value;
+        double inside = 0.0, cross = 0.0;
+#pragma unroll
+        for (int w = 0; w < kListWarps; ++w) {
+            inside += insides[w];
+            cross += crosses[w];
         }
+        const bool some = rest.S != 0.f;
+        const double down = some ? ((double)rest.m - (double)m) * inverse : -INFINITY;
+        const double up = inside == 0.0 ? -INFINITY : ((double)high - (double)m) * inverse;
+        const double factor = exp(tid == 0 ? down : up);
+        const double outside = some ? (double)rest.S * __shfl_sync(0xffffffffu, factor, 0) : 0.0;
+        const double listed = inside == 0.0 ? 0.0 : inside * __shfl_sync(0xffffffffu, factor, 1);
+        const double log_of = log(tid == 0 ? listed + outside : tid == 1 ? mass : tid == 2 ? p_rest : (double)rest.S);
+        const double log_all = empty ? 0.0 : __shfl_sync(0xffffffffu, log_of, 0);
+        const double log_mass = __shfl_sync(0xffffffffu, log_of, 1), log_p = __shfl_sync(0xffffffffu, log_of, 2);
+        const double log_S = __shfl_sync(0xffffffffu, log_of, 3);
+        if (tid != 0) return;
+        double x = mass;
+        if (!kTail && x != 0.0) {  // normalised over the list
+            cross = cross / x - log_mass;
+            x = x == x ? 1.0 : x;
+        }
+        double value = x == 0.0            ? 0.0
+                       : cross == INFINITY ? INFINITY
+                                           : cross + x * (((double)m - (double)high) * inverse + log_all);
+        if (kTail && p_rest > 0.0 && log_rest - log_sum >= kSmallestLogShare)
+            value += p_rest * (log_p - log_S - down + log_all);
+        if (loss) loss[r] = bad || x != x || log_sum != log_sum ? NAN : (float)value;
         if (stats) {
             stats[3 * r] = m;
             stats[3 * r + 1] = log_sum;
@@ -1193,7 +1216,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
     };
     if (!kGradient) {
         if (parts > 1) cluster_wait();
-        if (part != 0 || tid != 0) return;
+        if (part != 0 || tid >= 32) return;
         put_together();
         write_row();
         return;
@@ -1201,7 +1224,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
     const double weight = weights ? (double)weights[r] * inverse : inverse;
     DistillRow g;
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, out, k.L, tid, kRowThreads, [&]() {
+    write_dense<E, false>(row, slice, out, k.L, tid, T, [&]() {
         if (parts > 1) cluster_wait();
         put_together();
         const float P = kTail ? (float)mass : mass == 0.0 ? 0.f : mass == mass ? 1.f : NAN;
@@ -1213,7 +1236,7 @@ __global__ void __launch_bounds__(kRowThreads, 6) distill_kernel(
         const double share = kTail || mass == 0.0 ? weight : weight / mass;
         out[id] = Vec<E>::store(listed_gradient(g, logit, (float)(share * p), k.L));
     }
-    if (part == 0 && tid == 0) write_row();
+    if (part == 0 && tid < 32) write_row();
 }
 
 // The gradient from saved statistics; `parts` blocks share a row, none waits for another.
@@ -1300,12 +1323,11 @@ cudaError_t by_kind(lsx_dtype kind, F&& f) {
 }
 
 
-// How many blocks share a row: as many as fill the GPU, while each keeps a full pass of
-// its threads.
-int row_parts(int sm_count, size_t rows, size_t vectors, int threads, int resident) {
+// How many blocks share a row: as many as fill the GPU, while each keeps `least` vectors.
+int row_parts(int sm_count, size_t rows, size_t vectors, int least, int resident) {
     int parts = 1;
     while (parts < kMaxCluster && rows * parts * 2 <= (size_t)sm_count * resident &&
-           vectors / (parts * 2) >= (size_t)threads)
+           vectors / (parts * 2) >= (size_t)least)
         parts *= 2;
     return parts;
 }
@@ -1342,12 +1364,14 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
         const Scale k(z.temperature);
-        if (vectors < 1024)
+        // few alternatives of a short row: smaller blocks leave more rows on an SM
+        if (vectors < 1024 && (alternatives <= 24 || vectors <= 128))
             return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
-        return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, row_parts(sm_count, z.rows, vectors, 256, 4), 256,
-                               s, (const E*)z.data, (int)z.vocab, z.stride, k, tokens, (int)token_count,
-                               (int)alternatives, out);
+        // every block of a cluster selects all the alternatives of its slice: many of them pay in longer slices only
+        const int parts = row_parts(sm_count, z.rows, vectors, alternatives <= 24 ? 256 : 1024, 4);
+        return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, parts, 256, s, (const E*)z.data, (int)z.vocab,
+                               z.stride, k, tokens, (int)token_count, (int)alternatives, out);
     });
 }
 
@@ -1374,9 +1398,14 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
         int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
         if (gradient)  // the rows in flight have to stay in L2 until they are read again
             while (parts < kMaxCluster && vectors / parts > (size_t)kAgainVectors) parts *= 2;
-        auto kernel = gradient ? (teacher.stats ? distill_kernel<E, true, true> : distill_kernel<E, false, true>)
-                               : (teacher.stats ? distill_kernel<E, true, false> : distill_kernel<E, false, false>);
-        return launch_clusters(kernel, z.rows, parts, kRowThreads, s, (const E*)z.data, (int)z.vocab, z.stride,
+        auto pick = [&](auto threads) {
+            constexpr int T = decltype(threads)::value;
+            return gradient ? (teacher.stats ? distill_kernel<E, true, true, T> : distill_kernel<E, false, true, T>)
+                            : (teacher.stats ? distill_kernel<E, true, false, T> : distill_kernel<E, false, false, T>);
+        };
+        const bool brief = vectors < (size_t)kBriefVectors;  // smaller blocks leave more short rows on an SM
+        auto kernel = brief ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, kRowThreads>());
+        return launch_clusters(kernel, z.rows, parts, brief ? 128 : kRowThreads, s, (const E*)z.data, (int)z.vocab, z.stride,
                                Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats, (E*)gradient,
                                gradient_stride);
     });
