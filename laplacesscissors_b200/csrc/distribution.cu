@@ -758,7 +758,7 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
     const int vectors = part.hi - part.lo;
     const unsigned long long bound = key_bound(P, mine, top, vectors < T ? vectors : T);
     const uint32_t level = (uint32_t)(bound >> 32);
-    const int bound_at = (int)(0xffffffffu - (uint32_t)bound);  // (with a bound)
+    const uint32_t bound_at = 0xffffffffu - (uint32_t)bound;  // (a bisected bound may lie past the last vector)
     // the bound's logit; without a bound everything passes
     const float level_logit = bound ? total_order_value(level) : -INFINITY;
     auto offer_vector = [&](int j) {
@@ -775,7 +775,7 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
             if (v[e] < level_logit) continue;
             const int i = row.first(j) + e;
             const bool tie = bound && total_order_key(v[e] + 0.f) == level;
-            if ((!tie || j <= bound_at) && i >= 0 && i < row.vocab) {
+            if ((!tie || (uint32_t)j <= bound_at) && i >= 0 && i < row.vocab) {
                 const int pos = atomicAdd(&P.count, 1);
                 if (pos < cap) P.keys[pos] = order_key(v[e], (uint32_t)i);
             }
@@ -799,7 +799,7 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
         const int skip = __shfl_sync(0xffffffffu, acc.at, from);
         const bool tie = __shfl_sync(0xffffffffu, second, from) == level;
         if (rest) {
-            const int end = bound && tie && bound_at < part.hi ? bound_at + 1 : part.hi;
+            const int end = bound && tie && bound_at < (uint32_t)part.hi ? (int)bound_at + 1 : part.hi;
             for (int j = part.lo + who + (lane & (per - 1)) * T; j < end; j += per * T)
                 if (j != skip) offer_vector(j);
             if ((lane & (per - 1)) == 0 && part.head && who == 0 && skip != 0) offer_vector(0);

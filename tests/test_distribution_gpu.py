@@ -724,3 +724,34 @@ def test_peaked_rows_keep_the_small_rest(gpu, dev, dtype, vocab):
     y = torch.where(rest == -math.inf, 0.0, rest - top[:, None])
     entropy = log_sum - (torch.exp(rest - top[:, None]) * y).sum(1) / (1 + r)
     within(got.entropy, entropy, 2 * tol * entropy)
+
+
+def test_alternatives_at_neighbouring_values(gpu, dev):
+    """Rows of two neighbouring f32 values: the value that separates them is itself a logit, and
+    its ties have to stay candidates; with fewer, as many and more of the larger one than
+    alternatives."""
+    low = torch.nextafter(torch.tensor(2.0), torch.tensor(0.0)).item()
+    for vocab in (4099, 1031, 40000):
+        for larger in (5, 47, 50, 100, 127, 200, 600):
+            z = torch.full((3, vocab), low, device=dev)
+            g = torch.Generator().manual_seed(larger)
+            for r in range(3):
+                z[r, torch.randperm(vocab, generator=g)[:larger].to(dev)] = 2.0
+            z[2, ::3] = -math.inf
+            for k in (26, 48, 100, 128):
+                got = distribution.token_logprobs(gpu, z, alternatives=k)
+                assert torch.equal(got.top_ids.long(), order64(z, k)), (vocab, larger, k)
+
+
+@pytest.mark.parametrize("dtype", KINDS)
+def test_alternatives_of_coarse_logits(gpu, dev, dtype):
+    """Logits on a coarse grid tie everywhere; masks leave few, some or most of them."""
+    g = torch.Generator().manual_seed(71)
+    for vocab in (97, 257, 1025, 5000, 33000):
+        z = torch.randint(-6, 7, (24, vocab), generator=g).to(dtype)
+        for r in range(24):
+            z[r, torch.rand(vocab, generator=g) < [0.0, 0.5, 0.99][r % 3]] = -math.inf
+        z = z.to(dev)
+        for k in (1, 7, 20, 25, 30, 60, min(vocab, 128)):
+            got = distribution.token_logprobs(gpu, z, alternatives=k)
+            assert torch.equal(got.top_ids.long(), order64(z, k)), (vocab, k)
