@@ -1094,6 +1094,7 @@ __device__ __forceinline__ DistillRow distill_row(float m, float log_sum, float 
     g.a = scale * mass;
     g.empty = empty;
     g.dense = dense_zero();
+    if (bad) g.dense.a = NAN;
     if (!empty) {
         g.dense.m = m;
         g.dense.offset = tail ? log_rest * kLog2E : g.offset;
@@ -1104,7 +1105,7 @@ __device__ __forceinline__ DistillRow distill_row(float m, float log_sum, float 
 // The gradient at a listed token with the student's logit and the teacher's w p / T.
 __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logit, float value, float L) {
     const float y = max_nan(fmaf(logit - g.m, L, -g.offset), kLowestExponent);
-    return g.empty ? 0.f : fmaf(exp2_fast(y), g.a, -value);
+    return g.empty ? 0.f * g.a : fmaf(exp2_fast(y), g.a, -value);
 }
 
 // Loss and statistics of rows that stream through registers, without their listed

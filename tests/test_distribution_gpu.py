@@ -755,3 +755,14 @@ def test_alternatives_of_coarse_logits(gpu, dev, dtype):
         for k in (1, 7, 20, 25, 30, 60, min(vocab, 128)):
             got = distribution.token_logprobs(gpu, z, alternatives=k)
             assert torch.equal(got.top_ids.long(), order64(z, k)), (vocab, k)
+
+
+def test_distill_bad_slot_in_an_empty_row(gpu, dev):
+    z = torch.full((2, 40), -math.inf, device=dev)
+    ids = torch.tensor([[1, 40], [1, 2]], dtype=torch.int32, device=dev)
+    values = torch.zeros(2, 2, device=dev)
+    got = distribution.distill(gpu, z, ids, values, gradient=True)
+    back = distribution.distill_backward(gpu, z, ids, values, got.stats, torch.ones(2, device=dev))
+    for grad in (got.gradient, back):
+        assert bool(grad[0].isnan().all()) and not bool(grad[1].any())
+    assert bool(got.loss[0].isnan()) and float(got.loss[1]) == math.inf
