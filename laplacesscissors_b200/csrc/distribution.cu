@@ -3,13 +3,24 @@
 // of both with respect to the logits.
 //
 // Per row z[0..V) at temperature T, with m = max z and s = ln sum_i exp((z_i - m) / T),
-// the probabilities are q_i = exp((z_i - m) / T - s).  Every operator is one pass over
-// the row (two for a loss with its gradient): HBM traffic bounds it, and one exponential
-// per element (MUFU) comes next.
+// the probabilities are q_i = exp((z_i - m) / T - s).  The sums are one pass over the row,
+// a gradient is one more; HBM traffic bounds both where there is work enough, one
+// exponential per element (16 per clock and SM) comes next, and few short rows cost the
+// chain of their steps (load, sum, select, put together), about 5 us.
 //
 // Differences are formed before they are scaled: y = (z - r) * (log2 e / T) against a
 // reference r that is itself one of the logits, so the lowest value of a type, -inf
-// masks and logits far from zero all give the exponent their difference has.
+// masks and logits far from zero all give the exponent their difference has.  Sums are
+// f32 against the row's maximum, in an order that sizes alone decide, so results repeat
+// bit for bit; what small differences are made of (a list's mass, a loss) is f64.  A
+// 16-bit gradient is rounded once, when it is stored.
+//
+// Measured on B200 (6552 GB/s measured copy, a pass among others): log probabilities with 8
+// alternatives of 2048 x 151936 f32 191 us (99% of the copy's rate), with 20 of one row
+// 9.8 us, with 50 of 777 x 50257 f16 37 us (32%: the rows of an SM select at the same
+// time); their gradient, 2048 x 151936 bf16, 190 us (100%); a loss of 512 x 151936 f32 with 20
+// listed tokens 58 us (81%); loss and gradient of 2048 x 151936 bf16 332 us (57%: the logits
+// are read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -24,13 +35,20 @@
 namespace lsx {
 namespace {
 
-constexpr int kRowThreads = 256;
+constexpr int kRowThreads = 256;     // 5 or 6 such blocks on an SM: 512 or 1024 threads overlap a row's steps less
 constexpr int kPieceThreads = 128;   // of the gradient kernels
-constexpr int kListCap = 2048;     // candidate keys of one selection
-constexpr int kAgainVectors = 10000;    // a slice that is read again for its gradient, at most
-constexpr int kPieceVectors = 2048;      // a slice of the gradient kernels
-constexpr int kBriefVectors = 512;       // rows shorter than this are distilled by blocks of 128
-constexpr int kUnroll = 4;         // 16-byte loads in flight per thread
+constexpr int kListCap = 2048;       // candidate keys of one selection
+// Loss and gradient in one kernel read a slice twice.  A slice is at most this many vectors
+// (two blocks for a row of 151936 bf16): 1, 2, 4 and 8 blocks a row measured 342, 333, 366
+// and 444 us on 2048 of them; 190 rows of 128003 f32 69 us whole, 63 in quarters.
+constexpr int kAgainVectors = 10000;
+// Slices of the gradient kernels: 1200, 2048 and 3000 vectors measured 201, 190 and 196 us on
+// 2048 x 151936 bf16.
+constexpr int kPieceVectors = 2048;
+// Rows shorter than this are distilled by blocks of 128 threads, which leaves more of them on
+// an SM: 1084 x 396 f32 7.1 us against 12.3.
+constexpr int kBriefVectors = 512;
+constexpr int kUnroll = 4;           // 16-byte loads in flight per thread
 constexpr float kLog2E = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 // Exponents (base 2) below this are zero in f32 with room to spare; the bound keeps
@@ -472,8 +490,8 @@ struct Partial {
 };
 
 template <typename E>
-__device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Running<true>& acc, const Scale& k, Sums* scratch,
-                              int* owner) {
+__device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Running<true>& acc, const Scale& k,
+                              Sums* scratch, int* owner) {
     const Sums x = block_sums(acc, k.L, scratch);
     Partial p{x.m, x.S - 1.f, x.W, x.S != 0.f};
     if (x.S != 0.f && x.S < kPeaked) {  // the maximum is unique
@@ -486,7 +504,6 @@ __device__ Partial slice_sums(const Row<E>& row, const Slice& part, const Runnin
         }
         if (threadIdx.x < 32) {
             const Sums again = sum_without_maximum(row, part, *owner, x.m, k.L);
-            // (a thread's own element at x.m, if any, went with the owner's sums)
             scratch[32] = again;
         }
         const Sums rest = block_sums(others, k.L, scratch);
@@ -602,14 +619,15 @@ __device__ unsigned long long group_bound(Selection& P, unsigned long long mine,
     return P.bound;
 }
 
-// More, and few of few (`holders` threads have a key), are bounded by bisection: the largest value found that `top` keys reach.  It ends
-// once hardly more than `top` reach it, which takes about eight counts; keys that differ
-// in their low bits only (ties) take more, never more than 64 (29 rows of 5036, 93
-// alternatives: 11.5 us against 16.7 by groups).
+// More, and few of few (`holders` threads have a key), are bounded by bisection: the largest
+// value found that `top` keys reach.  It ends once hardly more than `top` reach it, which
+// takes about eight counts; keys that differ in their low bits only (ties) take more, never
+// more than 64 (29 rows of 5036, 93 alternatives: 11.5 us against 16.7 by groups).
 __device__ unsigned long long key_bound(Selection& P, unsigned long long mine, int top, int holders) {
     if (top * 10 <= holders) return group_bound(P, mine, top);
     const uint32_t high = (uint32_t)(mine >> 32);
-    const uint32_t most = __reduce_max_sync(0xffffffffu, high), least = __reduce_min_sync(0xffffffffu, mine ? high : ~0u);
+    const uint32_t most = __reduce_max_sync(0xffffffffu, high);
+    const uint32_t least = __reduce_min_sync(0xffffffffu, mine ? high : ~0u);
     if (threadIdx.x == 0) {
         P.most = 0u;
         P.least = ~0u;
@@ -622,7 +640,8 @@ __device__ unsigned long long key_bound(Selection& P, unsigned long long mine, i
     }
     if (__syncthreads_count(mine != 0ull) < top) return 0ull;
     // at least `top` keys reach lo, fewer than `top` reach hi
-    unsigned long long lo = (unsigned long long)P.least << 32, hi = ((unsigned long long)P.most << 32 | 0xffffffffull) + 1ull;
+    unsigned long long lo = (unsigned long long)P.least << 32;
+    unsigned long long hi = ((unsigned long long)P.most << 32 | 0xffffffffull) + 1ull;
     if (hi == 0ull) hi = ~0ull;  // (keys of NaN; 2^64 - 1 itself is token 0's, never short of the bound)
     const int enough = top + top / 4 + 4;
     while (hi - lo > 1ull) {
@@ -733,13 +752,6 @@ __device__ void select_by_pieces(Selection& P, const E* z, int begin, int end, i
     }
 }
 
-// The best tokens of a slice from what the threads met while they summed it.  A thread's
-// key is its best vector, ordered by (largest logit, lower vector number first); a bound
-// that `top` of these keys reach lies below the `top`-th best element.  So only elements at
-// or above it are candidates, about T ln(1 / (1 - top / T)) of them where the tokens lie at
-// random over T threads.  They are read again (from L2) at the threads' best vectors, and
-// in all their vectors only for threads that have a second one to offer.  More candidates
-// than the list holds are left to select_by_pieces.
 // Slices that are ranked whole: the shortest ones, and short ones with hardly a vector for
 // each alternative.
 template <typename E>
@@ -748,6 +760,13 @@ __device__ __forceinline__ bool ranked_whole(const Slice& part, int top) {
     return tokens <= 96 || (tokens <= 256 && top * 4 > (part.hi - part.lo) * 3);
 }
 
+// The best tokens of a slice from what the threads met while they summed it.  A thread's
+// key is its best vector, ordered by (largest logit, lower vector number first); a bound
+// that `top` of these keys reach lies below the `top`-th best element.  So only elements at
+// or above it are candidates, about T ln(1 / (1 - top / T)) of them where the tokens lie at
+// random over T threads.  They are read again (from L2) at the threads' best vectors, and
+// in all their vectors only for threads that have a second one to offer.  More candidates
+// than the list holds are left to select_by_pieces.
 template <typename E>
 __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& part, const E* z, int top,
                                   const Running<true>& acc, int cap) {
@@ -919,7 +938,8 @@ __device__ __forceinline__ void dense_vector(float* v, const Dense& d, float L) 
 }
 
 __device__ __forceinline__ void store16(void* p, uint4 w) {
-    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w) : "memory");
+    asm volatile("st.global.cs.v4.u32 [%0], {%1, %2, %3, %4};" ::"l"(p), "r"(w.x), "r"(w.y), "r"(w.z), "r"(w.w)
+                 : "memory");
 }
 
 // The dense gradient of a slice into `out` (the row's first element) by T threads.  `out`
@@ -1109,9 +1129,15 @@ __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logi
 }
 
 // Loss and statistics of rows that stream through registers, without their listed
-// elements, which have their own sums; with kGradient the row is then read again, from L2,
-// for its gradient.  A cluster of blocks shares a row: they exchange their sums (with
-// kGradient each takes the list for itself, else the first one).
+// elements, which have their own sums; with kGradient the row is then read again for its
+// gradient.  A cluster of blocks shares a row: they exchange their sums (with kGradient
+// each takes the list for itself, else the first one).
+//
+// With the gradient the logits cross HBM twice: the rows in flight (135 MB of 151936 bf16)
+// outlive neither L2 partition.  Keeping the slices in shared memory reads them once, but
+// clusters of 8 then move in lockstep and its 190 KB an SM bound the rows in flight: 315 us
+// against 332.  Passes over groups of rows that fit L2 (16 to 100 MB) cost 438 to 719 us:
+// each pair of launches adds its ramps.
 template <typename E, bool kTail, bool kGradient, int T>
 __global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
@@ -1370,7 +1396,6 @@ cudaError_t by_kind(lsx_dtype kind, F&& f) {
     }
 }
 
-
 // How many blocks share a row: as many as fill the GPU, while each keeps `least` vectors.
 int row_parts(int sm_count, size_t rows, size_t vectors, int least, int resident) {
     int parts = 1;
@@ -1412,12 +1437,16 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
         const Scale k(z.temperature);
-        // few alternatives of a short row: smaller blocks leave more rows on an SM
+        // few alternatives of a short row: smaller blocks leave more rows on an SM (750 x 253 f32
+        // with 8: 7.6 us against 12.1)
         if (vectors < 1024 && (alternatives <= 24 || vectors <= 128))
             return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
-        // every block of a cluster selects all the alternatives of its slice: many of them pay in longer slices only
-        const int parts = row_parts(sm_count, z.rows, vectors, alternatives <= 24 ? 256 : 1024, 4);
+        // A row is shared in slices of 1024 vectors or more, and from 4096 on: under that the
+        // cluster's exchange costs more than the shorter slice saves (a row of 32000 bf16 with 20
+        // alternatives 8.5 us whole, 10.1 halved; 64 rows of 8000 f32 7.9 whole, 9.7 in eighths; a
+        // row of 16384 f32 4.1 in quarters, 4.7 halved).
+        const int parts = vectors < 4096 ? 1 : row_parts(sm_count, z.rows, vectors, 1024, 4);
         return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, parts, 256, s, (const E*)z.data, (int)z.vocab,
                                z.stride, k, tokens, (int)token_count, (int)alternatives, out);
     });
@@ -1451,11 +1480,12 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
             return gradient ? (teacher.stats ? distill_kernel<E, true, true, T> : distill_kernel<E, false, true, T>)
                             : (teacher.stats ? distill_kernel<E, true, false, T> : distill_kernel<E, false, false, T>);
         };
-        const bool brief = vectors < (size_t)kBriefVectors;  // smaller blocks leave more short rows on an SM
-        auto kernel = brief ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, kRowThreads>());
-        return launch_clusters(kernel, z.rows, parts, brief ? 128 : kRowThreads, s, (const E*)z.data, (int)z.vocab, z.stride,
-                               Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats, (E*)gradient,
-                               gradient_stride);
+        const bool brief = vectors < (size_t)kBriefVectors;
+        auto kernel =
+            brief ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, kRowThreads>());
+        return launch_clusters(kernel, z.rows, parts, brief ? 128 : kRowThreads, s, (const E*)z.data, (int)z.vocab,
+                               z.stride, Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats,
+                               (E*)gradient, gradient_stride);
     });
 }
 
@@ -1493,7 +1523,8 @@ int check_gradient(const LogitRows& z, const void* gradient, size_t stride) {
     const uintptr_t a = reinterpret_cast<uintptr_t>(z.data), b = reinterpret_cast<uintptr_t>(gradient);
     LSX_ENSURE(b % e == 0, "the gradient is not aligned to its type");
     if (a == b && stride == z.stride) return LSX_OK;
-    const uintptr_t a_end = a + ((z.rows - 1) * z.stride + z.vocab) * e, b_end = b + ((z.rows - 1) * stride + z.vocab) * e;
+    const uintptr_t a_end = a + ((z.rows - 1) * z.stride + z.vocab) * e;
+    const uintptr_t b_end = b + ((z.rows - 1) * stride + z.vocab) * e;
     if (a_end <= b || b_end <= a) return LSX_OK;
     // two column blocks of one buffer
     if (stride == z.stride) {
@@ -1542,7 +1573,8 @@ int lsx_token_logprobs_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, 
 int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind, size_t rows, size_t vocab,
                                        size_t stride, double temperature, const uint32_t* tokens, size_t token_count,
                                        const float* stats, const float* entropy, const float* logprob_gradient,
-                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride, void* stream) {
+                                       const float* entropy_gradient, void* gradient_out, size_t gradient_stride,
+                                       void* stream) {
     const LogitRows z{logits, kind, rows, vocab, stride, temperature};
     LSX_TRY(check_rows(z));
     LSX_TRY(check_gradient(z, gradient_out, gradient_stride));
