@@ -17,7 +17,7 @@
 //
 // Measured on B200 (6552 GB/s measured copy, a pass among others): log probabilities with 8
 // alternatives of 2048 x 151936 f32 191 us (99% of the copy's rate), with 20 of one row
-// 9.8 us, with 50 of 777 x 50257 f16 37 us (32%: the rows of an SM select at the same
+// 9.8 us, with 50 of 777 x 50257 f16 33 us (36%: the rows of an SM select at the same
 // time); their gradient, 2048 x 151936 bf16, 190 us (100%); a loss of 512 x 151936 f32 with 20
 // listed tokens 58 us (81%); loss and gradient of 2048 x 151936 bf16 332 us (57%: the logits
 // are read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
@@ -840,9 +840,9 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
 // and rank their slices and send sums and best keys to the first one's shared memory,
 // which puts them together and writes the row's results.
 template <typename E, int T>
-__global__ void __launch_bounds__(T, 1280 / T) token_logprobs_kernel(const E* __restrict__ logits, int vocab, size_t stride,
-                                                          const Scale k, const uint32_t* __restrict__ tokens,
-                                                          int token_count, int top, LogprobOutputs out) {
+__global__ void __launch_bounds__(T, T <= 128 ? 10 : T <= 192 ? 7 : T <= 224 ? 6 : 5) token_logprobs_kernel(
+    const E* __restrict__ logits, int vocab, size_t stride, const Scale k, const uint32_t* __restrict__ tokens,
+    int token_count, int top, LogprobOutputs out) {
     __shared__ Sums scratch[33];
     __shared__ Partial shares[kMaxCluster];
     __shared__ Selection selection;
@@ -1437,18 +1437,28 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
         const Scale k(z.temperature);
+        auto launch = [&](auto threads, int parts) {
+            constexpr int T = decltype(threads)::value;
+            return launch_clusters(token_logprobs_kernel<E, T>, z.rows, parts, T, s, (const E*)z.data, (int)z.vocab,
+                                   z.stride, k, tokens, (int)token_count, (int)alternatives, out);
+        };
         // few alternatives of a short row: smaller blocks leave more rows on an SM (750 x 253 f32
         // with 8: 7.6 us against 12.1)
         if (vectors < 1024 && (alternatives <= 24 || vectors <= 128))
-            return launch_clusters(token_logprobs_kernel<E, 128>, z.rows, 1, 128, s, (const E*)z.data, (int)z.vocab,
-                                   z.stride, k, tokens, (int)token_count, (int)alternatives, out);
+            return launch(std::integral_constant<int, 128>(), 1);
+        // Rows that just miss being resident all at once get narrower blocks instead of a second
+        // wave (780 x 128256 f32 with 20 alternatives 74 us in blocks of 224, 89 of 256; 1000 x
+        // 32000 bf16 with 8 22 us in blocks of 192, 25 of 256).  With more waves the widest are
+        // the fastest (2048 x 151936 f32 with 8: 191 us of 256, 205 of 224).
+        const size_t blocks = z.rows, sms = (size_t)sm_count;
+        if (blocks > sms * 5 && blocks <= sms * 6) return launch(std::integral_constant<int, 224>(), 1);
+        if (blocks > sms * 6 && blocks <= sms * 7) return launch(std::integral_constant<int, 192>(), 1);
         // A row is shared in slices of 1024 vectors or more, and from 4096 on: under that the
         // cluster's exchange costs more than the shorter slice saves (a row of 32000 bf16 with 20
         // alternatives 8.5 us whole, 10.1 halved; 64 rows of 8000 f32 7.9 whole, 9.7 in eighths; a
         // row of 16384 f32 4.1 in quarters, 4.7 halved).
         const int parts = vectors < 4096 ? 1 : row_parts(sm_count, z.rows, vectors, 1024, 4);
-        return launch_clusters(token_logprobs_kernel<E, 256>, z.rows, parts, 256, s, (const E*)z.data, (int)z.vocab,
-                               z.stride, k, tokens, (int)token_count, (int)alternatives, out);
+        return launch(std::integral_constant<int, 256>(), parts);
     });
 }
 

@@ -766,3 +766,23 @@ def test_distill_bad_slot_in_an_empty_row(gpu, dev):
     for grad in (got.gradient, back):
         assert bool(grad[0].isnan().all()) and not bool(grad[1].any())
     assert bool(got.loss[0].isnan()) and float(got.loss[1]) == math.inf
+
+
+@pytest.mark.parametrize("rows", [741, 888, 889, 1036, 1037])
+@pytest.mark.parametrize("dtype", KINDS)
+def test_logprobs_of_a_full_wave(gpu, dev, dtype, rows):
+    """Numbers of rows around what a GPU of 148 SMs holds at once, masked in different measure,
+    with rows of one token, of none and of ties."""
+    for vocab, k in ((4102, 3), (9001, 128)):
+        z = make(dev, rows + k, rows, vocab, dtype, 1, masked=0.9)
+        z[::7] = -math.inf
+        z[::14, 11] = 1.5
+        z[1::7, ::2] = 3.0
+        z[2::7] = torch.linspace(-9, 9, vocab).to(dtype).to(dev)
+        z[3::7] = torch.finfo(dtype).min
+        tokens = torch.randint(-1, vocab, (rows, 2), dtype=torch.int32, device=dev)
+        check_logprobs(gpu, z, tokens, k, 0.9)
+        z[5, 100] = math.nan
+        got = distribution.token_logprobs(gpu, z, tokens, alternatives=k)
+        assert bool(got.entropy[5].isnan()) and not bool(got.entropy[6:].isnan().any())
+        assert torch.equal(got.top_ids.long(), order64(z, k))
