@@ -38,10 +38,16 @@ namespace {
 constexpr int kRowThreads = 256;     // 5 or 6 such blocks on an SM: 512 or 1024 threads overlap a row's steps less
 constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;       // candidate keys of one selection
-// Loss and gradient in one kernel read a slice twice.  A slice is at most this many vectors
-// (two blocks for a row of 151936 bf16): 1, 2, 4 and 8 blocks a row measured 342, 333, 366
-// and 444 us on 2048 of them; 190 rows of 128003 f32 69 us whole, 63 in quarters.
+// Loss and gradient in one kernel take a slice twice.  Longer ones pass through shared
+// memory (Stage): kStagedBlocks blocks of kStagedThreads threads on an SM, kPlaces chunks of
+// kChunk vectors a thread.  A slice is at most kAgainVectors (two blocks for a row of 151936
+// bf16), so that what does not stay there can stay in L2.
+constexpr int kStagedThreads = 256;
+constexpr int kStagedBlocks = 4;
+constexpr int kPlaces = 3;
+constexpr int kChunk = 3;
 constexpr int kAgainVectors = 10000;
+constexpr int kStagedVectors = 1024;
 // Slices of the gradient kernels: 1200, 2048 and 3000 vectors measured 201, 190 and 196 us on
 // 2048 x 151936 bf16.
 constexpr int kPieceVectors = 2048;
@@ -351,11 +357,12 @@ __device__ __forceinline__ Sums block_sums(const Running<kRanked>& a, float L, S
     return warp_sums(x, x.m, L);
 }
 
-// `begun` is called once, when the first loads are on their way.
-template <typename E, bool kExclude, bool kRanked, typename F>
+// `stage` is a Stage or nullptr; `begun` is called once, when the first loads are on their way.
+template <typename E, bool kExclude, bool kRanked, typename S, typename F>
 __device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& part, Marks* M, int count, const Scale& k,
-                                             Running<kRanked>& acc, F&& begun) {
+                                             Running<kRanked>& acc, const S& stage, F&& begun) {
     constexpr int n = Vec<E>::n;
+    constexpr bool kStaged = !std::is_same_v<S, std::nullptr_t>;
     auto add = [&](const float* v, int j) {
         float top = v[0];
 #pragma unroll
@@ -382,6 +389,14 @@ __device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& par
         add(v, j);
     };
     const int tid = threadIdx.x, T = blockDim.x;
+    if constexpr (kStaged) {
+        stage.begin();
+        begun();
+        if (part.head && tid == 0) take_ragged(0);
+        stage.read(take);
+        if (part.last && tid == T - 1) take_ragged(row.full1);
+        return;
+    }
     int j = part.lo + tid;
     uint4 w[kUnroll];
     bool whole = j + (kUnroll - 1) * T < part.hi;
@@ -412,6 +427,105 @@ __device__ __forceinline__ void stream_slice(const Row<E>& row, const Slice& par
     for (; j < part.hi; j += T) take(j, row.full(j));
     if (part.last && tid == T - 1) take_ragged(row.full1);
 }
+
+// ---- staged slices ----------------------------------------------------------------------
+// Copies of 16 bytes into shared memory that the copying thread alone waits for.  `keep`
+// marks what is read from global memory once more.
+__device__ __forceinline__ void copy16(uint4* shared, const void* global, bool keep) {
+    uint64_t kept, passing;
+    asm("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(kept));
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(passing));
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(
+                     (uint32_t)__cvta_generic_to_shared(shared)),
+                 "l"(global), "l"(keep ? kept : passing)
+                 : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// Until at most n of the thread's groups are under way.
+template <int n>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(n) : "memory");
+}
+
+// A slice that is taken twice, in chunks of kChunk vectors a thread, each thread for itself.
+// Three places in shared memory hold a chunk each: the first chunk stays in the first, the
+// others pass through the second and third in turn, where the last two stay.  So three
+// chunks are read from global memory once, the others twice.
+template <typename E, int T>
+struct Stage {
+    uint4* places;
+    const Row<E>& row;
+    int first, hi, chunks;
+    __device__ __forceinline__ Stage(uint4* shared, const Row<E>& row_, const Slice& part)
+        : places(shared + threadIdx.x), row(row_), first(part.lo + (int)threadIdx.x), hi(part.hi) {
+        chunks = first < hi ? (hi - first + T * kChunk - 1) / (T * kChunk) : 0;
+    }
+    __device__ __forceinline__ static int place(int chunk) { return chunk == 0 ? 0 : 1 + ((chunk - 1) & 1); }
+    // one group of copies, empty past the last chunk
+    __device__ __forceinline__ void start(int chunk, int at, bool keep) const {
+        if (chunk < chunks) {
+#pragma unroll
+            for (int u = 0; u < kChunk; ++u) {
+                const int j = first + (chunk * kChunk + u) * T;
+                if (j < hi) copy16(places + (at * kChunk + u) * T, row.base + (long long)j * Vec<E>::n, keep);
+            }
+        }
+        copies_commit();
+    }
+    template <typename F>
+    __device__ __forceinline__ void each(int chunk, int at, F&& take) const {
+        uint4 w[kChunk];
+#pragma unroll
+        for (int u = 0; u < kChunk; ++u) w[u] = places[(at * kChunk + u) * T];
+#pragma unroll
+        for (int u = 0; u < kChunk; ++u) {
+            const int j = first + (chunk * kChunk + u) * T;
+            if (j < hi) take(j, w[u]);
+        }
+    }
+    __device__ __forceinline__ bool passes(int chunk) const { return chunk > 0 && chunk < chunks - 2; }
+    __device__ __forceinline__ void begin() const {
+        for (int c = 0; c < kPlaces; ++c) start(c, c, passes(c));
+    }
+    template <typename F>
+    __device__ __forceinline__ void read(F&& take) const {
+        for (int c = 0; c < chunks; ++c) {
+            if (c == 0) {
+                copies_wait<2>();
+                each(0, 0, take);
+            } else {
+                copies_wait<1>();
+                each(c, place(c), take);
+                start(c + 2, place(c), passes(c + 2));
+            }
+        }
+        copies_wait<0>();
+    }
+    template <typename F>
+    __device__ __forceinline__ void read_again(F&& take) const {
+        const int again = chunks - kPlaces;  // chunks 1 to `again` come from global memory
+        if (again <= 0) {
+            for (int c = 0; c < chunks; ++c) each(c, c, take);
+            return;
+        }
+        const int second = place(chunks - 2), third = place(chunks - 1);
+        auto next = [&](int chunk, int at) { start(chunk <= again ? chunk : chunks, at, false); };
+        each(0, 0, take);
+        next(1, 0);
+        each(chunks - 2, second, take);
+        next(2, second);
+        each(chunks - 1, third, take);
+        next(3, third);
+        int turn = 0;
+        for (int c = 1; c <= again; ++c) {
+            copies_wait<2>();
+            const int at = turn == 0 ? 0 : turn == 1 ? second : third;
+            each(c, at, take);
+            next(c + 3, at);
+            turn = turn == 2 ? 0 : turn + 1;
+        }
+    }
+};
 
 // The vectors put aside, without their listed elements: thread t takes the one of t-th
 // lowest number, whatever order they came in, so that sums repeat.  Where there are more
@@ -862,7 +976,7 @@ __global__ void __launch_bounds__(T, T <= 128 ? 10 : T <= 192 ? 7 : T <= 224 ? 6
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
     Running<true> acc;
-    stream_slice<E, false>(row, slice, nullptr, 0, k, acc, []() {});
+    stream_slice<E, false>(row, slice, nullptr, 0, k, acc, nullptr, []() {});
     Partial sums = slice_sums(row, slice, acc, k, scratch, &owner);
     // clusters keep the upper half of the list for the blocks' best keys
     const int cap = parts > 1 ? kListCap / 2 : kListCap;
@@ -944,10 +1058,10 @@ __device__ __forceinline__ void store16(void* p, uint4 w) {
 
 // The dense gradient of a slice into `out` (the row's first element) by T threads.  `out`
 // may be the row.  `ready` gives the coefficients, once, after the first loads are on their
-// way.
-template <typename E, bool kLinear, typename F>
+// way.  `stage` is the one that stream_slice read through, or nullptr.
+template <typename E, bool kLinear, typename S, typename F>
 __device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part, E* out, float L, int tid, int T,
-                                            F&& ready) {
+                                            const S& stage, F&& ready) {
     constexpr int n = Vec<E>::n;
     // the output row may lie at another alignment than the logits
     const bool same = (reinterpret_cast<uintptr_t>(out) & 15) == (uintptr_t)(row.lead * sizeof(E));
@@ -974,6 +1088,13 @@ __device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part
             if (i >= 0 && i < row.vocab) out[i] = Vec<E>::store(v[e]);
         }
     };
+    if constexpr (!std::is_same_v<S, std::nullptr_t>) {
+        d = ready();
+        stage.read_again(put);
+        if (part.head && tid == 0) put_ragged(0);
+        if (part.last && tid == T - 1) put_ragged(row.full1);
+        return;
+    }
     int j = part.lo + tid;
     uint4 w[kUnroll];
     auto fetch = [&](int from) {
@@ -1039,9 +1160,9 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) logprobs_
     };
     E* out = gradient + r * gradient_stride;
     if (h != 0.f)
-        write_dense<E, true>(row, slice, out, k.L, tid, kPieceThreads, ready);
+        write_dense<E, true>(row, slice, out, k.L, tid, kPieceThreads, nullptr, ready);
     else
-        write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, ready);
+        write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, nullptr, ready);
     __syncthreads();
     if (id >= (uint32_t)vocab || (int)id < slice.begin || (int)id >= slice.end) return;
     // a token named several times adds up at its first slot
@@ -1133,13 +1254,14 @@ __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logi
 // gradient.  A cluster of blocks shares a row: they exchange their sums (with kGradient
 // each takes the list for itself, else the first one).
 //
-// With the gradient the logits cross HBM twice: the rows in flight (135 MB of 151936 bf16)
-// outlive neither L2 partition.  Keeping the slices in shared memory reads them once, but
-// clusters of 8 then move in lockstep and its 190 KB an SM bound the rows in flight: 315 us
-// against 332.  Passes over groups of rows that fit L2 (16 to 100 MB) cost 438 to 719 us:
-// each pair of launches adds its ramps.
-template <typename E, bool kTail, bool kGradient, int T>
-__global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
+// With the gradient a slice is taken twice, and the rows in flight outlive L2 in part only.
+// 2048 x 151936 bf16 with 64 listed tokens: 333 us with plain loads both times, 298 through
+// shared memory, 283 with L2 told which chunks return (5.3 TB/s if all of them came from HBM again).
+// Whole rows in shared memory, by clusters of 8, move in lockstep: 315 us.  Passes over
+// groups of rows that fit L2 (16 to 100 MB): 438 to 719 us, each pair of launches adds its
+// ramps.
+template <typename E, bool kTail, bool kGradient, int T, bool kStaged>
+__global__ void __launch_bounds__(T, kStaged ? kStagedBlocks : 6 * kRowThreads / T) distill_kernel(
     const E* logits, int vocab, size_t stride, const Scale k, double inverse, TeacherRows teacher,
     const float* __restrict__ weights, float* loss, float* stats, E* gradient, size_t gradient_stride) {
     __shared__ Sums scratch[33];
@@ -1148,6 +1270,7 @@ __global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     __shared__ float tops[kListWarps], highs[kListWarps];
     __shared__ double masses[kListWarps], insides[kListWarps], crosses[kListWarps];
     __shared__ int bad;
+    extern __shared__ uint4 places[];
     const int parts = cluster_size(), part = cluster_rank(), tid = threadIdx.x;
     if (parts > 1) cluster_arrive();  // waited for before the first store into another block
     const size_t r = blockIdx.x / (uint32_t)parts;
@@ -1155,6 +1278,12 @@ __global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     const E* z = logits + r * stride;
     const Row<E> row(z, vocab);
     const Slice slice(row, part, parts);
+    const auto stage = [&]() {
+        if constexpr (kStaged)
+            return Stage<E, T>(places, row, slice);
+        else
+            return nullptr;
+    }();
     const float* saved = kTail ? teacher.stats + 2 * r : nullptr;
     const bool lists = kGradient || part == 0;
     uint32_t id = kUnusedToken;
@@ -1165,7 +1294,7 @@ __global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     }
     bool kept = false;
     Running<false> acc;
-    stream_slice<E, true>(row, slice, &marks, count, k, acc, [&]() {
+    stream_slice<E, true>(row, slice, &marks, count, k, acc, stage, [&]() {
         for (int i = tid; i < kMarkWords; i += T) marks.bits[i] = 0;
         if (tid == 0) marks.asides = bad = 0;
         if (tid < kMaxSlots) marks.ids[tid] = id < (uint32_t)vocab ? id : kUnusedToken;
@@ -1298,7 +1427,7 @@ __global__ void __launch_bounds__(T, 6 * kRowThreads / T) distill_kernel(
     const double weight = weights ? (double)weights[r] * inverse : inverse;
     DistillRow g;
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, out, k.L, tid, T, [&]() {
+    write_dense<E, false>(row, slice, out, k.L, tid, T, stage, [&]() {
         if (parts > 1) cluster_wait();
         put_together();
         const float P = kTail ? (float)mass : mass == 0.0 ? 0.f : mass == mass ? 1.f : NAN;
@@ -1353,7 +1482,7 @@ __global__ void __launch_bounds__(kPieceThreads, 1024 / kPieceThreads) distill_g
         return all;
     };
     E* out = gradient + r * gradient_stride;
-    write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, [&]() {
+    write_dense<E, false>(row, slice, out, k.L, tid, kPieceThreads, nullptr, [&]() {
         ids[tid] = id < (uint32_t)vocab ? id : kUnusedToken;
         const bool bad = __syncthreads_or(id != kUnusedToken && id >= (uint32_t)vocab) != 0;
         kept = id < (uint32_t)vocab && !named_before(ids, tid);
@@ -1406,12 +1535,13 @@ int row_parts(int sm_count, size_t rows, size_t vectors, int least, int resident
 }
 
 template <typename... Params, typename... Args>
-cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, cudaStream_t s,
-                            Args... args) {
+cudaError_t launch_clusters(void (*kernel)(Params...), size_t rows, int parts, int threads, size_t shared,
+                            cudaStream_t s, Args... args) {
     if (rows * parts > 2147483647ull) return cudaErrorInvalidConfiguration;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(rows * parts));
     cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1439,7 +1569,7 @@ cudaError_t launch_token_logprobs(cudaStream_t s, int sm_count, const LogitRows&
         const Scale k(z.temperature);
         auto launch = [&](auto threads, int parts) {
             constexpr int T = decltype(threads)::value;
-            return launch_clusters(token_logprobs_kernel<E, T>, z.rows, parts, T, s, (const E*)z.data, (int)z.vocab,
+            return launch_clusters(token_logprobs_kernel<E, T>, z.rows, parts, T, 0, s, (const E*)z.data, (int)z.vocab,
                                    z.stride, k, tokens, (int)token_count, (int)alternatives, out);
         };
         // few alternatives of a short row: smaller blocks leave more rows on an SM (750 x 253 f32
@@ -1487,15 +1617,21 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
             while (parts < kMaxCluster && vectors / parts > (size_t)kAgainVectors) parts *= 2;
         auto pick = [&](auto threads) {
             constexpr int T = decltype(threads)::value;
-            return gradient ? (teacher.stats ? distill_kernel<E, true, true, T> : distill_kernel<E, false, true, T>)
-                            : (teacher.stats ? distill_kernel<E, true, false, T> : distill_kernel<E, false, false, T>);
+            return gradient ? (teacher.stats ? distill_kernel<E, true, true, T, false> : distill_kernel<E, false, true, T, false>)
+                            : (teacher.stats ? distill_kernel<E, true, false, T, false> : distill_kernel<E, false, false, T, false>);
         };
         const bool brief = vectors < (size_t)kBriefVectors;
+        const bool staged = gradient && vectors / parts >= (size_t)kStagedVectors;
         auto kernel =
             brief ? pick(std::integral_constant<int, 128>()) : pick(std::integral_constant<int, kRowThreads>());
-        return launch_clusters(kernel, z.rows, parts, brief ? 128 : kRowThreads, s, (const E*)z.data, (int)z.vocab,
-                               z.stride, Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats,
-                               (E*)gradient, gradient_stride);
+        if (staged)
+            kernel = teacher.stats ? distill_kernel<E, true, true, kStagedThreads, true>
+                                   : distill_kernel<E, false, true, kStagedThreads, true>;
+        const int threads = staged ? kStagedThreads : brief ? 128 : kRowThreads;
+        const size_t shared = staged ? (size_t)kPlaces * kChunk * kStagedThreads * sizeof(uint4) : 0;
+        return launch_clusters(kernel, z.rows, parts, threads, shared, s, (const E*)z.data, (int)z.vocab, z.stride,
+                               Scale(z.temperature), 1.0 / z.temperature, teacher, weights, loss, stats, (E*)gradient,
+                               gradient_stride);
     });
 }
 
