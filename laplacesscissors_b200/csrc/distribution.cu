@@ -38,10 +38,15 @@ namespace {
 constexpr int kRowThreads = 256;     // 5 or 6 such blocks on an SM: 512 or 1024 threads overlap a row's steps less
 constexpr int kPieceThreads = 128;   // of the gradient kernels
 constexpr int kListCap = 2048;       // candidate keys of one selection
-// Loss and gradient in one kernel take a slice twice.  Longer ones pass through shared
-// memory (Stage): kStagedBlocks blocks of kStagedThreads threads on an SM, kPlaces chunks of
-// kChunk vectors a thread.  A slice is at most kAgainVectors (two blocks for a row of 151936
-// bf16), so that what does not stay there can stay in L2.
+// Loss and gradient in one kernel take a slice twice.  From kStagedVectors on it passes
+// through shared memory (Stage): kStagedBlocks blocks of kStagedThreads threads on an SM,
+// kPlaces chunks of kChunk vectors a thread, 36 KB.  Of 2048 x 151936 bf16, 1000 x 50257 f16:
+// 285 and 57 us so, 299 and 62 with 5 blocks of chunks of 2, 304 and 69 with 3 blocks of 384,
+// 308 and 56 with 8 of 128.  100 x 32000 f32 (slices of 2000): 12.7 us staged, 16.1 not;
+// shorter ones are alike.
+// A slice is at most kAgainVectors (two blocks for a row of 151936 bf16), so that what does
+// not stay in shared memory can stay in L2: 2048 of these rows whole 306 us, halved 285, in
+// quarters 356.
 constexpr int kStagedThreads = 256;
 constexpr int kStagedBlocks = 4;
 constexpr int kPlaces = 3;
@@ -1613,8 +1618,13 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
         int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
-        if (gradient)  // the rows in flight have to stay in L2 until they are read again
+        if (gradient && vectors / parts > (size_t)kAgainVectors) {
             while (parts < kMaxCluster && vectors / parts > (size_t)kAgainVectors) parts *= 2;
+            // hardly more blocks than the SMs hold would leave them a second wave for a few (400 x
+            // 151936 bf16: 73 us halved, 67 whole; 500 rows of them 80 halved, 86 whole)
+            const size_t blocks = z.rows * parts, held = (size_t)sm_count * kStagedBlocks;
+            if (blocks > held && blocks * 2 <= held * 3) parts /= 2;
+        }
         auto pick = [&](auto threads) {
             constexpr int T = decltype(threads)::value;
             return gradient ? (teacher.stats ? distill_kernel<E, true, true, T, false> : distill_kernel<E, false, true, T, false>)

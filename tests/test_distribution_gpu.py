@@ -786,3 +786,25 @@ def test_logprobs_of_a_full_wave(gpu, dev, dtype, rows):
         got = distribution.token_logprobs(gpu, z, tokens, alternatives=k)
         assert bool(got.entropy[5].isnan()) and not bool(got.entropy[6:].isnan().any())
         assert torch.equal(got.top_ids.long(), order64(z, k))
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", KINDS)
+def test_distill_step_of_long_rows(gpu, dev, dtype, tail):
+    """Slices of one to many chunks a thread, in numbers of rows that take one to eight blocks
+    each; results repeat bit for bit, in place too."""
+    n = 16 // torch.empty(0, dtype=dtype).element_size()
+    for vectors, rows in ((1024, 600), (1025, 33), (2303, 600), (2305, 593), (3500, 593), (9999, 160), (20001, 3),
+                          (20003, 170)):
+        vocab = vectors * n + vectors % 3
+        z = make(dev, vectors, rows, vocab, dtype, n if vectors % 2 else 1, masked=0.2)
+        ids, values, stats = teacher_of(dev, rows, z, 128 if vectors % 2 else 20, 1.4, unused=0.1)
+        if not tail:
+            stats = None
+        weights = torch.rand(rows, device=dev) + 0.25
+        got = check_distill(gpu, z, ids, values, stats, weights, 1.4)
+        again = distribution.distill(gpu, z, ids, values, teacher_stats=stats, weights=weights, temperature=1.4,
+                                     gradient=True, out=(torch.empty_like(got.loss), torch.empty_like(got.stats), z))
+        assert again.gradient.data_ptr() == z.data_ptr()
+        assert torch.equal(got.loss, again.loss) and torch.equal(got.stats, again.stats)
+        assert torch.equal(got.gradient, again.gradient)
