@@ -19,8 +19,8 @@
 // alternatives of 2048 x 151936 f32 191 us (99% of the copy's rate), with 20 of one row
 // 9.8 us, with 50 of 777 x 50257 f16 33 us (36%: the rows of an SM select at the same
 // time); their gradient, 2048 x 151936 bf16, 190 us (100%); a loss of 512 x 151936 f32 with 20
-// listed tokens 58 us (81%); loss and gradient of 2048 x 151936 bf16 332 us (57%: the logits
-// are read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
+// listed tokens 58 us (82%); loss and gradient of 2048 x 151936 bf16 with 64 285 us (67%: most
+// of a row is read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -1530,7 +1530,9 @@ cudaError_t by_kind(lsx_dtype kind, F&& f) {
     }
 }
 
-// How many blocks share a row: as many as fill the GPU, while each keeps `least` vectors.
+// How many blocks share a row: as many as leave `resident` blocks to an SM, while each keeps
+// `least` vectors.  4 measured best where nothing is read twice (512 x 151936 f32, 20 listed
+// tokens: 58 us at 4, 70 at 8, 66 at 16).
 int row_parts(int sm_count, size_t rows, size_t vectors, int least, int resident) {
     int parts = 1;
     while (parts < kMaxCluster && rows * parts * 2 <= (size_t)sm_count * resident &&
@@ -1617,7 +1619,10 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
     return by_kind(z.kind, [&](auto* e) {
         using E = std::remove_cv_t<std::remove_pointer_t<decltype(e)>>;
         const size_t vectors = z.vocab / Vec<E>::n;
-        int parts = row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
+        // With the gradient 3 blocks an SM are faster than 4, and slices of 256 no faster than of
+        // 1024 (148 x 151936 bf16 32 us against 40; 60 x 50257 f16 14 us against 16).
+        int parts = gradient ? row_parts(sm_count, z.rows, vectors, 1024, 3)
+                             : row_parts(sm_count, z.rows, vectors, kRowThreads, 4);
         if (gradient && vectors / parts > (size_t)kAgainVectors) {
             while (parts < kMaxCluster && vectors / parts > (size_t)kAgainVectors) parts *= 2;
             // hardly more blocks than the SMs hold would leave them a second wave for a few (400 x
