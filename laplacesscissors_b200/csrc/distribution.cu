@@ -1261,7 +1261,7 @@ __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logi
 //
 // With the gradient a slice is taken twice, and the rows in flight outlive L2 in part only.
 // 2048 x 151936 bf16 with 64 listed tokens: 333 us with plain loads both times, 298 through
-// shared memory, 283 with L2 told which chunks return (5.3 TB/s if all of them came from HBM again).
+// shared memory, 283 with L2 told which chunks return.
 // Whole rows in shared memory, by clusters of 8, move in lockstep: 315 us.  Passes over
 // groups of rows that fit L2 (16 to 100 MB): 438 to 719 us, each pair of launches adds its
 // ramps.
