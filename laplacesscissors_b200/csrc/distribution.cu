@@ -19,7 +19,7 @@
 // alternatives of 2048 x 151936 f32 191 us (99% of the copy's rate), with 20 of one row
 // 9.8 us, with 50 of 777 x 50257 f16 33 us (36%: the rows of an SM select at the same
 // time); their gradient, 2048 x 151936 bf16, 190 us (100%); a loss of 512 x 151936 f32 with 20
-// listed tokens 58 us (82%); loss and gradient of 2048 x 151936 bf16 with 64 285 us (67%: most
+// listed tokens 58 us (82%); loss and gradient of 2048 x 151936 bf16 with 64 277 us (69%: most
 // of a row is read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -466,15 +466,25 @@ struct Stage {
         chunks = first < hi ? (hi - first + T * kChunk - 1) / (T * kChunk) : 0;
     }
     __device__ __forceinline__ static int place(int chunk) { return chunk == 0 ? 0 : 1 + ((chunk - 1) & 1); }
+    // Every chunk but a thread's last is whole and needs no bounds (2048 x 151936 bf16 277 us
+    // against 285).
+    template <typename F>
+    __device__ __forceinline__ void vectors(int chunk, F&& f) const {
+        const int j = first + chunk * kChunk * T;
+        if (j + (kChunk - 1) * T < hi) {
+#pragma unroll
+            for (int u = 0; u < kChunk; ++u) f(j + u * T, u);
+        } else if (chunk < chunks) {
+#pragma unroll
+            for (int u = 0; u < kChunk; ++u)
+                if (j + u * T < hi) f(j + u * T, u);
+        }
+    }
     // one group of copies, empty past the last chunk
     __device__ __forceinline__ void start(int chunk, int at, bool keep) const {
-        if (chunk < chunks) {
-#pragma unroll
-            for (int u = 0; u < kChunk; ++u) {
-                const int j = first + (chunk * kChunk + u) * T;
-                if (j < hi) copy16(places + (at * kChunk + u) * T, row.base + (long long)j * Vec<E>::n, keep);
-            }
-        }
+        vectors(chunk, [&](int j, int u) {
+            copy16(places + (at * kChunk + u) * T, row.base + (long long)j * Vec<E>::n, keep);
+        });
         copies_commit();
     }
     template <typename F>
@@ -482,11 +492,7 @@ struct Stage {
         uint4 w[kChunk];
 #pragma unroll
         for (int u = 0; u < kChunk; ++u) w[u] = places[(at * kChunk + u) * T];
-#pragma unroll
-        for (int u = 0; u < kChunk; ++u) {
-            const int j = first + (chunk * kChunk + u) * T;
-            if (j < hi) take(j, w[u]);
-        }
+        vectors(chunk, [&](int j, int u) { take(j, w[u]); });
     }
     __device__ __forceinline__ bool passes(int chunk) const { return chunk > 0 && chunk < chunks - 2; }
     __device__ __forceinline__ void begin() const {
@@ -1261,7 +1267,7 @@ __device__ __forceinline__ float listed_gradient(const DistillRow& g, float logi
 //
 // With the gradient a slice is taken twice, and the rows in flight outlive L2 in part only.
 // 2048 x 151936 bf16 with 64 listed tokens: 333 us with plain loads both times, 298 through
-// shared memory, 283 with L2 told which chunks return.
+// shared memory, 285 with L2 told which chunks return, 277 with bounds for the last chunk only.
 // Whole rows in shared memory, by clusters of 8, move in lockstep: 315 us.  Passes over
 // groups of rows that fit L2 (16 to 100 MB): 438 to 719 us, each pair of launches adds its
 // ramps.
@@ -1632,8 +1638,9 @@ cudaError_t launch_distill(cudaStream_t s, int sm_count, const LogitRows& z, con
         }
         auto pick = [&](auto threads) {
             constexpr int T = decltype(threads)::value;
-            return gradient ? (teacher.stats ? distill_kernel<E, true, true, T, false> : distill_kernel<E, false, true, T, false>)
-                            : (teacher.stats ? distill_kernel<E, true, false, T, false> : distill_kernel<E, false, false, T, false>);
+            if (gradient)
+                return teacher.stats ? distill_kernel<E, true, true, T, false> : distill_kernel<E, false, true, T, false>;
+            return teacher.stats ? distill_kernel<E, true, false, T, false> : distill_kernel<E, false, false, T, false>;
         };
         const bool brief = vectors < (size_t)kBriefVectors;
         const bool staged = gradient && vectors / parts >= (size_t)kStagedVectors;

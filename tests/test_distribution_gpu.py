@@ -808,3 +808,29 @@ def test_distill_step_of_long_rows(gpu, dev, dtype, tail):
         assert again.gradient.data_ptr() == z.data_ptr()
         assert torch.equal(got.loss, again.loss) and torch.equal(got.stats, again.stats)
         assert torch.equal(got.gradient, again.gradient)
+
+
+def test_two_captured_steps_of_long_rows_at_once(gpu, dev):
+    """Two graphs of steps over long rows, replayed on two streams at the same time, give what each
+    gives alone."""
+    graphs, wanted, held = [], [], []
+    for i, (rows, vocab, dtype) in enumerate([(250, 40003, torch.bfloat16), (90, 70001, torch.float32)]):
+        z = make(dev, i, rows, vocab, dtype)
+        ids, values, stats = teacher_of(dev, i, z, 24, 1.0)
+        alone = distribution.distill(gpu, z, ids, values, teacher_stats=stats, gradient=True)
+        out = (torch.empty_like(alone.loss), torch.empty_like(alone.stats), torch.empty_like(alone.gradient))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            distribution.distill(gpu, z, ids, values, teacher_stats=stats, gradient=True, out=out)
+        graphs.append((graph, torch.cuda.Stream(dev)))
+        wanted.append(alone)
+        held.append((z, ids, values, stats, out))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for graph, stream in graphs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for alone, (*_, out) in zip(wanted, held):
+        for a, b in zip((alone.loss, alone.stats, alone.gradient), out):
+            assert torch.equal(a, b)
