@@ -1222,9 +1222,11 @@ __device__ __forceinline__ double teacher_rest(double mass, const float* saved) 
     return mass < 1.0 ? 1.0 - mass : (mass >= 1.0 ? 0.0 : mass);
 }
 
-// The tokens outside the list are one outcome only where the student's share of them is
-// a normal f32 number (2^-126 and up).
-constexpr float kSmallestLogShare = -87.33654475f;
+// The tokens outside the list are one outcome where the student's share q_r of them is more
+// than 0 in 64 bits (2^-1074 and up): below that they are masked, with -inf or a type's lowest
+// value.  Neither the loss nor the gradient needs q_r itself: ln q_r is a difference of
+// logarithms and q_i / q_r an exponential of one, both in range however small q_r is.
+constexpr float kSmallestLogShare = -744.44007f;
 
 // What a row's gradient needs beside its list: listed elements get q a - value, q against
 // `offset`; the others are exponentiated against their own sum: 2^y = q_i / q_r stays in
