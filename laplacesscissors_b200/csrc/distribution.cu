@@ -75,6 +75,11 @@ struct Scale {
     float slack;    // kSlack powers of two as a difference of logits
     explicit Scale(double temperature)
         : L((float)(1.4426950408889634 / temperature)), inverse((float)(1.0 / temperature)), slack(kSlack / L) {}
+    // (a - b) / T.  The lowest value of f32 or bf16 is further from large logits than f32 reaches,
+    // which halves are not (exponents need no such care: theirs is 0 long before).
+    __device__ __forceinline__ float between(float a, float b) const {
+        return fmaf(0.5f, a, -0.5f * b) * (2.f * inverse);
+    }
 };
 
 // ---- 16 bytes of logits ------------------------------------------------------
@@ -1017,7 +1022,7 @@ __global__ void __launch_bounds__(T, T <= 128 ? 10 : T <= 192 ? 7 : T <= 224 ? 6
     }
     const bool empty = !sums.any;  // every logit is -inf
     const float m = sums.m, log_sum = empty ? 0.f : log1pf(sums.rest);
-    auto logprob = [&](float x) { return empty ? -INFINITY : (x - m) * k.inverse - log_sum; };
+    auto logprob = [&](float x) { return empty ? -INFINITY : k.between(x, m) - log_sum; };
     if (threadIdx.x == 0) {
         if (out.entropy) out.entropy[r] = empty ? 0.f : log_sum - sums.W / (1.f + sums.rest) * kLn2;
         if (out.stats) {
@@ -1386,7 +1391,7 @@ __global__ void __launch_bounds__(T, kStaged ? kStagedBlocks : 6 * kRowThreads /
         m = fmaxf(rest.m, high);
         const bool some = rest.S != 0.f, listed = inside != 0.0;
         empty = !some && !listed;
-        const float below = some ? (rest.m - m) * k.inverse : -INFINITY;
+        const float below = some ? k.between(rest.m, m) : -INFINITY;
         const float outside = some ? rest.S * expf(below) : 0.f;
         const float over = high == m ? (float)(inside - 1.0) + outside
                                      : (listed ? (float)inside * expf((high - m) * k.inverse) : 0.f) + (outside - 1.f);

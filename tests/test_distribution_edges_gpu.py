@@ -1,6 +1,7 @@
 """Edges of the operators on rows of logits (laplacesscissors_b200/distribution.py): a student
-whose share of the tokens outside the teacher's list is next to nothing.  The references compute
-from the definitions in 64 bits, in logarithms where 64 bits would leave nothing of a share."""
+whose share of the tokens outside the teacher's list is next to nothing, and logits whose
+difference f32 does not hold.  The references compute from the definitions in 64 bits, in
+logarithms where 64 bits would leave nothing of a share."""
 import math
 
 import pytest
@@ -89,3 +90,36 @@ def test_share_that_64_bits_do_not_hold(gpu, dev, dtype):
     others = torch.ones(3000, dtype=torch.bool, device=dev)
     others[[3, 5]] = False
     assert not bool(step.gradient[:, others].any())
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("vocab", [40, 4099, 70001])
+def test_differences_that_f32_does_not_hold(gpu, dev, dtype, vocab):
+    """The type's lowest value next to its largest: the difference passes f32's range, what it
+    gives at a temperature above 2 does not.  Half a step for each of two halved logits'
+    difference, 1/T and the product, and the statistics' 4."""
+    top, low = torch.finfo(dtype).max, torch.finfo(dtype).min
+    z = torch.full((3, vocab), low, dtype=dtype, device=dev)
+    z[:, 7] = top
+    z[1, 9] = top / 2
+    z[2] = top
+    z[2, 11] = low
+    tokens = torch.tensor([[7, 9, 11, 0]] * 3, dtype=torch.int32, device=dev)
+    ids = torch.tensor([[7, 30]] * 3, dtype=torch.int32, device=dev)
+    values = torch.zeros(3, 2, device=dev)
+    for T in (2.5, 4.0, 1000.0, 1e6):
+        d = z.double() / T
+        m, log_sum = d.amax(1, keepdim=True), torch.logsumexp(d - d.amax(1, keepdim=True), 1, keepdim=True)
+        log_q = d - m - log_sum
+        assert bool(log_q.isfinite().all())
+        got = distribution.token_logprobs(gpu, z, tokens, alternatives=20, temperature=T)
+        want = log_q.gather(1, tokens.long())
+        within(got.logprob, want, 4 * U * want.abs() + sum_tol(vocab))
+        want = log_q.gather(1, got.top_ids.long())
+        within(got.top_logprobs, want, 4 * U * want.abs() + sum_tol(vocab))
+        outside = d - m
+        outside[:, [7, 30]] = -math.inf
+        want = torch.logsumexp(outside, 1)
+        stats = distribution.distill(gpu, z, ids, values, teacher_stats=torch.zeros(3, 2, device=dev),
+                                     temperature=T).stats
+        within(stats[:, 2], want, 6 * U * want.abs() + sum_tol(vocab))
