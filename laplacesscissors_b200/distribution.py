@@ -10,7 +10,8 @@ between rows, token ids as int32 (-1 for an unused slot; another id outside the
 vocabulary makes the results it enters NaN).  Calls enqueue on torch's current stream
 on the Gpu's device, as torch's own operations do, copy nothing to the host and may be
 captured into a CUDA graph.  `out` takes tensors to write instead of new ones, in the
-order of the results (None where a result is not wanted)."""
+order of the results (None where a result is not wanted); they count as modified in
+place, so that torch's autograd notices where it had saved one."""
 from __future__ import annotations
 
 import ctypes as C
@@ -26,6 +27,7 @@ _DEFAULT_STREAM = 1  # cudaStreamLegacy
 _raw_stream = torch._C._cuda_getCurrentRawStream
 _F32, _I32 = torch.float32, torch.int32
 _logprobs = lib.lsx_token_logprobs_device
+_written = torch.autograd.graph.increment_version
 MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
 
 
@@ -122,6 +124,7 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
             None if ids is None or not k else _vector(d, ids, (rows, k), _I32, "out[3]"),
             None if values is None or not k else _vector(d, values, (rows, k), _F32, "out[4]"),
             None if logprobs is None or not k else _vector(d, logprobs, (rows, k), _F32, "out[5]"), _stream(d)))
+        _written([t for t, count in zip(out, (n, 1, 1, k, k, k)) if count and t is not None])
     return TokenLogprobs(logprob, entropy, stats, ids, values, logprobs)
 
 
@@ -145,6 +148,7 @@ def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor
     if rows:
         check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
                                                      temperature, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
+        _written(out)
     return out
 
 
@@ -182,6 +186,7 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if rows:
         check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature, *teacher,
                                      *at, grad.data_ptr() if gradient else None, grad_stride, _stream(gpu.device)))
+        _written([t for t in (out[0], out[1], grad) if t is not None])
     return Distillation(out[0], out[1], grad)
 
 
@@ -198,6 +203,7 @@ def distill_backward(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, 
     if rows:
         check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
                                               *teacher, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
+        _written(out)
     return out
 
 
