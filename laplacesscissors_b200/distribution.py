@@ -11,7 +11,13 @@ vocabulary makes the results it enters NaN).  Calls enqueue on torch's current s
 on the Gpu's device, as torch's own operations do, copy nothing to the host and may be
 captured into a CUDA graph.  `out` takes tensors to write instead of new ones, in the
 order of the results (None where a result is not wanted); they count as modified in
-place, so that torch's autograd notices where it had saved one."""
+place, so that torch's autograd notices where it had saved one.
+
+Autograd does not record the calls.  Logits that require grad are refused where their
+gradient would be lost without a word; a training step passes them on itself,
+    step = distill(gpu, logits.detach(), ids, values, weights=w, gradient=True)
+    logits.backward(step.gradient)
+and likewise with token_logprobs and token_logprobs_backward."""
 from __future__ import annotations
 
 import ctypes as C
@@ -80,6 +86,13 @@ def _count(t: torch.Tensor, rows: int, name: str) -> int:
     return t.shape[1]
 
 
+def _unrecorded(logits: torch.Tensor, name: str = "logits"):
+    """Refuses a tensor whose gradient autograd would not get."""
+    if logits.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} require grad, which autograd does not record here: pass {name}.detach(); gradients "
+                         "with respect to the logits come from the calls that return them")
+
+
 def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
     """The gradient's tensor and row stride: rows laid out like the logits'."""
     if out is None:
@@ -101,6 +114,7 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
     (m, s) and the `alternatives` largest logits of each row, in descending order
     with the lower id first among equals (lsx_token_logprobs_device)."""
     rows, vocab, stride, kind = _rows(gpu, logits)
+    _unrecorded(logits)
     n = _count(tokens, rows, "tokens") if tokens is not None else 0
     k = int(alternatives)
     if not 0 <= k <= min(MAX_SLOTS, vocab):
@@ -172,6 +186,9 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     weights * loss with respect to the logits, which out[2] may be."""
     rows, vocab, stride, kind = _rows(gpu, logits)
     teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
+    if not gradient:
+        _unrecorded(logits)
+        _unrecorded(teacher_logits, "teacher_logits")
     if weights is not None and not gradient:
         raise ValueError("weights scale the gradient only")
     if out is None:

@@ -1,10 +1,11 @@
 """What torch's autograd learns of the calls of laplacesscissors_b200/distribution.py: every tensor
-that a call writes counts as modified, and an `out` that a caller gives is what it gets back."""
+that a call writes counts as modified, and an `out` that a caller gives is what it gets back; a
+gradient handed to backward() reaches the weights behind the logits."""
 import pytest
 import torch
 
 from laplacesscissors_b200 import distribution
-from test_distribution_gpu import dev, make, teacher_of  # noqa: F401
+from test_distribution_gpu import dev, distill64, logprobs_gradient64, make, stored, teacher_of, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -67,3 +68,27 @@ def test_modification_is_counted_under_no_grad_and_capture(gpu, dev):
         mine = [t.clone() for t in out]  # inference tensors have no counter
         call(mine)
     assert all(torch.equal(a, b) for a, b in zip(mine, out))
+
+
+@pytest.mark.parametrize("step", ["distill", "logprobs"])
+def test_a_training_step(gpu, dev, step):
+    """Logits of a readout in 64 bits, rounded to f32 on their way: the weights' gradient is the
+    states' product with the formula's, within what the states make of its tolerance."""
+    g = torch.Generator().manual_seed(82)
+    states = torch.randn(6, 24, generator=g, dtype=torch.float64).to(dev)
+    weight = (torch.randn(24, 2003, generator=g, dtype=torch.float64) * 0.5).to(dev).requires_grad_()
+    logits = (states @ weight).float()
+    z = logits.detach()
+    ids, values, stats = teacher_of(dev, 83, z, 9, 1.0)
+    each = torch.linspace(0.5, 2, 6, device=dev)
+    if step == "distill":
+        logits.backward(distribution.distill(gpu, z, ids, values, teacher_stats=stats, weights=each,
+                                             gradient=True).gradient)
+        _, _, want, _, tol = distill64(z, ids, values, stats, each, 1.0)
+    else:
+        tokens = ids[:, :2].contiguous()
+        own = torch.stack([each, -each], 1)
+        f = distribution.token_logprobs(gpu, z, tokens)
+        logits.backward(distribution.token_logprobs_backward(gpu, z, tokens, f.stats, f.entropy, own, each))
+        want, tol = logprobs_gradient64(z, tokens, own, each, 1.0)
+    within(weight.grad, states.t() @ want, states.abs().t() @ stored(want, tol, torch.float32))

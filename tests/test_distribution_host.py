@@ -1,0 +1,50 @@
+"""Host side of laplacesscissors_b200/distribution.py and its callers: what torch's autograd would
+lose is refused.  No GPU: refusals come before anything is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from laplacesscissors_b200 import LsxError, distribution
+
+
+class HostGpu:
+    """Where CPU tensors say they are (get_device), with no context: a call that passes the Python
+    checks is refused by the library, which needs one."""
+    device = -1
+    handle = C.c_void_p(None)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    monkeypatch.setattr(distribution, "_stream", lambda device: 0)
+    return HostGpu()
+
+
+def rows(**kw):
+    return torch.zeros(2, 5, **kw)
+
+
+IDS, ONE = torch.zeros(2, 3, dtype=torch.int32), torch.ones(2)
+
+
+def test_logits_that_require_grad_are_refused(host):
+    z, values = rows(requires_grad=True), torch.zeros(2, 3)
+    for call in (lambda: distribution.token_logprobs(host, z, IDS),
+                 lambda: distribution.token_logprobs(host, z * 2),
+                 lambda: distribution.distill(host, z, IDS, values),
+                 lambda: distribution.distill(host, rows(), IDS, values.clone().requires_grad_())):
+        with pytest.raises(ValueError, match="detach"):
+            call()
+        with torch.no_grad(), pytest.raises(LsxError, match="context"):
+            call()
+
+
+def test_calls_that_give_the_gradient_take_logits_that_require_grad(host):
+    z, values = rows(requires_grad=True), torch.zeros(2, 3)
+    for call in (lambda: distribution.token_logprobs(host, z.detach(), IDS),
+                 lambda: distribution.distill(host, z, IDS, values, gradient=True),
+                 lambda: distribution.token_logprobs_backward(host, z, IDS, torch.zeros(2, 2), None, values),
+                 lambda: distribution.distill_backward(host, z, IDS, values, torch.zeros(2, 3), ONE)):
+        with pytest.raises(LsxError, match="context"):
+            call()
