@@ -30,7 +30,9 @@ from .gpu import Gpu
 
 _KINDS = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
 _DEFAULT_STREAM = 1  # cudaStreamLegacy
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# The raw handle that torch.cuda.current_stream wraps in an object, where torch has it by this name.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
+    (lambda device: torch.cuda.current_stream(device).cuda_stream)
 _F32, _I32 = torch.float32, torch.int32
 _logprobs = lib.lsx_token_logprobs_device
 _written = torch.autograd.graph.increment_version
@@ -103,8 +105,7 @@ def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
 
 
 def _stream(device: int) -> int:
-    """torch's current stream on the device, as lsx.h takes it (the raw handle that
-    torch.cuda.current_stream wraps in an object)."""
+    """torch's current stream on the device, as lsx.h takes it."""
     return _raw_stream(device) or _DEFAULT_STREAM
 
 

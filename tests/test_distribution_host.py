@@ -1,10 +1,14 @@
 """Host side of laplacesscissors_b200/distribution.py and its callers: what torch's autograd would
-lose is refused.  No GPU: refusals come before anything is launched."""
+lose is refused, and the module can be imported beside a torch without CUDA.  No GPU: refusals
+come before anything is launched."""
 import ctypes as C
+import subprocess
+import sys
 
 import pytest
 import torch
 
+from conftest import ROOT
 from laplacesscissors_b200 import LsxError, distribution
 
 
@@ -48,3 +52,13 @@ def test_calls_that_give_the_gradient_take_logits_that_require_grad(host):
                  lambda: distribution.distill_backward(host, z, IDS, values, torch.zeros(2, 3), ONE)):
         with pytest.raises(LsxError, match="context"):
             call()
+
+
+def test_import_without_the_raw_stream_of_a_cuda_build():
+    code = ("import torch\n"
+            "del torch._C._cuda_getCurrentRawStream\n"
+            "from laplacesscissors_b200 import distribution\n"
+            "class Stream: cuda_stream = 77\n"
+            "torch.cuda.current_stream = lambda device: Stream if device == 3 else None\n"
+            "assert distribution._stream(3) == 77\n")
+    subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True, timeout=300)
