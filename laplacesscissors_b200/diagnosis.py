@@ -329,14 +329,17 @@ def evaluate_cases(model: Model, cases, rotation: DeviceRotation | None = None,
     return Evaluation(before, after, correct_before, correct_after, records)
 
 
-def readout_divergence(model: Model, prompts, targets, rotation: DeviceRotation, alternatives: int = 20,
+def readout_divergence(model: Model, prompts, targets, rotation: DeviceRotation, alternatives: int | None = None,
                        temperature: float = 1.0, deadline: Deadline | None = None):
     """How far the edited readout's distributions are from the model's own at the scored
     positions of equal-shape cases (prompts [cases, P], targets [cases, n]): the unedited
-    pass gives each position's top `alternatives` and statistics, the edited one its
-    divergence from them, the other tokens counted as one outcome.  verify_cached compares
-    logits one prefix at a time; this compares probabilities for many at once.  Returns
-    (divergence f32 [cases, n], the unedited ScoredDistribution)."""
+    pass gives each position's top `alternatives` (by default 20, or the vocabulary where it
+    is smaller) and statistics, the edited one its divergence from them, the other tokens
+    counted as one outcome.  verify_cached compares logits one prefix at a time; this
+    compares probabilities for many at once.  Returns (divergence f32 [cases, n], the
+    unedited ScoredDistribution)."""
+    if alternatives is None:
+        alternatives = min(20, model.vocab_size())
     if deadline is not None:
         deadline.check()
     before = model.score_distribution(prompts, targets, alternatives=alternatives, temperature=temperature)

@@ -1,15 +1,17 @@
 """Host side of laplacesscissors_b200/distribution.py and its callers: what torch's autograd would
-lose is refused, and the module can be imported beside a torch without CUDA.  No GPU: refusals
-come before anything is launched."""
+lose is refused, the module can be imported beside a torch without CUDA, and the default call of
+diagnosis.readout_divergence suits any vocabulary.  No GPU: refusals come before anything is
+launched, and a model of plain Python stands in for the other calls."""
 import ctypes as C
 import subprocess
 import sys
 
+import numpy as np
 import pytest
 import torch
 
 from conftest import ROOT
-from laplacesscissors_b200 import LsxError, distribution
+from laplacesscissors_b200 import LsxError, diagnosis, distribution
 
 
 class HostGpu:
@@ -62,3 +64,30 @@ def test_import_without_the_raw_stream_of_a_cuda_build():
             "torch.cuda.current_stream = lambda device: Stream if device == 3 else None\n"
             "assert distribution._stream(3) == 77\n")
     subprocess.run([sys.executable, "-c", code], cwd=ROOT, check=True, timeout=300)
+
+
+class PlainModel:
+    def __init__(self, vocab):
+        self.vocab, self.asked = vocab, []
+
+    def vocab_size(self):
+        return self.vocab
+
+    def score_distribution(self, prompts, targets, rotation=None, alternatives=0, temperature=1.0):
+        self.asked.append(alternatives)
+        return _Scored()
+
+    def score_divergence(self, prompts, targets, ids, logits, stats, rotation, temperature):
+        return np.zeros((1, 1), np.float32)
+
+
+class _Scored:
+    top_ids = top_logits = stats = None
+
+
+@pytest.mark.parametrize("vocab, default", [(1, 1), (7, 7), (19, 19), (20, 20), (151936, 20)])
+def test_default_alternatives_suit_the_vocabulary(vocab, default):
+    model = PlainModel(vocab)
+    diagnosis.readout_divergence(model, [[1]], [[0]], None)
+    diagnosis.readout_divergence(model, [[1]], [[0]], None, 9)  # as asked, for the library to refuse
+    assert model.asked == [default, 9]
