@@ -34,6 +34,7 @@ _DEFAULT_STREAM = 1  # cudaStreamLegacy
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or \
     (lambda device: torch.cuda.current_stream(device).cuda_stream)
 _F32, _I32 = torch.float32, torch.int32
+_Tensor = torch.Tensor
 _logprobs = lib.lsx_token_logprobs_device
 _written = torch.autograd.graph.increment_version
 MAX_SLOTS = 128  # given tokens, alternatives or teacher tokens per row
@@ -56,7 +57,7 @@ class Distillation(NamedTuple):
 
 def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
     """(rows, vocab, stride, kind) of a matrix of rows on the Gpu's device."""
-    kind = _KINDS.get(logits.dtype) if isinstance(logits, torch.Tensor) and logits.dim() == 2 else None
+    kind = _KINDS.get(logits.dtype) if isinstance(logits, _Tensor) and logits.dim() == 2 else None
     if kind is None:
         raise ValueError(f"{name} must be a [rows, vocab] tensor of float32, float16 or bfloat16")
     if logits.get_device() != gpu.device:
@@ -76,21 +77,22 @@ def _rows(gpu: Gpu, logits: torch.Tensor, name: str = "logits"):
 
 def _vector(device: int, t: torch.Tensor, shape: tuple, dtype: torch.dtype, name: str) -> int:
     """Address of a contiguous tensor of this shape and type on the device."""
-    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device \
+    if isinstance(t, _Tensor) and t.dtype is dtype and t.shape == shape and t.get_device() == device \
             and t.is_contiguous():
         return t.data_ptr()
     raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on the Gpu's device")
 
 
 def _count(t: torch.Tensor, rows: int, name: str) -> int:
-    if not isinstance(t, torch.Tensor) or t.dim() != 2 or t.shape[0] != rows or t.shape[1] > MAX_SLOTS:
+    shape = t.shape if isinstance(t, _Tensor) else ()
+    if len(shape) != 2 or shape[0] != rows or shape[1] > MAX_SLOTS:
         raise ValueError(f"{name} must be [rows, at most {MAX_SLOTS}]")
-    return t.shape[1]
+    return shape[1]
 
 
-def _unrecorded(logits: torch.Tensor, name: str = "logits"):
-    """Refuses a tensor whose gradient autograd would not get."""
-    if logits.requires_grad and torch.is_grad_enabled():
+def _unrecorded(name: str):
+    """Refuses a tensor that requires grad while gradients are recorded: autograd would not get this one."""
+    if torch.is_grad_enabled():
         raise ValueError(f"{name} require grad, which autograd does not record here: pass {name}.detach(); gradients "
                          "with respect to the logits come from the calls that return them")
 
@@ -115,10 +117,11 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
     (m, s) and the `alternatives` largest logits of each row, in descending order
     with the lower id first among equals (lsx_token_logprobs_device)."""
     rows, vocab, stride, kind = _rows(gpu, logits)
-    _unrecorded(logits)
+    if logits.requires_grad:
+        _unrecorded("logits")
     n = _count(tokens, rows, "tokens") if tokens is not None else 0
     k = int(alternatives)
-    if not 0 <= k <= min(MAX_SLOTS, vocab):
+    if not 0 <= k <= MAX_SLOTS or k > vocab:
         raise ValueError(f"alternatives must be at most {MAX_SLOTS} and at most the vocabulary")
     if out is None:
         def new(wanted, *shape, dtype=_F32):
@@ -139,7 +142,11 @@ def token_logprobs(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor | None =
             None if ids is None or not k else _vector(d, ids, (rows, k), _I32, "out[3]"),
             None if values is None or not k else _vector(d, values, (rows, k), _F32, "out[4]"),
             None if logprobs is None or not k else _vector(d, logprobs, (rows, k), _F32, "out[5]"), _stream(d)))
-        _written([t for t, count in zip(out, (n, 1, 1, k, k, k)) if count and t is not None])
+        if n and k and not (logprob is None or entropy is None or stats is None or ids is None or values is None
+                            or logprobs is None):
+            _written(out)
+        else:
+            _written([t for t, count in zip(out, (n, 1, 1, k, k, k)) if count and t is not None])
     return TokenLogprobs(logprob, entropy, stats, ids, values, logprobs)
 
 
@@ -163,7 +170,7 @@ def token_logprobs_backward(gpu: Gpu, logits: torch.Tensor, tokens: torch.Tensor
     if rows:
         check(lib.lsx_token_logprobs_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride,
                                                      temperature, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
-        _written(out)
+        _written((out,))
     return out
 
 
@@ -187,9 +194,8 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     weights * loss with respect to the logits, which out[2] may be."""
     rows, vocab, stride, kind = _rows(gpu, logits)
     teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)
-    if not gradient:
-        _unrecorded(logits)
-        _unrecorded(teacher_logits, "teacher_logits")
+    if not gradient and (logits.requires_grad or teacher_logits.requires_grad):
+        _unrecorded("logits" if logits.requires_grad else "teacher_logits")
     if weights is not None and not gradient:
         raise ValueError("weights scale the gradient only")
     if out is None:
@@ -204,7 +210,10 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     if rows:
         check(lib.lsx_distill_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature, *teacher,
                                      *at, grad.data_ptr() if gradient else None, grad_stride, _stream(gpu.device)))
-        _written([t for t in (out[0], out[1], grad) if t is not None])
+        if out[0] is None or out[1] is None:
+            _written([t for t in (*out[:2], grad) if t is not None])
+        else:
+            _written((out[0], out[1], grad) if gradient else out[:2])
     return Distillation(out[0], out[1], grad)
 
 
@@ -221,7 +230,7 @@ def distill_backward(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, 
     if rows:
         check(lib.lsx_distill_backward_device(gpu.handle, logits.data_ptr(), kind, rows, vocab, stride, temperature,
                                               *teacher, *at, out.data_ptr(), out_stride, _stream(gpu.device)))
-        _written(out)
+        _written((out,))
     return out
 
 
