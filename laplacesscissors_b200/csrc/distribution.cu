@@ -968,9 +968,11 @@ __device__ void select_by_threads(Selection& P, const Row<E>& row, const Slice& 
 // ---- token_logprobs ------------------------------------------------------------------
 // One cluster of blocks per row (one block where there are rows enough): the blocks sum
 // and rank their slices and send sums and best keys to the first one's shared memory,
-// which puts them together and writes the row's results.
+// which puts them together and writes the row's results.  Its 22.6 KB of shared memory leave
+// nine blocks of 128 threads on an SM (a bound of ten only took registers: 3000 x 4000 f16 with
+// 20 alternatives 29.4 us, 26.6 so; 3000 x 500 bf16 with 100 76.9 and 77.4).
 template <typename E, int T>
-__global__ void __launch_bounds__(T, T <= 128 ? 10 : T <= 192 ? 7 : T <= 224 ? 6 : 5) token_logprobs_kernel(
+__global__ void __launch_bounds__(T, T <= 128 ? 9 : T <= 192 ? 7 : T <= 224 ? 6 : 5) token_logprobs_kernel(
     const E* __restrict__ logits, int vocab, size_t stride, const Scale k, const uint32_t* __restrict__ tokens,
     int token_count, int top, LogprobOutputs out) {
     __shared__ Sums scratch[33];
