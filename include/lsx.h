@@ -374,9 +374,11 @@ int lsx_readout_margin_fixed(lsx_ctx* ctx, const lsx_tensor* weight, const lsx_t
    m / T + s is its log-sum-exp.  Sums are held in f32 around the row's maximum or
    in f64.  -inf logits are tokens that cannot occur; a row of nothing else has
    statistics (-inf, 0), entropy 0, log probabilities -inf and a zero gradient.  A NaN
-   or +inf logit makes the row's results NaN.  In token lists 0xFFFFFFFF is an unused
+   or +inf logit makes the row's results NaN (of its statistics s; m passes over NaN, and
+   the alternatives' ids and logits are what they are).  In token lists 0xFFFFFFFF is an unused
    slot; any other id >= vocab makes the results it enters NaN.  All pointers are
-   device pointers.  Calls only enqueue, use no workspace and touch nothing of the
+   device pointers; what a call writes overlaps nothing that it reads or writes otherwise,
+   but for gradient_out as said below.  Calls only enqueue, use no workspace and touch nothing of the
    context but its device: `stream` is the cudaStream_t they run on, NULL for the
    context's own (the default stream is cudaStreamLegacy, 1).
 

@@ -11,9 +11,10 @@
 // Differences are formed before they are scaled: y = (z - r) * (log2 e / T) against a
 // reference r that is itself one of the logits, so the lowest value of a type, -inf
 // masks and logits far from zero all give the exponent their difference has.  Sums are
-// f32 against the row's maximum, in an order that sizes alone decide, so results repeat
-// bit for bit; what small differences are made of (a list's mass, a loss) is f64.  A
-// 16-bit gradient is rounded once, when it is stored.
+// f32 against the row's maximum, in an order that the sizes, the rows' alignment to 16 bytes
+// and the number of SMs decide, so results repeat bit for bit for the same call; what small
+// differences are made of (a list's mass, a loss) is f64.  A 16-bit gradient is rounded
+// once, when it is stored.
 //
 // Measured on B200 (6552 GB/s measured copy, a pass among others): log probabilities with 8
 // alternatives of 2048 x 151936 f32 191 us (99% of the copy's rate), with 20 of one row
@@ -21,6 +22,8 @@
 // time); their gradient, 2048 x 151936 bf16, 190 us (100%); a loss of 512 x 151936 f32 with 20
 // listed tokens 58 us (82%); loss and gradient of 2048 x 151936 bf16 with 64 277 us (69%: most
 // of a row is read twice); a gradient from saved statistics, 1000 x 50257 f16, 38 us (81%).
+// These are short runs at 1965 MHz.  Seconds of the largest calls meet the card's 1 kW: the
+// first of them takes 204 us at 1540 MHz, the fused step 311 at 1670.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <math.h>
@@ -44,9 +47,10 @@ constexpr int kListCap = 2048;       // candidate keys of one selection
 // 285 and 57 us so, 299 and 62 with 5 blocks of chunks of 2, 304 and 69 with 3 blocks of 384,
 // 308 and 56 with 8 of 128.  100 x 32000 f32 (slices of 2000): 12.7 us staged, 16.1 not;
 // shorter ones are alike.
-// A slice is at most kAgainVectors (two blocks for a row of 151936 bf16), so that what does
-// not stay in shared memory can stay in L2: 2048 of these rows whole 306 us, halved 285, in
-// quarters 356.
+// Rows are halved until a slice is at most kAgainVectors (two blocks for a row of 151936 bf16),
+// so that what does not stay in shared memory can stay in L2: 2048 of these rows whole 306 us,
+// halved 285, in quarters 356.  Slices are longer where a row would take more than kMaxCluster
+// blocks, and where one halving less saves a second wave (launch_distill).
 constexpr int kStagedThreads = 256;
 constexpr int kStagedBlocks = 4;
 constexpr int kPlaces = 3;
@@ -1075,7 +1079,8 @@ __device__ __forceinline__ void store16(void* p, uint4 w) {
 }
 
 // The dense gradient of a slice into `out` (the row's first element) by T threads.  `out`
-// may be the row.  `ready` gives the coefficients, once, after the first loads are on their
+// may be the row.  An `out` of another alignment to 16 bytes than the row is stored element by
+// element (1000 x 50257 f16: 137 us instead of 38).  `ready` gives the coefficients, once, after the first loads are on their
 // way.  `stage` is the one that stream_slice read through, or nullptr.
 template <typename E, bool kLinear, typename S, typename F>
 __device__ __forceinline__ void write_dense(const Row<E>& row, const Slice& part, E* out, float L, int tid, int T,

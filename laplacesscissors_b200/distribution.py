@@ -11,7 +11,10 @@ vocabulary makes the results it enters NaN).  Calls enqueue on torch's current s
 on the Gpu's device, as torch's own operations do, copy nothing to the host and may be
 captured into a CUDA graph.  `out` takes tensors to write instead of new ones, in the
 order of the results (None where a result is not wanted); they count as modified in
-place, so that torch's autograd notices where it had saved one.
+place, so that torch's autograd notices where it had saved one.  A gradient is written
+fastest into rows that lie to 16 bytes as the logits' do: for logits of padded rows into
+an `out` of the same row stride, or over the logits (1000 x 50257 f16: 38 us, 137 into
+contiguous rows).
 
 Autograd does not record the calls.  Logits that require grad are refused where their
 gradient would be lost without a word; a training step passes them on itself,
@@ -98,7 +101,7 @@ def _unrecorded(name: str):
 
 
 def _gradient(gpu: Gpu, logits: torch.Tensor, out: torch.Tensor | None):
-    """The gradient's tensor and row stride: rows laid out like the logits'."""
+    """The gradient's tensor and row stride; a new one is contiguous."""
     if out is None:
         out = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     elif out.shape != logits.shape or out.dtype != logits.dtype:
@@ -189,8 +192,8 @@ def distill(gpu: Gpu, logits: torch.Tensor, teacher_ids: torch.Tensor, teacher_l
     """Divergence of the student's rows from a teacher's top tokens
     (lsx_distill_device): teacher_ids int32 and teacher_logits f32 [rows, k],
     teacher_stats [rows, 2] the teacher's statistics at the same temperature (with
-    them the tokens outside the list count as one outcome, without them the teacher
-    is normalised over its list).  With `gradient` also the gradient of
+    them the tokens outside the list count as one outcome, left out only where the
+    student masks them all; without them the teacher is normalised over its list).  With `gradient` also the gradient of
     weights * loss with respect to the logits, which out[2] may be."""
     rows, vocab, stride, kind = _rows(gpu, logits)
     teacher = _teacher(gpu, rows, teacher_ids, teacher_logits, teacher_stats)

@@ -318,8 +318,8 @@ class Model:
     def score_divergence(self, prompts, targets, teacher_ids, teacher_logits, teacher_stats=None,
                          rotation: DeviceRotation | None = None, temperature: float = 1.0) -> np.ndarray:
         """Divergence f32 [cases, n] of each scored position from a teacher's listed tokens
-        [cases, n, k] (lsx_model_divergence_batch); with teacher_stats [cases, n, 2] the
-        tokens outside the list count as one outcome."""
+        [cases, n, k] (lsx_model_divergence_batch; 0xFFFFFFFF is an unused slot); with
+        teacher_stats [cases, n, 2] the tokens outside the list count as one outcome."""
         p, t = self._cases(prompts, targets)
         cases, n = t.shape
         ids = np.ascontiguousarray(teacher_ids, dtype=np.uint32)
