@@ -414,7 +414,7 @@ int lsx_token_logprobs_backward_device(lsx_ctx* ctx, const void* logits, lsx_dty
    and all tokens outside K form one more outcome, p_r = max(0, 1 - sum_K p_j) against
    the student's q_r: loss += p_r ln(p_r / q_r).  Where q_r is 0 in 64 bits (below
    2^-1074: the student masks all tokens outside K) that outcome is left out, p_r = 0, and
-   what remains of the loss may be negative; a masked token in K makes it +inf instead.
+   what remains of the loss may be negative; a token of K at -inf makes it +inf instead.
    stats_out [rows x 3]: (m, s) of the student and the log of
    sum_{i not in K} exp((z_i - m) / T) (-inf without teacher_stats).  With
    gradient_out also the gradient of weights[r] * loss (weights NULL: 1), with

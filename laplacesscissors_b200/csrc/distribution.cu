@@ -1403,7 +1403,8 @@ __global__ void __launch_bounds__(T, kStaged ? kStagedBlocks : 6 * kRowThreads /
         const float over = high == m ? (float)(inside - 1.0) + outside
                                      : (listed ? (float)inside * expf((high - m) * k.inverse) : 0.f) + (outside - 1.f);
         log_sum = empty ? 0.f : log1pf(over);
-        if (kTail && some) log_rest = logf(rest.S) + below;
+        // (without a listed token that the student holds both sums are one: q_r is 1, and exactly)
+        if (kTail && some) log_rest = listed ? logf(rest.S) + below : log_sum;
     };
     // By the first warp.  The loss may be a small difference of logarithms: they are taken
     // in 64 bits, one to a lane, so that the row waits for one of each function.

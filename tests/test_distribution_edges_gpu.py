@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from laplacesscissors_b200 import distribution
-from test_distribution_gpu import KINDS, U, check_distill, dev, stored, sum_tol, within  # noqa: F401
+from test_distribution_gpu import KINDS, U, check_distill, dev, make, stored, sum_tol, within  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -123,3 +123,39 @@ def test_differences_that_f32_does_not_hold(gpu, dev, dtype, vocab):
         stats = distribution.distill(gpu, z, ids, values, teacher_stats=torch.zeros(3, 2, device=dev),
                                      temperature=T).stats
         within(stats[:, 2], want, 6 * U * want.abs() + sum_tol(vocab))
+
+
+@pytest.mark.parametrize("vocab", [1, 8, 900, 2500, 20011, 70001])
+@pytest.mark.parametrize("dtype", KINDS)
+def test_unused_lists_ask_for_nothing(gpu, dev, dtype, vocab):
+    """A row that lists no token has p_r = q_r = 1: loss and gradient are 0, not next to it; so
+    has one whose listed tokens neither teacher nor student holds."""
+    z = make(dev, vocab, 6, vocab, dtype, 3, masked=0.2 if vocab > 1 else 0.0)
+    ids = torch.full((6, 7), -1, dtype=torch.int32, device=dev)
+    values = torch.randn(6, 7, generator=torch.Generator().manual_seed(vocab)).to(dev)
+    if vocab > 1:
+        ids[3:, 2] = 1
+        z[3:, 1] = values[3:, 2] = -math.inf
+    stats = torch.tensor([[1.0, 2.0]] * 6, device=dev)
+    weights = torch.linspace(0.5, 2, 6, device=dev)
+    for T in (1.0, 0.3, 2.0):
+        for teacher in (None, stats):
+            step = distribution.distill(gpu, z, ids, values, teacher_stats=teacher, weights=weights, temperature=T,
+                                        gradient=True)
+            back = distribution.distill_backward(gpu, z, ids, values, step.stats, weights, teacher_stats=teacher,
+                                                 temperature=T)
+            assert not bool(step.loss.any()) and not bool(step.gradient.any()) and not bool(back.any())
+
+
+def test_unused_lists_of_rows_of_every_spread(gpu, dev):
+    """Rows from nearly uniform to nearly one token: the logarithms of q_r's two sums are one."""
+    R = 4000
+    ids = torch.full((R, 3), -1, dtype=torch.int32, device=dev)
+    none, stats, ones = torch.zeros(R, 3, device=dev), torch.zeros(R, 2, device=dev), torch.ones(R, device=dev)
+    for vocab in (61, 700, 2999):
+        g = torch.Generator().manual_seed(vocab)
+        z = (torch.randn(R, vocab, generator=g) * torch.rand(R, 1, generator=g) * 12).to(dev)
+        step = distribution.distill(gpu, z, ids, none, teacher_stats=stats, gradient=True)
+        back = distribution.distill_backward(gpu, z, ids, none, step.stats, ones, teacher_stats=stats)
+        assert torch.equal(step.stats[:, 1], step.stats[:, 2])
+        assert not bool(step.loss.any()) and not bool(step.gradient.any()) and not bool(back.any())
