@@ -437,6 +437,119 @@ int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind
                                 const float* stats, const float* loss_gradient, void* gradient_out,
                                 size_t gradient_stride, void* stream);
 
+/* ------------------------------------------------- paged cache in 4 bits -- */
+/* Keys and values of many sequences in pages of a shared pool, four bits an element,
+   and attention over them.  The reference keeps one sequence's keys and values in f32
+   (src/model.rs:492, Gpu::attention, src/gpu.rs:454-501).
+
+   Tables.  Row s of `tables` [table_rows x table_width] lists sequence s's pages:
+   entry i holds its positions i * page_size and on; lengths[s] is how many positions it
+   has (at most table_width * page_size), and entries behind the last page in use are -1.
+   refs[p] counts the table entries that name page p; 0 is a free page.
+
+   Storage.  A layer's pages are [page_count][kv_heads][page_size / 16] cells of
+   18 * head_dim bytes, a cell the keys and values of 16 positions of one head.  Each 64
+   consecutive elements x of a head share f16 z = min x and s = max((max x - z) / 15, 0)
+   (the difference and quotient in f32); an element is kept as n = (x - z) / s rounded to
+   the nearest of 0..15, ties to even (0 where s = 0), and stands for s n + z.  A group
+   whose z or s is not finite (an element that is not, or beyond f16) has both NaN and
+   n = 0.  For position t (0..15) of the cell, element d and group g = d / 64, with D =
+   head_dim, whole divisions and bytes from the cell's start:
+     key n:     byte (32 g + 4 (t % 8) + d % 64 / 16) * 16 + t / 8 * 8 + d % 16 / 2, the
+                low four bits for even d
+     value n:   byte 8 D + (32 g + 4 (d % 8) + t % 8 / 2) * 16 + d / 16 % 4 * 4 + t % 2 * 2
+                + t / 8, the low four bits for d % 16 < 8
+     key s:     byte 16 D + 64 g + t % 8 / 2 * 16 + t / 8 * 8 + t % 2 * 2, z 4 bytes on
+     value s:   the same from 17 D
+   (the order in which the attention's matrix instructions take them).
+
+   All pointers in these entries are device pointers but the descriptions' own; calls only
+   enqueue, on `stream` (NULL: the context's; the default stream is cudaStreamLegacy, 1),
+   and what a call writes overlaps nothing that it reads or writes otherwise unless said. */
+typedef struct lsx_cache_view {  /* one layer's pages with the tables */
+    void* pages;                 /* 16-byte aligned */
+    size_t page_count;           /* pages of the pool */
+    size_t page_size;            /* positions of a page: a multiple of 16 */
+    size_t kv_heads, head_dim;   /* head_dim 64, 128, 192 or 256 */
+    const int32_t* tables;
+    size_t table_rows, table_width;
+    const int32_t* lengths;      /* [table_rows] */
+} lsx_cache_view;
+/* The rows of a call.  Its sequences are list[0 .. sequences - 1] (rows of the tables; NULL:
+   0 .. sequences - 1); sequence b owns the call's rows starts[b] .. starts[b + 1] - 1 (starts
+   ascending, [sequences + 1]; NULL: row b alone), which stand for its last positions,
+   lengths - count and on: the lengths count the call's own rows.  Rows of no sequence are
+   left as they are. */
+typedef struct lsx_cache_rows {
+    size_t rows;
+    size_t sequences;
+    const int32_t* list;
+    const int32_t* starts;
+} lsx_cache_rows;
+/* Pages of any kind in several layers: page p of layer l is page_bytes (a multiple of 16)
+   at data + l * layer_bytes + p * page_bytes. */
+typedef struct lsx_cache_pool {
+    void* data;
+    size_t layers, layer_bytes, page_bytes, page_count;
+} lsx_cache_pool;
+
+/* Bytes of one layer's page. */
+size_t lsx_cache_page_bytes(size_t kv_heads, size_t page_size, size_t head_dim);
+/* Writes the rows' keys and values (`kind` elements, rows k_row and heads k_head elements
+   apart) at their positions.  Rows before position 0 and positions without a page are
+   passed over.  No two sequences of a call may write to one page's same positions. */
+int lsx_cache_append_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, const void* k,
+                            const void* v, lsx_dtype kind, size_t k_row, size_t k_head, size_t v_row, size_t v_head,
+                            void* stream);
+/* The values that the rows' positions stand for, [rows x kv_heads x head_dim] of `kind`
+   each, s n + z rounded once to f32 and then to the kind: 0 before position 0, NaN where
+   there is no page. */
+int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, lsx_dtype kind,
+                          void* k_out, void* v_out, void* stream);
+/* Attention of the rows' queries over their sequences: with query head h reading key head
+   h / (q_heads / kv_heads), out = sum_t p_t v_t, p = softmax over t of scale * q . k_t, for
+   the positions t up to the row's own.  A row that sees no position is 0; one that sees a
+   position without a page, or belongs to a sequence outside the tables, is NaN, and so is one that sees
+   a NaN key or value.  Rows and heads lie as given, in elements.  workspace (16-byte aligned) holds
+   lsx_cache_attention_workspace_bytes(); calls that may overlap need one each. */
+int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, const void* q,
+                               lsx_dtype kind, size_t q_heads, size_t q_row, size_t q_head, double scale, void* out,
+                               size_t out_row, size_t out_head, void* workspace, size_t workspace_bytes, void* stream);
+size_t lsx_cache_attention_workspace_bytes(lsx_ctx* ctx, size_t head_dim);
+/* Gives sequences[i] (n of them, 1..=1024) counts[i] further positions: its length
+   grows, and the pages it needs are the lowest free ones, in the order of the list.  All
+   or nothing: *missing is how many pages were short (of the pool, or of a row of the
+   tables), and unless it is 0 nothing changes.  An entry outside the tables, and a sequence
+   named again, is passed over; so is a negative count. */
+int lsx_cache_reserve_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, size_t table_width, int32_t* lengths,
+                             int32_t* refs, size_t page_count, size_t page_size, const int32_t* sequences,
+                             const int32_t* counts, size_t n, int32_t* missing, void* stream);
+/* children[i] takes the positions of parents[i] (n of them, 1..=1024): whole pages are
+   shared, a partly filled last page is copied in all layers to the lowest free page, in the
+   order of the list, so that both may go on.  A child must be empty (and a child that is
+   empty is no useful parent): entries whose child is not, or was named before, or that name
+   a row outside the tables, are passed over.  All or nothing as lsx_cache_reserve_device.
+   pairs [n x 2] receives what was copied, (-1, -1) where nothing was. */
+int lsx_cache_fork_device(lsx_ctx* ctx, const lsx_cache_pool* pool, int32_t* tables, size_t table_rows,
+                          size_t table_width, int32_t* lengths, int32_t* refs, size_t page_size, const int32_t* parents,
+                          const int32_t* children, size_t n, int32_t* pairs, int32_t* missing, void* stream);
+/* Empties the sequences: their pages lose a reference each, and their rows of the tables
+   hold -1.  Entries outside the tables, and sequences named again, are passed over. */
+int lsx_cache_free_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, size_t table_width, int32_t* lengths,
+                          int32_t* refs, size_t page_count, size_t page_size, const int32_t* sequences, size_t n,
+                          void* stream);
+/* Moves pages so that those in use are the lowest: with n of them, the k-th page in use
+   from n on goes to the k-th free page below n, in all layers; tables_out and refs_out
+   are the tables and counts afterwards (they may be the tables and counts themselves). */
+int lsx_cache_compact_device(lsx_ctx* ctx, const lsx_cache_pool* pool, const int32_t* tables, size_t table_rows,
+                             size_t table_width, const int32_t* refs, int32_t* tables_out, int32_t* refs_out,
+                             void* workspace, size_t workspace_bytes, void* stream);
+size_t lsx_cache_compact_workspace_bytes(size_t page_count);
+/* Copies page pairs[i][0] to page pairs[i][1] in all layers, n pairs; one that names no
+   page of the pool is passed over.  No page may be the target of two pairs, nor source and
+   target both. */
+int lsx_cache_copy_device(lsx_ctx* ctx, const lsx_cache_pool* pool, const int32_t* pairs, size_t n, void* stream);
+
 /* ------------------------------------------------ plane-candidate feasibility -- */
 /* FeasibleSet (src/interval.rs:47-212): the open forbidden intervals of a plane
    rotation's half-angle tangent t in [-bound, bound], merged as quadratic

@@ -38,6 +38,21 @@ class ModelInfo(C.Structure):
     ]
 
 
+class CacheView(C.Structure):
+    _fields_ = [("pages", C.c_void_p), ("page_count", C.c_size_t), ("page_size", C.c_size_t), ("kv_heads", C.c_size_t),
+                ("head_dim", C.c_size_t), ("tables", C.c_void_p), ("table_rows", C.c_size_t), ("table_width", C.c_size_t),
+                ("lengths", C.c_void_p)]
+
+
+class CacheRows(C.Structure):
+    _fields_ = [("rows", C.c_size_t), ("sequences", C.c_size_t), ("list", C.c_void_p), ("starts", C.c_void_p)]
+
+
+class CachePool(C.Structure):
+    _fields_ = [("data", C.c_void_p), ("layers", C.c_size_t), ("layer_bytes", C.c_size_t), ("page_bytes", C.c_size_t),
+                ("page_count", C.c_size_t)]
+
+
 P = C.c_void_p
 PP = C.POINTER(C.c_void_p)
 SZ = C.c_size_t
@@ -116,6 +131,17 @@ SIGNATURES = {
     "lsx_token_logprobs_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, SZ, P, P, P, P, P, SZ, P]),
     "lsx_distill_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, P, SZ, P]),
     "lsx_distill_backward_device": (I, [P, P, I, SZ, SZ, SZ, D, P, P, SZ, P, P, P, P, SZ, P]),
+    "lsx_cache_page_bytes": (SZ, [SZ, SZ, SZ]),
+    "lsx_cache_append_device": (I, [P, P, P, P, P, I, SZ, SZ, SZ, SZ, P]),
+    "lsx_cache_read_device": (I, [P, P, P, I, P, P, P]),
+    "lsx_cache_attention_device": (I, [P, P, P, P, I, SZ, SZ, SZ, D, P, SZ, SZ, P, SZ, P]),
+    "lsx_cache_attention_workspace_bytes": (SZ, [P, SZ]),
+    "lsx_cache_reserve_device": (I, [P, P, SZ, SZ, P, P, SZ, SZ, P, P, SZ, P, P]),
+    "lsx_cache_fork_device": (I, [P, P, P, SZ, SZ, P, P, SZ, P, P, SZ, P, P, P]),
+    "lsx_cache_free_device": (I, [P, P, SZ, SZ, P, P, SZ, SZ, P, SZ, P]),
+    "lsx_cache_compact_device": (I, [P, P, P, SZ, SZ, P, P, P, P, SZ, P]),
+    "lsx_cache_compact_workspace_bytes": (SZ, [SZ]),
+    "lsx_cache_copy_device": (I, [P, P, P, SZ, P]),
     "lsx_feasible_create": (I, [D, PP]),
     "lsx_feasible_free": (I, [P]),
     "lsx_feasible_constrain": (I, [P, D, D, D]),
