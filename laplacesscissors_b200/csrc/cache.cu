@@ -5,6 +5,7 @@
 
 #include <algorithm>
 #include <limits>
+#include <type_traits>
 
 #include "cache.cuh"
 #include "device_common.cuh"
@@ -194,73 +195,688 @@ __global__ void __launch_bounds__(128) read_kernel(CacheView c, CacheRows r, T* 
 }
 
 // ---- attention -----------------------------------------------------------------
-// One block a (row, query head): 128 positions at a time, a score a thread, then an
-// element of the output a thread, with the running maximum and sum of the softmax.
-template <typename T>
-__global__ void __launch_bounds__(128) attention_kernel(const T* q, size_t q_row, size_t q_head, CacheView c,
-                                                        CacheRows r, uint32_t q_heads, float scale, T* out,
-                                                        size_t out_row, size_t out_head) {
-    const uint32_t row = blockIdx.x / q_heads, h = blockIdx.x % q_heads, head = h / (q_heads / c.kv_heads);
-    const int dim = (int)c.dim, groups = dim / kCacheGroup;
-    __shared__ float query[kMaxCacheDim], weight[128];
-    __shared__ float reduce[4];
-    const SequenceRows s = sequence_rows(c, r, sequence_of(r, row));
-    if ((int)row >= s.first + s.count || (int)row < s.first) return;
-    const int seen = s.length - s.count + (int)row - s.first + 1;
-    T* o = out + row * out_row + h * out_head;
-    for (int d = threadIdx.x; d < dim; d += 128) query[d] = to_f32(q[row * q_row + h * q_head + d]) * scale;
-    float most = -INFINITY, sum = 0.f, sums[2] = {0.f, 0.f};
-    const float nan = std::numeric_limits<float>::quiet_NaN();
-    __syncthreads();
-    for (int first = 0; first < seen; first += 128) {
-        const int position = first + (int)threadIdx.x, t = position % kCellTokens;
-        float score = -INFINITY;
-        if (position < seen) {
-            const uint8_t* cell = cell_of(c, s.table, (uint32_t)position, head);
-            score = cell ? 0.f : nan;
-            for (int g = 0; cell && g < groups; ++g) {
-                const __half* at = reinterpret_cast<const __half*>(cell + cell_key_steps(dim) + step_byte(t, g));
-                float dot = 0.f, plain = 0.f;
-                for (int d = g * 64; d < g * 64 + 64; d += 2) {
-                    const uint32_t byte = cell[key_byte(t, d)];
-                    dot = fmaf(query[d], (float)(byte & 15), dot);
-                    dot = fmaf(query[d + 1], (float)(byte >> 4), dot);
-                    plain += query[d] + query[d + 1];
-                }
-                score += __half2float(at[0]) * dot + __half2float(at[2]) * plain;
-            }
-        }
-        float top = score;
-        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
-        if (threadIdx.x % 32 == 0) reduce[threadIdx.x / 32] = top;
-        __syncthreads();
-        const float now = fmaxf(fmaxf(fmaxf(reduce[0], reduce[1]), fmaxf(reduce[2], reduce[3])), most);
-        const float against = now == -INFINITY ? 0.f : now;
-        weight[threadIdx.x] = position < seen ? expf(score - against) : 0.f;
-        const float keep = expf(most - against);
-        most = now;
-        sum *= keep;
-        for (int i = 0; i < 2; ++i) sums[i] *= keep;
-        __syncthreads();
-        for (int k = 0; k < 128 && first + k < seen; ++k) {
-            const float w = weight[k];
-            const uint8_t* cell = cell_of(c, s.table, (uint32_t)(first + k), head);
-            sum += w;
-            for (int i = 0, d = threadIdx.x; d < dim; d += 128, ++i) {
-                float x = nan;
-                if (cell) {
-                    const int u = (first + k) % kCellTokens;
-                    const __half* at = reinterpret_cast<const __half*>(cell + cell_value_steps(dim) + step_byte(u, d / 64));
-                    const uint32_t byte = cell[value_byte(dim, u, d / 16 * 16 + d % 8)];
-                    x = fmaf(__half2float(at[0]), (float)(d % 16 < 8 ? byte & 15 : byte >> 4), __half2float(at[2]));
-                }
-                sums[i] = fmaf(w, x, sums[i]);
-            }
-        }
-        __syncthreads();
+// Formulas.  With n, s, z a key's levels, steps and zeros, q . k = sum over its groups of
+// s (n . q) + z (1 . q), and with those of the values out = (sum over positions of p s n +
+// p z) / sum p.  The products n . q and (p s) n are matrix products on the tensor cores
+// (m16n8k16, f16 in, f32 sums) whose operand n needs no arithmetic: a level in bits 0-3 or
+// 4-7 of an f16 is the subnormal n 2^-24 or n 2^-20, exactly, so a word of eight levels
+// gives its four operand registers by one shift and four masks; what is over in the
+// powers of two goes into q (2^-4 for the second kind) and the scaling behind the sum.
+//
+// Rounding.  A query row is scaled by a power of two to below 2^14 and held as f16 hi + lo
+// (PAIR: 22 bits, hi in row r of the matrix instruction and lo in row r + 8, so that their
+// sums meet in one thread), or as f16 alone, which holds f16 and bf16 queries exactly
+// down to 2^-38 of the row's largest.  p s is scaled to below 2^15 by the largest step seen, and
+// held in the same two ways: PAIR keeps 22 bits, a single f16 11, half a step of an f16 result.
+// Everything else is f32; the softmax runs on powers of two with the running maximum.
+//
+// Work.  The cells (16 positions of one head) that the rows of a call see, in the order of
+// sequence, head, tile of rows and position, are cut into equal runs, one a block; the
+// first and last tile of a run may be shared with neighbours, whose parts
+// attention_merge_kernel adds up in a fixed order.  So any mix of lengths fills the card,
+// the workspace goes by the number of blocks, and nothing needs the lengths on the host.
+// A warp streams every fourth cell of the run through its own ring in shared memory (one
+// bulk copy a cell) with its own softmax; the warps' sums meet at a tile's end.
+// Cells that a block takes at least, where there are few: four a warp.
+constexpr int kLeastRun = 16;
+constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
+
+template <int GROUPS, int MT, bool PAIR>
+struct AttentionShape {
+    static constexpr int kDim = 64 * GROUPS, kRows = MT * (PAIR ? 8 : 16), kStage = cell_bytes(kDim);
+    // registers: 32 MT GROUPS sums a thread, beside them what a cell needs
+    static constexpr int kBlocksPerSm = MT * GROUPS <= 2 ? 3 : 2;
+    static constexpr int kStages = GROUPS == 1 ? 8 : GROUPS == 2 ? (kBlocksPerSm == 3 ? 6 : 8) : GROUPS == 3 ? 6 : 4;
+    static constexpr bool kSharedQuery = MT * GROUPS > 2;
+    static constexpr int kRing = kAttentionWarps * kStages * kStage;
+    static constexpr int kParts = kAttentionWarps * kRows * (kDim + 2) * 4;  // the warps' sums, in the ring's memory
+    static constexpr int kQuery = kSharedQuery ? MT * GROUPS * 4 * 32 * 16 : 0;
+    static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + 128 + kAttentionWarps * kStages * 8;
+};
+
+struct AttentionCall {
+    const void* q;
+    void* out;
+    size_t q_row, q_head, out_row, out_head;
+    uint32_t q_heads, group;   // query heads a key head
+    uint32_t tokens, subs;     // rows of a tile: `tokens` positions' (a power of two) heads, or a part of one position's
+    float scale;               // times log2 e
+    bool wide;                 // queries lie to 16 bytes
+    int4* tails;               // [blocks] tiles that a block starts and others finish
+    float* parts;              // [2 blocks][rows][dim + 2]
+};
+
+// A call's cells in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
+// a tile without visible positions counts as one cell, so that its rows get written.
+__device__ __forceinline__ int tile_count(const SequenceRows& s, int tokens) { return (s.count + tokens - 1) / tokens; }
+
+__device__ __forceinline__ int tile_seen(const SequenceRows& s, int tokens, int k) {
+    return s.length - s.count + min(s.count, (k + 1) * tokens);  // positions that its last row sees
+}
+
+__device__ __forceinline__ int tile_cells(const SequenceRows& s, int tokens, int k) {
+    return max(1, (tile_seen(s, tokens, k) + kCellTokens - 1) >> 4);
+}
+
+// Cells of the tiles before k (k below the tile count): the sum of floor((base + 15 + (i + 1) tokens) / 16), with
+// base = length - count, over the tiles that see anything, and 1 for those that do not.
+__device__ __forceinline__ long long cells_before(const SequenceRows& s, int tokens, int k) {
+    if (k == 0) return 0;
+    const int base = s.length - s.count;
+    const int blind = s.length <= 0 ? k : base >= 0 ? 0 : min(k, -base / tokens);
+    if (k <= blind) return k;
+    if (tokens > kCellTokens) {
+        const long long whole = (base + 15) >> 4, step = tokens / kCellTokens;
+        return blind + (k - blind) * whole + step * ((long long)k * (k + 1) - (long long)blind * (blind + 1)) / 2;
     }
-    for (int i = 0, d = threadIdx.x; d < dim; d += 128, ++i)
-        o[d] = from_f32<T>(s.table < 0 ? nan : seen > 0 ? sums[i] / sum : 0.f);
+    const int shift = 31 - __clz(tokens), m = kCellTokens >> shift, y = (base + 15) >> shift;
+    const auto sum = [m](long long n) {  // of floor(i / m) over i = 0 .. n
+        if (n < 0) return 0ll;
+        const long long q = n / m, r = n % m;
+        return m * q * (q - 1) / 2 + q * (r + 1);
+    };
+    return blind + sum((long long)y + k) - sum((long long)y + blind);
+}
+
+__device__ __forceinline__ long long sequence_cells(const SequenceRows& s, int tokens) {
+    const int tiles = tile_count(s, tokens);
+    return tiles ? cells_before(s, tokens, tiles - 1) + tile_cells(s, tokens, tiles - 1) : 0;
+}
+
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack_f16(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x += __shfl_xor_sync(0xffffffffu, x, 1);
+    return x + __shfl_xor_sync(0xffffffffu, x, 2);
+}
+__device__ __forceinline__ float quad_max(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+}
+
+// Sixteen consecutive elements as f32; `wide`: at a 16-byte boundary.
+template <typename T>
+__device__ __forceinline__ void load16(const T* x, bool wide, float (&out)[16]) {
+    if (wide) {
+        constexpr int kEach = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 16 / kEach; ++i) {
+            const uint4 raw = reinterpret_cast<const uint4*>(x)[i];
+            const T* e = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+            for (int k = 0; k < kEach; ++k) out[i * kEach + k] = to_f32(e[k]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) out[i] = to_f32(x[i]);
+    }
+}
+
+template <typename T, int GROUPS, int MT, bool PAIR>
+__global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT, PAIR>::kBlocksPerSm))
+    attention_kernel(CacheView c, CacheRows r, AttentionCall call) {
+    using Shape = AttentionShape<GROUPS, MT, PAIR>;
+    constexpr int D = Shape::kDim, RP = PAIR ? 1 : 2, kStages = Shape::kStages;
+    extern __shared__ __align__(128) uint8_t shared[];
+    __shared__ long long found[3];
+    const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32, quad = lane / 4, j = lane % 4;
+    uint8_t* ring = shared + warp * kStages * Shape::kStage;
+    float* warp_sums = reinterpret_cast<float*>(shared);
+    uint4* queries = reinterpret_cast<uint4*>(shared + (Shape::kShared - Shape::kQuery - 128 - kAttentionWarps * kStages * 8));
+    uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Shape::kShared - kAttentionWarps * kStages * 8) + warp * kStages;
+    const int tokens = (int)call.tokens;
+    const uint32_t tiles_of = c.kv_heads * call.subs;
+    pdl_launch_dependents();
+    if (lane == 0)
+        for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
+    fence_barrier_init();
+
+    // this block's run of cells
+    const uint32_t each = (r.count + kAttentionThreads - 1) / kAttentionThreads;
+    const uint32_t mine_first = min(threadIdx.x * each, r.count), mine_end = min(mine_first + each, r.count);
+    long long mine = 0;
+    for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_cells(sequence_rows(c, r, b), tokens) * tiles_of;
+    long long* scan = reinterpret_cast<long long*>(shared);
+    long long before = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const long long below = __shfl_up_sync(0xffffffffu, before, o);
+        if (lane >= o) before += below;
+    }
+    if (lane == 31) scan[warp] = before;
+    __syncthreads();
+    long long total = 0;
+    before -= mine;
+#pragma unroll
+    for (int w = 0; w < kAttentionWarps; ++w) {
+        if (w < warp) before += scan[w];
+        total += scan[w];
+    }
+    const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)kLeastRun);
+    long long at = run * blockIdx.x;
+    const long long end = min(at + run, total);
+    if (mine > 0 && before <= at && at < before + mine) {
+        for (uint32_t b = mine_first; b < mine_end; ++b) {
+            const long long cells = sequence_cells(sequence_rows(c, r, b), tokens) * tiles_of;
+            if (at < before + cells) {
+                found[0] = b;
+                found[1] = at - before;
+                break;
+            }
+            before += cells;
+        }
+    }
+    if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    if (at >= end) return;
+    uint32_t b = (uint32_t)found[0];
+    long long offset = found[1];
+    uint32_t parity = 0;
+    bool dead = false;  // a copy that did not arrive in time
+
+    while (at < end) {
+        const SequenceRows s = sequence_rows(c, r, b);
+        const long long one = sequence_cells(s, tokens);
+        if (offset >= one * tiles_of) {
+            ++b;
+            offset = 0;
+            continue;
+        }
+        const uint32_t head_sub = (uint32_t)(offset / one), head = head_sub / call.subs, sub = head_sub % call.subs;
+        const long long rest = offset % one;
+        int k = 0;
+        for (int high = tile_count(s, tokens); high - k > 1;) {  // cells_before(k) <= rest
+            const int middle = (k + high) / 2;
+            if (cells_before(s, tokens, middle) <= rest)
+                k = middle;
+            else
+                high = middle;
+        }
+        const int first = (int)(rest - cells_before(s, tokens, k)), cells = tile_cells(s, tokens, k);
+        const int last = (int)min((long long)cells, first + end - at);
+        at += last - first;
+        offset += last - first;
+
+        // the tile's rows: row i is head sub * rows + i of position k, or head i % group of position k * tokens + i / group
+        const int base = s.length - s.count;
+        const int seen = min(tile_seen(s, tokens, k), (int)min((long long)c.table_width * c.page_size, (long long)INT32_MAX));
+        const int least = base + k * tokens + 1;  // what the first row sees
+        const auto place = [&](int i, int& token, int& h) {
+            token = k * tokens + (call.subs > 1 ? 0 : i / (int)call.group);
+            h = call.subs > 1 ? (int)sub * Shape::kRows + i : i % (int)call.group;
+            return h < (int)call.group && token < min(s.count, (k + 1) * tokens);
+        };
+        const bool beyond = s.table < 0 || tile_seen(s, tokens, k) > seen;  // positions that no table entry covers
+
+        uint32_t query[Shape::kSharedQuery ? 1 : MT * GROUPS * 4][4];
+        float factor[MT][RP], zeros_of[MT][RP][GROUPS], most[MT][RP], sum[MT][RP], zeros[MT][RP][GROUPS];
+        int limit[MT][RP];
+        __syncthreads();  // the sums and queries of the tile before are read
+#pragma unroll
+        for (int t = 0; t < MT; ++t) {
+            uint32_t frag[GROUPS * 4][4];
+#pragma unroll
+            for (int p = 0; p < RP; ++p) {
+                const int i = t * (PAIR ? 8 : 16) + p * 8 + quad;
+                int token, h;
+                const bool row = place(i, token, h);
+                limit[t][p] = row ? base + token + 1 : 0;
+                const T* x = static_cast<const T*>(call.q) + (size_t)(s.first + token) * call.q_row +
+                             (size_t)(head * call.group + h) * call.q_head + 16 * j;
+                float values[GROUPS][16], top = 0.f;
+                bool fine = true;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    if (row) {
+                        load16(x + 64 * g, call.wide, values[g]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) values[g][e] = 0.f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        top = fmaxf(top, fabsf(values[g][e]));
+                        fine = fine && isfinite(values[g][e]);
+                    }
+                }
+                top = quad_max(top);
+                fine = quad_max(fine ? 0.f : 1.f) == 0.f;
+                // 2^power takes the largest into 2^13 .. 2^14
+                const int exponent = top > 0.f ? max(ilogbf(top), -100) : 0;
+                const int power = fine ? 13 - exponent : 0;
+                const float up = fine ? ldexpf(1.f, power) : 0.f;
+                factor[t][p] = fine ? call.scale * ldexpf(1.f, 24 - power) : std::numeric_limits<float>::quiet_NaN();
+                most[t][p] = -INFINITY;
+                sum[t][p] = 0.f;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    float plain = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        values[g][e] = fine ? values[g][e] * up : 0.f;
+                        plain += values[g][e];
+                    }
+                    zeros_of[t][p][g] = quad_sum(plain) * 0x1p-24f;
+                    zeros[t][p][g] = 0.f;
+                    // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
+#pragma unroll
+                    for (int w = 0; w < 2; ++w)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float down = e ? 0.0625f : 1.f;
+                            const float* y = values[g] + 8 * w + e;
+                            const float y0 = y[0] * down, y4 = y[4] * down, y2 = y[2] * down, y6 = y[6] * down;
+                            uint32_t(&f)[4] = frag[(g * 2 + w) * 2 + e];
+                            f[p] = pack_f16(y0, y4);
+                            f[2 + p] = pack_f16(y2, y6);
+                            if (PAIR) {
+                                const float2 a = unpack_f16(f[0]), d = unpack_f16(f[2]);
+                                f[1] = pack_f16(y0 - a.x, y4 - a.y);
+                                f[3] = pack_f16(y2 - d.x, y6 - d.y);
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int f = 0; f < GROUPS * 4; ++f) {
+                if constexpr (Shape::kSharedQuery) {
+                    if (warp == 0)
+                        queries[(t * GROUPS * 4 + f) * 32 + lane] = make_uint4(frag[f][0], frag[f][1], frag[f][2], frag[f][3]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) query[t * GROUPS * 4 + f][i] = frag[f][i];
+                }
+            }
+        }
+        if constexpr (Shape::kSharedQuery) __syncthreads();
+
+        float out[MT][8 * GROUPS][4];
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int n = 0; n < 8 * GROUPS; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[t][n][i] = 0.f;
+        uint32_t step_limit = 0;  // largest step (f16 bits) that p s times `lift` may hold
+        float lift = 0.f;
+
+        // ---- the stream of cells
+        const int stop = min(last, (seen + kCellTokens - 1) >> 4);  // cells beyond hold nothing
+        const int mine_cells = max(0, (stop - first - warp + kAttentionWarps - 1) / kAttentionWarps);
+        const uint32_t per_page = c.page_size / kCellTokens;
+        const auto page_of = [&](int n) {  // of this warp's n-th cell
+            if (n >= mine_cells) return 0xffffffffu;
+            const uint32_t cell = (uint32_t)(first + warp + n * kAttentionWarps);
+            return (uint32_t)c.tables[(size_t)s.table * c.table_width + cell / per_page];
+        };
+        uint32_t pages = page_of(lane), next_pages = page_of(32 + lane), gone = 0;
+        const auto issue = [&](int n) {
+            if (n >= mine_cells || dead) return;
+            if (n % 32 == 0 && n > 0) {
+                pages = next_pages;
+                next_pages = page_of(n + 32 + lane);
+            }
+            const uint32_t page = __shfl_sync(0xffffffffu, pages, n % 32);
+            const int stage = n % kStages;
+            if (page >= c.page_count) {
+                gone |= 1u << stage;
+                return;
+            }
+            gone &= ~(1u << stage);
+            if (lane == 0) {
+                const uint32_t cell = (uint32_t)(first + warp + n * kAttentionWarps);
+                const uint8_t* from = c.pages + (((size_t)page * c.kv_heads + head) * per_page + cell % per_page) * Shape::kStage;
+                mbar_expect_tx(bars + stage, Shape::kStage);
+                bulk_load(ring + stage * Shape::kStage, from, Shape::kStage, bars + stage);
+            }
+        };
+        fence_proxy_async_shared();  // the warps' sums lay in the ring
+        __syncthreads();
+#pragma unroll 1
+        for (int n = 0; n < kStages - 1; ++n) issue(n);
+
+#pragma unroll 1
+        for (int n = 0; n < mine_cells; ++n) {
+            __syncwarp();
+            issue(n + kStages - 1);
+            const int stage = n % kStages, cell = first + warp + n * kAttentionWarps;
+            const bool here = !(gone >> stage & 1);
+            if (!dead && here) {
+                dead = !mbar_wait_bounded(bars + stage, parity >> stage & 1);
+                parity ^= 1u << stage;
+            }
+            dead = __any_sync(0xffffffffu, dead);
+            if (!here || dead) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int p = 0; p < RP; ++p)
+                        if (dead || cell * kCellTokens < limit[t][p]) sum[t][p] = std::numeric_limits<float>::quiet_NaN();
+                if (!dead) continue;
+                for (int later = n + 1; here && later < min(n + kStages, mine_cells); ++later)  // what is in flight lands first
+                    if (!(gone >> later % kStages & 1)) mbar_wait_bounded(bars + later % kStages, parity >> later % kStages & 1);
+                break;
+            }
+            const uint8_t* held = ring + stage * Shape::kStage;
+            const int position = cell * kCellTokens + 2 * j;
+            const bool edge = (cell + 1) * kCellTokens > least;  // some row does not see all of it
+
+            // scores, in units that `factor` takes to powers of two: [row][2 j, 2 j + 1, 2 j + 8, 2 j + 9]
+            float score[MT][RP][4];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < RP; ++p)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) score[t][p][i] = 0.f;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const uint4 words = *reinterpret_cast<const uint4*>(held + (g * 32 + lane) * 16);
+                const uint4 raw = *reinterpret_cast<const uint4*>(held + cell_key_steps(D) + g * 64 + j * 16);
+                const float2 s0 = unpack_f16(raw.x), z0 = unpack_f16(raw.y), s1 = unpack_f16(raw.z), z1 = unpack_f16(raw.w);
+                const float step[4] = {s0.x, s0.y, s1.x, s1.y}, zero[4] = {z0.x, z0.y, z1.x, z1.y};
+                float dot[MT][2][4];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) dot[t][0][i] = dot[t][1][i] = 0.f;
+#pragma unroll
+                for (int w = 0; w < 2; ++w) {
+                    const uint32_t low = w ? words.y : words.x, high = w ? words.w : words.z;  // positions quad, quad + 8
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
+#pragma unroll
+                        for (int t = 0; t < MT; ++t) {
+                            uint32_t a[4];
+                            const int f = t * GROUPS * 4 + (g * 2 + w) * 2 + e;
+                            if constexpr (Shape::kSharedQuery) {
+                                const uint4 x = queries[f * 32 + lane];
+                                a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
+                            } else {
+                                a[0] = query[f][0], a[1] = query[f][1], a[2] = query[f][2], a[3] = query[f][3];
+                            }
+                            mma_f16(dot[t][0], a, low & mask, low >> 8 & mask);
+                            mma_f16(dot[t][1], a, high & mask, high >> 8 & mask);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int p = 0; p < RP; ++p)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float d = PAIR ? dot[t][i / 2][i % 2] + dot[t][i / 2][2 + i % 2] : dot[t][i / 2][2 * p + i % 2];
+                            score[t][p][i] = fmaf(step[i], d, fmaf(zero[i], zeros_of[t][p][g], score[t][p][i]));
+                        }
+            }
+            // weights
+            bool grows = false;
+            float now[MT][RP];
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < RP; ++p) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) score[t][p][i] *= factor[t][p];
+                    if (edge) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            if (position + i / 2 * 8 + i % 2 >= limit[t][p]) score[t][p][i] = -INFINITY;
+                    }
+                    const float top = fmaxf(fmaxf(score[t][p][0], score[t][p][1]), fmaxf(score[t][p][2], score[t][p][3]));
+                    now[t][p] = fmaxf(most[t][p], quad_max(top));
+                    grows = grows || now[t][p] > most[t][p];
+                }
+            if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int p = 0; p < RP; ++p) {
+                        const float keep = now[t][p] > most[t][p] ? exp2_approx(most[t][p] - now[t][p]) : 1.f;
+                        most[t][p] = now[t][p];
+                        sum[t][p] *= keep;
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) zeros[t][p][g] *= keep;
+#pragma unroll
+                        for (int n = 0; n < 8 * GROUPS; ++n) {
+                            if (PAIR) {
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) out[t][n][i] *= keep;
+                            } else {
+                                out[t][n][2 * p] *= keep;
+                                out[t][n][2 * p + 1] *= keep;
+                            }
+                        }
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < RP; ++p) {
+                    const float against = most[t][p] == -INFINITY ? 0.f : most[t][p];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        score[t][p][i] = exp2_approx(score[t][p][i] - against);
+                        sum[t][p] += score[t][p][i];
+                    }
+                }
+            // the values' steps; where one is larger than any before, the sums are scaled down
+            uint4 raw[GROUPS];
+            uint32_t top_step = 0;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                raw[g] = *reinterpret_cast<const uint4*>(held + cell_value_steps(D) + g * 64 + j * 16);
+                if (edge) {  // positions that no row sees may hold anything
+                    const auto cut = [&](uint32_t x, int from) {
+                        return x & (from < seen ? 0xffffu : 0u) | x & (from + 1 < seen ? 0xffff0000u : 0u);
+                    };
+                    raw[g].x = cut(raw[g].x, position), raw[g].y = cut(raw[g].y, position);
+                    raw[g].z = cut(raw[g].z, position + 8), raw[g].w = cut(raw[g].w, position + 8);
+                }
+                top_step = __vmaxu2(top_step, __vmaxu2(raw[g].x, raw[g].z));
+            }
+            top_step = max(top_step & 0xffffu, top_step >> 16);
+            if (__any_sync(0xffffffffu, top_step > step_limit)) {
+                // NaN steps make their products NaN and count for nothing here; 2^k <= the largest < 2^(k + 1)
+                uint32_t largest = 0;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    const uint32_t all[4] = {raw[g].x & 0xffffu, raw[g].x >> 16, raw[g].z & 0xffffu, raw[g].z >> 16};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (all[i] < 0x7c00u) largest = max(largest, all[i]);
+                }
+                largest = __reduce_max_sync(0xffffffffu, largest);
+                if (largest > step_limit) {
+                    const uint32_t e = max(largest >> 10, 1u);
+                    const float next = ldexpf(1.f, 29 - (int)e);
+                    const float keep = lift > 0.f ? next / lift : 0.f;
+                    lift = next;
+                    step_limit = ((e + 1) << 10) - 1;
+#pragma unroll
+                    for (int t = 0; t < MT; ++t)
+#pragma unroll
+                        for (int n = 0; n < 8 * GROUPS; ++n)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) out[t][n][i] *= keep;
+                }
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                const float2 s0 = unpack_f16(raw[g].x), z0 = unpack_f16(raw[g].y), s1 = unpack_f16(raw[g].z),
+                             z1 = unpack_f16(raw[g].w);
+                const float step[4] = {s0.x * lift, s0.y * lift, s1.x * lift, s1.y * lift};
+                const float zero[4] = {z0.x, z0.y, z1.x, z1.y};
+                uint32_t a[MT][4];
+#pragma unroll
+                for (int t = 0; t < MT; ++t)
+#pragma unroll
+                    for (int p = 0; p < RP; ++p) {
+                        float x[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            x[i] = score[t][p][i] * step[i];
+                            float y = score[t][p][i] * zero[i];
+                            // a position that this row does not see adds nothing, whatever it holds
+                            if (edge && position + i / 2 * 8 + i % 2 >= limit[t][p]) x[i] = y = 0.f;
+                            zeros[t][p][g] += y;
+                        }
+                        a[t][p] = pack_f16(x[0], x[1]);
+                        a[t][2 + p] = pack_f16(x[2], x[3]);
+                        if (PAIR) {
+                            const float2 d = unpack_f16(a[t][0]), e = unpack_f16(a[t][2]);
+                            a[t][1] = pack_f16(x[0] - d.x, x[1] - d.y);
+                            a[t][3] = pack_f16(x[2] - e.x, x[3] - e.y);
+                        }
+                    }
+                const uint4 words = *reinterpret_cast<const uint4*>(held + cell_values(D) + (g * 32 + lane) * 16);
+                const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+#pragma unroll
+                    for (int t = 0; t < MT; ++t) {
+                        mma_f16(out[t][(g * 4 + w) * 2], a[t], word[w] & 0x000f000fu, word[w] >> 8 & 0x000f000fu);
+                        mma_f16(out[t][(g * 4 + w) * 2 + 1], a[t], word[w] & 0x00f000f0u, word[w] >> 8 & 0x00f000f0u);
+                    }
+            }
+        }
+        if (beyond) {
+#pragma unroll
+            for (int t = 0; t < MT; ++t)
+#pragma unroll
+                for (int p = 0; p < RP; ++p)
+                    if (s.table < 0 || limit[t][p] > seen) sum[t][p] = std::numeric_limits<float>::quiet_NaN();
+        }
+
+        // ---- the warps' sums
+        const float even = lift > 0.f ? 0x1p24f / lift : 0.f, odd = even * 0.0625f;
+        __syncthreads();  // the rings are drained
+        float* mine_sums = warp_sums + warp * Shape::kRows * (D + 2);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+#pragma unroll
+            for (int p = 0; p < RP; ++p) {
+                float* row = mine_sums + (t * (PAIR ? 8 : 16) + p * 8 + quad) * (D + 2);
+                const float l = quad_sum(sum[t][p]);
+                if (j == 0) row[D] = most[t][p], row[D + 1] = l;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    const float z = quad_sum(zeros[t][p][g]);
+#pragma unroll
+                    for (int n = 8 * g; n < 8 * g + 8; ++n) {
+                        const float up = n % 2 ? odd : even;
+                        const float x = PAIR ? out[t][n][0] + out[t][n][2] : out[t][n][2 * p];
+                        const float y = PAIR ? out[t][n][1] + out[t][n][3] : out[t][n][2 * p + 1];
+                        *reinterpret_cast<float2*>(row + 8 * n + 2 * j) = make_float2(fmaf(x, up, z), fmaf(y, up, z));
+                    }
+                }
+            }
+        __syncthreads();
+        const bool whole = first == 0 && last == cells;
+        float* part = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * Shape::kRows * (D + 2);
+        for (int i = warp; i < Shape::kRows; i += kAttentionWarps) {
+            int token, h;
+            if (!place(i, token, h)) continue;
+            float top = -INFINITY, l = 0.f, weight[kAttentionWarps];
+#pragma unroll
+            for (int w = 0; w < kAttentionWarps; ++w) top = fmaxf(top, warp_sums[(w * Shape::kRows + i) * (D + 2) + D]);
+#pragma unroll
+            for (int w = 0; w < kAttentionWarps; ++w) {
+                const float* row = warp_sums + (w * Shape::kRows + i) * (D + 2);
+                weight[w] = exp2_approx(row[D] - (top == -INFINITY ? 0.f : top));
+                l += weight[w] * row[D + 1];
+            }
+            const float inverse = l == 0.f ? 0.f : 1.f / l;
+            T* to = static_cast<T*>(call.out) + (size_t)(s.first + token) * call.out_row +
+                    (size_t)(head * call.group + h) * call.out_head;
+            for (int d = lane; d < D; d += 32) {
+                float x = 0.f;
+#pragma unroll
+                for (int w = 0; w < kAttentionWarps; ++w) x = fmaf(weight[w], warp_sums[(w * Shape::kRows + i) * (D + 2) + d], x);
+                if (whole)
+                    to[d] = from_f32<T>(x * inverse);
+                else
+                    part[(size_t)i * (D + 2) + d] = x;
+            }
+            if (!whole && lane == 0) part[(size_t)i * (D + 2) + D] = top, part[(size_t)i * (D + 2) + D + 1] = l;
+        }
+        if (first == 0 && !whole && threadIdx.x == 0)
+            call.tails[blockIdx.x] = make_int4(1 + (int)((cells - last + run - 1) / run), (int)b, (int)head_sub, k);
+    }
+}
+
+// Adds up the parts of the tile that block blockIdx.x of attention_kernel started and others
+// finished, in their order; a block a row, a warp every eighth part.
+constexpr int kMergeWarps = 8;
+
+template <typename T>
+__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(CacheView c, CacheRows r, AttentionCall call,
+                                                                           int rows) {
+    pdl_wait();
+    const int block = (int)blockIdx.x / rows, i = (int)blockIdx.x % rows, D = (int)c.dim;
+    const int4 tail = call.tails[block];
+    if (tail.x == 0) return;
+    const SequenceRows s = sequence_rows(c, r, (uint32_t)tail.y);
+    const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs, k = tail.w, tokens = (int)call.tokens;
+    const int token = k * tokens + (call.subs > 1 ? 0 : i / (int)call.group);
+    const int h = call.subs > 1 ? sub * rows + i : i % (int)call.group;
+    if (h >= (int)call.group || token >= min(s.count, (k + 1) * tokens)) return;
+    const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
+    __shared__ float sums[kMergeWarps][kMaxCacheDim + 2];
+    const auto part = [&](int n) {
+        return call.parts + (((size_t)(block + n) * 2 + (n == 0)) * rows + i) * (D + 2);
+    };
+    float top = -INFINITY, l = 0.f, x[kMaxCacheDim / 32] = {};
+    for (int n = warp; n < tail.x; n += kMergeWarps) {
+        const float* p = part(n);
+        const float m = p[D], now = fmaxf(top, m), against = now == -INFINITY ? 0.f : now;
+        const float keep = exp2_approx(top - against), weight = exp2_approx(m - against);
+        top = now;
+        l = l * keep + p[D + 1] * weight;
+#pragma unroll
+        for (int e = 0; e < kMaxCacheDim / 32; ++e)
+            if (e * 32 < D) x[e] = x[e] * keep + p[e * 32 + lane] * weight;
+    }
+#pragma unroll
+    for (int e = 0; e < kMaxCacheDim / 32; ++e)
+        if (e * 32 < D) sums[warp][e * 32 + lane] = x[e];
+    if (lane == 0) sums[warp][kMaxCacheDim] = top, sums[warp][kMaxCacheDim + 1] = l;
+    __syncthreads();
+    top = -INFINITY, l = 0.f;
+    float weight[kMergeWarps];
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, sums[w][kMaxCacheDim]);
+#pragma unroll
+    for (int w = 0; w < kMergeWarps; ++w) {
+        weight[w] = exp2_approx(sums[w][kMaxCacheDim] - (top == -INFINITY ? 0.f : top));
+        l += weight[w] * sums[w][kMaxCacheDim + 1];
+    }
+    T* to = static_cast<T*>(call.out) + (size_t)(s.first + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
+    for (int d = (int)threadIdx.x; d < D; d += 32 * kMergeWarps) {
+        float y = 0.f;
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) y = fmaf(weight[w], sums[w][d], y);
+        to[d] = from_f32<T>(l == 0.f ? 0.f : y / l);
+    }
 }
 
 // ---- pages ---------------------------------------------------------------------
@@ -558,13 +1174,11 @@ int check_rows(const lsx_cache_rows* rows, const CacheView& view, CacheRows* out
 bool known_kind(lsx_dtype kind) { return kind == LSX_F32 || kind == LSX_F16 || kind == LSX_BF16; }
 
 // Rows of heads: `row` and `head` elements from one to the next, each head contiguous.
-int check_heads(const void* data, lsx_dtype kind, size_t rows, size_t heads, size_t dim, size_t row, size_t head,
-                const char* what) {
+int check_heads(const void* data, lsx_dtype kind, size_t row, size_t head, const char* what) {
     LSX_ENSURE(data, "invalid argument");
     LSX_ENSURE(known_kind(kind), "unknown dtype");
     LSX_ENSURE(reinterpret_cast<uintptr_t>(data) % dtype_bytes(kind) == 0, std::string(what) + " not aligned to the type");
     LSX_ENSURE(row <= (size_t)1 << 40 && head <= (size_t)1 << 40, std::string(what) + ": check the strides");
-    (void)rows, (void)heads, (void)dim;
     return LSX_OK;
 }
 
@@ -607,6 +1221,61 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
                             tables, tables_out, (uint64_t)entries, to_of);
 }
 
+// Blocks of attention_kernel on the card, and its workspace: the blocks' tails and two
+// parts each.
+template <int GROUPS, int MT, bool PAIR>
+size_t attention_bytes(int sm_count) {
+    using Shape = AttentionShape<GROUPS, MT, PAIR>;
+    return (size_t)sm_count * Shape::kBlocksPerSm * (16 + 2 * Shape::kRows * (Shape::kDim + 2) * 4);
+}
+
+size_t attention_workspace(int sm_count, size_t dim) {
+    switch (dim / kCacheGroup) {
+    case 1: return std::max(attention_bytes<1, 1, true>(sm_count), attention_bytes<1, 2, false>(sm_count));
+    case 2: return std::max(attention_bytes<2, 1, true>(sm_count), attention_bytes<2, 2, false>(sm_count));
+    case 3: return attention_bytes<3, 1, false>(sm_count);
+    default: return attention_bytes<4, 1, false>(sm_count);
+    }
+}
+
+template <typename T, int GROUPS, int MT, bool PAIR>
+cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r, AttentionCall call,
+                         void* workspace) {
+    using Shape = AttentionShape<GROUPS, MT, PAIR>;
+    const auto kernel = attention_kernel<T, GROUPS, MT, PAIR>;
+    const unsigned blocks = (unsigned)(sm_count * Shape::kBlocksPerSm);
+    call.tokens = 1;
+    while (call.tokens * 2 * call.group <= (uint32_t)Shape::kRows) call.tokens *= 2;
+    call.subs = (call.group + Shape::kRows - 1) / Shape::kRows;
+    call.tails = static_cast<int4*>(workspace);
+    call.parts = reinterpret_cast<float*>(call.tails + blocks);
+    cudaError_t status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+    if (status != cudaSuccess) return status;
+    kernel<<<blocks, kAttentionThreads, Shape::kShared, s>>>(c, r, call);
+    status = cudaGetLastError();
+    if (status != cudaSuccess) return status;
+    return launch_dependent(attention_merge_kernel<T>, blocks * Shape::kRows, 32 * kMergeWarps, 0, s, c, r, call, Shape::kRows);
+}
+
+// Rows of a tile by the rows that a sequence and key head has on average: eight in two parts
+// up to eight; f32 queries sixteen in two parts, f16 and bf16 sixteen or 32 in one (wide
+// heads leave registers for sixteen).
+template <typename T, int GROUPS>
+cudaError_t launch_attention(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r,
+                             const AttentionCall& call, void* workspace) {
+    const uint64_t rows = (uint64_t)((r.rows + r.count - 1) / r.count) * call.group;
+    if (rows > 8) {
+        if constexpr (std::is_same<T, float>::value) {
+            if constexpr (GROUPS <= 2) return launch_tiles<T, GROUPS, 2, true>(sm_count, s, c, r, call, workspace);
+        } else {
+            if constexpr (GROUPS <= 2)
+                if (rows > 16) return launch_tiles<T, GROUPS, 2, false>(sm_count, s, c, r, call, workspace);
+            return launch_tiles<T, GROUPS, 1, false>(sm_count, s, c, r, call, workspace);
+        }
+    }
+    return launch_tiles<T, GROUPS, 1, true>(sm_count, s, c, r, call, workspace);
+}
+
 }  // namespace
 }  // namespace lsx
 
@@ -632,8 +1301,8 @@ int lsx_cache_append_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_
     CacheRows r;
     LSX_TRY(check_view(view, &c));
     LSX_TRY(check_rows(rows, c, &r));
-    LSX_TRY(check_heads(k, kind, r.rows, c.kv_heads, c.dim, k_row, k_head, "keys"));
-    LSX_TRY(check_heads(v, kind, r.rows, c.kv_heads, c.dim, v_row, v_head, "values"));
+    LSX_TRY(check_heads(k, kind, k_row, k_head, "keys"));
+    LSX_TRY(check_heads(v, kind, v_row, v_head, "values"));
     LSX_CACHE_SCOPE();
     const uint64_t units = (uint64_t)r.rows * c.kv_heads * 2;
     LSX_ENSURE(units <= (uint64_t)INT32_MAX * 4, "too many rows and heads");
@@ -652,8 +1321,8 @@ int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_ca
     CacheRows r;
     LSX_TRY(check_view(view, &c));
     LSX_TRY(check_rows(rows, c, &r));
-    LSX_TRY(check_heads(k_out, kind, r.rows, c.kv_heads, c.dim, 0, 0, "keys"));
-    LSX_TRY(check_heads(v_out, kind, r.rows, c.kv_heads, c.dim, 0, 0, "values"));
+    LSX_TRY(check_heads(k_out, kind, 0, 0, "keys"));
+    LSX_TRY(check_heads(v_out, kind, 0, 0, "values"));
     LSX_CACHE_SCOPE();
     const uint64_t units = (uint64_t)r.rows * c.kv_heads * 2;
     LSX_ENSURE(units <= (uint64_t)INT32_MAX * 4, "too many rows and heads");
@@ -666,8 +1335,7 @@ int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_ca
 }
 
 size_t lsx_cache_attention_workspace_bytes(lsx_ctx* ctx, size_t head_dim) {
-    (void)ctx, (void)head_dim;
-    return 16;
+    return ctx ? attention_workspace(ctx->sm_count, head_dim) : 0;
 }
 
 int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, const void* q,
@@ -678,18 +1346,35 @@ int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const l
     LSX_TRY(check_view(view, &c));
     LSX_TRY(check_rows(rows, c, &r));
     LSX_ENSURE(q_heads > 0 && q_heads <= 65536 && q_heads % c.kv_heads == 0, "query heads are a multiple of key heads");
-    LSX_TRY(check_heads(q, kind, r.rows, q_heads, c.dim, q_row, q_head, "queries"));
-    LSX_TRY(check_heads(out, kind, r.rows, q_heads, c.dim, out_row, out_head, "output"));
+    LSX_TRY(check_heads(q, kind, q_row, q_head, "queries"));
+    LSX_TRY(check_heads(out, kind, out_row, out_head, "output"));
     LSX_ENSURE(scale == scale && scale < 1e30 && scale > -1e30, "check the scale");
     LSX_CACHE_SCOPE();
-    LSX_ENSURE(workspace && workspace_bytes >= lsx_cache_attention_workspace_bytes(ctx, c.dim), "workspace too small");
-    LSX_ENSURE((uint64_t)r.rows * q_heads <= INT32_MAX, "too many rows and heads");
+    LSX_ENSURE(workspace && reinterpret_cast<uintptr_t>(workspace) % 16 == 0 &&
+                   workspace_bytes >= attention_workspace(ctx->sm_count, c.dim),
+               "workspace too small or not aligned to 16 bytes");
+    AttentionCall call = {};
+    call.q = q;
+    call.out = out;
+    call.q_row = q_row;
+    call.q_head = q_head;
+    call.out_row = out_row;
+    call.out_head = out_head;
+    call.q_heads = (uint32_t)q_heads;
+    call.group = (uint32_t)(q_heads / c.kv_heads);
+    call.scale = (float)(scale * 1.4426950408889634);
+    const size_t e = dtype_bytes(kind);
+    call.wide = reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_row * e % 16 == 0 && q_head * e % 16 == 0;
     return by_kind(kind, [&](auto type) {
         using T = decltype(type);
-        attention_kernel<T><<<(unsigned)(r.rows * q_heads), 128, 0, on>>>((const T*)q, q_row, q_head, c, r,
-                                                                         (uint32_t)q_heads, (float)scale, (T*)out,
-                                                                         out_row, out_head);
-        LSX_CUDA(cudaGetLastError(), "cache attention");
+        cudaError_t status;
+        switch (c.dim / kCacheGroup) {
+        case 1: status = launch_attention<T, 1>(ctx->sm_count, on, c, r, call, workspace); break;
+        case 2: status = launch_attention<T, 2>(ctx->sm_count, on, c, r, call, workspace); break;
+        case 3: status = launch_attention<T, 3>(ctx->sm_count, on, c, r, call, workspace); break;
+        default: status = launch_attention<T, 4>(ctx->sm_count, on, c, r, call, workspace); break;
+        }
+        LSX_CUDA(status, "cache attention");
         return (int)LSX_OK;
     });
 }
