@@ -201,75 +201,80 @@ __global__ void __launch_bounds__(128) read_kernel(CacheView c, CacheRows r, T* 
 // (m16n8k16, f16 in, f32 sums) whose operand n needs no arithmetic: a level in bits 0-3 or
 // 4-7 of an f16 is the subnormal n 2^-24 or n 2^-20, exactly, so a word of eight levels
 // gives its four operand registers by one shift and four masks; what is over in the
-// powers of two goes into q (2^-4 for the second kind) and the scaling behind the sum.
+// powers of two goes into q (2^-4 for the second kind) and the scaling behind the sum.  The
+// cache is the instructions' 16-row operand (positions of the keys, elements of the
+// values) and the call's rows are its 8 columns, so that few rows leave little unused.
 //
-// Rounding.  A query row is scaled by a power of two to below 2^14 and held as f16 hi + lo
-// (PAIR: 22 bits, hi in row r of the matrix instruction and lo in row r + 8, so that their
-// sums meet in one thread), or as f16 alone, which holds f16 and bf16 queries exactly
-// down to 2^-38 of the row's largest.  p s is scaled to below 2^15 by the largest step seen, and
-// held in the same two ways: PAIR keeps 22 bits, a single f16 11, half a step of an f16 result.
-// Everything else is f32; the softmax runs on powers of two with the running maximum.
+// Rounding.  A query row is scaled by a power of two to below 2^14 and held as f16, which
+// holds f16 and bf16 queries exactly down to 2^-38 of the row's largest element, or for f32
+// (LOW) as f16 high and low parts of 22 bits.  A weight p is taken against a reference that
+// keeps p s below 2^15, and p s is held the same two ways: 11 bits are half a step of an
+// f16 result, twice 11 those of f32.  Everything else is f32.  The reference of a row moves
+// up where p s would pass 2^15, to leave 2^10 for the largest: what is 2^24 below
+// that still has 11 bits, and steady sequences hardly ever move it.
 //
-// Work.  The cells (16 positions of one head) that the rows of a call see, in the order of
-// sequence, head, tile of rows and position, are cut into equal runs, one a block; the
-// first and last tile of a run may be shared with neighbours, whose parts
+// Work.  The pairs of cells (32 positions of one head) that the rows of a call see, in the
+// order of sequence, head, tile of rows and position, are cut into equal runs, one a block;
+// the first and last tile of a run may be shared with neighbours, whose parts
 // attention_merge_kernel adds up in a fixed order.  So any mix of lengths fills the card,
 // the workspace goes by the number of blocks, and nothing needs the lengths on the host.
-// A warp streams every fourth cell of the run through its own ring in shared memory (one
-// bulk copy a cell) with its own softmax; the warps' sums meet at a tile's end.
-// Cells that a block takes at least, where there are few: four a warp.
-constexpr int kLeastRun = 16;
+// A warp streams every fourth pair of the run through its own ring in shared memory by bulk
+// copies, with its own softmax; the warps' sums meet at a tile's end.
+//
+// Pairs that a block takes at least, where there are few: two a warp.
+constexpr int kLeastRun = 8;
+constexpr int kPairTokens = 2 * kCellTokens;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
-template <int GROUPS, int MT, bool PAIR>
+template <int GROUPS, int NT, bool LOW>
 struct AttentionShape {
-    static constexpr int kDim = 64 * GROUPS, kRows = MT * (PAIR ? 8 : 16), kStage = cell_bytes(kDim);
-    // registers: 32 MT GROUPS sums a thread, beside them what a cell needs
-    static constexpr int kBlocksPerSm = MT * GROUPS <= 2 ? 3 : 2;
-    static constexpr int kStages = GROUPS == 1 ? 8 : GROUPS == 2 ? (kBlocksPerSm == 3 ? 6 : 8) : GROUPS == 3 ? 6 : 4;
-    static constexpr bool kSharedQuery = MT * GROUPS > 2;
+    static constexpr int kDim = 64 * GROUPS, kRows = 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
+    static constexpr int kLoad = NT * GROUPS;
+    static constexpr int kBlocksPerSm = kLoad <= 2 ? 4 : kLoad <= 4 && GROUPS < 4 ? 3 : 2;
+    // registers a thread: the sums and the queries, which go to shared memory where 75 are not left for the rest
+    static constexpr int kSums = 16 * kLoad, kQueries = (LOW ? 16 : 8) * kLoad;
+    static constexpr bool kSharedQuery = kSums + kQueries > (kBlocksPerSm == 2 ? 255 : 512 / kBlocksPerSm) - 75;
+    static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW ? 16 : 8) : 0;
+    static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
+    static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
+    static constexpr int kAtOnce = NT == 1 ? 2 : 1;  // cells whose weights a thread holds at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
     static constexpr int kParts = kAttentionWarps * kRows * (kDim + 2) * 4;  // the warps' sums, in the ring's memory
-    static constexpr int kQuery = kSharedQuery ? MT * GROUPS * 4 * 32 * 16 : 0;
-    static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + 128 + kAttentionWarps * kStages * 8;
+    static constexpr int kBars = kAttentionWarps * kStages * 8;
+    static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + kBars;
+    static_assert(kStages >= 2 && kBlocksPerSm * (kShared + 1200) <= 228 * 1024, "shared memory");
 };
 
 struct AttentionCall {
     const void* q;
     void* out;
     size_t q_row, q_head, out_row, out_head;
-    uint32_t q_heads, group;   // query heads a key head
+    uint32_t group;            // query heads a key head
     uint32_t tokens, subs;     // rows of a tile: `tokens` positions' (a power of two) heads, or a part of one position's
+    uint32_t used;             // of the tile's rows, those that hold any
     float scale;               // times log2 e
     bool wide;                 // queries lie to 16 bytes
     int4* tails;               // [blocks] tiles that a block starts and others finish
     float* parts;              // [2 blocks][rows][dim + 2]
 };
 
-// A call's cells in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
-// a tile without visible positions counts as one cell, so that its rows get written.
+// A call's pairs in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
+// a tile without visible positions counts as one pair, so that its rows get written.
 __device__ __forceinline__ int tile_count(const SequenceRows& s, int tokens) { return (s.count + tokens - 1) / tokens; }
 
-__device__ __forceinline__ int tile_seen(const SequenceRows& s, int tokens, int k) {
-    return s.length - s.count + min(s.count, (k + 1) * tokens);  // positions that its last row sees
+__device__ __forceinline__ int tile_pairs(const SequenceRows& s, int tokens, int k) {
+    const int seen = s.length - s.count + min(s.count, (k + 1) * tokens);  // positions that its last row sees
+    return max(1, (seen + kPairTokens - 1) >> 5);
 }
 
-__device__ __forceinline__ int tile_cells(const SequenceRows& s, int tokens, int k) {
-    return max(1, (tile_seen(s, tokens, k) + kCellTokens - 1) >> 4);
-}
-
-// Cells of the tiles before k (k below the tile count): the sum of floor((base + 15 + (i + 1) tokens) / 16), with
-// base = length - count, over the tiles that see anything, and 1 for those that do not.
-__device__ __forceinline__ long long cells_before(const SequenceRows& s, int tokens, int k) {
+// Pairs of the tiles before k (k below the tile count): the sum of floor((base + 31 + (i + 1) tokens) / 32), with
+// base = length - count, over the tiles that see anything, and 1 for those that do not.  tokens divides 32.
+__device__ __forceinline__ long long pairs_before(const SequenceRows& s, int tokens, int k) {
     if (k == 0) return 0;
     const int base = s.length - s.count;
     const int blind = s.length <= 0 ? k : base >= 0 ? 0 : min(k, -base / tokens);
     if (k <= blind) return k;
-    if (tokens > kCellTokens) {
-        const long long whole = (base + 15) >> 4, step = tokens / kCellTokens;
-        return blind + (k - blind) * whole + step * ((long long)k * (k + 1) - (long long)blind * (blind + 1)) / 2;
-    }
-    const int shift = 31 - __clz(tokens), m = kCellTokens >> shift, y = (base + 15) >> shift;
+    const int shift = 31 - __clz(tokens), m = kPairTokens >> shift, y = (base + kPairTokens - 1) >> shift;
     const auto sum = [m](long long n) {  // of floor(i / m) over i = 0 .. n
         if (n < 0) return 0ll;
         const long long q = n / m, r = n % m;
@@ -278,16 +283,24 @@ __device__ __forceinline__ long long cells_before(const SequenceRows& s, int tok
     return blind + sum((long long)y + k) - sum((long long)y + blind);
 }
 
-__device__ __forceinline__ long long sequence_cells(const SequenceRows& s, int tokens) {
+__device__ __forceinline__ long long sequence_pairs(const SequenceRows& s, int tokens) {
     const int tiles = tile_count(s, tokens);
-    return tiles ? cells_before(s, tokens, tiles - 1) + tile_cells(s, tokens, tiles - 1) : 0;
+    return tiles ? pairs_before(s, tokens, tiles - 1) + tile_pairs(s, tokens, tiles - 1) : 0;
 }
 
+// c += a b, and c = a b.
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm volatile(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+__device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 __device__ __forceinline__ uint32_t pack_f16(float low, float high) {
@@ -310,6 +323,23 @@ __device__ __forceinline__ float quad_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
     return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
 }
+// Over the threads of equal lane % 4.
+__device__ __forceinline__ float across_sum(float x) {
+    x += __shfl_xor_sync(0xffffffffu, x, 4);
+    x += __shfl_xor_sync(0xffffffffu, x, 8);
+    return x + __shfl_xor_sync(0xffffffffu, x, 16);
+}
+__device__ __forceinline__ float across_max(float x) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+    return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+}
+// An 8 x 8 matrix of f16, two neighbours of row lane / 4 a thread, transposed.
+__device__ __forceinline__ uint32_t transpose_f16(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
 
 // Sixteen consecutive elements as f32; `wide`: at a 16-byte boundary.
 template <typename T>
@@ -329,18 +359,20 @@ __device__ __forceinline__ void load16(const T* x, bool wide, float (&out)[16]) 
     }
 }
 
-template <typename T, int GROUPS, int MT, bool PAIR>
-__global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT, PAIR>::kBlocksPerSm))
+template <typename T, int GROUPS, int NT, bool LOW>
+__global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT, LOW>::kBlocksPerSm))
     attention_kernel(CacheView c, CacheRows r, AttentionCall call) {
-    using Shape = AttentionShape<GROUPS, MT, PAIR>;
-    constexpr int D = Shape::kDim, RP = PAIR ? 1 : 2, kStages = Shape::kStages;
+    using Shape = AttentionShape<GROUPS, NT, LOW>;
+    constexpr int D = Shape::kDim, kStages = Shape::kStages;
+    constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ long long found[3];
+    __shared__ long long found[2];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32, quad = lane / 4, j = lane % 4;
+    const float nan = std::numeric_limits<float>::quiet_NaN();
     uint8_t* ring = shared + warp * kStages * Shape::kStage;
     float* warp_sums = reinterpret_cast<float*>(shared);
-    uint4* queries = reinterpret_cast<uint4*>(shared + (Shape::kShared - Shape::kQuery - 128 - kAttentionWarps * kStages * 8));
-    uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Shape::kShared - kAttentionWarps * kStages * 8) + warp * kStages;
+    uint32_t* queries = reinterpret_cast<uint32_t*>(shared + Shape::kShared - Shape::kBars - Shape::kQuery);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Shape::kShared - Shape::kBars) + warp * kStages;
     const int tokens = (int)call.tokens;
     const uint32_t tiles_of = c.kv_heads * call.subs;
     pdl_launch_dependents();
@@ -348,11 +380,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT,
         for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
     fence_barrier_init();
 
-    // this block's run of cells
+    // this block's run of pairs
     const uint32_t each = (r.count + kAttentionThreads - 1) / kAttentionThreads;
     const uint32_t mine_first = min(threadIdx.x * each, r.count), mine_end = min(mine_first + each, r.count);
     long long mine = 0;
-    for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_cells(sequence_rows(c, r, b), tokens) * tiles_of;
+    for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_pairs(sequence_rows(c, r, b), tokens) * tiles_of;
     long long* scan = reinterpret_cast<long long*>(shared);
     long long before = mine;
 #pragma unroll
@@ -374,13 +406,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT,
     const long long end = min(at + run, total);
     if (mine > 0 && before <= at && at < before + mine) {
         for (uint32_t b = mine_first; b < mine_end; ++b) {
-            const long long cells = sequence_cells(sequence_rows(c, r, b), tokens) * tiles_of;
-            if (at < before + cells) {
+            const long long pairs = sequence_pairs(sequence_rows(c, r, b), tokens) * tiles_of;
+            if (at < before + pairs) {
                 found[0] = b;
                 found[1] = at - before;
                 break;
             }
-            before += cells;
+            before += pairs;
         }
     }
     if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -388,12 +420,12 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT,
     if (at >= end) return;
     uint32_t b = (uint32_t)found[0];
     long long offset = found[1];
-    uint32_t parity = 0;
-    bool dead = false;  // a copy that did not arrive in time
+    uint32_t phases = 0;  // a bit a stage: the phase that its barrier completes next
+    bool dead = false;    // a copy did not arrive in time
 
     while (at < end) {
         const SequenceRows s = sequence_rows(c, r, b);
-        const long long one = sequence_cells(s, tokens);
+        const long long one = sequence_pairs(s, tokens);
         if (offset >= one * tiles_of) {
             ++b;
             offset = 0;
@@ -402,407 +434,422 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT,
         const uint32_t head_sub = (uint32_t)(offset / one), head = head_sub / call.subs, sub = head_sub % call.subs;
         const long long rest = offset % one;
         int k = 0;
-        for (int high = tile_count(s, tokens); high - k > 1;) {  // cells_before(k) <= rest
+        for (int high = tile_count(s, tokens); high - k > 1;) {  // pairs_before(k) <= rest
             const int middle = (k + high) / 2;
-            if (cells_before(s, tokens, middle) <= rest)
+            if (pairs_before(s, tokens, middle) <= rest)
                 k = middle;
             else
                 high = middle;
         }
-        const int first = (int)(rest - cells_before(s, tokens, k)), cells = tile_cells(s, tokens, k);
-        const int last = (int)min((long long)cells, first + end - at);
+        const int first = (int)(rest - pairs_before(s, tokens, k)), pairs = tile_pairs(s, tokens, k);
+        const int last = (int)min((long long)pairs, first + end - at);
         at += last - first;
         offset += last - first;
 
         // the tile's rows: row i is head sub * rows + i of position k, or head i % group of position k * tokens + i / group
-        const int base = s.length - s.count;
-        const int seen = min(tile_seen(s, tokens, k), (int)min((long long)c.table_width * c.page_size, (long long)INT32_MAX));
+        const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
+        const int covered = (int)min((long long)c.table_width * c.page_size, (long long)INT32_MAX);
+        const int seen = min(base + tile_end, covered);
         const int least = base + k * tokens + 1;  // what the first row sees
         const auto place = [&](int i, int& token, int& h) {
             token = k * tokens + (call.subs > 1 ? 0 : i / (int)call.group);
             h = call.subs > 1 ? (int)sub * Shape::kRows + i : i % (int)call.group;
-            return h < (int)call.group && token < min(s.count, (k + 1) * tokens);
+            return h < (int)call.group && token < tile_end;
         };
-        const bool beyond = s.table < 0 || tile_seen(s, tokens, k) > seen;  // positions that no table entry covers
 
-        uint32_t query[Shape::kSharedQuery ? 1 : MT * GROUPS * 4][4];
-        float factor[MT][RP], zeros_of[MT][RP][GROUPS], most[MT][RP], sum[MT][RP], zeros[MT][RP][GROUPS];
-        int limit[MT][RP];
-        __syncthreads();  // the sums and queries of the tile before are read
-#pragma unroll
-        for (int t = 0; t < MT; ++t) {
-            uint32_t frag[GROUPS * 4][4];
-#pragma unroll
-            for (int p = 0; p < RP; ++p) {
-                const int i = t * (PAIR ? 8 : 16) + p * 8 + quad;
-                int token, h;
-                const bool row = place(i, token, h);
-                limit[t][p] = row ? base + token + 1 : 0;
-                const T* x = static_cast<const T*>(call.q) + (size_t)(s.first + token) * call.q_row +
-                             (size_t)(head * call.group + h) * call.q_head + 16 * j;
-                float values[GROUPS][16], top = 0.f;
-                bool fine = true;
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    if (row) {
-                        load16(x + 64 * g, call.wide, values[g]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) values[g][e] = 0.f;
+        // ---- the stream of pairs: warp w takes pairs first + w, first + w + 4, ..
+        const int stop = min(last, (seen + kPairTokens - 1) >> 5);  // pairs beyond hold nothing
+        const int mine_pairs = max(0, (stop - first - warp + kAttentionWarps - 1) / kAttentionWarps);
+        const uint32_t per_page = c.page_size / kCellTokens;
+        const bool together = per_page % 2 == 0;  // both cells lie in one page, one behind the other
+        const int32_t* table = c.tables + (size_t)max(s.table, 0) * c.table_width;
+        const uint32_t seen_cells = (uint32_t)max((seen + kCellTokens - 1) >> 4, 0);
+        const auto cell_of_pair = [&](int n) { return 2u * (uint32_t)(first + warp + n * kAttentionWarps); };
+        const auto page_of = [&](int n, uint32_t half) {  // of this warp's n-th pair
+            const uint32_t cell = cell_of_pair(n) + half;
+            return n < mine_pairs && cell < seen_cells ? (uint32_t)table[cell / per_page] : 0xffffffffu;
+        };
+        uint32_t pages = page_of(lane, 0), others = together ? 0 : page_of(lane, 1);
+        uint32_t within = cell_of_pair(0) % per_page;  // the next copy's first cell in its page
+        const uint32_t step_within = 2 * kAttentionWarps % per_page;
+        const uint8_t* head_cells = c.pages + (size_t)head * per_page * Shape::kCell;
+        const size_t page_bytes = (size_t)c.kv_heads * per_page * Shape::kCell;
+        int issued = 0, into = 0;
+        uint32_t gone = 0;  // two bits a stage: cells without a page
+        const auto issue = [&] {
+            if (issued >= mine_pairs || dead) return;
+            const uint32_t page = __shfl_sync(0xffffffffu, pages, issued & 31);
+            const uint32_t other = together ? page : __shfl_sync(0xffffffffu, others, issued & 31);
+            const uint32_t none = (page < c.page_count ? 0u : 1u) | (other < c.page_count ? 0u : 2u);
+            gone = (gone & ~(3u << 2 * into)) | none << 2 * into;
+            if (lane == 0) {
+                uint8_t* to = ring + into * Shape::kStage;
+                const uint8_t* from = head_cells + page * page_bytes + within * Shape::kCell;
+                if (none == 3) {
+                    mbar_arrive(bars + into);
+                } else if (together) {
+                    mbar_expect_tx(bars + into, Shape::kStage);
+                    bulk_load(to, from, Shape::kStage, bars + into);
+                } else {
+                    mbar_expect_tx(bars + into, none ? Shape::kCell : Shape::kStage);
+                    if (!(none & 1)) bulk_load(to, from, Shape::kCell, bars + into);
+                    if (!(none & 2)) {
+                        const uint32_t second = within + 1 == per_page ? 0 : within + 1;
+                        bulk_load(to + Shape::kCell, head_cells + other * page_bytes + second * Shape::kCell, Shape::kCell, bars + into);
                     }
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        top = fmaxf(top, fabsf(values[g][e]));
-                        fine = fine && isfinite(values[g][e]);
-                    }
-                }
-                top = quad_max(top);
-                fine = quad_max(fine ? 0.f : 1.f) == 0.f;
-                // 2^power takes the largest into 2^13 .. 2^14
-                const int exponent = top > 0.f ? max(ilogbf(top), -100) : 0;
-                const int power = fine ? 13 - exponent : 0;
-                const float up = fine ? ldexpf(1.f, power) : 0.f;
-                factor[t][p] = fine ? call.scale * ldexpf(1.f, 24 - power) : std::numeric_limits<float>::quiet_NaN();
-                most[t][p] = -INFINITY;
-                sum[t][p] = 0.f;
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    float plain = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) {
-                        values[g][e] = fine ? values[g][e] * up : 0.f;
-                        plain += values[g][e];
-                    }
-                    zeros_of[t][p][g] = quad_sum(plain) * 0x1p-24f;
-                    zeros[t][p][g] = 0.f;
-                    // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
-#pragma unroll
-                    for (int w = 0; w < 2; ++w)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float down = e ? 0.0625f : 1.f;
-                            const float* y = values[g] + 8 * w + e;
-                            const float y0 = y[0] * down, y4 = y[4] * down, y2 = y[2] * down, y6 = y[6] * down;
-                            uint32_t(&f)[4] = frag[(g * 2 + w) * 2 + e];
-                            f[p] = pack_f16(y0, y4);
-                            f[2 + p] = pack_f16(y2, y6);
-                            if (PAIR) {
-                                const float2 a = unpack_f16(f[0]), d = unpack_f16(f[2]);
-                                f[1] = pack_f16(y0 - a.x, y4 - a.y);
-                                f[3] = pack_f16(y2 - d.x, y6 - d.y);
-                            }
-                        }
                 }
             }
+            within += step_within;
+            if (within >= per_page) within -= per_page;
+            into = into + 1 == kStages ? 0 : into + 1;
+            if ((++issued & 31) == 0) {
+                pages = page_of(issued + lane, 0);
+                if (!together) others = page_of(issued + lane, 1);
+            }
+        };
+        fence_proxy_async_shared();  // the ring held other things
+        __syncthreads();             // which all threads have read
+#pragma unroll 1
+        for (int n = 0; n < kStages - 1; ++n) issue();
+
+        // ---- queries: the thread's columns of the score products are rows 2 j and 2 j + 1 of each eight
+        uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][LOW ? 4 : 2];
+        float factor[NT][2], plain[NT][2][GROUPS];
+        int limit[NT][2];
 #pragma unroll
-            for (int f = 0; f < GROUPS * 4; ++f) {
-                if constexpr (Shape::kSharedQuery) {
-                    if (warp == 0)
-                        queries[(t * GROUPS * 4 + f) * 32 + lane] = make_uint4(frag[f][0], frag[f][1], frag[f][2], frag[f][3]);
+        for (int t = 0; t < NT; ++t) {
+            int token, h;
+            const bool row = place(8 * t + quad, token, h);
+            const T* x = static_cast<const T*>(call.q) + (size_t)(s.first + token) * call.q_row +
+                         (size_t)(head * call.group + h) * call.q_head + 16 * j;
+            float values[GROUPS][16], top = 0.f;
+            bool fine = true;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                if (row) {
+                    load16(x + 64 * g, call.wide, values[g]);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) query[t * GROUPS * 4 + f][i] = frag[f][i];
+                    for (int e = 0; e < 16; ++e) values[g][e] = 0.f;
                 }
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    top = fmaxf(top, fabsf(values[g][e]));
+                    fine = fine && isfinite(values[g][e]);
+                }
+            }
+            top = quad_max(top);
+            fine = quad_max(fine ? 0.f : 1.f) == 0.f;
+            // 2^power takes the largest into 2^13 .. 2^14
+            const int power = fine && top > 0.f ? 13 - max(ilogbf(top), -100) : 0;
+            const float up = ldexpf(1.f, power);
+            const float of_row = fine ? call.scale * ldexpf(1.f, 24 - power) : nan;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                factor[t][i] = __shfl_sync(0xffffffffu, of_row, (2 * j + i) * 4);
+                limit[t][i] = __shfl_sync(0xffffffffu, row ? base + token + 1 : 0, (2 * j + i) * 4);
+            }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                float all = 0.f;
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    values[g][e] = fine ? values[g][e] * up : 0.f;
+                    all += values[g][e];
+                }
+                all = quad_sum(all) * 0x1p-24f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) plain[t][i][g] = __shfl_sync(0xffffffffu, all, (2 * j + i) * 4);
+                // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
+#pragma unroll
+                for (int w = 0; w < 2; ++w)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const float down = e ? 0.0625f : 1.f;
+                        const float* y = values[g] + 8 * w + e;
+                        const float y0 = y[0] * down, y4 = y[4] * down, y2 = y[2] * down, y6 = y[6] * down;
+                        const int f = (t * GROUPS + g) * 4 + w * 2 + e;
+                        uint32_t x0 = pack_f16(y0, y4), x1 = pack_f16(y2, y6), l0 = 0, l1 = 0;
+                        if (LOW) {
+                            const float2 a = unpack_f16(x0), d = unpack_f16(x1);
+                            l0 = pack_f16(y0 - a.x, y4 - a.y);
+                            l1 = pack_f16(y2 - d.x, y6 - d.y);
+                        }
+                        if constexpr (Shape::kSharedQuery) {
+                            if (warp == f % kAttentionWarps) {
+                                if constexpr (LOW)
+                                    reinterpret_cast<uint4*>(queries)[f * 32 + lane] = make_uint4(x0, x1, l0, l1);
+                                else
+                                    reinterpret_cast<uint2*>(queries)[f * 32 + lane] = make_uint2(x0, x1);
+                            }
+                        } else {
+                            query[f][0] = x0, query[f][1] = x1;
+                            if constexpr (LOW) query[f][2] = l0, query[f][3] = l1;
+                        }
+                    }
             }
         }
         if constexpr (Shape::kSharedQuery) __syncthreads();
 
-        float out[MT][8 * GROUPS][4];
+        float out[NT][4 * GROUPS][4], reference[NT][2], sum[NT][2], zeros[NT][2][GROUPS];
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < NT; ++t) {
 #pragma unroll
-            for (int n = 0; n < 8 * GROUPS; ++n)
+            for (int n = 0; n < 4 * GROUPS; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) out[t][n][i] = 0.f;
-        uint32_t step_limit = 0;  // largest step (f16 bits) that p s times `lift` may hold
-        float lift = 0.f;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                reference[t][i] = kNone;
+                sum[t][i] = 0.f;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) zeros[t][i][g] = 0.f;
+            }
+        }
 
-        // ---- the stream of cells
-        const int stop = min(last, (seen + kCellTokens - 1) >> 4);  // cells beyond hold nothing
-        const int mine_cells = max(0, (stop - first - warp + kAttentionWarps - 1) / kAttentionWarps);
-        const uint32_t per_page = c.page_size / kCellTokens;
-        const auto page_of = [&](int n) {  // of this warp's n-th cell
-            if (n >= mine_cells) return 0xffffffffu;
-            const uint32_t cell = (uint32_t)(first + warp + n * kAttentionWarps);
-            return (uint32_t)c.tables[(size_t)s.table * c.table_width + cell / per_page];
-        };
-        uint32_t pages = page_of(lane), next_pages = page_of(32 + lane), gone = 0;
-        const auto issue = [&](int n) {
-            if (n >= mine_cells || dead) return;
-            if (n % 32 == 0 && n > 0) {
-                pages = next_pages;
-                next_pages = page_of(n + 32 + lane);
-            }
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, n % 32);
-            const int stage = n % kStages;
-            if (page >= c.page_count) {
-                gone |= 1u << stage;
-                return;
-            }
-            gone &= ~(1u << stage);
-            if (lane == 0) {
-                const uint32_t cell = (uint32_t)(first + warp + n * kAttentionWarps);
-                const uint8_t* from = c.pages + (((size_t)page * c.kv_heads + head) * per_page + cell % per_page) * Shape::kStage;
-                mbar_expect_tx(bars + stage, Shape::kStage);
-                bulk_load(ring + stage * Shape::kStage, from, Shape::kStage, bars + stage);
-            }
-        };
-        fence_proxy_async_shared();  // the warps' sums lay in the ring
-        __syncthreads();
-#pragma unroll 1
-        for (int n = 0; n < kStages - 1; ++n) issue(n);
+        int stage = 0;
+        const uint32_t pick = quad & 1 ? 0x7632u : 0x5410u;  // a thread's position among two: its step and zero
 
-#pragma unroll 1
-        for (int n = 0; n < mine_cells; ++n) {
-            __syncwarp();
-            issue(n + kStages - 1);
-            const int stage = n % kStages, cell = first + warp + n * kAttentionWarps;
-            const bool here = !(gone >> stage & 1);
-            if (!dead && here) {
-                dead = !mbar_wait_bounded(bars + stage, parity >> stage & 1);
-                parity ^= 1u << stage;
-            }
-            dead = __any_sync(0xffffffffu, dead);
-            if (!here || dead) {
+        // kAtOnce cells at `held`, the first of them at position `start`.  EDGE: some row does not see all of
+        // their positions, or one is missing (bits of `none`).
+        const auto take = [&](auto edge_tag, const uint8_t* held, int start, uint32_t none) {
+            constexpr bool EDGE = decltype(edge_tag)::value;
+            constexpr int U = Shape::kAtOnce;
+            const int position = start + quad;  // the thread's positions: this and every eighth on
+            const auto there = [&](int u, int i) { return position + 16 * u + 8 * i < seen && !(none >> u & 1); };
+            // scores [row 2 j, 2 j + 1 of position, of position + 8], in units that `factor` takes to powers of two
+            float score[U][NT][4];
+            __half2 values[U][GROUPS][2];  // the values' steps and zeros
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int p = 0; p < RP; ++p)
-                        if (dead || cell * kCellTokens < limit[t][p]) sum[t][p] = std::numeric_limits<float>::quiet_NaN();
-                if (!dead) continue;
-                for (int later = n + 1; here && later < min(n + kStages, mine_cells); ++later)  // what is in flight lands first
-                    if (!(gone >> later % kStages & 1)) mbar_wait_bounded(bars + later % kStages, parity >> later % kStages & 1);
-                break;
-            }
-            const uint8_t* held = ring + stage * Shape::kStage;
-            const int position = cell * kCellTokens + 2 * j;
-            const bool edge = (cell + 1) * kCellTokens > least;  // some row does not see all of it
-
-            // scores, in units that `factor` takes to powers of two: [row][2 j, 2 j + 1, 2 j + 8, 2 j + 9]
-            float score[MT][RP][4];
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int p = 0; p < RP; ++p)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) score[t][p][i] = 0.f;
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const uint4 words = *reinterpret_cast<const uint4*>(held + (g * 32 + lane) * 16);
-                const uint4 raw = *reinterpret_cast<const uint4*>(held + cell_key_steps(D) + g * 64 + j * 16);
-                const float2 s0 = unpack_f16(raw.x), z0 = unpack_f16(raw.y), s1 = unpack_f16(raw.z), z1 = unpack_f16(raw.w);
-                const float step[4] = {s0.x, s0.y, s1.x, s1.y}, zero[4] = {z0.x, z0.y, z1.x, z1.y};
-                float dot[MT][2][4];
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) dot[t][0][i] = dot[t][1][i] = 0.f;
-#pragma unroll
-                for (int w = 0; w < 2; ++w) {
-                    const uint32_t low = w ? words.y : words.x, high = w ? words.w : words.z;  // positions quad, quad + 8
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
-#pragma unroll
-                        for (int t = 0; t < MT; ++t) {
-                            uint32_t a[4];
-                            const int f = t * GROUPS * 4 + (g * 2 + w) * 2 + e;
-                            if constexpr (Shape::kSharedQuery) {
-                                const uint4 x = queries[f * 32 + lane];
-                                a[0] = x.x, a[1] = x.y, a[2] = x.z, a[3] = x.w;
-                            } else {
-                                a[0] = query[f][0], a[1] = query[f][1], a[2] = query[f][2], a[3] = query[f][3];
-                            }
-                            mma_f16(dot[t][0], a, low & mask, low >> 8 & mask);
-                            mma_f16(dot[t][1], a, high & mask, high >> 8 & mask);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int p = 0; p < RP; ++p)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float d = PAIR ? dot[t][i / 2][i % 2] + dot[t][i / 2][2 + i % 2] : dot[t][i / 2][2 * p + i % 2];
-                            score[t][p][i] = fmaf(step[i], d, fmaf(zero[i], zeros_of[t][p][g], score[t][p][i]));
-                        }
-            }
-            // weights
-            bool grows = false;
-            float now[MT][RP];
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int p = 0; p < RP; ++p) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) score[t][p][i] *= factor[t][p];
-                    if (edge) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-                            if (position + i / 2 * 8 + i % 2 >= limit[t][p]) score[t][p][i] = -INFINITY;
-                    }
-                    const float top = fmaxf(fmaxf(score[t][p][0], score[t][p][1]), fmaxf(score[t][p][2], score[t][p][3]));
-                    now[t][p] = fmaxf(most[t][p], quad_max(top));
-                    grows = grows || now[t][p] > most[t][p];
-                }
-            if (__any_sync(0xffffffffu, grows)) {
-#pragma unroll
-                for (int t = 0; t < MT; ++t)
-#pragma unroll
-                    for (int p = 0; p < RP; ++p) {
-                        const float keep = now[t][p] > most[t][p] ? exp2_approx(most[t][p] - now[t][p]) : 1.f;
-                        most[t][p] = now[t][p];
-                        sum[t][p] *= keep;
-#pragma unroll
-                        for (int g = 0; g < GROUPS; ++g) zeros[t][p][g] *= keep;
-#pragma unroll
-                        for (int n = 0; n < 8 * GROUPS; ++n) {
-                            if (PAIR) {
-#pragma unroll
-                                for (int i = 0; i < 4; ++i) out[t][n][i] *= keep;
-                            } else {
-                                out[t][n][2 * p] *= keep;
-                                out[t][n][2 * p + 1] *= keep;
-                            }
-                        }
-                    }
-            }
-#pragma unroll
-            for (int t = 0; t < MT; ++t)
-#pragma unroll
-                for (int p = 0; p < RP; ++p) {
-                    const float against = most[t][p] == -INFINITY ? 0.f : most[t][p];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        score[t][p][i] = exp2_approx(score[t][p][i] - against);
-                        sum[t][p] += score[t][p][i];
-                    }
-                }
-            // the values' steps; where one is larger than any before, the sums are scaled down
-            uint4 raw[GROUPS];
-            uint32_t top_step = 0;
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                raw[g] = *reinterpret_cast<const uint4*>(held + cell_value_steps(D) + g * 64 + j * 16);
-                if (edge) {  // positions that no row sees may hold anything
-                    const auto cut = [&](uint32_t x, int from) {
-                        return x & (from < seen ? 0xffffu : 0u) | x & (from + 1 < seen ? 0xffff0000u : 0u);
-                    };
-                    raw[g].x = cut(raw[g].x, position), raw[g].y = cut(raw[g].y, position);
-                    raw[g].z = cut(raw[g].z, position + 8), raw[g].w = cut(raw[g].w, position + 8);
-                }
-                top_step = __vmaxu2(top_step, __vmaxu2(raw[g].x, raw[g].z));
-            }
-            top_step = max(top_step & 0xffffu, top_step >> 16);
-            if (__any_sync(0xffffffffu, top_step > step_limit)) {
-                // NaN steps make their products NaN and count for nothing here; 2^k <= the largest < 2^(k + 1)
-                uint32_t largest = 0;
+            for (int u = 0; u < U; ++u) {
+                const uint8_t* cell = held + u * Shape::kCell;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const uint32_t all[4] = {raw[g].x & 0xffffu, raw[g].x >> 16, raw[g].z & 0xffffu, raw[g].z >> 16};
+                    const uint4 words = *reinterpret_cast<const uint4*>(cell + (g * 32 + lane) * 16);
+                    const uint4 raw = *reinterpret_cast<const uint4*>(cell + cell_key_steps(D) + g * 64 + quad / 2 * 16);
+                    const float2 sz0 = unpack_f16(__byte_perm(raw.x, raw.y, pick)), sz1 = unpack_f16(__byte_perm(raw.z, raw.w, pick));
+                    float dot[NT][4];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        if (all[i] < 0x7c00u) largest = max(largest, all[i]);
+                    for (int w = 0; w < 2; ++w) {
+                        const uint32_t low = w ? words.y : words.x, high = w ? words.w : words.z;
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
+                            const uint32_t a[4] = {low & mask, high & mask, low >> 8 & mask, high >> 8 & mask};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                const int f = (n * GROUPS + g) * 4 + w * 2 + e;
+                                uint32_t b0, b1, b2 = 0, b3 = 0;
+                                if constexpr (Shape::kSharedQuery && LOW) {
+                                    const uint4 x = reinterpret_cast<const uint4*>(queries)[f * 32 + lane];
+                                    b0 = x.x, b1 = x.y, b2 = x.z, b3 = x.w;
+                                } else if constexpr (Shape::kSharedQuery) {
+                                    const uint2 x = reinterpret_cast<const uint2*>(queries)[f * 32 + lane];
+                                    b0 = x.x, b1 = x.y;
+                                } else {
+                                    b0 = query[f][0], b1 = query[f][1];
+                                    if constexpr (LOW) b2 = query[f][2], b3 = query[f][3];
+                                }
+                                if (w + e == 0)
+                                    mma_f16_first(dot[n], a, b0, b1);
+                                else
+                                    mma_f16(dot[n], a, b0, b1);
+                                if constexpr (LOW) mma_f16(dot[n], a, b2, b3);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float z0 = sz0.y * plain[n][i][g], z1 = sz1.y * plain[n][i][g];
+                            score[u][n][i] = fmaf(sz0.x, dot[n][i], g ? score[u][n][i] + z0 : z0);
+                            score[u][n][2 + i] = fmaf(sz1.x, dot[n][2 + i], g ? score[u][n][2 + i] + z1 : z1);
+                        }
                 }
-                largest = __reduce_max_sync(0xffffffffu, largest);
-                if (largest > step_limit) {
-                    const uint32_t e = max(largest >> 10, 1u);
-                    const float next = ldexpf(1.f, 29 - (int)e);
-                    const float keep = lift > 0.f ? next / lift : 0.f;
-                    lift = next;
-                    step_limit = ((e + 1) << 10) - 1;
 #pragma unroll
-                    for (int t = 0; t < MT; ++t)
+                for (int g = 0; g < GROUPS; ++g) {
+                    const uint4 raw = *reinterpret_cast<const uint4*>(cell + cell_value_steps(D) + g * 64 + quad / 2 * 16);
+                    uint32_t sz[2] = {__byte_perm(raw.x, raw.y, pick), __byte_perm(raw.z, raw.w, pick)};
 #pragma unroll
-                        for (int n = 0; n < 8 * GROUPS; ++n)
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) out[t][n][i] *= keep;
+                    for (int i = 0; i < 2; ++i) {
+                        if (EDGE && !there(u, i)) sz[i] = 0;  // what no row sees may hold anything
+                        values[u][g][i] = *reinterpret_cast<__half2*>(&sz[i]);
+                    }
                 }
             }
+            // weights
+            float weight[U][NT][4], most = 0.f;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                const float2 s0 = unpack_f16(raw[g].x), z0 = unpack_f16(raw[g].y), s1 = unpack_f16(raw[g].z),
-                             z1 = unpack_f16(raw[g].w);
-                const float step[4] = {s0.x * lift, s0.y * lift, s1.x * lift, s1.y * lift};
-                const float zero[4] = {z0.x, z0.y, z1.x, z1.y};
-                uint32_t a[MT][4];
+            for (int u = 0; u < U; ++u)
 #pragma unroll
-                for (int t = 0; t < MT; ++t)
+                for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int p = 0; p < RP; ++p) {
+                    for (int i = 0; i < 4; ++i) {
+                        score[u][n][i] *= factor[n][i % 2];
+                        if (EDGE && !(there(u, i / 2) && position + 16 * u + i / 2 * 8 < limit[n][i % 2])) score[u][n][i] = -INFINITY;
+                        weight[u][n][i] = exp2_approx(score[u][n][i] - reference[n][i % 2]);
+                        most = fmaxf(most, weight[u][n][i]);
+                    }
+            __half2 steps = values[0][0][0];
+#pragma unroll
+            for (int i = 1; i < 2 * U * GROUPS; ++i) steps = __hmax2(steps, values[i / (2 * GROUPS)][i / 2 % GROUPS][i % 2]);
+            const float largest = fmaxf(__low2float(steps), 0x1p-30f);
+            if (__any_sync(0xffffffffu, !(most * largest < 0x1p15f))) {
+                const float all = quad_max(across_max(largest));
+                const float above = (float)(ilogbf(all) + 1);  // 2^above is above these steps
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float top = fmaxf(score[0][n][i], score[0][n][2 + i]);
+                        if (U == 2) top = fmaxf(top, fmaxf(score[U - 1][n][i], score[U - 1][n][2 + i]));
+                        top = across_max(top);
+                        const float next = fmaxf(reference[n][i], top + above - 10.f);
+                        const float keep = exp2_approx(reference[n][i] - next);
+                        reference[n][i] = next;
+                        sum[n][i] *= keep;
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) zeros[n][i][g] *= keep;
+#pragma unroll
+                        for (int m = 0; m < 4 * GROUPS; ++m) {
+                            out[n][m][i] *= keep;
+                            out[n][m][2 + i] *= keep;
+                        }
+#pragma unroll
+                        for (int u = 0; u < U; ++u) {
+                            weight[u][n][i] = exp2_approx(score[u][n][i] - next);
+                            weight[u][n][2 + i] = exp2_approx(score[u][n][2 + i] - next);
+                        }
+                    }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float more = weight[0][n][i] + weight[0][n][2 + i];
+                    if (U == 2) more += weight[U - 1][n][i] + weight[U - 1][n][2 + i];
+                    sum[n][i] += more;
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint8_t* cell = held + u * Shape::kCell;
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g) {
+                    const float2 sz[2] = {__half22float2(values[u][g][0]), __half22float2(values[u][g][1])};
+                    uint32_t p0[NT], p1[NT], l0[NT], l1[NT];
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
                         float x[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            x[i] = score[t][p][i] * step[i];
-                            float y = score[t][p][i] * zero[i];
+                            x[i] = weight[u][n][i] * sz[i / 2].x;
                             // a position that this row does not see adds nothing, whatever it holds
-                            if (edge && position + i / 2 * 8 + i % 2 >= limit[t][p]) x[i] = y = 0.f;
-                            zeros[t][p][g] += y;
+                            const bool blind = EDGE && position + 16 * u + i / 2 * 8 >= limit[n][i % 2];
+                            if (blind) x[i] = 0.f;
+                            else zeros[n][i % 2][g] = fmaf(weight[u][n][i], sz[i / 2].y, zeros[n][i % 2][g]);
                         }
-                        a[t][p] = pack_f16(x[0], x[1]);
-                        a[t][2 + p] = pack_f16(x[2], x[3]);
-                        if (PAIR) {
-                            const float2 d = unpack_f16(a[t][0]), e = unpack_f16(a[t][2]);
-                            a[t][1] = pack_f16(x[0] - d.x, x[1] - d.y);
-                            a[t][3] = pack_f16(x[2] - e.x, x[3] - e.y);
+                        p0[n] = pack_f16(x[0], x[1]);
+                        p1[n] = pack_f16(x[2], x[3]);
+                        if constexpr (LOW) {
+                            const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
+                            l0[n] = transpose_f16(pack_f16(x[0] - a.x, x[1] - a.y));
+                            l1[n] = transpose_f16(pack_f16(x[2] - d.x, x[3] - d.y));
+                        }
+                        p0[n] = transpose_f16(p0[n]);
+                        p1[n] = transpose_f16(p1[n]);
+                    }
+                    const uint4 words = *reinterpret_cast<const uint4*>(cell + cell_values(D) + (g * 32 + lane) * 16);
+                    const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        const uint32_t a[4] = {word[w] & 0x000f000fu, word[w] & 0x00f000f0u, word[w] >> 8 & 0x000f000fu,
+                                               word[w] >> 8 & 0x00f000f0u};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) {
+                            mma_f16(out[n][g * 4 + w], a, p0[n], p1[n]);
+                            if constexpr (LOW) mma_f16(out[n][g * 4 + w], a, l0[n], l1[n]);
                         }
                     }
-                const uint4 words = *reinterpret_cast<const uint4*>(held + cell_values(D) + (g * 32 + lane) * 16);
-                const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+                }
+            }
+        };
+
+#pragma unroll 1
+        for (int n = 0; n < mine_pairs; ++n) {
+            __syncwarp();
+            issue();
+            const int pair = first + warp + n * kAttentionWarps;
+            const uint8_t* held = ring + stage * Shape::kStage;
+            uint32_t none = gone >> 2 * stage & 3;
+            if (!dead) dead = !mbar_wait_bounded(bars + stage, phases >> stage & 1);
+            phases ^= 1u << stage;
+            stage = stage + 1 == kStages ? 0 : stage + 1;
+            if (__any_sync(0xffffffffu, dead)) {  // what is in flight lands first
+                dead = true;
+                for (; ++n < issued; stage = stage + 1 == kStages ? 0 : stage + 1)
+                    mbar_wait_bounded(bars + stage, phases >> stage & 1);
 #pragma unroll
-                for (int w = 0; w < 4; ++w)
+                for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = nan;
+                break;
+            }
+            if (none | ((pair + 1) * kPairTokens > least)) {
 #pragma unroll
-                    for (int t = 0; t < MT; ++t) {
-                        mma_f16(out[t][(g * 4 + w) * 2], a[t], word[w] & 0x000f000fu, word[w] >> 8 & 0x000f000fu);
-                        mma_f16(out[t][(g * 4 + w) * 2 + 1], a[t], word[w] & 0x00f000f0u, word[w] >> 8 & 0x00f000f0u);
+                for (int t = 0; t < NT; ++t)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int sees = min(limit[t][i], seen);  // a missing cell among what the row sees
+                        if ((none & 1 && pair * kPairTokens < sees) || (none & 2 && pair * kPairTokens + kCellTokens < sees)) sum[t][i] = nan;
                     }
+#pragma unroll 1
+                for (int u = 0; u < 2; u += Shape::kAtOnce)
+                    take(std::true_type{}, held + u * Shape::kCell, pair * kPairTokens + u * kCellTokens, none >> u);
+            } else {
+#pragma unroll 1
+                for (int u = 0; u < 2; u += Shape::kAtOnce)
+                    take(std::false_type{}, held + u * Shape::kCell, pair * kPairTokens + u * kCellTokens, 0);
             }
         }
-        if (beyond) {
+        // rows that see positions which no table entry covers, or whose sequence has no table
 #pragma unroll
-            for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-                for (int p = 0; p < RP; ++p)
-                    if (s.table < 0 || limit[t][p] > seen) sum[t][p] = std::numeric_limits<float>::quiet_NaN();
-        }
+            for (int i = 0; i < 2; ++i)
+                if (s.table < 0 || limit[t][i] > covered) sum[t][i] = nan;
 
         // ---- the warps' sums
-        const float even = lift > 0.f ? 0x1p24f / lift : 0.f, odd = even * 0.0625f;
         __syncthreads();  // the rings are drained
         float* mine_sums = warp_sums + warp * Shape::kRows * (D + 2);
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
+        for (int t = 0; t < NT; ++t)
 #pragma unroll
-            for (int p = 0; p < RP; ++p) {
-                float* row = mine_sums + (t * (PAIR ? 8 : 16) + p * 8 + quad) * (D + 2);
-                const float l = quad_sum(sum[t][p]);
-                if (j == 0) row[D] = most[t][p], row[D + 1] = l;
+            for (int i = 0; i < 2; ++i) {
+                float* row = mine_sums + (8 * t + 2 * j + i) * (D + 2);
+                const float l = across_sum(sum[t][i]);
+                if (quad == 0) row[D] = reference[t][i], row[D + 1] = l;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const float z = quad_sum(zeros[t][p][g]);
+                    const float z = across_sum(zeros[t][i][g]);
 #pragma unroll
-                    for (int n = 8 * g; n < 8 * g + 8; ++n) {
-                        const float up = n % 2 ? odd : even;
-                        const float x = PAIR ? out[t][n][0] + out[t][n][2] : out[t][n][2 * p];
-                        const float y = PAIR ? out[t][n][1] + out[t][n][3] : out[t][n][2 * p + 1];
-                        *reinterpret_cast<float2*>(row + 8 * n + 2 * j) = make_float2(fmaf(x, up, z), fmaf(y, up, z));
+                    for (int m = 4 * g; m < 4 * g + 4; ++m) {
+                        row[16 * m + quad] = fmaf(out[t][m][i], 0x1p24f, z);
+                        row[16 * m + 8 + quad] = fmaf(out[t][m][2 + i], 0x1p20f, z);
                     }
                 }
             }
         __syncthreads();
-        const bool whole = first == 0 && last == cells;
+        const bool whole = first == 0 && last == pairs;
         float* part = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * Shape::kRows * (D + 2);
         for (int i = warp; i < Shape::kRows; i += kAttentionWarps) {
             int token, h;
             if (!place(i, token, h)) continue;
-            float top = -INFINITY, l = 0.f, weight[kAttentionWarps];
+            float top = kNone, l = 0.f, weight[kAttentionWarps];
 #pragma unroll
             for (int w = 0; w < kAttentionWarps; ++w) top = fmaxf(top, warp_sums[(w * Shape::kRows + i) * (D + 2) + D]);
 #pragma unroll
             for (int w = 0; w < kAttentionWarps; ++w) {
                 const float* row = warp_sums + (w * Shape::kRows + i) * (D + 2);
-                weight[w] = exp2_approx(row[D] - (top == -INFINITY ? 0.f : top));
+                weight[w] = exp2_approx(row[D] - top);
                 l += weight[w] * row[D + 1];
             }
             const float inverse = l == 0.f ? 0.f : 1.f / l;
@@ -820,19 +867,19 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, MT,
             if (!whole && lane == 0) part[(size_t)i * (D + 2) + D] = top, part[(size_t)i * (D + 2) + D + 1] = l;
         }
         if (first == 0 && !whole && threadIdx.x == 0)
-            call.tails[blockIdx.x] = make_int4(1 + (int)((cells - last + run - 1) / run), (int)b, (int)head_sub, k);
+            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), (int)b, (int)head_sub, k);
     }
 }
 
-// Adds up the parts of the tile that block blockIdx.x of attention_kernel started and others
-// finished, in their order; a block a row, a warp every eighth part.
-constexpr int kMergeWarps = 8;
+// Adds up the parts of the tile that a block of attention_kernel started and others
+// finished, in their order; a block a row, a warp every fourth part.
+constexpr int kMergeWarps = 4;
 
 template <typename T>
 __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(CacheView c, CacheRows r, AttentionCall call,
                                                                            int rows) {
     pdl_wait();
-    const int block = (int)blockIdx.x / rows, i = (int)blockIdx.x % rows, D = (int)c.dim;
+    const int block = (int)(blockIdx.x / call.used), i = (int)(blockIdx.x % call.used), D = (int)c.dim;
     const int4 tail = call.tails[block];
     if (tail.x == 0) return;
     const SequenceRows s = sequence_rows(c, r, (uint32_t)tail.y);
@@ -842,14 +889,11 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Cache
     if (h >= (int)call.group || token >= min(s.count, (k + 1) * tokens)) return;
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
     __shared__ float sums[kMergeWarps][kMaxCacheDim + 2];
-    const auto part = [&](int n) {
-        return call.parts + (((size_t)(block + n) * 2 + (n == 0)) * rows + i) * (D + 2);
-    };
-    float top = -INFINITY, l = 0.f, x[kMaxCacheDim / 32] = {};
+    float top = -1e30f, l = 0.f, x[kMaxCacheDim / 32] = {};
+#pragma unroll 4
     for (int n = warp; n < tail.x; n += kMergeWarps) {
-        const float* p = part(n);
-        const float m = p[D], now = fmaxf(top, m), against = now == -INFINITY ? 0.f : now;
-        const float keep = exp2_approx(top - against), weight = exp2_approx(m - against);
+        const float* p = call.parts + (((size_t)(block + n) * 2 + (n == 0)) * rows + i) * (D + 2);
+        const float m = p[D], now = fmaxf(top, m), keep = exp2_approx(top - now), weight = exp2_approx(m - now);
         top = now;
         l = l * keep + p[D + 1] * weight;
 #pragma unroll
@@ -861,13 +905,13 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Cache
         if (e * 32 < D) sums[warp][e * 32 + lane] = x[e];
     if (lane == 0) sums[warp][kMaxCacheDim] = top, sums[warp][kMaxCacheDim + 1] = l;
     __syncthreads();
-    top = -INFINITY, l = 0.f;
+    top = -1e30f, l = 0.f;
     float weight[kMergeWarps];
 #pragma unroll
     for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, sums[w][kMaxCacheDim]);
 #pragma unroll
     for (int w = 0; w < kMergeWarps; ++w) {
-        weight[w] = exp2_approx(sums[w][kMaxCacheDim] - (top == -INFINITY ? 0.f : top));
+        weight[w] = exp2_approx(sums[w][kMaxCacheDim] - top);
         l += weight[w] * sums[w][kMaxCacheDim + 1];
     }
     T* to = static_cast<T*>(call.out) + (size_t)(s.first + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
@@ -1223,30 +1267,40 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
 
 // Blocks of attention_kernel on the card, and its workspace: the blocks' tails and two
 // parts each.
-template <int GROUPS, int MT, bool PAIR>
+template <int GROUPS, int NT, bool LOW>
 size_t attention_bytes(int sm_count) {
-    using Shape = AttentionShape<GROUPS, MT, PAIR>;
+    using Shape = AttentionShape<GROUPS, NT, LOW>;
     return (size_t)sm_count * Shape::kBlocksPerSm * (16 + 2 * Shape::kRows * (Shape::kDim + 2) * 4);
+}
+
+template <int GROUPS>
+size_t attention_bytes(int sm_count) {
+    constexpr int kMost = GROUPS <= 2 ? 4 : 2;
+    return std::max({attention_bytes<GROUPS, 1, false>(sm_count), attention_bytes<GROUPS, 2, false>(sm_count),
+                     attention_bytes<GROUPS, kMost, false>(sm_count), attention_bytes<GROUPS, 1, true>(sm_count),
+                     attention_bytes<GROUPS, 2, true>(sm_count)});
 }
 
 size_t attention_workspace(int sm_count, size_t dim) {
     switch (dim / kCacheGroup) {
-    case 1: return std::max(attention_bytes<1, 1, true>(sm_count), attention_bytes<1, 2, false>(sm_count));
-    case 2: return std::max(attention_bytes<2, 1, true>(sm_count), attention_bytes<2, 2, false>(sm_count));
-    case 3: return attention_bytes<3, 1, false>(sm_count);
-    default: return attention_bytes<4, 1, false>(sm_count);
+    case 1: return attention_bytes<1>(sm_count);
+    case 2: return attention_bytes<2>(sm_count);
+    case 3: return attention_bytes<3>(sm_count);
+    default: return attention_bytes<4>(sm_count);
     }
 }
 
-template <typename T, int GROUPS, int MT, bool PAIR>
+template <typename T, int GROUPS, int NT>
 cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r, AttentionCall call,
                          void* workspace) {
-    using Shape = AttentionShape<GROUPS, MT, PAIR>;
-    const auto kernel = attention_kernel<T, GROUPS, MT, PAIR>;
+    constexpr bool kLow = std::is_same<T, float>::value;
+    using Shape = AttentionShape<GROUPS, NT, kLow>;
+    const auto kernel = attention_kernel<T, GROUPS, NT, kLow>;
     const unsigned blocks = (unsigned)(sm_count * Shape::kBlocksPerSm);
     call.tokens = 1;
     while (call.tokens * 2 * call.group <= (uint32_t)Shape::kRows) call.tokens *= 2;
     call.subs = (call.group + Shape::kRows - 1) / Shape::kRows;
+    call.used = std::min<uint32_t>(Shape::kRows, call.tokens * call.group);
     call.tails = static_cast<int4*>(workspace);
     call.parts = reinterpret_cast<float*>(call.tails + blocks);
     cudaError_t status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
@@ -1254,26 +1308,19 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     kernel<<<blocks, kAttentionThreads, Shape::kShared, s>>>(c, r, call);
     status = cudaGetLastError();
     if (status != cudaSuccess) return status;
-    return launch_dependent(attention_merge_kernel<T>, blocks * Shape::kRows, 32 * kMergeWarps, 0, s, c, r, call, Shape::kRows);
+    return launch_dependent(attention_merge_kernel<T>, blocks * call.used, 32 * kMergeWarps, 0, s, c, r, call, Shape::kRows);
 }
 
-// Rows of a tile by the rows that a sequence and key head has on average: eight in two parts
-// up to eight; f32 queries sixteen in two parts, f16 and bf16 sixteen or 32 in one (wide
-// heads leave registers for sixteen).
+// Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where
+// the sums of 32 rows fit the registers.
 template <typename T, int GROUPS>
 cudaError_t launch_attention(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r,
                              const AttentionCall& call, void* workspace) {
     const uint64_t rows = (uint64_t)((r.rows + r.count - 1) / r.count) * call.group;
-    if (rows > 8) {
-        if constexpr (std::is_same<T, float>::value) {
-            if constexpr (GROUPS <= 2) return launch_tiles<T, GROUPS, 2, true>(sm_count, s, c, r, call, workspace);
-        } else {
-            if constexpr (GROUPS <= 2)
-                if (rows > 16) return launch_tiles<T, GROUPS, 2, false>(sm_count, s, c, r, call, workspace);
-            return launch_tiles<T, GROUPS, 1, false>(sm_count, s, c, r, call, workspace);
-        }
-    }
-    return launch_tiles<T, GROUPS, 1, true>(sm_count, s, c, r, call, workspace);
+    if constexpr (GROUPS <= 2 && !std::is_same<T, float>::value)
+        if (rows > 16) return launch_tiles<T, GROUPS, 4>(sm_count, s, c, r, call, workspace);
+    if (rows > 8) return launch_tiles<T, GROUPS, 2>(sm_count, s, c, r, call, workspace);
+    return launch_tiles<T, GROUPS, 1>(sm_count, s, c, r, call, workspace);
 }
 
 }  // namespace
@@ -1360,7 +1407,6 @@ int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const l
     call.q_head = q_head;
     call.out_row = out_row;
     call.out_head = out_head;
-    call.q_heads = (uint32_t)q_heads;
     call.group = (uint32_t)(q_heads / c.kv_heads);
     call.scale = (float)(scale * 1.4426950408889634);
     const size_t e = dtype_bytes(kind);
