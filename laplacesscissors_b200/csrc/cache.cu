@@ -226,9 +226,12 @@ constexpr int kLeastRun = 8;
 constexpr int kPairTokens = 2 * kCellTokens;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
+// Floats of a row's part: its sums, its reference and the sum of its weights.
+constexpr int part_row(int dim) { return dim + 2; }
+
 template <int GROUPS, int NT, bool LOW>
 struct AttentionShape {
-    static constexpr int kDim = 64 * GROUPS, kRows = 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
+    static constexpr int kDim = 64 * GROUPS, kPart = part_row(kDim), kRows = 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
     static constexpr int kLoad = NT * GROUPS;
     static constexpr int kBlocksPerSm = kLoad <= 2 ? 4 : kLoad <= 4 && GROUPS < 4 ? 3 : 2;
     // registers a thread: the sums and the queries, which go to shared memory where 75 are not left for the rest
@@ -239,7 +242,7 @@ struct AttentionShape {
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
     static constexpr int kAtOnce = NT == 1 ? 2 : 1;  // cells whose weights a thread holds at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
-    static constexpr int kParts = kAttentionWarps * kRows * (kDim + 2) * 4;  // the warps' sums, in the ring's memory
+    static constexpr int kParts = kAttentionWarps * kRows * kPart * 4;  // the warps' sums, in the ring's memory
     static constexpr int kBars = kAttentionWarps * kStages * 8;
     static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + kBars;
     static_assert(kStages >= 2 && kBlocksPerSm * (kShared + 1200) <= 228 * 1024, "shared memory");
@@ -254,8 +257,9 @@ struct AttentionCall {
     uint32_t used;             // of the tile's rows, those that hold any
     float scale;               // times log2 e
     bool wide;                 // queries lie to 16 bytes
-    int4* tails;               // [blocks] tiles that a block starts and others finish
-    float* parts;              // [2 blocks][rows][dim + 2]
+    int4* tails;               // [blocks] tiles that a block starts and others finish: their parts, first row, key head and
+                               // part of it, positions
+    float* parts;              // [2 blocks][rows][part_row(dim)]
 };
 
 // A call's pairs in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
@@ -420,7 +424,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     if (at >= end) return;
     uint32_t b = (uint32_t)found[0];
     long long offset = found[1];
-    uint32_t phases = 0;  // a bit a stage: the phase that its barrier completes next
+    int stage = 0, into = 0;  // the ring's next stage to take and to fill
+    uint32_t phase = 0;       // that the barriers of this turn of the ring complete
     bool dead = false;    // a copy did not arrive in time
 
     while (at < end) {
@@ -431,8 +436,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             offset = 0;
             continue;
         }
-        const uint32_t head_sub = (uint32_t)(offset / one), head = head_sub / call.subs, sub = head_sub % call.subs;
-        const long long rest = offset % one;
+        const uint32_t head_sub = offset >> 32 ? (uint32_t)(offset / one) : (uint32_t)offset / (uint32_t)one;  // one <= offset or 0
+        const uint32_t head = head_sub / call.subs, sub = head_sub % call.subs;
+        const long long rest = offset - head_sub * one;
         int k = 0;
         for (int high = tile_count(s, tokens); high - k > 1;) {  // pairs_before(k) <= rest
             const int middle = (k + high) / 2;
@@ -464,48 +470,49 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         const bool together = per_page % 2 == 0;  // both cells lie in one page, one behind the other
         const int32_t* table = c.tables + (size_t)max(s.table, 0) * c.table_width;
         const uint32_t seen_cells = (uint32_t)max((seen + kCellTokens - 1) >> 4, 0);
-        const auto cell_of_pair = [&](int n) { return 2u * (uint32_t)(first + warp + n * kAttentionWarps); };
-        const auto page_of = [&](int n, uint32_t half) {  // of this warp's n-th pair
-            const uint32_t cell = cell_of_pair(n) + half;
-            return n < mine_pairs && cell < seen_cells ? (uint32_t)table[cell / per_page] : 0xffffffffu;
-        };
-        uint32_t pages = page_of(lane, 0), others = together ? 0 : page_of(lane, 1);
-        uint32_t within = cell_of_pair(0) % per_page;  // the next copy's first cell in its page
-        const uint32_t step_within = 2 * kAttentionWarps % per_page;
         const uint8_t* head_cells = c.pages + (size_t)head * per_page * Shape::kCell;
         const size_t page_bytes = (size_t)c.kv_heads * per_page * Shape::kCell;
-        int issued = 0, into = 0;
+        // Each lane looks up one of the next 32 pairs and copies it when a stage is free.
+        const uint8_t* from[2] = {nullptr, nullptr};
+        uint32_t absent[2] = {0, 0};  // of the 32, those whose first or second cell has no page
+        const auto look_up = [&](int n) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                if (u == 1 && together) {
+                    absent[1] = absent[0];
+                    break;
+                }
+                const uint32_t cell = 2u * (uint32_t)(first + warp + n * kAttentionWarps) + u;
+                from[u] = nullptr;
+                if (n < mine_pairs && cell < seen_cells) {
+                    const uint32_t slot = cell / per_page, page = (uint32_t)table[slot];
+                    if (page < c.page_count) from[u] = head_cells + page * page_bytes + (cell - slot * per_page) * Shape::kCell;
+                }
+                absent[u] = ~__ballot_sync(0xffffffffu, from[u] != nullptr);
+            }
+        };
+        look_up(lane);
+        int issued = 0;
         uint32_t gone = 0;  // two bits a stage: cells without a page
         const auto issue = [&] {
             if (issued >= mine_pairs || dead) return;
-            const uint32_t page = __shfl_sync(0xffffffffu, pages, issued & 31);
-            const uint32_t other = together ? page : __shfl_sync(0xffffffffu, others, issued & 31);
-            const uint32_t none = (page < c.page_count ? 0u : 1u) | (other < c.page_count ? 0u : 2u);
-            gone = (gone & ~(3u << 2 * into)) | none << 2 * into;
-            if (lane == 0) {
+            const int turn = issued & 31;
+            gone = (gone & ~(3u << 2 * into)) | (absent[0] >> turn & 1u) << 2 * into | (absent[1] >> turn & 1u) << (2 * into + 1);
+            if (lane == turn) {
                 uint8_t* to = ring + into * Shape::kStage;
-                const uint8_t* from = head_cells + page * page_bytes + within * Shape::kCell;
-                if (none == 3) {
-                    mbar_arrive(bars + into);
-                } else if (together) {
+                if (together && from[0]) {
                     mbar_expect_tx(bars + into, Shape::kStage);
-                    bulk_load(to, from, Shape::kStage, bars + into);
+                    bulk_load(to, from[0], Shape::kStage, bars + into);
+                } else if (!from[0] && !from[1]) {
+                    mbar_arrive(bars + into);
                 } else {
-                    mbar_expect_tx(bars + into, none ? Shape::kCell : Shape::kStage);
-                    if (!(none & 1)) bulk_load(to, from, Shape::kCell, bars + into);
-                    if (!(none & 2)) {
-                        const uint32_t second = within + 1 == per_page ? 0 : within + 1;
-                        bulk_load(to + Shape::kCell, head_cells + other * page_bytes + second * Shape::kCell, Shape::kCell, bars + into);
-                    }
+                    mbar_expect_tx(bars + into, from[0] && from[1] ? Shape::kStage : Shape::kCell);
+                    if (from[0]) bulk_load(to, from[0], Shape::kCell, bars + into);
+                    if (from[1]) bulk_load(to + Shape::kCell, from[1], Shape::kCell, bars + into);
                 }
             }
-            within += step_within;
-            if (within >= per_page) within -= per_page;
             into = into + 1 == kStages ? 0 : into + 1;
-            if ((++issued & 31) == 0) {
-                pages = page_of(issued + lane, 0);
-                if (!together) others = page_of(issued + lane, 1);
-            }
+            if ((++issued & 31) == 0) look_up(issued + lane);
         };
         fence_proxy_async_shared();  // the ring held other things
         __syncthreads();             // which all threads have read
@@ -607,7 +614,6 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             }
         }
 
-        int stage = 0;
         const uint32_t pick = quad & 1 ? 0x7632u : 0x5410u;  // a thread's position among two: its step and zero
 
         // kAtOnce cells at `held`, the first of them at position `start`.  EDGE: some row does not see all of
@@ -617,6 +623,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             constexpr int U = Shape::kAtOnce;
             const int position = start + quad;  // the thread's positions: this and every eighth on
             const auto there = [&](int u, int i) { return position + 16 * u + 8 * i < seen && !(none >> u & 1); };
+            const auto blind = [&](int u, int i, int n, int row) {
+                return !there(u, i) || position + 16 * u + 8 * i >= limit[n][row];
+            };
             // scores [row 2 j, 2 j + 1 of position, of position + 8], in units that `factor` takes to powers of two
             float score[U][NT][4];
             __half2 values[U][GROUPS][2];  // the values' steps and zeros
@@ -686,9 +695,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        score[u][n][i] *= factor[n][i % 2];
-                        if (EDGE && !(there(u, i / 2) && position + 16 * u + i / 2 * 8 < limit[n][i % 2])) score[u][n][i] = -INFINITY;
-                        weight[u][n][i] = exp2_approx(score[u][n][i] - reference[n][i % 2]);
+                        weight[u][n][i] = exp2_approx(fmaf(score[u][n][i], factor[n][i % 2], -reference[n][i % 2]));
+                        if (EDGE && blind(u, i / 2, n, i % 2)) weight[u][n][i] = 0.f;
                         most = fmaxf(most, weight[u][n][i]);
                     }
             __half2 steps = values[0][0][0];
@@ -702,8 +710,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        float top = fmaxf(score[0][n][i], score[0][n][2 + i]);
-                        if (U == 2) top = fmaxf(top, fmaxf(score[U - 1][n][i], score[U - 1][n][2 + i]));
+                        float top = -INFINITY;
+#pragma unroll
+                        for (int m = 0; m < 2 * U; ++m)
+                            if (!EDGE || !blind(m / 2, m % 2, n, i)) top = fmaxf(top, score[m / 2][n][m % 2 * 2 + i] * factor[n][i]);
                         top = across_max(top);
                         const float next = fmaxf(reference[n][i], top + above - 10.f);
                         const float keep = exp2_approx(reference[n][i] - next);
@@ -717,9 +727,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             out[n][m][2 + i] *= keep;
                         }
 #pragma unroll
-                        for (int u = 0; u < U; ++u) {
-                            weight[u][n][i] = exp2_approx(score[u][n][i] - next);
-                            weight[u][n][2 + i] = exp2_approx(score[u][n][2 + i] - next);
+                        for (int m = 0; m < 2 * U; ++m) {
+                            float& w = weight[m / 2][n][m % 2 * 2 + i];
+                            w = exp2_approx(fmaf(score[m / 2][n][m % 2 * 2 + i], factor[n][i], -next));
+                            if (EDGE && blind(m / 2, m % 2, n, i)) w = 0.f;
                         }
                     }
             }
@@ -745,8 +756,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         for (int i = 0; i < 4; ++i) {
                             x[i] = weight[u][n][i] * sz[i / 2].x;
                             // a position that this row does not see adds nothing, whatever it holds
-                            const bool blind = EDGE && position + 16 * u + i / 2 * 8 >= limit[n][i % 2];
-                            if (blind) x[i] = 0.f;
+                            if (EDGE && blind(u, i / 2, n, i % 2)) x[i] = 0.f;
                             else zeros[n][i % 2][g] = fmaf(weight[u][n][i], sz[i / 2].y, zeros[n][i % 2][g]);
                         }
                         p0[n] = pack_f16(x[0], x[1]);
@@ -781,14 +791,15 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             issue();
             const int pair = first + warp + n * kAttentionWarps;
             const uint8_t* held = ring + stage * Shape::kStage;
-            uint32_t none = gone >> 2 * stage & 3;
-            if (!dead) dead = !mbar_wait_bounded(bars + stage, phases >> stage & 1);
-            phases ^= 1u << stage;
-            stage = stage + 1 == kStages ? 0 : stage + 1;
-            if (__any_sync(0xffffffffu, dead)) {  // what is in flight lands first
+            const uint32_t none = gone >> 2 * stage & 3;
+            const bool late = dead || !mbar_wait_bounded(bars + stage, phase);
+            if (++stage == kStages) stage = 0, phase ^= 1;
+            if (__any_sync(0xffffffffu, late)) {
                 dead = true;
-                for (; ++n < issued; stage = stage + 1 == kStages ? 0 : stage + 1)
-                    mbar_wait_bounded(bars + stage, phases >> stage & 1);
+                while (++n < issued) {  // what is in flight lands first
+                    mbar_wait_bounded(bars + stage, phase);
+                    if (++stage == kStages) stage = 0, phase ^= 1;
+                }
 #pragma unroll
                 for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = nan;
                 break;
@@ -819,12 +830,12 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 
         // ---- the warps' sums
         __syncthreads();  // the rings are drained
-        float* mine_sums = warp_sums + warp * Shape::kRows * (D + 2);
+        float* mine_sums = warp_sums + warp * Shape::kRows * Shape::kPart;
 #pragma unroll
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float* row = mine_sums + (8 * t + 2 * j + i) * (D + 2);
+                float* row = mine_sums + (8 * t + 2 * j + i) * Shape::kPart;
                 const float l = across_sum(sum[t][i]);
                 if (quad == 0) row[D] = reference[t][i], row[D + 1] = l;
 #pragma unroll
@@ -839,16 +850,16 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             }
         __syncthreads();
         const bool whole = first == 0 && last == pairs;
-        float* part = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * Shape::kRows * (D + 2);
+        float* part = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * Shape::kRows * Shape::kPart;
         for (int i = warp; i < Shape::kRows; i += kAttentionWarps) {
             int token, h;
             if (!place(i, token, h)) continue;
             float top = kNone, l = 0.f, weight[kAttentionWarps];
 #pragma unroll
-            for (int w = 0; w < kAttentionWarps; ++w) top = fmaxf(top, warp_sums[(w * Shape::kRows + i) * (D + 2) + D]);
+            for (int w = 0; w < kAttentionWarps; ++w) top = fmaxf(top, warp_sums[(w * Shape::kRows + i) * Shape::kPart + D]);
 #pragma unroll
             for (int w = 0; w < kAttentionWarps; ++w) {
-                const float* row = warp_sums + (w * Shape::kRows + i) * (D + 2);
+                const float* row = warp_sums + (w * Shape::kRows + i) * Shape::kPart;
                 weight[w] = exp2_approx(row[D] - top);
                 l += weight[w] * row[D + 1];
             }
@@ -858,68 +869,117 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             for (int d = lane; d < D; d += 32) {
                 float x = 0.f;
 #pragma unroll
-                for (int w = 0; w < kAttentionWarps; ++w) x = fmaf(weight[w], warp_sums[(w * Shape::kRows + i) * (D + 2) + d], x);
+                for (int w = 0; w < kAttentionWarps; ++w) x = fmaf(weight[w], warp_sums[(w * Shape::kRows + i) * Shape::kPart + d], x);
                 if (whole)
                     to[d] = from_f32<T>(x * inverse);
                 else
-                    part[(size_t)i * (D + 2) + d] = x;
+                    part[(size_t)i * Shape::kPart + d] = x;
             }
-            if (!whole && lane == 0) part[(size_t)i * (D + 2) + D] = top, part[(size_t)i * (D + 2) + D + 1] = l;
+            if (!whole && lane == 0) part[(size_t)i * Shape::kPart + D] = top, part[(size_t)i * Shape::kPart + D + 1] = l;
         }
         if (first == 0 && !whole && threadIdx.x == 0)
-            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), (int)b, (int)head_sub, k);
+            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), s.first + k * tokens, (int)head_sub,
+                                               tile_end - k * tokens);
     }
 }
 
-// Adds up the parts of the tile that a block of attention_kernel started and others
-// finished, in their order; a block a row, a warp every fourth part.
-constexpr int kMergeWarps = 4;
+// Adds up the parts of the tiles that a block of attention_kernel started and others
+// finished, in a fixed order.  The blocks list those tiles and share their rows out; a row's
+// parts are dealt to eight warps.
+constexpr int kMergeWarps = 8, kMergeEach = 3;
 
-template <typename T>
-__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(CacheView c, CacheRows r, AttentionCall call,
-                                                                           int rows) {
-    pdl_wait();
-    const int block = (int)(blockIdx.x / call.used), i = (int)(blockIdx.x % call.used), D = (int)c.dim;
-    const int4 tail = call.tails[block];
-    if (tail.x == 0) return;
-    const SequenceRows s = sequence_rows(c, r, (uint32_t)tail.y);
-    const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs, k = tail.w, tokens = (int)call.tokens;
-    const int token = k * tokens + (call.subs > 1 ? 0 : i / (int)call.group);
-    const int h = call.subs > 1 ? sub * rows + i : i % (int)call.group;
-    if (h >= (int)call.group || token >= min(s.count, (k + 1) * tokens)) return;
+template <typename T, int GROUPS>
+__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(AttentionCall call, int rows, int blocks) {
+    constexpr int D = 64 * GROUPS, kRow = part_row(D), kEach = D / 32;
+    extern __shared__ int started[];  // [blocks] those with a tile to add up
+    __shared__ int counts[kMergeEach][kMergeWarps];
+    __shared__ float2 about_warp[kMergeWarps];  // reference and sum of the weights
+    __shared__ float sums[kMergeWarps][D];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
-    __shared__ float sums[kMergeWarps][kMaxCacheDim + 2];
-    float top = -1e30f, l = 0.f, x[kMaxCacheDim / 32] = {};
-#pragma unroll 4
-    for (int n = warp; n < tail.x; n += kMergeWarps) {
-        const float* p = call.parts + (((size_t)(block + n) * 2 + (n == 0)) * rows + i) * (D + 2);
-        const float m = p[D], now = fmaxf(top, m), keep = exp2_approx(top - now), weight = exp2_approx(m - now);
-        top = now;
-        l = l * keep + p[D + 1] * weight;
+    pdl_wait();
+    int found = 0;
+    for (int base = 0; base < blocks; base += kMergeEach * 32 * kMergeWarps) {
+        unsigned votes[kMergeEach];
 #pragma unroll
-        for (int e = 0; e < kMaxCacheDim / 32; ++e)
-            if (e * 32 < D) x[e] = x[e] * keep + p[e * 32 + lane] * weight;
+        for (int i = 0; i < kMergeEach; ++i) {
+            const int block = base + i * 32 * kMergeWarps + (int)threadIdx.x;
+            votes[i] = __ballot_sync(0xffffffffu, block < blocks && call.tails[block].x > 0);
+            if (lane == 0) counts[i][warp] = __popc(votes[i]);
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kMergeEach; ++i) {
+            int before = found;
+#pragma unroll
+            for (int w = 0; w < kMergeWarps; ++w) {
+                if (w < warp) before += counts[i][w];
+                found += counts[i][w];
+            }
+            if (votes[i] >> lane & 1)
+                started[before + __popc(votes[i] & ((1u << lane) - 1))] = base + i * 32 * kMergeWarps + (int)threadIdx.x;
+        }
+        __syncthreads();
     }
+    const int used = (int)call.used;
+    for (int item = (int)blockIdx.x; item < found * used; item += (int)gridDim.x) {
+        const int block = started[item / used], i = item % used;
+        const int4 tail = call.tails[block];
+        const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs;
+        const int token = call.subs > 1 ? 0 : i / (int)call.group;
+        const int h = call.subs > 1 ? sub * rows + i : i % (int)call.group;
+        if (h >= (int)call.group || token >= tail.w) continue;
+        float top = -1e30f, l = 0.f, x[kEach] = {};
+        for (int n = warp; n < tail.x; n += 4 * kMergeWarps) {  // four at a time, all loads ahead of their use
+            float2 about[4];
+            float row[4][kEach];
 #pragma unroll
-    for (int e = 0; e < kMaxCacheDim / 32; ++e)
-        if (e * 32 < D) sums[warp][e * 32 + lane] = x[e];
-    if (lane == 0) sums[warp][kMaxCacheDim] = top, sums[warp][kMaxCacheDim + 1] = l;
-    __syncthreads();
-    top = -1e30f, l = 0.f;
-    float weight[kMergeWarps];
+            for (int m = 0; m < 4; ++m) {
+                about[m] = make_float2(-1e30f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, sums[w][kMaxCacheDim]);
+                for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
+                const int from = n + m * kMergeWarps;
+                if (from < tail.x) {
+                    const float* p = call.parts + (((size_t)(block + from) * 2 + (from == 0)) * rows + i) * kRow;
+                    about[m] = *reinterpret_cast<const float2*>(p + D);
 #pragma unroll
-    for (int w = 0; w < kMergeWarps; ++w) {
-        weight[w] = exp2_approx(sums[w][kMaxCacheDim] - top);
-        l += weight[w] * sums[w][kMaxCacheDim + 1];
-    }
-    T* to = static_cast<T*>(call.out) + (size_t)(s.first + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
-    for (int d = (int)threadIdx.x; d < D; d += 32 * kMergeWarps) {
-        float y = 0.f;
+                    for (int e = 0; e < kEach; ++e) row[m][e] = p[e * 32 + lane];
+                }
+            }
+            const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
+            const float keep = exp2_approx(top - now);
+            top = now;
+            l *= keep;
 #pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) y = fmaf(weight[w], sums[w][d], y);
-        to[d] = from_f32<T>(l == 0.f ? 0.f : y / l);
+            for (int e = 0; e < kEach; ++e) x[e] *= keep;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                const float weight = exp2_approx(about[m].x - now);
+                l = fmaf(about[m].y, weight, l);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
+            }
+        }
+        __syncthreads();  // the row before is read
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
+        if (lane == 0) about_warp[warp] = make_float2(top, l);
+        __syncthreads();
+        top = -1e30f, l = 0.f;
+        float weight[kMergeWarps];
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, about_warp[w].x);
+#pragma unroll
+        for (int w = 0; w < kMergeWarps; ++w) {
+            weight[w] = exp2_approx(about_warp[w].x - top);
+            l = fmaf(about_warp[w].y, weight[w], l);
+        }
+        T* to = static_cast<T*>(call.out) + (size_t)(tail.y + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
+        for (int d = (int)threadIdx.x; d < D; d += 32 * kMergeWarps) {
+            float y = 0.f;
+#pragma unroll
+            for (int w = 0; w < kMergeWarps; ++w) y = fmaf(sums[w][d], weight[w], y);
+            to[d] = from_f32<T>(l == 0.f ? 0.f : y / l);
+        }
     }
 }
 
@@ -1270,7 +1330,7 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
 template <int GROUPS, int NT, bool LOW>
 size_t attention_bytes(int sm_count) {
     using Shape = AttentionShape<GROUPS, NT, LOW>;
-    return (size_t)sm_count * Shape::kBlocksPerSm * (16 + 2 * Shape::kRows * (Shape::kDim + 2) * 4);
+    return (size_t)sm_count * Shape::kBlocksPerSm * (16 + 2 * Shape::kRows * Shape::kPart * 4);
 }
 
 template <int GROUPS>
@@ -1308,7 +1368,8 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     kernel<<<blocks, kAttentionThreads, Shape::kShared, s>>>(c, r, call);
     status = cudaGetLastError();
     if (status != cudaSuccess) return status;
-    return launch_dependent(attention_merge_kernel<T>, blocks * call.used, 32 * kMergeWarps, 0, s, c, r, call, Shape::kRows);
+    return launch_dependent(attention_merge_kernel<T, GROUPS>, std::min(blocks * call.used, (unsigned)sm_count * 6), 32 * kMergeWarps,
+                            blocks * 4, s, call, Shape::kRows, (int)blocks);
 }
 
 // Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where
