@@ -221,9 +221,12 @@ __global__ void __launch_bounds__(128) read_kernel(CacheView c, CacheRows r, T* 
 // A warp streams every fourth pair of the run through its own ring in shared memory by bulk
 // copies, with its own softmax; the warps' sums meet at a tile's end.
 //
-// Pairs that a block takes at least, where there are few: two a warp.
-constexpr int kLeastRun = 8;
+// Cost that a block takes at least, where there is little: a tile and two pairs a warp.
+constexpr int kLeastRun = 12;
 constexpr int kPairTokens = 2 * kCellTokens;
+// What a tile costs beside its pairs (the first copies' latency, the queries, the sums), in
+// pairs: it counts so many more when the runs are cut.
+constexpr int kTileCost = 4;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
 // Floats of a row's part: its sums, its reference and the sum of its weights.
@@ -271,25 +274,26 @@ __device__ __forceinline__ int tile_pairs(const SequenceRows& s, int tokens, int
     return max(1, (seen + kPairTokens - 1) >> 5);
 }
 
-// Pairs of the tiles before k (k below the tile count): the sum of floor((base + 31 + (i + 1) tokens) / 32), with
+// Cost of the tiles before k (k below the tile count), kTileCost and their pairs each: the sum of floor((base + 31 + (i + 1) tokens) / 32), with
 // base = length - count, over the tiles that see anything, and 1 for those that do not.  tokens divides 32.
-__device__ __forceinline__ long long pairs_before(const SequenceRows& s, int tokens, int k) {
+__device__ __forceinline__ long long cost_before(const SequenceRows& s, int tokens, int k) {
     if (k == 0) return 0;
     const int base = s.length - s.count;
     const int blind = s.length <= 0 ? k : base >= 0 ? 0 : min(k, -base / tokens);
-    if (k <= blind) return k;
+    const long long fixed = (long long)k * kTileCost;
+    if (k <= blind) return fixed + k;
     const int shift = 31 - __clz(tokens), m = kPairTokens >> shift, y = (base + kPairTokens - 1) >> shift;
     const auto sum = [m](long long n) {  // of floor(i / m) over i = 0 .. n
         if (n < 0) return 0ll;
         const long long q = n / m, r = n % m;
         return m * q * (q - 1) / 2 + q * (r + 1);
     };
-    return blind + sum((long long)y + k) - sum((long long)y + blind);
+    return fixed + blind + sum((long long)y + k) - sum((long long)y + blind);
 }
 
-__device__ __forceinline__ long long sequence_pairs(const SequenceRows& s, int tokens) {
+__device__ __forceinline__ long long sequence_cost(const SequenceRows& s, int tokens) {
     const int tiles = tile_count(s, tokens);
-    return tiles ? pairs_before(s, tokens, tiles - 1) + tile_pairs(s, tokens, tiles - 1) : 0;
+    return tiles ? cost_before(s, tokens, tiles - 1) + kTileCost + tile_pairs(s, tokens, tiles - 1) : 0;
 }
 
 // c += a b, and c = a b.
@@ -388,7 +392,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     const uint32_t each = (r.count + kAttentionThreads - 1) / kAttentionThreads;
     const uint32_t mine_first = min(threadIdx.x * each, r.count), mine_end = min(mine_first + each, r.count);
     long long mine = 0;
-    for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_pairs(sequence_rows(c, r, b), tokens) * tiles_of;
+    for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_cost(sequence_rows(c, r, b), tokens) * tiles_of;
     long long* scan = reinterpret_cast<long long*>(shared);
     long long before = mine;
 #pragma unroll
@@ -410,13 +414,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     const long long end = min(at + run, total);
     if (mine > 0 && before <= at && at < before + mine) {
         for (uint32_t b = mine_first; b < mine_end; ++b) {
-            const long long pairs = sequence_pairs(sequence_rows(c, r, b), tokens) * tiles_of;
-            if (at < before + pairs) {
+            const long long cost = sequence_cost(sequence_rows(c, r, b), tokens) * tiles_of;
+            if (at < before + cost) {
                 found[0] = b;
                 found[1] = at - before;
                 break;
             }
-            before += pairs;
+            before += cost;
         }
     }
     if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -430,7 +434,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 
     while (at < end) {
         const SequenceRows s = sequence_rows(c, r, b);
-        const long long one = sequence_pairs(s, tokens);
+        const long long one = sequence_cost(s, tokens);
         if (offset >= one * tiles_of) {
             ++b;
             offset = 0;
@@ -440,17 +444,20 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         const uint32_t head = head_sub / call.subs, sub = head_sub % call.subs;
         const long long rest = offset - head_sub * one;
         int k = 0;
-        for (int high = tile_count(s, tokens); high - k > 1;) {  // pairs_before(k) <= rest
+        for (int high = tile_count(s, tokens); high - k > 1;) {  // cost_before(k) <= rest
             const int middle = (k + high) / 2;
-            if (pairs_before(s, tokens, middle) <= rest)
+            if (cost_before(s, tokens, middle) <= rest)
                 k = middle;
             else
                 high = middle;
         }
-        const int first = (int)(rest - pairs_before(s, tokens, k)), pairs = tile_pairs(s, tokens, k);
-        const int last = (int)min((long long)pairs, first + end - at);
-        at += last - first;
-        offset += last - first;
+        // the first kTileCost of a tile's cost stand for no pair
+        const int pairs = tile_pairs(s, tokens, k), from_cost = (int)(rest - cost_before(s, tokens, k));
+        const int to_cost = (int)min((long long)pairs + kTileCost, from_cost + end - at);
+        const int first = max(from_cost - kTileCost, 0), last = to_cost - kTileCost;
+        at += to_cost - from_cost;
+        offset += to_cost - from_cost;
+        if (last <= first) continue;
 
         // the tile's rows: row i is head sub * rows + i of position k, or head i % group of position k * tokens + i / group
         const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
@@ -584,10 +591,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         }
                         if constexpr (Shape::kSharedQuery) {
                             if (warp == f % kAttentionWarps) {
-                                if constexpr (LOW)
-                                    reinterpret_cast<uint4*>(queries)[f * 32 + lane] = make_uint4(x0, x1, l0, l1);
-                                else
-                                    reinterpret_cast<uint2*>(queries)[f * 32 + lane] = make_uint2(x0, x1);
+                                uint2* at = reinterpret_cast<uint2*>(queries) + f * (LOW ? 2 : 1) * 32 + lane;
+                                at[0] = make_uint2(x0, x1);
+                                if constexpr (LOW) at[32] = make_uint2(l0, l1);
                             }
                         } else {
                             query[f][0] = x0, query[f][1] = x1;
@@ -626,67 +632,71 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             const auto blind = [&](int u, int i, int n, int row) {
                 return !there(u, i) || position + 16 * u + 8 * i >= limit[n][row];
             };
-            // scores [row 2 j, 2 j + 1 of position, of position + 8], in units that `factor` takes to powers of two
-            float score[U][NT][4];
-            __half2 values[U][GROUPS][2];  // the values' steps and zeros
+            // n . q [row 2 j, 2 j + 1 of position, of position + 8]; steps over all cells and groups in turn, so that
+            // no product waits for the one before
+            float dot[U][GROUPS][NT][4];
+            uint4 words[U][GROUPS];
 #pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const uint8_t* cell = held + u * Shape::kCell;
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int g = 0; g < GROUPS; ++g)
+                    words[u][g] = *reinterpret_cast<const uint4*>(held + u * Shape::kCell + (g * 32 + lane) * 16);
+#pragma unroll
+            for (int w = 0; w < 2; ++w)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
+#pragma unroll
+                    for (int part = 0; part < (LOW ? 2 : 1); ++part)
+#pragma unroll
+                        for (int u = 0; u < U; ++u)
+#pragma unroll
+                            for (int g = 0; g < GROUPS; ++g) {
+                                const uint32_t low = w ? words[u][g].y : words[u][g].x, high = w ? words[u][g].w : words[u][g].z;
+                                const uint32_t a[4] = {low & mask, high & mask, low >> 8 & mask, high >> 8 & mask};
+#pragma unroll
+                                for (int n = 0; n < NT; ++n) {
+                                    const int f = (n * GROUPS + g) * 4 + w * 2 + e;
+                                    uint32_t b0, b1;
+                                    if constexpr (Shape::kSharedQuery) {
+                                        const uint2 x = reinterpret_cast<const uint2*>(queries)[(f * (LOW ? 2 : 1) + part) * 32 + lane];
+                                        b0 = x.x, b1 = x.y;
+                                    } else {
+                                        b0 = query[f][2 * part], b1 = query[f][2 * part + 1];
+                                    }
+                                    if (w + e + part == 0)
+                                        mma_f16_first(dot[u][g][n], a, b0, b1);
+                                    else
+                                        mma_f16(dot[u][g][n], a, b0, b1);
+                                }
+                            }
+                }
+            // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
+            float score[U][NT][4];
+            __half2 values[U][GROUPS][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const uint4 words = *reinterpret_cast<const uint4*>(cell + (g * 32 + lane) * 16);
-                    const uint4 raw = *reinterpret_cast<const uint4*>(cell + cell_key_steps(D) + g * 64 + quad / 2 * 16);
+                    const uint8_t* steps_of = held + u * Shape::kCell + g * 64 + quad / 2 * 16;
+                    const uint4 raw = *reinterpret_cast<const uint4*>(steps_of + cell_key_steps(D));
                     const float2 sz0 = unpack_f16(__byte_perm(raw.x, raw.y, pick)), sz1 = unpack_f16(__byte_perm(raw.z, raw.w, pick));
-                    float dot[NT][4];
-#pragma unroll
-                    for (int w = 0; w < 2; ++w) {
-                        const uint32_t low = w ? words.y : words.x, high = w ? words.w : words.z;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
-                            const uint32_t a[4] = {low & mask, high & mask, low >> 8 & mask, high >> 8 & mask};
-#pragma unroll
-                            for (int n = 0; n < NT; ++n) {
-                                const int f = (n * GROUPS + g) * 4 + w * 2 + e;
-                                uint32_t b0, b1, b2 = 0, b3 = 0;
-                                if constexpr (Shape::kSharedQuery && LOW) {
-                                    const uint4 x = reinterpret_cast<const uint4*>(queries)[f * 32 + lane];
-                                    b0 = x.x, b1 = x.y, b2 = x.z, b3 = x.w;
-                                } else if constexpr (Shape::kSharedQuery) {
-                                    const uint2 x = reinterpret_cast<const uint2*>(queries)[f * 32 + lane];
-                                    b0 = x.x, b1 = x.y;
-                                } else {
-                                    b0 = query[f][0], b1 = query[f][1];
-                                    if constexpr (LOW) b2 = query[f][2], b3 = query[f][3];
-                                }
-                                if (w + e == 0)
-                                    mma_f16_first(dot[n], a, b0, b1);
-                                else
-                                    mma_f16(dot[n], a, b0, b1);
-                                if constexpr (LOW) mma_f16(dot[n], a, b2, b3);
-                            }
-                        }
-                    }
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float z0 = sz0.y * plain[n][i][g], z1 = sz1.y * plain[n][i][g];
-                            score[u][n][i] = fmaf(sz0.x, dot[n][i], g ? score[u][n][i] + z0 : z0);
-                            score[u][n][2 + i] = fmaf(sz1.x, dot[n][2 + i], g ? score[u][n][2 + i] + z1 : z1);
+                            score[u][n][i] = fmaf(sz0.x, dot[u][g][n][i], g ? score[u][n][i] + z0 : z0);
+                            score[u][n][2 + i] = fmaf(sz1.x, dot[u][g][n][2 + i], g ? score[u][n][2 + i] + z1 : z1);
                         }
-                }
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) {
-                    const uint4 raw = *reinterpret_cast<const uint4*>(cell + cell_value_steps(D) + g * 64 + quad / 2 * 16);
-                    uint32_t sz[2] = {__byte_perm(raw.x, raw.y, pick), __byte_perm(raw.z, raw.w, pick)};
+                    const uint4 more = *reinterpret_cast<const uint4*>(steps_of + cell_value_steps(D));
+                    uint32_t sz[2] = {__byte_perm(more.x, more.y, pick), __byte_perm(more.z, more.w, pick)};
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (EDGE && !there(u, i)) sz[i] = 0;  // what no row sees may hold anything
                         values[u][g][i] = *reinterpret_cast<__half2*>(&sz[i]);
                     }
                 }
-            }
             // weights
             float weight[U][NT][4], most = 0.f;
 #pragma unroll
@@ -769,18 +779,17 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         p0[n] = transpose_f16(p0[n]);
                         p1[n] = transpose_f16(p1[n]);
                     }
-                    const uint4 words = *reinterpret_cast<const uint4*>(cell + cell_values(D) + (g * 32 + lane) * 16);
-                    const uint32_t word[4] = {words.x, words.y, words.z, words.w};
+                    const uint4 held_words = *reinterpret_cast<const uint4*>(cell + cell_values(D) + (g * 32 + lane) * 16);
+                    const uint32_t word[4] = {held_words.x, held_words.y, held_words.z, held_words.w};
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const uint32_t a[4] = {word[w] & 0x000f000fu, word[w] & 0x00f000f0u, word[w] >> 8 & 0x000f000fu,
-                                               word[w] >> 8 & 0x00f000f0u};
+                    for (int part = 0; part < (LOW ? 2 : 1); ++part)
 #pragma unroll
-                        for (int n = 0; n < NT; ++n) {
-                            mma_f16(out[n][g * 4 + w], a, p0[n], p1[n]);
-                            if constexpr (LOW) mma_f16(out[n][g * 4 + w], a, l0[n], l1[n]);
+                        for (int w = 0; w < 4; ++w) {
+                            const uint32_t a[4] = {word[w] & 0x000f000fu, word[w] & 0x00f000f0u, word[w] >> 8 & 0x000f000fu,
+                                                   word[w] >> 8 & 0x00f000f0u};
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) mma_f16(out[n][g * 4 + w], a, part ? l0[n] : p0[n], part ? l1[n] : p1[n]);
                         }
-                    }
                 }
             }
         };
