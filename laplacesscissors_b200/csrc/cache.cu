@@ -35,13 +35,13 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) {
 
 // Launches `kernel` so that its prologue may overlap the end of the kernel before it.
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t s,
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 blocks, unsigned threads, size_t smem, cudaStream_t s,
                              Args... args) {
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(blocks);
+    config.gridDim = blocks;
     config.blockDim = dim3(threads);
     config.dynamicSmemBytes = smem;
     config.stream = s;
@@ -226,7 +226,7 @@ constexpr int kLeastRun = 12;
 constexpr int kPairTokens = 2 * kCellTokens;
 // What a tile costs beside its pairs (the first copies' latency, the queries, the sums), in
 // pairs: it counts so many more when the runs are cut.
-constexpr int kTileCost = 4;
+constexpr int kTileCost = 6;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
 // Floats of a row's part: its sums, its reference and the sum of its weights.
@@ -260,8 +260,8 @@ struct AttentionCall {
     uint32_t used;             // of the tile's rows, those that hold any
     float scale;               // times log2 e
     bool wide;                 // queries lie to 16 bytes
-    int4* tails;               // [blocks] tiles that a block starts and others finish: their parts, first row, key head and
-                               // part of it, positions
+    int4* tails;               // [blocks] tiles that a block starts and others finish: their parts (0: none), first row, key
+                               // head and part of it, positions
     float* parts;              // [2 blocks][rows][part_row(dim)]
 };
 
@@ -349,23 +349,72 @@ __device__ __forceinline__ uint32_t transpose_f16(uint32_t x) {
     return y;
 }
 
-// Sixteen consecutive elements as f32; `wide`: at a 16-byte boundary.
+// Sixteen consecutive elements of a query as they lie in memory, four bytes of them a word.
+// Reduced to the largest magnitude's bits as f32 (above those of infinity for a NaN), and pairs
+// of them scaled to f16.
 template <typename T>
-__device__ __forceinline__ void load16(const T* x, bool wide, float (&out)[16]) {
-    if (wide) {
-        constexpr int kEach = 16 / sizeof(T);
+struct Query16 {
+    static constexpr int kWords = 4 * (int)sizeof(T);
+    uint32_t word[kWords];
+
+    __device__ __forceinline__ void load(const T* x, bool wide) {  // wide: at a 16-byte boundary
+        if (wide) {
 #pragma unroll
-        for (int i = 0; i < 16 / kEach; ++i) {
-            const uint4 raw = reinterpret_cast<const uint4*>(x)[i];
-            const T* e = reinterpret_cast<const T*>(&raw);
+            for (int i = 0; i < kWords / 4; ++i) {
+                const uint4 raw = reinterpret_cast<const uint4*>(x)[i];
+                word[4 * i] = raw.x, word[4 * i + 1] = raw.y, word[4 * i + 2] = raw.z, word[4 * i + 3] = raw.w;
+            }
+        } else if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int k = 0; k < kEach; ++k) out[i * kEach + k] = to_f32(e[k]);
+            for (int i = 0; i < kWords; ++i) word[i] = reinterpret_cast<const uint32_t*>(x)[i];
+        } else {
+            const uint16_t* h = reinterpret_cast<const uint16_t*>(x);
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) word[i] = h[2 * i] | (uint32_t)h[2 * i + 1] << 16;
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) out[i] = to_f32(x[i]);
     }
-}
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) word[i] = 0;
+    }
+    // The larger of `most` and the magnitudes, as bits: those of an f32, or two 16-bit values side by side.
+    __device__ __forceinline__ uint32_t most(uint32_t top) const {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            if constexpr (sizeof(T) == 4)
+                top = max(top, word[i] & 0x7fffffffu);
+            else
+                top = __vmaxu2(top, word[i] & 0x7fff7fffu);
+        }
+        return top;
+    }
+    static __device__ __forceinline__ uint32_t most_f32(uint32_t top) {
+        if constexpr (sizeof(T) == 4) return top;
+        const uint32_t half = max(top & 0xffffu, top >> 16);
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return half << 16;
+        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)half)));
+    }
+    __device__ __forceinline__ float value(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(word[i]);
+        const uint32_t bits = i % 2 ? word[i / 2] >> 16 : word[i / 2] & 0xffffu;
+        if constexpr (std::is_same<T, __nv_bfloat16>::value) return __uint_as_float(bits << 16);
+        return __half2float(__ushort_as_half((unsigned short)bits));
+    }
+};
+
+// 2^power for power in -126 .. 127.
+__device__ __forceinline__ float pow2(int power) { return __int_as_float((power + 127) << 23); }
+
+// A part of a tile that a block works on.
+struct TilePart {
+    int first, last;   // pairs, of
+    int pairs;         // those of the tile; 0 behind the run's last part
+    int row;           // first row of the call
+    int positions;     // that the rows stand for
+    int least, seen;   // what the first row sees; what the last sees and the table covers
+    int head, sub;     // key head, and which part of its query heads
+    int table;         // row of the tables, -1 for none
+};
 
 template <typename T, int GROUPS, int NT, bool LOW>
 __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT, LOW>::kBlocksPerSm))
@@ -374,26 +423,29 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     constexpr int D = Shape::kDim, kStages = Shape::kStages;
     constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
     extern __shared__ __align__(128) uint8_t shared[];
-    __shared__ long long found[2];
+    __shared__ TilePart part;
+    __shared__ long long scan[kAttentionWarps], found[2];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32, quad = lane / 4, j = lane % 4;
     const float nan = std::numeric_limits<float>::quiet_NaN();
     uint8_t* ring = shared + warp * kStages * Shape::kStage;
     float* warp_sums = reinterpret_cast<float*>(shared);
-    uint32_t* queries = reinterpret_cast<uint32_t*>(shared + Shape::kShared - Shape::kBars - Shape::kQuery);
+    uint2* queries = reinterpret_cast<uint2*>(shared + Shape::kShared - Shape::kBars - Shape::kQuery);
     uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Shape::kShared - Shape::kBars) + warp * kStages;
     const int tokens = (int)call.tokens;
     const uint32_t tiles_of = c.kv_heads * call.subs;
-    pdl_launch_dependents();
     if (lane == 0)
         for (int i = 0; i < kStages; ++i) mbar_init(bars + i, 1);
     fence_barrier_init();
+    pdl_launch_dependents();
+    pdl_wait();
 
-    // this block's run of pairs
+    const int covered = (int)min((long long)c.table_width * c.page_size, (long long)INT32_MAX);  // positions of a table row
+
+    // ---- the block's run: each thread takes some of the sequences
     const uint32_t each = (r.count + kAttentionThreads - 1) / kAttentionThreads;
     const uint32_t mine_first = min(threadIdx.x * each, r.count), mine_end = min(mine_first + each, r.count);
     long long mine = 0;
     for (uint32_t b = mine_first; b < mine_end; ++b) mine += sequence_cost(sequence_rows(c, r, b), tokens) * tiles_of;
-    long long* scan = reinterpret_cast<long long*>(shared);
     long long before = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -409,76 +461,117 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         if (w < warp) before += scan[w];
         total += scan[w];
     }
-    const long long run = max((total + gridDim.x - 1) / gridDim.x, (long long)kLeastRun);
-    long long at = run * blockIdx.x;
+    const long long shares = total + gridDim.x - 1;
+    const long long run = max(shares >> 32 ? shares / gridDim.x : (long long)((uint32_t)shares / gridDim.x), (long long)kLeastRun);
+    long long at = run * blockIdx.x, offset = 0;  // cost: the run's next, and that within sequence b
     const long long end = min(at + run, total);
+    uint32_t b = 0;
+    if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (at >= end) return;
     if (mine > 0 && before <= at && at < before + mine) {
-        for (uint32_t b = mine_first; b < mine_end; ++b) {
-            const long long cost = sequence_cost(sequence_rows(c, r, b), tokens) * tiles_of;
+        for (uint32_t n = mine_first; n < mine_end; ++n) {
+            const long long cost = sequence_cost(sequence_rows(c, r, n), tokens) * tiles_of;
             if (at < before + cost) {
-                found[0] = b;
+                found[0] = n;
                 found[1] = at - before;
                 break;
             }
             before += cost;
         }
     }
-    if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
     __syncthreads();
-    if (at >= end) return;
-    uint32_t b = (uint32_t)found[0];
-    long long offset = found[1];
+    b = (uint32_t)found[0];
+    offset = found[1];
+
+    // The first warp finds the next part of a tile in the run.
+    const auto next_part = [&] {
+        TilePart next;
+        next.pairs = 0;
+        while (at < end) {
+            const SequenceRows s = sequence_rows(c, r, b);
+            const long long one = sequence_cost(s, tokens);
+            if (offset >= one * tiles_of) {
+                ++b;
+                offset = 0;
+                continue;
+            }
+            const uint32_t head_sub = offset >> 32 ? (uint32_t)(offset / one) : (uint32_t)offset / (uint32_t)one;  // one <= offset or 0
+            const long long rest = offset - head_sub * one;
+            int k = 0;
+            for (int high = tile_count(s, tokens); high - k > 1;) {  // cost_before(k) <= rest
+                const int middle = (k + high) / 2;
+                if (cost_before(s, tokens, middle) <= rest)
+                    k = middle;
+                else
+                    high = middle;
+            }
+            // the first kTileCost of a tile's cost stand for no pair
+            const int pairs = tile_pairs(s, tokens, k), from_cost = (int)(rest - cost_before(s, tokens, k));
+            const int to_cost = (int)min((long long)pairs + kTileCost, from_cost + end - at);
+            at += to_cost - from_cost;
+            offset += to_cost - from_cost;
+            if (to_cost <= kTileCost) continue;
+            const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
+            next.first = max(from_cost - kTileCost, 0);
+            next.last = to_cost - kTileCost;
+            next.pairs = pairs;
+            next.row = s.first + k * tokens;
+            next.positions = tile_end - k * tokens;
+            next.least = base + k * tokens + 1;
+            next.seen = min(base + tile_end, covered);
+            next.head = (int)(call.subs == 1 ? head_sub : head_sub / call.subs);
+            next.sub = (int)(call.subs == 1 ? 0 : head_sub % call.subs);
+            next.table = s.table;
+            break;
+        }
+        if (lane == 0) part = next;
+    };
     int stage = 0, into = 0;  // the ring's next stage to take and to fill
     uint32_t phase = 0;       // that the barriers of this turn of the ring complete
-    bool dead = false;    // a copy did not arrive in time
+    bool dead = false;        // a copy did not arrive in time
+    const uint32_t per_page = c.page_size / kCellTokens;
+    const bool together = per_page % 2 == 0;  // both cells of a pair lie in one page, one behind the other
+    const size_t page_bytes = (size_t)c.kv_heads * per_page * Shape::kCell;
 
-    while (at < end) {
-        const SequenceRows s = sequence_rows(c, r, b);
-        const long long one = sequence_cost(s, tokens);
-        if (offset >= one * tiles_of) {
-            ++b;
-            offset = 0;
-            continue;
-        }
-        const uint32_t head_sub = offset >> 32 ? (uint32_t)(offset / one) : (uint32_t)offset / (uint32_t)one;  // one <= offset or 0
-        const uint32_t head = head_sub / call.subs, sub = head_sub % call.subs;
-        const long long rest = offset - head_sub * one;
-        int k = 0;
-        for (int high = tile_count(s, tokens); high - k > 1;) {  // cost_before(k) <= rest
-            const int middle = (k + high) / 2;
-            if (cost_before(s, tokens, middle) <= rest)
-                k = middle;
-            else
-                high = middle;
-        }
-        // the first kTileCost of a tile's cost stand for no pair
-        const int pairs = tile_pairs(s, tokens, k), from_cost = (int)(rest - cost_before(s, tokens, k));
-        const int to_cost = (int)min((long long)pairs + kTileCost, from_cost + end - at);
-        const int first = max(from_cost - kTileCost, 0), last = to_cost - kTileCost;
-        at += to_cost - from_cost;
-        offset += to_cost - from_cost;
-        if (last <= first) continue;
-
-        // the tile's rows: row i is head sub * rows + i of position k, or head i % group of position k * tokens + i / group
-        const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
-        const int covered = (int)min((long long)c.table_width * c.page_size, (long long)INT32_MAX);
-        const int seen = min(base + tile_end, covered);
-        const int least = base + k * tokens + 1;  // what the first row sees
+    for (;;) {
+        if (warp == 0) next_part();
+        fence_proxy_async_shared();  // the ring held sums and queries,
+        __syncthreads();             // which all threads have read
+        const int first = part.first, last = part.last, least = part.least, seen = part.seen, pairs = part.pairs;
+        const int head = part.head, sub = part.sub;
+        if (pairs == 0) return;
+        // row i of the tile: head sub * rows + i of the one position, or head i % group of position i / group
         const auto place = [&](int i, int& token, int& h) {
-            token = k * tokens + (call.subs > 1 ? 0 : i / (int)call.group);
-            h = call.subs > 1 ? (int)sub * Shape::kRows + i : i % (int)call.group;
-            return h < (int)call.group && token < tile_end;
+            token = call.subs > 1 ? 0 : i / (int)call.group;
+            h = call.subs > 1 ? sub * Shape::kRows + i : i % (int)call.group;
+            return h < (int)call.group && token < part.positions;
         };
+
+        // ---- the queries are on their way while the first copies are looked up
+        Query16<T> raw[NT][GROUPS];
+        int sees[NT];  // positions that the thread's row sees
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            int token, h;
+            const bool row = place(8 * t + quad, token, h);
+            sees[t] = row ? least + token : 0;
+            const T* x = static_cast<const T*>(call.q) + (size_t)(part.row + token) * call.q_row +
+                         (size_t)(head * (int)call.group + h) * call.q_head + 16 * j;
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) {
+                if (row)
+                    raw[t][g].load(x + 64 * g, call.wide);
+                else
+                    raw[t][g].clear();
+            }
+        }
 
         // ---- the stream of pairs: warp w takes pairs first + w, first + w + 4, ..
         const int stop = min(last, (seen + kPairTokens - 1) >> 5);  // pairs beyond hold nothing
         const int mine_pairs = max(0, (stop - first - warp + kAttentionWarps - 1) / kAttentionWarps);
-        const uint32_t per_page = c.page_size / kCellTokens;
-        const bool together = per_page % 2 == 0;  // both cells lie in one page, one behind the other
-        const int32_t* table = c.tables + (size_t)max(s.table, 0) * c.table_width;
+        const int32_t* table = c.tables + (size_t)max(part.table, 0) * c.table_width;
         const uint32_t seen_cells = (uint32_t)max((seen + kCellTokens - 1) >> 4, 0);
         const uint8_t* head_cells = c.pages + (size_t)head * per_page * Shape::kCell;
-        const size_t page_bytes = (size_t)c.kv_heads * per_page * Shape::kCell;
         // Each lane looks up one of the next 32 pairs and copies it when a stage is free.
         const uint8_t* from[2] = {nullptr, nullptr};
         uint32_t absent[2] = {0, 0};  // of the 32, those whose first or second cell has no page
@@ -521,77 +614,57 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             into = into + 1 == kStages ? 0 : into + 1;
             if ((++issued & 31) == 0) look_up(issued + lane);
         };
-        fence_proxy_async_shared();  // the ring held other things
-        __syncthreads();             // which all threads have read
 #pragma unroll 1
         for (int n = 0; n < kStages - 1; ++n) issue();
 
-        // ---- queries: the thread's columns of the score products are rows 2 j and 2 j + 1 of each eight
+        // ---- queries as the products' columns: the thread's rows of the results are 2 j and 2 j + 1 of each eight
         uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][LOW ? 4 : 2];
         float factor[NT][2], plain[NT][2][GROUPS];
         int limit[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            int token, h;
-            const bool row = place(8 * t + quad, token, h);
-            const T* x = static_cast<const T*>(call.q) + (size_t)(s.first + token) * call.q_row +
-                         (size_t)(head * call.group + h) * call.q_head + 16 * j;
-            float values[GROUPS][16], top = 0.f;
-            bool fine = true;
+            uint32_t top = 0;
 #pragma unroll
-            for (int g = 0; g < GROUPS; ++g) {
-                if (row) {
-                    load16(x + 64 * g, call.wide, values[g]);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) values[g][e] = 0.f;
-                }
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    top = fmaxf(top, fabsf(values[g][e]));
-                    fine = fine && isfinite(values[g][e]);
-                }
-            }
-            top = quad_max(top);
-            fine = quad_max(fine ? 0.f : 1.f) == 0.f;
+            for (int g = 0; g < GROUPS; ++g) top = raw[t][g].most(top);
+            top = Query16<T>::most_f32(top);
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const bool fine = top < 0x7f800000u;
             // 2^power takes the largest into 2^13 .. 2^14
-            const int power = fine && top > 0.f ? 13 - max(ilogbf(top), -100) : 0;
-            const float up = ldexpf(1.f, power);
-            const float of_row = fine ? call.scale * ldexpf(1.f, 24 - power) : nan;
+            const int power = fine && top ? 13 - max((int)(top >> 23) - 127, -100) : 0;
+            const float up = fine ? pow2(power) : 0.f, of_row = fine ? call.scale * pow2(12 - power) * 0x1p12f : nan;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 factor[t][i] = __shfl_sync(0xffffffffu, of_row, (2 * j + i) * 4);
-                limit[t][i] = __shfl_sync(0xffffffffu, row ? base + token + 1 : 0, (2 * j + i) * 4);
+                limit[t][i] = __shfl_sync(0xffffffffu, sees[t], (2 * j + i) * 4);
             }
+            // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
-                float all = 0.f;
-#pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    values[g][e] = fine ? values[g][e] * up : 0.f;
-                    all += values[g][e];
-                }
-                all = quad_sum(all) * 0x1p-24f;
-#pragma unroll
-                for (int i = 0; i < 2; ++i) plain[t][i][g] = __shfl_sync(0xffffffffu, all, (2 * j + i) * 4);
-                // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
+                float ones[4];  // the levels' factor of the zeros: the sum of the queries, with all levels 1
 #pragma unroll
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float down = e ? 0.0625f : 1.f;
-                        const float* y = values[g] + 8 * w + e;
-                        const float y0 = y[0] * down, y4 = y[4] * down, y2 = y[2] * down, y6 = y[6] * down;
+                        const float by = e ? up * 0.0625f : up;
+                        const auto value = [&](int i) { return fine ? raw[t][g].value(8 * w + e + i) * by : 0.f; };
+                        const float y0 = value(0), y4 = value(4), y2 = value(2), y6 = value(6);
                         const int f = (t * GROUPS + g) * 4 + w * 2 + e;
+                        const uint32_t one = e ? 0x00100010u : 0x00010001u, a[4] = {one, one, one, one};
                         uint32_t x0 = pack_f16(y0, y4), x1 = pack_f16(y2, y6), l0 = 0, l1 = 0;
+                        if (w + e == 0)
+                            mma_f16_first(ones, a, x0, x1);
+                        else
+                            mma_f16(ones, a, x0, x1);
                         if (LOW) {
-                            const float2 a = unpack_f16(x0), d = unpack_f16(x1);
-                            l0 = pack_f16(y0 - a.x, y4 - a.y);
-                            l1 = pack_f16(y2 - d.x, y6 - d.y);
+                            const float2 h0 = unpack_f16(x0), h1 = unpack_f16(x1);
+                            l0 = pack_f16(y0 - h0.x, y4 - h0.y);
+                            l1 = pack_f16(y2 - h1.x, y6 - h1.y);
+                            mma_f16(ones, a, l0, l1);
                         }
                         if constexpr (Shape::kSharedQuery) {
                             if (warp == f % kAttentionWarps) {
-                                uint2* at = reinterpret_cast<uint2*>(queries) + f * (LOW ? 2 : 1) * 32 + lane;
+                                uint2* at = queries + f * (LOW ? 2 : 1) * 32 + lane;
                                 at[0] = make_uint2(x0, x1);
                                 if constexpr (LOW) at[32] = make_uint2(l0, l1);
                             }
@@ -600,6 +673,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             if constexpr (LOW) query[f][2] = l0, query[f][3] = l1;
                         }
                     }
+                plain[t][0][g] = ones[0];
+                plain[t][1][g] = ones[1];
             }
         }
         if constexpr (Shape::kSharedQuery) __syncthreads();
@@ -647,7 +722,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
 #pragma unroll
-                    for (int part = 0; part < (LOW ? 2 : 1); ++part)
+                    for (int half = 0; half < (LOW ? 2 : 1); ++half)
 #pragma unroll
                         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -659,12 +734,12 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                                     const int f = (n * GROUPS + g) * 4 + w * 2 + e;
                                     uint32_t b0, b1;
                                     if constexpr (Shape::kSharedQuery) {
-                                        const uint2 x = reinterpret_cast<const uint2*>(queries)[(f * (LOW ? 2 : 1) + part) * 32 + lane];
+                                        const uint2 x = queries[(f * (LOW ? 2 : 1) + half) * 32 + lane];
                                         b0 = x.x, b1 = x.y;
                                     } else {
-                                        b0 = query[f][2 * part], b1 = query[f][2 * part + 1];
+                                        b0 = query[f][2 * half], b1 = query[f][2 * half + 1];
                                     }
-                                    if (w + e + part == 0)
+                                    if (w + e + half == 0)
                                         mma_f16_first(dot[u][g][n], a, b0, b1);
                                     else
                                         mma_f16(dot[u][g][n], a, b0, b1);
@@ -782,13 +857,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     const uint4 held_words = *reinterpret_cast<const uint4*>(cell + cell_values(D) + (g * 32 + lane) * 16);
                     const uint32_t word[4] = {held_words.x, held_words.y, held_words.z, held_words.w};
 #pragma unroll
-                    for (int part = 0; part < (LOW ? 2 : 1); ++part)
+                    for (int half = 0; half < (LOW ? 2 : 1); ++half)
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
                             const uint32_t a[4] = {word[w] & 0x000f000fu, word[w] & 0x00f000f0u, word[w] >> 8 & 0x000f000fu,
                                                    word[w] >> 8 & 0x00f000f0u};
 #pragma unroll
-                            for (int n = 0; n < NT; ++n) mma_f16(out[n][g * 4 + w], a, part ? l0[n] : p0[n], part ? l1[n] : p1[n]);
+                            for (int n = 0; n < NT; ++n) mma_f16(out[n][g * 4 + w], a, half ? l0[n] : p0[n], half ? l1[n] : p1[n]);
                         }
                 }
             }
@@ -835,7 +910,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i)
-                if (s.table < 0 || limit[t][i] > covered) sum[t][i] = nan;
+                if (part.table < 0 || limit[t][i] > covered) sum[t][i] = nan;
 
         // ---- the warps' sums
         __syncthreads();  // the rings are drained
@@ -859,8 +934,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             }
         __syncthreads();
         const bool whole = first == 0 && last == pairs;
-        float* part = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * Shape::kRows * Shape::kPart;
-        for (int i = warp; i < Shape::kRows; i += kAttentionWarps) {
+        float* to_add = call.parts + ((size_t)blockIdx.x * 2 + (first == 0)) * call.used * Shape::kPart;
+        for (int i = warp; i < (int)call.used; i += kAttentionWarps) {
             int token, h;
             if (!place(i, token, h)) continue;
             float top = kNone, l = 0.f, weight[kAttentionWarps];
@@ -873,8 +948,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 l += weight[w] * row[D + 1];
             }
             const float inverse = l == 0.f ? 0.f : 1.f / l;
-            T* to = static_cast<T*>(call.out) + (size_t)(s.first + token) * call.out_row +
-                    (size_t)(head * call.group + h) * call.out_head;
+            T* to = static_cast<T*>(call.out) + (size_t)(part.row + token) * call.out_row +
+                    (size_t)(head * (int)call.group + h) * call.out_head;
             for (int d = lane; d < D; d += 32) {
                 float x = 0.f;
 #pragma unroll
@@ -882,113 +957,85 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 if (whole)
                     to[d] = from_f32<T>(x * inverse);
                 else
-                    part[(size_t)i * Shape::kPart + d] = x;
+                    to_add[(size_t)i * Shape::kPart + d] = x;
             }
-            if (!whole && lane == 0) part[(size_t)i * Shape::kPart + D] = top, part[(size_t)i * Shape::kPart + D + 1] = l;
+            if (!whole && lane == 0) *reinterpret_cast<float2*>(to_add + (size_t)i * Shape::kPart + D) = make_float2(top, l);
         }
         if (first == 0 && !whole && threadIdx.x == 0)
-            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), s.first + k * tokens, (int)head_sub,
-                                               tile_end - k * tokens);
+            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), part.row,
+                                               head * (int)call.subs + sub, part.positions);
+        __syncthreads();  // the part and the sums are read
     }
 }
 
-// Adds up the parts of the tiles that a block of attention_kernel started and others
-// finished, in a fixed order.  The blocks list those tiles and share their rows out; a row's
-// parts are dealt to eight warps.
-constexpr int kMergeWarps = 8, kMergeEach = 3;
+// Adds up the parts of the tile that block blockIdx.x of attention_kernel started and others
+// finished, in a fixed order: up to four of its rows a block, sixteen warps that share them
+// and their parts out.  Most blocks find nothing to do.
+constexpr int kMergeWarps = 16, kMergeRows = 4;
 
 template <typename T, int GROUPS>
-__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(AttentionCall call, int rows, int blocks) {
-    constexpr int D = 64 * GROUPS, kRow = part_row(D), kEach = D / 32;
-    extern __shared__ int started[];  // [blocks] those with a tile to add up
-    __shared__ int counts[kMergeEach][kMergeWarps];
+__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(AttentionCall call, int rows) {
+    constexpr int D = 64 * GROUPS, kRow = part_row(D), kEach = D / 32, kAhead = 4;
     __shared__ float2 about_warp[kMergeWarps];  // reference and sum of the weights
     __shared__ float sums[kMergeWarps][D];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
+    const int used = min((int)call.used - (int)blockIdx.y * kMergeRows, kMergeRows), per_row = kMergeWarps / used;
+    pdl_launch_dependents();
     pdl_wait();
-    int found = 0;
-    for (int base = 0; base < blocks; base += kMergeEach * 32 * kMergeWarps) {
-        unsigned votes[kMergeEach];
+    const int4 tail = call.tails[blockIdx.x];  // parts, first row, key head and part of it, positions
+    if (tail.x == 0) return;
+    const int mine = warp / per_row, i = (int)blockIdx.y * kMergeRows + mine;
+    float top = -1e30f, l = 0.f, x[kEach] = {};
+    for (int n = mine < used ? warp % per_row : tail.x; n < tail.x; n += kAhead * per_row) {  // all loads ahead of their use
+        float2 about[kAhead];
+        float row[kAhead][kEach];
 #pragma unroll
-        for (int i = 0; i < kMergeEach; ++i) {
-            const int block = base + i * 32 * kMergeWarps + (int)threadIdx.x;
-            votes[i] = __ballot_sync(0xffffffffu, block < blocks && call.tails[block].x > 0);
-            if (lane == 0) counts[i][warp] = __popc(votes[i]);
-        }
-        __syncthreads();
+        for (int m = 0; m < kAhead; ++m) {
+            about[m] = make_float2(-1e30f, 0.f);
 #pragma unroll
-        for (int i = 0; i < kMergeEach; ++i) {
-            int before = found;
+            for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
+            const int from = n + m * per_row;
+            if (from < tail.x) {
+                const float* p = call.parts + (((size_t)((int)blockIdx.x + from) * 2 + (from == 0)) * call.used + i) * kRow;
+                about[m] = *reinterpret_cast<const float2*>(p + D);
 #pragma unroll
-            for (int w = 0; w < kMergeWarps; ++w) {
-                if (w < warp) before += counts[i][w];
-                found += counts[i][w];
+                for (int e = 0; e < kEach; ++e) row[m][e] = p[e * 32 + lane];
             }
-            if (votes[i] >> lane & 1)
-                started[before + __popc(votes[i] & ((1u << lane) - 1))] = base + i * 32 * kMergeWarps + (int)threadIdx.x;
         }
-        __syncthreads();
+        const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
+        const float keep = exp2_approx(top - now);
+        top = now;
+        l *= keep;
+#pragma unroll
+        for (int e = 0; e < kEach; ++e) x[e] *= keep;
+#pragma unroll
+        for (int m = 0; m < kAhead; ++m) {
+            const float weight = exp2_approx(about[m].x - now);
+            l = fmaf(about[m].y, weight, l);
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
+        }
     }
-    const int used = (int)call.used;
-    for (int item = (int)blockIdx.x; item < found * used; item += (int)gridDim.x) {
-        const int block = started[item / used], i = item % used;
-        const int4 tail = call.tails[block];
-        const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs;
-        const int token = call.subs > 1 ? 0 : i / (int)call.group;
-        const int h = call.subs > 1 ? sub * rows + i : i % (int)call.group;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
+    if (lane == 0) about_warp[warp] = make_float2(top, l);
+    __syncthreads();
+    const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs;
+    for (int d = (int)threadIdx.x; d < used * D; d += 32 * kMergeWarps) {
+        const int row = d / D, first = row * per_row, k = (int)blockIdx.y * kMergeRows + row;
+        const int token = call.subs > 1 ? 0 : k / (int)call.group;
+        const int h = call.subs > 1 ? sub * rows + k : k % (int)call.group;
         if (h >= (int)call.group || token >= tail.w) continue;
-        float top = -1e30f, l = 0.f, x[kEach] = {};
-        for (int n = warp; n < tail.x; n += 4 * kMergeWarps) {  // four at a time, all loads ahead of their use
-            float2 about[4];
-            float row[4][kEach];
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                about[m] = make_float2(-1e30f, 0.f);
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
-                const int from = n + m * kMergeWarps;
-                if (from < tail.x) {
-                    const float* p = call.parts + (((size_t)(block + from) * 2 + (from == 0)) * rows + i) * kRow;
-                    about[m] = *reinterpret_cast<const float2*>(p + D);
-#pragma unroll
-                    for (int e = 0; e < kEach; ++e) row[m][e] = p[e * 32 + lane];
-                }
-            }
-            const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
-            const float keep = exp2_approx(top - now);
-            top = now;
-            l *= keep;
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) x[e] *= keep;
-#pragma unroll
-            for (int m = 0; m < 4; ++m) {
-                const float weight = exp2_approx(about[m].x - now);
-                l = fmaf(about[m].y, weight, l);
-#pragma unroll
-                for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
-            }
-        }
-        __syncthreads();  // the row before is read
-#pragma unroll
-        for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
-        if (lane == 0) about_warp[warp] = make_float2(top, l);
-        __syncthreads();
         top = -1e30f, l = 0.f;
-        float weight[kMergeWarps];
-#pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) top = fmaxf(top, about_warp[w].x);
-#pragma unroll
-        for (int w = 0; w < kMergeWarps; ++w) {
-            weight[w] = exp2_approx(about_warp[w].x - top);
-            l = fmaf(about_warp[w].y, weight[w], l);
+        for (int w = first; w < first + per_row; ++w) top = fmaxf(top, about_warp[w].x);
+        float y = 0.f;
+        for (int w = first; w < first + per_row; ++w) {
+            const float weight = exp2_approx(about_warp[w].x - top);
+            l = fmaf(about_warp[w].y, weight, l);
+            y = fmaf(sums[w][d % D], weight, y);
         }
         T* to = static_cast<T*>(call.out) + (size_t)(tail.y + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
-        for (int d = (int)threadIdx.x; d < D; d += 32 * kMergeWarps) {
-            float y = 0.f;
-#pragma unroll
-            for (int w = 0; w < kMergeWarps; ++w) y = fmaf(sums[w][d], weight[w], y);
-            to[d] = from_f32<T>(l == 0.f ? 0.f : y / l);
-        }
+        to[d % D] = from_f32<T>(l == 0.f ? 0.f : y / l);
     }
 }
 
@@ -1329,7 +1376,7 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
     const size_t pieces = (pool.page_bytes / 16 + kCopyThreads * kCopyVectors - 1) / (kCopyThreads * kCopyVectors);
     const size_t work = std::max(count * pool.layers * pieces, (entries + kCopyThreads - 1) / kCopyThreads);
     const unsigned blocks = (unsigned)std::min<size_t>(work, (size_t)ctx->sm_count * 6);
-    return launch_dependent(copy_pages_kernel, blocks, kCopyThreads, 0, s, (uint8_t*)pool.data, (uint32_t)pool.layers,
+    return launch_dependent(copy_pages_kernel, dim3(blocks), kCopyThreads, 0, s, (uint8_t*)pool.data, (uint32_t)pool.layers,
                             pool.layer_bytes, pool.page_bytes, (uint32_t)pool.page_count, pairs, (uint32_t)count, moved,
                             tables, tables_out, (uint64_t)entries, to_of);
 }
@@ -1374,11 +1421,10 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     call.parts = reinterpret_cast<float*>(call.tails + blocks);
     cudaError_t status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
     if (status != cudaSuccess) return status;
-    kernel<<<blocks, kAttentionThreads, Shape::kShared, s>>>(c, r, call);
-    status = cudaGetLastError();
+    status = launch_dependent(kernel, dim3(blocks), kAttentionThreads, Shape::kShared, s, c, r, call);
     if (status != cudaSuccess) return status;
-    return launch_dependent(attention_merge_kernel<T, GROUPS>, std::min(blocks * call.used, (unsigned)sm_count * 6), 32 * kMergeWarps,
-                            blocks * 4, s, call, Shape::kRows, (int)blocks);
+    return launch_dependent(attention_merge_kernel<T, GROUPS>, dim3(blocks, (call.used + kMergeRows - 1) / kMergeRows),
+                            32 * kMergeWarps, 0, s, call, Shape::kRows);
 }
 
 // Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where
