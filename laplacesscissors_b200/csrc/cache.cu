@@ -222,11 +222,13 @@ __global__ void __launch_bounds__(128) read_kernel(CacheView c, CacheRows r, T* 
 // copies, with its own softmax; the warps' sums meet at a tile's end.
 //
 // Cost that a block takes at least, where there is little: a tile and two pairs a warp.
-constexpr int kLeastRun = 12;
+constexpr int kLeastRun = 20;
 constexpr int kPairTokens = 2 * kCellTokens;
+// Positions of a table row up to which tiles are not shared.
+constexpr int kWholeTokens = 512;
 // What a tile costs beside its pairs (the first copies' latency, the queries, the sums), in
 // pairs: it counts so many more when the runs are cut.
-constexpr int kTileCost = 6;
+constexpr int kTileCost = 12;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
 // Floats of a row's part: its sums, its reference and the sum of its weights.
@@ -235,15 +237,15 @@ constexpr int part_row(int dim) { return dim + 2; }
 template <int GROUPS, int NT, bool LOW>
 struct AttentionShape {
     static constexpr int kDim = 64 * GROUPS, kPart = part_row(kDim), kRows = 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
-    static constexpr int kLoad = NT * GROUPS;
-    static constexpr int kBlocksPerSm = kLoad <= 2 ? 4 : kLoad <= 4 && GROUPS < 4 ? 3 : 2;
-    // registers a thread: the sums and the queries, which go to shared memory where 75 are not left for the rest
-    static constexpr int kSums = 16 * kLoad, kQueries = (LOW ? 16 : 8) * kLoad;
-    static constexpr bool kSharedQuery = kSums + kQueries > (kBlocksPerSm == 2 ? 255 : 512 / kBlocksPerSm) - 75;
+    // registers a thread: the sums and the queries, beside some 75 for the rest; where those are not left the
+    // queries go to shared memory
+    static constexpr int kLoad = NT * GROUPS, kHeld = (LOW ? 32 : 24) * kLoad;
+    static constexpr int kBlocksPerSm = kHeld <= 64 ? 4 : kHeld <= 96 ? 3 : 2;
+    static constexpr bool kSharedQuery = kHeld > (kBlocksPerSm == 4 ? 53 : kBlocksPerSm == 3 ? 96 : 180);
     static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW ? 16 : 8) : 0;
     static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
-    static constexpr int kAtOnce = NT == 1 ? 2 : 1;  // cells whose weights a thread holds at the same time
+    static constexpr int kAtOnce = NT == 1 && GROUPS <= 2 ? 2 : 1;  // cells whose weights a thread holds at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
     static constexpr int kParts = kAttentionWarps * kRows * kPart * 4;  // the warps' sums, in the ring's memory
     static constexpr int kBars = kAttentionWarps * kStages * 8;
@@ -260,8 +262,9 @@ struct AttentionCall {
     uint32_t used;             // of the tile's rows, those that hold any
     float scale;               // times log2 e
     bool wide;                 // queries lie to 16 bytes
-    int4* tails;               // [blocks] tiles that a block starts and others finish: their parts (0: none), first row, key
-                               // head and part of it, positions
+    bool whole;                // tiles are not shared
+    int* shares;               // [blocks] parts of the tile that a block starts and others finish, 0 where there is none
+    int4* tails;               // [blocks] that tile's first row, key head, part of it, and positions
     float* parts;              // [2 blocks][rows][part_row(dim)]
 };
 
@@ -466,7 +469,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     long long at = run * blockIdx.x, offset = 0;  // cost: the run's next, and that within sequence b
     const long long end = min(at + run, total);
     uint32_t b = 0;
-    if (threadIdx.x == 0) call.tails[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (threadIdx.x == 0) call.shares[blockIdx.x] = 0;
     if (at >= end) return;
     if (mine > 0 && before <= at && at < before + mine) {
         for (uint32_t n = mine_first; n < mine_end; ++n) {
@@ -507,10 +510,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             }
             // the first kTileCost of a tile's cost stand for no pair
             const int pairs = tile_pairs(s, tokens, k), from_cost = (int)(rest - cost_before(s, tokens, k));
-            const int to_cost = (int)min((long long)pairs + kTileCost, from_cost + end - at);
+            const int to_cost = call.whole ? pairs + kTileCost : (int)min((long long)pairs + kTileCost, from_cost + end - at);
             at += to_cost - from_cost;
             offset += to_cost - from_cost;
-            if (to_cost <= kTileCost) continue;
+            if (to_cost <= kTileCost || (call.whole && from_cost > 0)) continue;
             const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
             next.first = max(from_cost - kTileCost, 0);
             next.last = to_cost - kTileCost;
@@ -961,81 +964,103 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             }
             if (!whole && lane == 0) *reinterpret_cast<float2*>(to_add + (size_t)i * Shape::kPart + D) = make_float2(top, l);
         }
-        if (first == 0 && !whole && threadIdx.x == 0)
-            call.tails[blockIdx.x] = make_int4(1 + (int)((pairs - last + run - 1) / run), part.row,
-                                               head * (int)call.subs + sub, part.positions);
+        if (first == 0 && !whole && threadIdx.x == 0) {
+            call.shares[blockIdx.x] = 1 + (int)((pairs - last + run - 1) / run);
+            call.tails[blockIdx.x] = make_int4(part.row, head, sub, part.positions);
+        }
         __syncthreads();  // the part and the sums are read
     }
 }
 
-// Adds up the parts of the tile that block blockIdx.x of attention_kernel started and others
-// finished, in a fixed order: up to four of its rows a block, sixteen warps that share them
-// and their parts out.  Most blocks find nothing to do.
-constexpr int kMergeWarps = 16, kMergeRows = 4;
+// Adds up the parts of the tiles that a block of attention_kernel started and others
+// finished, in a fixed order.  Each block lists those tiles (few blocks that read all marks
+// start sooner than one for each block before them) and takes some, `most` rows at a time;
+// its sixteen warps share the rows and their parts out.
+constexpr int kMergeWarps = 16;
 
 template <typename T, int GROUPS>
-__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(AttentionCall call, int rows) {
+__global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(AttentionCall call, int rows, int most, int blocks) {
     constexpr int D = 64 * GROUPS, kRow = part_row(D), kEach = D / 32, kAhead = 4;
+    extern __shared__ int started[];  // [blocks] those that started a shared tile
+    __shared__ int counts[kMergeWarps];
     __shared__ float2 about_warp[kMergeWarps];  // reference and sum of the weights
     __shared__ float sums[kMergeWarps][D];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
-    const int used = min((int)call.used - (int)blockIdx.y * kMergeRows, kMergeRows), per_row = kMergeWarps / used;
     pdl_launch_dependents();
     pdl_wait();
-    const int4 tail = call.tails[blockIdx.x];  // parts, first row, key head and part of it, positions
-    if (tail.x == 0) return;
-    const int mine = warp / per_row, i = (int)blockIdx.y * kMergeRows + mine;
-    float top = -1e30f, l = 0.f, x[kEach] = {};
-    for (int n = mine < used ? warp % per_row : tail.x; n < tail.x; n += kAhead * per_row) {  // all loads ahead of their use
-        float2 about[kAhead];
-        float row[kAhead][kEach];
+    int tiles = 0;
+    for (int base = 0; base < blocks; base += 32 * kMergeWarps) {
+        const int block = base + (int)threadIdx.x;
+        const unsigned votes = __ballot_sync(0xffffffffu, block < blocks && call.shares[block] > 0);
+        if (lane == 0) counts[warp] = __popc(votes);
+        __syncthreads();
+        int before = tiles;
 #pragma unroll
-        for (int m = 0; m < kAhead; ++m) {
-            about[m] = make_float2(-1e30f, 0.f);
+        for (int w = 0; w < kMergeWarps; ++w) {
+            if (w < warp) before += counts[w];
+            tiles += counts[w];
+        }
+        if (votes >> lane & 1) started[before + __popc(votes & ((1u << lane) - 1))] = block;
+        __syncthreads();
+    }
+    const int pieces = ((int)call.used + most - 1) / most;
+    for (int item = (int)blockIdx.x; item < tiles * pieces; item += (int)gridDim.x) {
+        const int block = started[item / pieces], first_row = item % pieces * most;
+        const int count = call.shares[block], used = min((int)call.used - first_row, most), per_row = kMergeWarps / used;
+        const int4 tail = call.tails[block];
+        const int mine = warp / per_row, i = first_row + mine;
+        float top = -1e30f, l = 0.f, x[kEach] = {};
+        for (int n = mine < used ? warp % per_row : count; n < count; n += kAhead * per_row) {  // all loads ahead of their use
+            float2 about[kAhead];
+            float row[kAhead][kEach];
 #pragma unroll
-            for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
-            const int from = n + m * per_row;
-            if (from < tail.x) {
-                const float* p = call.parts + (((size_t)((int)blockIdx.x + from) * 2 + (from == 0)) * call.used + i) * kRow;
-                about[m] = *reinterpret_cast<const float2*>(p + D);
+            for (int m = 0; m < kAhead; ++m) {
+                about[m] = make_float2(-1e30f, 0.f);
 #pragma unroll
-                for (int e = 0; e < kEach; ++e) row[m][e] = p[e * 32 + lane];
+                for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
+                const int from = n + m * per_row;
+                if (from < count) {
+                    const float* p = call.parts + (((size_t)(block + from) * 2 + (from == 0)) * call.used + i) * kRow;
+                    about[m] = *reinterpret_cast<const float2*>(p + D);
+#pragma unroll
+                    for (int e = 0; e < kEach; ++e) row[m][e] = p[e * 32 + lane];
+                }
+            }
+            const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
+            const float keep = exp2_approx(top - now);
+            top = now;
+            l *= keep;
+#pragma unroll
+            for (int e = 0; e < kEach; ++e) x[e] *= keep;
+#pragma unroll
+            for (int m = 0; m < kAhead; ++m) {
+                const float weight = exp2_approx(about[m].x - now);
+                l = fmaf(about[m].y, weight, l);
+#pragma unroll
+                for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
             }
         }
-        const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
-        const float keep = exp2_approx(top - now);
-        top = now;
-        l *= keep;
 #pragma unroll
-        for (int e = 0; e < kEach; ++e) x[e] *= keep;
-#pragma unroll
-        for (int m = 0; m < kAhead; ++m) {
-            const float weight = exp2_approx(about[m].x - now);
-            l = fmaf(about[m].y, weight, l);
-#pragma unroll
-            for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
+        for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
+        if (lane == 0) about_warp[warp] = make_float2(top, l);
+        __syncthreads();
+        for (int d = (int)threadIdx.x; d < used * D; d += 32 * kMergeWarps) {
+            const int row = d / D, first = row * per_row, k = first_row + row;
+            const int token = call.subs > 1 ? 0 : k / (int)call.group;
+            const int h = call.subs > 1 ? tail.z * rows + k : k % (int)call.group;
+            if (h >= (int)call.group || token >= tail.w) continue;
+            top = -1e30f, l = 0.f;
+            for (int w = first; w < first + per_row; ++w) top = fmaxf(top, about_warp[w].x);
+            float y = 0.f;
+            for (int w = first; w < first + per_row; ++w) {
+                const float weight = exp2_approx(about_warp[w].x - top);
+                l = fmaf(about_warp[w].y, weight, l);
+                y = fmaf(sums[w][d % D], weight, y);
+            }
+            T* to = static_cast<T*>(call.out) + (size_t)(tail.x + token) * call.out_row + (size_t)(tail.y * (int)call.group + h) * call.out_head;
+            to[d % D] = from_f32<T>(l == 0.f ? 0.f : y / l);
         }
-    }
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
-    if (lane == 0) about_warp[warp] = make_float2(top, l);
-    __syncthreads();
-    const int head = tail.z / (int)call.subs, sub = tail.z % (int)call.subs;
-    for (int d = (int)threadIdx.x; d < used * D; d += 32 * kMergeWarps) {
-        const int row = d / D, first = row * per_row, k = (int)blockIdx.y * kMergeRows + row;
-        const int token = call.subs > 1 ? 0 : k / (int)call.group;
-        const int h = call.subs > 1 ? sub * rows + k : k % (int)call.group;
-        if (h >= (int)call.group || token >= tail.w) continue;
-        top = -1e30f, l = 0.f;
-        for (int w = first; w < first + per_row; ++w) top = fmaxf(top, about_warp[w].x);
-        float y = 0.f;
-        for (int w = first; w < first + per_row; ++w) {
-            const float weight = exp2_approx(about_warp[w].x - top);
-            l = fmaf(about_warp[w].y, weight, l);
-            y = fmaf(sums[w][d % D], weight, y);
-        }
-        T* to = static_cast<T*>(call.out) + (size_t)(tail.y + token) * call.out_row + (size_t)(head * (int)call.group + h) * call.out_head;
-        to[d % D] = from_f32<T>(l == 0.f ? 0.f : y / l);
+        __syncthreads();
     }
 }
 
@@ -1386,7 +1411,7 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
 template <int GROUPS, int NT, bool LOW>
 size_t attention_bytes(int sm_count) {
     using Shape = AttentionShape<GROUPS, NT, LOW>;
-    return (size_t)sm_count * Shape::kBlocksPerSm * (16 + 2 * Shape::kRows * Shape::kPart * 4);
+    return (size_t)sm_count * Shape::kBlocksPerSm * (20 + 2 * Shape::kRows * Shape::kPart * 4);
 }
 
 template <int GROUPS>
@@ -1417,14 +1442,22 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     while (call.tokens * 2 * call.group <= (uint32_t)Shape::kRows) call.tokens *= 2;
     call.subs = (call.group + Shape::kRows - 1) / Shape::kRows;
     call.used = std::min<uint32_t>(Shape::kRows, call.tokens * call.group);
+    // Where a row of the tables covers few positions nothing is gained by sharing a tile, and the second launch is
+    // left out (one sequence of 9 positions: 8.3 us with it, 5.9 without).
+    call.whole = (uint64_t)c.table_width * c.page_size <= kWholeTokens;
     call.tails = static_cast<int4*>(workspace);
-    call.parts = reinterpret_cast<float*>(call.tails + blocks);
+    call.shares = reinterpret_cast<int*>(call.tails + blocks);
+    call.parts = reinterpret_cast<float*>(call.shares + blocks);
     cudaError_t status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
     if (status != cudaSuccess) return status;
     status = launch_dependent(kernel, dim3(blocks), kAttentionThreads, Shape::kShared, s, c, r, call);
     if (status != cudaSuccess) return status;
-    return launch_dependent(attention_merge_kernel<T, GROUPS>, dim3(blocks, (call.used + kMergeRows - 1) / kMergeRows),
-                            32 * kMergeWarps, 0, s, call, Shape::kRows);
+    if (call.whole) return cudaSuccess;
+    // rows that a block takes at a time: with few tiles each has many parts, for all warps of a block
+    const uint64_t tiles = ((uint64_t)r.rows / call.tokens + r.count) * c.kv_heads * call.subs;  // at most
+    const unsigned most = tiles * kMergeWarps <= blocks ? 1 : 4, pieces = (call.used + most - 1) / most;
+    return launch_dependent(attention_merge_kernel<T, GROUPS>, dim3((unsigned)std::min<uint64_t>(tiles * pieces, 2 * (unsigned)sm_count)),
+                            32 * kMergeWarps, blocks * 4, s, call, Shape::kRows, (int)most, (int)blocks);
 }
 
 // Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where
