@@ -4,6 +4,7 @@
 #include <cuda_fp16.h>
 
 #include <algorithm>
+#include <atomic>
 #include <limits>
 #include <type_traits>
 
@@ -101,18 +102,49 @@ __device__ __forceinline__ uint8_t* cell_of(const CacheView& c, int table, uint3
 }
 
 // ---- append and read -----------------------------------------------------------
-// (x - z) / s rounded to nearest, ties to even, in 64 bits, which hold x - z of any f32 x that is not lost
-// beside z.
-__device__ __noinline__ float exact_level(float x, float z, float s) { return (float)rint(((double)x - (double)z) / (double)s); }
+// Levels.  (x - z) / s is rounded to nearest, ties to even, exactly.  Its f32 value `about` (inv = 1 / s, 0 for s = 0;
+// clamped to 0..15) is off by less than 15 * 3 * 2^-24, so it decides unless it lies within 2^-16 of a tie; f16 and
+// bf16 elements lie on one in a thousand cases.
+constexpr float kRound = 0x1.8p23f;  // an f32 plus this has its integer in the last bits
+__device__ __forceinline__ float about_level(float x, float z, float inv) { return fminf(fmaxf((x - z) * inv, 0.f), 15.f); }
 
-// The level 0..15 of x in a group with zero z and step s (inv = 1 / s, 0 for s = 0), as the low bits of an f32 of
-// 2^23: the f32 quotient is off by less than 15 * 3 * 2^-24, so only where it lies within 2^-16 of a tie it
-// is formed exactly.
+// The level next to a tie k + 1/2, by the sign of (x - z) - (k + 1/2) s: x - z is a + low exactly (Knuth's sum of
+// two), (k + 1/2) s has 16 bits, and its difference from the close a is exact and, unless it is 0, above low.
+__device__ __forceinline__ float tied_level(float x, float z, float s, float about) {
+    const float k = floorf(about), a = x - z, b = a - x, low = (x - (a - b)) + (-z - b);
+    const float side = fmaf(-(k + 0.5f), s, a) + low;
+    return side > 0.f || (side == 0.f && ((int)k & 1)) ? k + 1.f : k;
+}
 __device__ __forceinline__ uint32_t level_of(float x, float z, float s, float inv) {
-    const float t = fminf(fmaxf((x - z) * inv, 0.f), 15.f);
-    float n = t + 0x1.8p23f;  // the sum's last bit is 1
-    if (fabsf(t - (n - 0x1.8p23f)) > 0.5f - 0x1p-16f && s > 0.f) n = fminf(fmaxf(exact_level(x, z, s), 0.f), 15.f) + 0x1.8p23f;
-    return __float_as_uint(n) & 15;
+    const float about = about_level(x, z, inv);
+    float level = about + kRound;
+    if (fabsf(about - (level - kRound)) > 0.5f - 0x1p-16f) level = tied_level(x, z, s, about) + kRound;
+    return __float_as_uint(level) & 15;
+}
+
+// The extremes of a group; NaN where one of its elements is.
+__device__ __forceinline__ void extremes(const float (&x)[64], float& low, float& high) {
+    low = high = x[0];
+#pragma unroll
+    for (int e = 1; e < 64; ++e) {
+        asm("min.NaN.f32 %0, %0, %1;" : "+f"(low) : "f"(x[e]));
+        asm("max.NaN.f32 %0, %0, %1;" : "+f"(high) : "f"(x[e]));
+    }
+}
+template <typename T2, typename T>
+__device__ __forceinline__ void extremes_of_pairs(const T (&x)[64], float& low, float& high) {
+    T2 least = *reinterpret_cast<const T2*>(x), most = least;
+#pragma unroll
+    for (int e = 2; e < 64; e += 2) {
+        least = __hmin2_nan(least, *reinterpret_cast<const T2*>(x + e));
+        most = __hmax2_nan(most, *reinterpret_cast<const T2*>(x + e));
+    }
+    low = to_f32(__hmin_nan(least.x, least.y));
+    high = to_f32(__hmax_nan(most.x, most.y));
+}
+__device__ __forceinline__ void extremes(const __half (&x)[64], float& low, float& high) { extremes_of_pairs<__half2>(x, low, high); }
+__device__ __forceinline__ void extremes(const __nv_bfloat16 (&x)[64], float& low, float& high) {
+    extremes_of_pairs<__nv_bfloat162>(x, low, high);
 }
 
 // A group's zero and step from its extremes, and 1 / step; false where they cannot be held.
@@ -188,43 +220,49 @@ __global__ void __launch_bounds__(128) append_rows_kernel(const T* k, const T* v
     }
 }
 
-// Many rows a sequence: one warp a (sixteen rows of the call, head), and those cells whose first new position is
-// among the rows.  A lane takes a position's group of keys or values whole, sixteen positions side by side, so
-// that nothing is exchanged; a cell that is new throughout is put together in shared memory and
-// written in one go.  (12 thousand rows of 8 x 128 bf16: 21 us; the kernel above 100 us.)
+// Many rows a sequence: a warp a group of 64 elements for a (sixteen rows of the call, head), and those cells
+// whose first new position is among the rows.  A lane takes a position's group of keys or values whole,
+// sixteen positions side by side, so that nothing is exchanged; a cell that is new throughout is put
+// together in shared memory and written in one go.
 constexpr int kCellWarps = 4;
 
+template <int GROUPS>
+constexpr int kAppendUnits = GROUPS == 1 ? 4 : GROUPS == 2 ? 2 : 1;  // (rows, head)s of a block
+
 template <typename T, int GROUPS>
-__global__ void __launch_bounds__(32 * kCellWarps) append_cells_kernel(const T* k, const T* v, size_t k_row, size_t k_head,
-                                                                       size_t v_row, size_t v_head, bool wide, CacheView c,
-                                                                       CacheRows r) {
-    constexpr int D = 64 * GROUPS, kEach = 16 / sizeof(T);
-    __shared__ __align__(16) uint8_t cells[kCellWarps][cell_bytes(D)];
+__global__ void __launch_bounds__(32 * GROUPS * kAppendUnits<GROUPS>) append_cells_kernel(
+    const T* k, const T* v, size_t k_row, size_t k_head, size_t v_row, size_t v_head, bool wide, CacheView c, CacheRows r) {
+    constexpr int D = 64 * GROUPS, kEach = 16 / sizeof(T), kUnits = kAppendUnits<GROUPS>;
+    __shared__ __align__(16) uint8_t cells[kUnits][cell_bytes(D)];
     pdl_wait();
     pdl_launch_dependents();
-    const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
-    const uint64_t unit = (uint64_t)blockIdx.x * kCellWarps + warp;
+    const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32, i = warp % GROUPS;
+    const uint64_t unit = (uint64_t)blockIdx.x * kUnits + warp / GROUPS;
+    uint8_t* shared_cell = cells[warp / GROUPS];
+    const auto meet = [&] {  // the unit's warps
+        if constexpr (GROUPS == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(warp / GROUPS + 1), "n"(32 * GROUPS) : "memory");
+    };
     const uint32_t first = (uint32_t)(unit / c.kv_heads) * kCellTokens, head = (uint32_t)(unit % c.kv_heads);
     if (first >= r.rows) return;
     RowPlace mine = {};
     if (lane < kCellTokens && first + lane < r.rows) mine = row_place(c, r, first + lane, head);
     // a cell begins here, or the sequence's rows begin inside it (those before position 0 have none)
     unsigned begins = __ballot_sync(0xffffffffu, mine.cell && (mine.first || mine.position % kCellTokens == 0));
+    // sixteen lanes a group of the keys, then of the values
+    const int part = 2 * i + lane / 16, g = part % GROUPS, n = lane % 16;
+    const bool value = part >= GROUPS;
     for (; begins; begins &= begins - 1) {
         const int at = __ffs(begins) - 1;
         const uint32_t row = first + at;
         uint8_t* cell = reinterpret_cast<uint8_t*>(__shfl_sync(0xffffffffu, (unsigned long long)mine.cell, at));
-        const int t0 = __shfl_sync(0xffffffffu, mine.position, at) % kCellTokens;
-        const int count = min(kCellTokens - t0, __shfl_sync(0xffffffffu, mine.after, at));
-        uint8_t* to = count == kCellTokens ? cells[warp] : cell;
-#pragma unroll 1
-        for (int i = 0; i < GROUPS; ++i) {
-            // sixteen lanes a group of the keys, then of the values
-            const int part = 2 * i + lane / 16, g = part % GROUPS, n = lane % 16, t = t0 + n;
-            const bool value = part >= GROUPS;
-            if (n >= count) continue;
-            const T* x = value ? v + (row + n) * v_row + head * v_head : k + (row + n) * k_row + head * k_head;
-            x += 64 * g;
+        const int t = __shfl_sync(0xffffffffu, mine.position, at) % kCellTokens + n;
+        const int count = min(kCellTokens + n - t, __shfl_sync(0xffffffffu, mine.after, at));
+        uint8_t* to = count == kCellTokens ? shared_cell : cell;
+        if (n < count) {
+            const T* x = (value ? v + (row + n) * v_row + head * v_head : k + (row + n) * k_row + head * k_head) + 64 * g;
             __align__(16) T raw[64];
             if (wide) {
 #pragma unroll
@@ -234,44 +272,38 @@ __global__ void __launch_bounds__(32 * kCellWarps) append_cells_kernel(const T* 
 #pragma unroll
                 for (int e = 0; e < 64; ++e) raw[e] = x[e];
             }
-            float low = to_f32(raw[0]), high = low;
-            bool finite = isfinite(low);
-#pragma unroll
-            for (int e = 1; e < 64; ++e) {
-                const float y = to_f32(raw[e]);
-                low = fminf(low, y);
-                high = fmaxf(high, y);
-                finite = finite && isfinite(y);
-            }
+            float low, high;
+            extremes(raw, low, high);
             __half zero, step;
             float inv;
-            finite = group_steps(low, high, finite, zero, step, inv);
-            const float z = finite ? __half2float(zero) : 0.f, s = finite ? __half2float(step) : 0.f;
-            const auto level = [&](int e) { return finite ? level_of(to_f32(raw[e]), z, s, inv) : 0u; };
-            if (value) {
+            group_steps(low, high, isfinite(low) && isfinite(high), zero, step, inv);  // a zero that is NaN makes all levels 0
+            const float z = __half2float(zero), s = __half2float(step);
+            uint8_t* part_of = to + (value ? value_byte(D, t, 64 * g) : key_byte(t, 64 * g));
 #pragma unroll
-                for (int e = 0; e < 32; ++e)
-                    to[value_byte(D, t, 64 * g + e / 8 * 16 + e % 8)] = (uint8_t)(level(e / 8 * 16 + e % 8) | level(e / 8 * 16 + e % 8 + 8) << 4);
-            } else {
+            for (int e = 0; e < 4; ++e) {  // sixteen elements: a lane of the keys' layout, a word of the values'
+                uint32_t level[16];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
+                for (int m = 0; m < 16; ++m) level[m] = level_of(to_f32(raw[16 * e + m]), z, s, inv);
+                if (value) {
+#pragma unroll
+                    for (int m = 0; m < 8; ++m) part_of[4 * e + 64 * m] = (uint8_t)(level[m] | level[m + 8] << 4);
+                } else {
                     uint32_t words[2] = {0, 0};
 #pragma unroll
-                    for (int m = 0; m < 16; ++m) words[m / 8] |= level(16 * e + m) << 4 * (m % 8);
-                    *reinterpret_cast<uint2*>(to + key_byte(t, 64 * g + 16 * e)) = make_uint2(words[0], words[1]);
+                    for (int m = 0; m < 16; ++m) words[m / 8] |= level[m] << 4 * (m % 8);
+                    *reinterpret_cast<uint2*>(part_of + 16 * e) = make_uint2(words[0], words[1]);
                 }
             }
             __half* steps = reinterpret_cast<__half*>(to + (value ? cell_value_steps(D) : cell_key_steps(D)) + step_byte(t, g));
             steps[0] = step;
             steps[2] = zero;
         }
-        __syncwarp();
         if (count == kCellTokens) {
+            meet();
 #pragma unroll
-            for (int e = 0; e < (cell_bytes(D) / 16 + 31) / 32; ++e)
-                if (e * 32 + lane < cell_bytes(D) / 16)
-                    reinterpret_cast<uint4*>(cell)[e * 32 + lane] = reinterpret_cast<const uint4*>(cells[warp])[e * 32 + lane];
-            __syncwarp();
+            for (int e = i * 32 + lane; e < cell_bytes(D) / 16; e += 32 * GROUPS)
+                reinterpret_cast<uint4*>(cell)[e] = reinterpret_cast<const uint4*>(shared_cell)[e];
+            meet();
         }
     }
 }
@@ -1583,31 +1615,32 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
 // us, cells 4.6; 12 thousand in 5 sequences: rows 100, cells 21.)
 bool by_cells(const CacheRows& r) { return r.rows >= 8 * (uint64_t)r.count; }
 
-unsigned cell_blocks(const CacheView& c, const CacheRows& r) {
-    return (unsigned)(((uint64_t)(r.rows + kCellTokens - 1) / kCellTokens * c.kv_heads + kCellWarps - 1) / kCellWarps);
+unsigned cell_blocks(const CacheView& c, const CacheRows& r, unsigned units) {
+    return (unsigned)(((uint64_t)(r.rows + kCellTokens - 1) / kCellTokens * c.kv_heads + units - 1) / units);
 }
 
 template <typename T>
 cudaError_t launch_append(cudaStream_t s, const T* k, const T* v, size_t k_row, size_t k_head, size_t v_row, size_t v_head,
                           bool wide, const CacheView& c, const CacheRows& r) {
-    const auto cells = [&](auto kernel) {
-        return launch_dependent(kernel, dim3(cell_blocks(c, r)), 32 * kCellWarps, 0, s, k, v, k_row, k_head, v_row, v_head, wide, c, r);
+    const auto cells = [&](auto kernel, unsigned groups, unsigned units) {
+        return launch_dependent(kernel, dim3(cell_blocks(c, r, units)), 32 * groups * units, 0, s, k, v, k_row, k_head, v_row, v_head,
+                                wide, c, r);
     };
     if (!by_cells(r))
         return launch_dependent(append_rows_kernel<T>, dim3((unsigned)(((uint64_t)r.rows * c.kv_heads * 2 + 3) / 4)), 128, 0, s, k, v,
                                 k_row, k_head, v_row, v_head, c, r);
     switch (c.dim / kCacheGroup) {
-    case 1: return cells(append_cells_kernel<T, 1>);
-    case 2: return cells(append_cells_kernel<T, 2>);
-    case 3: return cells(append_cells_kernel<T, 3>);
-    default: return cells(append_cells_kernel<T, 4>);
+    case 1: return cells(append_cells_kernel<T, 1>, 1, kAppendUnits<1>);
+    case 2: return cells(append_cells_kernel<T, 2>, 2, kAppendUnits<2>);
+    case 3: return cells(append_cells_kernel<T, 3>, 3, kAppendUnits<3>);
+    default: return cells(append_cells_kernel<T, 4>, 4, kAppendUnits<4>);
     }
 }
 
 template <typename T>
 cudaError_t launch_read(cudaStream_t s, T* k, T* v, const CacheView& c, const CacheRows& r) {
     const auto cells = [&](auto kernel) {
-        return launch_dependent(kernel, dim3(cell_blocks(c, r)), 32 * kCellWarps, 0, s, c, r, k, v);
+        return launch_dependent(kernel, dim3(cell_blocks(c, r, kCellWarps)), 32 * kCellWarps, 0, s, c, r, k, v);
     };
     if (!by_cells(r))
         return launch_dependent(read_rows_kernel<T>, dim3((unsigned)(((uint64_t)r.rows * c.kv_heads * 2 + 3) / 4)), 128, 0, s, c, r, k, v);
@@ -1661,7 +1694,13 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     call.tails = static_cast<int4*>(workspace);
     call.shares = reinterpret_cast<int*>(call.tails + blocks);
     call.parts = reinterpret_cast<float*>(call.shares + blocks);
-    cudaError_t status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+    static std::atomic<uint64_t> allowed{0};  // devices that know the kernel's shared memory
+    int device = 0;
+    cudaError_t status = cudaGetDevice(&device);
+    if (status == cudaSuccess && (device >= 64 || !(allowed.load(std::memory_order_acquire) >> device & 1))) {
+        status = cudaFuncSetAttribute((const void*)kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::kShared);
+        if (status == cudaSuccess && device < 64) allowed.fetch_or(1ull << device, std::memory_order_release);
+    }
     if (status != cudaSuccess) return status;
     status = launch_dependent(kernel, dim3(blocks), kAttentionThreads, Shape::kShared, s, c, r, call);
     if (status != cudaSuccess) return status;
