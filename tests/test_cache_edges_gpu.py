@@ -1,0 +1,207 @@
+"""The paged cache as programs run it: captured and replayed, on other streams, from two threads, twice at
+once, with pages far into a large pool, and twice with the same answer."""
+import threading
+
+import numpy as np
+import pytest
+import torch
+
+import cache_reference as ref
+from laplacesscissors_b200 import cache
+from test_cache_gpu import check, make, queries, tensor
+
+pytestmark = pytest.mark.gpu
+
+
+def filled(gpu, seed, lengths, heads=2, D=64, layers=1, page_size=16, longest=1024):
+    """A PagedCache whose sequences hold random keys and values."""
+    held = cache.PagedCache(gpu, layers=layers, pages=sum(-(-n // page_size) for n in lengths) + 20, kv_heads=heads, head_dim=D,
+                            sequences=len(lengths), longest=longest, page_size=page_size)
+    assert int(held.reserve(tensor(range(len(lengths))), tensor(lengths))) == 0
+    starts = tensor(np.concatenate([[0], np.cumsum(lengths)]))
+    for layer in range(layers):
+        held.append(layer, *(queries(seed + i, sum(lengths), heads, D, torch.bfloat16) for i in (2 * layer, 2 * layer + 1)), starts)
+    return held
+
+
+def reference(held, layer=0):
+    return ref.Reference(held.pool[layer].cpu().numpy(), held.tables.cpu().numpy(), held.lengths.cpu().numpy())
+
+
+class Step:
+    """A decode step of all sequences, captured: reserve, append, attention."""
+
+    def __init__(self, gpu, seed, lengths, D=64):
+        self.held = filled(gpu, seed, lengths, D=D)
+        n = len(lengths)
+        self.names, self.ones = tensor(range(n)), tensor([1] * n)
+        self.k, self.v, self.q = (queries(seed + i, n, h, D, torch.float32) for i, h in ((10, 2), (11, 2), (12, 6)))
+        self.missing = tensor([0])
+        self.out = torch.zeros_like(self.q)
+        self.run()  # once before the capture
+        torch.cuda.synchronize()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph):
+            self.run()
+
+    def run(self):
+        self.held.reserve(self.names, self.ones, missing=self.missing)
+        self.held.append(0, self.k, self.v)
+        self.held.attention(0, self.q, out=self.out)
+
+    def check(self, length_of_first):
+        assert int(self.missing) == 0 and int(self.held.lengths[0]) == length_of_first
+        r = reference(self.held)
+        expected = r.attention(self.q.double().cpu().numpy(), self.q.shape[2] ** -0.5)[0]
+        assert np.allclose(self.out.cpu().numpy(), expected, rtol=1e-4, atol=1e-4)
+
+
+def test_a_captured_step_follows_the_lengths(gpu):
+    s = Step(gpu, 1, [5, 31, 200, 630])
+    length = 6
+    for count in (1, 3, 12):
+        for i in range(count):
+            s.k.normal_()
+            s.v.normal_()
+            s.q.normal_()
+            s.graph.replay()
+        length += count
+        torch.cuda.synchronize()
+        s.check(length)
+
+
+def test_two_captured_steps_at_once(gpu):
+    steps = [Step(gpu, 2, [700, 31, 650]), Step(gpu, 3, [5, 800, 90, 13], D=128)]
+    streams = [torch.cuda.Stream() for _ in steps]
+    torch.cuda.synchronize()
+    for _ in range(8):
+        for s, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                s.graph.replay()
+    torch.cuda.synchronize()
+    for s, first in zip(steps, (709, 14)):
+        s.check(first)
+
+
+def test_two_streams_and_two_threads(gpu):
+    caches = [filled(gpu, 20 + i, [900, 3, 400 + i]) for i in range(2)]
+    expected = [reference(c).attention(queries(30 + i, 3, 4, 64, torch.float32).double().cpu().numpy(), 0.125)[0]
+                for i, c in enumerate(caches)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        q = queries(30 + i, 3, 4, 64, torch.float32)
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.default_stream())
+        with torch.cuda.stream(stream):
+            for _ in range(30):
+                got = caches[i].attention(0, q)
+                stream.synchronize()
+                if not np.allclose(got.cpu().numpy(), expected[i], rtol=1e-4, atol=1e-4):
+                    wrong.append(i)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_the_same_call_repeats_its_bits(gpu, dtype):
+    held, _ = make(40, [3000, 17, 900, 2500], heads=2, D=128, size=64)
+    q = queries(41, 4, 8, 128, dtype)
+    first = cache.attention(gpu, q, *held)
+    for _ in range(10):
+        assert torch.equal(cache.attention(gpu, q, *held), first)
+
+
+def test_calls_follow_the_current_stream(gpu):
+    held, r = make(42, [200, 64], D=64)
+    q = queries(43, 2, 4, 64, torch.float32)
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(20_000_000)
+        moved = q * 2
+        got = cache.attention(gpu, moved, *held)
+        back = got + 0
+    stream.synchronize()
+    expected = r.attention((q * 2).double().cpu().numpy(), 0.125)[0]
+    assert np.allclose(back.cpu().numpy(), expected, rtol=1e-4, atol=1e-4)
+
+
+def test_tensors_that_a_call_writes_count_as_modified(gpu):
+    held = filled(gpu, 44, [20, 30])
+    x = queries(45, 2, 2, 64, torch.float32)
+    before = held.pool._version
+    held.append(0, x, x)
+    assert held.pool._version > before
+    out = torch.zeros(2, 2, 64, device="cuda")
+    before = out._version
+    held.attention(0, x, out=out)
+    assert out._version > before
+
+
+def test_pages_far_into_a_large_pool(gpu):
+    """Bytes past 2^32 from the pool's start, in its second layer too."""
+    heads, D, size, count = 8, 128, 64, 60000  # 4.4 GB a layer
+    pool = torch.empty((2, *cache.pages_shape(count, heads, size, D)), dtype=torch.uint8, device="cuda")
+    tables = tensor([[count - 1, 3, count - 2, -1], [count - 7, count - 30, -1, -1], [-1] * 4])
+    lengths = tensor([150, 100, 0])
+    refs = torch.zeros(count, dtype=torch.int32, device="cuda")
+    refs[tables[tables >= 0].long()] = 1
+    refs[:40000] = 1
+    starts = tensor([0, 150, 250])
+    k, v = (queries(50 + i, 250, heads, D, torch.bfloat16) for i in range(2))
+    for layer in range(2):
+        cache.append(gpu, k + layer, v, pool[layer], tables, lengths, starts)
+    missing = cache.fork(gpu, pool, tables, lengths, refs, tensor([0]), tensor([2]), size)
+    assert int(missing) == 0 and tables[2].tolist() == [count - 1, 3, 40000, -1]
+    for layer in range(2):
+        for rows, at in ((150, 0), (100, 1), (150, 2)):
+            got = cache.read(gpu, pool[layer], tables, lengths, tensor([0, rows]), sequences=tensor([at]), rows=rows)
+            first = 150 if at == 1 else 0
+            expected = ref.dequantise(*ref.quantise((k + layer)[first:first + rows].float().cpu().numpy()))
+            assert np.allclose(got[0].cpu().numpy(), expected, rtol=2.0 ** -23, atol=0)
+        small = [1, 3, count - 1, count - 2, count - 7, count - 30, 40000]
+        pages = pool[layer][small].cpu().numpy()
+        index = {p: i for i, p in enumerate(small)}
+        local = np.array([[index.get(p, -1) for p in row] for row in tables.tolist()], np.int32)
+        r = ref.Reference(pages, local, lengths.cpu().numpy())
+        check(gpu, (pool[layer], tables, lengths), r, queries(60, 3, 16, D, torch.bfloat16))
+    kept = [pool[layer, 40000].clone() for layer in range(2)]
+    refs[:39000] = 0
+    refs[3] = 1
+    got = cache.compact(gpu, pool, tables, refs)
+    live = int((refs > 0).sum())
+    assert int(got.tables.max()) < live and int((got.refs > 0).sum()) == live and not got.refs[live:].any()
+    for layer in range(2):
+        assert torch.equal(pool[layer, int(got.tables[2, 2])], kept[layer])
+
+
+@pytest.mark.parametrize("rows,sequences", [(1, 1), (1, 300), (2000, 300), (129, 128)])
+def test_many_sequences(gpu, rows, sequences):
+    """More sequences than threads look them up, most without rows."""
+    rng = np.random.default_rng(rows)
+    lengths = rng.integers(0, 40, sequences).tolist()
+    held, r = make(70, lengths, heads=1, D=64, size=16)
+    cuts = np.sort(rng.integers(0, rows + 1, sequences - 1))
+    starts = np.concatenate([[0], cuts, [rows]])
+    check(gpu, held, r, queries(71, rows, 2, 64, torch.float32), starts)
+    k, v = (queries(72 + i, rows, 1, 64, torch.float16) for i in range(2))
+    cache.append(gpu, k, v, *held, tensor(starts))
+    r.append(k.float().cpu().numpy(), v.float().cpu().numpy(), starts)
+    assert np.array_equal(held[0].cpu().numpy(), r.pages)
+
+
+def test_sequences_that_share_pages(gpu):
+    held = cache.PagedCache(gpu, layers=1, pages=30, kv_heads=2, head_dim=64, sequences=6, longest=200, page_size=16)
+    assert int(held.reserve(tensor([0]), tensor([90]))) == 0
+    kv = [queries(81 + i, 90, 2, 64, torch.float32) for i in range(2)]
+    held.append(0, *kv, tensor([0, 90]), tensor([0]))
+    assert int(held.fork(tensor([0] * 5), tensor([1, 2, 3, 4, 5]))) == 0
+    r = reference(held)
+    check(gpu, (held.pool[0], held.tables, held.lengths), r, queries(83, 6, 4, 64, torch.float32))
+    starts = [0, 20, 25, 45, 46, 46, 60]
+    check(gpu, (held.pool[0], held.tables, held.lengths), r, queries(84, 60, 4, 64, torch.bfloat16), starts)
