@@ -220,6 +220,12 @@ int lsx_model_score(lsx_model* model, const uint32_t* prompt, size_t prompt_leng
    touch the model's own cursor or cache. */
 int lsx_model_generate_batch(lsx_model* model, const uint32_t* prompts, size_t batch, size_t prompt_length,
                              size_t maximum, uint32_t* tokens_out);
+/* The same with the sequences' caches held in `cache_bits` bits an element: 32, f32 as above, or
+   4, pages as lsx_cache_append_device keeps them (a seventh of the memory, and of what each step
+   reads of it).  The prompts' own attention takes their keys and values before rounding; the
+   steps, from the last prompt token on, take what the cache holds. */
+int lsx_model_generate_batch_cache(lsx_model* model, const uint32_t* prompts, size_t batch, size_t prompt_length,
+                                   size_t maximum, size_t cache_bits, uint32_t* tokens_out);
 /* lsx_model_score over `cases` independent cases of equal shape at once (the
    per-case loop of scaling::evaluate, src/scaling.rs:181-216, batched): prompts
    [cases x prompt_length], targets [cases x count].  Per scored position:

@@ -114,6 +114,7 @@ SIGNATURES = {
     "lsx_model_generate": (I, [P, UP, SZ, SZ, UP, SZ, P, UP, C.POINTER(SZ), C.POINTER(I), FP, FP]),
     "lsx_model_score": (I, [P, UP, SZ, UP, SZ, P, DP, UP, FP, FP]),
     "lsx_model_generate_batch": (I, [P, UP, SZ, SZ, SZ, UP]),
+    "lsx_model_generate_batch_cache": (I, [P, UP, SZ, SZ, SZ, SZ, UP]),
     "lsx_model_score_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, DP, UP, DP, FP]),
     "lsx_model_distribution_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, D, SZ, FP, FP, FP, UP, FP, FP]),
     "lsx_model_divergence_batch": (I, [P, UP, SZ, SZ, UP, SZ, P, D, UP, FP, SZ, FP, FP]),

@@ -1282,7 +1282,76 @@ static bool launch_cached_attention(cudaStream_t s, const float* qkv, const floa
                         splits, hi, lo) == cudaSuccess;
 }
 
-int BatchedScorer::generate_batch(const uint32_t* prompts, size_t batch, size_t P, size_t maximum,
+// f32 rows as the next GEMM's two bf16 terms.
+__global__ void __launch_bounds__(256) split_planes_kernel(const float* x, size_t n, __nv_bfloat16* hi, __nv_bfloat16* lo) {
+    pdl_launch_dependents();
+    pdl_wait();
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) {
+        const __nv_bfloat16 h = __float2bfloat16_rn(x[i]);
+        hi[i] = h;
+        lo[i] = __float2bfloat16_rn(x[i] - __bfloat162float(h));
+    }
+}
+
+// The paged caches, empty, in the allocation that the f32 caches use otherwise.
+int BatchedScorer::open_paged(size_t batch, size_t P, size_t maximum, Paged* paged, uint32_t** history) {
+    const FusedConfig& c = config_;
+    constexpr size_t kPage = 64;
+    const size_t width = (P + maximum + kPage - 1) / kPage, pages = batch * width;
+    size_t total = 0;
+    const auto room = [&](size_t bytes) {
+        const size_t at = total;
+        total += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    paged->layer_bytes = pages * lsx_cache_page_bytes(c.kvheads, kPage, c.head_dim);
+    paged->workspace_bytes = lsx_cache_attention_workspace_bytes(ctx_, c.head_dim);
+    const size_t pool = room(paged->layer_bytes * layers_.size()), tables = room(pages * 4), lengths = room(batch * 4),
+                 refs = room(pages * 4), lists = room((4 * batch + 2) * 4), out = room(batch * c.qheads * c.head_dim * 4),
+                 workspace = room(paged->workspace_bytes), tokens = room(maximum * batch * 4);
+    cudaStream_t s = ctx_->stream;
+    LSX_CUDA(cudaStreamSynchronize(s), "batched generation");
+    if (total > batch_cache_bytes_) {
+        if (batch_cache_) cudaFree(batch_cache_);
+        batch_cache_ = nullptr;
+        batch_cache_bytes_ = 0;
+        LSX_CUDA(cudaMalloc(&batch_cache_, total), "batched generation caches");
+        batch_cache_bytes_ = total;
+    }
+    uint8_t* base = (uint8_t*)batch_cache_;
+    paged->tables = (int32_t*)(base + tables);
+    paged->lengths = (int32_t*)(base + lengths);
+    paged->refs = (int32_t*)(base + refs);
+    paged->names = (int32_t*)(base + lists);
+    paged->prompt_counts = paged->names + batch;
+    paged->step_counts = paged->prompt_counts + batch;
+    paged->starts = paged->step_counts + batch;
+    paged->missing = paged->starts + batch + 1;
+    paged->out = (float*)(base + out);
+    paged->workspace = base + workspace;
+    *history = (uint32_t*)(base + tokens);
+    paged->view = lsx_cache_view{base + pool, pages, kPage, (size_t)c.kvheads, (size_t)c.head_dim, paged->tables, batch, width,
+                                 paged->lengths};
+    paged->prompt = lsx_cache_rows{batch * (P - 1), batch, nullptr, paged->starts};
+    paged->step = lsx_cache_rows{batch, batch, nullptr, nullptr};
+    std::vector<int32_t> lists_host(4 * batch + 2, 0);
+    for (size_t b = 0; b < batch; ++b) {
+        lists_host[b] = (int32_t)b;
+        lists_host[batch + b] = (int32_t)(P - 1);
+        lists_host[2 * batch + b] = 1;
+        lists_host[3 * batch + b] = (int32_t)(b * (P - 1));
+    }
+    lists_host[4 * batch] = (int32_t)(batch * (P - 1));
+    LSX_CUDA(cudaMemcpyAsync(paged->names, lists_host.data(), lists_host.size() * 4, cudaMemcpyHostToDevice, s), "cache lists");
+    LSX_CUDA(cudaMemsetAsync(paged->tables, 0xff, pages * 4, s), "cache tables");
+    LSX_CUDA(cudaMemsetAsync(paged->lengths, 0, batch * 4, s), "cache lengths");
+    LSX_CUDA(cudaMemsetAsync(paged->refs, 0, pages * 4, s), "cache counts");
+    LSX_CUDA(cudaStreamSynchronize(s), "cache lists");  // the host's lists go out of scope
+    return lsx_cache_reserve_device(ctx_, paged->tables, batch, width, paged->lengths, paged->refs, pages, kPage, paged->names,
+                                    paged->prompt_counts, batch, paged->missing, nullptr);
+}
+
+int BatchedScorer::generate_batch(const uint32_t* prompts, size_t batch, size_t P, size_t maximum, int cache_bits,
                                   uint32_t* tokens_out) {
     const FusedConfig& c = config_;
     LSX_ENSURE(prompts && tokens_out && batch > 0 && batch <= 1024 && P >= 2 && maximum > 0,
@@ -1290,7 +1359,9 @@ int BatchedScorer::generate_batch(const uint32_t* prompts, size_t batch, size_t 
     for (size_t i = 0; i < batch * P; ++i) LSX_ENSURE(prompts[i] < (uint32_t)c.vocab, "check the prompt token range");
     const int H = c.hidden, D = c.head_dim, QH = c.qheads, KVH = c.kvheads, I = c.intermediate, V = c.vocab;
     const int R = QH / KVH, dpl = D / 32;
-    LSX_ENSURE(R == 1 || R == 2 || (R == 4 && dpl <= 4), "batched generation: unsupported group ratio");
+    const bool paged_cache = cache_bits == 4;
+    LSX_ENSURE(cache_bits == 4 || cache_bits == 32, "the caches hold 4 or 32 bits an element");
+    LSX_ENSURE(paged_cache || R == 1 || R == 2 || (R == 4 && dpl <= 4), "batched generation: unsupported group ratio");
     const size_t cap = P + maximum, kw = (size_t)KVH * D, B = batch;
     // per layer: keys, then values, each [batch][kvheads][capacity][head_dim]
     const size_t case_stride = cap * kw, layer_stride = 2 * B * case_stride;
@@ -1301,26 +1372,35 @@ int BatchedScorer::generate_batch(const uint32_t* prompts, size_t batch, size_t 
     const size_t part_floats = B * QH * (size_t)splits * (D + 2);
     const size_t need = (layer_stride * layers_.size() + part_floats) * 4 + maximum * B * 4 + 256;
     cudaStream_t s = ctx_->stream;
-    LSX_CUDA(cudaStreamSynchronize(s), "batched generation");
-    if (need > batch_cache_bytes_) {
-        if (batch_cache_) cudaFree(batch_cache_);
-        batch_cache_ = nullptr;
-        batch_cache_bytes_ = 0;
-        LSX_CUDA(cudaMalloc(&batch_cache_, need), "batched generation caches");
-        batch_cache_bytes_ = need;
+    Paged paged;
+    float* part = nullptr;
+    uint32_t* history = nullptr;
+    if (paged_cache) {
+        LSX_TRY(open_paged(B, P, maximum, &paged, &history));
+    } else {
+        LSX_CUDA(cudaStreamSynchronize(s), "batched generation");
+        if (need > batch_cache_bytes_) {
+            if (batch_cache_) cudaFree(batch_cache_);
+            batch_cache_ = nullptr;
+            batch_cache_bytes_ = 0;
+            LSX_CUDA(cudaMalloc(&batch_cache_, need), "batched generation caches");
+            batch_cache_bytes_ = need;
+        }
+        part = batch_cache_ + layer_stride * layers_.size();
+        history = (uint32_t*)(part + part_floats);
     }
-    float* part = batch_cache_ + layer_stride * layers_.size();
-    uint32_t* history = (uint32_t*)(part + part_floats);
 
     // the prompts less their last token: one batched forward into the sequences' caches
     std::vector<uint32_t> head_tokens(B * (P - 1));
     for (size_t b = 0; b < B; ++b)
         for (size_t t = 0; t + 1 < P; ++t) head_tokens[b * (P - 1) + t] = prompts[b * P + t];
-    batch_keys_ = batch_cache_;
+    batch_keys_ = paged_cache ? nullptr : batch_cache_;
+    batch_paged_ = paged_cache ? &paged : nullptr;
     batch_case_stride_ = case_stride;
     batch_layer_stride_ = layer_stride;
     const int rc = run(head_tokens.data(), B, P - 1, 0, 0, nullptr, nullptr, Outputs{}, true);
     batch_keys_ = nullptr;
+    batch_paged_ = nullptr;
     LSX_TRY(rc);
 
     // decode: one row per sequence and step, the whole loop on the device
@@ -1358,17 +1438,34 @@ int BatchedScorer::generate_batch(const uint32_t* prompts, size_t batch, size_t 
         LSX_CUDA(chain_launch(embed_rows_kernel, dim3(M), dim3(256), 0, s, c.embedding, c.embedding_kind,
                               c.embedding_scale, (const uint32_t*)d_tokens, H, x),
                  "embedding rows");
+        if (paged_cache)
+            LSX_TRY(lsx_cache_reserve_device(ctx_, paged.tables, B, paged.view.table_width, paged.lengths, paged.refs,
+                                             paged.view.page_count, paged.view.page_size, paged.names, paged.step_counts, B,
+                                             paged.missing, nullptr));
         for (size_t li = 0; li < layers_.size(); ++li) {
             const FusedLayer& Ly = layers_[li];
-            float* bk = batch_cache_ + li * layer_stride;
-            float* bv = bk + layer_stride / 2;
+            float* bk = paged_cache ? nullptr : batch_cache_ + li * layer_stride;
+            float* bv = paged_cache ? nullptr : bk + layer_stride / 2;
             LSX_CUDA(chain_launch(rms_planes_kernel, dim3(M), dim3(256), 0, s, (const float*)x, (const int*)nullptr, H,
                                   Ly.input_gain, c.eps, hi, lo, (float*)nullptr),
                      "batched decode norm");
             LSX_TRY(gemm_planes_enqueue(ctx_, hi, lo, M, H, Ly.wqkv, qkvw, Ly.bqkv, work, qkvw, false, status));
             const float2* rp = rope + (size_t)pos * half;
             bool ok;
-            if (D == 128) {
+            if (paged_cache) {
+                const auto roped = D == 128 ? qk_rope_kernel<4> : D == 64 ? qk_rope_kernel<2> : qk_rope_kernel<8>;
+                LSX_CUDA(chain_launch(roped, dim3(qk_blocks), dim3(256), 0, s, work, M, 1, QH, KVH, Ly.q_gain, Ly.k_gain, c.qk_eps,
+                                      rp),
+                         "batched decode rope");
+                const lsx_cache_view view = paged.layer(li);
+                LSX_TRY(lsx_cache_append_device(ctx_, &view, &paged.step, work + QH * D, work + (QH + KVH) * D, LSX_F32, qkvw, D,
+                                                qkvw, D, nullptr));
+                LSX_TRY(lsx_cache_attention_device(ctx_, &view, &paged.step, work, LSX_F32, QH, qkvw, D, c.scale, paged.out,
+                                                   (size_t)QH * D, D, paged.workspace, paged.workspace_bytes, nullptr));
+                const size_t n = B * QH * D;
+                ok = chain_launch(split_planes_kernel, dim3((unsigned)std::min<size_t>((n + 255) / 256, 148 * 8)), dim3(256), 0, s,
+                                  (const float*)paged.out, n, hi, lo) == cudaSuccess;
+            } else if (D == 128) {
                 LSX_CUDA(chain_launch(qk_rope_kernel<4>, dim3(qk_blocks), dim3(256), 0, s, work, M, 1, QH, KVH,
                                       Ly.q_gain, Ly.k_gain, c.qk_eps, rp),
                          "batched decode rope");
@@ -1567,7 +1664,11 @@ int BatchedScorer::run(const uint32_t* tokens, size_t cases, size_t T, size_t fi
         LSX_CUDA(cudaGetLastError(), "attention");
         if (write_cache) {
             const size_t kv = (size_t)M * KVH * D;
-            if (batch_keys_) {  // per-sequence caches of generate_batch
+            if (batch_paged_) {
+                const lsx_cache_view view = batch_paged_->layer(li);
+                LSX_TRY(lsx_cache_append_device(ctx_, &view, &batch_paged_->prompt, work + QH * D, work + (QH + KVH) * D, LSX_F32,
+                                                qkvw, D, qkvw, D, nullptr));
+            } else if (batch_keys_) {  // per-sequence caches of generate_batch
                 float* bk = batch_keys_ + li * batch_layer_stride_;
                 float* bv = bk + batch_layer_stride_ / 2;
                 kv_store_kernel<<<(int)std::min<size_t>((kv + 255) / 256, 148 * 16), 256, 0, s>>>(

@@ -54,9 +54,27 @@ public:
     // the first P - 1 prompt tokens of every sequence in one batched forward into
     // per-sequence KV caches, then one row per sequence per step through the GEMMs and
     // an attention over each sequence's own cache; tokens_out [batch, maximum] (host).
-    int generate_batch(const uint32_t* prompts, size_t batch, size_t P, size_t maximum, uint32_t* tokens_out);
+    // With cache_bits 4 the caches are pages held in 4 bits (cache.cu), else f32.
+    int generate_batch(const uint32_t* prompts, size_t batch, size_t P, size_t maximum, int cache_bits,
+                       uint32_t* tokens_out);
 
 private:
+    // Paged caches of generate_batch in 4 bits, in one allocation with what their calls take.
+    struct Paged {
+        lsx_cache_view view{};  // of the first layer
+        lsx_cache_rows prompt{}, step{};
+        size_t layer_bytes = 0, workspace_bytes = 0;
+        int32_t *tables = nullptr, *lengths = nullptr, *refs = nullptr, *names = nullptr, *starts = nullptr,
+                *prompt_counts = nullptr, *step_counts = nullptr, *missing = nullptr;
+        float* out = nullptr;  // [batch, query heads * head_dim]
+        void* workspace = nullptr;
+        lsx_cache_view layer(size_t l) const {
+            lsx_cache_view v = view;
+            v.pages = (uint8_t*)v.pages + l * layer_bytes;
+            return v;
+        }
+    };
+    int open_paged(size_t batch, size_t P, size_t maximum, Paged* paged, uint32_t** history);
     struct Layout {
         size_t x, work, planes, logits, rope, tokens, targets, rows, nll, argmax, margin, status, total;
     };
@@ -69,6 +87,7 @@ private:
     float* batch_cache_ = nullptr;
     size_t batch_cache_bytes_ = 0;
     float* batch_keys_ = nullptr;
+    const Paged* batch_paged_ = nullptr;  // run() appends the prefill rows here while it is set
     size_t batch_case_stride_ = 0, batch_layer_stride_ = 0;
     lsx_ctx* ctx_ = nullptr;
     FusedConfig config_{};

@@ -1559,6 +1559,11 @@ int lsx_model_score(lsx_model* m, const uint32_t* prompt, size_t prompt_length, 
 // the last go through the decoder together, one tensor-core GEMM per projection.
 int lsx_model_generate_batch(lsx_model* m, const uint32_t* prompts, size_t batch, size_t prompt_length,
                              size_t maximum, uint32_t* tokens_out) {
+    return lsx_model_generate_batch_cache(m, prompts, batch, prompt_length, maximum, 32, tokens_out);
+}
+
+int lsx_model_generate_batch_cache(lsx_model* m, const uint32_t* prompts, size_t batch, size_t prompt_length,
+                                   size_t maximum, size_t cache_bits, uint32_t* tokens_out) {
     LSX_ENSURE(m && prompts && tokens_out, "invalid argument");
     LSX_ENSURE(batch > 0 && prompt_length >= 2 && maximum > 0,
                "give at least one sequence, two prompt tokens and one generated token");
@@ -1566,7 +1571,8 @@ int lsx_model_generate_batch(lsx_model* m, const uint32_t* prompts, size_t batch
     if (!m->fused) return fail(LSX_E_UNSUPPORTED, "batched generation needs the fused weight layout");
     cudaSetDevice(m->ctx->device);
     LSX_TRY(ensure_batched(m));
-    return m->batched->generate_batch(prompts, batch, prompt_length, maximum, tokens_out);
+    LSX_ENSURE(cache_bits == 4 || cache_bits == 32, "the caches hold 4 or 32 bits an element");
+    return m->batched->generate_batch(prompts, batch, prompt_length, maximum, (int)cache_bits, tokens_out);
 }
 
 static int score_batch(lsx_model* m, const uint32_t* prompts, size_t cases, size_t prompt_length,

@@ -199,12 +199,14 @@ class Model:
         check(lib.lsx_model_head_image(self._h, _dp(v), _fp(out)))
         return out
 
-    def generate_batch(self, prompts, maximum: int) -> np.ndarray:
+    def generate_batch(self, prompts, maximum: int, cache_bits: int = 32) -> np.ndarray:
         """Greedy generation of several equal-length prompts at once
-        (lsx_model_generate_batch): prompts [batch, P] -> tokens [batch, maximum]."""
+        (lsx_model_generate_batch): prompts [batch, P] -> tokens [batch, maximum].  With
+        cache_bits=4 the sequences' keys and values are held in 4 bits
+        (lsx_model_generate_batch_cache)."""
         p = np.ascontiguousarray(np.atleast_2d(prompts), dtype=np.uint32)
         out = np.empty((p.shape[0], int(maximum)), dtype=np.uint32)
-        check(lib.lsx_model_generate_batch(self._h, _up(p), p.shape[0], p.shape[1], int(maximum), _up(out)))
+        check(lib.lsx_model_generate_batch_cache(self._h, _up(p), p.shape[0], p.shape[1], int(maximum), int(cache_bits), _up(out)))
         return out
 
     def head_images(self, gpu: Gpu, vectors) -> np.ndarray:
