@@ -519,6 +519,30 @@ __device__ __forceinline__ void mma_f16_first(float (&c)[4], const uint32_t (&a)
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
+// Two f32 in one register pair, for the instructions that take both: the values of rows 2 j and 2 j + 1.
+struct Two {
+    unsigned long long bits;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(bits) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ explicit Two(float a) : Two(a, a) {}
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(bits)); }
+};
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits), "l"(c.bits));
+    return d;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+    return d;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
+    return d;
+}
+
 __device__ __forceinline__ uint32_t pack_f16(float low, float high) {
     const __half2 h = __floats2half2_rn(low, high);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -827,7 +851,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 
         // ---- queries as the products' columns: the thread's rows of the results are 2 j and 2 j + 1 of each eight
         uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][LOW ? 4 : 2];
-        float factor[NT][2], plain[NT][2][GROUPS];
+        float factor[NT][2];
+        Two plain[NT][GROUPS];
         int limit[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -881,13 +906,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             if constexpr (LOW) query[f][2] = l0, query[f][3] = l1;
                         }
                     }
-                plain[t][0][g] = ones[0];
-                plain[t][1][g] = ones[1];
+                plain[t][g] = Two(ones[0], ones[1]);
             }
         }
         if constexpr (Shape::kSharedQuery) __syncthreads();
 
-        float out[NT][4 * GROUPS][4], reference[NT][2], sum[NT][2], zeros[NT][2][GROUPS];
+        float out[NT][4 * GROUPS][4], reference[NT][2], sum[NT][2];
+        Two zeros[NT][GROUPS];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
@@ -898,9 +923,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             for (int i = 0; i < 2; ++i) {
                 reference[t][i] = kNone;
                 sum[t][i] = 0.f;
-#pragma unroll
-                for (int g = 0; g < GROUPS; ++g) zeros[t][i][g] = 0.f;
             }
+#pragma unroll
+            for (int g = 0; g < GROUPS; ++g) zeros[t][g] = Two(0.f);
         }
 
         const uint32_t pick = quad & 1 ? 0x7632u : 0x5410u;  // a thread's position among two: its step and zero
@@ -955,7 +980,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             }
                 }
             // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
-            float score[U][NT][4];
+            Two score[U][NT][2];  // of position, of position + 8
             __half2 values[U][GROUPS][2];
 #pragma unroll
             for (int u = 0; u < U; ++u)
@@ -968,9 +993,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float z0 = sz0.y * plain[n][i][g], z1 = sz1.y * plain[n][i][g];
-                            score[u][n][i] = fmaf(sz0.x, dot[u][g][n][i], g ? score[u][n][i] + z0 : z0);
-                            score[u][n][2 + i] = fmaf(sz1.x, dot[u][g][n][2 + i], g ? score[u][n][2 + i] + z1 : z1);
+                            const float2 sz = i ? sz1 : sz0;
+                            const float (&d)[4] = dot[u][g][n];
+                            const Two zero = g ? fma(Two(sz.y), plain[n][g], score[u][n][i]) : Two(sz.y) * plain[n][g];
+                            score[u][n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
                         }
                     const uint4 more = *reinterpret_cast<const uint4*>(steps_of + cell_value_steps(D));
                     uint32_t sz[2] = {__byte_perm(more.x, more.y, pick), __byte_perm(more.z, more.w, pick)};
@@ -988,7 +1014,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        weight[u][n][i] = exp2_approx(fmaf(score[u][n][i], factor[n][i % 2], -reference[n][i % 2]));
+                        if (i % 2 == 0) {
+                            const Two against(-reference[n][0], -reference[n][1]);
+                            fma(score[u][n][i / 2], Two(factor[n][0], factor[n][1]), against).get(weight[u][n][i], weight[u][n][i + 1]);
+                        }
+                        weight[u][n][i] = exp2_approx(weight[u][n][i]);
                         if (EDGE && blind(u, i / 2, n, i % 2)) weight[u][n][i] = 0.f;
                         most = fmaxf(most, weight[u][n][i]);
                     }
@@ -1004,16 +1034,21 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float top = -INFINITY;
+                        float mine[2 * U];
 #pragma unroll
-                        for (int m = 0; m < 2 * U; ++m)
-                            if (!EDGE || !blind(m / 2, m % 2, n, i)) top = fmaxf(top, score[m / 2][n][m % 2 * 2 + i] * factor[n][i]);
+                        for (int m = 0; m < 2 * U; ++m) {
+                            float rows[2];
+                            score[m / 2][n][m % 2].get(rows[0], rows[1]);
+                            mine[m] = rows[i];
+                            if (!EDGE || !blind(m / 2, m % 2, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
+                        }
                         top = across_max(top);
                         const float next = fmaxf(reference[n][i], top + above - 10.f);
                         const float keep = exp2_approx(reference[n][i] - next);
                         reference[n][i] = next;
                         sum[n][i] *= keep;
 #pragma unroll
-                        for (int g = 0; g < GROUPS; ++g) zeros[n][i][g] *= keep;
+                        for (int g = 0; g < GROUPS; ++g) zeros[n][g] = zeros[n][g] * (i ? Two(1.f, keep) : Two(keep, 1.f));
 #pragma unroll
                         for (int m = 0; m < 4 * GROUPS; ++m) {
                             out[n][m][i] *= keep;
@@ -1022,7 +1057,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                         for (int m = 0; m < 2 * U; ++m) {
                             float& w = weight[m / 2][n][m % 2 * 2 + i];
-                            w = exp2_approx(fmaf(score[m / 2][n][m % 2 * 2 + i], factor[n][i], -next));
+                            w = exp2_approx(fmaf(mine[m], factor[n][i], -next));
                             if (EDGE && blind(m / 2, m % 2, n, i)) w = 0.f;
                         }
                     }
@@ -1046,11 +1081,17 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     for (int n = 0; n < NT; ++n) {
                         float x[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            x[i] = weight[u][n][i] * sz[i / 2].x;
-                            // a position that this row does not see adds nothing, whatever it holds
-                            if (EDGE && blind(u, i / 2, n, i % 2)) x[i] = 0.f;
-                            else zeros[n][i % 2][g] = fmaf(weight[u][n][i], sz[i / 2].y, zeros[n][i % 2][g]);
+                        for (int i = 0; i < 2; ++i) {
+                            const Two w(weight[u][n][2 * i], weight[u][n][2 * i + 1]);
+                            (w * Two(sz[i].x)).get(x[2 * i], x[2 * i + 1]);
+                            if (EDGE) {  // a position that a row does not see adds nothing, whatever it holds
+                                const bool skip[2] = {blind(u, i, n, 0), blind(u, i, n, 1)};
+                                if (skip[0]) x[2 * i] = 0.f;
+                                if (skip[1]) x[2 * i + 1] = 0.f;
+                                zeros[n][g] = fma(w, Two(skip[0] ? 0.f : sz[i].y, skip[1] ? 0.f : sz[i].y), zeros[n][g]);
+                            } else {
+                                zeros[n][g] = fma(w, Two(sz[i].y), zeros[n][g]);
+                            }
                         }
                         p0[n] = pack_f16(x[0], x[1]);
                         p1[n] = pack_f16(x[2], x[3]);
@@ -1132,7 +1173,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 if (quad == 0) row[D] = reference[t][i], row[D + 1] = l;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const float z = across_sum(zeros[t][i][g]);
+                    float of_rows[2];
+                    zeros[t][g].get(of_rows[0], of_rows[1]);
+                    const float z = across_sum(of_rows[i]);
 #pragma unroll
                     for (int m = 4 * g; m < 4 * g + 4; ++m) {
                         row[16 * m + quad] = fmaf(out[t][m][i], 0x1p24f, z);
