@@ -210,11 +210,14 @@ def _pool(device: int, pool: torch.Tensor):
     """(lsx_cache_pool, pages)."""
     if not (isinstance(pool, _Tensor) and pool.dim() >= 3 and pool.get_device() == device and pool.numel()):
         raise ValueError("the pool must be a [layers, pages, ...] tensor on the Gpu's device")
-    layer = pool[0]
-    stride, elements, pages, width = pool.stride(0), layer.numel(), pool.size(1), pool.element_size()
-    if not layer.is_contiguous() or (pool.size(0) > 1 and stride < elements):
-        raise ValueError("a layer's pages must be contiguous, and layers must not overlap")
-    return _POOL(pool.data_ptr(), pool.size(0), stride * width, elements // pages * width, pages), pages
+    layers, pages, width = pool.size(0), pool.size(1), pool.element_size()
+    elements = pool.numel() // layers
+    stride = elements
+    if not pool.is_contiguous():
+        stride = pool.stride(0)
+        if not pool[0].is_contiguous() or (layers > 1 and stride < elements):
+            raise ValueError("a layer's pages must be contiguous, and layers must not overlap")
+    return _POOL(pool.data_ptr(), layers, stride * width, elements // pages * width, pages), pages
 
 
 def _state(device: int, tables, lengths, refs):
