@@ -203,8 +203,8 @@ def _shape(case):
             n = rng.randint(min(length, case["queries"] // 2), n)
         lengths.append(length)
         queries.append(n)
-    if not case["ragged"] and case["sequences"] > 8 and case["spread"]:
-        lengths[3] = 0  # a sequence that holds nothing yet
+    if case["op"] == "attention" and not case["ragged"] and case["sequences"] > 8 and case["spread"]:
+        lengths[3] = 0  # a sequence that holds nothing yet (one that is appended to holds its rows)
     return lengths, queries
 
 
