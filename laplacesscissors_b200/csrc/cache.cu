@@ -1695,8 +1695,7 @@ cudaError_t launch_read(cudaStream_t s, T* k, T* v, const CacheView& c, const Ca
     }
 }
 
-// Blocks of attention_kernel on the card, and its workspace: the blocks' tails and two
-// parts each.
+// attention_kernel's workspace: two parts of a tile a block that the card holds, and what the block starts.
 template <int GROUPS, int NT, bool LOW>
 size_t attention_bytes(int sm_count) {
     using Shape = AttentionShape<GROUPS, NT, LOW>;
@@ -1755,14 +1754,17 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
                             32 * kMergeWarps, blocks * 4, s, call, Shape::kRows, (int)most, (int)blocks);
 }
 
-// Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where
-// the sums of 32 rows fit the registers.
+// Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where the sums of 32 fit
+// the registers.  The time goes by the rows of the tiles, used or not, and little by how many a tile has
+// (12 sequences of 6001 positions, bf16, 8 x 128: 20 rows 75 us in tiles of 16 and 74 of 32, 48 rows 102 and 127, two
+// parts of prompts 1116 and 1069), so tiles of 32 are taken where they leave few more rows unused.
 template <typename T, int GROUPS>
 cudaError_t launch_attention(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r,
                              const AttentionCall& call, void* workspace) {
     const uint64_t rows = (uint64_t)((r.rows + r.count - 1) / r.count) * call.group;
     if constexpr (GROUPS <= 2 && !std::is_same<T, float>::value)
-        if (rows > 16) return launch_tiles<T, GROUPS, 4>(sm_count, s, c, r, call, workspace);
+        if (rows > 16 && ((rows + 31) / 32 * 32 - (rows + 15) / 16 * 16) * 25 <= rows)
+            return launch_tiles<T, GROUPS, 4>(sm_count, s, c, r, call, workspace);
     if (rows > 8) return launch_tiles<T, GROUPS, 2>(sm_count, s, c, r, call, workspace);
     return launch_tiles<T, GROUPS, 1>(sm_count, s, c, r, call, workspace);
 }
