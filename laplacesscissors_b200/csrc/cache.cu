@@ -414,7 +414,11 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // holds f16 and bf16 queries exactly down to 2^-38 of the row's largest element, or for f32
 // (LOW) as f16 high and low parts of 22 bits.  A weight p is taken against a reference that
 // keeps p s below 2^15, and p s is held the same two ways: 11 bits are half a step of an
-// f16 result, twice 11 those of f32.  Everything else is f32.  The reference of a row moves
+// f16 result, twice 11 those of f32.  Everything else is f32.  The sum of p s n and that of p z
+// are often large beside what is left of them, and the tensor cores cut what they add to a sum:
+// f32 calls take n - 8 and z + 8 s instead, whose sums are as small as the result (16 x 4113
+// positions: 4.5e-7 of the result's size off, 1.8e-5 without; with the keys' as they lie 1.0e-6,
+// and 35.4 us instead of 37.1).  The reference of a row moves
 // up where p s would pass 2^15, to leave 2^10 for the largest: what is 2^24 below
 // that still has 11 bits, and steady sequences hardly ever move it.
 //
@@ -445,14 +449,15 @@ struct AttentionShape {
     // registers a thread: the sums and the queries, beside some 75 for the rest; where those are not left the
     // queries go to shared memory
     static constexpr int kLoad = NT * GROUPS, kHeld = (LOW ? 32 : 24) * kLoad;
-    static constexpr int kBlocksPerSm = kHeld <= 64 ? 4 : kHeld <= 96 ? 3 : 2;
-    static constexpr bool kSharedQuery = kHeld > (kBlocksPerSm == 4 ? 53 : kBlocksPerSm == 3 ? 96 : 180);
+    static constexpr int kBlocksPerSm = kHeld <= 48 ? 4 : kHeld <= 96 ? 3 : 2;
+    static constexpr bool kSharedQuery = kHeld > 180;
     static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW ? 16 : 8) : 0;
     static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
     static constexpr int kAtOnce = NT == 1 && GROUPS <= 2 ? 2 : 1;  // cells whose weights a thread holds at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
     static constexpr int kParts = kAttentionWarps * kRows * kPart * 4;  // the warps' sums, in the ring's memory
+    static constexpr int kAside = kAttentionWarps * NT * (4 * GROUPS + 1) * 32;  // sums put aside, four floats each
     static constexpr int kBars = kAttentionWarps * kStages * 8;
     static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + kBars;
     static_assert(kStages >= 2 && kBlocksPerSm * (kShared + 1200) <= 228 * 1024, "shared memory");
@@ -470,7 +475,8 @@ struct AttentionCall {
     bool whole;                // tiles are not shared
     int* shares;               // [blocks] parts of the tile that a block starts and others finish, 0 where there is none
     int4* tails;               // [blocks] that tile's first row, key head, part of it, and positions
-    float* parts;              // [2 blocks][rows][part_row(dim)]
+    float* parts;              // [2 blocks][used][part_row(dim)]
+    float4* aside;             // [warps][rows / 8][dim / 16 + 1][32]: sums that a thread puts aside
 };
 
 // A call's pairs in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
@@ -574,6 +580,20 @@ __device__ __forceinline__ float across_max(float x) {
     x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
     return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
 }
+// Two levels of a word as f16, those in bits 0-3 (ODD: 4-7) of its halves: times 2^-24 (2^-20) as subnormals, or
+// CENTRED: less 8, from 1024 + n (64 + n), whose last bits the level fills.
+template <bool ODD, bool CENTRED>
+__device__ __forceinline__ uint32_t levels_f16(uint32_t word) {
+    const uint32_t bits = word & (ODD ? 0x00f000f0u : 0x000f000fu);
+    if constexpr (!CENTRED) {
+        return bits;
+    } else {
+        uint32_t x;
+        asm("add.f16x2 %0, %1, %2;" : "=r"(x) : "r"(bits | (ODD ? 0x54005400u : 0x64006400u)), "r"(ODD ? 0xd480d480u : 0xe408e408u));
+        return x;
+    }
+}
+
 // An 8 x 8 matrix of f16, two neighbours of row lane / 4 a thread, transposed.
 __device__ __forceinline__ uint32_t transpose_f16(uint32_t x) {
     uint32_t y;
@@ -865,13 +885,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             const bool fine = top < 0x7f800000u;
             // 2^power takes the largest into 2^13 .. 2^14
             const int power = fine && top ? 13 - max((int)(top >> 23) - 127, -100) : 0;
-            const float up = fine ? pow2(power) : 0.f, of_row = fine ? call.scale * pow2(12 - power) * 0x1p12f : nan;
+            const float up = fine ? pow2(power) : 0.f, of_row = fine ? call.scale * pow2(LOW ? -power : 12 - power) * (LOW ? 1.f : 0x1p12f) : nan;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 factor[t][i] = __shfl_sync(0xffffffffu, of_row, (2 * j + i) * 4);
                 limit[t][i] = __shfl_sync(0xffffffffu, sees[t], (2 * j + i) * 4);
             }
-            // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6, the odd ones' levels 16 times as large
+            // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6; as subnormals the odd ones' levels are 16 times as large
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
                 float ones[4];  // the levels' factor of the zeros: the sum of the queries, with all levels 1
@@ -879,11 +899,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int w = 0; w < 2; ++w)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const float by = e ? up * 0.0625f : up;
+                        const float by = e && !LOW ? up * 0.0625f : up;
                         const auto value = [&](int i) { return fine ? raw[t][g].value(8 * w + e + i) * by : 0.f; };
                         const float y0 = value(0), y4 = value(4), y2 = value(2), y6 = value(6);
                         const int f = (t * GROUPS + g) * 4 + w * 2 + e;
-                        const uint32_t one = e ? 0x00100010u : 0x00010001u, a[4] = {one, one, one, one};
+                        const uint32_t one = LOW ? 0x3c003c00u : e ? 0x00100010u : 0x00010001u, a[4] = {one, one, one, one};
                         uint32_t x0 = pack_f16(y0, y4), x1 = pack_f16(y2, y6), l0 = 0, l1 = 0;
                         if (w + e == 0)
                             mma_f16_first(ones, a, x0, x1);
@@ -953,7 +973,6 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             for (int w = 0; w < 2; ++w)
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    const uint32_t mask = e ? 0x00f000f0u : 0x000f000fu;
 #pragma unroll
                     for (int half = 0; half < (LOW ? 2 : 1); ++half)
 #pragma unroll
@@ -961,7 +980,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                             for (int g = 0; g < GROUPS; ++g) {
                                 const uint32_t low = w ? words[u][g].y : words[u][g].x, high = w ? words[u][g].w : words[u][g].z;
-                                const uint32_t a[4] = {low & mask, high & mask, low >> 8 & mask, high >> 8 & mask};
+                                const uint32_t a[4] = {e ? levels_f16<true, LOW>(low) : levels_f16<false, LOW>(low),
+                                                       e ? levels_f16<true, LOW>(high) : levels_f16<false, LOW>(high),
+                                                       e ? levels_f16<true, LOW>(low >> 8) : levels_f16<false, LOW>(low >> 8),
+                                                       e ? levels_f16<true, LOW>(high >> 8) : levels_f16<false, LOW>(high >> 8)};
 #pragma unroll
                                 for (int n = 0; n < NT; ++n) {
                                     const int f = (n * GROUPS + g) * 4 + w * 2 + e;
@@ -993,7 +1015,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const float2 sz = i ? sz1 : sz0;
+                            float2 sz = i ? sz1 : sz0;
+                            if (LOW) sz.y = fmaf(8.f, sz.x, sz.y);  // s (n - 8) + (z + 8 s)
                             const float (&d)[4] = dot[u][g][n];
                             const Two zero = g ? fma(Two(sz.y), plain[n][g], score[u][n][i]) : Two(sz.y) * plain[n][g];
                             score[u][n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
@@ -1075,7 +1098,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 const uint8_t* cell = held + u * Shape::kCell;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    const float2 sz[2] = {__half22float2(values[u][g][0]), __half22float2(values[u][g][1])};
+                    float2 sz[2] = {__half22float2(values[u][g][0]), __half22float2(values[u][g][1])};
+                    if (LOW) sz[0].y = fmaf(8.f, sz[0].x, sz[0].y), sz[1].y = fmaf(8.f, sz[1].x, sz[1].y);
                     uint32_t p0[NT], p1[NT], l0[NT], l1[NT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
@@ -1109,12 +1133,42 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     for (int half = 0; half < (LOW ? 2 : 1); ++half)
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
-                            const uint32_t a[4] = {word[w] & 0x000f000fu, word[w] & 0x00f000f0u, word[w] >> 8 & 0x000f000fu,
-                                                   word[w] >> 8 & 0x00f000f0u};
+                            const uint32_t a[4] = {levels_f16<false, LOW>(word[w]), levels_f16<true, LOW>(word[w]),
+                                                   levels_f16<false, LOW>(word[w] >> 8), levels_f16<true, LOW>(word[w] >> 8)};
 #pragma unroll
                             for (int n = 0; n < NT; ++n) mma_f16(out[n][g * 4 + w], a, half ? l0[n] : p0[n], half ? l1[n] : p1[n]);
                         }
                 }
+            }
+        };
+
+        // The tensor cores cut what they add to a sum, half a unit of its last place a time, so that long sums drift.
+        // They are put aside in the workspace, a thread's own, and go on from 0; at the end (!away) they are added.
+        constexpr int kPutAside = LOW ? 32 : 128;  // pairs: 2^-24 x 2 x 64, or 2^-24 x 256, of the sum
+        const auto put_aside = [&](bool more, bool away) {  // more: something was put aside before
+            float4* mine = call.aside + ((size_t)blockIdx.x * kAttentionWarps + warp) * (NT * (4 * GROUPS + 1) * 32) + lane;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float4* of = mine + t * (4 * GROUPS + 1) * 32;
+                float keep[2] = {0.f, 0.f};
+                if (more) {  // the references that it was taken against
+                    const float4 against = of[4 * GROUPS * 32];
+                    keep[0] = exp2_approx(against.x - reference[t][0]), keep[1] = exp2_approx(against.y - reference[t][1]);
+                }
+#pragma unroll
+                for (int m = 0; m < 4 * GROUPS; ++m) {
+                    float(&x)[4] = out[t][m];
+                    if (more) {
+                        const float4 y = of[m * 32];
+                        x[0] = fmaf(y.x, keep[0], x[0]), x[1] = fmaf(y.y, keep[1], x[1]);
+                        x[2] = fmaf(y.z, keep[0], x[2]), x[3] = fmaf(y.w, keep[1], x[3]);
+                    }
+                    if (away) {
+                        of[m * 32] = make_float4(x[0], x[1], x[2], x[3]);
+                        x[0] = x[1] = x[2] = x[3] = 0.f;
+                    }
+                }
+                if (away) of[4 * GROUPS * 32] = make_float4(reference[t][0], reference[t][1], 0.f, 0.f);
             }
         };
 
@@ -1153,6 +1207,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int u = 0; u < 2; u += Shape::kAtOnce)
                     take(std::false_type{}, held + u * Shape::kCell, pair * kPairTokens + u * kCellTokens, 0);
             }
+            if ((n + 1) % kPutAside == 0 || (n + 1 == mine_pairs && mine_pairs > kPutAside)) put_aside(n >= kPutAside, n + 1 < mine_pairs);
         }
         // rows that see positions which no table entry covers, or whose sequence has no table
 #pragma unroll
@@ -1178,8 +1233,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     const float z = across_sum(of_rows[i]);
 #pragma unroll
                     for (int m = 4 * g; m < 4 * g + 4; ++m) {
-                        row[16 * m + quad] = fmaf(out[t][m][i], 0x1p24f, z);
-                        row[16 * m + 8 + quad] = fmaf(out[t][m][2 + i], 0x1p20f, z);
+                        row[16 * m + quad] = fmaf(out[t][m][i], LOW ? 1.f : 0x1p24f, z);
+                        row[16 * m + 8 + quad] = fmaf(out[t][m][2 + i], LOW ? 1.f : 0x1p20f, z);
                     }
                 }
             }
@@ -1699,7 +1754,7 @@ cudaError_t launch_read(cudaStream_t s, T* k, T* v, const CacheView& c, const Ca
 template <int GROUPS, int NT, bool LOW>
 size_t attention_bytes(int sm_count) {
     using Shape = AttentionShape<GROUPS, NT, LOW>;
-    return (size_t)sm_count * Shape::kBlocksPerSm * (20 + 2 * Shape::kRows * Shape::kPart * 4);
+    return (size_t)sm_count * Shape::kBlocksPerSm * (20 + 2 * Shape::kRows * Shape::kPart * 4 + Shape::kAside * 16);
 }
 
 template <int GROUPS>
@@ -1734,8 +1789,9 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
     // left out (one sequence of 9 positions: 8.3 us with it, 5.9 without).
     call.whole = (uint64_t)c.table_width * c.page_size <= kWholeTokens;
     call.tails = static_cast<int4*>(workspace);
-    call.shares = reinterpret_cast<int*>(call.tails + blocks);
-    call.parts = reinterpret_cast<float*>(call.shares + blocks);
+    call.aside = reinterpret_cast<float4*>(call.tails + blocks);
+    call.parts = reinterpret_cast<float*>(call.aside + (size_t)blocks * Shape::kAside);
+    call.shares = reinterpret_cast<int*>(call.parts + (size_t)blocks * 2 * Shape::kRows * Shape::kPart);
     static std::atomic<uint64_t> allowed{0};  // devices that know the kernel's shared memory
     int device = 0;
     cudaError_t status = cudaGetDevice(&device);

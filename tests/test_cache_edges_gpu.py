@@ -205,3 +205,38 @@ def test_sequences_that_share_pages(gpu):
     check(gpu, (held.pool[0], held.tables, held.lengths), r, queries(83, 6, 4, 64, torch.float32))
     starts = [0, 20, 25, 45, 46, 46, 60]
     check(gpu, (held.pool[0], held.tables, held.lengths), r, queries(84, 60, 4, 64, torch.bfloat16), starts)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_long_runs_do_not_drift(gpu, dtype):
+    """More positions than fit a sum on the tensor cores, for every warp: 32 sequences of some 40 thousand, whose
+    tables name the same pages again and again."""
+    heads, D, size, n = 8, 64, 64, 32
+    held, r = make(90, [64 * 200], heads=heads, D=D, size=size, spare=0)
+    rng = np.random.default_rng(91)
+    lengths = rng.integers(39000, 41000, n)
+    tables = rng.integers(0, 200, (n, 641)).astype(np.int32)
+    q = queries(92, n, 2 * heads, D, dtype, 0.3)  # weights of one size, so that all positions count
+    got = cache.attention(gpu, q, held[0], tensor(tables), tensor(lengths)).double()
+    order = held[1][0].cpu().numpy()
+    k, v, k_wide, v_wide = (torch.from_numpy(a).cuda() for a in r.values(0, 64 * 200))
+    place = np.empty(200, np.int64)
+    place[order[:200]] = np.arange(200)
+    for b in range(0, n, 3):
+        at = np.arange(lengths[b])
+        at = torch.from_numpy(place[tables[b][at // size]] * size + at % size).cuda()
+        z = torch.einsum("hgd,thd->hgt", q[b].double().view(heads, 2, D), k[at]) / 8
+        p = torch.softmax(z, 2)
+        expected = torch.einsum("hgt,thd->hgd", p, v[at]).reshape(2 * heads, D)
+        wide = torch.einsum("hgt,thd->hgd", p, v_wide[at]).reshape(2 * heads, D)
+        bound = torch.einsum("hgd,thd->hgt", q[b].double().abs().view(heads, 2, D), k_wide[at]).amax(2).reshape(-1, 1) / 8
+        # scores as in test_cache_gpu.tolerance; the sums are put aside after 64 (f16, bf16: 256) steps, which cut up to
+        # 2^-23 of the sum each, and meet in f32
+        weight = 2 * torch.expm1((D / 8 + 16) * 2.0 ** -22 * bound) + 2.0 ** -20
+        steps = (2 * 64 if dtype is torch.float32 else 256) * 2.0 ** -23
+        single = 0 if dtype is torch.float32 else 2.0 ** -11
+        allowed = (weight + steps + 64 * 2.0 ** -24 + single) * wide + torch.finfo(dtype).eps / 2 * expected.abs()
+        error = (got[b] - expected).abs()
+        assert (error <= allowed).all(), float((error - allowed).max())
+        if dtype is torch.float32:
+            assert float(error.norm() / expected.norm()) < 1e-5
