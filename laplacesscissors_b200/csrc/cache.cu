@@ -449,12 +449,12 @@ struct AttentionShape {
     // registers a thread: the sums and the queries, beside some 75 for the rest; where those are not left the
     // queries go to shared memory
     static constexpr int kLoad = NT * GROUPS, kHeld = (LOW ? 32 : 24) * kLoad;
-    static constexpr int kBlocksPerSm = kHeld <= 48 ? 4 : kHeld <= 96 ? 3 : 2;
+    static constexpr int kBlocksPerSm = kHeld <= 48 ? 4 : kHeld <= 96 && (NT == 1 || LOW) ? 3 : 2;
     static constexpr bool kSharedQuery = kHeld > 180;
     static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW ? 16 : 8) : 0;
     static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
-    static constexpr int kAtOnce = NT == 1 && GROUPS <= 2 ? 2 : 1;  // cells whose weights a thread holds at the same time
+    static constexpr int kAtOnce = GROUPS <= 2 && (NT == 1 || !LOW) ? 2 : 1;  // cells whose products are under way at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
     static constexpr int kParts = kAttentionWarps * kRows * kPart * 4;  // the warps' sums, in the ring's memory
     static constexpr int kAside = kAttentionWarps * NT * (4 * GROUPS + 1) * 32;  // sums put aside, four floats each
@@ -1001,11 +1001,12 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                                 }
                             }
                 }
-            // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
-            Two score[U][NT][2];  // of position, of position + 8
-            __half2 values[U][GROUPS][2];
+            // then cell by cell, while the products of the next one are under way
 #pragma unroll
-            for (int u = 0; u < U; ++u)
+            for (int u = 0; u < U; ++u) {
+            // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
+            Two score[NT][2];  // of position, of position + 8
+            __half2 values[GROUPS][2];
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     const uint8_t* steps_of = held + u * Shape::kCell + g * 64 + quad / 2 * 16;
@@ -1018,36 +1019,34 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             float2 sz = i ? sz1 : sz0;
                             if (LOW) sz.y = fmaf(8.f, sz.x, sz.y);  // s (n - 8) + (z + 8 s)
                             const float (&d)[4] = dot[u][g][n];
-                            const Two zero = g ? fma(Two(sz.y), plain[n][g], score[u][n][i]) : Two(sz.y) * plain[n][g];
-                            score[u][n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
+                            const Two zero = g ? fma(Two(sz.y), plain[n][g], score[n][i]) : Two(sz.y) * plain[n][g];
+                            score[n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
                         }
                     const uint4 more = *reinterpret_cast<const uint4*>(steps_of + cell_value_steps(D));
                     uint32_t sz[2] = {__byte_perm(more.x, more.y, pick), __byte_perm(more.z, more.w, pick)};
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (EDGE && !there(u, i)) sz[i] = 0;  // what no row sees may hold anything
-                        values[u][g][i] = *reinterpret_cast<__half2*>(&sz[i]);
+                        values[g][i] = *reinterpret_cast<__half2*>(&sz[i]);
                     }
                 }
             // weights
-            float weight[U][NT][4], most = 0.f;
-#pragma unroll
-            for (int u = 0; u < U; ++u)
+            float weight[NT][4], most = 0.f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (i % 2 == 0) {
                             const Two against(-reference[n][0], -reference[n][1]);
-                            fma(score[u][n][i / 2], Two(factor[n][0], factor[n][1]), against).get(weight[u][n][i], weight[u][n][i + 1]);
+                            fma(score[n][i / 2], Two(factor[n][0], factor[n][1]), against).get(weight[n][i], weight[n][i + 1]);
                         }
-                        weight[u][n][i] = exp2_approx(weight[u][n][i]);
-                        if (EDGE && blind(u, i / 2, n, i % 2)) weight[u][n][i] = 0.f;
-                        most = fmaxf(most, weight[u][n][i]);
+                        weight[n][i] = exp2_approx(weight[n][i]);
+                        if (EDGE && blind(u, i / 2, n, i % 2)) weight[n][i] = 0.f;
+                        most = fmaxf(most, weight[n][i]);
                     }
-            __half2 steps = values[0][0][0];
+            __half2 steps = values[0][0];
 #pragma unroll
-            for (int i = 1; i < 2 * U * GROUPS; ++i) steps = __hmax2(steps, values[i / (2 * GROUPS)][i / 2 % GROUPS][i % 2]);
+            for (int i = 1; i < 2 * GROUPS; ++i) steps = __hmax2(steps, values[i / 2][i % 2]);
             const float largest = fmaxf(__low2float(steps), 0x1p-30f);
             if (__any_sync(0xffffffffu, !(most * largest < 0x1p15f))) {
                 const float all = quad_max(across_max(largest));
@@ -1057,13 +1056,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float top = -INFINITY;
-                        float mine[2 * U];
+                        float mine[2];
 #pragma unroll
-                        for (int m = 0; m < 2 * U; ++m) {
+                        for (int m = 0; m < 2; ++m) {
                             float rows[2];
-                            score[m / 2][n][m % 2].get(rows[0], rows[1]);
+                            score[n][m].get(rows[0], rows[1]);
                             mine[m] = rows[i];
-                            if (!EDGE || !blind(m / 2, m % 2, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
+                            if (!EDGE || !blind(u, m, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
                         }
                         top = across_max(top);
                         const float next = fmaxf(reference[n][i], top + above - 10.f);
@@ -1078,27 +1077,21 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             out[n][m][2 + i] *= keep;
                         }
 #pragma unroll
-                        for (int m = 0; m < 2 * U; ++m) {
-                            float& w = weight[m / 2][n][m % 2 * 2 + i];
+                        for (int m = 0; m < 2; ++m) {
+                            float& w = weight[n][2 * m + i];
                             w = exp2_approx(fmaf(mine[m], factor[n][i], -next));
-                            if (EDGE && blind(m / 2, m % 2, n, i)) w = 0.f;
+                            if (EDGE && blind(u, m, n, i)) w = 0.f;
                         }
                     }
             }
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float more = weight[0][n][i] + weight[0][n][2 + i];
-                    if (U == 2) more += weight[U - 1][n][i] + weight[U - 1][n][2 + i];
-                    sum[n][i] += more;
-                }
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
+                for (int i = 0; i < 2; ++i) sum[n][i] += weight[n][i] + weight[n][2 + i];
                 const uint8_t* cell = held + u * Shape::kCell;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
-                    float2 sz[2] = {__half22float2(values[u][g][0]), __half22float2(values[u][g][1])};
+                    float2 sz[2] = {__half22float2(values[g][0]), __half22float2(values[g][1])};
                     if (LOW) sz[0].y = fmaf(8.f, sz[0].x, sz[0].y), sz[1].y = fmaf(8.f, sz[1].x, sz[1].y);
                     uint32_t p0[NT], p1[NT], l0[NT], l1[NT];
 #pragma unroll
@@ -1106,7 +1099,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         float x[4];
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            const Two w(weight[u][n][2 * i], weight[u][n][2 * i + 1]);
+                            const Two w(weight[n][2 * i], weight[n][2 * i + 1]);
                             (w * Two(sz[i].x)).get(x[2 * i], x[2 * i + 1]);
                             if (EDGE) {  // a position that a row does not see adds nothing, whatever it holds
                                 const bool skip[2] = {blind(u, i, n, 0), blind(u, i, n, 1)};
@@ -1759,10 +1752,8 @@ size_t attention_bytes(int sm_count) {
 
 template <int GROUPS>
 size_t attention_bytes(int sm_count) {
-    constexpr int kMost = GROUPS <= 2 ? 4 : 2;
     return std::max({attention_bytes<GROUPS, 1, false>(sm_count), attention_bytes<GROUPS, 2, false>(sm_count),
-                     attention_bytes<GROUPS, kMost, false>(sm_count), attention_bytes<GROUPS, 1, true>(sm_count),
-                     attention_bytes<GROUPS, 2, true>(sm_count)});
+                     attention_bytes<GROUPS, 1, true>(sm_count), attention_bytes<GROUPS, 2, true>(sm_count)});
 }
 
 size_t attention_workspace(int sm_count, size_t dim) {
@@ -1810,17 +1801,13 @@ cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const
                             32 * kMergeWarps, blocks * 4, s, call, Shape::kRows, (int)most, (int)blocks);
 }
 
-// Rows of a tile by the rows that a sequence and key head has on average: 8, 16, or 32 where the sums of 32 fit
-// the registers.  The time goes by the rows of the tiles, used or not, and little by how many a tile has
-// (12 sequences of 6001 positions, bf16, 8 x 128: 20 rows 75 us in tiles of 16 and 74 of 32, 48 rows 102 and 127, two
-// parts of prompts 1116 and 1069), so tiles of 32 are taken where they leave few more rows unused.
+// Rows of a tile by the rows that a sequence and key head has on average.  The time goes by the tiles' rows, used or
+// not (12 sequences of 6001 positions, bf16, 8 x 128, 20 rows: 75 us in tiles of 16 and 112 of 64; parts of prompts 1089 us in
+// tiles of 16, 1421 of 8), and a step of eight rows or fewer by what it reads.
 template <typename T, int GROUPS>
 cudaError_t launch_attention(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r,
                              const AttentionCall& call, void* workspace) {
     const uint64_t rows = (uint64_t)((r.rows + r.count - 1) / r.count) * call.group;
-    if constexpr (GROUPS <= 2 && !std::is_same<T, float>::value)
-        if (rows > 16 && ((rows + 31) / 32 * 32 - (rows + 15) / 16 * 16) * 25 <= rows)
-            return launch_tiles<T, GROUPS, 4>(sm_count, s, c, r, call, workspace);
     if (rows > 8) return launch_tiles<T, GROUPS, 2>(sm_count, s, c, r, call, workspace);
     return launch_tiles<T, GROUPS, 1>(sm_count, s, c, r, call, workspace);
 }
