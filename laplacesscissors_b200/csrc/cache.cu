@@ -417,10 +417,13 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // f16 result, twice 11 those of f32.  Everything else is f32.  The sum of p s n and that of p z
 // are often large beside what is left of them, and the tensor cores cut what they add to a sum:
 // f32 calls take n - 8 and z + 8 s instead, whose sums are as small as the result (16 x 4113
-// positions: 4.5e-7 of the result's size off, 1.8e-5 without; with the keys' as they lie 1.0e-6,
-// and 35.4 us instead of 37.1).  The reference of a row moves
-// up where p s would pass 2^15, to leave 2^10 for the largest: what is 2^24 below
-// that still has 11 bits, and steady sequences hardly ever move it.
+// positions: 4.5e-7 of the result's size off, 1.8e-5 without; 37.1 us, 32.2 without).  The
+// reference of a row moves up where p s would pass 2^15, to leave 2^10 for the largest: what is
+// 2^24 below that still has 11 bits, and steady sequences hardly ever move it.
+//
+// The low parts of f32 are products of their own.  Where a tile has four rows at most (HALF) they
+// take the columns that would be left unused, four further on, and the halves are added by one
+// exchange: half the products (16 x 4113 positions: 34.5 us instead of 37.1).
 //
 // Work.  The pairs of cells (32 positions of one head) that the rows of a call see, in the
 // order of sequence, head, tile of rows and position, are cut into equal runs, one a block;
@@ -443,15 +446,17 @@ constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 // Floats of a row's part: its sums, its reference and the sum of its weights.
 constexpr int part_row(int dim) { return dim + 2; }
 
-template <int GROUPS, int NT, bool LOW>
+// GROUPS: of 64 elements; NT: eights of a tile's rows; LOW: f32; HALF: four rows, the low parts beside them.
+template <int GROUPS, int NT, bool LOW, bool HALF>
 struct AttentionShape {
-    static constexpr int kDim = 64 * GROUPS, kPart = part_row(kDim), kRows = 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
+    static constexpr int kDim = 64 * GROUPS, kPart = part_row(kDim), kRows = HALF ? 4 : 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
     // registers a thread: the sums and the queries, beside some 75 for the rest; where those are not left the
-    // queries go to shared memory
-    static constexpr int kLoad = NT * GROUPS, kHeld = (LOW ? 32 : 24) * kLoad;
-    static constexpr int kBlocksPerSm = kHeld <= 48 ? 4 : kHeld <= 96 && (NT == 1 || LOW) ? 3 : 2;
+    // queries go to shared memory.  Blocks of an SM, measured in us (three, four): one row of 128, 131072 positions,
+    // 39.3 and 42.7; parts of prompts in heads of 64 526 and 440; in heads of 128, three 1083 and two 1089.
+    static constexpr int kLoad = NT * GROUPS, kHeld = (LOW && !HALF ? 32 : 24) * kLoad;
+    static constexpr int kBlocksPerSm = kHeld <= 24 || (NT == 2 && kHeld <= 48) ? 4 : kHeld <= 96 && (NT == 1 || LOW) ? 3 : 2;
     static constexpr bool kSharedQuery = kHeld > 180;
-    static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW ? 16 : 8) : 0;
+    static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW && !HALF ? 16 : 8) : 0;
     static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
     static constexpr int kAtOnce = GROUPS <= 2 && (NT == 1 || !LOW) ? 2 : 1;  // cells whose products are under way at the same time
@@ -668,10 +673,12 @@ struct TilePart {
     int table;         // row of the tables, -1 for none
 };
 
-template <typename T, int GROUPS, int NT, bool LOW>
-__global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT, LOW>::kBlocksPerSm))
+template <typename T, int GROUPS, int NT, bool LOW, bool HALF>
+__global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT, LOW, HALF>::kBlocksPerSm))
     attention_kernel(CacheView c, CacheRows r, AttentionCall call) {
-    using Shape = AttentionShape<GROUPS, NT, LOW>;
+    using Shape = AttentionShape<GROUPS, NT, LOW, HALF>;
+    constexpr bool BOTH = LOW && !HALF;  // low parts by products of their own
+    static_assert(!HALF || (LOW && NT == 1), "four rows");
     constexpr int D = Shape::kDim, kStages = Shape::kStages;
     constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
     extern __shared__ __align__(128) uint8_t shared[];
@@ -805,7 +812,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
             int token, h;
-            const bool row = place(8 * t + quad, token, h);
+            const bool row = place(HALF ? quad % 4 : 8 * t + quad, token, h);
             sees[t] = row ? least + token : 0;
             const T* x = static_cast<const T*>(call.q) + (size_t)(part.row + token) * call.q_row +
                          (size_t)(head * (int)call.group + h) * call.q_head + 16 * j;
@@ -870,7 +877,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         for (int n = 0; n < kStages - 1; ++n) issue();
 
         // ---- queries as the products' columns: the thread's rows of the results are 2 j and 2 j + 1 of each eight
-        uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][LOW ? 4 : 2];
+        uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][BOTH ? 4 : 2];
         float factor[NT][2];
         Two plain[NT][GROUPS];
         int limit[NT][2];
@@ -888,8 +895,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             const float up = fine ? pow2(power) : 0.f, of_row = fine ? call.scale * pow2(LOW ? -power : 12 - power) * (LOW ? 1.f : 0x1p12f) : nan;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                factor[t][i] = __shfl_sync(0xffffffffu, of_row, (2 * j + i) * 4);
-                limit[t][i] = __shfl_sync(0xffffffffu, sees[t], (2 * j + i) * 4);
+                const int holder = (HALF ? (2 * j + i) % 4 : 2 * j + i) * 4;
+                factor[t][i] = __shfl_sync(0xffffffffu, of_row, holder);
+                limit[t][i] = __shfl_sync(0xffffffffu, sees[t], holder);
             }
             // word w (8 elements), step e: elements e, e + 4 and e + 2, e + 6; as subnormals the odd ones' levels are 16 times as large
 #pragma unroll
@@ -905,27 +913,30 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         const int f = (t * GROUPS + g) * 4 + w * 2 + e;
                         const uint32_t one = LOW ? 0x3c003c00u : e ? 0x00100010u : 0x00010001u, a[4] = {one, one, one, one};
                         uint32_t x0 = pack_f16(y0, y4), x1 = pack_f16(y2, y6), l0 = 0, l1 = 0;
-                        if (w + e == 0)
-                            mma_f16_first(ones, a, x0, x1);
-                        else
-                            mma_f16(ones, a, x0, x1);
                         if (LOW) {
                             const float2 h0 = unpack_f16(x0), h1 = unpack_f16(x1);
                             l0 = pack_f16(y0 - h0.x, y4 - h0.y);
                             l1 = pack_f16(y2 - h1.x, y6 - h1.y);
-                            mma_f16(ones, a, l0, l1);
                         }
+                        if (HALF && quad >= 4) x0 = l0, x1 = l1;
+                        if (w + e == 0)
+                            mma_f16_first(ones, a, x0, x1);
+                        else
+                            mma_f16(ones, a, x0, x1);
+                        if (BOTH) mma_f16(ones, a, l0, l1);
                         if constexpr (Shape::kSharedQuery) {
                             if (warp == f % kAttentionWarps) {
-                                uint2* at = queries + f * (LOW ? 2 : 1) * 32 + lane;
+                                uint2* at = queries + f * (BOTH ? 2 : 1) * 32 + lane;
                                 at[0] = make_uint2(x0, x1);
-                                if constexpr (LOW) at[32] = make_uint2(l0, l1);
+                                if constexpr (BOTH) at[32] = make_uint2(l0, l1);
                             }
                         } else {
                             query[f][0] = x0, query[f][1] = x1;
-                            if constexpr (LOW) query[f][2] = l0, query[f][3] = l1;
+                            if constexpr (BOTH) query[f][2] = l0, query[f][3] = l1;
                         }
                     }
+                if (HALF)
+                    for (int i = 0; i < 2; ++i) ones[i] += __shfl_xor_sync(0xffffffffu, ones[i], 2);
                 plain[t][g] = Two(ones[0], ones[1]);
             }
         }
@@ -974,7 +985,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
 #pragma unroll
-                    for (int half = 0; half < (LOW ? 2 : 1); ++half)
+                    for (int half = 0; half < (BOTH ? 2 : 1); ++half)
 #pragma unroll
                         for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -989,7 +1000,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                                     const int f = (n * GROUPS + g) * 4 + w * 2 + e;
                                     uint32_t b0, b1;
                                     if constexpr (Shape::kSharedQuery) {
-                                        const uint2 x = queries[(f * (LOW ? 2 : 1) + half) * 32 + lane];
+                                        const uint2 x = queries[(f * (BOTH ? 2 : 1) + half) * 32 + lane];
                                         b0 = x.x, b1 = x.y;
                                     } else {
                                         b0 = query[f][2 * half], b1 = query[f][2 * half + 1];
@@ -1004,9 +1015,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             // then cell by cell, while the products of the next one are under way
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-            // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
-            Two score[NT][2];  // of position, of position + 8
-            __half2 values[GROUPS][2];
+                // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
+                Two score[NT][2];  // of position, of position + 8
+                __half2 values[GROUPS][2];
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     const uint8_t* steps_of = held + u * Shape::kCell + g * 64 + quad / 2 * 16;
@@ -1018,7 +1029,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         for (int i = 0; i < 2; ++i) {
                             float2 sz = i ? sz1 : sz0;
                             if (LOW) sz.y = fmaf(8.f, sz.x, sz.y);  // s (n - 8) + (z + 8 s)
-                            const float (&d)[4] = dot[u][g][n];
+                            float (&d)[4] = dot[u][g][n];
+                            if (HALF) {  // the high and low parts' columns lie four apart
+                                d[2 * i] += __shfl_xor_sync(0xffffffffu, d[2 * i], 2);
+                                d[2 * i + 1] += __shfl_xor_sync(0xffffffffu, d[2 * i + 1], 2);
+                            }
                             const Two zero = g ? fma(Two(sz.y), plain[n][g], score[n][i]) : Two(sz.y) * plain[n][g];
                             score[n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
                         }
@@ -1030,8 +1045,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         values[g][i] = *reinterpret_cast<__half2*>(&sz[i]);
                     }
                 }
-            // weights
-            float weight[NT][4], most = 0.f;
+                // weights
+                float weight[NT][4], most = 0.f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -1044,50 +1059,50 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         if (EDGE && blind(u, i / 2, n, i % 2)) weight[n][i] = 0.f;
                         most = fmaxf(most, weight[n][i]);
                     }
-            __half2 steps = values[0][0];
+                __half2 steps = values[0][0];
 #pragma unroll
-            for (int i = 1; i < 2 * GROUPS; ++i) steps = __hmax2(steps, values[i / 2][i % 2]);
-            const float largest = fmaxf(__low2float(steps), 0x1p-30f);
-            if (__any_sync(0xffffffffu, !(most * largest < 0x1p15f))) {
-                const float all = quad_max(across_max(largest));
-                const float above = (float)(ilogbf(all) + 1);  // 2^above is above these steps
+                for (int i = 1; i < 2 * GROUPS; ++i) steps = __hmax2(steps, values[i / 2][i % 2]);
+                const float largest = fmaxf(__low2float(steps), 0x1p-30f);
+                if (__any_sync(0xffffffffu, !(most * largest < 0x1p15f))) {
+                    const float all = quad_max(across_max(largest));
+                    const float above = (float)(ilogbf(all) + 1);  // 2^above is above these steps
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float top = -INFINITY;
+                            float mine[2];
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                float rows[2];
+                                score[n][m].get(rows[0], rows[1]);
+                                mine[m] = rows[i];
+                                if (!EDGE || !blind(u, m, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
+                            }
+                            top = across_max(top);
+                            const float next = fmaxf(reference[n][i], top + above - 10.f);
+                            const float keep = exp2_approx(reference[n][i] - next);
+                            reference[n][i] = next;
+                            sum[n][i] *= keep;
+#pragma unroll
+                            for (int g = 0; g < GROUPS; ++g) zeros[n][g] = zeros[n][g] * (i ? Two(1.f, keep) : Two(keep, 1.f));
+#pragma unroll
+                            for (int m = 0; m < 4 * GROUPS; ++m) {
+                                out[n][m][i] *= keep;
+                                out[n][m][2 + i] *= keep;
+                            }
+#pragma unroll
+                            for (int m = 0; m < 2; ++m) {
+                                float& w = weight[n][2 * m + i];
+                                w = exp2_approx(fmaf(mine[m], factor[n][i], -next));
+                                if (EDGE && blind(u, m, n, i)) w = 0.f;
+                            }
+                        }
+                }
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float top = -INFINITY;
-                        float mine[2];
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            float rows[2];
-                            score[n][m].get(rows[0], rows[1]);
-                            mine[m] = rows[i];
-                            if (!EDGE || !blind(u, m, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
-                        }
-                        top = across_max(top);
-                        const float next = fmaxf(reference[n][i], top + above - 10.f);
-                        const float keep = exp2_approx(reference[n][i] - next);
-                        reference[n][i] = next;
-                        sum[n][i] *= keep;
-#pragma unroll
-                        for (int g = 0; g < GROUPS; ++g) zeros[n][g] = zeros[n][g] * (i ? Two(1.f, keep) : Two(keep, 1.f));
-#pragma unroll
-                        for (int m = 0; m < 4 * GROUPS; ++m) {
-                            out[n][m][i] *= keep;
-                            out[n][m][2 + i] *= keep;
-                        }
-#pragma unroll
-                        for (int m = 0; m < 2; ++m) {
-                            float& w = weight[n][2 * m + i];
-                            w = exp2_approx(fmaf(mine[m], factor[n][i], -next));
-                            if (EDGE && blind(u, m, n, i)) w = 0.f;
-                        }
-                    }
-            }
-#pragma unroll
-            for (int n = 0; n < NT; ++n)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) sum[n][i] += weight[n][i] + weight[n][2 + i];
+                    for (int i = 0; i < 2; ++i) sum[n][i] += weight[n][i] + weight[n][2 + i];
                 const uint8_t* cell = held + u * Shape::kCell;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
@@ -1114,8 +1129,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         p1[n] = pack_f16(x[2], x[3]);
                         if constexpr (LOW) {
                             const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
-                            l0[n] = transpose_f16(pack_f16(x[0] - a.x, x[1] - a.y));
-                            l1[n] = transpose_f16(pack_f16(x[2] - d.x, x[3] - d.y));
+                            const uint32_t low0 = pack_f16(x[0] - a.x, x[1] - a.y), low1 = pack_f16(x[2] - d.x, x[3] - d.y);
+                            if constexpr (BOTH)
+                                l0[n] = transpose_f16(low0), l1[n] = transpose_f16(low1);
+                            else if (j >= 2)
+                                p0[n] = low0, p1[n] = low1;
                         }
                         p0[n] = transpose_f16(p0[n]);
                         p1[n] = transpose_f16(p1[n]);
@@ -1123,7 +1141,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     const uint4 held_words = *reinterpret_cast<const uint4*>(cell + cell_values(D) + (g * 32 + lane) * 16);
                     const uint32_t word[4] = {held_words.x, held_words.y, held_words.z, held_words.w};
 #pragma unroll
-                    for (int half = 0; half < (LOW ? 2 : 1); ++half)
+                    for (int half = 0; half < (BOTH ? 2 : 1); ++half)
 #pragma unroll
                         for (int w = 0; w < 4; ++w) {
                             const uint32_t a[4] = {levels_f16<false, LOW>(word[w]), levels_f16<true, LOW>(word[w]),
@@ -1216,9 +1234,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         for (int t = 0; t < NT; ++t)
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float* row = mine_sums + (8 * t + 2 * j + i) * Shape::kPart;
+                float* row = mine_sums + (8 * t + (HALF ? (2 * j + i) % 4 : 2 * j + i)) * Shape::kPart;
+                const bool mine = !HALF || j < 2;  // the others hold the same rows
                 const float l = across_sum(sum[t][i]);
-                if (quad == 0) row[D] = reference[t][i], row[D + 1] = l;
+                if (quad == 0 && mine) row[D] = reference[t][i], row[D + 1] = l;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     float of_rows[2];
@@ -1226,8 +1245,14 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     const float z = across_sum(of_rows[i]);
 #pragma unroll
                     for (int m = 4 * g; m < 4 * g + 4; ++m) {
-                        row[16 * m + quad] = fmaf(out[t][m][i], LOW ? 1.f : 0x1p24f, z);
-                        row[16 * m + 8 + quad] = fmaf(out[t][m][2 + i], LOW ? 1.f : 0x1p20f, z);
+                        float x = out[t][m][i], y = out[t][m][2 + i];
+                        if (HALF) {
+                            x += __shfl_xor_sync(0xffffffffu, x, 2);
+                            y += __shfl_xor_sync(0xffffffffu, y, 2);
+                        }
+                        if (!mine) continue;
+                        row[16 * m + quad] = fmaf(x, LOW ? 1.f : 0x1p24f, z);
+                        row[16 * m + 8 + quad] = fmaf(y, LOW ? 1.f : 0x1p20f, z);
                     }
                 }
             }
@@ -1702,8 +1727,7 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
                             tables, tables_out, (uint64_t)entries, to_of);
 }
 
-// Whether a sequence has so many rows on average that its cells are taken whole.  (16 rows of 8 x 128: rows 3.1
-// us, cells 4.6; 12 thousand in 5 sequences: rows 100, cells 21.)
+// Whether a sequence has so many rows on average that its cells are taken whole.
 bool by_cells(const CacheRows& r) { return r.rows >= 8 * (uint64_t)r.count; }
 
 unsigned cell_blocks(const CacheView& c, const CacheRows& r, unsigned units) {
@@ -1744,16 +1768,17 @@ cudaError_t launch_read(cudaStream_t s, T* k, T* v, const CacheView& c, const Ca
 }
 
 // attention_kernel's workspace: two parts of a tile a block that the card holds, and what the block starts.
-template <int GROUPS, int NT, bool LOW>
+template <int GROUPS, int NT, bool LOW, bool HALF = false>
 size_t attention_bytes(int sm_count) {
-    using Shape = AttentionShape<GROUPS, NT, LOW>;
+    using Shape = AttentionShape<GROUPS, NT, LOW, HALF>;
     return (size_t)sm_count * Shape::kBlocksPerSm * (20 + 2 * Shape::kRows * Shape::kPart * 4 + Shape::kAside * 16);
 }
 
 template <int GROUPS>
 size_t attention_bytes(int sm_count) {
     return std::max({attention_bytes<GROUPS, 1, false>(sm_count), attention_bytes<GROUPS, 2, false>(sm_count),
-                     attention_bytes<GROUPS, 1, true>(sm_count), attention_bytes<GROUPS, 2, true>(sm_count)});
+                     attention_bytes<GROUPS, 1, true>(sm_count), attention_bytes<GROUPS, 2, true>(sm_count),
+                     attention_bytes<GROUPS, 1, true, true>(sm_count)});
 }
 
 size_t attention_workspace(int sm_count, size_t dim) {
@@ -1765,12 +1790,12 @@ size_t attention_workspace(int sm_count, size_t dim) {
     }
 }
 
-template <typename T, int GROUPS, int NT>
+template <typename T, int GROUPS, int NT, bool HALF = false>
 cudaError_t launch_tiles(int sm_count, cudaStream_t s, const CacheView& c, const CacheRows& r, AttentionCall call,
                          void* workspace) {
     constexpr bool kLow = std::is_same<T, float>::value;
-    using Shape = AttentionShape<GROUPS, NT, kLow>;
-    const auto kernel = attention_kernel<T, GROUPS, NT, kLow>;
+    using Shape = AttentionShape<GROUPS, NT, kLow, HALF>;
+    const auto kernel = attention_kernel<T, GROUPS, NT, kLow, HALF>;
     const unsigned blocks = (unsigned)(sm_count * Shape::kBlocksPerSm);
     call.tokens = 1;
     while (call.tokens * 2 * call.group <= (uint32_t)Shape::kRows) call.tokens *= 2;
@@ -1809,6 +1834,8 @@ cudaError_t launch_attention(int sm_count, cudaStream_t s, const CacheView& c, c
                              const AttentionCall& call, void* workspace) {
     const uint64_t rows = (uint64_t)((r.rows + r.count - 1) / r.count) * call.group;
     if (rows > 8) return launch_tiles<T, GROUPS, 2>(sm_count, s, c, r, call, workspace);
+    if constexpr (std::is_same<T, float>::value)
+        if (rows <= 4) return launch_tiles<T, GROUPS, 1, true>(sm_count, s, c, r, call, workspace);
     return launch_tiles<T, GROUPS, 1>(sm_count, s, c, r, call, workspace);
 }
 
