@@ -1727,8 +1727,12 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
                             tables, tables_out, (uint64_t)entries, to_of);
 }
 
-// Whether a sequence has so many rows on average that its cells are taken whole.
-bool by_cells(const CacheRows& r) { return r.rows >= 8 * (uint64_t)r.count; }
+// Whether cells are taken whole: where the call has many heads of rows, and a sequence has several on average.
+// (Appended in bf16, 8 x 128, by rows and by cells: 100 in one sequence 2.9 and 8.4 us, 16 of 16 5.4 and 8.8, 128
+// of 8 11.5 and 9.5, 5 of 2500 101 and 35; 128 of 4 7.4 and 15.1.)
+bool by_cells(const CacheView& c, const CacheRows& r) {
+    return (uint64_t)r.rows * c.kv_heads >= 8192 && r.rows >= 8 * (uint64_t)r.count;
+}
 
 unsigned cell_blocks(const CacheView& c, const CacheRows& r, unsigned units) {
     return (unsigned)(((uint64_t)(r.rows + kCellTokens - 1) / kCellTokens * c.kv_heads + units - 1) / units);
@@ -1741,7 +1745,7 @@ cudaError_t launch_append(cudaStream_t s, const T* k, const T* v, size_t k_row, 
         return launch_dependent(kernel, dim3(cell_blocks(c, r, units)), 32 * groups * units, 0, s, k, v, k_row, k_head, v_row, v_head,
                                 wide, c, r);
     };
-    if (!by_cells(r))
+    if (!by_cells(c, r))
         return launch_dependent(append_rows_kernel<T>, dim3((unsigned)(((uint64_t)r.rows * c.kv_heads * 2 + 3) / 4)), 128, 0, s, k, v,
                                 k_row, k_head, v_row, v_head, c, r);
     switch (c.dim / kCacheGroup) {
@@ -1757,7 +1761,7 @@ cudaError_t launch_read(cudaStream_t s, T* k, T* v, const CacheView& c, const Ca
     const auto cells = [&](auto kernel) {
         return launch_dependent(kernel, dim3(cell_blocks(c, r, kCellWarps)), 32 * kCellWarps, 0, s, c, r, k, v);
     };
-    if (!by_cells(r))
+    if (!by_cells(c, r))
         return launch_dependent(read_rows_kernel<T>, dim3((unsigned)(((uint64_t)r.rows * c.kv_heads * 2 + 3) / 4)), 128, 0, s, c, r, k, v);
     switch (c.dim / kCacheGroup) {
     case 1: return cells(read_cells_kernel<T, 1>);

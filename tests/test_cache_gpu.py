@@ -97,6 +97,52 @@ def test_append_writes_the_documented_bytes(gpu, dtype, D, counts):
             assert (got[starts[-1]:] == 7).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 192, 256])
+@pytest.mark.parametrize("size", [16, 48])
+@pytest.mark.parametrize("strided", [False, True])
+def test_append_and_read_of_many_heads_of_rows(gpu, dtype, D, size, strided):
+    counts, heads = [70, 0, 9, 1, 52, 17], 80  # enough for cells to be taken whole
+    held, r = make(D + size, [73, 5, 9, 40, 33, 17], D=D, heads=heads, size=size)  # 52 rows, 33 positions
+    r.tables[0, 2], r.tables[5, 0] = -1, 10 ** 9
+    held = (held[0], tensor(r.tables), tensor(r.lengths))
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    n = int(starts[-1])
+    assert n * heads >= 8192 and n >= 8 * len(counts)
+    rng = np.random.default_rng(5)
+    wide = D + 1 if strided else D  # rows that lie to no 16 bytes
+    k, v = (tensor(rng.standard_normal((n + 1, heads, wide)) * 3, torch.float32).to(dtype)[..., :D] for _ in range(2))
+    cache.append(gpu, k, v, *held, tensor(starts))
+    r.append(k.float().cpu().numpy(), v.float().cpu().numpy(), starts)
+    assert np.array_equal(held[0].cpu().numpy(), r.pages)
+    back = [torch.full((n + 1, heads, D), 7.0, dtype=dtype, device="cuda") for _ in range(2)]
+    cache.read(gpu, *held, tensor(starts), out=back)
+    for got, e in zip(back, r.read(n, starts)):
+        got = got.double().cpu().numpy()
+        nan = np.isnan(e)
+        assert (np.isnan(got[:n]) == nan).all() and (got[n:] == 7).all()
+        # s n + z rounded to f32, then to the type: half a step of each
+        assert (abs(got[:n] - e)[~nan] <= (torch.finfo(dtype).eps / 2 + 2.0 ** -24) * abs(e)[~nan] * 1.001).all()
+
+
+@pytest.mark.parametrize("values", ["ties", "not finite"])
+def test_cells_taken_whole_hold_values_at_the_ends(gpu, values):
+    held, r = make(4, [300, 41], D=64, heads=40)
+    starts = [0, 200, 241]
+    x = np.random.default_rng(6).standard_normal((241, 40, 64)).astype(np.float32)
+    if values == "ties":
+        x[:] = np.arange(64) % 31 * 0.5 + (np.arange(241)[:, None, None] - 120)
+        x[::3] = np.nextafter(x[::3], np.float32(1e9))
+    else:
+        x[3, :, 5], x[17, 1, 9], x[18, 2, 60], x[40], x[41] = np.nan, np.inf, -np.inf, 3.25, 0
+        x[60, :, 0], x[61, :, 0], x[62, :, 1] = 1e30, -60000, 65519.0
+        x[70:90] *= 10.0 ** np.linspace(-9, 4, 20)[:, None, None]
+    k = tensor(x, torch.float32)
+    cache.append(gpu, k, k.flip(2), *held, tensor(starts))
+    r.append(x, x[..., ::-1], starts)
+    assert np.array_equal(held[0].cpu().numpy(), r.pages)
+
+
 def test_append_one_row_a_sequence_and_a_list(gpu):
     held, r = make(1, [3, 40, 33, 97, 64], D=128)
     k, v = (queries(i, 4, 2, 128, torch.float32) for i in (1, 2))
