@@ -508,8 +508,8 @@ int lsx_cache_append_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_
                             const void* v, lsx_dtype kind, size_t k_row, size_t k_head, size_t v_row, size_t v_head,
                             void* stream);
 /* The values that the rows' positions stand for, [rows x kv_heads x head_dim] of `kind`
-   each, s n + z rounded once to f32 and then to the kind: 0 before position 0, NaN where
-   there is no page. */
+   each at 16-byte boundaries, s n + z rounded once to f32 and then to the kind: 0 before
+   position 0, NaN where there is no page. */
 int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, lsx_dtype kind,
                           void* k_out, void* v_out, void* stream);
 /* Attention of the rows' queries over their sequences: with query head h reading key head
@@ -540,7 +540,8 @@ int lsx_cache_fork_device(lsx_ctx* ctx, const lsx_cache_pool* pool, int32_t* tab
                           size_t table_width, int32_t* lengths, int32_t* refs, size_t page_size, const int32_t* parents,
                           const int32_t* children, size_t n, int32_t* pairs, int32_t* missing, void* stream);
 /* Empties the sequences: their pages lose a reference each, and their rows of the tables
-   hold -1.  Entries outside the tables, and sequences named again, are passed over. */
+   hold -1.  Entries outside the tables, and sequences named again, are passed over; n is
+   65536 at most. */
 int lsx_cache_free_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, size_t table_width, int32_t* lengths,
                           int32_t* refs, size_t page_count, size_t page_size, const int32_t* sequences, size_t n,
                           void* stream);

@@ -279,8 +279,8 @@ def fork(gpu: Gpu, pool: torch.Tensor, tables: torch.Tensor, lengths: torch.Tens
 
 def free(gpu: Gpu, tables: torch.Tensor, lengths: torch.Tensor, refs: torch.Tensor, sequences: torch.Tensor,
          page_size: int) -> None:
-    """Empties the sequences (int32); pages that no other sequence shares become free
-    (lsx_cache_free_device)."""
+    """Empties the sequences (int32, at most 65536); pages that no other sequence shares
+    become free (lsx_cache_free_device)."""
     device = gpu.device
     state = _state(device, tables, lengths, refs)
     listed = _ints(device, sequences, None, "sequences")

@@ -1977,7 +1977,7 @@ int lsx_cache_free_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, size
                           int32_t* refs, size_t page_count, size_t page_size, const int32_t* sequences, size_t n,
                           void* stream) {
     LSX_TRY(check_tables(tables, table_rows, table_width, lengths, refs, page_count, page_size));
-    LSX_ENSURE(sequences && n > 0 && n <= (size_t)1 << 20, "name 1..=2^20 sequences");
+    LSX_ENSURE(sequences && n > 0 && n <= (size_t)kMaxFreed, "name 1..=65536 sequences");
     LSX_CACHE_SCOPE();
     free_kernel<<<(unsigned)n, 256, 0, on>>>(tables, (uint32_t)table_rows, (uint32_t)table_width, lengths, refs,
                                              (uint32_t)page_count, (uint32_t)page_size, sequences);

@@ -12,6 +12,7 @@ constexpr int kCellTokens = 16;     // positions of a cell
 constexpr int kCacheGroup = 64;     // elements that share a step and a zero
 constexpr int kMaxCacheDim = 256;   // widest head
 constexpr int kMaxListed = 1024;    // sequences that one call forks or extends
+constexpr int kMaxFreed = 65536;    // and empties: each is looked for among those before it
 
 // The bytes of a cell for heads of `dim` elements, and where its parts start.
 __host__ __device__ constexpr int cell_bytes(int dim) { return 18 * dim; }

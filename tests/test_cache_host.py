@@ -111,6 +111,8 @@ def test_page_calls_are_refused(host):
                  lambda: cache.free(host, *state, listed, 1 << 17), lambda: cache.copy_pages(host, pool[:, :, :3].contiguous(), ints(1, 2))):
         with pytest.raises(LsxError):
             call()
+    with pytest.raises(LsxError, match="65536"):
+        cache.free(host, *state, ints(65537), 16)
     for call in (lambda: cache.reserve(host, *state, listed, listed, 16), lambda: cache.fork(host, pool, *state, listed, listed, 16),
                  lambda: cache.free(host, *state, listed, 16), lambda: cache.compact(host, pool, tables, refs),
                  lambda: cache.copy_pages(host, pool, ints(2, 2))):
