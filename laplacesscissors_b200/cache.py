@@ -77,7 +77,7 @@ def _view(device: int, pages: torch.Tensor, tables: torch.Tensor, lengths: torch
         raise ValueError(_PAGES)
     count, heads, cells, width = pages.shape
     dim = width // 18
-    if width % (18 * GROUP):
+    if width % (18 * GROUP) or not (heads and cells and dim):
         raise ValueError(_PAGES)
     at, rows, entries = _table(device, tables)
     return _VIEW(pages.data_ptr(), count, cells * 16, heads, dim, at, rows, entries, _ints(device, lengths, rows, "lengths")), \

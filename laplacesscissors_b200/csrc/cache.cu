@@ -1671,6 +1671,7 @@ int check_rows(const lsx_cache_rows* rows, const CacheView& view, CacheRows* out
     LSX_ENSURE(rows, "invalid argument");
     LSX_ENSURE(rows->rows > 0 && rows->rows <= (size_t)1 << 26 && rows->sequences <= (size_t)1 << 20 && rows->sequences > 0,
                "check the numbers of rows and sequences");
+    LSX_ENSURE((uint64_t)rows->rows * view.kv_heads <= (uint64_t)1 << 31, "a call takes 2^31 rows of heads at most");
     LSX_ENSURE(rows->list || rows->sequences <= view.table_rows, "more sequences than the tables have rows");
     LSX_ENSURE(rows->starts || rows->rows == rows->sequences, "without starts each sequence has one row");
     *out = CacheRows{rows->list, rows->starts, (uint32_t)rows->sequences, (uint32_t)rows->rows};

@@ -120,6 +120,20 @@ def test_page_calls_are_refused(host):
             call()
 
 
+def test_pages_of_nothing_and_calls_beyond_the_grid(host):
+    _, tables, lengths = held()
+    for shape in ((3, 0, 2, 18 * 64), (3, 2, 0, 18 * 64), (3, 2, 2, 0)):
+        with pytest.raises(ValueError, match="pages"):
+            cache.attention(host, torch.zeros(4, 2, shape[3] // 18), torch.zeros(shape, dtype=torch.uint8), tables, lengths)
+    address = 1 << 20
+    for rows, heads, word in ((1 << 16, 1 << 15, b"context"), ((1 << 16) + 1, 1 << 15, b"rows of heads"), (1 << 26, 33, b"rows of heads")):
+        view = CacheView(pages=address, page_count=3, page_size=32, kv_heads=heads, head_dim=64, tables=address, table_rows=4,
+                         table_width=5, lengths=address)
+        listed = CacheRows(rows=rows, sequences=4, starts=address)
+        assert lib.lsx_cache_append_device(None, C.byref(view), C.byref(listed), address, address, 0, 0, 0, 0, 0, None) != 0
+        assert word in lib.lsx_last_error()
+
+
 def test_calls_of_nothing(host):
     x = torch.zeros(0, 2, 64)
     cache.append(host, x, x, *held(), sequences=ints(0))
