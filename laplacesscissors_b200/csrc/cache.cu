@@ -678,6 +678,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     attention_kernel(CacheView c, CacheRows r, AttentionCall call) {
     using Shape = AttentionShape<GROUPS, NT, LOW, HALF>;
     constexpr bool BOTH = LOW && !HALF;  // low parts by products of their own
+    // What 11 bits leave of p s acts on n; taken from the sum of p z eight times, it acts on n - 8.  Where the
+    // result has 11 bits too that shows (60 sequences of 5000 positions, f16: 2.4e-4 of the result's size off,
+    // 2.2e-4 with it, 2.1e-4 by the result's own rounding; 46.1 us, 45.4 without), not in the 8 of bf16.
+    constexpr bool kCentred = std::is_same<T, __half>::value;
     static_assert(!HALF || (LOW && NT == 1), "four rows");
     constexpr int D = Shape::kDim, kStages = Shape::kStages;
     constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
@@ -1127,6 +1131,11 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         }
                         p0[n] = pack_f16(x[0], x[1]);
                         p1[n] = pack_f16(x[2], x[3]);
+                        if constexpr (kCentred) {  // what the rounding leaves, times 8
+                            const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
+                            zeros[n][g] = fma(Two(8.f), Two(x[0], x[1]) + Two(-a.x, -a.y), zeros[n][g]);
+                            zeros[n][g] = fma(Two(8.f), Two(x[2], x[3]) + Two(-d.x, -d.y), zeros[n][g]);
+                        }
                         if constexpr (LOW) {
                             const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
                             const uint32_t low0 = pack_f16(x[0] - a.x, x[1] - a.y), low1 = pack_f16(x[2] - d.x, x[3] - d.y);
