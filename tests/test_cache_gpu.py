@@ -222,6 +222,16 @@ def test_several_rows_a_sequence(gpu, dtype, size, group, heads):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 192, 256])
+@pytest.mark.parametrize("counts,group", [([1] * 11 + [37], 1), ([2, 0, 1, 1, 5, 0, 0, 1], 2), ([1, 1, 1, 9, 0, 0], 4), ([1] * 15 + [50], 4)])
+def test_few_rows_but_for_one_sequence(gpu, dtype, D, counts, group):
+    lengths = [max(n, 700 * (i % 3 == 0) + 13 * i) for i, n in enumerate(counts)]
+    held, r = make(group + D, lengths, D=D)
+    starts = np.concatenate([[0], np.cumsum(counts)])
+    check(gpu, held, r, queries(group, int(starts[-1]), 2 * group, D, dtype), starts)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
 def test_more_rows_than_positions_and_rows_of_no_sequence(gpu, dtype):
     held, r = make(8, [3, 0, 40], D=128)
     starts = [2, 9, 13, 17]
