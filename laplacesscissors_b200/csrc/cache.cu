@@ -229,6 +229,8 @@ constexpr int kCellWarps = 4;
 template <int GROUPS>
 constexpr int kAppendUnits = GROUPS == 1 ? 4 : GROUPS == 2 ? 2 : 1;  // (rows, head)s of a block
 
+static_assert(kAppendUnits<2> <= 2 && kAppendUnits<3> == 1 && kAppendUnits<4> == 1, "two barriers");
+
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(32 * GROUPS * kAppendUnits<GROUPS>) append_cells_kernel(
     const T* k, const T* v, size_t k_row, size_t k_head, size_t v_row, size_t v_head, bool wide, CacheView c, CacheRows r) {
@@ -239,11 +241,15 @@ __global__ void __launch_bounds__(32 * GROUPS * kAppendUnits<GROUPS>) append_cel
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32, i = warp % GROUPS;
     const uint64_t unit = (uint64_t)blockIdx.x * kUnits + warp / GROUPS;
     uint8_t* shared_cell = cells[warp / GROUPS];
-    const auto meet = [&] {  // the unit's warps
+    // The unit's warps.  Barriers named by a register count as all sixteen, which leaves four blocks an SM
+    // (30000 rows of 8 x 128 in bf16: 67 us, 80 with four blocks).
+    const auto meet = [&] {
         if constexpr (GROUPS == 1)
             __syncwarp();
+        else if (kUnits == 1 || warp / GROUPS == 0)
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * GROUPS) : "memory");
         else
-            asm volatile("bar.sync %0, %1;" ::"r"(warp / GROUPS + 1), "n"(32 * GROUPS) : "memory");
+            asm volatile("bar.sync 2, %0;" ::"n"(32 * GROUPS) : "memory");
     };
     const uint32_t first = (uint32_t)(unit / c.kv_heads) * kCellTokens, head = (uint32_t)(unit % c.kv_heads);
     if (first >= r.rows) return;
@@ -1740,7 +1746,7 @@ cudaError_t launch_copy(lsx_ctx* ctx, cudaStream_t s, const lsx_cache_pool& pool
 
 // Whether cells are taken whole: where the call has many heads of rows, and a sequence has several on average.
 // (Appended in bf16, 8 x 128, by rows and by cells: 100 in one sequence 2.9 and 8.4 us, 16 of 16 5.4 and 8.8, 128
-// of 8 11.5 and 9.5, 5 of 2500 101 and 35; 128 of 4 7.4 and 15.1.)
+// of 8 11.5 and 9.5, 5 of 2500 101 and 30; 128 of 4 7.4 and 15.1.)
 bool by_cells(const CacheView& c, const CacheRows& r) {
     return (uint64_t)r.rows * c.kv_heads >= 8192 && r.rows >= 8 * (uint64_t)r.count;
 }
