@@ -52,13 +52,6 @@ cudaError_t launch_dependent(void (*kernel)(Params...), dim3 blocks, unsigned th
 }
 
 // ---- rows of a call ------------------------------------------------------------
-struct SequenceRows {
-    int table;   // row of the tables, -1 when the list names none
-    int first;   // its first row of the call
-    int count;   // its rows
-    int length;  // its positions, those of the rows last
-};
-
 __device__ __forceinline__ SequenceRows sequence_rows(const CacheView& c, const CacheRows& r, uint32_t b) {
     SequenceRows s;
     s.table = r.sequences ? r.sequences[b] : (int)b;
@@ -439,15 +432,8 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // A warp streams every fourth pair of the run through its own ring in shared memory by bulk
 // copies, with its own softmax; the warps' sums meet at a tile's end.
 //
-// Cost that a block takes at least, where there is little: a tile and two pairs a warp.
-constexpr int kLeastRun = 20;
-constexpr int kPairTokens = 2 * kCellTokens;
 // Positions of a table row up to which tiles are not shared.
 constexpr int kWholeTokens = 512;
-// What a tile costs beside its pairs (the first copies' latency, the queries, the sums), in
-// pairs: it counts so many more when the runs are cut (61 sequences of about 5000 positions, f16: 70 us
-// with 1, 61 with 4, 45 with 12).
-constexpr int kTileCost = 12;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
 // Floats of a row's part: its sums, its reference and the sum of its weights.
@@ -490,37 +476,6 @@ struct AttentionCall {
     float* parts;              // [2 blocks][used][part_row(dim)]
     float4* aside;             // [warps][rows / 8][dim / 16 + 1][32]: sums that a thread puts aside
 };
-
-// A call's pairs in order.  Tile k of a sequence holds its rows' positions k * tokens and on;
-// a tile without visible positions counts as one pair, so that its rows get written.
-__device__ __forceinline__ int tile_count(const SequenceRows& s, int tokens) { return (s.count + tokens - 1) / tokens; }
-
-__device__ __forceinline__ int tile_pairs(const SequenceRows& s, int tokens, int k) {
-    const int seen = s.length - s.count + min(s.count, (k + 1) * tokens);  // positions that its last row sees
-    return max(1, (seen + kPairTokens - 1) >> 5);
-}
-
-// Cost of the tiles before k (k below the tile count), kTileCost and their pairs each: the sum of floor((base + 31 + (i + 1) tokens) / 32), with
-// base = length - count, over the tiles that see anything, and 1 for those that do not.  tokens divides 32.
-__device__ __forceinline__ long long cost_before(const SequenceRows& s, int tokens, int k) {
-    if (k == 0) return 0;
-    const int base = s.length - s.count;
-    const int blind = s.length <= 0 ? k : base >= 0 ? 0 : min(k, -base / tokens);
-    const long long fixed = (long long)k * kTileCost;
-    if (k <= blind) return fixed + k;
-    const int shift = 31 - __clz(tokens), m = kPairTokens >> shift, y = (base + kPairTokens - 1) >> shift;
-    const auto sum = [m](long long n) {  // of floor(i / m) over i = 0 .. n
-        if (n < 0) return 0ll;
-        const long long q = n / m, r = n % m;
-        return m * q * (q - 1) / 2 + q * (r + 1);
-    };
-    return fixed + blind + sum((long long)y + k) - sum((long long)y + blind);
-}
-
-__device__ __forceinline__ long long sequence_cost(const SequenceRows& s, int tokens) {
-    const int tiles = tile_count(s, tokens);
-    return tiles ? cost_before(s, tokens, tiles - 1) + kTileCost + tile_pairs(s, tokens, tiles - 1) : 0;
-}
 
 // c += a b, and c = a b.
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -733,64 +688,44 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     }
     const long long shares = total + gridDim.x - 1;
     const long long run = max(shares >> 32 ? shares / gridDim.x : (long long)((uint32_t)shares / gridDim.x), (long long)kLeastRun);
-    long long at = run * blockIdx.x, offset = 0;  // cost: the run's next, and that within sequence b
-    const long long end = min(at + run, total);
-    uint32_t b = 0;
+    Run left;
+    left.at = run * blockIdx.x;
+    left.end = min(left.at + run, total);
     if (threadIdx.x == 0) call.shares[blockIdx.x] = 0;
-    if (at >= end) return;
-    if (mine > 0 && before <= at && at < before + mine) {
+    if (left.at >= left.end) return;
+    if (mine > 0 && before <= left.at && left.at < before + mine) {
         for (uint32_t n = mine_first; n < mine_end; ++n) {
             const long long cost = sequence_cost(sequence_rows(c, r, n), tokens) * tiles_of;
-            if (at < before + cost) {
+            if (left.at < before + cost) {
                 found[0] = n;
-                found[1] = at - before;
+                found[1] = left.at - before;
                 break;
             }
             before += cost;
         }
     }
     __syncthreads();
-    b = (uint32_t)found[0];
-    offset = found[1];
+    left.sequence = (uint32_t)found[0];
+    left.offset = found[1];
 
     // The first warp finds the next part of a tile in the run.
     const auto next_part = [&] {
         TilePart next;
         next.pairs = 0;
-        while (at < end) {
-            const SequenceRows s = sequence_rows(c, r, b);
-            const long long one = sequence_cost(s, tokens);
-            if (offset >= one * tiles_of) {
-                ++b;
-                offset = 0;
-                continue;
-            }
-            const uint32_t head_sub = offset >> 32 ? (uint32_t)(offset / one) : (uint32_t)offset / (uint32_t)one;  // one <= offset or 0
-            const long long rest = offset - head_sub * one;
-            int k = 0;
-            for (int high = tile_count(s, tokens); high - k > 1;) {  // cost_before(k) <= rest
-                const int middle = (k + high) / 2;
-                if (cost_before(s, tokens, middle) <= rest)
-                    k = middle;
-                else
-                    high = middle;
-            }
-            // the first kTileCost of a tile's cost stand for no pair
-            const int pairs = tile_pairs(s, tokens, k), from_cost = (int)(rest - cost_before(s, tokens, k));
-            const int to_cost = call.whole ? pairs + kTileCost : (int)min((long long)pairs + kTileCost, from_cost + end - at);
-            at += to_cost - from_cost;
-            offset += to_cost - from_cost;
-            if (to_cost <= kTileCost || (call.whole && from_cost > 0)) continue;
-            const int base = s.length - s.count, tile_end = min(s.count, (k + 1) * tokens);
-            next.first = max(from_cost - kTileCost, 0);
-            next.last = to_cost - kTileCost;
-            next.pairs = pairs;
-            next.row = s.first + k * tokens;
-            next.positions = tile_end - k * tokens;
-            next.least = base + k * tokens + 1;
+        while (left.at < left.end) {
+            const SequenceRows s = sequence_rows(c, r, left.sequence);
+            RunTile tile;
+            if (!next_tile(left, s, tokens, tiles_of, call.whole, tile)) continue;
+            const int base = s.length - s.count, tile_end = min(s.count, (tile.k + 1) * tokens);
+            next.first = tile.first;
+            next.last = tile.last;
+            next.pairs = tile.pairs;
+            next.row = s.first + tile.k * tokens;
+            next.positions = tile_end - tile.k * tokens;
+            next.least = base + tile.k * tokens + 1;
             next.seen = min(base + tile_end, covered);
-            next.head = (int)(call.subs == 1 ? head_sub : head_sub / call.subs);
-            next.sub = (int)(call.subs == 1 ? 0 : head_sub % call.subs);
+            next.head = (int)(call.subs == 1 ? tile.head : tile.head / call.subs);
+            next.sub = (int)(call.subs == 1 ? 0 : tile.head % call.subs);
             next.table = s.table;
             break;
         }

@@ -4,11 +4,11 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "cache_runs.cuh"
 #include "lsx.h"
 
 namespace lsx {
 
-constexpr int kCellTokens = 16;     // positions of a cell
 constexpr int kCacheGroup = 64;     // elements that share a step and a zero
 constexpr int kMaxCacheDim = 256;   // widest head
 constexpr int kMaxListed = 1024;    // sequences that one call forks or extends
