@@ -772,10 +772,10 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         }
 
         // ---- the stream of pairs: warp w takes pairs first + w, first + w + 4, ..
-        const int stop = min(last, (seen + kPairTokens - 1) >> 5);  // pairs beyond hold nothing
+        const int stop = min(last, seen <= 0 ? 0 : ((seen - 1) >> 5) + 1);  // pairs beyond hold nothing
         const int mine_pairs = max(0, (stop - first - warp + kAttentionWarps - 1) / kAttentionWarps);
         const int32_t* table = c.tables + (size_t)max(part.table, 0) * c.table_width;
-        const uint32_t seen_cells = (uint32_t)max((seen + kCellTokens - 1) >> 4, 0);
+        const uint32_t seen_cells = seen <= 0 ? 0 : ((seen - 1) >> 4) + 1;
         const uint8_t* head_cells = c.pages + (size_t)head * per_page * Shape::kCell;
         // Each lane looks up one of the next 32 pairs and copies it when a stage is free.
         const uint8_t* from[2] = {nullptr, nullptr};
@@ -1153,7 +1153,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = nan;
                 break;
             }
-            if (none | ((pair + 1) * kPairTokens > least)) {
+            if (none || pair >= least >> 5) {  // some row does not see all of the pair's positions
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
 #pragma unroll

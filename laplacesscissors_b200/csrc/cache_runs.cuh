@@ -43,7 +43,7 @@ LSX_RUNS int tile_count(const SequenceRows& s, int tokens) { return (s.count + t
 
 LSX_RUNS int tile_pairs(const SequenceRows& s, int tokens, int k) {
     const int seen = s.length - s.count + least_of(s.count, (k + 1) * tokens);  // positions that its last row sees
-    return most_of(1, (seen + kPairTokens - 1) >> 5);
+    return seen <= kPairTokens ? 1 : ((seen - 1) >> 5) + 1;
 }
 
 // Sum of floor(i / m) over i = 0 .. n.
@@ -64,8 +64,9 @@ LSX_RUNS long long cost_before(const SequenceRows& s, int tokens, int k) {
     if (k <= blind) return fixed + k;
     int shift = 0;
     while (tokens >> (shift + 1)) ++shift;
-    const int m = kPairTokens >> shift, y = (base + kPairTokens - 1) >> shift;
-    return fixed + blind + sum_of_quotients((long long)y + k, m) - sum_of_quotients((long long)y + blind, m);
+    const int m = kPairTokens >> shift;
+    const long long y = ((long long)base + kPairTokens - 1) >> shift;  // a length may be 2^31 - 1
+    return fixed + blind + sum_of_quotients(y + k, m) - sum_of_quotients(y + blind, m);
 }
 
 LSX_RUNS long long sequence_cost(const SequenceRows& s, int tokens) {

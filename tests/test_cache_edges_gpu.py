@@ -240,3 +240,27 @@ def test_long_runs_do_not_drift(gpu, dtype):
         assert (error <= allowed).all(), float((error - allowed).max())
         if dtype is torch.float32:
             assert float(error.norm() / expected.norm()) < 1e-5
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_lengths_at_the_end_of_their_type(gpu, dtype):
+    """A sequence of 2^31 - 16 positions whose table names one page again and again: the attention over it is
+    that over the page, and rows behind it, of a length that no table covers, are NaN."""
+    held, r = make(95, [16], heads=1, D=64, size=16, spare=0)
+    width = (2 ** 31 - 1) // 16
+    tables = torch.zeros((2, width), dtype=torch.int32, device="cuda")
+    lengths = tensor([16 * width, 2 ** 31 - 1])
+    q = queries(96, 21, 1, 64, dtype)
+    got = cache.attention(gpu, q, held[0], tables, lengths, tensor([0, 1, 21]))
+    # row i of the second's twenty sees 2^31 - 20 + i positions, of which the table covers 16 * width
+    seen = np.array([16 * width] + [2 ** 31 - 20 + i for i in range(20)])
+    fine = seen <= 16 * width
+    assert fine.sum() == 6 and torch.equal(torch.isnan(got).all(2).all(1).cpu(), torch.from_numpy(~fine))
+    k, v, _, _ = r.values(0, 16)
+    z = np.einsum("bhd,td->bht", q.double().cpu().numpy(), k[:, 0]) / 8
+    p = np.exp(z - z.max(2, keepdims=True))
+    expected = np.einsum("bht,td->bhd", p / p.sum(2, keepdims=True), v[:, 0])
+    # a thread adds less than 2 * 10^5 weights (3 tiles of 2^26 pairs over 2000 warps, two a pair) and as many products
+    # with the zeros, each addition off by 2^-25 of the sum at most, all alike where the terms are: 6e-3 each
+    error = abs(got.double().cpu().numpy() - expected)[fine]
+    assert (error <= 1.2e-2 * abs(v).max() + torch.finfo(dtype).eps / 2 * abs(expected[fine])).all(), error.max()

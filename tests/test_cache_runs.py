@@ -112,3 +112,12 @@ def test_every_pair_once_and_in_order(cut, tokens, whole):
 def test_long_prompts(cut, counts, lengths, tokens, heads):
     for blocks in (296, 444, 592):
         assert cut(counts, lengths, tokens, heads, blocks) == 0
+
+
+# Lengths up to 2^31 - 1, whose pairs end beyond what 32 bits with a sign hold.
+@pytest.mark.parametrize("tokens", [1, 2, 8, 16])
+@pytest.mark.parametrize("length", [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 31 - 33, 2 ** 31 - 300])
+def test_lengths_at_the_end_of_their_type(cut, tokens, length):
+    for counts in ([1], [100], [3000, 1, 70]):
+        for blocks in (296, 444, 592):
+            assert cut(counts, [length] * len(counts), tokens, 2, blocks) == 0
