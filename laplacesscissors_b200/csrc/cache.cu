@@ -411,14 +411,17 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 //
 // Rounding.  A query row is scaled by a power of two to below 2^14 and held as f16, which
 // holds f16 and bf16 queries exactly down to 2^-38 of the row's largest element, or for f32
-// (LOW) as f16 high and low parts of 22 bits.  A weight p is taken against a reference that
-// keeps p s below 2^15, and p s is held the same two ways: 11 bits are half a step of an
-// f16 result, twice 11 those of f32.  Everything else is f32.  The sum of p s n and that of p z
+// (LOW) as f16 high and low parts of 22 bits.  A weight p is taken against a reference of its row, and
+// p s times a unit of its row and group is held the same two ways: 11 bits are half a step of an
+// f16 result, twice 11 those of f32.  The unit keeps that product below 2^15; where it might pass (or a weight 2^20) the
+// reference becomes the row's largest score and the unit leaves 2^7 for the largest product that the row has met in the group,
+// so that 2^-21 of that still has 11 bits, and 2^-10 of it 22, whatever the other groups' steps are and
+// whatever steps positions of little weight have.  (Steps 2^20 apart in two groups and a unit for both: 8.5e-5 of the smaller
+// group's size off in f32.)  Steady sequences hardly ever move it: the units cost 36.1 instead of 34.6 us at 16 x 4113
+// positions in f32.  Everything else is f32.  The sum of p s n and that of p z
 // are often large beside what is left of them, and the tensor cores cut what they add to a sum:
 // f32 calls take n - 8 and z + 8 s instead, whose sums are as small as the result (16 x 4113
-// positions: 4.5e-7 of the result's size off, 1.8e-5 without; 37.1 us, 32.2 without).  The
-// reference of a row moves up where p s would pass 2^15, to leave 2^10 for the largest: what is
-// 2^24 below that still has 11 bits, and steady sequences hardly ever move it.
+// positions: 4.5e-7 of the result's size off, 1.8e-5 without; 37.1 us, 32.2 without).
 //
 // The low parts of f32 are products of their own.  Where a tile has four rows at most (HALF) they
 // take the columns that would be left unused, four further on, and the halves are added by one
@@ -443,21 +446,22 @@ constexpr int part_row(int dim) { return dim + 2; }
 template <int GROUPS, int NT, bool LOW, bool HALF>
 struct AttentionShape {
     static constexpr int kDim = 64 * GROUPS, kPart = part_row(kDim), kRows = HALF ? 4 : 8 * NT, kCell = cell_bytes(kDim), kStage = 2 * kCell;
-    // registers a thread: the sums and the queries, beside some 75 for the rest; where those are not left the
+    // registers a thread: the sums and the queries, beside 75 and more for the rest; where those are not left the
     // queries go to shared memory.  Blocks of an SM, measured in us (three, four): one row of 128, 131072 positions,
-    // 39.3 and 42.7; parts of prompts in heads of 64 526 and 440; in heads of 128, three 1083 and two 1089.
+    // 39.3 and 42.7; parts of prompts in heads of 64 526 and 440; (two, three) one row of 256, 62 and 87.
     static constexpr int kLoad = NT * GROUPS, kHeld = (LOW && !HALF ? 32 : 24) * kLoad;
-    static constexpr int kBlocksPerSm = kHeld <= 24 || (NT == 2 && kHeld <= 48) ? 4 : kHeld <= 96 && (NT == 1 || LOW) ? 3 : 2;
+    static constexpr int kBlocksPerSm = kHeld <= 24 || (NT == 2 && kHeld <= 48) ? 4 : kHeld <= 96 && GROUPS < 4 && (NT == 1 || LOW) ? 3 : 2;
     static constexpr bool kSharedQuery = kHeld > 180;
     static constexpr int kQuery = kSharedQuery ? kLoad * 4 * 32 * (LOW && !HALF ? 16 : 8) : 0;
-    static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery) / (kAttentionWarps * kStage);
+    static constexpr int kPlain = kSharedQuery ? kAttentionWarps * kLoad * 4 * 8 : 0;
+    static constexpr int kRoom = (228 * 1024 / kBlocksPerSm - 1400 - kQuery - kPlain) / (kAttentionWarps * kStage);
     static constexpr int kStages = kRoom > 6 ? 6 : kRoom;
     static constexpr int kAtOnce = GROUPS <= 2 && (NT == 1 || !LOW) ? 2 : 1;  // cells whose products are under way at the same time
     static constexpr int kRing = kAttentionWarps * kStages * kStage;
     static constexpr int kParts = kAttentionWarps * kRows * kPart * 4;  // the warps' sums, in the ring's memory
     static constexpr int kAside = kAttentionWarps * NT * (4 * GROUPS + 1) * 32;  // sums put aside, four floats each
     static constexpr int kBars = kAttentionWarps * kStages * 8;
-    static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kQuery + kBars;
+    static constexpr int kShared = (kRing > kParts ? kRing : kParts) + kPlain + kQuery + kBars;
     static_assert(kStages >= 2 && kBlocksPerSm * (kShared + 1200) <= 228 * 1024, "shared memory");
 };
 
@@ -515,6 +519,18 @@ __device__ __forceinline__ Two operator+(Two a, Two b) {
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.bits) : "l"(a.bits), "l"(b.bits));
     return d;
 }
+
+__device__ __forceinline__ Two both(Two a) { return a; }
+// The same held as bf16, in one register.
+struct PackedTwo {
+    uint32_t bits;
+    __device__ __forceinline__ PackedTwo() {}
+    __device__ __forceinline__ PackedTwo(float a, float b) {
+        const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+        bits = *reinterpret_cast<const uint32_t*>(&x);
+    }
+};
+__device__ __forceinline__ Two both(PackedTwo a) { return Two(__uint_as_float(a.bits << 16), __uint_as_float(a.bits & 0xffff0000u)); }
 
 __device__ __forceinline__ uint32_t pack_f16(float low, float high) {
     const __half2 h = __floats2half2_rn(low, high);
@@ -647,6 +663,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     static_assert(!HALF || (LOW && NT == 1), "four rows");
     constexpr int D = Shape::kDim, kStages = Shape::kStages;
     constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
+    constexpr float kMostUnit = 0x1p100f, kRoom = 0x1p7f;
+    // Units of two rows; one register each where there are many (up to 6 rows a sequence of heads of 256, bf16: 72 us, 75 in two).
+    using Units = std::conditional_t<(NT * GROUPS > 4), PackedTwo, Two>;
     extern __shared__ __align__(128) uint8_t shared[];
     __shared__ TilePart part;
     __shared__ long long scan[kAttentionWarps], found[2];
@@ -655,6 +674,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     uint8_t* ring = shared + warp * kStages * Shape::kStage;
     float* warp_sums = reinterpret_cast<float*>(shared);
     uint2* queries = reinterpret_cast<uint2*>(shared + Shape::kShared - Shape::kBars - Shape::kQuery);
+    float2* warp_plain = reinterpret_cast<float2*>(shared + Shape::kShared - Shape::kBars - Shape::kQuery - Shape::kPlain) +
+                         warp * Shape::kPlain / (8 * kAttentionWarps) + j;
     uint64_t* bars = reinterpret_cast<uint64_t*>(shared + Shape::kShared - Shape::kBars) + warp * kStages;
     const int tokens = (int)call.tokens;
     const uint32_t tiles_of = c.kv_heads * call.subs;
@@ -825,7 +846,15 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         // ---- queries as the products' columns: the thread's rows of the results are 2 j and 2 j + 1 of each eight
         uint32_t query[Shape::kSharedQuery ? 1 : NT * GROUPS * 4][BOTH ? 4 : 2];
         float factor[NT][2];
-        Two plain[NT][GROUPS];
+        Two plain_of[Shape::kSharedQuery ? 1 : NT][GROUPS];
+        const auto plain = [&](int n, int g) -> Two {
+            if constexpr (Shape::kSharedQuery) {
+                const float2 x = warp_plain[(n * GROUPS + g) * 4];
+                return Two(x.x, x.y);
+            } else {
+                return plain_of[n][g];
+            }
+        };
         int limit[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -883,26 +912,35 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     }
                 if (HALF)
                     for (int i = 0; i < 2; ++i) ones[i] += __shfl_xor_sync(0xffffffffu, ones[i], 2);
-                plain[t][g] = Two(ones[0], ones[1]);
+                if constexpr (Shape::kSharedQuery) {
+                    if (quad == 0) warp_plain[(t * GROUPS + g) * 4] = make_float2(ones[0], ones[1]);
+                } else {
+                    plain_of[t][g] = Two(ones[0], ones[1]);
+                }
             }
         }
         if constexpr (Shape::kSharedQuery) __syncthreads();
 
-        float out[NT][4 * GROUPS][4], reference[NT][2], sum[NT][2];
-        Two zeros[NT][GROUPS];
+        float out[NT][4 * GROUPS][4], reference[NT][2];
+        Two sum[NT], zeros[NT][GROUPS];
+        Units unit[NT][GROUPS], eighth[kCentred ? NT : 1][GROUPS];  // and 8 over it
+        float most_unit[GROUPS];  // the largest unit of a group among the thread's rows
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) most_unit[g] = kMostUnit;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
 #pragma unroll
             for (int n = 0; n < 4 * GROUPS; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) out[t][n][i] = 0.f;
+            reference[t][0] = reference[t][1] = kNone;
+            sum[t] = Two(0.f);
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                reference[t][i] = kNone;
-                sum[t][i] = 0.f;
+            for (int g = 0; g < GROUPS; ++g) {
+                zeros[t][g] = Two(0.f);
+                unit[t][g] = Units(kMostUnit, kMostUnit);
+                if constexpr (kCentred) eighth[t][g] = Units(8.f / kMostUnit, 8.f / kMostUnit);
             }
-#pragma unroll
-            for (int g = 0; g < GROUPS; ++g) zeros[t][g] = Two(0.f);
         }
 
         const uint32_t pick = quad & 1 ? 0x7632u : 0x5410u;  // a thread's position among two: its step and zero
@@ -980,7 +1018,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                                 d[2 * i] += __shfl_xor_sync(0xffffffffu, d[2 * i], 2);
                                 d[2 * i + 1] += __shfl_xor_sync(0xffffffffu, d[2 * i + 1], 2);
                             }
-                            const Two zero = g ? fma(Two(sz.y), plain[n][g], score[n][i]) : Two(sz.y) * plain[n][g];
+                            const Two zero = g ? fma(Two(sz.y), plain(n, g), score[n][i]) : Two(sz.y) * plain(n, g);
                             score[n][i] = fma(Two(sz.x), Two(d[2 * i], d[2 * i + 1]), zero);
                         }
                     const uint4 more = *reinterpret_cast<const uint4*>(steps_of + cell_value_steps(D));
@@ -991,7 +1029,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         values[g][i] = *reinterpret_cast<__half2*>(&sz[i]);
                     }
                 }
-                // weights
+                // weights; `largest`: the most that a weight of 1 times a step and a unit may be here
                 float weight[NT][4], most = 0.f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
@@ -1005,50 +1043,87 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                         if (EDGE && blind(u, i / 2, n, i % 2)) weight[n][i] = 0.f;
                         most = fmaxf(most, weight[n][i]);
                     }
-                __half2 steps = values[0][0];
+                float largest = 0x1p-5f;
 #pragma unroll
-                for (int i = 1; i < 2 * GROUPS; ++i) steps = __hmax2(steps, values[i / 2][i % 2]);
-                const float largest = fmaxf(__low2float(steps), 0x1p-30f);
+                for (int g = 0; g < GROUPS; ++g) largest = fmaxf(largest, most_unit[g] * __low2float(__hmax2(values[g][0], values[g][1])));
                 if (__any_sync(0xffffffffu, !(most * largest < 0x1p15f))) {
-                    const float all = quad_max(across_max(largest));
-                    const float above = (float)(ilogbf(all) + 1);  // 2^above is above these steps
+                    // a row's largest weight so far becomes 1, and its products with the group's steps kRoom at most
+                    float top[NT][2], keep[NT][2];
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float top = -INFINITY;
-                            float mine[2];
+                            top[n][i] = -INFINITY;
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
                                 float rows[2];
                                 score[n][m].get(rows[0], rows[1]);
-                                mine[m] = rows[i];
-                                if (!EDGE || !blind(u, m, n, i)) top = fmaxf(top, mine[m] * factor[n][i]);
+                                if (!EDGE || !blind(u, m, n, i)) top[n][i] = fmaxf(top[n][i], rows[i] * factor[n][i]);
                             }
-                            top = across_max(top);
-                            const float next = fmaxf(reference[n][i], top + above - 10.f);
-                            const float keep = exp2_approx(reference[n][i] - next);
+                        }
+#pragma unroll
+                    for (int o = 4; o < 32; o *= 2)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) top[n][i] = fmaxf(top[n][i], __shfl_xor_sync(0xffffffffu, top[n][i], o));
+                    __nv_bfloat162 here[NT][GROUPS];  // of both rows: units need no more than bf16 holds
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const float next = fmaxf(reference[n][i], top[n][i]);
+                            keep[n][i] = exp2_approx(reference[n][i] - next);
                             reference[n][i] = next;
-                            sum[n][i] *= keep;
-#pragma unroll
-                            for (int g = 0; g < GROUPS; ++g) zeros[n][g] = zeros[n][g] * (i ? Two(1.f, keep) : Two(keep, 1.f));
-#pragma unroll
-                            for (int m = 0; m < 4 * GROUPS; ++m) {
-                                out[n][m][i] *= keep;
-                                out[n][m][2 + i] *= keep;
-                            }
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
-                                float& w = weight[n][2 * m + i];
-                                w = exp2_approx(fmaf(mine[m], factor[n][i], -next));
+                                float rows[2], &w = weight[n][2 * m + i];
+                                score[n][m].get(rows[0], rows[1]);
+                                w = exp2_approx(fmaf(rows[i], factor[n][i], -next));
                                 if (EDGE && blind(u, m, n, i)) w = 0.f;
                             }
                         }
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) {
+                            const float s[2] = {__low2float(values[g][0]), __low2float(values[g][1])};
+                            here[n][g] = __floats2bfloat162_rn(fmaxf(weight[n][0] * s[0], weight[n][2] * s[1]), fmaxf(weight[n][1] * s[0], weight[n][3] * s[1]));
+                        }
+                    }
+#pragma unroll
+                    for (int o = 4; o < 32; o *= 2)
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+#pragma unroll
+                            for (int g = 0; g < GROUPS; ++g) here[n][g] = __hmax2(here[n][g], __shfl_xor_sync(0xffffffffu, here[n][g], o));
+#pragma unroll
+                    for (int g = 0; g < GROUPS; ++g) most_unit[g] = 0.f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        sum[n] = sum[n] * Two(keep[n][0], keep[n][1]);
+#pragma unroll
+                        for (int g = 0; g < GROUPS; ++g) {
+                            const float2 product = __bfloat1622float2(here[n][g]);
+                            float was[2], now[2], by[2];
+                            both(unit[n][g]).get(was[0], was[1]);
+#pragma unroll
+                            for (int i = 0; i < 2; ++i)
+                                now[i] = fminf(fminf(__fdividef(was[i], keep[n][i]), kMostUnit), __fdividef(kRoom, i ? product.y : product.x));
+                            unit[n][g] = Units(now[0], now[1]);
+                            both(unit[n][g]).get(now[0], now[1]);
+                            if constexpr (kCentred) eighth[n][g] = Units(__fdividef(8.f, now[0]), __fdividef(8.f, now[1]));
+                            most_unit[g] = fmaxf(most_unit[g], fmaxf(now[0], now[1]));
+#pragma unroll
+                            for (int i = 0; i < 2; ++i) by[i] = keep[n][i] * __fdividef(now[i], was[i]);
+#pragma unroll
+                            for (int m = 4 * g; m < 4 * g + 4; ++m)
+#pragma unroll
+                                for (int i = 0; i < 4; ++i) out[n][m][i] *= by[i % 2];
+                            zeros[n][g] = zeros[n][g] * Two(keep[n][0], keep[n][1]);
+                        }
+                    }
                 }
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) sum[n][i] += weight[n][i] + weight[n][2 + i];
+                for (int n = 0; n < NT; ++n) sum[n] = sum[n] + (Two(weight[n][0], weight[n][1]) + Two(weight[n][2], weight[n][3]));
                 const uint8_t* cell = held + u * Shape::kCell;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
@@ -1057,35 +1132,34 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     uint32_t p0[NT], p1[NT], l0[NT], l1[NT];
 #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        float x[4];
+                        uint32_t low[2];
+                        const Two units = both(unit[n][g]);
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const Two w(weight[n][2 * i], weight[n][2 * i + 1]);
-                            (w * Two(sz[i].x)).get(x[2 * i], x[2 * i + 1]);
+                            float x[2];
+                            (w * units * Two(__low2float(values[g][i]))).get(x[0], x[1]);
                             if (EDGE) {  // a position that a row does not see adds nothing, whatever it holds
                                 const bool skip[2] = {blind(u, i, n, 0), blind(u, i, n, 1)};
-                                if (skip[0]) x[2 * i] = 0.f;
-                                if (skip[1]) x[2 * i + 1] = 0.f;
+                                if (skip[0]) x[0] = 0.f;
+                                if (skip[1]) x[1] = 0.f;
                                 zeros[n][g] = fma(w, Two(skip[0] ? 0.f : sz[i].y, skip[1] ? 0.f : sz[i].y), zeros[n][g]);
                             } else {
                                 zeros[n][g] = fma(w, Two(sz[i].y), zeros[n][g]);
                             }
+                            uint32_t& high = i ? p1[n] : p0[n];
+                            high = pack_f16(x[0], x[1]);
+                            if constexpr (LOW || kCentred) {  // what the rounding leaves
+                                const float2 as = unpack_f16(high);
+                                if constexpr (LOW)
+                                    low[i] = pack_f16(x[0] - as.x, x[1] - as.y);
+                                else
+                                    zeros[n][g] = fma(both(eighth[n][g]), Two(x[0], x[1]) + Two(-as.x, -as.y), zeros[n][g]);
+                            }
                         }
-                        p0[n] = pack_f16(x[0], x[1]);
-                        p1[n] = pack_f16(x[2], x[3]);
-                        if constexpr (kCentred) {  // what the rounding leaves, times 8
-                            const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
-                            zeros[n][g] = fma(Two(8.f), Two(x[0], x[1]) + Two(-a.x, -a.y), zeros[n][g]);
-                            zeros[n][g] = fma(Two(8.f), Two(x[2], x[3]) + Two(-d.x, -d.y), zeros[n][g]);
-                        }
-                        if constexpr (LOW) {
-                            const float2 a = unpack_f16(p0[n]), d = unpack_f16(p1[n]);
-                            const uint32_t low0 = pack_f16(x[0] - a.x, x[1] - a.y), low1 = pack_f16(x[2] - d.x, x[3] - d.y);
-                            if constexpr (BOTH)
-                                l0[n] = transpose_f16(low0), l1[n] = transpose_f16(low1);
-                            else if (j >= 2)
-                                p0[n] = low0, p1[n] = low1;
-                        }
+                        if constexpr (BOTH) l0[n] = transpose_f16(low[0]), l1[n] = transpose_f16(low[1]);
+                        if constexpr (HALF)
+                            if (j >= 2) p0[n] = low[0], p1[n] = low[1];
                         p0[n] = transpose_f16(p0[n]);
                         p1[n] = transpose_f16(p1[n]);
                     }
@@ -1120,13 +1194,17 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                 for (int m = 0; m < 4 * GROUPS; ++m) {
                     float(&x)[4] = out[t][m];
+                    float units[2];
+                    both(unit[t][m / 4]).get(units[0], units[1]);
                     if (more) {
                         const float4 y = of[m * 32];
-                        x[0] = fmaf(y.x, keep[0], x[0]), x[1] = fmaf(y.y, keep[1], x[1]);
-                        x[2] = fmaf(y.z, keep[0], x[2]), x[3] = fmaf(y.w, keep[1], x[3]);
+                        const float by[2] = {keep[0] * units[0], keep[1] * units[1]};
+                        x[0] = fmaf(y.x, by[0], x[0]), x[1] = fmaf(y.y, by[1], x[1]);
+                        x[2] = fmaf(y.z, by[0], x[2]), x[3] = fmaf(y.w, by[1], x[3]);
                     }
                     if (away) {
-                        of[m * 32] = make_float4(x[0], x[1], x[2], x[3]);
+                        const float by[2] = {1.f / units[0], 1.f / units[1]};
+                        of[m * 32] = make_float4(x[0] * by[0], x[1] * by[1], x[2] * by[0], x[3] * by[1]);
                         x[0] = x[1] = x[2] = x[3] = 0.f;
                     }
                 }
@@ -1150,17 +1228,20 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     if (++stage == kStages) stage = 0, phase ^= 1;
                 }
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sum[t][0] = sum[t][1] = nan;
+                for (int t = 0; t < NT; ++t) sum[t] = Two(nan);
                 break;
             }
             if (none || pair >= least >> 5) {  // some row does not see all of the pair's positions
 #pragma unroll
-                for (int t = 0; t < NT; ++t)
+                for (int t = 0; t < NT; ++t) {
+                    float gone_of[2];
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int sees = min(limit[t][i], seen);  // a missing cell among what the row sees
-                        if ((none & 1 && pair * kPairTokens < sees) || (none & 2 && pair * kPairTokens + kCellTokens < sees)) sum[t][i] = nan;
+                        gone_of[i] = (none & 1 && pair * kPairTokens < sees) || (none & 2 && pair * kPairTokens + kCellTokens < sees) ? nan : 0.f;
                     }
+                    sum[t] = sum[t] + Two(gone_of[0], gone_of[1]);
+                }
 #pragma unroll 1
                 for (int u = 0; u < 2; u += Shape::kAtOnce)
                     take(std::true_type{}, held + u * Shape::kCell, pair * kPairTokens + u * kCellTokens, none >> u);
@@ -1174,9 +1255,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         // rows that see positions which no table entry covers, or whose sequence has no table
 #pragma unroll
         for (int t = 0; t < NT; ++t)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-                if (part.table < 0 || limit[t][i] > covered) sum[t][i] = nan;
+            sum[t] = sum[t] + Two(part.table < 0 || limit[t][0] > covered ? nan : 0.f, part.table < 0 || limit[t][1] > covered ? nan : 0.f);
 
         // ---- the warps' sums
         __syncthreads();  // the rings are drained
@@ -1187,11 +1266,15 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             for (int i = 0; i < 2; ++i) {
                 float* row = mine_sums + (8 * t + (HALF ? (2 * j + i) % 4 : 2 * j + i)) * Shape::kPart;
                 const bool mine = !HALF || j < 2;  // the others hold the same rows
-                const float l = across_sum(sum[t][i]);
+                float sums[2], units[2];
+                sum[t].get(sums[0], sums[1]);
+                const float l = across_sum(sums[i]);
                 if (quad == 0 && mine) row[D] = reference[t][i], row[D + 1] = l;
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     float of_rows[2];
+                    both(unit[t][g]).get(units[0], units[1]);
+                    const float by = 1.f / units[i];
                     zeros[t][g].get(of_rows[0], of_rows[1]);
                     const float z = across_sum(of_rows[i]);
 #pragma unroll
@@ -1202,8 +1285,8 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             y += __shfl_xor_sync(0xffffffffu, y, 2);
                         }
                         if (!mine) continue;
-                        row[16 * m + quad] = fmaf(x, LOW ? 1.f : 0x1p24f, z);
-                        row[16 * m + 8 + quad] = fmaf(y, LOW ? 1.f : 0x1p20f, z);
+                        row[16 * m + quad] = fmaf(x, LOW ? by : by * 0x1p24f, z);
+                        row[16 * m + 8 + quad] = fmaf(y, LOW ? by : by * 0x1p20f, z);
                     }
                 }
             }

@@ -313,6 +313,42 @@ def test_values_of_many_magnitudes(gpu, dtype):
     check(gpu, held, r, queries(15, 24, 2, 64, dtype), [0, 4, 24])
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D,ratios", [(128, (1e3, 1e-3)), (128, (1e-4, 1e4)), (256, (3e3, 1e-4, 1.0, 1e-3)), (192, (1e-5, 2e4, 1e-1))])
+@pytest.mark.parametrize("rows", [1, 5, 30])
+def test_groups_of_many_magnitudes(gpu, dtype, D, ratios, rows):
+    """Groups of a head whose steps lie 2^20 and more apart: each is as near to its own sum p (15 s + |z|)."""
+    held, r = make(17, [160, 75], D=D, heads=1, size=16)
+    k, v = (np.random.default_rng(i).standard_normal((235, 1, D)).astype(np.float32) for i in (3, 4))
+    v *= np.repeat(np.array(ratios, np.float32), 64)
+    starts = [0, 160, 235]
+    r.append(k, v, starts)
+    cache.append(gpu, tensor(k, torch.float32), tensor(v, torch.float32), *held, tensor(starts))
+    check(gpu, held, r, queries(16, 2 * rows, 2, D, dtype), [0, rows, 2 * rows])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("rows", [1, 4, 17])
+@pytest.mark.parametrize("groups", ["all", "first"])
+def test_large_values_of_little_weight(gpu, dtype, D, rows, groups):
+    """In each sequence a position whose values are 2^28 times the others' and whose weight is below 2^-60 of theirs: what
+    the others leave, one of them above all, is held as it is without it."""
+    lengths = list(range(rows + 11, rows + 23))
+    held, r = make(18, lengths, D=D, heads=1, size=16)
+    rng = np.random.default_rng(9)
+    starts = np.concatenate([[0], np.cumsum(lengths)])
+    k, v = (0.02 * rng.standard_normal((starts[-1], 1, D)).astype(np.float32) for _ in range(2))
+    v *= np.float32(5e-3)
+    k[starts[:-1] + 5] -= 1.0
+    k[starts[:-1] + 7] += 0.2
+    v[starts[:-1] + 5, :, :D if groups == "all" else 64] *= np.float32(3e8)
+    r.append(k, v, starts)
+    cache.append(gpu, tensor(k, torch.float32), tensor(v, torch.float32), *held, tensor(starts))
+    q = (42 / D * (1 + 0.01 * queries(17, 12 * rows, 2, D, torch.float32))).to(dtype)  # scores of 42 less: 2^-60
+    check(gpu, held, r, q, list(range(0, 12 * rows + 1, rows)), scale=1.0)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
 def test_scales(gpu, scale):
     held, r = make(14, [70, 19], D=128)
