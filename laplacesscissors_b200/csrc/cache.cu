@@ -418,7 +418,9 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // so that 2^-21 of that still has 11 bits, and 2^-10 of it 22, whatever the other groups' steps are and
 // whatever steps positions of little weight have.  (Steps 2^20 apart in two groups and a unit for both: 8.5e-5 of the smaller
 // group's size off in f32.)  Steady sequences hardly ever move it: the units cost 36.1 instead of 34.6 us at 16 x 4113
-// positions in f32.  Everything else is f32.  The sum of p s n and that of p z
+// positions in f32.  A score stays in the products' units and its difference from the reference takes the scale and the powers of
+// two: taken by the scores they would round away what a score of 2^31 and more has over the next, and pass what f32 holds (1% of
+// the time).  Everything else is f32.  The sum of p s n and that of p z
 // are often large beside what is left of them, and the tensor cores cut what they add to a sum:
 // f32 calls take n - 8 and z + 8 s instead, whose sums are as small as the result (16 x 4113
 // positions: 4.5e-7 of the result's size off, 1.8e-5 without; 37.1 us, 32.2 without).
@@ -439,8 +441,11 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 constexpr int kWholeTokens = 512;
 constexpr int kAttentionWarps = 4, kAttentionThreads = 32 * kAttentionWarps;
 
-// Floats of a row's part: its sums, its reference and the sum of its weights.
-constexpr int part_row(int dim) { return dim + 2; }
+// Floats of a row's part: its sums, its reference, the sum of its weights and its scores' factor.
+constexpr int part_row(int dim) { return dim + 4; }
+// The reference of a row that has seen nothing: below all scores, which are below 2^45 (heads of 256 elements, steps and
+// zeros below 2^16, levels below 2^4, queries below 2^14), and still a number when it is taken from one.
+constexpr float kNoReference = -0x1p100f;
 
 // GROUPS: of 64 elements; NT: eights of a tile's rows; LOW: f32; HALF: four rows, the low parts beside them.
 template <int GROUPS, int NT, bool LOW, bool HALF>
@@ -662,7 +667,6 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
     constexpr bool kCentred = std::is_same<T, __half>::value;
     static_assert(!HALF || (LOW && NT == 1), "four rows");
     constexpr int D = Shape::kDim, kStages = Shape::kStages;
-    constexpr float kNone = -1e30f;  // the reference of a row that has seen nothing
     constexpr float kMostUnit = 0x1p100f, kRoom = 0x1p7f;
     // Units of two rows; one register each where there are many (up to 6 rows a sequence of heads of 256, bf16: 72 us, 75 in two).
     using Units = std::conditional_t<(NT * GROUPS > 4), PackedTwo, Two>;
@@ -867,7 +871,9 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             const bool fine = top < 0x7f800000u;
             // 2^power takes the largest into 2^13 .. 2^14
             const int power = fine && top ? 13 - max((int)(top >> 23) - 127, -100) : 0;
-            const float up = fine ? pow2(power) : 0.f, of_row = fine ? call.scale * pow2(LOW ? -power : 12 - power) * (LOW ? 1.f : 0x1p12f) : nan;
+            // a row that is not finite gives NaN; the scale's sign goes to the queries, its size into the scores' differences
+            const float up = fine ? copysignf(pow2(power), call.scale) : nan;
+            const float of_row = fminf(fabsf(call.scale) * pow2(LOW ? -power : 12 - power) * (LOW ? 1.f : 0x1p12f), std::numeric_limits<float>::max());
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int holder = (HALF ? (2 * j + i) % 4 : 2 * j + i) * 4;
@@ -883,7 +889,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         const float by = e && !LOW ? up * 0.0625f : up;
-                        const auto value = [&](int i) { return fine ? raw[t][g].value(8 * w + e + i) * by : 0.f; };
+                        const auto value = [&](int i) { return fine ? raw[t][g].value(8 * w + e + i) * by : nan; };
                         const float y0 = value(0), y4 = value(4), y2 = value(2), y6 = value(6);
                         const int f = (t * GROUPS + g) * 4 + w * 2 + e;
                         const uint32_t one = LOW ? 0x3c003c00u : e ? 0x00100010u : 0x00010001u, a[4] = {one, one, one, one};
@@ -933,7 +939,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             for (int n = 0; n < 4 * GROUPS; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) out[t][n][i] = 0.f;
-            reference[t][0] = reference[t][1] = kNone;
+            reference[t][0] = reference[t][1] = kNoReference;
             sum[t] = Two(0.f);
 #pragma unroll
             for (int g = 0; g < GROUPS; ++g) {
@@ -999,7 +1005,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
             // then cell by cell, while the products of the next one are under way
 #pragma unroll
             for (int u = 0; u < U; ++u) {
-                // scores, in units that `factor` takes to powers of two, and the values' steps and zeros
+                // scores, whose differences `factor` takes to powers of two, and the values' steps and zeros
                 Two score[NT][2];  // of position, of position + 8
                 __half2 values[GROUPS][2];
 #pragma unroll
@@ -1037,7 +1043,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                     for (int i = 0; i < 4; ++i) {
                         if (i % 2 == 0) {
                             const Two against(-reference[n][0], -reference[n][1]);
-                            fma(score[n][i / 2], Two(factor[n][0], factor[n][1]), against).get(weight[n][i], weight[n][i + 1]);
+                            ((score[n][i / 2] + against) * Two(factor[n][0], factor[n][1])).get(weight[n][i], weight[n][i + 1]);
                         }
                         weight[n][i] = exp2_approx(weight[n][i]);
                         if (EDGE && blind(u, i / 2, n, i % 2)) weight[n][i] = 0.f;
@@ -1058,7 +1064,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                             for (int m = 0; m < 2; ++m) {
                                 float rows[2];
                                 score[n][m].get(rows[0], rows[1]);
-                                if (!EDGE || !blind(u, m, n, i)) top[n][i] = fmaxf(top[n][i], rows[i] * factor[n][i]);
+                                if (!EDGE || !blind(u, m, n, i)) top[n][i] = fmaxf(top[n][i], rows[i]);
                             }
                         }
 #pragma unroll
@@ -1073,13 +1079,13 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const float next = fmaxf(reference[n][i], top[n][i]);
-                            keep[n][i] = exp2_approx(reference[n][i] - next);
+                            keep[n][i] = exp2_approx((reference[n][i] - next) * factor[n][i]);
                             reference[n][i] = next;
 #pragma unroll
                             for (int m = 0; m < 2; ++m) {
                                 float rows[2], &w = weight[n][2 * m + i];
                                 score[n][m].get(rows[0], rows[1]);
-                                w = exp2_approx(fmaf(rows[i], factor[n][i], -next));
+                                w = exp2_approx((rows[i] - next) * factor[n][i]);
                                 if (EDGE && blind(u, m, n, i)) w = 0.f;
                             }
                         }
@@ -1189,7 +1195,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 float keep[2] = {0.f, 0.f};
                 if (more) {  // the references that it was taken against
                     const float4 against = of[4 * GROUPS * 32];
-                    keep[0] = exp2_approx(against.x - reference[t][0]), keep[1] = exp2_approx(against.y - reference[t][1]);
+                    keep[0] = exp2_approx((against.x - reference[t][0]) * factor[t][0]), keep[1] = exp2_approx((against.y - reference[t][1]) * factor[t][1]);
                 }
 #pragma unroll
                 for (int m = 0; m < 4 * GROUPS; ++m) {
@@ -1269,7 +1275,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 float sums[2], units[2];
                 sum[t].get(sums[0], sums[1]);
                 const float l = across_sum(sums[i]);
-                if (quad == 0 && mine) row[D] = reference[t][i], row[D + 1] = l;
+                if (quad == 0 && mine) row[D] = reference[t][i], row[D + 1] = l, row[D + 2] = factor[t][i];
 #pragma unroll
                 for (int g = 0; g < GROUPS; ++g) {
                     float of_rows[2];
@@ -1296,13 +1302,14 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
         for (int i = warp; i < (int)call.used; i += kAttentionWarps) {
             int token, h;
             if (!place(i, token, h)) continue;
-            float top = kNone, l = 0.f, weight[kAttentionWarps];
+            const float factor_of = warp_sums[i * Shape::kPart + D + 2];
+            float top = kNoReference, l = 0.f, weight[kAttentionWarps];
 #pragma unroll
             for (int w = 0; w < kAttentionWarps; ++w) top = fmaxf(top, warp_sums[(w * Shape::kRows + i) * Shape::kPart + D]);
 #pragma unroll
             for (int w = 0; w < kAttentionWarps; ++w) {
                 const float* row = warp_sums + (w * Shape::kRows + i) * Shape::kPart;
-                weight[w] = exp2_approx(row[D] - top);
+                weight[w] = exp2_approx((row[D] - top) * factor_of);
                 l += weight[w] * row[D + 1];
             }
             const float inverse = l == 0.f ? 0.f : 1.f / l;
@@ -1317,7 +1324,7 @@ __global__ void __launch_bounds__(kAttentionThreads, (AttentionShape<GROUPS, NT,
                 else
                     to_add[(size_t)i * Shape::kPart + d] = x;
             }
-            if (!whole && lane == 0) *reinterpret_cast<float2*>(to_add + (size_t)i * Shape::kPart + D) = make_float2(top, l);
+            if (!whole && lane == 0) *reinterpret_cast<float4*>(to_add + (size_t)i * Shape::kPart + D) = make_float4(top, l, factor_of, 0.f);
         }
         if (first == 0 && !whole && threadIdx.x == 0) {
             call.shares[blockIdx.x] = 1 + (int)((pairs - last + run - 1) / run);
@@ -1339,6 +1346,7 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Atten
     extern __shared__ int started[];  // [blocks] those that started a shared tile
     __shared__ int counts[kMergeWarps];
     __shared__ float2 about_warp[kMergeWarps];  // reference and sum of the weights
+    __shared__ float factors[kMergeWarps];
     __shared__ float sums[kMergeWarps][D];
     const int warp = (int)threadIdx.x / 32, lane = (int)threadIdx.x % 32;
     pdl_launch_dependents();
@@ -1364,13 +1372,15 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Atten
         const int count = call.shares[block], used = min((int)call.used - first_row, most), per_row = kMergeWarps / used;
         const int4 tail = call.tails[block];
         const int mine = warp / per_row, i = first_row + mine;
-        float top = -1e30f, l = 0.f, x[kEach] = {};
+        // (the first part's; all have the same)
+        const float factor = call.parts[((size_t)(block * 2 + 1) * call.used + min(i, (int)call.used - 1)) * kRow + D + 2];
+        float top = kNoReference, l = 0.f, x[kEach] = {};
         for (int n = mine < used ? warp % per_row : count; n < count; n += kAhead * per_row) {  // all loads ahead of their use
             float2 about[kAhead];
             float row[kAhead][kEach];
 #pragma unroll
             for (int m = 0; m < kAhead; ++m) {
-                about[m] = make_float2(-1e30f, 0.f);
+                about[m] = make_float2(kNoReference, 0.f);
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) row[m][e] = 0.f;
                 const int from = n + m * per_row;
@@ -1382,14 +1392,14 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Atten
                 }
             }
             const float now = fmaxf(top, fmaxf(fmaxf(about[0].x, about[1].x), fmaxf(about[2].x, about[3].x)));
-            const float keep = exp2_approx(top - now);
+            const float keep = exp2_approx((top - now) * factor);
             top = now;
             l *= keep;
 #pragma unroll
             for (int e = 0; e < kEach; ++e) x[e] *= keep;
 #pragma unroll
             for (int m = 0; m < kAhead; ++m) {
-                const float weight = exp2_approx(about[m].x - now);
+                const float weight = exp2_approx((about[m].x - now) * factor);
                 l = fmaf(about[m].y, weight, l);
 #pragma unroll
                 for (int e = 0; e < kEach; ++e) x[e] = fmaf(row[m][e], weight, x[e]);
@@ -1397,18 +1407,18 @@ __global__ void __launch_bounds__(32 * kMergeWarps) attention_merge_kernel(Atten
         }
 #pragma unroll
         for (int e = 0; e < kEach; ++e) sums[warp][e * 32 + lane] = x[e];
-        if (lane == 0) about_warp[warp] = make_float2(top, l);
+        if (lane == 0) about_warp[warp] = make_float2(top, l), factors[warp] = factor;
         __syncthreads();
         for (int d = (int)threadIdx.x; d < used * D; d += 32 * kMergeWarps) {
             const int row = d / D, first = row * per_row, k = first_row + row;
             const int token = call.subs > 1 ? 0 : k / (int)call.group;
             const int h = call.subs > 1 ? tail.z * rows + k : k % (int)call.group;
             if (h >= (int)call.group || token >= tail.w) continue;
-            top = -1e30f, l = 0.f;
+            top = kNoReference, l = 0.f;
             for (int w = first; w < first + per_row; ++w) top = fmaxf(top, about_warp[w].x);
             float y = 0.f;
             for (int w = first; w < first + per_row; ++w) {
-                const float weight = exp2_approx(about_warp[w].x - top);
+                const float weight = exp2_approx((about_warp[w].x - top) * factors[first]);
                 l = fmaf(about_warp[w].y, weight, l);
                 y = fmaf(sums[w][d % D], weight, y);
             }

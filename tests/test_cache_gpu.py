@@ -349,6 +349,47 @@ def test_large_values_of_little_weight(gpu, dtype, D, rows, groups):
     check(gpu, held, r, q, list(range(0, 12 * rows + 1, rows)), scale=1.0)
 
 
+@pytest.mark.parametrize("dtype,size,scale", [
+    (torch.float32, 1e12, 1.0), (torch.float32, 1e12, -1.0), (torch.float32, 1e32, 1.0), (torch.float32, 3e37, 0.125),
+    (torch.float32, 3e37, -1e20), (torch.float32, 1.0, 1e29), (torch.float16, 1e4, 1e9),
+    (torch.float16, 1e-3, -1e28), (torch.bfloat16, 1e12, 1.0), (torch.bfloat16, 1e32, -1.0), (torch.bfloat16, 3e37, 1e15)])
+@pytest.mark.parametrize("sign", [0, 1, -1])
+@pytest.mark.parametrize("rows,length", [(1, 40), (9, 90), (1, 3000)])
+def test_scores_of_any_size(gpu, dtype, size, scale, sign, rows, length):
+    """Scores up to 10^60 apart, all of one sign or not: the position with the largest has all the weight."""
+    held, r = make(19, [length, length], D=64, heads=1, offset=8.0 if sign else 1.0)
+    k, v, k_wide, v_wide = r.values(0, length)
+    q = queries(18, 2 * rows, 4, 64, torch.float32)
+    if sign:  # along the keys' mean, so that all scores have its sign
+        mean = np.concatenate([k, r.values(1, length)[0]]).mean((0, 1))
+        q = q * 0.05 + sign * tensor(mean / abs(mean).max(), torch.float32)
+    q = (q / 6 * size).to(dtype)
+    got = cache.attention(gpu, q, *held, tensor([0, rows, 2 * rows]), scale=scale).double().cpu().numpy()
+    x = q.double().cpu().numpy()
+    used = 0
+    for row in range(2 * rows):
+        k, v, k_wide, v_wide = (a[:length - rows + 1 + row % rows, 0] for a in r.values(row // rows, length))
+        for h in range(4):
+            z = k @ x[row, h] * np.sign(scale)
+            order = np.argsort(z)[::-1]
+            # the score's rounding as in `tolerance`, of differences: further apart than that, and by 40 in the exponent
+            apart = z[order[0]] - z[order[1]]
+            if apart < 2 * (64 / 8 + 16) * 2.0 ** -22 * (k_wide @ abs(x[row, h])).max() or apart * abs(scale) < 60:
+                continue
+            used += 1
+            error = abs(got[row, h] - v[order[0]])
+            single = 0 if dtype is torch.float32 else 2.0 ** -11
+            assert (error <= (2.0 ** -19 + single) * v_wide[order[0]] + torch.finfo(dtype).eps / 2 * abs(v[order[0]])).all(), (row, h)
+    assert used > 4 * rows
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_large_queries_and_small_scales(gpu, dtype):
+    held, r = make(20, [70, 19], D=128)
+    check(gpu, held, r, (queries(16, 2, 4, 128, torch.float32) * 1e35).to(dtype), scale=1e-36)
+    check(gpu, held, r, (queries(16, 2, 4, 128, torch.float32) * 1e-35).to(dtype), scale=1e29)
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.3, 2.5])
 def test_scales(gpu, scale):
     held, r = make(14, [70, 19], D=128)
