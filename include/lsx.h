@@ -450,8 +450,11 @@ int lsx_distill_backward_device(lsx_ctx* ctx, const void* logits, lsx_dtype kind
 
    Tables.  Row s of `tables` [table_rows x table_width] lists sequence s's pages:
    entry i holds its positions i * page_size and on; lengths[s] is how many positions it
-   has (at most table_width * page_size), and entries behind the last page in use are -1.
-   refs[p] counts the table entries that name page p; 0 is a free page.
+   has (at most table_width * page_size), and entries behind the row's last page are -1.
+   refs[p] counts the table entries that name page p; 0 is a free page.  A caller may lower a length to
+   take positions back: the pages behind the new end stay the row's own, without a gap, for the
+   next ones, until it is emptied.  Not to the inside of a page that other rows name (one that
+   was whole when the sequence was forked): what is appended there would be theirs too.
 
    Storage.  A layer's pages are [page_count][kv_heads][page_size / 16] cells of
    18 * head_dim bytes, a cell the keys and values of 16 positions of one head.  Each 64
@@ -523,7 +526,8 @@ int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const l
                                size_t out_row, size_t out_head, void* workspace, size_t workspace_bytes, void* stream);
 size_t lsx_cache_attention_workspace_bytes(lsx_ctx* ctx, size_t head_dim);
 /* Gives sequences[i] (n of them, 1..=1024) counts[i] further positions: its length
-   grows, and the pages it needs are the lowest free ones, in the order of the list.  All
+   grows, and the pages it needs beside those that its row names are the lowest free ones, in
+   the order of the list.  All
    or nothing: *missing is how many pages were short (of the pool, or of a row of the
    tables), and unless it is 0 nothing changes.  An entry outside the tables, and a sequence
    named again, is passed over; so is a negative count. */
@@ -532,15 +536,15 @@ int lsx_cache_reserve_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, s
                              const int32_t* counts, size_t n, int32_t* missing, void* stream);
 /* children[i] takes the positions of parents[i] (n of them, 1..=1024): whole pages are
    shared, a partly filled last page is copied in all layers to the lowest free page, in the
-   order of the list, so that both may go on.  A child must be empty (and a child that is
-   empty is no useful parent): entries whose child is not, or was named before, or that name
+   order of the list, so that both may go on.  A child must be empty, with no pages in its row
+   (and a child that is empty is no useful parent): entries whose child is not, or was named before, or that name
    a row outside the tables, are passed over.  All or nothing as lsx_cache_reserve_device.
    pairs [n x 2] receives what was copied, (-1, -1) where nothing was. */
 int lsx_cache_fork_device(lsx_ctx* ctx, const lsx_cache_pool* pool, int32_t* tables, size_t table_rows,
                           size_t table_width, int32_t* lengths, int32_t* refs, size_t page_size, const int32_t* parents,
                           const int32_t* children, size_t n, int32_t* pairs, int32_t* missing, void* stream);
-/* Empties the sequences: their pages lose a reference each, and their rows of the tables
-   hold -1.  Entries outside the tables, and sequences named again, are passed over; n is
+/* Empties the sequences: the pages of their rows, behind a lowered end too, lose a reference
+   each, and the rows hold -1.  Entries outside the tables, and sequences named again, are passed over; n is
    65536 at most. */
 int lsx_cache_free_device(lsx_ctx* ctx, int32_t* tables, size_t table_rows, size_t table_width, int32_t* lengths,
                           int32_t* refs, size_t page_count, size_t page_size, const int32_t* sequences, size_t n,

@@ -16,7 +16,9 @@ src/gpu.rs:454-501).  These work on torch CUDA tensors:
 A call's sequences are rows 0, 1, .. of the tables, or those that `sequences` (int32)
 lists; `starts` (int32, one more than the sequences, ascending) says which of the call's
 rows belong to each, its last positions; without it each sequence has one row.  The
-lengths count the call's own rows: reserve positions, append, then attend.
+lengths count the call's own rows: reserve positions, append, then attend.  Positions
+are taken back by lowering `lengths` in place: their pages stay with the sequence for
+the next reserve, or until it is freed (lsx.h says where that ends: at a forked page).
 
 Calls enqueue on torch's current stream on the Gpu's device, copy nothing to the host
 and may be captured into a CUDA graph.  `PagedCache` holds the tensors and passes them."""

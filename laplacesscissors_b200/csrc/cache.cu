@@ -1488,13 +1488,31 @@ __device__ __forceinline__ bool named_before(const int* list, int i) {
     return false;
 }
 
+// How many entries of a row of the tables name pages, `held` of them at least: those of a sequence that was shortened
+// go on behind its end.
+__device__ __forceinline__ long long pages_in(const int32_t* row, uint32_t width, uint32_t page_count, long long held) {
+    const auto none = [&](long long slot) { return slot >= width || (uint32_t)row[slot] >= page_count; };
+    if (none(held)) return held;
+    long long low = held, high = width;  // an entry that names one, and one that does not
+    for (long long step = 1; high - low > 1; step *= 2) {  // at twice the distance while there are pages, then by halves
+        const long long middle = min(low + step, (low + high) / 2);
+        if (none(middle)) {
+            high = middle;
+            step = 1;
+        } else {
+            low = middle;
+        }
+    }
+    return high;
+}
+
 // lsx_cache_reserve_device.  One block: entry i of the list is thread i's.
 __global__ void __launch_bounds__(1024) reserve_kernel(int32_t* tables, uint32_t table_rows, uint32_t width,
                                                        int32_t* lengths, int32_t* refs, uint32_t page_count,
                                                        uint32_t page_size, const int32_t* sequences,
                                                        const int32_t* counts, uint32_t n, int32_t* missing) {
     __shared__ int list[kMaxListed];
-    __shared__ long long starts[kMaxListed + 1];
+    __shared__ long long starts[kMaxListed + 1], firsts[kMaxListed];
     __shared__ long long parts[32];
     const int i = (int)threadIdx.x;
     list[i] = i < (int)n ? sequences[i] : -1;
@@ -1502,10 +1520,12 @@ __global__ void __launch_bounds__(1024) reserve_kernel(int32_t* tables, uint32_t
     const int s = list[i];
     const bool valid = i < (int)n && (uint32_t)s < table_rows && !named_before(list, i);
     const long long before = valid ? max(lengths[s], 0) : 0, after = before + (valid ? max(counts[i], 0) : 0);
-    const long long held = (before + page_size - 1) / page_size, needed = (after + page_size - 1) / page_size;
-    long long beyond, total;
+    const long long needed = (after + page_size - 1) / page_size;
+    long long held = (before + page_size - 1) / page_size, beyond, total;
+    if (valid) held = pages_in(tables + (size_t)s * width, width, page_count, held);
     block_prefix(max(needed - (long long)width, 0ll), parts, &beyond);
-    starts[i] = block_prefix(needed - held, parts, &total);
+    starts[i] = block_prefix(max(needed - held, 0ll), parts, &total);
+    firsts[i] = held;
     if (i == 0) starts[kMaxListed] = total;
     __syncthreads();
     if (beyond > 0) {  // a row of the tables is too short: nothing changes
@@ -1521,8 +1541,7 @@ __global__ void __launch_bounds__(1024) reserve_kernel(int32_t* tables, uint32_t
             else
                 high = middle;
         }
-        const long long slot = ((long long)max(lengths[list[low]], 0) + page_size - 1) / page_size + rank - starts[low];
-        tables[(size_t)list[low] * width + slot] = page;
+        tables[(size_t)list[low] * width + firsts[low] + rank - starts[low]] = page;
         refs[page] = 1;
     });
     __syncthreads();
@@ -1553,7 +1572,7 @@ __global__ void __launch_bounds__(1024) fork_kernel(int32_t* tables, uint32_t ta
     __syncthreads();
     const int child = list[i], parent = i < (int)n ? parents[i] : -1;
     bool valid = (uint32_t)child < table_rows && (uint32_t)parent < table_rows && lengths[child] <= 0 &&
-                 !named_before(list, i);
+                 (uint32_t)tables[(size_t)child * width] >= page_count && !named_before(list, i);
     const long long held = valid ? max(lengths[parent], 0) : 0;
     valid = held > 0 && held <= (long long)width * page_size;
     source[i] = valid ? parent : -1;
@@ -1601,10 +1620,15 @@ __global__ void __launch_bounds__(256) free_kernel(int32_t* tables, uint32_t tab
     if (__syncthreads_or(earlier)) return;
     const long long held = max(lengths[s], 0);
     const long long pages = min((held + page_size - 1) / page_size, (long long)width);
-    for (long long w = threadIdx.x; w < pages; w += 256) {
-        const int page = tables[(size_t)s * width + w];
-        tables[(size_t)s * width + w] = -1;
-        if ((uint32_t)page < page_count) atomicSub(refs + page, 1);
+    for (long long base = 0; base < width; base += 256) {  // and those behind the end, which go on without a gap
+        const long long w = base + threadIdx.x;
+        const int page = w < width ? tables[(size_t)s * width + w] : -1;
+        const bool some = (uint32_t)page < page_count;
+        if (w < pages || some) {
+            tables[(size_t)s * width + w] = -1;
+            if (some) atomicSub(refs + page, 1);
+        }
+        if (!__syncthreads_or(base + 256 < pages || (some && threadIdx.x == 255))) break;
     }
     __syncthreads();
     if (threadIdx.x == 0) lengths[s] = 0;

@@ -242,3 +242,75 @@ def test_a_search_over_sequences(gpu):
     add([7, 2, 0], [5, 1, 20])
     held.compact()
     look()
+
+
+class Counted:
+    """Tables, lengths and refs whose counts are those of the tables, whatever was done."""
+
+    def __init__(self, pages, rows, width, size=16):
+        self.size = size
+        self.tables = tensor(np.full((rows, width), -1))
+        self.lengths, self.refs = tensor([0] * rows), tensor([0] * pages)
+        self.state = (self.tables, self.lengths, self.refs)
+
+    def look(self):
+        t, refs = self.tables.cpu().numpy(), self.refs.cpu().numpy()
+        assert np.array_equal(refs, np.bincount(t[t >= 0], minlength=len(refs)))
+        for row, n in zip(t, self.lengths.tolist()):
+            held = int((row >= 0).sum())
+            assert (row[:held] >= 0).all() and held >= -(-n // self.size)  # no gaps, and pages for all positions
+        return t
+
+    def reserve(self, gpu, sequences, counts):
+        missing = int(cache.reserve(gpu, *self.state, tensor(sequences), tensor(counts), self.size))
+        self.look()
+        return missing
+
+
+def test_positions_taken_back_keep_their_pages(gpu):
+    """Drafts that were rejected: a length that was lowered across pages loses none of them."""
+    s = Counted(pages=30, rows=4, width=40)
+    assert s.reserve(gpu, [0, 1, 2], [100, 33, 16]) == 0
+    before = s.look()
+    for lower, more, used in ((70, 20, 7), (32, 1, 7), (0, 112, 7), (97, 30, 8), (1, 300, 19)):
+        s.lengths[0] = lower
+        assert s.reserve(gpu, [3, 0, 1], [0, more, 0]) == 0
+        now = s.look()
+        assert int(s.lengths[0]) == lower + more and (now[0] >= 0).sum() == used and np.array_equal(now[0, :7], before[0, :7])
+        assert np.array_equal(now[1:], before[1:])
+    assert int((s.refs > 0).sum()) == 23
+    s.lengths[0], s.lengths[1] = 5, 0
+    assert s.reserve(gpu, [0, 1, 3], [16 * 18, 48, 16 * 8]) == 1  # a row's own pages, then the seven that are free
+    assert s.lengths.tolist() == [5, 0, 16, 0]
+    assert s.reserve(gpu, [0, 1, 3], [16 * 18, 48, 16 * 6]) == 0
+    s.lengths[0], s.lengths[1] = 3, 0
+    cache.free(gpu, *s.state, tensor([0, 1]), s.size)
+    t = s.look()
+    assert (t[:2] == -1).all() and int((s.refs > 0).sum()) == 7
+
+
+@pytest.mark.parametrize("pages,width", [(700, 600), (700, 256), (700, 257), (2000, 1900)])
+def test_long_rows_taken_back(gpu, pages, width):
+    s = Counted(pages, rows=3, width=width)
+    assert s.reserve(gpu, [0, 1], [16 * width, 40]) == 0
+    for lower in (16 * (width - 1), 16 * 255 + 1, 16 * 256, 17, 0):
+        s.lengths[0] = lower
+        assert s.reserve(gpu, [0], [16 * width - lower]) == 0
+        assert int((s.refs > 0).sum()) == width + 3
+    s.lengths[0] = 16 * (width // 2)
+    cache.free(gpu, *s.state, tensor([0]), s.size)
+    assert s.look()[0].max() == -1 and int((s.refs > 0).sum()) == 3
+
+
+def test_a_child_that_kept_its_pages_is_not_empty(gpu):
+    s = Counted(pages=20, rows=4, width=6)
+    assert s.reserve(gpu, [0, 1], [40, 20]) == 0
+    pool = torch.zeros((2, 20, 16), dtype=torch.uint8, device="cuda")
+    s.lengths[1] = 0
+    assert int(cache.fork(gpu, pool, *s.state, tensor([0, 0]), tensor([1, 2]), s.size)) == 0
+    s.look()
+    assert s.lengths.tolist() == [40, 0, 40, 0]
+    cache.free(gpu, *s.state, tensor([1]), s.size)
+    assert int(cache.fork(gpu, pool, *s.state, tensor([0]), tensor([1]), s.size)) == 0
+    s.look()
+    assert s.lengths.tolist() == [40, 40, 40, 0]
