@@ -1940,7 +1940,6 @@ int lsx_cache_append_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_
     LSX_TRY(check_heads(k, kind, k_row, k_head, "keys"));
     LSX_TRY(check_heads(v, kind, v_row, v_head, "values"));
     LSX_CACHE_SCOPE();
-    LSX_ENSURE((uint64_t)r.rows * c.kv_heads <= INT32_MAX, "too many rows and heads");
     const size_t e = dtype_bytes(kind);
     const bool wide = (reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 &&
                       (k_row | k_head | v_row | v_head) * e % 16 == 0;
@@ -1961,7 +1960,6 @@ int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_ca
     LSX_TRY(check_heads(v_out, kind, 0, 0, "values"));
     LSX_CACHE_SCOPE();
     LSX_ENSURE((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16 == 0, "outputs are not aligned to 16 bytes");
-    LSX_ENSURE((uint64_t)r.rows * c.kv_heads <= INT32_MAX, "too many rows and heads");
     return by_kind(kind, [&](auto type) {
         using T = decltype(type);
         LSX_CUDA(launch_read<T>(on, (T*)k_out, (T*)v_out, c, r), "cache read");
