@@ -7,7 +7,7 @@ import pytest
 import torch
 
 import cache_reference as ref
-from laplacesscissors_b200 import cache
+from laplacesscissors_b200 import LsxError, cache
 from test_cache_gpu import check, make, queries, tensor
 
 pytestmark = pytest.mark.gpu
@@ -264,3 +264,66 @@ def test_lengths_at_the_end_of_their_type(gpu, dtype):
     # with the zeros, each addition off by 2^-25 of the sum at most, all alike where the terms are: 6e-3 each
     error = abs(got.double().cpu().numpy() - expected)[fine]
     assert (error <= 1.2e-2 * abs(v).max() + torch.finfo(dtype).eps / 2 * abs(expected[fine])).all(), error.max()
+
+
+def test_as_many_rows_of_heads_as_a_call_takes(gpu):
+    """2^31 rows of heads, all of them the same ones, appended; of their pages one is there."""
+    rows, heads, D = 1 << 16, 1 << 15, 64
+    pages = torch.zeros(cache.pages_shape(1, heads, 16, D), dtype=torch.uint8, device="cuda")
+    tables = torch.full((1, rows // 16), -1, dtype=torch.int32, device="cuda")
+    tables[0, 2000] = 0
+    base = queries(97, 1, heads, D, torch.bfloat16)
+    k, v = base.expand(rows, heads, D), base.flip(2).contiguous().expand(rows, heads, D)
+    cache.append(gpu, k, v, pages, tables, tensor([rows]), tensor([0, rows]))
+    raw = ref.encode(base[0].float().cpu().numpy(), base[0].flip(1).float().cpu().numpy())
+    expected = np.zeros((heads, 18 * D), np.uint8)
+    for index in ref.cell_index(D):
+        expected[:, index] = raw
+    assert np.array_equal(pages[0, :, 0].cpu().numpy(), expected)
+    with pytest.raises(LsxError, match="rows of heads"):
+        cache.append(gpu, base.expand(rows + 1, heads, D), base.expand(rows + 1, heads, D), pages, tables, tensor([rows + 1]),
+                     tensor([0, rows + 1]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_long_sums_do_not_drift(gpu, dtype):
+    """Warps with thousands of pairs of cells each: 200 thousand positions for 256 sequences of 8 heads, whose tables name
+    the same pages again and again, values of one sign so that every cut goes the same way."""
+    heads, D, size, n, length = 8, 64, 64, 256, 200_000
+    held, r = make(98, [64 * 40], heads=heads, D=D, size=size, spare=0)
+    rng = np.random.default_rng(99)
+    order = held[1][0, :40].cpu().numpy()
+    raw = ref.encode(*(np.abs(rng.standard_normal((2, 64 * 40, heads, D))).astype(np.float32)))
+    pages = held[0].cpu().numpy()
+    for t, index in enumerate(ref.cell_index(D)):  # position t of every cell
+        at = np.ix_(order, range(heads), range(size // 16), index)
+        pages[at] = raw[t::16].reshape(40, size // 16, heads, -1).transpose(0, 2, 1, 3)
+    width = -(-length // size)
+    tables = rng.integers(0, 40, (n, width)).astype(np.int32)
+    q = queries(100, n, heads, D, dtype, 0.1)
+    got = cache.attention(gpu, q, tensor(pages, torch.uint8), tensor(tables), tensor([length] * n)).double()
+    place = np.empty(40, np.int64)
+    place[order] = np.arange(40)
+    k, v, _, _ = (torch.from_numpy(a.reshape(40, size, heads, D)).cuda() for a in ref.decode(raw))
+    drift, worst = [], []
+    for b in range(0, n, 16):
+        count = torch.from_numpy(np.bincount(place[tables[b]], minlength=40).astype(np.float64)).cuda()  # how often each page
+        last = (length - 1) % size + 1
+        z = torch.einsum("hd,pthd->hpt", q[b].double(), k) / 8
+        w = torch.exp(z - z.amax((1, 2), keepdim=True)) * count[None, :, None]
+        end = place[tables[b, -1]]
+        w[:, end, last:] *= (count[end] - 1) / count[end]
+        expected = torch.einsum("hpt,pthd->hd", w, v) / w.sum((1, 2))[:, None]
+        error = (got[b] - expected) / expected
+        drift.append(error.mean())
+        worst.append(error.abs().max())
+    # 12.8 million pairs (32 positions of a head) over 2400 warps are 5300 a warp.  Cut by half a unit, 2^-24 of the sum, at each of
+    # 2 (f32 4) steps a pair, a sum that is not put aside ends 5300 * 2 * 2^-24 / 2 = 3e-4 too small on average.  Put
+    # aside, 256 (f32 128) steps leave 2^-24 * 256 / 2 = 8e-6, and the f32 sums of some 20000 terms a thread, which round to
+    # nearest, 2e-6 or so.  The result's rounding (f16 2^-11, bf16 2^-8 at most) is to both sides and, over 512 elements of 16
+    # sequences, 1/50 of half a step on average: 5e-6, 4e-5.
+    allowed = {torch.float32: 1e-5, torch.float16: 2e-5, torch.bfloat16: 6e-5}[dtype]
+    mean = abs(float(torch.stack(drift).mean()))
+    assert mean < allowed, mean
+    if dtype is torch.float32:
+        assert float(torch.stack(worst).max()) < 2e-5

@@ -143,6 +143,37 @@ def test_cells_taken_whole_hold_values_at_the_ends(gpu, values):
     assert np.array_equal(held[0].cpu().numpy(), r.pages)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("strided", [False, True])
+def test_cells_taken_whole_hold_values_at_the_ends_in_all_types(gpu, dtype, D, strided):
+    """NaN and infinities at even, odd, first and last elements of a group, alone in their row; ties; groups of one
+    value, of zeros of both signs, and of what no f16 holds."""
+    held, r = make(21, [300, 41], D=D, heads=40)
+    starts = [0, 200, 241]
+    x = np.random.default_rng(22).standard_normal((241, 40, D)).astype(np.float32)
+    for i, bad in enumerate((np.nan, np.inf, -np.inf)):
+        for j, at in enumerate((0, 1, 30, 33, 62, 63, D - 64, D - 1)):
+            x[3 + 8 * i + j, i::2, at] = bad
+    x[40], x[41], x[42, :, ::2] = 3.25, 0, -0.0
+    x[43, :, 0], x[44, :, 63], x[45, :, 1], x[46, :, 62] = 65504, -65504, 60000, -60000
+    x[47] = 60000 * (-1.0) ** np.arange(D)  # a step within f16
+    # levels and ties between them: s = 1 about several zeros, each of which all three types hold
+    x[50:114] = np.arange(D) % 31 * 0.5 + (np.arange(64)[:, None, None] - 32)
+    x[114:130] = (np.arange(D) % 31 * 0.5 + np.arange(16)[:, None, None]) * 2.0 ** -6
+    x[130:170] *= 10.0 ** np.linspace(-9, 4, 40)[:, None, None]
+    if dtype is not torch.float16:
+        x[171, 1::3, 5], x[172, ::2, 6], x[173, :, 0] = 1e30, -3e38, 65520.0  # the last rounds to infinity in f16
+    wide = D + 1 if strided else D
+    k = torch.zeros((241, 40, wide), device="cuda").to(dtype)[..., :D]
+    k.copy_(tensor(x, torch.float32))
+    v = torch.zeros((241, 40, wide), device="cuda").to(dtype)[..., :D]
+    v.copy_(k.flip(2))
+    cache.append(gpu, k, v, *held, tensor(starts))
+    r.append(k.float().cpu().numpy(), v.float().cpu().numpy(), starts)
+    assert np.array_equal(held[0].cpu().numpy(), r.pages)
+
+
 def test_append_one_row_a_sequence_and_a_list(gpu):
     held, r = make(1, [3, 40, 33, 97, 64], D=128)
     k, v = (queries(i, 4, 2, 128, torch.float32) for i in (1, 2))

@@ -105,3 +105,19 @@ def test_wide_heads_and_many_pages(gpu):
     rounded = model.generate_batch(prompts, 3, cache_bits=4)
     _, _, margin, _ = model.score_batch(prompts, rounded[:, :1])
     assert (margin[:, 0] > -0.5).all(), margin  # rounding moves logits of standard deviation 1 by tenths
+
+
+@pytest.mark.parametrize("P,maximum", [(125, 9), (187, 9)])
+def test_every_step_over_pages(gpu, P, maximum):
+    """Heads of 128, prompts over several pages and steps that pass a border of theirs: each token is the one of the plain
+    model over a rounded cache, or as good as it."""
+    root = synth.cached_checkpoint("QWEN3_4B", seed=13, layers=2, vocab=8192)
+    model, plain = lsx.Model.load(root, gpu, 400), PlainModel(root)
+    prompts = np.stack([synth.prompt_tokens(90 + b, P, 8192) for b in range(2)])
+    tokens = model.generate_batch(prompts, maximum, cache_bits=4)
+    for prompt, made in zip(prompts, tokens):
+        z = plain.logits(np.concatenate([prompt, made[:-1]]).astype(int), P - 1)
+        # as above; here a level moves one score among a hundred or more by 2 * 0.4 / 11, the output by a thousandth of a unit
+        # row and less, and some hundred elements of the cache may lie that near to a border: 1e-2 of a logit at most
+        short = z.max(1) - z[np.arange(maximum), made]
+        assert (short < 1e-2).all(), short
