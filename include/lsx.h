@@ -519,7 +519,9 @@ int lsx_cache_read_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_ca
    h / (q_heads / kv_heads), out = sum_t p_t v_t, p = softmax over t of scale * q . k_t, for
    the positions t up to the row's own.  A row that sees no position is 0; one that sees a
    position without a page, or belongs to a sequence outside the tables, is NaN, and so is one that sees
-   a NaN key or value.  Rows and heads lie as given, in elements.  workspace (16-byte aligned) holds
+   a NaN key or value.  Sums are f32.  f32 calls hold queries and weights in 22 bits, f16 and bf16
+   calls queries exactly and weights in 11; a query's elements below 2^-34 (f32: 2^-39) of its largest are rounded to that,
+   and exponentials are 2^-22 off.  Rows and heads lie as given, in elements.  workspace (16-byte aligned) holds
    lsx_cache_attention_workspace_bytes(); calls that may overlap need one each. */
 int lsx_cache_attention_device(lsx_ctx* ctx, const lsx_cache_view* view, const lsx_cache_rows* rows, const void* q,
                                lsx_dtype kind, size_t q_heads, size_t q_row, size_t q_head, double scale, void* out,

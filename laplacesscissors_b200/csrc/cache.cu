@@ -410,24 +410,28 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // values) and the call's rows are its 8 columns, so that few rows leave little unused.
 //
 // Rounding.  A query row is scaled by a power of two to below 2^14 and held as f16, which
-// holds f16 and bf16 queries exactly down to 2^-38 of the row's largest element, or for f32
-// (LOW) as f16 high and low parts of 22 bits.  A weight p is taken against a reference of its row, and
-// p s times a unit of its row and group is held the same two ways: 11 bits are half a step of an
-// f16 result, twice 11 those of f32.  The unit keeps that product below 2^15; where it might pass (or a weight 2^20) the
-// reference becomes the row's largest score and the unit leaves 2^7 for the largest product that the row has met in the group,
-// so that 2^-21 of that still has 11 bits, and 2^-10 of it 22, whatever the other groups' steps are and
-// whatever steps positions of little weight have.  (Steps 2^20 apart in two groups and a unit for both: 8.5e-5 of the smaller
-// group's size off in f32.)  Steady sequences hardly ever move it: the units cost 36.1 instead of 34.6 us at 16 x 4113
-// positions in f32.  A score stays in the products' units and its difference from the reference takes the scale and the powers of
+// holds f16 and bf16 queries exactly down to 2^-38 of the row's largest element, 2^-34 where they meet levels in
+// bits 4-7, or for f32 (LOW) as f16 high and low parts: 22 bits, and none below 2^-39 of the row's largest.
+// A score stays in the products' units and its difference from the row's reference takes the scale and the powers of
 // two: taken by the scores they would round away what a score of 2^31 and more has over the next, and pass what f32 holds (1% of
-// the time).  Everything else is f32.  The sum of p s n and that of p z
+// the time).
+//
+// A weight p is taken against that reference, and p s times a unit of its row and group is held the same two ways: 11 bits are
+// half a step of an f16 result, twice 11 those of f32.  The unit keeps that product below 2^15; where it might pass (or a
+// weight 2^20) the reference becomes the row's largest score and the unit leaves 2^7 for the largest product that the row
+// has met in the group, so that 2^-21 of that still has 11 bits, and 2^-10 of it 22, whatever the other groups' steps are and
+// whatever steps positions of little weight have.  (With one reference for all groups, groups whose steps are 2^30 apart were
+// 1e-3 off in f32.)  Steady sequences move it once.  It costs 5% where registers are short: 16 x 4113 positions f32 36.9 instead
+// of 34.6 us, parts of prompts bf16 1138 instead of 1089, up to 6 rows of heads of 256 77 instead of 70.
+//
+// Everything else is f32, and exp2 by the hardware (2^-22 of a weight).  The sum of p s n and that of p z
 // are often large beside what is left of them, and the tensor cores cut what they add to a sum:
 // f32 calls take n - 8 and z + 8 s instead, whose sums are as small as the result (16 x 4113
-// positions: 4.5e-7 of the result's size off, 1.8e-5 without; 37.1 us, 32.2 without).
+// positions: 4.5e-7 of the result's size off, 1.8e-5 without).
 //
 // The low parts of f32 are products of their own.  Where a tile has four rows at most (HALF) they
 // take the columns that would be left unused, four further on, and the halves are added by one
-// exchange: half the products (16 x 4113 positions: 34.5 us instead of 37.1).
+// exchange: half the products (16 x 4113 positions: 34.5 us instead of 37.1, before the units).
 //
 // Work.  The pairs of cells (32 positions of one head) that the rows of a call see, in the
 // order of sequence, head, tile of rows and position, are cut into equal runs, one a block;
