@@ -420,9 +420,10 @@ __global__ void __launch_bounds__(32 * kCellWarps) read_cells_kernel(CacheView c
 // half a step of an f16 result, twice 11 those of f32.  The unit keeps that product below 2^15; where it might pass (or a
 // weight 2^20) the reference becomes the row's largest score and the unit leaves 2^7 for the largest product that the row
 // has met in the group, so that 2^-21 of that still has 11 bits, and 2^-10 of it 22, whatever the other groups' steps are and
-// whatever steps positions of little weight have.  (With one reference for all groups, groups whose steps are 2^30 apart were
-// 1e-3 off in f32.)  Steady sequences move it once.  It costs 5% where registers are short: 16 x 4113 positions f32 36.9 instead
-// of 34.6 us, parts of prompts bf16 1138 instead of 1089, up to 6 rows of heads of 256 77 instead of 70.
+// whatever steps positions of little weight have.  (With one reference for all groups, a group whose steps are 1e-8 of the
+// other's was 7.0e-3 of its size off in f32, now 4.9e-7.)  Steady sequences move it about once.  It costs registers and code: with the
+// scores' differences 16 x 4113 positions in f32 take 37.7 instead of 34.6 us, parts of prompts in bf16 1144 instead of 1089, up to
+// 6 rows of heads of 256 78.7 instead of 70.1.
 //
 // Everything else is f32, and exp2 by the hardware (2^-22 of a weight).  The sum of p s n and that of p z
 // are often large beside what is left of them, and the tensor cores cut what they add to a sum:
